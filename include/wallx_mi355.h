@@ -479,6 +479,74 @@ int wx_swiglu_bwd(const void* gate, const void* up, const void* dh, void* hmid, 
 int wx_swiglu_bwd_tiled(const void* gate_tiled, const void* up_tiled, int64_t tiled_rows, const void* dh, void* hmid,
                         void* dgate, void* dup, int64_t rows, int64_t cols, wx_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * RMS norm of every head of q and k (weights of head_dim channels shared by the heads) and M-RoPE of the result in one pass:
+ *   r = 1 / sqrt(mean(x^2) + eps), n = x r w, y = n cos + rotate_half(n) sin, in fp32, rounded once.
+ * No counterpart in the reference (its decoder has no such norm); for decoders that norm their queries and keys, in the place
+ * of a norm op in front of wx_mrope_apply_packed / wx_mrope_apply_positions.  q and k [batch, heads, seq, head_dim] through
+ * (batch, head, position) strides in elements, last dimension contiguous, rows 16-byte aligned; q_out and k_out contiguous in that
+ * order of dimensions.  inv_freq == NULL: table_or_positions is the packed table of wx_mrope_table (bf16 tensors only); otherwise
+ * it is position_ids int64 [3, batch, seq] and the angles are evaluated in the kernel, to better than fp32 at any position.
+ * head_dim: a power of two of 16-byte chunks (2 to 64); sections that end on chunks of 8 channels.
+ * wx_qk_norm_rope_bwd: from the gradients of q_out and k_out those of q and k (contiguous; either may be NULL) and of the two
+ * weights (either or both may be NULL; with one, workspace of wx_qk_norm_rope_bwd_workspace_bytes(head_dim) bytes). */
+int wx_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, float eps,
+                    const void* table_or_positions, const float* inv_freq, void* q_out, void* k_out, int64_t batch, int64_t seq,
+                    int n_q_heads, int n_kv_heads, int head_dim, const int64_t q_strides[3], const int64_t k_strides[3],
+                    const int mrope_section[3], int layout, int dtype, wx_stream_t stream);
+size_t wx_qk_norm_rope_bwd_workspace_bytes(int head_dim);
+int wx_qk_norm_rope_bwd(const void* grad_q_out, const void* grad_k_out, const void* q, const void* k, const void* q_weight,
+                        const void* k_weight, float eps, const void* table_or_positions, const float* inv_freq, void* grad_q,
+                        void* grad_k, void* grad_q_weight, void* grad_k_weight, int64_t batch, int64_t seq, int n_q_heads,
+                        int n_kv_heads, int head_dim, const int64_t gq_strides[3], const int64_t gk_strides[3],
+                        const int64_t q_strides[3], const int64_t k_strides[3], const int mrope_section[3], int layout, int dtype,
+                        void* workspace, size_t workspace_bytes, wx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Attention: out = softmax(scale q k^T) v with n_q_heads a multiple of n_kv_heads, in place of scaled_dot_product_attention under
+ * the decoder's mask (act.py:616-637).  Query i of sequence b sees the keys [lo, hi) with
+ *   lo = max(0, key_ranges[b][i][0]), hi = min(n_keys, key_lengths[b], key_ranges[b][i][1], causal: length - n_queries + i + 1)
+ * (key_ranges int32 [batch, n_queries, 2] and key_lengths int32 [batch] on the device, either may be NULL; length is the
+ * clamped key_lengths[b], or n_keys without): causal masks whose queries are the last of the keys, one run of tokens that see each
+ * other, padding on either side, packed sequences, windows.  A query that sees nothing gets zeros.  Keys that a query does not see
+ * have no influence on its row, whatever they hold (NaN and infinities too).
+ * q [batch, n_q_heads, n_queries, head_dim], k and v [batch, n_kv_heads, n_keys, head_dim] through (batch, head, position)
+ * strides in elements (rows 16-byte aligned, no negative strides); out [batch, n_queries, n_q_heads, head_dim], contiguous.
+ * bf16 or fp16, head_dim 64, 80 or 128; scale > 0.  Scores, softmax and sums in fp32; the probabilities enter the second product in
+ * the tensors' type.  lse (may be NULL): fp32 [batch, n_kv_heads, n_queries * group], group = n_q_heads / n_kv_heads, entry
+ * i * group + g of query i and head g of the group: the base-2 logarithm of the sum of powers, what wx_attention_bwd reads.
+ * workspace: wx_attention_workspace_bytes() bytes for the same sizes (0 for most; few rows over many keys are split). */
+size_t wx_attention_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys, int head_dim);
+int wx_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_ranges,
+                     const int32_t* key_lengths, int causal, int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries,
+                     int64_t n_keys, int head_dim, const int64_t q_strides[3], const int64_t k_strides[3],
+                     const int64_t v_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
+                     wx_stream_t stream);
+/* Its backward: the probabilities are recomputed from lse.  out, lse: what the forward returned; grad_out through strides like q;
+ * grad_q [batch, n_queries, n_q_heads, head_dim], grad_k and grad_v [batch, n_keys, n_kv_heads, head_dim], contiguous, every element
+ * written.  No atomics: the same inputs give the same bits.  At most 1024 query heads to a key / value head. */
+size_t wx_attention_bwd_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys, int head_dim);
+int wx_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* grad_out,
+                     void* grad_q, void* grad_k, void* grad_v, const int32_t* key_ranges, const int32_t* key_lengths, int causal,
+                     int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys, int head_dim,
+                     const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                     const int64_t grad_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
+                     wx_stream_t stream);
+
+/* A quantised key / value cache: codes e4m3 [batch, n_kv_heads, capacity, head_dim] and a scale fp32 [batch, n_kv_heads, capacity] for
+ * keys and values each; a value is code * scale.  wx_kv_cache_write puts token s < lengths[b] (NULL: all) of k and v
+ * [batch, n_kv_heads, seq, head_dim] (strides as above) at position start[b] + s, with scale = max(max |x| / 448, 2^-126) of its
+ * row and code = x / scale rounded to nearest even; positions outside [0, capacity) are dropped and nothing else of the cache is
+ * touched.  A row that holds NaN or an infinity reads back as NaN.
+ * wx_cached_attention: wx_attention_fwd over such a cache (contiguous), without lse.  bf16 or fp16, head_dim 64, 80 or 128. */
+int wx_kv_cache_write(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                      const int32_t* start, const int32_t* lengths, int64_t batch, int n_kv_heads, int64_t seq, int64_t capacity,
+                      int head_dim, const int64_t k_strides[3], const int64_t v_strides[3], int dtype, wx_stream_t stream);
+int wx_cached_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                        void* out, const int32_t* key_ranges, const int32_t* key_lengths, int causal, int64_t batch, int n_q_heads,
+                        int n_kv_heads, int64_t n_queries, int64_t capacity, int head_dim, const int64_t q_strides[3], float scale,
+                        int dtype, void* workspace, size_t workspace_bytes, wx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,226 @@
+// Shared device code of the attention kernels (attention_fwd.hip, attention_bwd.hip), gfx950.
+//
+// Rows.  The G = Hq / Hkv query heads that share a key / value head are packed beside each other: row r of a
+// (sequence, key / value head) pair is query r / G of head hkv * G + r % G.  A tile of rows then covers few queries, so a
+// causal tile wastes little past the diagonal, one read of a key tile serves all heads of the group, and a single
+// query fills G rows of a matrix product instead of one.
+//
+// Products.  All run on v_mfma_f32_32x32x16 with the scores transposed, S^T = K Q^T: the accumulator's column is the row
+// (lane & 31) and its registers are keys 8 g + 4 h + i (register 4 g + i, h = lane >> 5).  The softmax of a row is then
+// a reduction over a lane's own registers and one exchange between the lane halves, and the probabilities are already
+// the B operand of O^T = V^T P^T if the contraction takes its 16 keys of step t in the order 16 t + 8 (j / 4) + 4 h + j % 4:
+// nothing crosses lanes, the A operand is read in that order by transposing LDS reads.
+//
+// LDS tiles hold a row of D 2-byte values per key (query), in chunks of 16 bytes, pitch 128 (D = 64), 192 (80) or 256 bytes
+// (128).  chunk c of row r is kept at chunk c ^ swizzle(r): 16 consecutive rows read at one chunk (b128) and 4 rows read at
+// four neighbouring chunks (transposing b64) fall into different banks.
+#pragma once
+
+#include "common.h"
+
+namespace wx {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 att_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 att_bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 att_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 att_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 att_f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_huge_valf();
+
+struct AttnMask {
+  const int2* ranges;   // [batch, n_queries] (lo, hi) or null
+  const int32_t* lens;  // [batch] or null
+  int causal;
+};
+
+// [lo, hi) of the keys that query i of sequence b sees; lo = hi = 0 when there are none.
+__device__ __forceinline__ void key_range(const AttnMask& m, int b, int i, int n_queries, int n_keys, int& lo, int& hi) {
+  int len = n_keys;
+  if (m.lens != nullptr) {
+    len = m.lens[b];
+    len = len < 0 ? 0 : (len > n_keys ? n_keys : len);
+  }
+  lo = 0;
+  hi = len;
+  if (m.causal) hi = min(hi, len - n_queries + i + 1);
+  if (m.ranges != nullptr) {
+    const int2 r = m.ranges[static_cast<int64_t>(b) * n_queries + i];
+    lo = max(lo, r.x);
+    hi = min(hi, r.y);
+  }
+  if (hi <= lo) lo = hi = 0;
+}
+
+template <int D>
+struct AttnTile {
+  static constexpr int kPitch = D == 64 ? 128 : (D == 80 ? 192 : 256);
+  static constexpr int kChunks = kPitch / 16;
+  static constexpr int kSteps = D / 16;         // contraction steps over the head
+  static constexpr int kOut = (D + 31) / 32;    // 32-channel tiles of an output (the last one of D = 80 is half padding)
+  __device__ static __forceinline__ int swizzle(int row) {
+    if constexpr (kPitch == 256) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (kPitch == 128) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+  }
+  __device__ static __forceinline__ int at(int row, int chunk) { return row * kPitch + ((chunk ^ swizzle(row)) << 4); }
+};
+
+#define WX_LDS(p) ((__attribute__((address_space(3))) void*)(p))
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t v = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  void* p = reinterpret_cast<void*>((static_cast<uint64_t>(hi) << 32) | lo);
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, static_cast<int>(bytes), 0x00020000);
+}
+constexpr uint32_t kRsrcBytes = 0x7ffffff0u;  // offsets from here on read as zero
+constexpr uint32_t kOutside = 0x80000000u;
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (DT == WX_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(att_bf16x8, a), __builtin_bit_cast(att_bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(att_f16x8, a), __builtin_bit_cast(att_f16x8, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == WX_BF16) {
+    const att_bf16x2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    const att_f16x2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};  // (to nearest; the packed convert rounds to zero)
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// B operand of contraction step t (keys 16 t .. 16 t + 15 in the order above) from the accumulator registers of 32 keys.
+template <int DT>
+__device__ __forceinline__ u32x4 pack_step(const f32x16& p, int t) {
+  const int r = 8 * t;
+  return u32x4{pack2<DT>(p[r], p[r + 1]), pack2<DT>(p[r + 2], p[r + 3]), pack2<DT>(p[r + 4], p[r + 5]), pack2<DT>(p[r + 6], p[r + 7])};
+}
+
+// The value of this lane's partner in the other half (lane ^ 32) and its own: max / sum of the two in both.
+__device__ __forceinline__ float both_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+__device__ __forceinline__ int wave_min_i(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = min(x, __shfl_xor(x, d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_max_i(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// A operand, contraction over the head: row (lane & 31) of 32 rows from `row0`, channels 16 t + 8 h .. + 7.
+template <int D>
+__device__ __forceinline__ u32x4 read_rows(const unsigned char* tile, int row0, int t, int lane) {
+  using T = AttnTile<D>;
+  const int r = lane & 31;  // (row0 is a multiple of 32: the swizzle does not see it)
+  return *reinterpret_cast<const u32x4*>(tile + row0 * T::kPitch + T::at(r, 2 * t + (lane >> 5)));
+}
+
+// A operand, contraction over the tile's rows: channel 32 o + (lane & 31), rows 16 t + 8 (j / 4) + 4 h + j % 4 from `row0`.
+// ds_read_b64_tr_b16: lane j of 16 gives the address of 4 consecutive channels of row j >> 2 and receives channel j of the 4 rows.
+template <int D>
+__device__ __forceinline__ u32x4 read_cols(const unsigned char* tile, int row0, int t, int o, int lane) {
+  using T = AttnTile<D>;
+  const int h = lane >> 5, q = (lane >> 2) & 3, row = 4 * h + q;
+  const int chunk = 4 * o + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+  const unsigned char* base = tile + (row0 + 16 * t) * T::kPitch + 8 * (lane & 1);
+  typedef __attribute__((address_space(3))) att_bf16x4* P;
+  const att_bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((P)(base + T::at(row, chunk)));
+  const att_bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((P)(base + T::at(row + 8, chunk)));
+  const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+  return u32x4{x[0], x[1], y[0], y[1]};
+}
+
+// 16 consecutive rows of a tile, straight from global memory to LDS, by one wavefront.  `offset(row)` is the byte offset of
+// tile row `row` (0..15 from the wavefront's first) from the descriptor's base, or kOutside: such rows become zeros.
+template <int D, class Offset>
+__device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, int lane, Offset offset) {
+  using T = AttnTile<D>;
+#pragma unroll
+  for (int i = 0; i < T::kChunks / 4; ++i) {
+    const int n = i * 64 + lane, row = n / T::kChunks, chunk = (n % T::kChunks) ^ T::swizzle(row);
+    uint32_t off = offset(row);
+    off += off == kOutside ? 0u : static_cast<uint32_t>(chunk) * 16u;
+    if (T::kChunks * 8 > D && chunk >= D / 8) off = kOutside;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(off), 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ void attn_barrier() {  // (no fences: they would drain the loads in flight)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+constexpr int attn_wait(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(attn_wait(0, 15));
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(attn_wait(63, 0));
+  asm volatile("" ::: "memory");
+}
+
+// Transposed accumulators (channel 32 o + 8 g + 4 h + i, row lane & 31) to one row of 2-byte values: the halves trade groups so
+// that a lane stores 8 consecutive channels, 16 bytes, at a time.  `dst` is the lane's row or null.
+template <int DT, int D>
+__device__ __forceinline__ void store_row(const f32x16* acc, float factor, uint16_t* dst, int lane) {
+  const int h = lane >> 5;
+#pragma unroll
+  for (int o = 0; o < AttnTile<D>::kOut; ++o)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      if (32 * o + 8 * g >= D) continue;
+      const f32x16& x = acc[o];
+      uint32_t a[2], b[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        a[u] = pack2<DT>(x[4 * g + 2 * u] * factor, x[4 * g + 2 * u + 1] * factor);
+        b[u] = pack2<DT>(x[4 * g + 4 + 2 * u] * factor, x[4 * g + 5 + 2 * u] * factor);
+      }
+      u32x4 v;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const auto r = __builtin_amdgcn_permlane32_swap(a[u], b[u], false, false);
+        v[u] = r[0];
+        v[2 + u] = r[1];
+      }
+      if (dst != nullptr) *reinterpret_cast<u32x4*>(dst + 32 * o + 8 * (g + h)) = v;
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ float load_half(const uint16_t* p) { return Elem<DT>::load(*p); }
+
+}  // namespace wx

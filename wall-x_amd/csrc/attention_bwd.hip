@@ -1,0 +1,567 @@
+// Attention backward (gfx950): with P = exp2(c S - L) recomputed from the scores and the forward's base-2 log-sum-exp L,
+//   delta = rowsum(dO O),  dS = P (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
+// Two kernels, seven matrix products in place of the five that share one pass: the first walks the keys of a tile of rows (dQ),
+// the second the rows of a tile of keys (dK, dV, all heads of the group in turn).  Every sum is then one wavefront's own, in a
+// fixed order: no atomics, the same gradients every time.
+#include "attention.h"
+
+namespace wx {
+
+int attention_check(const char* who, int64_t batch, int n_q, int n_kv, int64_t n_queries, int64_t n_keys, int head_dim, int dtype, float scale);
+int attention_check_strides(const char* who, const char* name, const int64_t* st, int elem_bytes, int64_t span, int64_t heads);
+
+namespace {
+
+struct BwdArgs {
+  const uint16_t *q, *k, *v, *g;  // g = dO
+  int64_t qs[3], ks[3], vs[3], gs[3];
+  const uint16_t* out;            // [batch, n_queries, n_q, D]
+  const float* lse;               // [batch, n_kv, rows]
+  uint16_t *dq, *dk, *dv;         // [batch, n_queries, n_q, D], [batch, n_keys, n_kv, D]
+  AttnMask mask;
+  int batch, n_q, n_kv, n_queries, n_keys, group;
+  int rows, row_blocks;           // rows of a pair, and 32-row blocks of them
+  float c, scale;
+  uint32_t* info;                 // [pair, row_block] blocks of kInfoWords
+  int2* bounds;                   // [pair, row_block] the keys that any row of the block sees
+  int key_tiles, splits;
+  float* part;                    // splits > 1: [pair, split, n_keys, 2, D]
+};
+
+// What the second kernel reads of 32 rows: L, delta, lo and hi of each, then the keys that all rows with keys see.
+constexpr int kInfoWords = 4 * 32 + 4;
+
+__device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64_t* st, int b, int h, int i) {
+  return p + b * st[0] + h * st[1] + i * st[2];
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
+  using T = AttnTile<D>;
+  constexpr int KB = 64, kTileBytes = KB * T::kPitch;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * kTileBytes];
+  __shared__ int2 s_bounds[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int pairs = a.batch * a.n_kv, row_tiles = (a.row_blocks + 3) / 4;
+  int pair, tile;
+  {
+    const int id = blockIdx.x;
+    if (pairs % 8 == 0) {
+      const int per = pairs / 8, x = id % 8, j = id / 8;
+      pair = x + 8 * (j % per);
+      tile = row_tiles - 1 - j / per;
+    } else {
+      pair = id % pairs;
+      tile = row_tiles - 1 - id / pairs;
+    }
+    pair = __builtin_amdgcn_readfirstlane(pair);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+  }
+  const int b = pair / a.n_kv, hk = pair - b * a.n_kv;
+  const int row = tile * 128 + wave * 32 + (lane & 31);
+  const bool live = row < a.rows;
+  const int qi = (live ? row : 0) / a.group, hq = hk * a.group + (live ? row : 0) % a.group;
+  int lo = 0, hi = 0;
+  if (live) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
+  const bool some = hi > lo;
+  int w_lo = wave_min_i(some ? lo : 0x7fffffff);
+  const int w_hi = wave_max_i(hi);
+  const int f_lo = wave_max_i(some ? lo : 0), f_hi = wave_min_i(some ? hi : 0x7fffffff);
+  w_lo = min(w_lo, w_hi);
+  if (lane == 0) s_bounds[wave] = int2{w_hi > w_lo ? w_lo : 0x7fffffff, w_hi};
+  __syncthreads();
+  int g_lo = 0x7fffffff, g_hi = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    g_lo = min(g_lo, s_bounds[u].x);
+    g_hi = max(g_hi, s_bounds[u].y);
+  }
+  g_hi = __builtin_amdgcn_readfirstlane(g_hi);
+  g_lo = __builtin_amdgcn_readfirstlane(min(g_lo, g_hi));
+  const int iters = (g_hi - g_lo + KB - 1) / KB;
+
+  const char* kp = reinterpret_cast<const char*>(a.k + b * a.ks[0] + hk * a.ks[1]);
+  const char* vp = reinterpret_cast<const char*>(a.v + b * a.vs[0] + hk * a.vs[1]);
+  const int64_t k_step = a.ks[2] * 2, v_step = a.vs[2] * 2;
+  auto fetch = [&](int it) {
+    unsigned char* slot = lds + (it & 1) * 2 * kTileBytes;
+    const int k0 = g_lo + it * KB, left = g_hi - k0, r0 = wave * 16;
+    stage16<D>(attn_rsrc(kp + k0 * k_step, kRsrcBytes), slot + r0 * T::kPitch, lane,
+               [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(k_step)) : kOutside; });
+    stage16<D>(attn_rsrc(vp + k0 * v_step, kRsrcBytes), slot + kTileBytes + r0 * T::kPitch, lane,
+               [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(v_step)) : kOutside; });
+  };
+  if (iters > 0) fetch(0);
+
+  u32x4 qf[T::kSteps], gf[T::kSteps];
+  float delta = 0.f;
+  {
+    const uint16_t* q = row_of(a.q, a.qs, b, hq, qi);
+    const uint16_t* g = row_of(a.g, a.gs, b, hq, qi);
+    const uint16_t* o = a.out + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      const u32x4 zero = {0u, 0u, 0u, 0u};
+      qf[t] = some ? *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h) : zero;
+      gf[t] = some ? *reinterpret_cast<const u32x4*>(g + 16 * t + 8 * h) : zero;
+      const u32x4 of = some ? *reinterpret_cast<const u32x4*>(o + 16 * t + 8 * h) : zero;
+      float x[8], y[8];
+      unpack16<DT>(gf[t], x);
+      unpack16<DT>(of, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+    }
+  }
+  delta = both_sum(delta);
+  const float lse = some ? a.lse[static_cast<int64_t>(pair) * a.rows + row] : kInf;
+  const int block = tile * 4 + wave;
+  if (block < a.row_blocks) {
+    const int64_t at = static_cast<int64_t>(pair) * a.row_blocks + block;
+    uint32_t* info = a.info + at * kInfoWords;
+    info[(h ? 64 : 0) + (lane & 31)] = h ? static_cast<uint32_t>(lo) : __float_as_uint(lse);
+    info[(h ? 96 : 32) + (lane & 31)] = h ? static_cast<uint32_t>(hi) : __float_as_uint(delta);
+    if (lane == 0) {
+      *reinterpret_cast<int4*>(info + 128) = int4{f_lo, f_hi, 0, 0};
+      a.bounds[at] = int2{w_lo, w_hi};
+    }
+  }
+
+  f32x16 acc[T::kOut];
+#pragma unroll
+  for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
+  for (int it = 0; it < iters; ++it) {
+    wait_loads();
+    attn_barrier();
+    if (it + 1 < iters) fetch(it + 1);
+    const unsigned char *tk = lds + (it & 1) * 2 * kTileBytes, *tv = tk + kTileBytes;
+#pragma unroll
+    for (int n = 0; n < KB / 32; ++n) {
+      const int k0 = g_lo + it * KB + 32 * n;
+      if (k0 >= w_hi || k0 + 32 <= w_lo) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int t = 0; t < T::kSteps; ++t) {
+        s = mfma<DT>(read_rows<D>(tk, 32 * n, t, lane), qf[t], s);
+        dp = mfma<DT>(read_rows<D>(tv, 32 * n, t, lane), gf[t], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+      if (k0 < f_lo || k0 + 32 > f_hi) {
+        const uint32_t span = static_cast<uint32_t>(hi - lo);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = static_cast<uint32_t>(k0 + 4 * h + 8 * (r / 4) + r % 4 - lo) < span ? s[r] : 0.f;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u32x4 ds = pack_step<DT>(s, t);
+#pragma unroll
+        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tk, 32 * n, t, o, lane), ds, acc[o]);
+      }
+    }
+  }
+
+  bool bad = false;
+#pragma unroll
+  for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (32 * o + 8 * (r / 4) < D) bad = bad || acc[o][r] != acc[o][r];
+  if (!some) {
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
+  }
+  store_row<DT, D>(acc, a.scale, live ? a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D : nullptr, lane);
+  // Rows whose sum is not a number, in plain loops over the keys that they see: 0 * inf may have come from one that they do not.
+  uint64_t redo = __ballot(bad && some);
+  redo = (redo | redo >> 32) & 0xffffffffull;
+  while (redo != 0) {
+    const int r = __builtin_ctzll(redo);
+    redo &= redo - 1;
+    const int row_r = __shfl(row, r), lo_r = __shfl(lo, r), hi_r = __shfl(hi, r);
+    const float lse_r = __shfl(lse, r), delta_r = __shfl(delta, r);
+    const int i_r = row_r / a.group, hq_r = hk * a.group + row_r % a.group;
+    const uint16_t *q = row_of(a.q, a.qs, b, hq_r, i_r), *g = row_of(a.g, a.gs, b, hq_r, i_r);
+    float sum[2] = {0.f, 0.f};
+    for (int first = lo_r; first < hi_r; first += 64) {
+      const int key = first + lane;
+      float ds = 0.f;
+      if (key < hi_r) {
+        const uint16_t *kr = row_of(a.k, a.ks, b, hk, key), *vr = row_of(a.v, a.vs, b, hk, key);
+        float s = 0.f, dp = 0.f;
+        for (int d = 0; d < D; ++d) {
+          s = __builtin_fmaf(Elem<DT>::load(q[d]), Elem<DT>::load(kr[d]), s);
+          dp = __builtin_fmaf(Elem<DT>::load(g[d]), Elem<DT>::load(vr[d]), dp);
+        }
+        ds = exp2f(s * a.c - lse_r) * (dp - delta_r);
+      }
+      const int n = min(64, hi_r - first);
+      for (int j = 0; j < n; ++j) {
+        const float x = __shfl(ds, j);
+        const uint16_t* kr = row_of(a.k, a.ks, b, hk, first + j);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (lane + 64 * u < D) sum[u] = __builtin_fmaf(x, Elem<DT>::load(kr[lane + 64 * u]), sum[u]);
+      }
+    }
+    uint16_t* dst = a.dq + ((static_cast<int64_t>(b) * a.n_queries + i_r) * a.n_q + hq_r) * D;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sum[u] * a.scale));
+  }
+}
+
+// A wavefront holds 32 keys (K and V as B operands, dK^T and dV^T as accumulators); the workgroup's four share the tiles of 32 rows
+// of Q and dO that pass through LDS.  S has rows in its registers here and a key per column, so that P and dS are the B operands of
+// dV^T = dO^T P and dK^T = Q^T dS as they stand.
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
+  using T = AttnTile<D>;
+  constexpr int kTileBytes = 32 * T::kPitch, kInfoBytes = 1024, kSlot = 2 * kTileBytes + kInfoBytes;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kSlot];
+  __shared__ int s_first[4], s_last[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int pairs = a.batch * a.n_kv;
+  int pair, tile, split;
+  {
+    int id = blockIdx.x;
+    split = id % a.splits;
+    id /= a.splits;
+    if (pairs % 8 == 0) {
+      const int per = pairs / 8, x = id % 8, j = id / 8;
+      pair = x + 8 * (j % per);
+      tile = j / per;
+    } else {
+      pair = id % pairs;
+      tile = id / pairs;
+    }
+    pair = __builtin_amdgcn_readfirstlane(pair);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    split = __builtin_amdgcn_readfirstlane(split);
+  }
+  const int b = pair / a.n_kv, hk = pair - b * a.n_kv;
+  const int k0 = tile * 128, key = k0 + wave * 32 + (lane & 31);
+  const bool live = key < a.n_keys;
+  const int wk = k0 + wave * 32;  // this wavefront's first key
+
+  // the row blocks that see any of the workgroup's keys: from the first to the last that does
+  int first = 0x7fffffff, last = -1;
+  {
+    const int2* bounds = a.bounds + static_cast<int64_t>(pair) * a.row_blocks;
+    for (int t = tid; t < a.row_blocks; t += 256) {
+      const int2 x = bounds[t];
+      if (x.x < k0 + 128 && x.y > k0 && x.y > x.x) {
+        first = min(first, t);
+        last = t;
+      }
+    }
+    first = wave_min_i(first);
+    last = wave_max_i(last);
+    if (lane == 0) s_first[wave] = first, s_last[wave] = last;
+    __syncthreads();
+    first = min(min(s_first[0], s_first[1]), min(s_first[2], s_first[3]));
+    last = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
+    const int n = last < first ? 0 : last - first + 1;
+    const int t0 = static_cast<int>(static_cast<int64_t>(n) * split / a.splits), t1 = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / a.splits);
+    last = __builtin_amdgcn_readfirstlane(first + t1);
+    first = __builtin_amdgcn_readfirstlane(first + t0);  // blocks [first, last)
+    if (n == 0) first = last = 0;
+  }
+
+  const uint32_t magic = 0xffffffffu / static_cast<uint32_t>(a.group) + 1;  // (group <= 1024; 0 for a group of 1)
+  const uint16_t* qb = a.q + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[1];
+  const uint16_t* gb = a.g + b * a.gs[0] + static_cast<int64_t>(hk) * a.group * a.gs[1];
+  const char* src = reinterpret_cast<const char*>(wave < 2 ? qb : gb);
+  const int64_t pos_step = (wave < 2 ? a.qs[2] : a.gs[2]) * 2;
+  const int head_step = static_cast<int>((wave < 2 ? a.qs[1] : a.gs[1]) * 2), pos_step32 = static_cast<int>(pos_step);
+  const uint32_t* info_base = a.info + static_cast<int64_t>(pair) * a.row_blocks * kInfoWords;
+  auto fetch = [&](int t, unsigned char* slot) {
+    const int row0 = t * 32, i0 = row0 / a.group, rem = row0 - i0 * a.group, r0 = (wave & 1) * 16;
+    stage16<D>(attn_rsrc(src + __builtin_amdgcn_readfirstlane(i0) * pos_step, kRsrcBytes), slot + (wave >> 1) * kTileBytes + r0 * T::kPitch, lane, [&](int r) {
+      const uint32_t x = static_cast<uint32_t>(rem + r0 + r), di = magic ? __umulhi(x, magic) : x, hd = x - di * a.group;
+      return row0 + r0 + r < a.rows ? di * static_cast<uint32_t>(pos_step32) + hd * static_cast<uint32_t>(head_step) : kOutside;
+    });
+    if (wave == 0)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(attn_rsrc(info_base + static_cast<int64_t>(t) * kInfoWords, kInfoWords * 4), WX_LDS(slot + 2 * kTileBytes), 16,
+                                               lane * 16, 0, 0, 0);
+  };
+  if (first < last) fetch(first, lds);
+
+  u32x4 kf[T::kSteps], vf[T::kSteps];
+  {
+    const uint16_t* k = row_of(a.k, a.ks, b, hk, live ? key : 0);
+    const uint16_t* v = row_of(a.v, a.vs, b, hk, live ? key : 0);
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      kf[t] = live ? *reinterpret_cast<const u32x4*>(k + 16 * t + 8 * h) : u32x4{0u, 0u, 0u, 0u};
+      vf[t] = live ? *reinterpret_cast<const u32x4*>(v + 16 * t + 8 * h) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  f32x16 dk[T::kOut], dv[T::kOut];
+#pragma unroll
+  for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[o][r] = dv[o][r] = 0.f;
+
+  for (int t = first; t < last; ++t) {
+    wait_loads();
+    attn_barrier();
+    if (t + 1 < last) fetch(t + 1, lds + ((t + 1 - first) & 1) * kSlot);
+    const unsigned char *tq = lds + ((t - first) & 1) * kSlot, *tg = tq + kTileBytes;
+    const float* info = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
+    const int2 full = *reinterpret_cast<const int2*>(info + 128);
+    const int f_lo = __builtin_amdgcn_readfirstlane(full.x), f_hi = __builtin_amdgcn_readfirstlane(full.y);
+    f32x16 s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+    for (int u = 0; u < T::kSteps; ++u) {
+      s = mfma<DT>(read_rows<D>(tq, 0, u, lane), kf[u], s);
+      dp = mfma<DT>(read_rows<D>(tg, 0, u, lane), vf[u], dp);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 lse = *reinterpret_cast<const float4*>(info + 8 * g + 4 * h), delta = *reinterpret_cast<const float4*>(info + 32 + 8 * g + 4 * h);
+      const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {delta.x, delta.y, delta.z, delta.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * g + i;
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -ls[i]));
+        dp[r] = s[r] * (dp[r] - de[i]);
+      }
+    }
+    if (wk < f_lo || wk + 32 > f_hi) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int4 lo = *reinterpret_cast<const int4*>(info + 64 + 8 * g + 4 * h), hi = *reinterpret_cast<const int4*>(info + 96 + 8 * g + 4 * h);
+        const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool see = key >= l4[i] && key < h4[i];
+          s[4 * g + i] = see ? s[4 * g + i] : 0.f;
+          dp[4 * g + i] = see ? dp[4 * g + i] : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const u32x4 p = pack_step<DT>(s, u), ds = pack_step<DT>(dp, u);
+#pragma unroll
+      for (int o = 0; o < T::kOut; ++o) {
+        dv[o] = mfma<DT>(read_cols<D>(tg, 0, u, o, lane), p, dv[o]);
+        dk[o] = mfma<DT>(read_cols<D>(tq, 0, u, o, lane), ds, dk[o]);
+      }
+    }
+  }
+
+  bool bad = false;
+#pragma unroll
+  for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (32 * o + 8 * (r / 4) < D) bad = bad || dk[o][r] != dk[o][r] || dv[o][r] != dv[o][r];
+  const int64_t to = ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D;
+  const int64_t part = ((static_cast<int64_t>(pair) * a.splits + split) * a.n_keys) * 2 * D;
+  if (a.splits == 1) {
+    store_row<DT, D>(dk, a.scale, live ? a.dk + to : nullptr, lane);
+    store_row<DT, D>(dv, 1.f, live ? a.dv + to : nullptr, lane);
+  } else if (live) {
+    float* dst = a.part + part + static_cast<int64_t>(key) * 2 * D;
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * o + 8 * g < D) {
+          *reinterpret_cast<float4*>(dst + 32 * o + 8 * g + 4 * h) = float4{dk[o][4 * g], dk[o][4 * g + 1], dk[o][4 * g + 2], dk[o][4 * g + 3]};
+          *reinterpret_cast<float4*>(dst + D + 32 * o + 8 * g + 4 * h) = float4{dv[o][4 * g], dv[o][4 * g + 1], dv[o][4 * g + 2], dv[o][4 * g + 3]};
+        }
+  }
+  // Keys whose sums are not numbers, in plain loops over the rows that see them.
+  uint64_t redo = __ballot(bad && live);
+  redo = (redo | redo >> 32) & 0xffffffffull;
+  while (redo != 0) {
+    const int r = __builtin_ctzll(redo);
+    redo &= redo - 1;
+    const int key_r = wk + r;
+    const uint16_t *kr = row_of(a.k, a.ks, b, hk, key_r), *vr = row_of(a.v, a.vs, b, hk, key_r);
+    float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
+    for (int t = first * 32; t < min(last * 32, a.rows); t += 64) {
+      const int row = t + lane;
+      float p = 0.f, ds = 0.f;
+      bool see = false;
+      if (row < a.rows && row < last * 32) {
+        const uint32_t* info = info_base + static_cast<int64_t>(row / 32) * kInfoWords + row % 32;
+        see = key_r >= static_cast<int>(info[64]) && key_r < static_cast<int>(info[96]);
+        if (see) {
+          const int hq = hk * a.group + row % a.group;
+          const uint16_t *q = row_of(a.q, a.qs, b, hq, row / a.group), *g = row_of(a.g, a.gs, b, hq, row / a.group);
+          float s = 0.f, d = 0.f;
+          for (int e = 0; e < D; ++e) {
+            s = __builtin_fmaf(Elem<DT>::load(q[e]), Elem<DT>::load(kr[e]), s);
+            d = __builtin_fmaf(Elem<DT>::load(g[e]), Elem<DT>::load(vr[e]), d);
+          }
+          p = exp2f(s * a.c - __uint_as_float(info[0]));
+          ds = p * (d - __uint_as_float(info[32]));
+        }
+      }
+      uint64_t seen = __ballot(see);
+      while (seen != 0) {
+        const int j = __builtin_ctzll(seen);
+        seen &= seen - 1;
+        const float pj = __shfl(p, j), dj = __shfl(ds, j);
+        const int hq = hk * a.group + (t + j) % a.group;
+        const uint16_t *q = row_of(a.q, a.qs, b, hq, (t + j) / a.group), *g = row_of(a.g, a.gs, b, hq, (t + j) / a.group);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (lane + 64 * u < D) {
+            sk[u] = __builtin_fmaf(dj, Elem<DT>::load(q[lane + 64 * u]), sk[u]);
+            sv[u] = __builtin_fmaf(pj, Elem<DT>::load(g[lane + 64 * u]), sv[u]);
+          }
+      }
+    }
+    const int64_t to_r = ((static_cast<int64_t>(b) * a.n_keys + key_r) * a.n_kv + hk) * D;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 64 * u < D) {
+        if (a.splits == 1) {
+          a.dk[to_r + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sk[u] * a.scale));
+          a.dv[to_r + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sv[u]));
+        } else {
+          float* dst = a.part + part + static_cast<int64_t>(key_r) * 2 * D + lane + 64 * u;
+          dst[0] = sk[u];
+          dst[D] = sv[u];
+        }
+      }
+  }
+}
+
+// dK and dV of a key from the splits' sums: a thread per 4 channels.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
+  const int64_t n = static_cast<int64_t>(a.batch) * a.n_kv * a.n_keys * (2 * D / 4), id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= n) return;
+  const int64_t at = id / (2 * D / 4);
+  const int e = static_cast<int>(id - at * (2 * D / 4)) * 4;
+  const int pair = static_cast<int>(at / a.n_keys), key = static_cast<int>(at - static_cast<int64_t>(pair) * a.n_keys);
+  const float* src = a.part + (static_cast<int64_t>(pair) * a.splits * a.n_keys + key) * 2 * D + e;
+  float4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < a.splits; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(i) * a.n_keys * 2 * D);
+    s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+  }
+  const float f = e < D ? a.scale : 1.f;
+  const int b = pair / a.n_kv, hk = pair % a.n_kv;
+  uint16_t* dst = (e < D ? a.dk + e : a.dv + e - D) + ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D;
+  *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<DT>(s.x * f, s.y * f), pack2<DT>(s.z * f, s.w * f)};
+}
+
+// Splits of the rows that a tile of keys walks, where the tiles alone leave CUs idle.
+int bwd_splits(int64_t pairs, int64_t n_keys, int64_t row_blocks) {
+  const int64_t tiles = pairs * ((n_keys + 127) / 128), cus = device_cu_count();
+  if (tiles == 0 || tiles >= 2 * cus) return 1;
+  const int64_t want = (2 * cus + tiles - 1) / tiles, most = row_blocks / 8;  // (at least 8 blocks of rows each)
+  const int64_t n = want < most ? want : most;
+  return static_cast<int>(n < 1 ? 1 : (n > 64 ? 64 : n));
+}
+
+struct Workspace {
+  size_t info, bounds, part, total;
+};
+Workspace layout(int64_t pairs, int64_t rows, int64_t n_keys, int head_dim) {
+  const int64_t blocks = (rows + 31) / 32;
+  const int splits = bwd_splits(pairs, n_keys, blocks);
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  Workspace w{};
+  w.info = 0;
+  w.bounds = up(static_cast<size_t>(pairs) * blocks * kInfoWords * 4);
+  w.part = w.bounds + up(static_cast<size_t>(pairs) * blocks * sizeof(int2));
+  w.total = w.part + (splits > 1 ? static_cast<size_t>(pairs) * splits * n_keys * 2 * head_dim * sizeof(float) : 0);
+  return w;
+}
+
+template <int DT, int D>
+int launch_bwd(BwdArgs& a, hipStream_t s) {
+  const int64_t pairs = static_cast<int64_t>(a.batch) * a.n_kv;
+  const int64_t row_tiles = pairs * ((a.row_blocks + 3) / 4), key_tiles = pairs * a.key_tiles * a.splits;
+  const int64_t join = a.splits > 1 ? (pairs * a.n_keys * (2 * D / 4) + 255) / 256 : 0;
+  if (row_tiles > 0x7fffffffll || key_tiles > 0x7fffffffll || join > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows");
+  const dim3 block(256);
+  if (row_tiles > 0) {
+    hipLaunchKernelGGL((attn_dq_kernel<DT, D>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
+    if (int rc = check_launch("attn_dq_kernel")) return rc;
+  }
+  if (key_tiles > 0) {
+    hipLaunchKernelGGL((attn_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(key_tiles)), block, 0, s, a);
+    if (int rc = check_launch("attn_dkv_kernel")) return rc;
+  }
+  if (join > 0) {
+    hipLaunchKernelGGL((attn_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(join)), block, 0, s, a);
+    return check_launch("attn_dkv_join_kernel");
+  }
+  return WX_OK;
+}
+
+}  // namespace
+}  // namespace wx
+
+using namespace wx;
+
+extern "C" size_t wx_attention_bwd_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys,
+                                                   int head_dim) {
+  if (batch <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_queries < 0 || n_keys < 0 || head_dim <= 0) return 0;
+  return layout(batch * n_kv_heads, n_queries * (n_q_heads / n_kv_heads), n_keys, head_dim).total;
+}
+
+extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* grad_out,
+                                void* grad_q, void* grad_k, void* grad_v, const int32_t* key_ranges, const int32_t* key_lengths,
+                                int causal, int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys,
+                                int head_dim, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                                const int64_t grad_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                wx_stream_t stream) {
+  const char* who = "wx_attention_bwd";
+  if (int rc = attention_check(who, batch, n_q_heads, n_kv_heads, n_queries, n_keys, head_dim, dtype, scale)) return rc;
+  if (!q_strides || !k_strides || !v_strides || !grad_strides) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null strides", who);
+  if (batch == 0 || n_q_heads == 0) return WX_OK;
+  const int group = n_q_heads / n_kv_heads;
+  if (group > 1024) return fail(WX_ERR_UNSUPPORTED, "%s: more than 1024 query heads to a key / value head", who);
+  if ((n_queries > 0 && (!q || !out || !lse || !grad_out || !grad_q)) || (n_keys > 0 && (!k || !v || !grad_k || !grad_v)))
+    return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  for (const void* p : {q, k, v, out, grad_out, static_cast<const void*>(grad_q), static_cast<const void*>(grad_k), static_cast<const void*>(grad_v),
+                        static_cast<const void*>(workspace)})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(key_ranges) & 7) return fail(WX_ERR_INVALID_ARGUMENT, "%s: key_ranges must be 8-byte aligned", who);
+  if (int rc = attention_check_strides(who, "q", q_strides, 2, 34, group)) return rc;
+  if (int rc = attention_check_strides(who, "k", k_strides, 2, 64, 1)) return rc;
+  if (int rc = attention_check_strides(who, "v", v_strides, 2, 64, 1)) return rc;
+  if (int rc = attention_check_strides(who, "grad_out", grad_strides, 2, 34, group)) return rc;
+  BwdArgs a{};
+  a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v), a.g = static_cast<const uint16_t*>(grad_out);
+  for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i], a.ks[i] = k_strides[i], a.vs[i] = v_strides[i], a.gs[i] = grad_strides[i];
+  a.out = static_cast<const uint16_t*>(out), a.lse = lse;
+  a.dq = static_cast<uint16_t*>(grad_q), a.dk = static_cast<uint16_t*>(grad_k), a.dv = static_cast<uint16_t*>(grad_v);
+  a.mask = {reinterpret_cast<const int2*>(key_ranges), key_lengths, causal};
+  a.batch = static_cast<int>(batch), a.n_q = n_q_heads, a.n_kv = n_kv_heads, a.n_queries = static_cast<int>(n_queries), a.n_keys = static_cast<int>(n_keys);
+  a.group = group, a.rows = static_cast<int>(n_queries) * group, a.row_blocks = (a.rows + 31) / 32;
+  a.c = scale * kLog2e, a.scale = scale;
+  const int64_t pairs = batch * n_kv_heads;
+  a.key_tiles = (a.n_keys + 127) / 128;
+  a.splits = bwd_splits(pairs, n_keys, a.row_blocks);
+  const Workspace w = layout(pairs, a.rows, n_keys, head_dim);
+  if (w.total > 0 && (!workspace || workspace_bytes < w.total)) return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_bwd_workspace_bytes)", who);
+  char* ws = static_cast<char*>(workspace);
+  a.info = reinterpret_cast<uint32_t*>(ws + w.info), a.bounds = reinterpret_cast<int2*>(ws + w.bounds), a.part = reinterpret_cast<float*>(ws + w.part);
+  hipStream_t s = as_stream(stream);
+  if (dtype == WX_BF16) {
+    if (head_dim == 64) return launch_bwd<WX_BF16, 64>(a, s);
+    if (head_dim == 80) return launch_bwd<WX_BF16, 80>(a, s);
+    return launch_bwd<WX_BF16, 128>(a, s);
+  }
+  if (head_dim == 64) return launch_bwd<WX_F16, 64>(a, s);
+  if (head_dim == 80) return launch_bwd<WX_F16, 80>(a, s);
+  return launch_bwd<WX_F16, 128>(a, s);
+}

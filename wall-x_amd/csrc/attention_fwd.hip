@@ -1,0 +1,627 @@
+// Attention forward: O = softmax(scale Q K^T over the keys of each query's range) V, one pass over the keys with a running
+// maximum and sum, for keys and values in the queries' type or quantised to e4m3 with a scale per token (gfx950).
+#include "attention.h"
+
+namespace wx {
+namespace {
+
+struct FwdArgs {
+  const void *q, *k, *v;
+  int64_t qs[3], ks[3], vs[3];   // strides in elements: batch, head, position
+  const float *k_scale, *v_scale;  // e4m3: [batch, n_kv, n_keys]
+  uint16_t* out;                 // [batch, n_queries, n_q, D]
+  float* lse;                    // [batch, n_kv, n_queries * group], base 2, or null
+  AttnMask mask;
+  int batch, n_q, n_kv, n_queries, n_keys, group;
+  int rows, row_tiles, splits;
+  float c;                       // scale * log2(e)
+  float* part;                   // splits > 1: [pair, split, rows, D] sums, then [pair, split, rows] (maximum, sum)
+};
+
+__device__ __forceinline__ float2* part_stats(const FwdArgs& a, int d) {
+  return reinterpret_cast<float2*>(a.part + static_cast<int64_t>(a.batch) * a.n_kv * a.splits * a.rows * d);
+}
+
+// two e4m3 values to two of the compute type (exact)
+template <int DT, bool HI>
+__device__ __forceinline__ uint32_t widen2(uint32_t x) {
+  if constexpr (DT == WX_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HI));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HI));
+}
+
+template <int DT, bool F8>
+__device__ __forceinline__ float load_kv(const void* p, int64_t i) {
+  if constexpr (F8) {
+    const uint32_t x = static_cast<const uint8_t*>(p)[i];
+    return Elem<DT>::load(widen2<DT, false>(x) & 0xffffu);
+  } else {
+    return Elem<DT>::load(static_cast<const uint16_t*>(p)[i]);
+  }
+}
+
+// One row by one wavefront in plain loops: for rows whose tile holds a key that they do not see with a value that is not
+// finite (0 * inf in the matrix product).  Lane l gets channels l and l + 64 of the unscaled sum.
+template <int DT, int D, bool F8>
+__device__ __forceinline__ void plain_row(const FwdArgs& a, int b, int hk, int row, int lo, int hi, int lane, float& m, float& l,
+                                          float (&o)[2]) {
+  const int i = row / a.group, hq = hk * a.group + row % a.group;
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + hq * a.qs[1] + i * a.qs[2];
+  const int64_t kb = b * a.ks[0] + hk * a.ks[1], vb = b * a.vs[0] + hk * a.vs[1], sb = (static_cast<int64_t>(b) * a.n_kv + hk) * a.n_keys;
+  m = -kInf;
+  l = 0.f;
+  o[0] = o[1] = 0.f;
+  for (int first = lo; first < hi; first += 64) {
+    const int key = first + lane;
+    float s = -kInf;
+    if (key < hi) {
+      float dot = 0.f;
+      for (int d = 0; d < D; ++d) dot = __builtin_fmaf(Elem<DT>::load(q[d]), load_kv<DT, F8>(a.k, kb + key * a.ks[2] + d), dot);
+      s = F8 ? dot * a.k_scale[sb + key] : dot;
+    }
+    const float mn = fmaxf(m, wave_max(s)), mc = mn == -kInf ? 0.f : mn * a.c;
+    const float alpha = exp2f(m * a.c - mc), p = key < hi ? exp2f(s * a.c - mc) : 0.f;
+    l = l * alpha + wave_sum(p);
+    o[0] *= alpha;
+    o[1] *= alpha;
+    const int n = min(64, hi - first);
+    for (int j = 0; j < n; ++j) {
+      float pj = __shfl(p, j);
+      if constexpr (F8) pj *= a.v_scale[sb + first + j];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (lane + 64 * u < D) o[u] = __builtin_fmaf(pj, load_kv<DT, F8>(a.v, vb + (first + j) * a.vs[2] + lane + 64 * u), o[u]);
+    }
+    m = mn;
+  }
+}
+
+// RW of the workgroup's four wavefronts take 32 rows each; the other factor, KW = 4 / RW, shares the keys: wavefront group kw
+// takes every KW-th tile of KB keys, and the groups' sums are joined in LDS at the end.
+// Many rows (RW = 4): a tile of 64 keys serves 128 rows, loaded straight to LDS one tile ahead.  Few rows (RW = 1): 32 rows, four
+// tiles in flight per workgroup, each loaded through its wavefront's registers (no barrier in the loop).
+// e4m3 tiles are widened to the compute type on their way to LDS (exactly); their scales multiply the scores and the
+// probabilities, a value per key.
+template <int DT, int D, bool F8, int RW>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
+  using T = AttnTile<D>;
+  constexpr int KW = 4 / RW, KB = RW == 4 ? 64 : 32, NT = KB / 32;
+  constexpr bool kDirect = !F8 && RW > 1;
+  constexpr int kBufs = RW == 1 ? 1 : 2;
+  constexpr int kTileBytes = KB * T::kPitch;
+  constexpr int kScaleBytes = F8 ? 2 * KB * 4 : 0;
+  constexpr int kSlot = 2 * kTileBytes + kScaleBytes;
+  constexpr int kTiles = KW * kBufs * kSlot;
+  constexpr int kJoin = KW > 1 ? 4 * 32 * (D + 4) * 4 + 4 * 32 * 8 : 0;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kTiles > kJoin ? kTiles : kJoin];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = wave % RW, kw = wave / RW, h = lane >> 5;
+
+  // Workgroup -> (pair, row tile, split).  Neighbouring workgroups go to different XCDs: with many pairs each XCD keeps its own
+  // pairs, whose keys then stay in its L2.  The last row tiles first: under a causal mask they are the longest.
+  const int pairs = a.batch * a.n_kv;
+  int pair, tile, split;
+  {
+    int id = blockIdx.x;
+    split = id % a.splits;
+    id /= a.splits;
+    if (pairs % 8 == 0) {
+      const int per = pairs / 8, x = id % 8, j = id / 8;
+      pair = x + 8 * (j % per);
+      tile = a.row_tiles - 1 - j / per;
+    } else {
+      pair = id % pairs;
+      tile = a.row_tiles - 1 - id / pairs;
+    }
+    pair = __builtin_amdgcn_readfirstlane(pair);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    split = __builtin_amdgcn_readfirstlane(split);
+  }
+  const int b = pair / a.n_kv, hk = pair - b * a.n_kv;
+  const int row = tile * 32 * RW + rw * 32 + (lane & 31);
+  const bool live = row < a.rows;
+  const int qi = (live ? row : 0) / a.group, hq = hk * a.group + (live ? row : 0) % a.group;
+
+  int lo = 0, hi = 0;
+  if (live) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
+  const bool some = hi > lo;
+  int w_lo = wave_min_i(some ? lo : 0x7fffffff), w_hi = wave_max_i(hi);   // any row of the wavefront sees [w_lo, w_hi)
+  const int f_lo = wave_max_i(some ? lo : 0), f_hi = wave_min_i(some ? hi : 0x7fffffff);  // every row that sees something sees [f_lo, f_hi)
+  if (w_lo > w_hi) w_lo = w_hi;
+  // the workgroup's keys
+  int g_lo = w_lo, g_hi = w_hi;
+  if constexpr (RW > 1) {
+    __shared__ int2 bounds[RW];
+    if (kw == 0 && lane == 0) bounds[rw] = int2{w_hi > w_lo ? w_lo : 0x7fffffff, w_hi};
+    __syncthreads();
+    g_lo = 0x7fffffff, g_hi = 0;
+#pragma unroll
+    for (int u = 0; u < RW; ++u) {
+      g_lo = min(g_lo, bounds[u].x);
+      g_hi = max(g_hi, bounds[u].y);
+    }
+    g_lo = __builtin_amdgcn_readfirstlane(min(g_lo, g_hi));
+    g_hi = __builtin_amdgcn_readfirstlane(g_hi);
+  }
+  {  // this split's share of the tiles
+    const int n = (g_hi - g_lo + KB - 1) / KB;
+    const int t0 = static_cast<int>(static_cast<int64_t>(n) * split / a.splits), t1 = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / a.splits);
+    g_hi = min(g_hi, g_lo + t1 * KB);
+    g_lo += t0 * KB;
+  }
+  const int s_lo = max(lo, g_lo), s_hi = min(hi, g_hi);
+  const int tiles = __builtin_amdgcn_readfirstlane((g_hi - g_lo + KB - 1) / KB), iters = (tiles + KW - 1) / KW;
+
+  u32x4 qf[T::kSteps];
+  {
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + hq * a.qs[1] + qi * a.qs[2];
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) qf[t] = live ? *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h) : u32x4{0u, 0u, 0u, 0u};
+  }
+
+  constexpr int kElem = F8 ? 1 : 2;
+  const char* kp = static_cast<const char*>(a.k) + (b * a.ks[0] + hk * a.ks[1]) * kElem;
+  const char* vp = static_cast<const char*>(a.v) + (b * a.vs[0] + hk * a.vs[1]) * kElem;
+  const int64_t k_step = a.ks[2] * kElem, v_step = a.vs[2] * kElem;  // (KB of them fit 31 bits: checked on the host)
+  const float* ksc = F8 ? a.k_scale + (static_cast<int64_t>(b) * a.n_kv + hk) * a.n_keys : nullptr;
+  const float* vsc = F8 ? a.v_scale + (static_cast<int64_t>(b) * a.n_kv + hk) * a.n_keys : nullptr;
+
+  // ---- staging
+  constexpr int kChunk = F8 ? D / 16 : D / 8;                      // 16-byte pieces of a row in memory
+  constexpr int kLoaders = RW * 64;                                // threads of one key group
+  constexpr int kPieces = (KB * kChunk + kLoaders - 1) / kLoaders; // per thread
+  const int gt = rw * 64 + lane;
+  u32x4 pk[kDirect ? 1 : kPieces], pv[kDirect ? 1 : kPieces];
+  float pks = 0.f, pvs = 0.f;
+  auto key0 = [&](int it) { return g_lo + (it * KW + kw) * KB; };
+  auto fetch = [&](int it, unsigned char* slot) {  // a tile on its way: to LDS, or into registers
+    const int k0 = key0(it), left = g_hi - k0;  // (may be <= 0: zeros)
+    if (left <= 0 && RW == 1) return;
+    const int64_t at = left > 0 ? k0 : 0;
+    const auto rk = attn_rsrc(kp + at * k_step, kRsrcBytes), rv = attn_rsrc(vp + at * v_step, kRsrcBytes);
+    if constexpr (kDirect) {
+#pragma unroll
+      for (int u = 0; u < KB / 16 / RW; ++u) {
+        const int r0 = (rw + u * RW) * 16;
+        stage16<D>(rk, slot + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(k_step)) : kOutside; });
+        stage16<D>(rv, slot + kTileBytes + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(v_step)) : kOutside; });
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        const int n = u * kLoaders + gt, r = n / kChunk, c = n % kChunk;
+        const bool in = r < left && r < KB;
+        pk[u] = __builtin_amdgcn_raw_buffer_load_b128(rk, in ? r * static_cast<int>(k_step) + c * 16 : static_cast<int>(kOutside), 0, 0);
+        pv[u] = __builtin_amdgcn_raw_buffer_load_b128(rv, in ? r * static_cast<int>(v_step) + c * 16 : static_cast<int>(kOutside), 0, 0);
+      }
+      if constexpr (F8) {
+        const bool in = gt < left && gt < KB;
+        pks = in ? ksc[k0 + gt] : 0.f;
+        pvs = in ? vsc[k0 + gt] : 0.f;
+      }
+    }
+  };
+  auto put = [&](unsigned char* slot) {  // registers -> LDS
+    if constexpr (!kDirect) {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        const int n = u * kLoaders + gt, r = n / kChunk, c = n % kChunk;
+        if (KB * kChunk % kLoaders != 0 && r >= KB) continue;
+        if constexpr (F8) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x0 = pk[u][2 * half], x1 = pk[u][2 * half + 1], y0 = pv[u][2 * half], y1 = pv[u][2 * half + 1];
+            *reinterpret_cast<u32x4*>(slot + T::at(r, 2 * c + half)) = u32x4{widen2<DT, false>(x0), widen2<DT, true>(x0), widen2<DT, false>(x1), widen2<DT, true>(x1)};
+            *reinterpret_cast<u32x4*>(slot + kTileBytes + T::at(r, 2 * c + half)) = u32x4{widen2<DT, false>(y0), widen2<DT, true>(y0), widen2<DT, false>(y1), widen2<DT, true>(y1)};
+          }
+        } else {
+          *reinterpret_cast<u32x4*>(slot + T::at(r, c)) = pk[u];
+          *reinterpret_cast<u32x4*>(slot + kTileBytes + T::at(r, c)) = pv[u];
+        }
+      }
+      if constexpr (F8)
+        if (gt < KB) {
+          reinterpret_cast<float*>(slot + 2 * kTileBytes)[gt] = pks;
+          reinterpret_cast<float*>(slot + 2 * kTileBytes)[KB + gt] = pvs;
+        }
+    }
+  };
+
+  // ---- the sums
+  f32x16 acc[T::kOut];
+#pragma unroll
+  for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
+  float m = -kInf, l = 0.f;  // running maximum (both halves alike) and this lane's share of the sum
+
+  auto step = [&](const unsigned char* tk, int k0) {
+    const unsigned char* tv = tk + kTileBytes;
+    const float* scales = reinterpret_cast<const float*>(tk + 2 * kTileBytes);
+    f32x16 s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+#pragma unroll
+      for (int t = 0; t < T::kSteps; ++t) s[n] = mfma<DT>(read_rows<D>(tk, 32 * n, t, lane), qf[t], s[n]);
+    }
+    if constexpr (F8) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 f = *reinterpret_cast<const float4*>(scales + 32 * n + 8 * g + 4 * h);
+          s[n][4 * g] *= f.x, s[n][4 * g + 1] *= f.y, s[n][4 * g + 2] *= f.z, s[n][4 * g + 3] *= f.w;
+        }
+    }
+    if (k0 < f_lo || k0 + KB > f_hi || k0 + KB > g_hi) {  // some row does not see all of the tile
+      const uint32_t span = static_cast<uint32_t>(s_hi > s_lo ? s_hi - s_lo : 0);
+      const int first = k0 + 4 * h - s_lo;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t at = static_cast<uint32_t>(first + 32 * n + 8 * (r / 4) + r % 4);
+          s[n][r] = at < span ? s[n][r] : -kInf;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+    top = both_max(top);
+    // The maximum is only there to keep the powers in range: it moves (and the sums are rescaled) when a score exceeds it
+    // by more than 2^8, not with every new maximum.
+    if (__any((top - m) * a.c > 8.f)) {
+      const float mn = fmaxf(m, top), alpha = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[o][r] *= alpha;
+    }
+    const float mc = m == -kInf ? 0.f : m * a.c;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.c, -mc));
+        sum += s[n][r];
+      }
+    l += sum;
+    if constexpr (F8) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 f = *reinterpret_cast<const float4*>(scales + KB + 32 * n + 8 * g + 4 * h);
+          s[n][4 * g] *= f.x, s[n][4 * g + 1] *= f.y, s[n][4 * g + 2] *= f.z, s[n][4 * g + 3] *= f.w;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u32x4 p = pack_step<DT>(s[n], t);
+#pragma unroll
+        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tv, 32 * n, t, o, lane), p, acc[o]);
+      }
+  };
+
+  unsigned char* mine = lds + kw * kBufs * kSlot;
+  if (iters > 0) fetch(0, mine);
+  for (int it = 0; it < iters; ++it) {
+    const int k0 = key0(it);
+    unsigned char* slot = mine + (kBufs == 2 ? (it & 1) * kSlot : 0);
+    if constexpr (kDirect) {
+      wait_loads();
+      attn_barrier();
+      if (it + 1 < iters) fetch(it + 1, mine + ((it + 1) & 1) * kSlot);
+    } else {
+      if (RW > 1 || k0 < g_hi) put(slot);
+      if (it + 1 < iters) fetch(it + 1, slot);
+      wait_lds();
+      if constexpr (RW > 1) attn_barrier();
+    }
+    if (k0 < w_hi && k0 + KB > w_lo && k0 < g_hi) step(slot, k0);
+  }
+  l = both_sum(l);
+
+  // ---- the result: joined over the key groups, then either the row itself or this split's part of it
+  bool bad = false;  // (0 * inf from a key of a tile that this row does not see, or a value that is not finite that it does)
+  uint16_t* out = a.out + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
+  const int64_t stat = static_cast<int64_t>(pair) * a.rows + row;
+  const int64_t part = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row;
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (32 * o + 8 * (r / 4) < D) bad = bad || acc[o][r] != acc[o][r];
+    const float inv = some && l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    store_row<DT, D>(acc, some ? inv : 0.f, live ? out : nullptr, lane);
+    if (!some && live) {  // (0 * NaN above)
+#pragma unroll
+      for (int c = 0; c < D / 8; c += 2) *reinterpret_cast<u32x4*>(out + 8 * (c + h)) = u32x4{0u, 0u, 0u, 0u};
+    }
+    if (a.lse != nullptr && live && h == 0) a.lse[stat] = some ? __builtin_fmaf(m, a.c, __builtin_amdgcn_logf(l)) : kInf;
+    uint64_t redo = __ballot(bad && some && live);
+    redo = (redo | redo >> 32) & 0xffffffffull;
+    while (redo != 0) {
+      const int r = __builtin_ctzll(redo);
+      redo &= redo - 1;
+      const int row_r = __shfl(row, r), lo_r = __shfl(lo, r), hi_r = __shfl(hi, r);
+      float m2, l2, o2[2];
+      plain_row<DT, D, F8>(a, b, hk, row_r, lo_r, hi_r, lane, m2, l2, o2);
+      uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.n_queries + row_r / a.group) * a.n_q + hk * a.group + row_r % a.group) * D;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(o2[u] / l2));
+    }
+  } else {
+    // every key group's sums to LDS, scaled to the common maximum; then each thread adds up a few channels of a row
+    float2* stats = reinterpret_cast<float2*>(lds + 4 * 32 * (D + 4) * 4);
+    float* sums = reinterpret_cast<float*>(lds);
+    __syncthreads();
+    if (h == 0) stats[wave * 32 + lane] = float2{m, l};
+    __syncthreads();
+    float top = -kInf;
+#pragma unroll
+    for (int u = 0; u < KW; ++u) top = fmaxf(top, stats[(u * RW + rw) * 32 + (lane & 31)].x);
+    const float f = m == -kInf ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.c);
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * o + 8 * g < D)
+          *reinterpret_cast<float4*>(sums + (wave * 32 + (lane & 31)) * (D + 4) + 32 * o + 8 * g + 4 * h) =
+              float4{acc[o][4 * g] * f, acc[o][4 * g + 1] * f, acc[o][4 * g + 2] * f, acc[o][4 * g + 3] * f};
+    __syncthreads();
+    // wavefront (kw, rw) finishes rows rw * 32 + kw * (32 / KW) ..., D / 8 lanes a row
+    constexpr int kMine = 32 / KW, kLanes = 16;
+#pragma unroll 1
+    for (int first = 0; first < kMine; first += 64 / kLanes) {
+      const int r = kw * kMine + first + lane / kLanes, ch = lane % kLanes;
+      const int row_r = tile * 32 * RW + rw * 32 + r;
+      float top_r = -kInf, l_r = 0.f;
+#pragma unroll
+      for (int u = 0; u < KW; ++u) top_r = fmaxf(top_r, stats[(u * RW + rw) * 32 + r].x);
+#pragma unroll
+      for (int u = 0; u < KW; ++u) {
+        const float2 st = stats[(u * RW + rw) * 32 + r];
+        l_r += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top_r) * a.c);
+      }
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (ch < D / 8)
+#pragma unroll
+        for (int u = 0; u < KW; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += sums[((u * RW + rw) * 32 + r) * (D + 4) + ch * 8 + e];
+      bool wrong = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wrong = wrong || v[e] != v[e];
+      int lo_r = 0, hi_r = 0;
+      if (row_r < a.rows) key_range(a.mask, b, row_r / a.group, a.n_queries, a.n_keys, lo_r, hi_r);
+      const bool some_r = hi_r > lo_r;
+      const int slo = max(lo_r, g_lo), shi = min(hi_r, g_hi);
+      const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + row_r / a.group) * a.n_q + hk * a.group + row_r % a.group) * D;
+      const int64_t to_part = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_r;
+      if (row_r < a.rows && ch < D / 8) {
+        if (a.splits > 1) {
+          float4* dst = reinterpret_cast<float4*>(a.part + to_part * D + ch * 8);
+          dst[0] = float4{v[0], v[1], v[2], v[3]};
+          dst[1] = float4{v[4], v[5], v[6], v[7]};
+          if (ch == 0) part_stats(a, D)[to_part] = float2{top_r, l_r};
+        } else {
+          const float inv = some_r ? 1.f / l_r : 0.f;
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = some_r ? v[e] * inv : 0.f;
+          *reinterpret_cast<u32x4*>(a.out + to + ch * 8) = pack16<DT>(w);
+          if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(pair) * a.rows + row_r] = some_r ? __builtin_fmaf(top_r, a.c, __builtin_amdgcn_logf(l_r)) : kInf;
+        }
+      }
+      uint64_t redo = __ballot(wrong && row_r < a.rows && shi > slo);
+      while (redo != 0) {
+        const int at = __builtin_ctzll(redo) / kLanes * kLanes;
+        redo &= ~(0xffffull << at);
+        const int row_x = __shfl(row_r, at), lo_x = __shfl(slo, at), hi_x = __shfl(shi, at);
+        float m2, l2, o2[2];
+        plain_row<DT, D, F8>(a, b, hk, row_x, lo_x, hi_x, lane, m2, l2, o2);
+        const int64_t px = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_x;
+        uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.n_queries + row_x / a.group) * a.n_q + hk * a.group + row_x % a.group) * D;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (lane + 64 * u < D) {
+            if (a.splits > 1) a.part[px * D + lane + 64 * u] = o2[u];
+            else dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(o2[u] / l2));
+          }
+        if (a.splits > 1 && lane == 0) part_stats(a, D)[px] = float2{m2, l2};
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: a wavefront per row, lane l channels l and l + 64.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (at >= static_cast<int64_t>(a.batch) * a.n_kv * a.rows) return;
+  const int pair = static_cast<int>(at / a.rows), row = static_cast<int>(at - static_cast<int64_t>(pair) * a.rows);
+  const float2* stats = part_stats(a, D) + static_cast<int64_t>(pair) * a.splits * a.rows + row;
+  const float* part = a.part + (static_cast<int64_t>(pair) * a.splits * a.rows + row) * D;
+  float top = -kInf;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, stats[static_cast<int64_t>(s) * a.rows].x);
+  top = wave_max(top);
+  float l = 0.f, o[2] = {0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 st = stats[static_cast<int64_t>(s) * a.rows];
+    const float f = st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c);
+    l += st.y * f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 64 * u < D && st.x != -kInf) o[u] += part[static_cast<int64_t>(s) * a.rows * D + lane + 64 * u] * f;
+  }
+  const int b = pair / a.n_kv, hk = pair % a.n_kv;
+  const int i = row / a.group, hq = hk * a.group + row % a.group;
+  int lo, hi;
+  key_range(a.mask, b, i, a.n_queries, a.n_keys, lo, hi);
+  uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(hi > lo ? o[u] / l : 0.f));
+  if (a.lse != nullptr && lane == 0) a.lse[at] = hi > lo ? __builtin_fmaf(top, a.c, __builtin_amdgcn_logf(l)) : kInf;
+}
+
+// How a call is spread over the chip: wavefronts of the workgroup that take rows (4, 2 or 1), and splits of the keys.
+struct FwdPlan {
+  int row_waves, splits;
+};
+constexpr int kMaxSplits = 256;
+FwdPlan plan(int64_t pairs, int64_t rows, int64_t keys) {
+  const int cus = device_cu_count();
+  FwdPlan p{4, 1};
+  // Rows that fill 128-row workgroups two to a CU take those; otherwise smaller row tiles, whose wavefronts share the keys.
+  if (rows <= 32) p.row_waves = 1;
+  else if (rows <= 64 || pairs * ((rows + 127) / 128) < 2 * cus) p.row_waves = 2;
+  const int64_t groups = pairs * ((rows + 32 * p.row_waves - 1) / (32 * p.row_waves));
+  if (p.row_waves < 4 && groups > 0 && groups < 2 * cus) {
+    // too few workgroups for the chip: the keys in parts of at least two tiles for each of a workgroup's key groups
+    const int64_t want = (2 * cus + groups - 1) / groups, most = keys / (32 * (4 / p.row_waves) * 2);
+    const int64_t n = want < most ? want : most;
+    p.splits = static_cast<int>(n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n));
+  }
+  return p;
+}
+
+template <int DT, int D, bool F8>
+int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
+  a.splits = p.splits;
+  a.row_tiles = (a.rows + 32 * p.row_waves - 1) / (32 * p.row_waves);
+  const int64_t blocks = static_cast<int64_t>(a.batch) * a.n_kv * a.row_tiles * a.splits;
+  if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
+  const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+  switch (p.row_waves) {
+    case 1: hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 1>), grid, block, 0, s, a); break;
+    case 2: hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 2>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 4>), grid, block, 0, s, a); break;
+  }
+  if (int rc = check_launch("attn_fwd_kernel")) return rc;
+  if (a.splits > 1) {
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.n_kv * a.rows;
+    hipLaunchKernelGGL((attn_join_kernel<DT, D>), dim3(static_cast<unsigned>((rows + 3) / 4)), block, 0, s, a);
+    return check_launch("attn_join_kernel");
+  }
+  return WX_OK;
+}
+
+template <bool F8>
+int dispatch_fwd(FwdArgs& a, const FwdPlan& p, int head_dim, int dtype, hipStream_t s) {
+  if (dtype == WX_BF16) {
+    if (head_dim == 64) return launch_fwd<WX_BF16, 64, F8>(a, p, s);
+    if (head_dim == 80) return launch_fwd<WX_BF16, 80, F8>(a, p, s);
+    return launch_fwd<WX_BF16, 128, F8>(a, p, s);
+  }
+  if (head_dim == 64) return launch_fwd<WX_F16, 64, F8>(a, p, s);
+  if (head_dim == 80) return launch_fwd<WX_F16, 80, F8>(a, p, s);
+  return launch_fwd<WX_F16, 128, F8>(a, p, s);
+}
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+}  // namespace
+
+// Shared by the forward and the backward: sizes, types and strides that the kernels take.
+int attention_check(const char* who, int64_t batch, int n_q, int n_kv, int64_t n_queries, int64_t n_keys, int head_dim, int dtype,
+                    float scale) {
+  if (batch < 0 || n_q < 0 || n_kv < 0 || n_queries < 0 || n_keys < 0) return fail(WX_ERR_INVALID_ARGUMENT, "%s: negative size", who);
+  if (head_dim != 64 && head_dim != 80 && head_dim != 128)
+    return fail(WX_ERR_UNSUPPORTED, "%s: head_dim %d must be 64, 80 or 128", who, head_dim);
+  if (dtype != WX_BF16 && dtype != WX_F16) return fail(WX_ERR_UNSUPPORTED, "%s: dtype %d must be bf16 or fp16", who, dtype);
+  if (n_kv == 0 ? n_q != 0 : n_q % n_kv != 0)
+    return fail(WX_ERR_INVALID_ARGUMENT, "%s: %d query heads are no multiple of %d key / value heads", who, n_q, n_kv);
+  if (!(scale > 0.f) || !(scale < 1e30f)) return fail(WX_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", who);
+  const int64_t group = n_kv ? n_q / n_kv : 0;
+  if (n_keys > 0x3fffffffll || (group && n_queries > 0x3fffffffll / group) || batch > 0x7fffffffll / (n_kv ? n_kv : 1))
+    return fail(WX_ERR_UNSUPPORTED, "%s: more than 2^30 - 1 rows or keys", who);
+  return WX_OK;
+}
+
+// 16-byte rows, and `span` positions and `heads` heads of 2 (1) byte elements within 31 bits of a tile's first byte
+int attention_check_strides(const char* who, const char* name, const int64_t* st, int elem_bytes, int64_t span, int64_t heads) {
+  const int64_t unit = 16 / elem_bytes;
+  for (int i = 0; i < 3; ++i)
+    if (st[i] % unit != 0 || st[i] < 0) return fail(WX_ERR_UNSUPPORTED, "%s: %s's strides must be positive and keep rows 16-byte aligned", who, name);
+  const int64_t most = 0x7ff00000ll / elem_bytes;
+  if (st[2] > most / span || (heads > 1 && st[1] > (most - st[2] * span) / (heads - 1)))
+    return fail(WX_ERR_UNSUPPORTED, "%s: %s's strides are too large", who, name);
+  return WX_OK;
+}
+
+}  // namespace wx
+
+using namespace wx;
+
+extern "C" size_t wx_attention_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys,
+                                               int head_dim) {
+  if (batch <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_queries <= 0 || n_keys < 0 || head_dim <= 0) return 0;
+  const int64_t rows = n_queries * (n_q_heads / n_kv_heads);
+  const FwdPlan p = plan(batch * n_kv_heads, rows, n_keys);
+  return p.splits == 1 ? 0 : static_cast<size_t>(batch) * n_kv_heads * p.splits * rows * (head_dim + 2) * sizeof(float);
+}
+
+static int forward(const char* who, const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, bool f8,
+                   void* out, float* lse, const int32_t* key_ranges, const int32_t* key_lengths, int causal, int64_t batch,
+                   int n_q, int n_kv, int64_t n_queries, int64_t n_keys, int head_dim, const int64_t* qs, const int64_t* ks,
+                   const int64_t* vs, float scale, int dtype, void* workspace, size_t workspace_bytes, wx_stream_t stream) {
+  if (int rc = attention_check(who, batch, n_q, n_kv, n_queries, n_keys, head_dim, dtype, scale)) return rc;
+  if (!qs || !ks || !vs) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null strides", who);
+  if (batch == 0 || n_q == 0 || n_queries == 0) return WX_OK;
+  if (!q || !out || (n_keys > 0 && (!k || !v || (f8 && (!k_scale || !v_scale))))) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out)) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(key_ranges) & 7) return fail(WX_ERR_INVALID_ARGUMENT, "%s: key_ranges must be 8-byte aligned", who);
+  const int group = n_q / n_kv;
+  if (int rc = attention_check_strides(who, "q", qs, 2, 1, 1)) return rc;
+  if (int rc = attention_check_strides(who, "k", ks, f8 ? 1 : 2, 64, 1)) return rc;
+  if (int rc = attention_check_strides(who, "v", vs, f8 ? 1 : 2, 64, 1)) return rc;
+  FwdArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  for (int i = 0; i < 3; ++i) a.qs[i] = qs[i], a.ks[i] = ks[i], a.vs[i] = vs[i];
+  a.k_scale = k_scale, a.v_scale = v_scale;
+  a.out = static_cast<uint16_t*>(out), a.lse = lse;
+  a.mask = {reinterpret_cast<const int2*>(key_ranges), key_lengths, causal};
+  a.batch = static_cast<int>(batch), a.n_q = n_q, a.n_kv = n_kv, a.n_queries = static_cast<int>(n_queries), a.n_keys = static_cast<int>(n_keys);
+  a.group = group, a.rows = static_cast<int>(n_queries) * group;
+  a.c = scale * kLog2e;
+  const FwdPlan p = plan(batch * n_kv, a.rows, n_keys);
+  if (p.splits > 1) {
+    if (!workspace || workspace_bytes < wx_attention_workspace_bytes(batch, n_q, n_kv, n_queries, n_keys, head_dim))
+      return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_workspace_bytes)", who);
+    if (misaligned(workspace)) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
+    a.part = static_cast<float*>(workspace);
+  }
+  return f8 ? dispatch_fwd<true>(a, p, head_dim, dtype, as_stream(stream)) : dispatch_fwd<false>(a, p, head_dim, dtype, as_stream(stream));
+}
+
+extern "C" int wx_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_ranges,
+                                const int32_t* key_lengths, int causal, int64_t batch, int n_q_heads, int n_kv_heads,
+                                int64_t n_queries, int64_t n_keys, int head_dim, const int64_t q_strides[3], const int64_t k_strides[3],
+                                const int64_t v_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                wx_stream_t stream) {
+  return forward("wx_attention_fwd", q, k, v, nullptr, nullptr, false, out, lse, key_ranges, key_lengths, causal, batch, n_q_heads,
+                 n_kv_heads, n_queries, n_keys, head_dim, q_strides, k_strides, v_strides, scale, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int wx_cached_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                                   void* out, const int32_t* key_ranges, const int32_t* key_lengths, int causal, int64_t batch,
+                                   int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t capacity, int head_dim,
+                                   const int64_t q_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                   wx_stream_t stream) {
+  const int64_t st[3] = {n_kv_heads * capacity * head_dim, capacity * head_dim, head_dim};
+  return forward("wx_cached_attention", q, k_cache, v_cache, k_scale, v_scale, true, out, nullptr, key_ranges, key_lengths, causal, batch,
+                 n_q_heads, n_kv_heads, n_queries, capacity, head_dim, q_strides, st, st, scale, dtype, workspace, workspace_bytes, stream);
+}

@@ -520,6 +520,345 @@ __global__ __launch_bounds__(256) void mrope_table_kernel(const int64_t* __restr
   out[gid] = f32_to_bf16_bits(cv) | (f32_to_bf16_bits(sv) << 16);
 }
 
+// ------------------------------------------------------------------------------------------------
+// RMS norm of every head of q and k and the rotary embedding of the result in one pass, with its gradients.
+//   r = 1 / sqrt(mean(x^2) + eps),  n = x r w,  y = n cos + rotate_half(n) sin
+//   backward: gn = gy cos + rotate_half^T(gy sin),  dw = sum gn x r,  dx = r (gn w - x r^2 mean(gn w x))
+// All in fp32, rounded once, where a norm op and a rotary op round (and move) the heads in between.  HBM-bound: the forward reads
+// and writes the heads once, the backward reads them and the gradient and writes as much as one of the two.  As in
+// mrope_rows_kernel a thread owns 16 bytes of a head's channels of one token and walks over heads; a head's sums are exchanged
+// between its lanes.  cos and sin come from the packed table or from the position ids: there the angle, and what is left of it beside
+// whole turns (2 pi in two parts), is formed in 64 bits, since the fp32 product is off by 1e-3 at position 30000 and by 0.05 at 10^6.
+struct NormRope {
+  const void *q, *k;          // [batch, heads, seq, head_dim] through strides
+  const void *gq, *gk;        // backward: the outputs' gradients, through strides
+  const void *wq, *wk;        // [head_dim]
+  void *q_out, *k_out;        // [batch, heads, seq, head_dim], contiguous
+  const void *cos_t, *sin_t;  // as for mrope_rows_kernel
+  float* partial;             // backward: [workgroups, 2, head_dim] sums of the weights' gradients, or null
+  Strides sq, sk, sgq, sgk;
+  int64_t n_tokens, seq;
+  int n_q, n_kv, head_dim, heads_per_group;
+  float eps;
+  AxisTable ax;
+};
+
+template <int L>
+__device__ __forceinline__ float head_sum(float v, int lanes) {
+  if constexpr (L == 16) {
+#define WX_ROR_ADD(N) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true))
+    WX_ROR_ADD(8);
+    WX_ROR_ADD(4);
+    WX_ROR_ADD(2);
+    WX_ROR_ADD(1);
+#undef WX_ROR_ADD
+  } else {
+    for (int d = 1; d < lanes; d <<= 1) v += __shfl_xor(v, d);
+  }
+  return v;
+}
+
+// cos and sin of channels [d0, d0 + 16 / size) of a token, in fp32
+template <int DT, int SRC>
+__device__ __forceinline__ void cos_sin_f32(const NormRope& a, int64_t token, int d0, bool hi, float* c, float* s) {
+  constexpr int kEpc = 16 / Elem<DT>::kBytes;
+  const int half = a.head_dim / 2;
+  if constexpr (SRC == kSrcPacked) {
+    const int width = static_cast<int>(reinterpret_cast<uintptr_t>(a.sin_t));
+    const uint32_t* t = static_cast<const uint32_t*>(a.cos_t) + token * width + ((hi && width != a.head_dim) ? d0 - half : d0);
+#pragma unroll
+    for (int i = 0; i < kEpc; i += 4) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(t + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[i + e] = __uint_as_float(v[e] << 16);
+        s[i + e] = __uint_as_float(v[e] & 0xffff0000u);
+      }
+    }
+  } else {
+    const int64_t pos = static_cast<const int64_t*>(a.cos_t)[a.ax.axis[d0] * a.n_tokens + token];
+    const float* inv_freq = static_cast<const float*>(a.sin_t) + (hi ? d0 - half : d0);
+#pragma unroll
+    for (int e = 0; e < kEpc; ++e) {
+      const double angle = static_cast<double>(pos) * static_cast<double>(inv_freq[e]);
+      const double turns = __builtin_rint(angle * 0.15915494309189535);
+      const double rest = __builtin_fma(-turns, 2.4492935982947064e-16, __builtin_fma(-turns, 6.283185307179586, angle));
+      const float near = static_cast<float>(rest), err = static_cast<float>(rest - static_cast<double>(near));
+      float sv, cv;
+      sincosf(near, &sv, &cv);
+      c[e] = __builtin_fmaf(-sv, err, cv);  // (to fp32 of the cosine also where it is small)
+      s[e] = __builtin_fmaf(cv, err, sv);
+    }
+  }
+}
+
+template <int DT, int L>
+__device__ __forceinline__ const u32x4* head_chunk(const void* p, const Strides& st, int64_t b, int h, int64_t s, int d0) {
+  return reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + (b * st.b + h * st.h + s * st.s + d0) * Elem<DT>::kBytes);
+}
+
+template <int DT, int L, int SRC>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRope a) {
+  constexpr int kEpc = 16 / Elem<DT>::kBytes;
+  const int lanes = L ? L : a.head_dim / kEpc;
+  const int64_t gid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int chunk = static_cast<int>(gid % lanes), d0 = chunk * kEpc;
+  int64_t token = gid / lanes;
+  const bool live = token < a.n_tokens, hi = chunk >= lanes / 2;
+  if (!live) token = a.n_tokens - 1;  // (takes part in the lane exchanges)
+  const int64_t b = token / a.seq, s = token - b * a.seq;
+  const int first = blockIdx.y * a.heads_per_group, last = min(first + a.heads_per_group, a.n_q + a.n_kv);
+  float c[kEpc], sn[kEpc], w[2][kEpc];
+  u32x4 raw[kRowsHeadBatch];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < kRowsHeadBatch; ++u)
+      if (h0 + u < last)
+        raw[u] = __builtin_nontemporal_load(h0 + u < a.n_q ? head_chunk<DT, L>(a.q, a.sq, b, h0 + u, s, d0) : head_chunk<DT, L>(a.k, a.sk, b, h0 + u - a.n_q, s, d0));
+  };
+  load(first);
+  if (a.n_q > 0) unpack16<DT>(static_cast<const u32x4*>(a.wq)[chunk], w[0]);
+  if (a.n_kv > 0) unpack16<DT>(static_cast<const u32x4*>(a.wk)[chunk], w[1]);
+  cos_sin_f32<DT, SRC>(a, token, d0, hi, c, sn);
+  const float sign = hi ? 1.f : -1.f;  // rotate_half(n) = (-n_hi, n_lo)
+#pragma unroll
+  for (int e = 0; e < kEpc; ++e) sn[e] *= sign;
+  for (int h0 = first; h0 < last; h0 += kRowsHeadBatch) {
+    if (h0 > first) load(h0);
+#pragma unroll
+    for (int u = 0; u < kRowsHeadBatch; ++u) {
+      const int h = h0 + u;
+      if (h >= last) continue;  // uniform over the workgroup
+      const bool is_q = h < a.n_q;
+      float x[kEpc], n[kEpc], o[kEpc], sum = 0.f;
+      unpack16<DT>(raw[u], x);
+#pragma unroll
+      for (int e = 0; e < kEpc; ++e) sum = __builtin_fmaf(x[e], x[e], sum);
+      const float r = rsqrtf(head_sum<L>(sum, lanes) / a.head_dim + a.eps);
+#pragma unroll
+      for (int e = 0; e < kEpc; ++e) n[e] = x[e] * r * (is_q ? w[0][e] : w[1][e]);
+#pragma unroll
+      for (int e = 0; e < kEpc; ++e) {
+        float np;
+        if constexpr (L == 16) np = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(n[e]), 0x128, 0xF, 0xF, true));
+        else np = __shfl_xor(n[e], lanes / 2);
+        o[e] = __builtin_fmaf(n[e], c[e], np * sn[e]);
+      }
+      if (live) {
+        char* out = static_cast<char*>(is_q ? a.q_out : a.k_out);
+        const int64_t heads = is_q ? a.n_q : a.n_kv, hh = is_q ? h : h - a.n_q;
+        __builtin_nontemporal_store(pack16<DT>(o), reinterpret_cast<u32x4*>(out + (((b * heads + hh) * a.seq + s) * a.head_dim + d0) * Elem<DT>::kBytes));
+      }
+    }
+  }
+}
+
+// The gradients.  A workgroup takes every gridDim.x-th run of tokens of its group of heads and keeps its sums of the weights'
+// gradients in registers until it is through.
+constexpr int kNormBwdBatch = 3;
+template <int DT, int L, int SRC>
+__global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(NormRope a) {
+  constexpr int kEpc = 16 / Elem<DT>::kBytes;
+  const int lanes = L ? L : a.head_dim / kEpc, per = 256 / lanes;
+  const int chunk = threadIdx.x % lanes, d0 = chunk * kEpc;
+  const bool hi = chunk >= lanes / 2;
+  const int first = blockIdx.y * a.heads_per_group, last = min(first + a.heads_per_group, a.n_q + a.n_kv);
+  float w[2][kEpc], dw[2][kEpc] = {};
+  if (a.n_q > 0) unpack16<DT>(static_cast<const u32x4*>(a.wq)[chunk], w[0]);
+  if (a.n_kv > 0) unpack16<DT>(static_cast<const u32x4*>(a.wk)[chunk], w[1]);
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * per; t0 < a.n_tokens; t0 += static_cast<int64_t>(gridDim.x) * per) {
+    int64_t token = t0 + threadIdx.x / lanes;
+    const bool live = token < a.n_tokens;
+    if (!live) token = a.n_tokens - 1;
+    const int64_t b = token / a.seq, s = token - b * a.seq;
+    u32x4 rx[kNormBwdBatch], rg[kNormBwdBatch];
+    auto load = [&](int h0) {
+#pragma unroll
+      for (int u = 0; u < kNormBwdBatch; ++u) {
+        const int h = h0 + u;
+        if (h >= last) continue;
+        rx[u] = __builtin_nontemporal_load(h < a.n_q ? head_chunk<DT, L>(a.q, a.sq, b, h, s, d0) : head_chunk<DT, L>(a.k, a.sk, b, h - a.n_q, s, d0));
+        rg[u] = __builtin_nontemporal_load(h < a.n_q ? head_chunk<DT, L>(a.gq, a.sgq, b, h, s, d0) : head_chunk<DT, L>(a.gk, a.sgk, b, h - a.n_q, s, d0));
+      }
+    };
+    load(first);
+    float c[kEpc], sn[kEpc];
+    cos_sin_f32<DT, SRC>(a, token, d0, hi, c, sn);
+    const float sign = hi ? -1.f : 1.f;  // rotate_half^T(y) = (y_hi, -y_lo), of the partner's product with its own sine
+#pragma unroll
+    for (int e = 0; e < kEpc; ++e) sn[e] = sign * __shfl_xor(sn[e], lanes / 2);
+    for (int h0 = first; h0 < last; h0 += kNormBwdBatch) {
+      if (h0 > first) load(h0);
+#pragma unroll
+      for (int u = 0; u < kNormBwdBatch; ++u) {
+        const int h = h0 + u;
+        if (h >= last) continue;
+        const bool is_q = h < a.n_q;
+        float x[kEpc], g[kEpc], gn[kEpc], o[kEpc], s1 = 0.f, s2 = 0.f;
+        unpack16<DT>(rx[u], x);
+        unpack16<DT>(rg[u], g);
+#pragma unroll
+        for (int e = 0; e < kEpc; ++e) {
+          float gp;
+          if constexpr (L == 16) gp = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(g[e]), 0x128, 0xF, 0xF, true));
+          else gp = __shfl_xor(g[e], lanes / 2);
+          gn[e] = __builtin_fmaf(g[e], c[e], gp * sn[e]);
+          s1 = __builtin_fmaf(x[e], x[e], s1);
+          s2 = __builtin_fmaf(gn[e] * (is_q ? w[0][e] : w[1][e]), x[e], s2);
+        }
+        const float r = rsqrtf(head_sum<L>(s1, lanes) / a.head_dim + a.eps);
+        const float back = r * r * (head_sum<L>(s2, lanes) / a.head_dim);
+#pragma unroll
+        for (int e = 0; e < kEpc; ++e) o[e] = r * __builtin_fmaf(-x[e], back, gn[e] * (is_q ? w[0][e] : w[1][e]));
+        if (live) {
+          const float f = r;
+#pragma unroll
+          for (int e = 0; e < kEpc; ++e) {
+            if (is_q) dw[0][e] = __builtin_fmaf(gn[e], x[e] * f, dw[0][e]);
+            else dw[1][e] = __builtin_fmaf(gn[e], x[e] * f, dw[1][e]);
+          }
+          char* out = static_cast<char*>(is_q ? a.q_out : a.k_out);
+          if (out != nullptr) {
+            const int64_t heads = is_q ? a.n_q : a.n_kv, hh = is_q ? h : h - a.n_q;
+            __builtin_nontemporal_store(pack16<DT>(o), reinterpret_cast<u32x4*>(out + (((b * heads + hh) * a.seq + s) * a.head_dim + d0) * Elem<DT>::kBytes));
+          }
+        }
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+  __shared__ float sums[4][2][kMaxHeadDim];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < kEpc; ++e) {
+      float v = dw[i][e];
+      for (int d = lanes; d < 64; d <<= 1) v += __shfl_xor(v, d);
+      if ((threadIdx.x & 63) < lanes) sums[threadIdx.x >> 6][i][d0 + e] = v;
+    }
+  __syncthreads();
+  const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+  for (int i = threadIdx.x; i < 2 * a.head_dim; i += 256) {
+    const int which = i / a.head_dim, d = i - which * a.head_dim;
+    a.partial[block * 2 * a.head_dim + i] = (sums[0][which][d] + sums[1][which][d]) + (sums[2][which][d] + sums[3][which][d]);
+  }
+}
+
+// The weights' gradients from the workgroups' sums: 16 columns a workgroup, 64 threads to a column, in a fixed order.
+template <int DT>
+__global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __restrict__ partial, void* __restrict__ dwq, void* __restrict__ dwk,
+                                                                int n_partials, int head_dim) {
+  __shared__ float sums[64][17];
+  const int col = threadIdx.x % 16, group = threadIdx.x / 16, c = blockIdx.x * 16 + col;
+  float acc = 0.f;
+  for (int p = group; p < n_partials; p += 8 * 64) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = p + u * 64 < n_partials ? partial[static_cast<int64_t>(p + u * 64) * 2 * head_dim + c] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc += v[u];
+  }
+  sums[group][col] = acc;
+  __syncthreads();
+#pragma unroll
+  for (int half = 32; half > 0; half >>= 1) {
+    if (group < half) sums[group][col] += sums[group + half][col];
+    __syncthreads();
+  }
+  if (group != 0) return;
+  void* dst = c < head_dim ? dwq : dwk;
+  const int d = c < head_dim ? c : c - head_dim;
+  if (dst == nullptr) return;
+  if constexpr (DT == WX_F32) static_cast<float*>(dst)[d] = sums[0][col];
+  else static_cast<uint16_t*>(dst)[d] = static_cast<uint16_t>(Elem<DT>::store(sums[0][col]));
+}
+
+// Workgroups of the forward (backward: at most kNormBlocks partial sums): tokens over x, and where those alone leave CUs idle
+// groups of heads over y.
+constexpr int64_t kNormBlocks = 2048;
+struct NormGrid {
+  int64_t x;
+  int y, heads_per_group;
+};
+NormGrid norm_grid(int64_t n_tokens, int heads, int lanes, bool backward) {
+  const int64_t cus = device_cu_count();
+  NormGrid g;
+  g.x = (n_tokens * lanes + 255) / 256;
+  const int batch = backward ? kNormBwdBatch : kRowsHeadBatch;
+  int groups = 1;
+  if (g.x < 4 * cus) {
+    const int64_t want = (4 * cus + g.x - 1) / (g.x > 0 ? g.x : 1), most = (heads + batch - 1) / batch;
+    groups = static_cast<int>(want < most ? want : most);
+  }
+  if (groups < 1) groups = 1;
+  if (groups > 256) groups = 256;
+  g.heads_per_group = (heads + groups - 1) / groups;
+  g.y = (heads + g.heads_per_group - 1) / g.heads_per_group;
+  if (backward && g.x * g.y > kNormBlocks) g.x = kNormBlocks / g.y;
+  return g;
+}
+
+template <int SRC>
+int launch_norm_rope(NormRope& a, bool backward, int64_t batch, void* dwq, void* dwk, const int sec[3], int layout, int dtype, wx_stream_t stream) {
+  const char* who = backward ? "wx_qk_norm_rope_bwd" : "wx_qk_norm_rope";
+  if (batch < 0 || a.seq < 0 || a.n_q < 0 || a.n_kv < 0) return fail(WX_ERR_INVALID_ARGUMENT, "%s: negative size", who);
+  if (a.head_dim <= 0 || a.head_dim % 16 != 0 || a.head_dim > kMaxHeadDim)
+    return fail(WX_ERR_UNSUPPORTED, "%s: head_dim %d must be a multiple of 16 and <= %d", who, a.head_dim, kMaxHeadDim);
+  if (!(a.eps >= 0.f)) return fail(WX_ERR_INVALID_ARGUMENT, "%s: eps must be non-negative", who);
+  if (dtype != WX_F32 && dtype != WX_F16 && dtype != WX_BF16) return fail(WX_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+  if (SRC == kSrcPacked && dtype != WX_BF16) return fail(WX_ERR_UNSUPPORTED, "%s: the packed table is bf16", who);
+  if (!sec) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null section", who);
+  a.n_tokens = batch * a.seq;
+  const int heads = a.n_q + a.n_kv, epc = dtype == WX_F32 ? 4 : 8, lanes = a.head_dim / epc;
+  if (int rc = build_axis_table(sec, a.head_dim, layout, a.ax)) return rc;
+  bool rows_ok = lanes >= 2 && lanes <= 64 && (lanes & (lanes - 1)) == 0;
+  for (int c = 0; c < a.head_dim / 8 && rows_ok; ++c) rows_ok = a.ax.uniform[c] != 0;
+  if (!rows_ok) return fail(WX_ERR_UNSUPPORTED, "%s: needs a head of 2..64 16-byte chunks (a power of two) and sections that end on chunk boundaries", who);
+  hipStream_t s = as_stream(stream);
+  const dim3 block(256);
+  const bool empty = a.n_tokens == 0 || heads == 0;
+  if (empty && !(backward && (dwq || dwk))) return WX_OK;
+  NormGrid g{0, 0, 1};
+  if (!empty) {
+    if (!a.cos_t || (SRC != kSrcPacked && !a.sin_t) || (a.n_q && (!a.q || !a.wq || (backward && !a.gq) || (!backward && !a.q_out))) ||
+        (a.n_kv && (!a.k || !a.wk || (backward && !a.gk) || (!backward && !a.k_out))))
+      return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    for (const void* p : {a.q, a.k, a.gq, a.gk, a.wq, a.wk, static_cast<const void*>(a.q_out), static_cast<const void*>(a.k_out)})
+      if (reinterpret_cast<uintptr_t>(p) & 15) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
+    for (const Strides* st : {&a.sq, &a.sk, &a.sgq, &a.sgk})
+      if (st->b % epc != 0 || st->h % epc != 0 || st->s % epc != 0) return fail(WX_ERR_UNSUPPORTED, "%s: strides must keep rows 16-byte aligned", who);
+    if constexpr (SRC == kSrcPacked) {
+      if (reinterpret_cast<uintptr_t>(a.cos_t) & 15) return fail(WX_ERR_INVALID_ARGUMENT, "%s: the table must be 16-byte aligned", who);
+      a.sin_t = reinterpret_cast<const void*>(static_cast<uintptr_t>(packed_table_width(a.ax, a.head_dim)));
+    }
+    g = norm_grid(a.n_tokens, heads, lanes, backward);
+    if (g.x > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
+    a.heads_per_group = g.heads_per_group;
+    const dim3 grid(static_cast<unsigned>(g.x), static_cast<unsigned>(g.y));
+#define WX_NORM(DT, L)                                                                                     \
+  if (backward) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<DT, L, SRC>), grid, block, 0, s, a);           \
+  else hipLaunchKernelGGL((qk_norm_rope_kernel<DT, L, SRC>), grid, block, 0, s, a)
+    if constexpr (SRC == kSrcPacked) {
+      if (lanes == 16) { WX_NORM(WX_BF16, 16); } else { WX_NORM(WX_BF16, 0); }
+    } else if (dtype == WX_F32) {
+      WX_NORM(WX_F32, 0);
+    } else if (dtype == WX_F16) {
+      if (lanes == 16) { WX_NORM(WX_F16, 16); } else { WX_NORM(WX_F16, 0); }
+    } else {
+      if (lanes == 16) { WX_NORM(WX_BF16, 16); } else { WX_NORM(WX_BF16, 0); }
+    }
+#undef WX_NORM
+    if (int rc = check_launch(who)) return rc;
+  }
+  if (!backward || (!dwq && !dwk)) return WX_OK;
+  const dim3 sum_grid(static_cast<unsigned>(2 * a.head_dim / 16)), sum_block(1024);
+  const int n = static_cast<int>(g.x * g.y);
+  if (dtype == WX_F32) hipLaunchKernelGGL(norm_weight_grad_kernel<WX_F32>, sum_grid, sum_block, 0, s, a.partial, dwq, dwk, n, a.head_dim);
+  else if (dtype == WX_F16) hipLaunchKernelGGL(norm_weight_grad_kernel<WX_F16>, sum_grid, sum_block, 0, s, a.partial, dwq, dwk, n, a.head_dim);
+  else hipLaunchKernelGGL(norm_weight_grad_kernel<WX_BF16>, sum_grid, sum_block, 0, s, a.partial, dwq, dwk, n, a.head_dim);
+  return check_launch("norm_weight_grad_kernel");
+}
+
 }  // namespace
 }  // namespace wx
 
@@ -644,4 +983,43 @@ extern "C" int wx_qkv_rope_bwd(const void* grad_q, const void* grad_k, const voi
     if (int rc = check_launch("qkv_rope_bwd_kernel")) return rc;
   }
   return grad_bias ? launch_column_sums(partial, grad_bias, blocks, heads * 128, s) : WX_OK;
+}
+
+extern "C" int wx_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, float eps, const void* table_or_positions,
+                               const float* inv_freq, void* q_out, void* k_out, int64_t batch, int64_t seq, int n_q_heads, int n_kv_heads,
+                               int head_dim, const int64_t q_strides[3], const int64_t k_strides[3], const int mrope_section[3], int layout,
+                               int dtype, wx_stream_t stream) {
+  using namespace wx;
+  if (!q_strides || !k_strides) return fail(WX_ERR_INVALID_ARGUMENT, "wx_qk_norm_rope: null strides");
+  NormRope a{};
+  a.q = q, a.k = k, a.wq = q_weight, a.wk = k_weight, a.eps = eps, a.cos_t = table_or_positions, a.sin_t = inv_freq, a.q_out = q_out, a.k_out = k_out;
+  a.seq = seq, a.n_q = n_q_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
+  a.sq = {q_strides[0], q_strides[1], q_strides[2]}, a.sk = {k_strides[0], k_strides[1], k_strides[2]};
+  return inv_freq ? launch_norm_rope<kSrcPositions>(a, false, batch, nullptr, nullptr, mrope_section, layout, dtype, stream)
+                  : launch_norm_rope<kSrcPacked>(a, false, batch, nullptr, nullptr, mrope_section, layout, dtype, stream);
+}
+
+extern "C" size_t wx_qk_norm_rope_bwd_workspace_bytes(int head_dim) {
+  return head_dim <= 0 ? 0 : static_cast<size_t>(wx::kNormBlocks) * 2 * head_dim * sizeof(float);
+}
+
+extern "C" int wx_qk_norm_rope_bwd(const void* grad_q_out, const void* grad_k_out, const void* q, const void* k, const void* q_weight,
+                                   const void* k_weight, float eps, const void* table_or_positions, const float* inv_freq, void* grad_q,
+                                   void* grad_k, void* grad_q_weight, void* grad_k_weight, int64_t batch, int64_t seq, int n_q_heads,
+                                   int n_kv_heads, int head_dim, const int64_t gq_strides[3], const int64_t gk_strides[3],
+                                   const int64_t q_strides[3], const int64_t k_strides[3], const int mrope_section[3], int layout, int dtype,
+                                   void* workspace, size_t workspace_bytes, wx_stream_t stream) {
+  using namespace wx;
+  const char* who = "wx_qk_norm_rope_bwd";
+  if (!q_strides || !k_strides || !gq_strides || !gk_strides) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null strides", who);
+  if ((grad_q_weight || grad_k_weight) && (!workspace || workspace_bytes < wx_qk_norm_rope_bwd_workspace_bytes(head_dim)))
+    return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_qk_norm_rope_bwd_workspace_bytes)", who);
+  NormRope a{};
+  a.gq = grad_q_out, a.gk = grad_k_out, a.q = q, a.k = k, a.wq = q_weight, a.wk = k_weight, a.eps = eps, a.cos_t = table_or_positions, a.sin_t = inv_freq;
+  a.q_out = grad_q, a.k_out = grad_k, a.partial = (grad_q_weight || grad_k_weight) ? static_cast<float*>(workspace) : nullptr;
+  a.seq = seq, a.n_q = n_q_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
+  a.sq = {q_strides[0], q_strides[1], q_strides[2]}, a.sk = {k_strides[0], k_strides[1], k_strides[2]};
+  a.sgq = {gq_strides[0], gq_strides[1], gq_strides[2]}, a.sgk = {gk_strides[0], gk_strides[1], gk_strides[2]};
+  return inv_freq ? launch_norm_rope<kSrcPositions>(a, true, batch, grad_q_weight, grad_k_weight, mrope_section, layout, dtype, stream)
+                  : launch_norm_rope<kSrcPacked>(a, true, batch, grad_q_weight, grad_k_weight, mrope_section, layout, dtype, stream);
 }

@@ -98,6 +98,37 @@ def qkv_rope_bwd(grad_q, grad_k, grad_v, table, batch, seq, n_q_heads, n_kv_head
     return native.qkv_rope_bwd(grad_q, grad_k, grad_v, table, batch, seq, n_q_heads, n_kv_heads, want_bias)
 
 
+def qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout: str = "hf"):
+    """No counterpart in backend.py: the norm of q and k per head with the rotary embedding of the result."""
+    return native.qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout)
+
+
+def qk_norm_rope_bwd(grad_q, grad_k, q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout: str = "hf",
+                     want=(True, True, True, True)):
+    """No counterpart in backend.py: the gradients of qk_norm_rope."""
+    return native.qk_norm_rope_bwd(grad_q, grad_k, q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout, want)
+
+
+def attention_fwd(q, k, v, key_ranges=None, key_lengths=None, causal=False, scale=None, want_lse=False):
+    """No counterpart in backend.py: attention under key ranges (act.py:616-637's mask among others)."""
+    return native.attention_fwd(q, k, v, key_ranges, key_lengths, causal, scale, want_lse)
+
+
+def attention_bwd(grad_out, q, k, v, out, lse, key_ranges=None, key_lengths=None, causal=False, scale=None):
+    """No counterpart in backend.py: the gradients of attention_fwd."""
+    return native.attention_bwd(grad_out, q, k, v, out, lse, key_ranges, key_lengths, causal, scale)
+
+
+def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths=None):
+    """No counterpart in backend.py: keys and values quantised into a cache."""
+    return native.kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths)
+
+
+def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key_lengths=None, causal=False, scale=None):
+    """No counterpart in backend.py: attention over such a cache."""
+    return native.cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges, key_lengths, causal, scale)
+
+
 def get_rope_index(input_ids, image_grid_thw, video_grid_thw, second_per_grid_ts, attention_mask,
                    spatial_merge_size, image_token_id, video_token_id, vision_start_token_id, tokens_per_second):
     """backend.py:302-352 (forwards to the native op named rope_index)."""

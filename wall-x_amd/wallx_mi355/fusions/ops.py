@@ -17,7 +17,7 @@ import warnings
 
 import torch
 
-from .. import _lib
+from .. import _lib, native
 from . import backend
 
 # The forwards and backwards below hand plain calls to the native host module first (_lib.host(): checks, outputs and
@@ -472,6 +472,155 @@ def qkv_projection_with_rope(hidden_states, qkv_weight, qkv_bias, rope_table, nu
     q, k, v = out.split([nq * D, nkv * D, nkv * D], dim=-1)
     return (q.view(B, S, nq, D).transpose(1, 2), k.view(B, S, nkv, D).transpose(1, 2),
             v.view(B, S, nkv, D).transpose(1, 2))
+
+
+# ----------------------------------------------------------------------------- norm of q and k with M-RoPE
+class QKNormRoPE(torch.autograd.Function):
+    """The RMS norm of every head of q and k and the rotary embedding of the result in one launch; the backward recomputes
+    the norm from q and k, which are all it keeps."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout):
+        ctx.save_for_backward(q, k, q_weight, k_weight, source, inv_freq)
+        ctx.rope = (mrope_section, eps, layout)
+        return backend.qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_q, grad_k):
+        q, k, q_weight, k_weight, source, inv_freq = ctx.saved_tensors
+        grads = backend.qk_norm_rope_bwd(grad_q, grad_k, q, k, q_weight, k_weight, source, inv_freq, *ctx.rope, want=ctx.needs_input_grad[:4])
+        return (*grads, None, None, None, None, None)
+
+
+def _qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout):
+    for name, t in (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
+        if t.is_cpu:
+            raise RuntimeError(f"[Error] The input `{name}` of qk_norm_rope op is on the device: CPU!")
+    if len(mrope_section) != 3:
+        raise RuntimeError("[Error] The input `mrope_section` of qk_norm_rope op must be a list of 3 integers!")
+    section = tuple(int(v) for v in mrope_section)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+        return QKNormRoPE.apply(q, k, q_weight, k_weight, source, inv_freq, section, eps, layout)
+    return backend.qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, section, eps, layout)
+
+
+def qk_norm_rope_from_table(q, k, q_weight, k_weight, table, mrope_section, eps=1e-6, layout="hf"):
+    """(q', k') = multimodal_rope_from_table of the RMS norm of q and k per head: not in the reference's op set, for decoders that
+    norm their queries and keys.
+
+        n = x * rsqrt(mean(x^2, -1) + eps) * weight;  q', k' = M-RoPE(n)
+
+    q [B, Hq, S, D], k [B, Hkv, S, D] through their strides, weights [D] shared by the heads; contiguous outputs.  Everything
+    between the input and the output is fp32 with one rounding (a norm op followed by the rope op rounds three times).  bf16;
+    `table`, `mrope_section` and `layout` as for multimodal_rope_from_table.  Differentiable in q, k and both weights."""
+    return _qk_norm_rope(q, k, q_weight, k_weight, table, None, mrope_section, eps, layout)
+
+
+def qk_norm_rope_from_positions(q, k, q_weight, k_weight, position_ids, inv_freq, mrope_section, eps=1e-6, layout="hf"):
+    """qk_norm_rope_from_table with the angles evaluated from position_ids [3, B, S] int64 and inv_freq [D / 2] fp32 (to better
+    than the fp32 product, at any position); bf16, fp16 or fp32."""
+    return _qk_norm_rope(q, k, q_weight, k_weight, position_ids.contiguous(), inv_freq.to(torch.float32).contiguous(), mrope_section, eps, layout)
+
+
+# ----------------------------------------------------------------------------- attention
+class Attention(torch.autograd.Function):
+    """Keeps q, k, v, the output and a number per row of the scores; the backward recomputes the probabilities."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, key_ranges, key_lengths, causal, scale):
+        out, lse = backend.attention_fwd(q, k, v, key_ranges, key_lengths, causal, scale, want_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, key_ranges, key_lengths)
+        ctx.mask = (causal, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, key_ranges, key_lengths = ctx.saved_tensors
+        grads = backend.attention_bwd(grad_out, q, k, v, out, lse, key_ranges, key_lengths, *ctx.mask)
+        return (*(g if w else None for g, w in zip(grads, ctx.needs_input_grad)), None, None, None, None)
+
+
+def attention(q, k, v, key_ranges=None, key_lengths=None, causal=False, scale=None):
+    """softmax(scale q k^T) v, [B, Hq, Sq, D] over token-major memory (what the o projection reads without a copy); stands where
+    the reference calls scaled_dot_product_attention or flash attention (vl.py:868-893, 1000-1042, 1108-1130).
+
+    q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D] with Hq a multiple of Hkv, bf16 or fp16, D 64, 80 or 128, read through their strides;
+    scale defaults to D ** -0.5.  Query i of row b sees the keys from max(0, key_ranges[b, i, 0]) up to, not including, the
+    smallest of Sk, key_ranges[b, i, 1], key_lengths[b] and, with causal=True, key_lengths[b] - Sq + i + 1 (Sk without lengths): the
+    queries are the last Sq keys.  key_ranges int32 [B, Sq, 2] (attention_key_ranges builds the model's), key_lengths int32 [B], on
+    the device and never read by the host.  A query that sees no key gets zeros, and keys that a query does not see do not
+    influence its row whatever they hold.  Few queries over many keys (generation) are spread over the keys.  Differentiable in q, k
+    and v; the backward writes the same bits every time."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.is_cpu:
+            raise RuntimeError(f"[Error] The input `{name}` of attention op is on the device: CPU!")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return Attention.apply(q, k, v, key_ranges, key_lengths, causal, scale)
+    return backend.attention_fwd(q, k, v, key_ranges, key_lengths, causal, scale)[0]
+
+
+def attention_key_ranges(token_types, attention_mask=None):
+    """key_ranges int32 [B, S, 2] of the reference's mask (act.py:616-637) for `attention`: causal, and the action tokens of a row
+    (token_types [B, S], nonzero; one run of positions, as the data pipeline lays them out) see each other.  attention_mask
+    [B, S], nonzero for the tokens that count: padding on either side, which sees nothing and is seen by none.  In checked mode
+    (native.set_checked) rows whose action tokens or unpadded tokens are not one run raise."""
+    if token_types.dim() != 2 or (attention_mask is not None and attention_mask.shape != token_types.shape):
+        raise RuntimeError("token_types and attention_mask must be [batch, seq]")
+    S = token_types.size(1)
+    types = token_types != 0
+    at = torch.arange(S, device=types.device)
+    if S == 0:
+        return torch.zeros((*types.shape, 2), dtype=torch.int32, device=types.device)
+    if attention_mask is None:
+        lo, end, keep = torch.zeros_like(types, dtype=torch.int64), S, None
+    else:
+        keep = attention_mask != 0
+        types = types & keep
+        lo = torch.where(keep, at, S).amin(1, keepdim=True).expand(types.shape)
+        end = torch.where(keep, at + 1, 0).amax(1, keepdim=True)
+    if native.is_checked():
+        for name, x in (("action", types), ("unpadded", keep)):
+            if x is not None and bool((x[:, 1:] & ~x[:, :-1]).sum(1).add(x[:, 0]).gt(1).any()):
+                raise ValueError(f"attention_key_ranges: the {name} tokens of a row are not one run")
+    block_end = torch.where(types, at + 1, 0).amax(1, keepdim=True)
+    hi = torch.where(types, torch.maximum(block_end, at + 1), at + 1)
+    if keep is not None:
+        hi = torch.where(keep, torch.minimum(hi, torch.as_tensor(end)), lo)
+    return torch.stack((lo, hi), -1).to(torch.int32)
+
+
+# ----------------------------------------------------------------------------- quantised key / value cache
+def quantized_kv_cache(batch, num_key_value_heads, capacity, head_dim, device):
+    """(k_cache, v_cache, k_scale, v_scale) for kv_cache_write and cached_attention: e4m3 codes [B, Hkv, capacity, D] and fp32 scales
+    [B, Hkv, capacity], half of a bf16 cache's bytes.  Zeroed."""
+    codes = [torch.zeros((batch, num_key_value_heads, capacity, head_dim), dtype=torch.float8_e4m3fn, device=device) for _ in range(2)]
+    return (*codes, *(torch.zeros((batch, num_key_value_heads, capacity), dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths=None):
+    """Writes k and v [B, Hkv, S, D] (bf16 or fp16, through their strides) into the caches in place, quantised: token s < lengths[b]
+    of row b (all without lengths) to position start[b] + s, with scale = max(max |x| / 448, 2^-126) per token and head and
+    code = e4m3(x / scale).  start, lengths int32 [B] on the device, never read by the host.  Positions outside the cache are
+    dropped; the rest of it stays as it is.  Not differentiable."""
+    for name, t in (("k", k), ("v", v)):
+        if t.is_cpu:
+            raise RuntimeError(f"[Error] The input `{name}` of kv_cache_write op is on the device: CPU!")
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise RuntimeError("kv_cache_write is not differentiable: call it under torch.no_grad() or on detached tensors")
+    backend.kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths)
+
+
+def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key_lengths=None, causal=False, scale=None):
+    """`attention` of q [B, Hq, Sq, D] over a quantised cache, read as it is: key_lengths int32 [B] tokens of it are filled; with
+    causal=True the queries are the last Sq of them (generation; without, as in a denoise step, all of them see all).  Inference
+    only."""
+    if q.is_cpu:
+        raise RuntimeError("[Error] The input `q` of cached_attention op is on the device: CPU!")
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError("cached_attention is not differentiable: call it under torch.no_grad() or on detached tensors")
+    return backend.cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges, key_lengths, causal, scale)
 
 
 # ----------------------------------------------------------------------------- index builders

@@ -519,6 +519,219 @@ def qkv_rope_bwd(grad_q, grad_k, grad_v, table: torch.Tensor, B: int, S: int, n_
     return g, bias
 
 
+# ----------------------------------------------------------------------------- norm of q and k with M-RoPE
+def _same_device(*named) -> None:
+    first = named[0][1]
+    for name, t in named:
+        if t is None:
+            continue
+        _need_cuda(name, t)
+        if t.device != first.device:
+            raise RuntimeError("All tensors must be on the same device")
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """`t` [B, H, S, D] as the attention and norm kernels read it through strides: contiguous last dimension, rows on 16
+    bytes; a copy where it is not."""
+    unit = 16 // t.element_size()
+    sb, sh, ss, sd = t.stride()
+    B, H, S, D = t.shape
+    if (sd == 1 or D == 1) and t.data_ptr() % 16 == 0 and (B == 1 or sb % unit == 0) and (H == 1 or sh % unit == 0) and (S == 1 or ss % unit == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _packed16(t: torch.Tensor) -> torch.Tensor:
+    """`t` contiguous and on 16 bytes, a copy where it is not."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _row_strides(t: torch.Tensor):
+    """Batch, head and position strides for the library; a dimension of one has none."""
+    return _lib.i64x3([st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])])
+
+
+def _norm_rope_args(q, k, q_weight, k_weight, source, inv_freq, mrope_section, layout):
+    _same_device(("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("table" if inv_freq is None else "position_ids", source), ("inv_freq", inv_freq))
+    if q.dim() != 4 or k.dim() != 4:
+        raise RuntimeError("q and k must be [B, H, S, D] tensors")
+    B, Hq, S, D = q.shape
+    if (k.size(0), k.size(2), k.size(3)) != (B, S, D):
+        raise RuntimeError("q/k shapes are inconsistent")
+    if not (q.dtype == k.dtype == q_weight.dtype == k_weight.dtype) or q.dtype not in _DTYPES:
+        raise RuntimeError("q, k and the weights must share one dtype (bfloat16, float16 or float32)")
+    if tuple(q_weight.shape) != (D,) or tuple(k_weight.shape) != (D,):
+        raise RuntimeError(f"q_weight and k_weight must be [{D}]")
+    if len(mrope_section) != 3:
+        raise RuntimeError("mrope_section must have 3 entries")
+    section = _lib.i32x3([int(v) for v in mrope_section])
+    if inv_freq is None:
+        width = _table_width(D, section, layout)
+        if q.dtype != torch.bfloat16:
+            raise RuntimeError("All tensors must be BFloat16 with a table; use the position ids")
+        if tuple(source.shape) != (B * S, width) or source.dtype != torch.int32 or not source.is_contiguous():
+            raise RuntimeError(f"table must be a contiguous int32 [{B * S}, {width}] tensor from mrope_table with the same "
+                               f"mrope_section and layout ({layout!r})")
+    else:
+        if tuple(source.shape) != (3, B, S) or source.dtype != torch.int64 or not source.is_contiguous():
+            raise RuntimeError(f"position_ids must be contiguous int64 [3, {B}, {S}]")
+        if tuple(inv_freq.shape) != (D // 2,) or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+            raise RuntimeError(f"inv_freq must be contiguous fp32 [{D // 2}]")
+    return B, Hq, k.size(1), S, D, section
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps: float, layout: str = "hf"):
+    """(q', k') = M-RoPE of the RMS norm per head of q [B, Hq, S, D] and k [B, Hkv, S, D] (any batch / head / position strides),
+    contiguous.  source: mrope_table's table with inv_freq None, or position_ids [3, B, S] int64 with inv_freq [D / 2] fp32."""
+    B, Hq, Hk, S, D, section = _norm_rope_args(q, k, q_weight, k_weight, source, inv_freq, mrope_section, layout)
+    q, k, q_weight, k_weight = _rows16(q), _rows16(k), _packed16(q_weight), _packed16(k_weight)
+    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    with _DeviceGuard(q):
+        _lib.call("wx_qk_norm_rope", _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(source), _ptr(inv_freq), _ptr(q_out),
+                  _ptr(k_out), B, S, Hq, Hk, D, _row_strides(q), _row_strides(k), section, _layout_code(layout), _DTYPES[q.dtype], _stream(q))
+    return q_out, k_out
+
+
+def qk_norm_rope_bwd(grad_q, grad_k, q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps: float, layout: str = "hf",
+                     want=(True, True, True, True)):
+    """The gradients of qk_norm_rope's q, k, q_weight and k_weight (None where not wanted)."""
+    B, Hq, Hk, S, D, section = _norm_rope_args(q, k, q_weight, k_weight, source, inv_freq, mrope_section, layout)
+    _same_device(("q", q), ("gradient", grad_q), ("gradient", grad_k))
+    if grad_q.shape != q.shape or grad_k.shape != k.shape or grad_q.dtype != q.dtype or grad_k.dtype != k.dtype:
+        raise RuntimeError("the gradients must have the shapes and the dtype of q and k")
+    q, k, grad_q, grad_k, q_weight, k_weight = _rows16(q), _rows16(k), _rows16(grad_q), _rows16(grad_k), _packed16(q_weight), _packed16(k_weight)
+    outs = [torch.empty(t.shape, dtype=q.dtype, device=q.device) if w else None for t, w in zip((q, k, q_weight, k_weight), want)]
+    n_work = _lib.load().wx_qk_norm_rope_bwd_workspace_bytes(D) if want[2] or want[3] else 0
+    work = torch.empty(n_work, dtype=torch.uint8, device=q.device)
+    with _DeviceGuard(q):
+        _lib.call("wx_qk_norm_rope_bwd", _ptr(grad_q), _ptr(grad_k), _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(source),
+                  _ptr(inv_freq), _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]), _ptr(outs[3]), B, S, Hq, Hk, D, _row_strides(grad_q),
+                  _row_strides(grad_k), _row_strides(q), _row_strides(k), section, _layout_code(layout), _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
+    return outs
+
+
+# ----------------------------------------------------------------------------- attention
+_ATTENTION_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def _attention_args(q, n_keys, n_kv, key_ranges, key_lengths, scale):
+    B, Hq, Sq, D = q.shape
+    if q.dtype not in _ATTENTION_DTYPES:
+        raise RuntimeError("q must be BFloat16 or Half")
+    if n_kv == 0 or Hq % n_kv:
+        raise RuntimeError(f"{Hq} query heads are no multiple of {n_kv} key / value heads")
+    if key_ranges is not None and (tuple(key_ranges.shape) != (B, Sq, 2) or key_ranges.dtype != torch.int32):
+        raise RuntimeError(f"key_ranges must be int32 [{B}, {Sq}, 2]")
+    if key_lengths is not None and (tuple(key_lengths.shape) != (B,) or key_lengths.dtype != torch.int32):
+        raise RuntimeError(f"key_lengths must be int32 [{B}]")
+    return (None if key_ranges is None else _packed16(key_ranges), None if key_lengths is None else key_lengths.contiguous(),
+            D ** -0.5 if scale is None else float(scale))
+
+
+def _attention_shapes(q, k, v):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise RuntimeError(f"{name} must be a [B, H, S, D] tensor")
+    if k.shape != v.shape or (k.size(0), k.size(3)) != (q.size(0), q.size(3)):
+        raise RuntimeError("q/k/v shapes are inconsistent")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise RuntimeError("q, k and v must share one dtype")
+
+
+def attention_fwd(q, k, v, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None, want_lse: bool = False):
+    """(out [B, Hq, Sq, D] over token-major memory, lse or None): softmax(scale q k^T) v of q [B, Hq, Sq, D] over k and v
+    [B, Hkv, Sk, D] (any strides), query i of row b seeing the keys [lo, hi) of key_ranges int32 [B, Sq, 2], below key_lengths
+    int32 [B] and, with causal, up to its own position when the queries are the last of the keys."""
+    _same_device(("q", q), ("k", k), ("v", v), ("key_ranges", key_ranges), ("key_lengths", key_lengths))
+    _attention_shapes(q, k, v)
+    key_ranges, key_lengths, scale = _attention_args(q, k.size(2), k.size(1), key_ranges, key_lengths, scale)
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    B, Hq, Sq, D = q.shape
+    Hk, Sk = k.size(1), k.size(2)
+    out = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hk, Sq * (Hq // Hk)), dtype=torch.float32, device=q.device) if want_lse else None
+    with _DeviceGuard(q):
+        n_work = _lib.load().wx_attention_workspace_bytes(B, Hq, Hk, Sq, Sk, D)
+        work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
+        _lib.call("wx_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(key_ranges), _ptr(key_lengths), int(bool(causal)), B, Hq, Hk,
+                  Sq, Sk, D, _row_strides(q), _row_strides(k), _row_strides(v), scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
+    return out.transpose(1, 2), lse
+
+
+def attention_bwd(grad_out, q, k, v, out, lse, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None):
+    """(grad_q, grad_k, grad_v) over token-major memory, from what attention_fwd took and returned."""
+    _same_device(("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse), ("gradient", grad_out), ("key_ranges", key_ranges), ("key_lengths", key_lengths))
+    _attention_shapes(q, k, v)
+    key_ranges, key_lengths, scale = _attention_args(q, k.size(2), k.size(1), key_ranges, key_lengths, scale)
+    if grad_out.shape != q.shape or grad_out.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
+        raise RuntimeError("the gradient and the output must have q's shape and dtype")
+    q, k, v, grad_out = _rows16(q), _rows16(k), _rows16(v), _rows16(grad_out)
+    B, Hq, Sq, D = q.shape
+    Hk, Sk = k.size(1), k.size(2)
+    tokens = out.transpose(1, 2)
+    tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hk, Sq * (Hq // Hk)) or not lse.is_contiguous():
+        raise RuntimeError("lse must be what attention_fwd returned")
+    dq = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+    with _DeviceGuard(q):
+        n_work = _lib.load().wx_attention_bwd_workspace_bytes(B, Hq, Hk, Sq, Sk, D)
+        work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
+        _lib.call("wx_attention_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(tokens), _ptr(lse), _ptr(grad_out), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(key_ranges),
+                  _ptr(key_lengths), int(bool(causal)), B, Hq, Hk, Sq, Sk, D, _row_strides(q), _row_strides(k), _row_strides(v), _row_strides(grad_out),
+                  scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
+    return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2)
+
+
+# ----------------------------------------------------------------------------- quantised key / value cache
+def _cache_args(k_cache, v_cache, k_scale, v_scale):
+    if k_cache.dim() != 4:
+        raise RuntimeError("the caches must be [B, Hkv, capacity, D] tensors")
+    for name, t, like, dtype in (("k_cache", k_cache, k_cache.shape, torch.float8_e4m3fn), ("v_cache", v_cache, k_cache.shape, torch.float8_e4m3fn),
+                                 ("k_scale", k_scale, k_cache.shape[:3], torch.float32), ("v_scale", v_scale, k_cache.shape[:3], torch.float32)):
+        if t.dtype != dtype or tuple(t.shape) != tuple(like) or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous {str(dtype).replace('torch.', '')} {list(like)} tensor")
+
+
+def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths=None) -> None:
+    """Quantises token s < lengths[b] (int32 [B]; None: all) of k and v [B, Hkv, S, D] (any strides) into position start[b] + s
+    (int32 [B]) of the caches, e4m3 [B, Hkv, capacity, D] with scales fp32 [B, Hkv, capacity]; positions outside are dropped."""
+    _same_device(("k", k), ("v", v), ("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale), ("start", start), ("lengths", lengths))
+    _cache_args(k_cache, v_cache, k_scale, v_scale)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _ATTENTION_DTYPES:
+        raise RuntimeError("k and v must be BFloat16 or Half [B, Hkv, S, D] tensors of one shape and dtype")
+    B, Hk, S, D = k.shape
+    if (k_cache.size(0), k_cache.size(1), k_cache.size(3)) != (B, Hk, D):
+        raise RuntimeError("k and the caches differ in batch, heads or head size")
+    for name, t in (("start", start), ("lengths", lengths)):
+        if t is not None and (tuple(t.shape) != (B,) or t.dtype != torch.int32):
+            raise RuntimeError(f"{name} must be int32 [{B}]")
+    k, v, start = _rows16(k), _rows16(v), start.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    with _DeviceGuard(k):
+        _lib.call("wx_kv_cache_write", _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(start), _ptr(lengths), B, Hk, S,
+                  k_cache.size(2), D, _row_strides(k), _row_strides(v), _DTYPES[k.dtype], _stream(k))
+
+
+def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None):
+    """attention_fwd's result over a quantised cache (kv_cache_write)."""
+    _same_device(("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale), ("key_ranges", key_ranges), ("key_lengths", key_lengths))
+    _cache_args(k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 4 or (k_cache.size(0), k_cache.size(3)) != (q.size(0), q.size(3)):
+        raise RuntimeError("q must be a [B, H, S, D] tensor of the cache's batch and head size")
+    B, Hk, C, D = k_cache.shape
+    key_ranges, key_lengths, scale = _attention_args(q, C, Hk, key_ranges, key_lengths, scale)
+    q = _rows16(q)
+    Hq, Sq = q.size(1), q.size(2)
+    out = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device=q.device)
+    with _DeviceGuard(q):
+        n_work = _lib.load().wx_attention_workspace_bytes(B, Hq, Hk, Sq, C, D)
+        work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
+        _lib.call("wx_cached_attention", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(out), _ptr(key_ranges), _ptr(key_lengths),
+                  int(bool(causal)), B, Hq, Hk, Sq, C, D, _row_strides(q), scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
+    return out.transpose(1, 2)
+
+
 # ----------------------------------------------------------------------------- index builders
 def rope_index(input_ids, image_grid_thw, video_grid_thw, second_per_grid_ts, attention_mask,
                spatial_merge_size: int, image_token_id: int, video_token_id: int, vision_start_token_id: int,
