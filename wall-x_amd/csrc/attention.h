@@ -137,42 +137,61 @@ __device__ __forceinline__ int wave_max_i(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
-// A operand, contraction over the head: row (lane & 31) of 32 rows from `row0`, channels 16 t + 8 h .. + 7.
+// Byte offsets, in a tile, of what a lane reads of its first block: the other blocks lie at constant distances and exclusive-ors.
+//   rows  A operand, contraction over the head: row lane & 31 of 32 rows, channels 16 t + 8 h .. + 7 of step t
+//   cols  A operand, contraction over the tile's rows: channel 32 o + (lane & 31), rows 16 t + 8 (j / 4) + 4 h + j % 4
 template <int D>
-__device__ __forceinline__ u32x4 read_rows(const unsigned char* tile, int row0, int t, int lane) {
-  using T = AttnTile<D>;
-  const int r = lane & 31;  // (row0 is a multiple of 32: the swizzle does not see it)
-  return *reinterpret_cast<const u32x4*>(tile + row0 * T::kPitch + T::at(r, 2 * t + (lane >> 5)));
+__device__ __forceinline__ int rows_base(int lane) {
+  return AttnTile<D>::at(lane & 31, lane >> 5);
 }
-
-// A operand, contraction over the tile's rows: channel 32 o + (lane & 31), rows 16 t + 8 (j / 4) + 4 h + j % 4 from `row0`.
-// ds_read_b64_tr_b16: lane j of 16 gives the address of 4 consecutive channels of row j >> 2 and receives channel j of the 4 rows.
+// (ds_read_b64_tr_b16: lane j of 16 gives the address of 4 consecutive channels of row j >> 2 and receives channel j of the 4 rows)
 template <int D>
-__device__ __forceinline__ u32x4 read_cols(const unsigned char* tile, int row0, int t, int o, int lane) {
+__device__ __forceinline__ int cols_base(int lane) {
+  return AttnTile<D>::at(4 * (lane >> 5) + ((lane >> 2) & 3), 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
+}
+template <int D>
+__device__ __forceinline__ u32x4 read_rows(const unsigned char* tile, int row0, int t, int base) {
   using T = AttnTile<D>;
-  const int h = lane >> 5, q = (lane >> 2) & 3, row = 4 * h + q;
-  const int chunk = 4 * o + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-  const unsigned char* base = tile + (row0 + 16 * t) * T::kPitch + 8 * (lane & 1);
+  // chunk 2 t + h of a swizzled row: 2 t is an exclusive-or of the bits that the swizzle reaches and a sum above them
+  constexpr int kXor = T::kPitch == 256 ? 255 : (T::kPitch == 128 ? 127 : 63);
+  const int c = 32 * t;
+  return *reinterpret_cast<const u32x4*>(tile + (base ^ (c & kXor)) + (c & ~kXor) + row0 * T::kPitch);  // (row0: a multiple of 16)
+}
+template <int D>
+__device__ __forceinline__ u32x4 read_cols(const unsigned char* tile, int row0, int t, int o, int base) {
+  using T = AttnTile<D>;
+  constexpr int kXor = T::kPitch == 256 ? 255 : (T::kPitch == 128 ? 127 : 63);
+  const int c = 64 * o;
   typedef __attribute__((address_space(3))) att_bf16x4* P;
-  const att_bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((P)(base + T::at(row, chunk)));
-  const att_bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((P)(base + T::at(row + 8, chunk)));
+  const unsigned char* at = tile + (row0 + 16 * t) * T::kPitch + (c & ~kXor);
+  const att_bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((P)(at + (base ^ (c & kXor))));
+  const att_bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((P)(at + 8 * T::kPitch + (base ^ (c & kXor) ^ 32)));  // 8 rows on: swizzle ^ 2
   const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
   return u32x4{x[0], x[1], y[0], y[1]};
 }
 
-// 16 consecutive rows of a tile, straight from global memory to LDS, by one wavefront.  `offset(row)` is the byte offset of
-// tile row `row` (0..15 from the wavefront's first) from the descriptor's base, or kOutside: such rows become zeros.
+// 16 consecutive rows of a tile, straight from global memory to LDS, by one wavefront: instruction i fills 1 KiB.  `offset(row)` is
+// the byte offset of tile row `row` (0..15 from the wavefront's first) from the descriptor's base, or kOutside: such rows become zeros.
+template <int D, class Offset>
+__device__ __forceinline__ uint32_t stage_offset(int i, int lane, Offset offset) {
+  using T = AttnTile<D>;
+  const int n = i * 64 + lane, row = n / T::kChunks, chunk = (n % T::kChunks) ^ T::swizzle(row);
+  const uint32_t off = offset(row);
+  if (off == kOutside || (T::kChunks * 8 > D && chunk >= D / 8)) return kOutside;
+  return off + static_cast<uint32_t>(chunk) * 16u;
+}
 template <int D, class Offset>
 __device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, int lane, Offset offset) {
-  using T = AttnTile<D>;
 #pragma unroll
-  for (int i = 0; i < T::kChunks / 4; ++i) {
-    const int n = i * 64 + lane, row = n / T::kChunks, chunk = (n % T::kChunks) ^ T::swizzle(row);
-    uint32_t off = offset(row);
-    off += off == kOutside ? 0u : static_cast<uint32_t>(chunk) * 16u;
-    if (T::kChunks * 8 > D && chunk >= D / 8) off = kOutside;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(off), 0, 0, 0);
-  }
+  for (int i = 0; i < AttnTile<D>::kChunks / 4; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(stage_offset<D>(i, lane, offset)), 0, 0, 0);
+}
+// The same from offsets that were made before (all rows inside).
+template <int D>
+__device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, const uint32_t* offsets) {
+#pragma unroll
+  for (int i = 0; i < AttnTile<D>::kChunks / 4; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(offsets[i]), 0, 0, 0);
 }
 
 __device__ __forceinline__ void attn_barrier() {  // (no fences: they would drain the loads in flight)

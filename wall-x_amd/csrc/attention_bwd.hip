@@ -83,15 +83,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   const char* kp = reinterpret_cast<const char*>(a.k + b * a.ks[0] + hk * a.ks[1]);
   const char* vp = reinterpret_cast<const char*>(a.v + b * a.vs[0] + hk * a.vs[1]);
   const int64_t k_step = a.ks[2] * 2, v_step = a.vs[2] * 2;
-  auto fetch = [&](int it) {
-    unsigned char* slot = lds + (it & 1) * 2 * kTileBytes;
+  uint32_t k_off[T::kChunks / 4], v_off[T::kChunks / 4];
+#pragma unroll
+  for (int i = 0; i < T::kChunks / 4; ++i) {
+    k_off[i] = stage_offset<D>(i, lane, [&](int r) { return static_cast<uint32_t>((wave * 16 + r) * static_cast<int>(k_step)); });
+    v_off[i] = stage_offset<D>(i, lane, [&](int r) { return static_cast<uint32_t>((wave * 16 + r) * static_cast<int>(v_step)); });
+  }
+  auto fetch = [&](int it, unsigned char* slot) {
     const int k0 = g_lo + it * KB, left = g_hi - k0, r0 = wave * 16;
-    stage16<D>(attn_rsrc(kp + k0 * k_step, kRsrcBytes), slot + r0 * T::kPitch, lane,
-               [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(k_step)) : kOutside; });
-    stage16<D>(attn_rsrc(vp + k0 * v_step, kRsrcBytes), slot + kTileBytes + r0 * T::kPitch, lane,
-               [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(v_step)) : kOutside; });
+    const auto rk = attn_rsrc(kp + k0 * k_step, kRsrcBytes), rv = attn_rsrc(vp + k0 * v_step, kRsrcBytes);
+    if (left >= KB) {
+      stage16<D>(rk, slot + r0 * T::kPitch, k_off);
+      stage16<D>(rv, slot + kTileBytes + r0 * T::kPitch, v_off);
+    } else {
+      stage16<D>(rk, slot + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(k_step)) : kOutside; });
+      stage16<D>(rv, slot + kTileBytes + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(v_step)) : kOutside; });
+    }
   };
-  if (iters > 0) fetch(0);
+  if (iters > 0) fetch(0, lds);
 
   u32x4 qf[T::kSteps], gf[T::kSteps];
   float delta = 0.f;
@@ -131,11 +140,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
-  for (int it = 0; it < iters; ++it) {
+  const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
+  auto turn = [&](int it, unsigned char* tk, unsigned char* other) {
     wait_loads();
     attn_barrier();
-    if (it + 1 < iters) fetch(it + 1);
-    const unsigned char *tk = lds + (it & 1) * 2 * kTileBytes, *tv = tk + kTileBytes;
+    if (it + 1 < iters) fetch(it + 1, other);
+    const unsigned char* tv = tk + kTileBytes;
 #pragma unroll
     for (int n = 0; n < KB / 32; ++n) {
       const int k0 = g_lo + it * KB + 32 * n;
@@ -145,8 +155,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
       for (int t = 0; t < T::kSteps; ++t) {
-        s = mfma<DT>(read_rows<D>(tk, 32 * n, t, lane), qf[t], s);
-        dp = mfma<DT>(read_rows<D>(tv, 32 * n, t, lane), gf[t], dp);
+        s = mfma<DT>(read_rows<D>(tk, 32 * n, t, rows_at), qf[t], s);
+        dp = mfma<DT>(read_rows<D>(tv, 32 * n, t, rows_at), gf[t], dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
@@ -159,9 +169,13 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       for (int t = 0; t < 2; ++t) {
         const u32x4 ds = pack_step<DT>(s, t);
 #pragma unroll
-        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tk, 32 * n, t, o, lane), ds, acc[o]);
+        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tk, 32 * n, t, o, cols_at), ds, acc[o]);
       }
     }
+  };
+  for (int it = 0; it < iters; it += 2) {  // (the two slots' addresses are constants)
+    turn(it, lds, lds + 2 * kTileBytes);
+    if (it + 1 < iters) turn(it + 1, lds + 2 * kTileBytes, lds);
   }
 
   bool bad = false;
@@ -225,6 +239,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   constexpr int kTileBytes = 32 * T::kPitch, kInfoBytes = 1024, kSlot = 2 * kTileBytes + kInfoBytes;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kSlot];
   __shared__ int s_first[4], s_last[4];
+  __shared__ u32x4 s_offsets[256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int pairs = a.batch * a.n_kv;
   int pair, tile, split;
@@ -280,12 +295,36 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   const int64_t pos_step = (wave < 2 ? a.qs[2] : a.gs[2]) * 2;
   const int head_step = static_cast<int>((wave < 2 ? a.qs[1] : a.gs[1]) * 2), pos_step32 = static_cast<int>(pos_step);
   const uint32_t* info_base = a.info + static_cast<int64_t>(pair) * a.row_blocks * kInfoWords;
+  // Offsets of a block's rows from its first: the same for every block where the group divides 32 or 32 the group.  They are kept in
+  // LDS, for want of registers.
+  const bool regular = 32 % a.group == 0 || a.group % 32 == 0;
+  {
+    const int in_group = a.group < 32 ? a.group : 32, r0 = (wave & 1) * 16;
+    uint32_t off[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < T::kChunks / 4; ++i)
+      off[i] = stage_offset<D>(i, lane, [&](int r) {
+        const int di = (r0 + r) / in_group, hd = (r0 + r) - di * in_group;
+        return static_cast<uint32_t>(di * pos_step32 + hd * head_step);
+      });
+    s_offsets[tid] = u32x4{off[0], off[1], off[2], off[3]};
+  }
   auto fetch = [&](int t, unsigned char* slot) {
     const int row0 = t * 32, i0 = row0 / a.group, rem = row0 - i0 * a.group, r0 = (wave & 1) * 16;
-    stage16<D>(attn_rsrc(src + __builtin_amdgcn_readfirstlane(i0) * pos_step, kRsrcBytes), slot + (wave >> 1) * kTileBytes + r0 * T::kPitch, lane, [&](int r) {
-      const uint32_t x = static_cast<uint32_t>(rem + r0 + r), di = magic ? __umulhi(x, magic) : x, hd = x - di * a.group;
-      return row0 + r0 + r < a.rows ? di * static_cast<uint32_t>(pos_step32) + hd * static_cast<uint32_t>(head_step) : kOutside;
-    });
+    const char* base = src + __builtin_amdgcn_readfirstlane(i0) * pos_step;
+    unsigned char* to = slot + (wave >> 1) * kTileBytes + r0 * T::kPitch;
+    if (regular && row0 + 32 <= a.rows) {
+      const u32x4 o = s_offsets[tid];
+      const uint32_t off[4] = {o[0], o[1], o[2], o[3]};
+      stage16<D>(attn_rsrc(base + __builtin_amdgcn_readfirstlane(rem) * static_cast<int64_t>(head_step), kRsrcBytes), to, off);
+    } else {
+      int here = lane;
+      asm volatile("" : "+v"(here));  // (what this path needs is made here, not kept over the loop)
+      stage16<D>(attn_rsrc(base, kRsrcBytes), to, here, [&](int r) {
+        const uint32_t x = static_cast<uint32_t>(rem + r0 + r), di = magic ? __umulhi(x, magic) : x, hd = x - di * a.group;
+        return row0 + r0 + r < a.rows ? di * static_cast<uint32_t>(pos_step32) + hd * static_cast<uint32_t>(head_step) : kOutside;
+      });
+    }
     if (wave == 0)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(attn_rsrc(info_base + static_cast<int64_t>(t) * kInfoWords, kInfoWords * 4), WX_LDS(slot + 2 * kTileBytes), 16,
                                                lane * 16, 0, 0, 0);
@@ -308,6 +347,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[o][r] = dv[o][r] = 0.f;
 
+  const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
   for (int t = first; t < last; ++t) {
     wait_loads();
     attn_barrier();
@@ -316,13 +356,16 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     const float* info = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
     const int2 full = *reinterpret_cast<const int2*>(info + 128);
     const int f_lo = __builtin_amdgcn_readfirstlane(full.x), f_hi = __builtin_amdgcn_readfirstlane(full.y);
+    // (an exclusive-or per read in place of an address register for each: the accumulators leave none)
+    int rows_at = rows_first, cols_at = cols_first;
+    asm volatile("" : "+v"(rows_at), "+v"(cols_at));
     f32x16 s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
     for (int u = 0; u < T::kSteps; ++u) {
-      s = mfma<DT>(read_rows<D>(tq, 0, u, lane), kf[u], s);
-      dp = mfma<DT>(read_rows<D>(tg, 0, u, lane), vf[u], dp);
+      s = mfma<DT>(read_rows<D>(tq, 0, u, rows_at), kf[u], s);
+      dp = mfma<DT>(read_rows<D>(tg, 0, u, rows_at), vf[u], dp);
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -342,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool see = key >= l4[i] && key < h4[i];
+          const bool see = (key >= l4[i]) & (key < h4[i]);
           s[4 * g + i] = see ? s[4 * g + i] : 0.f;
           dp[4 * g + i] = see ? dp[4 * g + i] : 0.f;
         }
@@ -353,8 +396,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
       const u32x4 p = pack_step<DT>(s, u), ds = pack_step<DT>(dp, u);
 #pragma unroll
       for (int o = 0; o < T::kOut; ++o) {
-        dv[o] = mfma<DT>(read_cols<D>(tg, 0, u, o, lane), p, dv[o]);
-        dk[o] = mfma<DT>(read_cols<D>(tq, 0, u, o, lane), ds, dk[o]);
+        dv[o] = mfma<DT>(read_cols<D>(tg, 0, u, o, cols_at), p, dv[o]);
+        dk[o] = mfma<DT>(read_cols<D>(tq, 0, u, o, cols_at), ds, dk[o]);
       }
     }
   }

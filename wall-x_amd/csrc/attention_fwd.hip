@@ -172,6 +172,15 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   const int gt = rw * 64 + lane;
   u32x4 pk[kDirect ? 1 : kPieces], pv[kDirect ? 1 : kPieces];
   float pks = 0.f, pvs = 0.f;
+  uint32_t k_off[kDirect ? T::kChunks / 4 : 1], v_off[kDirect ? T::kChunks / 4 : 1];
+  if constexpr (kDirect) {
+#pragma unroll
+    for (int i = 0; i < T::kChunks / 4; ++i) {
+      k_off[i] = stage_offset<D>(i, lane, [&](int r) { return static_cast<uint32_t>((rw * 16 + r) * static_cast<int>(k_step)); });
+      v_off[i] = stage_offset<D>(i, lane, [&](int r) { return static_cast<uint32_t>((rw * 16 + r) * static_cast<int>(v_step)); });
+    }
+  }
+  const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
   auto key0 = [&](int it) { return g_lo + (it * KW + kw) * KB; };
   auto fetch = [&](int it, unsigned char* slot) {  // a tile on its way: to LDS, or into registers
     const int k0 = key0(it), left = g_hi - k0;  // (may be <= 0: zeros)
@@ -179,9 +188,12 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
     const int64_t at = left > 0 ? k0 : 0;
     const auto rk = attn_rsrc(kp + at * k_step, kRsrcBytes), rv = attn_rsrc(vp + at * v_step, kRsrcBytes);
     if constexpr (kDirect) {
-#pragma unroll
-      for (int u = 0; u < KB / 16 / RW; ++u) {
-        const int r0 = (rw + u * RW) * 16;
+      static_assert(KB == 16 * RW, "a wavefront loads 16 rows");
+      const int r0 = rw * 16;
+      if (left >= KB) {  // all rows are there: the offsets stay the same from tile to tile
+        stage16<D>(rk, slot + r0 * T::kPitch, k_off);
+        stage16<D>(rv, slot + kTileBytes + r0 * T::kPitch, v_off);
+      } else {
         stage16<D>(rk, slot + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(k_step)) : kOutside; });
         stage16<D>(rv, slot + kTileBytes + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(v_step)) : kOutside; });
       }
@@ -243,7 +255,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
 #pragma unroll
-      for (int t = 0; t < T::kSteps; ++t) s[n] = mfma<DT>(read_rows<D>(tk, 32 * n, t, lane), qf[t], s[n]);
+      for (int t = 0; t < T::kSteps; ++t) s[n] = mfma<DT>(read_rows<D>(tk, 32 * n, t, rows_at), qf[t], s[n]);
     }
     if constexpr (F8) {
 #pragma unroll
@@ -307,26 +319,33 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
       for (int t = 0; t < 2; ++t) {
         const u32x4 p = pack_step<DT>(s[n], t);
 #pragma unroll
-        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tv, 32 * n, t, o, lane), p, acc[o]);
+        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tv, 32 * n, t, o, cols_at), p, acc[o]);
       }
   };
 
   unsigned char* mine = lds + kw * kBufs * kSlot;
   if (iters > 0) fetch(0, mine);
-  for (int it = 0; it < iters; ++it) {
+  auto turn = [&](int it, unsigned char* slot, unsigned char* other) {
     const int k0 = key0(it);
-    unsigned char* slot = mine + (kBufs == 2 ? (it & 1) * kSlot : 0);
     if constexpr (kDirect) {
       wait_loads();
       attn_barrier();
-      if (it + 1 < iters) fetch(it + 1, mine + ((it + 1) & 1) * kSlot);
+      if (it + 1 < iters) fetch(it + 1, other);
     } else {
       if (RW > 1 || k0 < g_hi) put(slot);
-      if (it + 1 < iters) fetch(it + 1, slot);
+      if (it + 1 < iters) fetch(it + 1, other);
       wait_lds();
       if constexpr (RW > 1) attn_barrier();
     }
     if (k0 < w_hi && k0 + KB > w_lo && k0 < g_hi) step(slot, k0);
+  };
+  if constexpr (kBufs == 1) {
+    for (int it = 0; it < iters; ++it) turn(it, mine, mine);
+  } else {
+    for (int it = 0; it < iters; it += 2) {  // (the two slots' addresses are constants)
+      turn(it, mine, mine + kSlot);
+      if (it + 1 < iters) turn(it + 1, mine + kSlot, mine);
+    }
   }
   l = both_sum(l);
 
@@ -445,43 +464,59 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   }
 }
 
-// Joins the splits of a row: a wavefront per row, lane l channels l and l + 64.
+constexpr int kMaxSplits = 256;
+
+// Joins the splits of a row: a workgroup per row, every wavefront a quarter of the splits, lane l channels l and l + 64.
+// (A wavefront per row took 24 us for 128 rows of 32 splits: one dependent load after the other.)
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (at >= static_cast<int64_t>(a.batch) * a.n_kv * a.rows) return;
+  __shared__ float s_top[4], s_sum[4], s_weight[kMaxSplits], s_out[4][128];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t at = blockIdx.x;
   const int pair = static_cast<int>(at / a.rows), row = static_cast<int>(at - static_cast<int64_t>(pair) * a.rows);
   const float2* stats = part_stats(a, D) + static_cast<int64_t>(pair) * a.splits * a.rows + row;
   const float* part = a.part + (static_cast<int64_t>(pair) * a.splits * a.rows + row) * D;
-  float top = -kInf;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, stats[static_cast<int64_t>(s) * a.rows].x);
-  top = wave_max(top);
-  float l = 0.f, o[2] = {0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 st = stats[static_cast<int64_t>(s) * a.rows];
-    const float f = st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c);
-    l += st.y * f;
+  const float2 st = tid < a.splits ? stats[static_cast<int64_t>(tid) * a.rows] : float2{-kInf, 0.f};
+  const float wave_top = wave_max(st.x);
+  if (lane == 0) s_top[wave] = wave_top;
+  __syncthreads();
+  const float top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  // (a split that the row sees nothing of has no part, whatever stands in its place)
+  const float f = st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c);
+  s_weight[tid] = f;
+  const float wave_l = wave_sum(st.y * f);
+  if (lane == 0) s_sum[wave] = wave_l;
+  __syncthreads();
+  const float l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  float o[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int s = wave; s < a.splits; s += 4) {
+    const float w = s_weight[s];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < D && st.x != -kInf) o[u] += part[static_cast<int64_t>(s) * a.rows * D + lane + 64 * u] * f;
+      if (lane + 64 * u < D) {
+        const float x = part[static_cast<int64_t>(s) * a.rows * D + lane + 64 * u];
+        o[u] += w == 0.f ? 0.f : x * w;
+      }
   }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) s_out[wave][lane + 64 * u] = o[u];
+  __syncthreads();
   const int b = pair / a.n_kv, hk = pair % a.n_kv;
   const int i = row / a.group, hq = hk * a.group + row % a.group;
   int lo, hi;
   key_range(a.mask, b, i, a.n_queries, a.n_keys, lo, hi);
-  uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D;
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(hi > lo ? o[u] / l : 0.f));
-  if (a.lse != nullptr && lane == 0) a.lse[at] = hi > lo ? __builtin_fmaf(top, a.c, __builtin_amdgcn_logf(l)) : kInf;
+  if (tid < D) {
+    const float sum = (s_out[0][tid] + s_out[1][tid]) + (s_out[2][tid] + s_out[3][tid]);
+    a.out[((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D + tid] = static_cast<uint16_t>(Elem<DT>::store(hi > lo ? sum / l : 0.f));
+  }
+  if (a.lse != nullptr && tid == 0) a.lse[at] = hi > lo ? __builtin_fmaf(top, a.c, __builtin_amdgcn_logf(l)) : kInf;
 }
 
 // How a call is spread over the chip: wavefronts of the workgroup that take rows (4, 2 or 1), and splits of the keys.
 struct FwdPlan {
   int row_waves, splits;
 };
-constexpr int kMaxSplits = 256;
 FwdPlan plan(int64_t pairs, int64_t rows, int64_t keys) {
   const int cus = device_cu_count();
   FwdPlan p{4, 1};
@@ -513,7 +548,8 @@ int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
   if (a.splits > 1) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.n_kv * a.rows;
-    hipLaunchKernelGGL((attn_join_kernel<DT, D>), dim3(static_cast<unsigned>((rows + 3) / 4)), block, 0, s, a);
+    if (rows > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
+    hipLaunchKernelGGL((attn_join_kernel<DT, D>), dim3(static_cast<unsigned>(rows)), block, 0, s, a);
     return check_launch("attn_join_kernel");
   }
   return WX_OK;
