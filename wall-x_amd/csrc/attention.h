@@ -126,16 +126,38 @@ __device__ __forceinline__ float wave_max(float x) {
   for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
   return x;
 }
-__device__ __forceinline__ int wave_min_i(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x = min(x, __shfl_xor(x, d));
-  return __builtin_amdgcn_readfirstlane(x);
+// Smallest / largest of the 32 values that a wavefront's halves both hold, the same in all lanes: rotations inside each row of 16
+// lanes, then the first lanes of two rows.
+template <bool MAX>
+__device__ __forceinline__ int wave_extreme(int x) {
+#define WX_STEP(N)                                                           \
+  {                                                                          \
+    const int y = __builtin_amdgcn_update_dpp(x, x, 0x120 + N, 0xF, 0xF, false); \
+    x = MAX ? max(x, y) : min(x, y);                                         \
+  }
+  WX_STEP(8)
+  WX_STEP(4)
+  WX_STEP(2)
+  WX_STEP(1)
+#undef WX_STEP
+  const int a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+  return MAX ? max(a, b) : min(a, b);
 }
-__device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d));
-  return __builtin_amdgcn_readfirstlane(x);
-}
+
+// n / d for n < 2^31 by a multiplication: the host makes the factor (a division by a number from memory is some 20 instructions,
+// and a workgroup's coordinates take half a dozen).
+struct Divider {
+  uint32_t d, factor, shift;
+  Divider() = default;
+  explicit Divider(uint32_t by) : d(by) {
+    shift = 0;
+    while ((1ull << shift) < by) ++shift;
+    factor = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), factor) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
 
 // Byte offsets, in a tile, of what a lane reads of its first block: the other blocks lie at constant distances and exclusive-ors.
 //   rows  A operand, contraction over the head: row lane & 31 of 32 rows, channels 16 t + 8 h .. + 7 of step t
@@ -192,6 +214,12 @@ __device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned ch
 #pragma unroll
   for (int i = 0; i < AttnTile<D>::kChunks / 4; ++i)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(offsets[i]), 0, 0, 0);
+}
+
+// Two wavefronts share a SIMD.  Left alike they fall into step, both in the matrix products and then both in the softmax; with the
+// one in the odd slot (hardware register HW_ID, bits 3:0) ahead at every issue, one computes while the other multiplies.
+__device__ __forceinline__ void stagger_waves() {
+  if (__builtin_amdgcn_s_getreg((3 << 11) | 4) & 1) __builtin_amdgcn_s_setprio(1);
 }
 
 __device__ __forceinline__ void attn_barrier() {  // (no fences: they would drain the loads in flight)

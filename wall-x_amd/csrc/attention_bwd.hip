@@ -25,6 +25,7 @@ struct BwdArgs {
   uint32_t* info;                 // [pair, row_block] blocks of kInfoWords
   int2* bounds;                   // [pair, row_block] the keys that any row of the block sees
   int key_tiles, splits;
+  Divider by_splits, by_pairs, by_kv, by_group, by_in_group;  // by_pairs: of an XCD where they are dealt to XCDs, else all
   float* part;                    // splits > 1: [pair, split, n_keys, 2, D]
 };
 
@@ -47,26 +48,38 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   {
     const int id = blockIdx.x;
     if (pairs % 8 == 0) {
-      const int per = pairs / 8, x = id % 8, j = id / 8;
-      pair = x + 8 * (j % per);
-      tile = row_tiles - 1 - j / per;
+      const int j = id >> 3, t = a.by_pairs.div(j);
+      pair = (id & 7) + 8 * (j - t * (pairs >> 3));
+      tile = row_tiles - 1 - t;
     } else {
-      pair = id % pairs;
-      tile = row_tiles - 1 - id / pairs;
+      const int t = a.by_pairs.div(id);
+      pair = id - t * pairs;
+      tile = row_tiles - 1 - t;
     }
-    pair = __builtin_amdgcn_readfirstlane(pair);
-    tile = __builtin_amdgcn_readfirstlane(tile);
   }
-  const int b = pair / a.n_kv, hk = pair - b * a.n_kv;
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
   const int row = tile * 128 + wave * 32 + (lane & 31);
   const bool live = row < a.rows;
-  const int qi = (live ? row : 0) / a.group, hq = hk * a.group + (live ? row : 0) % a.group;
+  const int in_row = live ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
+  u32x4 qf[T::kSteps], gf[T::kSteps], of[T::kSteps];  // (asked for before anything that depends on memory; a row past the last reads the first)
+  {
+    const uint16_t* q = row_of(a.q, a.qs, b, hq, qi);
+    const uint16_t* g = row_of(a.g, a.gs, b, hq, qi);
+    const uint16_t* o = a.out + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      qf[t] = *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h);
+      gf[t] = *reinterpret_cast<const u32x4*>(g + 16 * t + 8 * h);
+      of[t] = *reinterpret_cast<const u32x4*>(o + 16 * t + 8 * h);
+    }
+  }
+  float lse = a.lse[static_cast<int64_t>(pair) * a.rows + in_row];
   int lo = 0, hi = 0;
   if (live) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
   const bool some = hi > lo;
-  int w_lo = wave_min_i(some ? lo : 0x7fffffff);
-  const int w_hi = wave_max_i(hi);
-  const int f_lo = wave_max_i(some ? lo : 0), f_hi = wave_min_i(some ? hi : 0x7fffffff);
+  int w_lo = wave_extreme<false>(some ? lo : 0x7fffffff);
+  const int w_hi = wave_extreme<true>(hi);
+  const int f_lo = wave_extreme<true>(some ? lo : 0), f_hi = wave_extreme<false>(some ? hi : 0x7fffffff);
   w_lo = min(w_lo, w_hi);
   if (lane == 0) s_bounds[wave] = int2{w_hi > w_lo ? w_lo : 0x7fffffff, w_hi};
   __syncthreads();
@@ -102,27 +115,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   };
   if (iters > 0) fetch(0, lds);
 
-  u32x4 qf[T::kSteps], gf[T::kSteps];
   float delta = 0.f;
-  {
-    const uint16_t* q = row_of(a.q, a.qs, b, hq, qi);
-    const uint16_t* g = row_of(a.g, a.gs, b, hq, qi);
-    const uint16_t* o = a.out + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
 #pragma unroll
-    for (int t = 0; t < T::kSteps; ++t) {
-      const u32x4 zero = {0u, 0u, 0u, 0u};
-      qf[t] = some ? *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h) : zero;
-      gf[t] = some ? *reinterpret_cast<const u32x4*>(g + 16 * t + 8 * h) : zero;
-      const u32x4 of = some ? *reinterpret_cast<const u32x4*>(o + 16 * t + 8 * h) : zero;
-      float x[8], y[8];
-      unpack16<DT>(gf[t], x);
-      unpack16<DT>(of, y);
+  for (int t = 0; t < T::kSteps; ++t) {
+    float x[8], y[8];
+    unpack16<DT>(gf[t], x);
+    unpack16<DT>(of[t], y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
-    }
+    for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
   }
-  delta = both_sum(delta);
-  const float lse = some ? a.lse[static_cast<int64_t>(pair) * a.rows + row] : kInf;
+  delta = some ? both_sum(delta) : 0.f;
+  lse = some ? lse : kInf;
   const int block = tile * 4 + wave;
   if (block < a.row_blocks) {
     const int64_t at = static_cast<int64_t>(pair) * a.row_blocks + block;
@@ -140,6 +143,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
+  stagger_waves();
   const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
   auto turn = [&](int it, unsigned char* tk, unsigned char* other) {
     wait_loads();
@@ -245,21 +249,19 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   int pair, tile, split;
   {
     int id = blockIdx.x;
-    split = id % a.splits;
-    id /= a.splits;
+    const int rest = a.by_splits.div(id);
+    split = id - rest * a.splits;
+    id = rest;
     if (pairs % 8 == 0) {
-      const int per = pairs / 8, x = id % 8, j = id / 8;
-      pair = x + 8 * (j % per);
-      tile = j / per;
+      const int j = id >> 3;
+      tile = a.by_pairs.div(j);
+      pair = (id & 7) + 8 * (j - tile * (pairs >> 3));
     } else {
-      pair = id % pairs;
-      tile = id / pairs;
+      tile = a.by_pairs.div(id);
+      pair = id - tile * pairs;
     }
-    pair = __builtin_amdgcn_readfirstlane(pair);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    split = __builtin_amdgcn_readfirstlane(split);
   }
-  const int b = pair / a.n_kv, hk = pair - b * a.n_kv;
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
   const int k0 = tile * 128, key = k0 + wave * 32 + (lane & 31);
   const bool live = key < a.n_keys;
   const int wk = k0 + wave * 32;  // this wavefront's first key
@@ -275,20 +277,20 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         last = t;
       }
     }
-    first = wave_min_i(first);
-    last = wave_max_i(last);
-    if (lane == 0) s_first[wave] = first, s_last[wave] = last;
+    const int w_first = min(wave_extreme<false>(first), wave_extreme<false>(__shfl_xor(first, 32)));
+    const int w_last = max(wave_extreme<true>(last), wave_extreme<true>(__shfl_xor(last, 32)));
+    if (lane == 0) s_first[wave] = w_first, s_last[wave] = w_last;
     __syncthreads();
     first = min(min(s_first[0], s_first[1]), min(s_first[2], s_first[3]));
     last = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
     const int n = last < first ? 0 : last - first + 1;
-    const int t0 = static_cast<int>(static_cast<int64_t>(n) * split / a.splits), t1 = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / a.splits);
-    last = __builtin_amdgcn_readfirstlane(first + t1);
+    const int each = a.by_splits.div(n), more = n - each * a.splits;  // the first `more` splits take one more
+    const int t0 = split * each + min(split, more);
+    last = __builtin_amdgcn_readfirstlane(first + t0 + each + (split < more ? 1 : 0));
     first = __builtin_amdgcn_readfirstlane(first + t0);  // blocks [first, last)
     if (n == 0) first = last = 0;
   }
 
-  const uint32_t magic = 0xffffffffu / static_cast<uint32_t>(a.group) + 1;  // (group <= 1024; 0 for a group of 1)
   const uint16_t* qb = a.q + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[1];
   const uint16_t* gb = a.g + b * a.gs[0] + static_cast<int64_t>(hk) * a.group * a.gs[1];
   const char* src = reinterpret_cast<const char*>(wave < 2 ? qb : gb);
@@ -304,13 +306,13 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
 #pragma unroll
     for (int i = 0; i < T::kChunks / 4; ++i)
       off[i] = stage_offset<D>(i, lane, [&](int r) {
-        const int di = (r0 + r) / in_group, hd = (r0 + r) - di * in_group;
+        const int di = a.by_in_group.div(r0 + r), hd = (r0 + r) - di * in_group;
         return static_cast<uint32_t>(di * pos_step32 + hd * head_step);
       });
     s_offsets[tid] = u32x4{off[0], off[1], off[2], off[3]};
   }
   auto fetch = [&](int t, unsigned char* slot) {
-    const int row0 = t * 32, i0 = row0 / a.group, rem = row0 - i0 * a.group, r0 = (wave & 1) * 16;
+    const int row0 = t * 32, i0 = a.by_group.div(row0), rem = row0 - i0 * a.group, r0 = (wave & 1) * 16;
     const char* base = src + __builtin_amdgcn_readfirstlane(i0) * pos_step;
     unsigned char* to = slot + (wave >> 1) * kTileBytes + r0 * T::kPitch;
     if (regular && row0 + 32 <= a.rows) {
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
       int here = lane;
       asm volatile("" : "+v"(here));  // (what this path needs is made here, not kept over the loop)
       stage16<D>(attn_rsrc(base, kRsrcBytes), to, here, [&](int r) {
-        const uint32_t x = static_cast<uint32_t>(rem + r0 + r), di = magic ? __umulhi(x, magic) : x, hd = x - di * a.group;
+        const uint32_t x = static_cast<uint32_t>(rem + r0 + r), di = static_cast<uint32_t>(a.by_group.div(static_cast<int>(x))), hd = x - di * a.group;
         return row0 + r0 + r < a.rows ? di * static_cast<uint32_t>(pos_step32) + hd * static_cast<uint32_t>(head_step) : kOutside;
       });
     }
@@ -347,6 +349,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[o][r] = dv[o][r] = 0.f;
 
+  stagger_waves();
   const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
   for (int t = first; t < last; ++t) {
     wait_loads();
@@ -533,6 +536,9 @@ int launch_bwd(BwdArgs& a, hipStream_t s) {
   const int64_t row_tiles = pairs * ((a.row_blocks + 3) / 4), key_tiles = pairs * a.key_tiles * a.splits;
   const int64_t join = a.splits > 1 ? (pairs * a.n_keys * (2 * D / 4) + 255) / 256 : 0;
   if (row_tiles > 0x7fffffffll || key_tiles > 0x7fffffffll || join > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows");
+  const int all = static_cast<int>(pairs);
+  a.by_splits = Divider(a.splits), a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_in_group = Divider(a.group < 32 ? a.group : 32);
+  a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all);
   const dim3 block(256);
   if (row_tiles > 0) {
     hipLaunchKernelGGL((attn_dq_kernel<DT, D>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);

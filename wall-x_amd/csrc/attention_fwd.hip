@@ -14,6 +14,7 @@ struct FwdArgs {
   AttnMask mask;
   int batch, n_q, n_kv, n_queries, n_keys, group;
   int rows, row_tiles, splits;
+  Divider by_splits, by_pairs, by_kv, by_group;  // by_pairs: of an XCD where they are dealt to XCDs, else all
   float c;                       // scale * log2(e)
   float* part;                   // splits > 1: [pair, split, rows, D] sums, then [pair, split, rows] (maximum, sum)
 };
@@ -102,30 +103,35 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   int pair, tile, split;
   {
     int id = blockIdx.x;
-    split = id % a.splits;
-    id /= a.splits;
+    const int rest = a.by_splits.div(id);
+    split = id - rest * a.splits;
+    id = rest;
     if (pairs % 8 == 0) {
-      const int per = pairs / 8, x = id % 8, j = id / 8;
-      pair = x + 8 * (j % per);
-      tile = a.row_tiles - 1 - j / per;
+      const int j = id >> 3, t = a.by_pairs.div(j);
+      pair = (id & 7) + 8 * (j - t * (pairs >> 3));
+      tile = a.row_tiles - 1 - t;
     } else {
-      pair = id % pairs;
-      tile = a.row_tiles - 1 - id / pairs;
+      const int t = a.by_pairs.div(id);
+      pair = id - t * pairs;
+      tile = a.row_tiles - 1 - t;
     }
-    pair = __builtin_amdgcn_readfirstlane(pair);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    split = __builtin_amdgcn_readfirstlane(split);
   }
-  const int b = pair / a.n_kv, hk = pair - b * a.n_kv;
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
   const int row = tile * 32 * RW + rw * 32 + (lane & 31);
   const bool live = row < a.rows;
-  const int qi = (live ? row : 0) / a.group, hq = hk * a.group + (live ? row : 0) % a.group;
+  const int in_row = live ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
 
+  u32x4 qf[T::kSteps];  // (asked for before anything that depends on memory)
+  {
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + hq * a.qs[1] + qi * a.qs[2];
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) qf[t] = *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h);  // (a row past the last reads the first)
+  }
   int lo = 0, hi = 0;
   if (live) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
   const bool some = hi > lo;
-  int w_lo = wave_min_i(some ? lo : 0x7fffffff), w_hi = wave_max_i(hi);   // any row of the wavefront sees [w_lo, w_hi)
-  const int f_lo = wave_max_i(some ? lo : 0), f_hi = wave_min_i(some ? hi : 0x7fffffff);  // every row that sees something sees [f_lo, f_hi)
+  int w_lo = wave_extreme<false>(some ? lo : 0x7fffffff), w_hi = wave_extreme<true>(hi);   // any row of the wavefront sees [w_lo, w_hi)
+  const int f_lo = wave_extreme<true>(some ? lo : 0), f_hi = wave_extreme<false>(some ? hi : 0x7fffffff);  // every row that sees something sees [f_lo, f_hi)
   if (w_lo > w_hi) w_lo = w_hi;
   // the workgroup's keys
   int g_lo = w_lo, g_hi = w_hi;
@@ -144,19 +150,13 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   }
   {  // this split's share of the tiles
     const int n = (g_hi - g_lo + KB - 1) / KB;
-    const int t0 = static_cast<int>(static_cast<int64_t>(n) * split / a.splits), t1 = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / a.splits);
+    const int each = a.by_splits.div(n), more = n - each * a.splits;  // the first `more` splits take one more
+    const int t0 = split * each + min(split, more), t1 = t0 + each + (split < more ? 1 : 0);
     g_hi = min(g_hi, g_lo + t1 * KB);
     g_lo += t0 * KB;
   }
   const int s_lo = max(lo, g_lo), s_hi = min(hi, g_hi);
   const int tiles = __builtin_amdgcn_readfirstlane((g_hi - g_lo + KB - 1) / KB), iters = (tiles + KW - 1) / KW;
-
-  u32x4 qf[T::kSteps];
-  {
-    const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + hq * a.qs[1] + qi * a.qs[2];
-#pragma unroll
-    for (int t = 0; t < T::kSteps; ++t) qf[t] = live ? *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h) : u32x4{0u, 0u, 0u, 0u};
-  }
 
   constexpr int kElem = F8 ? 1 : 2;
   const char* kp = static_cast<const char*>(a.k) + (b * a.ks[0] + hk * a.ks[1]) * kElem;
@@ -323,6 +323,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
       }
   };
 
+  stagger_waves();
   unsigned char* mine = lds + kw * kBufs * kSlot;
   if (iters > 0) fetch(0, mine);
   auto turn = [&](int it, unsigned char* slot, unsigned char* other) {
@@ -423,10 +424,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) wrong = wrong || v[e] != v[e];
       int lo_r = 0, hi_r = 0;
-      if (row_r < a.rows) key_range(a.mask, b, row_r / a.group, a.n_queries, a.n_keys, lo_r, hi_r);
+      if (row_r < a.rows) key_range(a.mask, b, a.by_group.div(row_r), a.n_queries, a.n_keys, lo_r, hi_r);
       const bool some_r = hi_r > lo_r;
       const int slo = max(lo_r, g_lo), shi = min(hi_r, g_hi);
-      const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + row_r / a.group) * a.n_q + hk * a.group + row_r % a.group) * D;
+      const int i_r = a.by_group.div(row_r);
+      const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i_r) * a.n_q + hk * a.group + row_r - i_r * a.group) * D;
       const int64_t to_part = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_r;
       if (row_r < a.rows && ch < D / 8) {
         if (a.splits > 1) {
@@ -502,8 +504,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
 #pragma unroll
   for (int u = 0; u < 2; ++u) s_out[wave][lane + 64 * u] = o[u];
   __syncthreads();
-  const int b = pair / a.n_kv, hk = pair % a.n_kv;
-  const int i = row / a.group, hq = hk * a.group + row % a.group;
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
+  const int i = a.by_group.div(row), hq = hk * a.group + row - i * a.group;
   int lo, hi;
   key_range(a.mask, b, i, a.n_queries, a.n_keys, lo, hi);
   if (tid < D) {
@@ -537,6 +539,8 @@ template <int DT, int D, bool F8>
 int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
   a.splits = p.splits;
   a.row_tiles = (a.rows + 32 * p.row_waves - 1) / (32 * p.row_waves);
+  const int pairs = a.batch * a.n_kv;
+  a.by_splits = Divider(p.splits), a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_pairs = Divider(pairs % 8 == 0 ? pairs / 8 : pairs);
   const int64_t blocks = static_cast<int64_t>(a.batch) * a.n_kv * a.row_tiles * a.splits;
   if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
