@@ -15,10 +15,14 @@
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
+#include <optional>
 #include <string>
 #include <type_traits>
 
@@ -38,10 +42,21 @@ struct Entry {
   decltype(&wx_permute_rows) permute;
   decltype(&wx_unpermute_rows) unpermute;
   decltype(&wx_unpermute_rows_bwd_clear) unpermute_bwd;
+  decltype(&wx_qk_norm_rope) norm_rope;
+  decltype(&wx_qk_norm_rope_bwd_workspace_bytes) norm_rope_bwd_bytes;
+  decltype(&wx_qk_norm_rope_bwd) norm_rope_bwd;
+  decltype(&wx_attention_workspace_bytes) attention_bytes;
+  decltype(&wx_attention_fwd) attention;
+  decltype(&wx_attention_bwd_workspace_bytes) attention_bwd_bytes;
+  decltype(&wx_attention_bwd) attention_bwd;
+  decltype(&wx_kv_cache_write) cache_write;
+  decltype(&wx_cached_attention) cached_attention;
 } entry;
 const char* const kNames[] = {"wx_last_error_string", "wx_mrope_apply", "wx_mrope_apply_bwd", "wx_mrope_apply_positions",
                               "wx_mrope_apply_packed", "wx_mrope_table_width", "wx_partition_workspace_bytes", "wx_partition_build",
-                              "wx_permute_rows", "wx_unpermute_rows", "wx_unpermute_rows_bwd_clear"};
+                              "wx_permute_rows", "wx_unpermute_rows", "wx_unpermute_rows_bwd_clear", "wx_qk_norm_rope",
+                              "wx_qk_norm_rope_bwd_workspace_bytes", "wx_qk_norm_rope_bwd", "wx_attention_workspace_bytes", "wx_attention_fwd",
+                              "wx_attention_bwd_workspace_bytes", "wx_attention_bwd", "wx_kv_cache_write", "wx_cached_attention"};
 constexpr int kEntries = sizeof(kNames) / sizeof(kNames[0]);
 static_assert(sizeof(Entry) == kEntries * sizeof(void*), "a name per entry point");
 
@@ -255,6 +270,298 @@ PyObject* unpermute_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the norm of q and k with the rotary embedding, attention, the cache.  Forward and backward are autograd nodes of their own here:
+// a Python autograd.Function around native calls costs 50 us of a training pass, as much as the norm's kernels on 5000 tokens take.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+// [B, H, S, D] as the kernels read it through strides: contiguous heads, rows on 16 bytes
+bool rows16(const at::Tensor& t) {
+  if (t.dim() != 4 || (t.stride(3) != 1 && t.size(3) != 1)) return false;
+  const int64_t unit = 16 / t.element_size();
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && (t.stride(i) % unit != 0 || t.stride(i) < 0)) return false;
+  return t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+at::Tensor as_rows16(const at::Tensor& t) { return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+bool packed16(const at::Tensor& t) { return t.is_contiguous() && (t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0); }
+
+struct RowStrides {
+  int64_t v[3];
+  explicit RowStrides(const at::Tensor& t) {
+    for (int i = 0; i < 3; ++i) v[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  }
+};
+
+// [B, H, S, D] over token-major memory, no view of anything: a caller may write into it in place
+at::Tensor token_major(int64_t B, int64_t H, int64_t S, int64_t D, const at::TensorOptions& options) {
+  return at::empty_strided({B, H, S, D}, {S * H * D, D, H * D, 1}, options);
+}
+
+// As run(), for code under an autograd node: the library's errors are exceptions there.
+template <typename F>
+void launch(const at::Tensor& t, F f) {
+  const c10::DeviceGuard guard(t.device());
+  const int rc = f();
+  TORCH_CHECK(rc == 0, "wallx_mi355: ", entry.last_error(), " (status ", rc, ")");
+}
+
+bool optional(PyObject* o, const at::Tensor*& t) {
+  t = nullptr;
+  return o == Py_None || (t = plain(o)) != nullptr;
+}
+bool to_double(PyObject* o, double& v) {
+  if (!PyFloat_CheckExact(o)) return false;
+  v = PyFloat_AS_DOUBLE(o);
+  return true;
+}
+bool needs_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+PyObject* wrap_all(const variable_list& v) { return v.size() == 1 ? wrap(v[0]) : pair(v[0], v[1]); }
+
+struct NormRope : torch::autograd::Function<NormRope> {
+  static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k, const Variable& wq, const Variable& wk, const Variable& source,
+                               const std::optional<at::Tensor>& inv_freq, at::IntArrayRef section, double eps, int64_t layout) {
+    const at::Tensor freq = inv_freq.value_or(at::Tensor());
+    at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+    const int sec[3] = {static_cast<int>(section[0]), static_cast<int>(section[1]), static_cast<int>(section[2])};
+    launch(q, [&] {
+      return entry.norm_rope(ptr(q), ptr(k), ptr(wq), ptr(wk), static_cast<float>(eps), ptr(source), freq.defined() ? static_cast<const float*>(ptr(freq)) : nullptr,
+                             ptr(qo), ptr(ko), q.size(0), q.size(2), static_cast<int>(q.size(1)), static_cast<int>(k.size(1)), static_cast<int>(q.size(3)),
+                             RowStrides(q).v, RowStrides(k).v, sec, static_cast<int>(layout), dtype_code(q.scalar_type()), stream_of(q));
+    });
+    if (ctx) {
+      ctx->save_for_backward({q, k, wq, wk, source, freq});
+      ctx->saved_data["section"] = section.vec();
+      ctx->saved_data["eps"] = eps;
+      ctx->saved_data["layout"] = layout;
+    }
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3], &source = saved[4], &freq = saved[5];
+    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope's backward is not differentiable");
+    const std::vector<int64_t> section = ctx->saved_data["section"].toIntVector();
+    const int sec[3] = {static_cast<int>(section[0]), static_cast<int>(section[1]), static_cast<int>(section[2])};
+    const int layout = static_cast<int>(ctx->saved_data["layout"].toInt());
+    variable_list out(9);
+    launch(q, [&] {
+      const at::Tensor gq = as_rows16(grads[0]), gk = as_rows16(grads[1]);
+      const at::Tensor* like[4] = {&q, &k, &wq, &wk};
+      for (int i = 0; i < 4; ++i)
+        if (ctx->needs_input_grad(i)) out[i] = at::empty(like[i]->sizes(), q.options());
+      const int D = static_cast<int>(q.size(3));
+      const bool weights = out[2].defined() || out[3].defined();
+      const size_t bytes = weights ? entry.norm_rope_bwd_bytes(D) : 0;
+      const at::Tensor work = weights ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
+      auto at_ = [&](int i) { return out[i].defined() ? ptr(out[i]) : nullptr; };
+      return entry.norm_rope_bwd(ptr(gq), ptr(gk), ptr(q), ptr(k), ptr(wq), ptr(wk), static_cast<float>(ctx->saved_data["eps"].toDouble()), ptr(source),
+                                 freq.defined() ? static_cast<const float*>(ptr(freq)) : nullptr, at_(0), at_(1), at_(2), at_(3), q.size(0), q.size(2),
+                                 static_cast<int>(q.size(1)), static_cast<int>(k.size(1)), D, RowStrides(gq).v, RowStrides(gk).v, RowStrides(q).v,
+                                 RowStrides(k).v, sec, layout, dtype_code(q.scalar_type()), weights ? ptr(work) : nullptr, bytes, stream_of(q));
+    });
+    return out;
+  }
+};
+
+// norm_rope(q, k, q_weight, k_weight, source, inv_freq or None, section, eps, layout) -> (q_out, k_out) or None.
+PyObject* norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int sec[3], layout;
+  double eps;
+  const at::Tensor* freq;
+  if (n != 9 || !entry.norm_rope || !optional(args[5], freq) || !section_of(args[6], sec) || !to_double(args[7], eps) || !layout_of(args[8], layout)) return none();
+  const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *wq = plain(args[2]), *wk = plain(args[3]), *source = plain(args[4]);
+  if (!q || !k || !wq || !wk || !source || !rows16(*q) || !rows16(*k)) return none();
+  const int64_t B = q->size(0), S = q->size(2), D = q->size(3);
+  const at::ScalarType dt = q->scalar_type();
+  if (k->size(0) != B || k->size(2) != S || k->size(3) != D || dtype_code(dt) < 0 || q->size(1) > INT32_MAX || k->size(1) > INT32_MAX || D > INT32_MAX) return none();
+  for (const at::Tensor* t : {k, wq, wk, source, freq})
+    if (t && t->device() != q->device()) return none();
+  for (const at::Tensor* w : {wq, wk})
+    if (w->scalar_type() != dt || w->dim() != 1 || w->size(0) != D || !packed16(*w)) return none();
+  if (k->scalar_type() != dt || !packed16(*source)) return none();
+  if (freq) {
+    if (source->dim() != 3 || source->size(0) != 3 || source->size(1) != B || source->size(2) != S || source->scalar_type() != at::kLong) return none();
+    if (freq->dim() != 1 || freq->size(0) != D / 2 || freq->scalar_type() != at::kFloat || !freq->is_contiguous() || freq->numel() == 0) return none();
+  } else {
+    const int width = entry.table_width(static_cast<int>(D), sec, layout);
+    if (width < 0 || source->dim() != 2 || source->size(0) != B * S || source->size(1) != width || source->scalar_type() != at::kInt || dt != at::kBFloat16) return none();
+  }
+  const int64_t section[3] = {sec[0], sec[1], sec[2]};
+  const std::optional<at::Tensor> inv_freq = freq ? std::optional<at::Tensor>(*freq) : std::nullopt;
+  variable_list out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    out = needs_grad({q, k, wq, wk}) ? NormRope::apply(*q, *k, *wq, *wk, *source, inv_freq, at::IntArrayRef(section, 3), eps, static_cast<int64_t>(layout))
+                                     : NormRope::forward(nullptr, *q, *k, *wq, *wk, *source, inv_freq, at::IntArrayRef(section, 3), eps, layout);
+  }
+  return wrap_all(out);
+  END_HANDLE_TH_ERRORS
+}
+
+const int32_t* ints(const at::Tensor& t) { return t.defined() ? static_cast<const int32_t*>(ptr(t)) : nullptr; }
+
+struct Attention : torch::autograd::Function<Attention> {
+  static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k, const Variable& v, const std::optional<at::Tensor>& key_ranges,
+                               const std::optional<at::Tensor>& key_lengths, bool causal, double scale) {
+    const at::Tensor ranges = key_ranges.value_or(at::Tensor()), lengths = key_lengths.value_or(at::Tensor());
+    const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
+    at::Tensor out, lse;
+    launch(q, [&] {
+      out = token_major(B, Hq, Sq, D, q.options());
+      if (ctx) lse = at::empty({B, Hk, Sq * (Hq / Hk)}, q.options().dtype(at::kFloat));
+      const size_t bytes = entry.attention_bytes(B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D));
+      const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
+      return entry.attention(ptr(q), ptr(k), ptr(v), ptr(out), ctx ? static_cast<float*>(ptr(lse)) : nullptr, ints(ranges), ints(lengths), causal, B,
+                             static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D), RowStrides(q).v, RowStrides(k).v, RowStrides(v).v,
+                             static_cast<float>(scale), dtype_code(q.scalar_type()), bytes ? ptr(work) : nullptr, bytes, stream_of(q));
+    });
+    if (ctx) {
+      ctx->save_for_backward({q, k, v, out, lse, ranges, lengths});
+      ctx->saved_data["causal"] = causal;
+      ctx->saved_data["scale"] = scale;
+    }
+    return {out};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &ranges = saved[5], &lengths = saved[6];
+    TORCH_CHECK(!at::GradMode::is_enabled(), "attention's backward is not differentiable");
+    const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
+    at::Tensor dq, dk, dv;
+    launch(q, [&] {
+      const at::Tensor g = as_rows16(grads[0]);
+      dq = token_major(B, Hq, Sq, D, q.options());
+      dk = token_major(B, Hk, Sk, D, q.options());
+      dv = token_major(B, Hk, Sk, D, q.options());
+      at::Tensor tokens = out.transpose(1, 2);  // (saved-tensor hooks may hand it back in another order)
+      if (!packed16(tokens)) tokens = tokens.clone(at::MemoryFormat::Contiguous);
+      const size_t bytes = entry.attention_bwd_bytes(B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D));
+      const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
+      return entry.attention_bwd(ptr(q), ptr(k), ptr(v), ptr(tokens), static_cast<const float*>(ptr(lse)), ptr(g), ptr(dq), ptr(dk), ptr(dv), ints(ranges),
+                                 ints(lengths), ctx->saved_data["causal"].toBool(), B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D),
+                                 RowStrides(q).v, RowStrides(k).v, RowStrides(v).v, RowStrides(g).v, static_cast<float>(ctx->saved_data["scale"].toDouble()),
+                                 dtype_code(q.scalar_type()), bytes ? ptr(work) : nullptr, bytes, stream_of(q));
+    });
+    variable_list r(7);
+    if (ctx->needs_input_grad(0)) r[0] = dq;
+    if (ctx->needs_input_grad(1)) r[1] = dk;
+    if (ctx->needs_input_grad(2)) r[2] = dv;
+    return r;
+  }
+};
+
+// The mask and the scale that attention's two forms share.
+struct MaskArgs {
+  const at::Tensor *ranges, *lengths;
+  bool causal;
+  double scale;
+  bool from(PyObject* r, PyObject* l, PyObject* c, PyObject* s, const at::Tensor& q) {
+    if (!optional(r, ranges) || !optional(l, lengths) || !PyBool_Check(c)) return false;
+    causal = c == Py_True;
+    scale = 1.0 / std::sqrt(static_cast<double>(q.size(3)));
+    if (s != Py_None && !to_double(s, scale)) return false;
+    const int64_t B = q.size(0), S = q.size(2);
+    if (ranges && (ranges->dim() != 3 || ranges->size(0) != B || ranges->size(1) != S || ranges->size(2) != 2 || ranges->scalar_type() != at::kInt || !packed16(*ranges)))
+      return false;
+    if (lengths && (lengths->dim() != 1 || lengths->size(0) != B || lengths->scalar_type() != at::kInt || !lengths->is_contiguous())) return false;
+    for (const at::Tensor* t : {ranges, lengths})
+      if (t && t->device() != q.device()) return false;
+    return true;
+  }
+};
+bool attention_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+bool heads_fit(int64_t Hq, int64_t Hk) { return Hk > 0 && Hq % Hk == 0 && Hq <= INT32_MAX; }
+
+// attention(q, k, v, key_ranges, key_lengths, causal, scale) -> out or None.
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !entry.attention) return none();
+  const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *v = plain(args[2]);
+  MaskArgs m;
+  if (!q || !k || !v || !rows16(*q) || !rows16(*k) || !rows16(*v) || !m.from(args[3], args[4], args[5], args[6], *q)) return none();
+  if (!k->sizes().equals(v->sizes()) || k->size(0) != q->size(0) || k->size(3) != q->size(3) || !heads_fit(q->size(1), k->size(1)) || q->size(3) > 1024) return none();
+  if (!attention_type(q->scalar_type()) || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || k->device() != q->device() ||
+      v->device() != q->device())
+    return none();
+  const std::optional<at::Tensor> ranges = m.ranges ? std::optional<at::Tensor>(*m.ranges) : std::nullopt,
+                                  lengths = m.lengths ? std::optional<at::Tensor>(*m.lengths) : std::nullopt;
+  variable_list out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    out = needs_grad({q, k, v}) ? Attention::apply(*q, *k, *v, ranges, lengths, m.causal, m.scale) : Attention::forward(nullptr, *q, *k, *v, ranges, lengths, m.causal, m.scale);
+  }
+  return wrap(out[0]);
+  END_HANDLE_TH_ERRORS
+}
+
+// k_cache, v_cache, k_scale, v_scale on q's device in the layout that the kernels take
+bool cache_of(PyObject* const* args, const at::Tensor& q, const at::Tensor* (&c)[4]) {
+  for (int i = 0; i < 4; ++i) {
+    if ((c[i] = plain(args[i])) == nullptr || !packed16(*c[i]) || c[i]->device() != q.device()) return false;
+    if (c[i]->scalar_type() != (i < 2 ? at::kFloat8_e4m3fn : at::kFloat)) return false;
+  }
+  if (c[0]->dim() != 4 || !c[1]->sizes().equals(c[0]->sizes()) || c[0]->size(0) != q.size(0) || c[0]->size(3) != q.size(3) || q.size(3) > 1024) return false;
+  for (int i = 2; i < 4; ++i)
+    if (!c[i]->sizes().equals(c[0]->sizes().slice(0, 3))) return false;
+  return true;
+}
+
+// cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges, key_lengths, causal, scale) -> out or None.
+PyObject* cached_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !entry.cached_attention) return none();
+  const at::Tensor *q = plain(args[0]), *c[4];
+  MaskArgs m;
+  if (!q || !rows16(*q) || !cache_of(args + 1, *q, c) || !m.from(args[5], args[6], args[7], args[8], *q)) return none();
+  if (!attention_type(q->scalar_type()) || !heads_fit(q->size(1), c[0]->size(1)) || needs_grad({q})) return none();
+  const int64_t B = q->size(0), Hq = q->size(1), Sq = q->size(2), D = q->size(3), Hk = c[0]->size(1), C = c[0]->size(2);
+  at::Tensor out;
+  const bool ok = run(*q, [&] {
+    out = token_major(B, Hq, Sq, D, q->options());
+    const size_t bytes = entry.attention_bytes(B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, C, static_cast<int>(D));
+    const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q->options().dtype(at::kByte)) : at::Tensor();
+    return entry.cached_attention(ptr(*q), ptr(*c[0]), ptr(*c[1]), static_cast<const float*>(ptr(*c[2])), static_cast<const float*>(ptr(*c[3])), ptr(out),
+                                  m.ranges ? ints(*m.ranges) : nullptr, m.lengths ? ints(*m.lengths) : nullptr, m.causal, B, static_cast<int>(Hq),
+                                  static_cast<int>(Hk), Sq, C, static_cast<int>(D), RowStrides(*q).v, static_cast<float>(m.scale),
+                                  dtype_code(q->scalar_type()), bytes ? ptr(work) : nullptr, bytes, stream_of(*q));
+  });
+  return ok ? wrap(out) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths) -> True or None.
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !entry.cache_write) return none();
+  const at::Tensor *k = plain(args[0]), *v = plain(args[1]), *c[4], *start = plain(args[6]), *lengths;
+  if (!k || !v || !start || !optional(args[7], lengths) || !rows16(*k) || !rows16(*v) || !cache_of(args + 2, *k, c)) return none();
+  if (!v->sizes().equals(k->sizes()) || c[0]->size(1) != k->size(1) || k->size(1) > INT32_MAX || !attention_type(k->scalar_type()) || v->scalar_type() != k->scalar_type() ||
+      v->device() != k->device() || needs_grad({k, v}))
+    return none();
+  for (const at::Tensor* t : {start, lengths})
+    if (t && (t->dim() != 1 || t->size(0) != k->size(0) || t->scalar_type() != at::kInt || !t->is_contiguous() || t->device() != k->device())) return none();
+  const bool ok = run(*k, [&] {
+    return entry.cache_write(ptr(*k), ptr(*v), ptr(*c[0]), ptr(*c[1]), static_cast<float*>(ptr(*c[2])), static_cast<float*>(ptr(*c[3])), ints(*start),
+                             lengths ? ints(*lengths) : nullptr, k->size(0), static_cast<int>(k->size(1)), k->size(2), c[0]->size(2), static_cast<int>(k->size(3)),
+                             RowStrides(*k).v, RowStrides(*v).v, dtype_code(k->scalar_type()), stream_of(*k));
+  });
+  if (!ok) return nullptr;
+  for (const at::Tensor* t : c)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // (written in place, as an in-place op would)
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // names() -> the entry points in the order bind() takes their addresses in.
 PyObject* names(PyObject*, PyObject*) {
   PyObject* const r = PyTuple_New(kEntries);
@@ -282,6 +589,10 @@ PyMethodDef methods[] = {{"rope", WX_FAST(rope), nullptr},
                          {"permute", WX_FAST(permute), nullptr},
                          {"unpermute", WX_FAST(unpermute), nullptr},
                          {"unpermute_bwd", WX_FAST(unpermute_bwd), nullptr},
+                         {"norm_rope", WX_FAST(norm_rope), nullptr},
+                         {"attention", WX_FAST(attention), nullptr},
+                         {"cached_attention", WX_FAST(cached_attention), nullptr},
+                         {"cache_write", WX_FAST(cache_write), nullptr},
                          {"bind", WX_FAST(bind), nullptr},
                          {"names", names, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

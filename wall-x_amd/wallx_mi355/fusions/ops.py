@@ -494,6 +494,11 @@ class QKNormRoPE(torch.autograd.Function):
 
 
 def _qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout):
+    made = _lib.host().norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout)
+    if made is not None:
+        return made
+    if inv_freq is not None:
+        source, inv_freq = source.contiguous(), inv_freq.to(torch.float32).contiguous()
     for name, t in (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
         if t.is_cpu:
             raise RuntimeError(f"[Error] The input `{name}` of qk_norm_rope op is on the device: CPU!")
@@ -520,7 +525,7 @@ def qk_norm_rope_from_table(q, k, q_weight, k_weight, table, mrope_section, eps=
 def qk_norm_rope_from_positions(q, k, q_weight, k_weight, position_ids, inv_freq, mrope_section, eps=1e-6, layout="hf"):
     """qk_norm_rope_from_table with the angles evaluated from position_ids [3, B, S] int64 and inv_freq [D / 2] fp32 (to better
     than the fp32 product, at any position); bf16, fp16 or fp32."""
-    return _qk_norm_rope(q, k, q_weight, k_weight, position_ids.contiguous(), inv_freq.to(torch.float32).contiguous(), mrope_section, eps, layout)
+    return _qk_norm_rope(q, k, q_weight, k_weight, position_ids, inv_freq, mrope_section, eps, layout)
 
 
 # ----------------------------------------------------------------------------- attention
@@ -553,6 +558,9 @@ def attention(q, k, v, key_ranges=None, key_lengths=None, causal=False, scale=No
     the device and never read by the host.  A query that sees no key gets zeros, and keys that a query does not see do not
     influence its row whatever they hold.  Few queries over many keys (generation) are spread over the keys.  Differentiable in q, k
     and v; the backward writes the same bits every time."""
+    made = _lib.host().attention(q, k, v, key_ranges, key_lengths, causal, scale)
+    if made is not None:
+        return made
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.is_cpu:
             raise RuntimeError(f"[Error] The input `{name}` of attention op is on the device: CPU!")
@@ -604,6 +612,8 @@ def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths=None
     of row b (all without lengths) to position start[b] + s, with scale = max(max |x| / 448, 2^-126) per token and head and
     code = e4m3(x / scale).  start, lengths int32 [B] on the device, never read by the host.  Positions outside the cache are
     dropped; the rest of it stays as it is.  Not differentiable."""
+    if _lib.host().cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths):
+        return
     for name, t in (("k", k), ("v", v)):
         if t.is_cpu:
             raise RuntimeError(f"[Error] The input `{name}` of kv_cache_write op is on the device: CPU!")
@@ -616,6 +626,9 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key
     """`attention` of q [B, Hq, Sq, D] over a quantised cache, read as it is: key_lengths int32 [B] tokens of it are filled; with
     causal=True the queries are the last Sq of them (generation; without, as in a denoise step, all of them see all).  Inference
     only."""
+    made = _lib.host().cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges, key_lengths, causal, scale)
+    if made is not None:
+        return made
     if q.is_cpu:
         raise RuntimeError("[Error] The input `q` of cached_attention op is on the device: CPU!")
     if torch.is_grad_enabled() and q.requires_grad:

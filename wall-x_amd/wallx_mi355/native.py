@@ -638,6 +638,11 @@ def _attention_shapes(q, k, v):
         raise RuntimeError("q, k and v must share one dtype")
 
 
+def _token_major(B, H, S, D, like):
+    """[B, H, S, D] over token-major memory, no view of another tensor: a caller may write into it in place."""
+    return torch.empty_strided((B, H, S, D), (S * H * D, D, H * D, 1), dtype=like.dtype, device=like.device)
+
+
 def attention_fwd(q, k, v, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None, want_lse: bool = False):
     """(out [B, Hq, Sq, D] over token-major memory, lse or None): softmax(scale q k^T) v of q [B, Hq, Sq, D] over k and v
     [B, Hkv, Sk, D] (any strides), query i of row b seeing the keys [lo, hi) of key_ranges int32 [B, Sq, 2], below key_lengths
@@ -648,14 +653,14 @@ def attention_fwd(q, k, v, key_ranges=None, key_lengths=None, causal: bool = Fal
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     B, Hq, Sq, D = q.shape
     Hk, Sk = k.size(1), k.size(2)
-    out = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device=q.device)
+    out = _token_major(B, Hq, Sq, D, q)
     lse = torch.empty((B, Hk, Sq * (Hq // Hk)), dtype=torch.float32, device=q.device) if want_lse else None
     with _DeviceGuard(q):
         n_work = _lib.load().wx_attention_workspace_bytes(B, Hq, Hk, Sq, Sk, D)
         work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
         _lib.call("wx_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(key_ranges), _ptr(key_lengths), int(bool(causal)), B, Hq, Hk,
                   Sq, Sk, D, _row_strides(q), _row_strides(k), _row_strides(v), scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
-    return out.transpose(1, 2), lse
+    return out, lse
 
 
 def attention_bwd(grad_out, q, k, v, out, lse, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None):
@@ -669,18 +674,17 @@ def attention_bwd(grad_out, q, k, v, out, lse, key_ranges=None, key_lengths=None
     B, Hq, Sq, D = q.shape
     Hk, Sk = k.size(1), k.size(2)
     tokens = out.transpose(1, 2)
-    tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
+    tokens = _packed16(tokens)
     if lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hk, Sq * (Hq // Hk)) or not lse.is_contiguous():
         raise RuntimeError("lse must be what attention_fwd returned")
-    dq = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+    dq, dk, dv = _token_major(B, Hq, Sq, D, q), _token_major(B, Hk, Sk, D, q), _token_major(B, Hk, Sk, D, q)
     with _DeviceGuard(q):
         n_work = _lib.load().wx_attention_bwd_workspace_bytes(B, Hq, Hk, Sq, Sk, D)
         work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
         _lib.call("wx_attention_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(tokens), _ptr(lse), _ptr(grad_out), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(key_ranges),
                   _ptr(key_lengths), int(bool(causal)), B, Hq, Hk, Sq, Sk, D, _row_strides(q), _row_strides(k), _row_strides(v), _row_strides(grad_out),
                   scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
-    return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2)
+    return dq, dk, dv
 
 
 # ----------------------------------------------------------------------------- quantised key / value cache
@@ -711,6 +715,9 @@ def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths=None
     with _DeviceGuard(k):
         _lib.call("wx_kv_cache_write", _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(start), _ptr(lengths), B, Hk, S,
                   k_cache.size(2), D, _row_strides(k), _row_strides(v), _DTYPES[k.dtype], _stream(k))
+    for t in (k_cache, v_cache, k_scale, v_scale):
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)  # (written in place, as an in-place op would)
 
 
 def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None):
@@ -723,13 +730,13 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key
     key_ranges, key_lengths, scale = _attention_args(q, C, Hk, key_ranges, key_lengths, scale)
     q = _rows16(q)
     Hq, Sq = q.size(1), q.size(2)
-    out = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device=q.device)
+    out = _token_major(B, Hq, Sq, D, q)
     with _DeviceGuard(q):
         n_work = _lib.load().wx_attention_workspace_bytes(B, Hq, Hk, Sq, C, D)
         work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
         _lib.call("wx_cached_attention", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(out), _ptr(key_ranges), _ptr(key_lengths),
                   int(bool(causal)), B, Hq, Hk, Sq, C, D, _row_strides(q), scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
-    return out.transpose(1, 2)
+    return out
 
 
 # ----------------------------------------------------------------------------- index builders
