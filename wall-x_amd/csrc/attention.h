@@ -37,22 +37,27 @@ struct AttnMask {
   int causal;
 };
 
-// [lo, hi) of the keys that query i of sequence b sees; lo = hi = 0 when there are none.
-__device__ __forceinline__ void key_range(const AttnMask& m, int b, int i, int n_queries, int n_keys, int& lo, int& hi) {
-  int len = n_keys;
-  if (m.lens != nullptr) {
-    len = m.lens[b];
-    len = len < 0 ? 0 : (len > n_keys ? n_keys : len);
-  }
-  lo = 0;
-  hi = len;
+// [lo, hi) of the keys that query i of sequence b sees; lo = hi = 0 when there are none.  What the mask holds in memory is asked
+// for first (mask_row), so that it does not wait behind what is asked for in between.
+struct MaskRow {
+  int len;
+  int2 range;
+};
+__device__ __forceinline__ MaskRow mask_row(const AttnMask& m, int b, int i, int n_queries, int n_keys) {
+  MaskRow r{n_keys, int2{0, n_keys}};
+  if (m.ranges != nullptr) r.range = m.ranges[static_cast<int64_t>(b) * n_queries + i];
+  if (m.lens != nullptr) r.len = m.lens[b];
+  return r;
+}
+__device__ __forceinline__ void key_range(const AttnMask& m, const MaskRow& r, int i, int n_queries, int n_keys, int& lo, int& hi) {
+  const int len = r.len < 0 ? 0 : (r.len > n_keys ? n_keys : r.len);
+  lo = max(0, r.range.x);
+  hi = min(len, r.range.y);
   if (m.causal) hi = min(hi, len - n_queries + i + 1);
-  if (m.ranges != nullptr) {
-    const int2 r = m.ranges[static_cast<int64_t>(b) * n_queries + i];
-    lo = max(lo, r.x);
-    hi = min(hi, r.y);
-  }
   if (hi <= lo) lo = hi = 0;
+}
+__device__ __forceinline__ void key_range(const AttnMask& m, int b, int i, int n_queries, int n_keys, int& lo, int& hi) {
+  key_range(m, mask_row(m, b, i, n_queries, n_keys), i, n_queries, n_keys, lo, hi);
 }
 
 template <int D>
@@ -216,11 +221,18 @@ __device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned ch
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(offsets[i]), 0, 0, 0);
 }
 
-// Two wavefronts share a SIMD.  Left alike they fall into step, both in the matrix products and then both in the softmax; with the
-// one in the odd slot (hardware register HW_ID, bits 3:0) ahead at every issue, one computes while the other multiplies.
-__device__ __forceinline__ void stagger_waves() {
-  if (__builtin_amdgcn_s_getreg((3 << 11) | 4) & 1) __builtin_amdgcn_s_setprio(1);
+// One LDS array per (size, index).  A kernel's two slots for tiles are arrays of their own, at constant addresses in a loop unrolled
+// by two: where both were parts of one array the compiler took the transposing reads of a tile for reads of what the loads in
+// flight write, and waited for the next tile in the middle of every tile.
+template <int BYTES, int ID>
+__device__ __forceinline__ unsigned char* lds_slot() {
+  __shared__ __attribute__((aligned(1024))) unsigned char s[BYTES];
+  return s;
 }
+
+// Keeps the order in which the code stands.  Left to itself the scheduler asks for an operand from LDS right in front of the product
+// that needs it and waits for each; the loops below ask a few products ahead and put other work between the products.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 __device__ __forceinline__ void attn_barrier() {  // (no fences: they would drain the loads in flight)
   asm volatile("" ::: "memory");
@@ -232,6 +244,12 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(attn_wait(0, 15));
   asm volatile("" ::: "memory");
+}
+// behind this wavefront's own LDS writes; loads from memory stay in flight
+__device__ __forceinline__ void attn_lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(attn_wait(63, 0));
+  attn_barrier();
 }
 __device__ __forceinline__ void wait_lds() {
   asm volatile("" ::: "memory");

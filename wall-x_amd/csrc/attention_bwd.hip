@@ -61,7 +61,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   const int row = tile * 128 + wave * 32 + (lane & 31);
   const bool live = row < a.rows;
   const int in_row = live ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
-  u32x4 qf[T::kSteps], gf[T::kSteps], of[T::kSteps];  // (asked for before anything that depends on memory; a row past the last reads the first)
+  const MaskRow row_mask = mask_row(a.mask, b, qi, a.n_queries, a.n_keys);
+  in_order();
+  u32x4 qf[T::kSteps], gf[T::kSteps], of[T::kSteps];  // (asked for behind the mask and before anything that waits for it; a row past the last reads the first)
   {
     const uint16_t* q = row_of(a.q, a.qs, b, hq, qi);
     const uint16_t* g = row_of(a.g, a.gs, b, hq, qi);
@@ -74,15 +76,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
     }
   }
   float lse = a.lse[static_cast<int64_t>(pair) * a.rows + in_row];
+  in_order();
   int lo = 0, hi = 0;
-  if (live) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
+  if (live) key_range(a.mask, row_mask, qi, a.n_queries, a.n_keys, lo, hi);
   const bool some = hi > lo;
   int w_lo = wave_extreme<false>(some ? lo : 0x7fffffff);
   const int w_hi = wave_extreme<true>(hi);
   const int f_lo = wave_extreme<true>(some ? lo : 0), f_hi = wave_extreme<false>(some ? hi : 0x7fffffff);
   w_lo = min(w_lo, w_hi);
   if (lane == 0) s_bounds[wave] = int2{w_hi > w_lo ? w_lo : 0x7fffffff, w_hi};
-  __syncthreads();
+  attn_lds_barrier();
   int g_lo = 0x7fffffff, g_hi = 0;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -143,7 +146,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
-  stagger_waves();
   const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
   auto turn = [&](int it, unsigned char* tk, unsigned char* other) {
     wait_loads();
@@ -349,7 +351,6 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[o][r] = dv[o][r] = 0.f;
 
-  stagger_waves();
   const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
   for (int t = first; t < last; ++t) {
     wait_loads();

@@ -91,9 +91,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   constexpr int kTileBytes = KB * T::kPitch;
   constexpr int kScaleBytes = F8 ? 2 * KB * 4 : 0;
   constexpr int kSlot = 2 * kTileBytes + kScaleBytes;
-  constexpr int kTiles = KW * kBufs * kSlot;
-  constexpr int kJoin = KW > 1 ? 4 * 32 * (D + 4) * 4 + 4 * 32 * 8 : 0;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[kTiles > kJoin ? kTiles : kJoin];
+  constexpr int kTiles = KW * kSlot;                                      // of one buffer
+  constexpr int kJoinStats = 4 * 32 * (64 + 4) * 4, kJoin = KW > 1 ? kJoinStats + 4 * 32 * 8 : 0;  // 64 channels at a time
+  unsigned char* const lds = lds_slot<(kTiles > kJoin ? kTiles : kJoin), 0>();
+  unsigned char* const lds1 = lds_slot<(kBufs == 2 ? kTiles : 16), 1>();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave % RW, kw = wave / RW, h = lane >> 5;
 
@@ -121,14 +122,17 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   const bool live = row < a.rows;
   const int in_row = live ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
 
-  u32x4 qf[T::kSteps];  // (asked for before anything that depends on memory)
+  const MaskRow row_mask = mask_row(a.mask, b, qi, a.n_queries, a.n_keys);
+  in_order();
+  u32x4 qf[T::kSteps];  // (asked for behind the mask and before anything that waits for it)
   {
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + hq * a.qs[1] + qi * a.qs[2];
 #pragma unroll
     for (int t = 0; t < T::kSteps; ++t) qf[t] = *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h);  // (a row past the last reads the first)
   }
+  in_order();
   int lo = 0, hi = 0;
-  if (live) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
+  if (live) key_range(a.mask, row_mask, qi, a.n_queries, a.n_keys, lo, hi);
   const bool some = hi > lo;
   int w_lo = wave_extreme<false>(some ? lo : 0x7fffffff), w_hi = wave_extreme<true>(hi);   // any row of the wavefront sees [w_lo, w_hi)
   const int f_lo = wave_extreme<true>(some ? lo : 0), f_hi = wave_extreme<false>(some ? hi : 0x7fffffff);  // every row that sees something sees [f_lo, f_hi)
@@ -138,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   if constexpr (RW > 1) {
     __shared__ int2 bounds[RW];
     if (kw == 0 && lane == 0) bounds[rw] = int2{w_hi > w_lo ? w_lo : 0x7fffffff, w_hi};
-    __syncthreads();
+    attn_lds_barrier();
     g_lo = 0x7fffffff, g_hi = 0;
 #pragma unroll
     for (int u = 0; u < RW; ++u) {
@@ -246,24 +250,41 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
     for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
   float m = -kInf, l = 0.f;  // running maximum (both halves alike) and this lane's share of the sum
 
+  // One tile: the scores, then the powers and the products with the values.  A product's operand is asked for kAhead products
+  // before it, and the second half's powers are found under the first half's products.
   auto step = [&](const unsigned char* tk, int k0) {
+    constexpr int kAhead = D == 80 ? 3 : 4, kScores = NT * T::kSteps, kProducts = NT * 2 * T::kOut;
     const unsigned char* tv = tk + kTileBytes;
     const float* scales = reinterpret_cast<const float*>(tk + 2 * kTileBytes);
+    int rows_here = rows_at, cols_here = cols_at;  // (the addresses are made from these here: kept over the loop they would be spilled)
+    asm volatile("" : "+v"(rows_here), "+v"(cols_here));
+    auto read_k = [&](int i) { return read_rows<D>(tk, 32 * (i % NT), i / NT, rows_here); };
+    auto read_v = [&](int i) { return read_cols<D>(tv, 32 * (i / (2 * T::kOut)), i / T::kOut % 2, i % T::kOut, cols_here); };
     f32x16 s[NT];
+    u32x4 f[kAhead];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+    in_order();
 #pragma unroll
-      for (int t = 0; t < T::kSteps; ++t) s[n] = mfma<DT>(read_rows<D>(tk, 32 * n, t, rows_at), qf[t], s[n]);
+    for (int i = 0; i < kScores; ++i) {
+      s[i % NT] = mfma<DT>(f[i % kAhead], qf[i / NT], s[i % NT]);
+      if (i + kAhead < kScores) f[i % kAhead] = read_k(i + kAhead);
+      in_order();
     }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = read_v(i);
+    in_order();
     if constexpr (F8) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float4 f = *reinterpret_cast<const float4*>(scales + 32 * n + 8 * g + 4 * h);
-          s[n][4 * g] *= f.x, s[n][4 * g + 1] *= f.y, s[n][4 * g + 2] *= f.z, s[n][4 * g + 3] *= f.w;
+          const float4 x = *reinterpret_cast<const float4*>(scales + 32 * n + 8 * g + 4 * h);
+          s[n][4 * g] *= x.x, s[n][4 * g + 1] *= x.y, s[n][4 * g + 2] *= x.z, s[n][4 * g + 3] *= x.w;
         }
     }
     if (k0 < f_lo || k0 + KB > f_hi || k0 + KB > g_hi) {  // some row does not see all of the tile
@@ -277,12 +298,12 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
           s[n][r] = at < span ? s[n][r] : -kInf;
         }
     }
-    float top = s[0][0];
+    float tops[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-    top = both_max(top);
+      for (int r = 0; r < 16; r += 2) tops[r / 2 % 4] = fmaxf(fmaxf(tops[r / 2 % 4], s[n][r]), s[n][r + 1]);
+    const float top = both_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
     // The maximum is only there to keep the powers in range: it moves (and the sums are rescaled) when a score exceeds it
     // by more than 2^8, not with every new maximum.
     if (__any((top - m) * a.c > 8.f)) {
@@ -295,36 +316,38 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
         for (int r = 0; r < 16; ++r) acc[o][r] *= alpha;
     }
     const float mc = m == -kInf ? 0.f : m * a.c;
-    float sum = 0.f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.c, -mc));
-        sum += s[n][r];
+    float sums[2] = {0.f, 0.f};
+    auto power = [&](int n, int r) {  // of registers r and r + 1
+      s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.c, -mc));
+      s[n][r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r + 1], a.c, -mc));
+      sums[0] += s[n][r];
+      sums[1] += s[n][r + 1];
+      if constexpr (F8) {
+        const float2 x = *reinterpret_cast<const float2*>(scales + KB + 32 * n + 8 * (r / 4) + 4 * h + r % 4);
+        s[n][r] *= x.x, s[n][r + 1] *= x.y;
       }
-    l += sum;
-    if constexpr (F8) {
+    };
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int u = 0; u < 8; ++u) power(0, 2 * u);
+    u32x4 p[2] = {pack_step<DT>(s[0], 0), pack_step<DT>(s[0], 1)};
+    in_order();
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 f = *reinterpret_cast<const float4*>(scales + KB + 32 * n + 8 * g + 4 * h);
-          s[n][4 * g] *= f.x, s[n][4 * g + 1] *= f.y, s[n][4 * g + 2] *= f.z, s[n][4 * g + 3] *= f.w;
-        }
+    for (int i = 0; i < kProducts; ++i) {
+      const int n = i / (2 * T::kOut), t = i / T::kOut % 2, o = i % T::kOut, at = i % (2 * T::kOut);
+      if (n > 0 && at == 0) p[0] = pack_step<DT>(s[n], 0), p[1] = pack_step<DT>(s[n], 1);
+      acc[o] = mfma<DT>(f[i % kAhead], p[t], acc[o]);
+      if (i + kAhead < kProducts) f[i % kAhead] = read_v(i + kAhead);
+      if (n + 1 < NT) {
+        const int each = (8 + 2 * T::kOut - 1) / (2 * T::kOut);
+#pragma unroll
+        for (int u = at * each; u < (at + 1) * each && u < 8; ++u) power(n + 1, 2 * u);
+      }
+      in_order();
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const u32x4 p = pack_step<DT>(s[n], t);
-#pragma unroll
-        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tv, 32 * n, t, o, cols_at), p, acc[o]);
-      }
+    l += sums[0] + sums[1];
   };
 
-  stagger_waves();
-  unsigned char* mine = lds + kw * kBufs * kSlot;
+  unsigned char *mine = lds + kw * kSlot, *other_slot = lds1 + (kBufs == 2 ? kw * kSlot : 0);
   if (iters > 0) fetch(0, mine);
   auto turn = [&](int it, unsigned char* slot, unsigned char* other) {
     const int k0 = key0(it);
@@ -343,9 +366,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   if constexpr (kBufs == 1) {
     for (int it = 0; it < iters; ++it) turn(it, mine, mine);
   } else {
-    for (int it = 0; it < iters; it += 2) {  // (the two slots' addresses are constants)
-      turn(it, mine, mine + kSlot);
-      if (it + 1 < iters) turn(it + 1, mine + kSlot, mine);
+    for (int it = 0; it < iters; it += 2) {
+      turn(it, mine, other_slot);
+      if (it + 1 < iters) turn(it + 1, other_slot, mine);
     }
   }
   l = both_sum(l);
@@ -382,8 +405,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
         if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(o2[u] / l2));
     }
   } else {
-    // every key group's sums to LDS, scaled to the common maximum; then each thread adds up a few channels of a row
-    float2* stats = reinterpret_cast<float2*>(lds + 4 * 32 * (D + 4) * 4);
+    // Every key group's sums to LDS, 64 channels at a time, scaled to the common maximum; then a thread adds up 8 channels of a row.
+    float2* stats = reinterpret_cast<float2*>(lds + kJoinStats);
     float* sums = reinterpret_cast<float*>(lds);
     __syncthreads();
     if (h == 0) stats[wave * 32 + lane] = float2{m, l};
@@ -393,74 +416,82 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
     for (int u = 0; u < KW; ++u) top = fmaxf(top, stats[(u * RW + rw) * 32 + (lane & 31)].x);
     const float f = m == -kInf ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.c);
 #pragma unroll
-    for (int o = 0; o < T::kOut; ++o)
+    for (int c0 = 0; c0 < D; c0 += 64) {
+      if (c0 > 0) __syncthreads();
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * o + 8 * g < D)
-          *reinterpret_cast<float4*>(sums + (wave * 32 + (lane & 31)) * (D + 4) + 32 * o + 8 * g + 4 * h) =
-              float4{acc[o][4 * g] * f, acc[o][4 * g + 1] * f, acc[o][4 * g + 2] * f, acc[o][4 * g + 3] * f};
-    __syncthreads();
-    // wavefront (kw, rw) finishes rows rw * 32 + kw * (32 / KW) ..., D / 8 lanes a row
-    constexpr int kMine = 32 / KW, kLanes = 16;
-#pragma unroll 1
-    for (int first = 0; first < kMine; first += 64 / kLanes) {
-      const int r = kw * kMine + first + lane / kLanes, ch = lane % kLanes;
-      const int row_r = tile * 32 * RW + rw * 32 + r;
-      float top_r = -kInf, l_r = 0.f;
+      for (int o = c0 / 32; o < (c0 + 64) / 32 && o < T::kOut; ++o)
 #pragma unroll
-      for (int u = 0; u < KW; ++u) top_r = fmaxf(top_r, stats[(u * RW + rw) * 32 + r].x);
+        for (int g = 0; g < 4; ++g)
+          if (32 * o + 8 * g < D)
+            *reinterpret_cast<float4*>(sums + (wave * 32 + (lane & 31)) * 68 + 32 * o - c0 + 8 * g + 4 * h) =
+                float4{acc[o][4 * g] * f, acc[o][4 * g + 1] * f, acc[o][4 * g + 2] * f, acc[o][4 * g + 3] * f};
+      __syncthreads();
+      // wavefront (kw, rw) finishes rows rw * 32 + kw * (32 / KW) ..., 8 lanes a row
+      constexpr int kMine = 32 / KW, kLanes = 8;
 #pragma unroll
-      for (int u = 0; u < KW; ++u) {
-        const float2 st = stats[(u * RW + rw) * 32 + r];
-        l_r += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top_r) * a.c);
-      }
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (ch < D / 8)
+      for (int first = 0; first < kMine; first += 64 / kLanes) {
+        const int r = kw * kMine + first + lane / kLanes, ch = c0 / 8 + lane % kLanes;
+        const int row_r = tile * 32 * RW + rw * 32 + r;
+        const bool mine_r = row_r < a.rows && ch < D / 8;
+        float top_r = -kInf, l_r = 0.f;
 #pragma unroll
-        for (int u = 0; u < KW; ++u)
+        for (int u = 0; u < KW; ++u) top_r = fmaxf(top_r, stats[(u * RW + rw) * 32 + r].x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += sums[((u * RW + rw) * 32 + r) * (D + 4) + ch * 8 + e];
-      bool wrong = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) wrong = wrong || v[e] != v[e];
-      int lo_r = 0, hi_r = 0;
-      if (row_r < a.rows) key_range(a.mask, b, a.by_group.div(row_r), a.n_queries, a.n_keys, lo_r, hi_r);
-      const bool some_r = hi_r > lo_r;
-      const int slo = max(lo_r, g_lo), shi = min(hi_r, g_hi);
-      const int i_r = a.by_group.div(row_r);
-      const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i_r) * a.n_q + hk * a.group + row_r - i_r * a.group) * D;
-      const int64_t to_part = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_r;
-      if (row_r < a.rows && ch < D / 8) {
-        if (a.splits > 1) {
-          float4* dst = reinterpret_cast<float4*>(a.part + to_part * D + ch * 8);
-          dst[0] = float4{v[0], v[1], v[2], v[3]};
-          dst[1] = float4{v[4], v[5], v[6], v[7]};
-          if (ch == 0) part_stats(a, D)[to_part] = float2{top_r, l_r};
-        } else {
-          const float inv = some_r ? 1.f / l_r : 0.f;
-          float w[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = some_r ? v[e] * inv : 0.f;
-          *reinterpret_cast<u32x4*>(a.out + to + ch * 8) = pack16<DT>(w);
-          if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(pair) * a.rows + row_r] = some_r ? __builtin_fmaf(top_r, a.c, __builtin_amdgcn_logf(l_r)) : kInf;
+        for (int u = 0; u < KW; ++u) {
+          const float2 st = stats[(u * RW + rw) * 32 + r];
+          l_r += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top_r) * a.c);
         }
-      }
-      uint64_t redo = __ballot(wrong && row_r < a.rows && shi > slo);
-      while (redo != 0) {
-        const int at = __builtin_ctzll(redo) / kLanes * kLanes;
-        redo &= ~(0xffffull << at);
-        const int row_x = __shfl(row_r, at), lo_x = __shfl(slo, at), hi_x = __shfl(shi, at);
-        float m2, l2, o2[2];
-        plain_row<DT, D, F8>(a, b, hk, row_x, lo_x, hi_x, lane, m2, l2, o2);
-        const int64_t px = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_x;
-        uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.n_queries + row_x / a.group) * a.n_q + hk * a.group + row_x % a.group) * D;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (ch < D / 8)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (lane + 64 * u < D) {
-            if (a.splits > 1) a.part[px * D + lane + 64 * u] = o2[u];
-            else dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(o2[u] / l2));
+          for (int u = 0; u < KW; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += sums[((u * RW + rw) * 32 + r) * 68 + (ch * 8 - c0) + e];
+        bool wrong = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wrong = wrong || v[e] != v[e];
+        const int i_r = row_r < a.rows ? a.by_group.div(row_r) : 0;
+        int lo_r = 0, hi_r = 0;
+        if (row_r < a.rows) key_range(a.mask, b, i_r, a.n_queries, a.n_keys, lo_r, hi_r);
+        const bool some_r = hi_r > lo_r;
+        const int slo = max(lo_r, g_lo), shi = min(hi_r, g_hi);
+        const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i_r) * a.n_q + hk * a.group + row_r - i_r * a.group) * D;
+        const int64_t to_part = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_r;
+        if (mine_r) {
+          if (a.splits > 1) {
+            float4* dst = reinterpret_cast<float4*>(a.part + to_part * D + ch * 8);
+            dst[0] = float4{v[0], v[1], v[2], v[3]};
+            dst[1] = float4{v[4], v[5], v[6], v[7]};
+            if (ch == 0) part_stats(a, D)[to_part] = float2{top_r, l_r};
+          } else {
+            const float inv = some_r ? 1.f / l_r : 0.f;
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = some_r ? v[e] * inv : 0.f;
+            *reinterpret_cast<u32x4*>(a.out + to + ch * 8) = pack16<DT>(w);
+            if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(pair) * a.rows + row_r] = some_r ? __builtin_fmaf(top_r, a.c, __builtin_amdgcn_logf(l_r)) : kInf;
           }
-        if (a.splits > 1 && lane == 0) part_stats(a, D)[px] = float2{m2, l2};
+        }
+        uint64_t redo = __ballot(wrong && mine_r && shi > slo);
+        while (redo != 0) {
+          const int at = __builtin_ctzll(redo) / kLanes * kLanes;
+          redo &= ~(0xffull << at);
+          const int row_x = __shfl(row_r, at), lo_x = __shfl(slo, at), hi_x = __shfl(shi, at);
+          const float top_x = __shfl(top_r, at);
+          float m2, l2, o2[2];
+          plain_row<DT, D, F8>(a, b, hk, row_x, lo_x, hi_x, lane, m2, l2, o2);
+          const int c = c0 + lane;
+          if (c < D) {  // the same channels and the same maximum as above
+            if (a.splits > 1) {
+              const float scale = m2 == -kInf ? 1.f : exp2f((m2 - top_x) * a.c);
+              a.part[((static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_x) * D + c] = o2[c0 / 64] * scale;
+            } else {
+              const int i_x = a.by_group.div(row_x);
+              a.out[((static_cast<int64_t>(b) * a.n_queries + i_x) * a.n_q + hk * a.group + row_x - i_x * a.group) * D + c] =
+                  static_cast<uint16_t>(Elem<DT>::store(o2[c0 / 64] / l2));
+            }
+          }
+        }
       }
     }
   }
