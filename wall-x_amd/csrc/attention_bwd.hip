@@ -24,9 +24,10 @@ struct BwdArgs {
   float c, scale;
   uint32_t* info;                 // [pair, row_block] blocks of kInfoWords
   int2* bounds;                   // [pair, row_block] the keys that any row of the block sees
-  int key_tiles, splits;
-  Divider by_splits, by_pairs, by_kv, by_group, by_in_group;  // by_pairs: of an XCD where they are dealt to XCDs, else all
+  int key_tiles, splits, unit;    // a workgroup walks at most `unit` row blocks of a key tile; splits of them cover all
+  Divider by_splits, by_pairs, by_kv, by_group, by_in_group, by_unit, by_tiles;  // by_pairs: of an XCD where they are dealt to XCDs, else all
   float* part;                    // splits > 1: [pair, split, n_keys, 2, D]
+  int32_t* units;                 // splits > 1: [pair, key tile] the splits that wrote theirs
 };
 
 // What the second kernel reads of 32 rows: L, delta, lo and hi of each, then the keys that all rows with keys see.
@@ -236,17 +237,25 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   }
 }
 
-// A wavefront holds 32 keys (K and V as B operands, dK^T and dV^T as accumulators); the workgroup's four share the tiles of 32 rows
-// of Q and dO that pass through LDS.  S has rows in its registers here and a key per column, so that P and dS are the B operands of
-// dV^T = dO^T P and dK^T = Q^T dS as they stand.
+// A wavefront holds 32 keys (K and V as B operands, dK^T and dV^T as accumulators) and takes every second block of 32 rows of Q and dO
+// that see them; two such wavefronts make the 64 keys of a workgroup, and the other two take the blocks in between.  S has rows in its
+// registers here and a key per column, so that P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+//
+// Under a causal mask the first keys are seen by all rows and the last by few: a tile's rows are cut into units of the same
+// length, so that the longest workgroup is a unit and not a tile.  A tile of one unit writes its gradients, the others' units write
+// their sums, which attn_dkv_join_kernel adds up.
+constexpr int kKeyTile = 64;
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   using T = AttnTile<D>;
   constexpr int kTileBytes = 32 * T::kPitch, kInfoBytes = 1024, kSlot = 2 * kTileBytes + kInfoBytes;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kSlot];
+  constexpr int kSums = T::kOut * 16 * 64 * 4;  // one wavefront's sums of one gradient
+  unsigned char* const lds0 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 0>();
+  unsigned char* const lds1 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 1>();
   __shared__ int s_first[4], s_last[4];
-  __shared__ u32x4 s_offsets[256];
+  __shared__ u32x4 s_offsets[2][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int half = wave & 1, rg = wave >> 1;
   const int pairs = a.batch * a.n_kv;
   int pair, tile, split;
   {
@@ -264,9 +273,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     }
   }
   const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
-  const int k0 = tile * 128, key = k0 + wave * 32 + (lane & 31);
+  const int k0 = tile * kKeyTile, wk = k0 + half * 32, key = wk + (lane & 31);
   const bool live = key < a.n_keys;
-  const int wk = k0 + wave * 32;  // this wavefront's first key
 
   // the row blocks that see any of the workgroup's keys: from the first to the last that does
   int first = 0x7fffffff, last = -1;
@@ -274,7 +282,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     const int2* bounds = a.bounds + static_cast<int64_t>(pair) * a.row_blocks;
     for (int t = tid; t < a.row_blocks; t += 256) {
       const int2 x = bounds[t];
-      if (x.x < k0 + 128 && x.y > k0 && x.y > x.x) {
+      if (x.x < k0 + kKeyTile && x.y > k0 && x.y > x.x) {
         first = min(first, t);
         last = t;
       }
@@ -285,55 +293,63 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     __syncthreads();
     first = min(min(s_first[0], s_first[1]), min(s_first[2], s_first[3]));
     last = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
-    const int n = last < first ? 0 : last - first + 1;
-    const int each = a.by_splits.div(n), more = n - each * a.splits;  // the first `more` splits take one more
-    const int t0 = split * each + min(split, more);
-    last = __builtin_amdgcn_readfirstlane(first + t0 + each + (split < more ? 1 : 0));
-    first = __builtin_amdgcn_readfirstlane(first + t0);  // blocks [first, last)
-    if (n == 0) first = last = 0;
   }
+  const int blocks = last < first ? 0 : __builtin_amdgcn_readfirstlane(last - first + 1);
+  const int units = a.by_unit.div(blocks + a.unit - 1);  // (of a tile that nothing sees: none, and its first split writes zeros)
+  if (a.splits > 1 && split == 0 && tid == 0) a.units[static_cast<int64_t>(pair) * a.key_tiles + tile] = units;
+  if (split > 0 && split >= units) return;
+  first = blocks == 0 ? 0 : __builtin_amdgcn_readfirstlane(first + split * a.unit);
+  last = blocks == 0 ? 0 : first + min(a.unit, blocks - split * a.unit);  // blocks [first, last)
+  const bool whole = units <= 1;
 
   const uint16_t* qb = a.q + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[1];
   const uint16_t* gb = a.g + b * a.gs[0] + static_cast<int64_t>(hk) * a.group * a.gs[1];
-  const char* src = reinterpret_cast<const char*>(wave < 2 ? qb : gb);
-  const int64_t pos_step = (wave < 2 ? a.qs[2] : a.gs[2]) * 2;
-  const int head_step = static_cast<int>((wave < 2 ? a.qs[1] : a.gs[1]) * 2), pos_step32 = static_cast<int>(pos_step);
+  const char* src = reinterpret_cast<const char*>(half == 0 ? qb : gb);  // this wavefront loads its group's queries, or their gradients
+  const int64_t pos_step = (half == 0 ? a.qs[2] : a.gs[2]) * 2;
+  const int head_step = static_cast<int>((half == 0 ? a.qs[1] : a.gs[1]) * 2), pos_step32 = static_cast<int>(pos_step);
   const uint32_t* info_base = a.info + static_cast<int64_t>(pair) * a.row_blocks * kInfoWords;
   // Offsets of a block's rows from its first: the same for every block where the group divides 32 or 32 the group.  They are kept in
   // LDS, for want of registers.
   const bool regular = 32 % a.group == 0 || a.group % 32 == 0;
-  {
-    const int in_group = a.group < 32 ? a.group : 32, r0 = (wave & 1) * 16;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
     uint32_t off[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < T::kChunks / 4; ++i)
       off[i] = stage_offset<D>(i, lane, [&](int r) {
-        const int di = a.by_in_group.div(r0 + r), hd = (r0 + r) - di * in_group;
+        const int di = a.by_in_group.div(16 * u + r), hd = (16 * u + r) - di * (a.group < 32 ? a.group : 32);
         return static_cast<uint32_t>(di * pos_step32 + hd * head_step);
       });
-    s_offsets[tid] = u32x4{off[0], off[1], off[2], off[3]};
+    s_offsets[u][tid] = u32x4{off[0], off[1], off[2], off[3]};
   }
   auto fetch = [&](int t, unsigned char* slot) {
-    const int row0 = t * 32, i0 = a.by_group.div(row0), rem = row0 - i0 * a.group, r0 = (wave & 1) * 16;
+    const int row0 = t * 32, i0 = a.by_group.div(row0), rem = row0 - i0 * a.group;
     const char* base = src + __builtin_amdgcn_readfirstlane(i0) * pos_step;
-    unsigned char* to = slot + (wave >> 1) * kTileBytes + r0 * T::kPitch;
+    unsigned char* to = slot + half * kTileBytes;
     if (regular && row0 + 32 <= a.rows) {
-      const u32x4 o = s_offsets[tid];
-      const uint32_t off[4] = {o[0], o[1], o[2], o[3]};
-      stage16<D>(attn_rsrc(base + __builtin_amdgcn_readfirstlane(rem) * static_cast<int64_t>(head_step), kRsrcBytes), to, off);
+      const auto r = attn_rsrc(base + __builtin_amdgcn_readfirstlane(rem) * static_cast<int64_t>(head_step), kRsrcBytes);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x4 o = s_offsets[u][tid];
+        const uint32_t off[4] = {o[0], o[1], o[2], o[3]};
+        stage16<D>(r, to + u * 16 * T::kPitch, off);
+      }
     } else {
       int here = lane;
       asm volatile("" : "+v"(here));  // (what this path needs is made here, not kept over the loop)
-      stage16<D>(attn_rsrc(base, kRsrcBytes), to, here, [&](int r) {
-        const uint32_t x = static_cast<uint32_t>(rem + r0 + r), di = static_cast<uint32_t>(a.by_group.div(static_cast<int>(x))), hd = x - di * a.group;
-        return row0 + r0 + r < a.rows ? di * static_cast<uint32_t>(pos_step32) + hd * static_cast<uint32_t>(head_step) : kOutside;
-      });
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        stage16<D>(attn_rsrc(base, kRsrcBytes), to + u * 16 * T::kPitch, here, [&](int r) {
+          const uint32_t x = static_cast<uint32_t>(rem + 16 * u + r), di = static_cast<uint32_t>(a.by_group.div(static_cast<int>(x))), hd = x - di * a.group;
+          return row0 + 16 * u + r < a.rows ? di * static_cast<uint32_t>(pos_step32) + hd * static_cast<uint32_t>(head_step) : kOutside;
+        });
     }
-    if (wave == 0)
+    if (half == 1)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(attn_rsrc(info_base + static_cast<int64_t>(t) * kInfoWords, kInfoWords * 4), WX_LDS(slot + 2 * kTileBytes), 16,
                                                lane * 16, 0, 0, 0);
   };
-  if (first < last) fetch(first, lds);
+  unsigned char *mine = lds0 + rg * kSlot, *other = lds1 + rg * kSlot;
+  if (first + rg < last) fetch(first + rg, mine);
 
   u32x4 kf[T::kSteps], vf[T::kSteps];
   {
@@ -352,11 +368,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     for (int r = 0; r < 16; ++r) dk[o][r] = dv[o][r] = 0.f;
 
   const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
-  for (int t = first; t < last; ++t) {
+  auto turn = [&](int t, unsigned char* tq, unsigned char* next) {
     wait_loads();
     attn_barrier();
-    if (t + 1 < last) fetch(t + 1, lds + ((t + 1 - first) & 1) * kSlot);
-    const unsigned char *tq = lds + ((t - first) & 1) * kSlot, *tg = tq + kTileBytes;
+    if (t + 2 < last) fetch(t + 2, next);
+    if (t >= last) return;
+    const unsigned char* tg = tq + kTileBytes;
     const float* info = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
     const int2 full = *reinterpret_cast<const int2*>(info + 128);
     const int f_lo = __builtin_amdgcn_readfirstlane(full.x), f_hi = __builtin_amdgcn_readfirstlane(full.y);
@@ -404,29 +421,45 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         dk[o] = mfma<DT>(read_cols<D>(tq, 0, u, o, cols_at), ds, dk[o]);
       }
     }
+  };
+  for (int t = first; t < last; t += 4) {
+    turn(t + rg, mine, other);
+    if (t + 2 < last) turn(t + 2 + rg, other, mine);
   }
 
+  // The two row groups' sums: the first gets the others' dK and finishes it, the second dV.
+  __syncthreads();
+  {
+    float* give = reinterpret_cast<float*>(rg == 0 ? lds1 : lds0) + half * (kSums / 4) + lane;
+    const float* take = reinterpret_cast<const float*>(rg == 0 ? lds0 : lds1) + half * (kSums / 4) + lane;
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) give[(16 * o + r) * 64] = rg == 0 ? dv[o][r] : dk[o][r];
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[o][r] = (rg == 0 ? dk[o][r] : dv[o][r]) + take[(16 * o + r) * 64];  // (from here on: what this group finishes)
+  }
   bool bad = false;
 #pragma unroll
   for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      if (32 * o + 8 * (r / 4) < D) bad = bad || dk[o][r] != dk[o][r] || dv[o][r] != dv[o][r];
-  const int64_t to = ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D;
-  const int64_t part = ((static_cast<int64_t>(pair) * a.splits + split) * a.n_keys) * 2 * D;
-  if (a.splits == 1) {
-    store_row<DT, D>(dk, a.scale, live ? a.dk + to : nullptr, lane);
-    store_row<DT, D>(dv, 1.f, live ? a.dv + to : nullptr, lane);
+      if (32 * o + 8 * (r / 4) < D) bad = bad || dk[o][r] != dk[o][r];
+  const float scale = rg == 0 ? a.scale : 1.f;
+  uint16_t* const grad = rg == 0 ? a.dk : a.dv;
+  const int64_t part = (static_cast<int64_t>(pair) * a.splits + split) * a.n_keys * 2 * D + rg * D;
+  if (whole) {
+    store_row<DT, D>(dk, scale, live ? grad + ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D : nullptr, lane);
   } else if (live) {
     float* dst = a.part + part + static_cast<int64_t>(key) * 2 * D;
 #pragma unroll
     for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        if (32 * o + 8 * g < D) {
-          *reinterpret_cast<float4*>(dst + 32 * o + 8 * g + 4 * h) = float4{dk[o][4 * g], dk[o][4 * g + 1], dk[o][4 * g + 2], dk[o][4 * g + 3]};
-          *reinterpret_cast<float4*>(dst + D + 32 * o + 8 * g + 4 * h) = float4{dv[o][4 * g], dv[o][4 * g + 1], dv[o][4 * g + 2], dv[o][4 * g + 3]};
-        }
+        if (32 * o + 8 * g < D) *reinterpret_cast<float4*>(dst + 32 * o + 8 * g + 4 * h) = float4{dk[o][4 * g], dk[o][4 * g + 1], dk[o][4 * g + 2], dk[o][4 * g + 3]};
   }
   // Keys whose sums are not numbers, in plain loops over the rows that see them.
   uint64_t redo = __ballot(bad && live);
@@ -436,10 +469,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     redo &= redo - 1;
     const int key_r = wk + r;
     const uint16_t *kr = row_of(a.k, a.ks, b, hk, key_r), *vr = row_of(a.v, a.vs, b, hk, key_r);
-    float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
+    float sum[2] = {0.f, 0.f};
     for (int t = first * 32; t < min(last * 32, a.rows); t += 64) {
       const int row = t + lane;
-      float p = 0.f, ds = 0.f;
+      float x = 0.f;  // the row's P, or its dS
       bool see = false;
       if (row < a.rows && row < last * 32) {
         const uint32_t* info = info_base + static_cast<int64_t>(row / 32) * kInfoWords + row % 32;
@@ -452,72 +485,67 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
             s = __builtin_fmaf(Elem<DT>::load(q[e]), Elem<DT>::load(kr[e]), s);
             d = __builtin_fmaf(Elem<DT>::load(g[e]), Elem<DT>::load(vr[e]), d);
           }
-          p = exp2f(s * a.c - __uint_as_float(info[0]));
-          ds = p * (d - __uint_as_float(info[32]));
+          x = exp2f(s * a.c - __uint_as_float(info[0]));
+          if (rg == 0) x *= d - __uint_as_float(info[32]);
         }
       }
       uint64_t seen = __ballot(see);
       while (seen != 0) {
         const int j = __builtin_ctzll(seen);
         seen &= seen - 1;
-        const float pj = __shfl(p, j), dj = __shfl(ds, j);
+        const float xj = __shfl(x, j);
         const int hq = hk * a.group + (t + j) % a.group;
-        const uint16_t *q = row_of(a.q, a.qs, b, hq, (t + j) / a.group), *g = row_of(a.g, a.gs, b, hq, (t + j) / a.group);
+        const uint16_t* w = rg == 0 ? row_of(a.q, a.qs, b, hq, (t + j) / a.group) : row_of(a.g, a.gs, b, hq, (t + j) / a.group);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (lane + 64 * u < D) {
-            sk[u] = __builtin_fmaf(dj, Elem<DT>::load(q[lane + 64 * u]), sk[u]);
-            sv[u] = __builtin_fmaf(pj, Elem<DT>::load(g[lane + 64 * u]), sv[u]);
-          }
+          if (lane + 64 * u < D) sum[u] = __builtin_fmaf(xj, Elem<DT>::load(w[lane + 64 * u]), sum[u]);
       }
     }
-    const int64_t to_r = ((static_cast<int64_t>(b) * a.n_keys + key_r) * a.n_kv + hk) * D;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       if (lane + 64 * u < D) {
-        if (a.splits == 1) {
-          a.dk[to_r + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sk[u] * a.scale));
-          a.dv[to_r + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sv[u]));
-        } else {
-          float* dst = a.part + part + static_cast<int64_t>(key_r) * 2 * D + lane + 64 * u;
-          dst[0] = sk[u];
-          dst[D] = sv[u];
-        }
+        if (whole) grad[((static_cast<int64_t>(b) * a.n_keys + key_r) * a.n_kv + hk) * D + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sum[u] * scale));
+        else a.part[part + static_cast<int64_t>(key_r) * 2 * D + lane + 64 * u] = sum[u];
       }
   }
 }
 
-// dK and dV of a key from the splits' sums: a thread per 4 channels.
+// dK and dV of the keys of a tile of several units, from the units' sums: a workgroup per tile, a thread per 4 channels.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
-  const int64_t n = static_cast<int64_t>(a.batch) * a.n_kv * a.n_keys * (2 * D / 4), id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (id >= n) return;
-  const int64_t at = id / (2 * D / 4);
-  const int e = static_cast<int>(id - at * (2 * D / 4)) * 4;
-  const int pair = static_cast<int>(at / a.n_keys), key = static_cast<int>(at - static_cast<int64_t>(pair) * a.n_keys);
-  const float* src = a.part + (static_cast<int64_t>(pair) * a.splits * a.n_keys + key) * 2 * D + e;
-  float4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < a.splits; ++i) {
-    const float4 x = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(i) * a.n_keys * 2 * D);
-    s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+  const int pair = a.by_tiles.div(blockIdx.x), tile = blockIdx.x - pair * a.key_tiles;
+  const int units = a.units[static_cast<int64_t>(pair) * a.key_tiles + tile];
+  if (units <= 1) return;
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
+  const int64_t step = static_cast<int64_t>(a.n_keys) * 2 * D;
+  for (int i = threadIdx.x; i < kKeyTile * (2 * D / 4); i += 256) {
+    const int key = tile * kKeyTile + i / (2 * D / 4), e = i % (2 * D / 4) * 4;
+    if (key >= a.n_keys) break;
+    const float* src = a.part + static_cast<int64_t>(pair) * a.splits * step + static_cast<int64_t>(key) * 2 * D + e;
+    float4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int u = 0; u < units; ++u) {
+      const float4 x = *reinterpret_cast<const float4*>(src + u * step);
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
+    const float f = e < D ? a.scale : 1.f;
+    uint16_t* dst = (e < D ? a.dk + e : a.dv + e - D) + ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D;
+    *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<DT>(s.x * f, s.y * f), pack2<DT>(s.z * f, s.w * f)};
   }
-  const float f = e < D ? a.scale : 1.f;
-  const int b = pair / a.n_kv, hk = pair % a.n_kv;
-  uint16_t* dst = (e < D ? a.dk + e : a.dv + e - D) + ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D;
-  *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<DT>(s.x * f, s.y * f), pack2<DT>(s.z * f, s.w * f)};
 }
 
-// Splits of the rows that a tile of keys walks, where the tiles alone leave CUs idle.
+// Units that the rows of a key tile are cut into: about four workgroups to each place on the chip (two to a CU), where the tiles alone
+// are fewer, of at least 16 blocks each.
 int bwd_splits(int64_t pairs, int64_t n_keys, int64_t row_blocks) {
-  const int64_t tiles = pairs * ((n_keys + 127) / 128), cus = device_cu_count();
-  if (tiles == 0 || tiles >= 2 * cus) return 1;
-  const int64_t want = (2 * cus + tiles - 1) / tiles, most = row_blocks / 8;  // (at least 8 blocks of rows each)
+  const int64_t tiles = pairs * ((n_keys + kKeyTile - 1) / kKeyTile), places = 2 * device_cu_count();
+  if (tiles == 0 || tiles >= 4 * places) return 1;
+  const int64_t want = (4 * places + tiles - 1) / tiles, most = row_blocks / 16;
   const int64_t n = want < most ? want : most;
   return static_cast<int>(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
 
 struct Workspace {
-  size_t info, bounds, part, total;
+  size_t info, bounds, units, part, total;
 };
 Workspace layout(int64_t pairs, int64_t rows, int64_t n_keys, int head_dim) {
   const int64_t blocks = (rows + 31) / 32;
@@ -526,7 +554,8 @@ Workspace layout(int64_t pairs, int64_t rows, int64_t n_keys, int head_dim) {
   Workspace w{};
   w.info = 0;
   w.bounds = up(static_cast<size_t>(pairs) * blocks * kInfoWords * 4);
-  w.part = w.bounds + up(static_cast<size_t>(pairs) * blocks * sizeof(int2));
+  w.units = w.bounds + up(static_cast<size_t>(pairs) * blocks * sizeof(int2));
+  w.part = w.units + up(static_cast<size_t>(pairs) * ((n_keys + kKeyTile - 1) / kKeyTile) * sizeof(int32_t));
   w.total = w.part + (splits > 1 ? static_cast<size_t>(pairs) * splits * n_keys * 2 * head_dim * sizeof(float) : 0);
   return w;
 }
@@ -535,11 +564,11 @@ template <int DT, int D>
 int launch_bwd(BwdArgs& a, hipStream_t s) {
   const int64_t pairs = static_cast<int64_t>(a.batch) * a.n_kv;
   const int64_t row_tiles = pairs * ((a.row_blocks + 3) / 4), key_tiles = pairs * a.key_tiles * a.splits;
-  const int64_t join = a.splits > 1 ? (pairs * a.n_keys * (2 * D / 4) + 255) / 256 : 0;
+  const int64_t join = a.splits > 1 ? pairs * a.key_tiles : 0;
   if (row_tiles > 0x7fffffffll || key_tiles > 0x7fffffffll || join > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows");
   const int all = static_cast<int>(pairs);
   a.by_splits = Divider(a.splits), a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_in_group = Divider(a.group < 32 ? a.group : 32);
-  a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all);
+  a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all), a.by_unit = Divider(a.unit), a.by_tiles = Divider(a.key_tiles > 0 ? a.key_tiles : 1);
   const dim3 block(256);
   if (row_tiles > 0) {
     hipLaunchKernelGGL((attn_dq_kernel<DT, D>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
@@ -599,12 +628,13 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   a.group = group, a.rows = static_cast<int>(n_queries) * group, a.row_blocks = (a.rows + 31) / 32;
   a.c = scale * kLog2e, a.scale = scale;
   const int64_t pairs = batch * n_kv_heads;
-  a.key_tiles = (a.n_keys + 127) / 128;
+  a.key_tiles = (a.n_keys + kKeyTile - 1) / kKeyTile;
   a.splits = bwd_splits(pairs, n_keys, a.row_blocks);
+  a.unit = a.row_blocks > 0 ? (a.row_blocks + a.splits - 1) / a.splits : 1;
   const Workspace w = layout(pairs, a.rows, n_keys, head_dim);
   if (w.total > 0 && (!workspace || workspace_bytes < w.total)) return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_bwd_workspace_bytes)", who);
   char* ws = static_cast<char*>(workspace);
-  a.info = reinterpret_cast<uint32_t*>(ws + w.info), a.bounds = reinterpret_cast<int2*>(ws + w.bounds), a.part = reinterpret_cast<float*>(ws + w.part);
+  a.info = reinterpret_cast<uint32_t*>(ws + w.info), a.bounds = reinterpret_cast<int2*>(ws + w.bounds), a.units = reinterpret_cast<int32_t*>(ws + w.units), a.part = reinterpret_cast<float*>(ws + w.part);
   hipStream_t s = as_stream(stream);
   if (dtype == WX_BF16) {
     if (head_dim == 64) return launch_bwd<WX_BF16, 64>(a, s);
