@@ -215,10 +215,10 @@ __device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned ch
 }
 // The same from offsets that were made before (all rows inside).
 template <int D>
-__device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, const uint32_t* offsets) {
+__device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, const uint32_t* offsets, int further = 0) {
 #pragma unroll
   for (int i = 0; i < AttnTile<D>::kChunks / 4; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(offsets[i]), 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, WX_LDS(lds + i * 1024), 16, static_cast<int>(offsets[i]), further, 0, 0);
 }
 
 // One LDS array per (size, index).  A kernel's two slots for tiles are arrays of their own, at constant addresses in a loop unrolled

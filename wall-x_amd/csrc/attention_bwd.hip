@@ -41,7 +41,7 @@ template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   using T = AttnTile<D>;
   constexpr int KB = 64, kTileBytes = KB * T::kPitch;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * kTileBytes];
+  unsigned char *const lds0 = lds_slot<2 * kTileBytes, 0>(), *const lds1 = lds_slot<2 * kTileBytes, 1>();
   __shared__ int2 s_bounds[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int pairs = a.batch * a.n_kv, row_tiles = (a.row_blocks + 3) / 4;
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       stage16<D>(rv, slot + kTileBytes + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * static_cast<int>(v_step)) : kOutside; });
     }
   };
-  if (iters > 0) fetch(0, lds);
+  if (iters > 0) fetch(0, lds0);
 
   float delta = 0.f;
 #pragma unroll
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
-  const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
+  const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
   auto turn = [&](int it, unsigned char* tk, unsigned char* other) {
     wait_loads();
     attn_barrier();
@@ -157,32 +157,56 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
     for (int n = 0; n < KB / 32; ++n) {
       const int k0 = g_lo + it * KB + 32 * n;
       if (k0 >= w_hi || k0 + 32 <= w_lo) continue;
+      // A product's operand is asked for kAhead products before it; the second half's powers are found under the first half's products.
+      constexpr int kAhead = D == 80 ? 2 : 3, kScores = 2 * T::kSteps, kProducts = 2 * T::kOut;
+      int rows_at = rows_first, cols_at = cols_first;
+      asm volatile("" : "+v"(rows_at), "+v"(cols_at));
+      auto read_s = [&](int i) { return read_rows<D>(i % 2 == 0 ? tk : tv, 32 * n, i / 2, rows_at); };
+      auto read_k = [&](int i) { return read_cols<D>(tk, 32 * n, i / T::kOut, i % T::kOut, cols_at); };
       f32x16 s, dp;
+      u32x4 f[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) f[i] = read_s(i);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+      in_order();
 #pragma unroll
-      for (int t = 0; t < T::kSteps; ++t) {
-        s = mfma<DT>(read_rows<D>(tk, 32 * n, t, rows_at), qf[t], s);
-        dp = mfma<DT>(read_rows<D>(tv, 32 * n, t, rows_at), gf[t], dp);
+      for (int i = 0; i < kScores; ++i) {
+        if (i % 2 == 0) s = mfma<DT>(f[i % kAhead], qf[i / 2], s);
+        else dp = mfma<DT>(f[i % kAhead], gf[i / 2], dp);
+        if (i + kAhead < kScores) f[i % kAhead] = read_s(i + kAhead);
+        in_order();
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+      for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
+      in_order();
       if (k0 < f_lo || k0 + 32 > f_hi) {
         const uint32_t span = static_cast<uint32_t>(hi - lo);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = static_cast<uint32_t>(k0 + 4 * h + 8 * (r / 4) + r % 4 - lo) < span ? s[r] : 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = static_cast<uint32_t>(k0 + 4 * h + 8 * (r / 4) + r % 4 - lo) < span ? s[r] : -kInf;
       }
+      auto slope = [&](int r) { s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta); };
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const u32x4 ds = pack_step<DT>(s, t);
+      for (int r = 0; r < 8; ++r) slope(r);
+      u32x4 ds = pack_step<DT>(s, 0);
+      in_order();
 #pragma unroll
-        for (int o = 0; o < T::kOut; ++o) acc[o] = mfma<DT>(read_cols<D>(tk, 32 * n, t, o, cols_at), ds, acc[o]);
+      for (int i = 0; i < kProducts; ++i) {
+        if (i == T::kOut) ds = pack_step<DT>(s, 1);
+        acc[i % T::kOut] = mfma<DT>(f[i % kAhead], ds, acc[i % T::kOut]);
+        if (i + kAhead < kProducts) f[i % kAhead] = read_k(i + kAhead);
+        if (i < T::kOut) {
+          constexpr int each = (8 + T::kOut - 1) / T::kOut;
+#pragma unroll
+          for (int r = 8 + i * each; r < 8 + (i + 1) * each && r < 16; ++r) slope(r);
+        }
+        in_order();
       }
     }
   };
-  for (int it = 0; it < iters; it += 2) {  // (the two slots' addresses are constants)
-    turn(it, lds, lds + 2 * kTileBytes);
-    if (it + 1 < iters) turn(it + 1, lds + 2 * kTileBytes, lds);
+  for (int it = 0; it < iters; it += 2) {
+    turn(it, lds0, lds1);
+    if (it + 1 < iters) turn(it + 1, lds1, lds0);
   }
 
   bool bad = false;
@@ -248,29 +272,28 @@ constexpr int kKeyTile = 64;
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   using T = AttnTile<D>;
-  constexpr int kTileBytes = 32 * T::kPitch, kInfoBytes = 1024, kSlot = 2 * kTileBytes + kInfoBytes;
+  constexpr int kTileBytes = 32 * T::kPitch, kInfoBytes = (kInfoWords * 4 + 63) / 64 * 64, kSlot = 2 * kTileBytes + kInfoBytes;
   constexpr int kSums = T::kOut * 16 * 64 * 4;  // one wavefront's sums of one gradient
   unsigned char* const lds0 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 0>();
   unsigned char* const lds1 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 1>();
   __shared__ int s_first[4], s_last[4];
-  __shared__ u32x4 s_offsets[2][256];
+  __shared__ u32x4 s_offsets[256];
+  // (D = 128: two of V's operands stand in LDS, read in front of their products; with all in registers one was spilled, and the wait
+  // for its memory was a wait for the next block's as well)
+  constexpr int kHeld = D == 128 ? T::kSteps - 2 : T::kSteps;
+  __shared__ u32x4 s_v[kHeld < T::kSteps ? T::kSteps - kHeld : 1][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int half = wave & 1, rg = wave >> 1;
   const int pairs = a.batch * a.n_kv;
+  // (the pair varies fastest: dealt to the XCDs by their split, a tile's first units, which are always there, all went to a few)
   int pair, tile, split;
   {
-    int id = blockIdx.x;
-    const int rest = a.by_splits.div(id);
-    split = id - rest * a.splits;
-    id = rest;
-    if (pairs % 8 == 0) {
-      const int j = id >> 3;
-      tile = a.by_pairs.div(j);
-      pair = (id & 7) + 8 * (j - tile * (pairs >> 3));
-    } else {
-      tile = a.by_pairs.div(id);
-      pair = id - tile * pairs;
-    }
+    const int id = blockIdx.x, from = pairs % 8 == 0 ? id >> 3 : id, per = pairs % 8 == 0 ? pairs >> 3 : pairs;
+    const int rest = a.by_pairs.div(from);
+    pair = pairs % 8 == 0 ? (id & 7) + 8 * (from - rest * per) : from - rest * per;
+    tile = a.by_splits.div(rest);
+    split = rest - tile * a.splits + tile;  // (and turned from tile to tile, for few pairs)
+    split -= a.by_splits.div(split) * a.splits;
   }
   const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
   const int k0 = tile * kKeyTile, wk = k0 + half * 32, key = wk + (lane & 31);
@@ -311,16 +334,17 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   // Offsets of a block's rows from its first: the same for every block where the group divides 32 or 32 the group.  They are kept in
   // LDS, for want of registers.
   const bool regular = 32 % a.group == 0 || a.group % 32 == 0;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  const int in_group = a.group < 32 ? a.group : 32;
+  const int second = in_group == 32 ? 16 * head_step : a.by_in_group.div(16) * pos_step32;  // from the first 16 rows to the others
+  {
     uint32_t off[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < T::kChunks / 4; ++i)
       off[i] = stage_offset<D>(i, lane, [&](int r) {
-        const int di = a.by_in_group.div(16 * u + r), hd = (16 * u + r) - di * (a.group < 32 ? a.group : 32);
+        const int di = a.by_in_group.div(r), hd = r - di * in_group;
         return static_cast<uint32_t>(di * pos_step32 + hd * head_step);
       });
-    s_offsets[u][tid] = u32x4{off[0], off[1], off[2], off[3]};
+    s_offsets[tid] = u32x4{off[0], off[1], off[2], off[3]};
   }
   auto fetch = [&](int t, unsigned char* slot) {
     const int row0 = t * 32, i0 = a.by_group.div(row0), rem = row0 - i0 * a.group;
@@ -328,12 +352,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     unsigned char* to = slot + half * kTileBytes;
     if (regular && row0 + 32 <= a.rows) {
       const auto r = attn_rsrc(base + __builtin_amdgcn_readfirstlane(rem) * static_cast<int64_t>(head_step), kRsrcBytes);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const u32x4 o = s_offsets[u][tid];
-        const uint32_t off[4] = {o[0], o[1], o[2], o[3]};
-        stage16<D>(r, to + u * 16 * T::kPitch, off);
-      }
+      const u32x4 o = s_offsets[tid];
+      const uint32_t off[4] = {o[0], o[1], o[2], o[3]};
+      stage16<D>(r, to, off);
+      stage16<D>(r, to + 16 * T::kPitch, off, second);
     } else {
       int here = lane;
       asm volatile("" : "+v"(here));  // (what this path needs is made here, not kept over the loop)
@@ -344,21 +366,23 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
           return row0 + 16 * u + r < a.rows ? di * static_cast<uint32_t>(pos_step32) + hd * static_cast<uint32_t>(head_step) : kOutside;
         });
     }
-    if (half == 1)
+    if (half == 1 && lane < kInfoWords / 4)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(attn_rsrc(info_base + static_cast<int64_t>(t) * kInfoWords, kInfoWords * 4), WX_LDS(slot + 2 * kTileBytes), 16,
                                                lane * 16, 0, 0, 0);
   };
   unsigned char *mine = lds0 + rg * kSlot, *other = lds1 + rg * kSlot;
   if (first + rg < last) fetch(first + rg, mine);
 
-  u32x4 kf[T::kSteps], vf[T::kSteps];
+  u32x4 kf[T::kSteps], vf[kHeld];
   {
     const uint16_t* k = row_of(a.k, a.ks, b, hk, live ? key : 0);
     const uint16_t* v = row_of(a.v, a.vs, b, hk, live ? key : 0);
 #pragma unroll
     for (int t = 0; t < T::kSteps; ++t) {
       kf[t] = live ? *reinterpret_cast<const u32x4*>(k + 16 * t + 8 * h) : u32x4{0u, 0u, 0u, 0u};
-      vf[t] = live ? *reinterpret_cast<const u32x4*>(v + 16 * t + 8 * h) : u32x4{0u, 0u, 0u, 0u};
+      const u32x4 x = live ? *reinterpret_cast<const u32x4*>(v + 16 * t + 8 * h) : u32x4{0u, 0u, 0u, 0u};
+      if (t < kHeld) vf[t] = x;
+      else s_v[t - kHeld][tid] = x;
     }
   }
   f32x16 dk[T::kOut], dv[T::kOut];
@@ -380,16 +404,38 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     // (an exclusive-or per read in place of an address register for each: the accumulators leave none)
     int rows_at = rows_first, cols_at = cols_first;
     asm volatile("" : "+v"(rows_at), "+v"(cols_at));
+    // A product's operand is asked for kAhead products before it; the second half's powers are found under the first half's products.
+    constexpr int kAhead = 2, kScores = 2 * T::kSteps, kProducts = 4 * T::kOut;
+    auto read_s = [&](int i) { return read_rows<D>(i % 2 == 0 ? tq : tg, 0, i / 2, rows_at); };
+    auto read_g = [&](int i) { return read_cols<D>(i % 2 == 0 ? tg : tq, 0, i / (2 * T::kOut), i / 2 % T::kOut, cols_at); };
     f32x16 s, dp;
+    u32x4 f[kAhead], w = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = read_s(i);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+    in_order();
 #pragma unroll
-    for (int u = 0; u < T::kSteps; ++u) {
-      s = mfma<DT>(read_rows<D>(tq, 0, u, rows_at), kf[u], s);
-      dp = mfma<DT>(read_rows<D>(tg, 0, u, rows_at), vf[u], dp);
+    for (int i = 0; i < kScores; ++i) {
+      if (i % 2 == 0) s = mfma<DT>(f[i % kAhead], kf[i / 2], s);
+      else dp = mfma<DT>(f[i % kAhead], i / 2 < kHeld ? vf[i / 2 < kHeld ? i / 2 : 0] : w, dp);
+      if (i + kAhead < kScores) f[i % kAhead] = read_s(i + kAhead);
+      if (i % 2 == 1 && i / 2 + 1 >= kHeld && i / 2 + 1 < T::kSteps) w = s_v[i / 2 + 1 - kHeld][tid];
+      in_order();
     }
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int i = 0; i < kAhead; ++i) f[i] = read_g(i);
+    in_order();
+    if (wk < f_lo || wk + 32 > f_hi) {  // some row does not see all of the keys
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int4 lo = *reinterpret_cast<const int4*>(info + 64 + 8 * g + 4 * h), hi = *reinterpret_cast<const int4*>(info + 96 + 8 * g + 4 * h);
+        const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g + i] = ((key >= l4[i]) & (key < h4[i])) ? s[4 * g + i] : -kInf;
+      }
+    }
+    auto slope = [&](int g) {  // P and dS of registers 4 g .. + 3
       const float4 lse = *reinterpret_cast<const float4*>(info + 8 * g + 4 * h), delta = *reinterpret_cast<const float4*>(info + 32 + 8 * g + 4 * h);
       const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {delta.x, delta.y, delta.z, delta.w};
 #pragma unroll
@@ -398,28 +444,21 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -ls[i]));
         dp[r] = s[r] * (dp[r] - de[i]);
       }
-    }
-    if (wk < f_lo || wk + 32 > f_hi) {
+    };
+    slope(0);
+    slope(1);
+    u32x4 p = pack_step<DT>(s, 0), ds = pack_step<DT>(dp, 0);
+    in_order();
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int4 lo = *reinterpret_cast<const int4*>(info + 64 + 8 * g + 4 * h), hi = *reinterpret_cast<const int4*>(info + 96 + 8 * g + 4 * h);
-        const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool see = (key >= l4[i]) & (key < h4[i]);
-          s[4 * g + i] = see ? s[4 * g + i] : 0.f;
-          dp[4 * g + i] = see ? dp[4 * g + i] : 0.f;
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const u32x4 p = pack_step<DT>(s, u), ds = pack_step<DT>(dp, u);
-#pragma unroll
-      for (int o = 0; o < T::kOut; ++o) {
-        dv[o] = mfma<DT>(read_cols<D>(tg, 0, u, o, cols_at), p, dv[o]);
-        dk[o] = mfma<DT>(read_cols<D>(tq, 0, u, o, cols_at), ds, dk[o]);
-      }
+    for (int i = 0; i < kProducts; ++i) {
+      const int o = i / 2 % T::kOut;
+      if (i == 2 * T::kOut) p = pack_step<DT>(s, 1), ds = pack_step<DT>(dp, 1);
+      if (i % 2 == 0) dv[o] = mfma<DT>(f[i % kAhead], p, dv[o]);
+      else dk[o] = mfma<DT>(f[i % kAhead], ds, dk[o]);
+      if (i + kAhead < kProducts) f[i % kAhead] = read_g(i + kAhead);
+      if (i == 0) slope(2);
+      if (i == T::kOut) slope(3);
+      in_order();
     }
   };
   for (int t = first; t < last; t += 4) {
@@ -534,12 +573,12 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
   }
 }
 
-// Units that the rows of a key tile are cut into: about four workgroups to each place on the chip (two to a CU), where the tiles alone
+// Units that the rows of a key tile are cut into: about three workgroups to each place on the chip (two to a CU), where the tiles alone
 // are fewer, of at least 16 blocks each.
 int bwd_splits(int64_t pairs, int64_t n_keys, int64_t row_blocks) {
   const int64_t tiles = pairs * ((n_keys + kKeyTile - 1) / kKeyTile), places = 2 * device_cu_count();
-  if (tiles == 0 || tiles >= 4 * places) return 1;
-  const int64_t want = (4 * places + tiles - 1) / tiles, most = row_blocks / 16;
+  if (tiles == 0 || tiles >= 3 * places) return 1;
+  const int64_t want = (3 * places + tiles - 1) / tiles, most = row_blocks / 16;
   const int64_t n = want < most ? want : most;
   return static_cast<int>(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
