@@ -13,7 +13,7 @@ ST = _lib.i64x3((4096, 128, 256))
 
 def _fwd(p, batch=1, nq=2, nkv=1, sq=4, sk=4, d=128, qs=ST, ks=ST, vs=ST, scale=0.1, dtype=BF16, q=None, ranges=None):
     lib = _lib.load()
-    return lib.wx_attention_fwd(p if q is None else q, p, p, p, None, ranges, None, 0, batch, nq, nkv, sq, sk, d, qs, ks, vs, scale, dtype, None, 0, None)
+    return lib.wx_attention_fwd(p if q is None else q, p, p, p, None, None, ranges, None, 0, batch, nq, nkv, sq, sk, d, qs, ks, vs, scale, dtype, None, 0, None)
 
 
 @pytest.fixture()
@@ -52,7 +52,7 @@ def test_attention_backward_refuses(buf):
     lib = _lib.load()
 
     def bwd(nq=2, nkv=1, sq=4, sk=4, d=128, dtype=BF16, gs=ST, x=p, ws=None, n=0):
-        return lib.wx_attention_bwd(x, x, x, x, x, x, x, x, x, None, None, 0, 1, nq, nkv, sq, sk, d, ST, ST, ST, gs, 0.1, dtype, ws, n, None)
+        return lib.wx_attention_bwd(x, x, x, x, x, None, x, x, x, x, None, None, 0, 1, nq, nkv, sq, sk, d, ST, ST, ST, gs, 0.1, dtype, ws, n, None)
 
     assert bwd(d=72) == -2 and bwd(dtype=F32) == -2 and bwd(nq=3, nkv=2) == -1
     assert bwd(x=None) == -1 and bwd(gs=None) == -1 and bwd(gs=_lib.i64x3((4096, 129, 256))) == -2
@@ -60,7 +60,7 @@ def test_attention_backward_refuses(buf):
     assert bwd(nq=1025) == -2 and b"1024" in lib.wx_last_error_string()
     assert bwd() == -3 and b"workspace" in lib.wx_last_error_string()
     assert bwd(ws=p, n=lib.wx_attention_bwd_workspace_bytes(1, 2, 1, 4, 4, 128) - 1) == -3
-    assert lib.wx_attention_bwd(*([None] * 11), 0, 0, 2, 1, 4, 4, 128, ST, ST, ST, ST, 0.1, BF16, None, 0, None) == 0
+    assert lib.wx_attention_bwd(*([None] * 12), 0, 0, 2, 1, 4, 4, 128, ST, ST, ST, ST, 0.1, BF16, None, 0, None) == 0
 
 
 def test_cache_refuses(buf):

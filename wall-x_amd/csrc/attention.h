@@ -285,7 +285,37 @@ __device__ __forceinline__ void store_row(const f32x16* acc, float factor, uint1
     }
 }
 
+// What rounding the output to its type leaves, for the backward's delta = rowsum(dO O): with O as rounded, delta's error is a
+// quarter of dQ's.  e5m2, in units of 2^-10 (a value of 28672 and more keeps 57344 units of it).
+constexpr float kRestUnits = 1024.f;
 template <int DT>
-__device__ __forceinline__ float load_half(const uint16_t* p) { return Elem<DT>::load(*p); }
+__device__ __forceinline__ float rest_of(float x) {
+  const float r = (x - Elem<DT>::round(x)) * kRestUnits;
+  return fminf(fmaxf(r, -57344.f), 57344.f);
+}
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, float c, float d) {
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_bf8_f32(c, d, __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false), true));
+}
+// ... of a row of transposed accumulators, 8 bytes at a time as in store_row.
+template <int DT, int D>
+__device__ __forceinline__ void store_rest(const f32x16* acc, float factor, uint8_t* dst, int lane) {
+  const int h = lane >> 5;
+#pragma unroll
+  for (int o = 0; o < AttnTile<D>::kOut; ++o)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      if (32 * o + 8 * g >= D) continue;
+      uint32_t v[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = rest_of<DT>(acc[o][4 * (g + u) + i] * factor);
+        v[u] = pack_rest(r[0], r[1], r[2], r[3]);
+      }
+      const auto x = __builtin_amdgcn_permlane32_swap(v[0], v[1], false, false);
+      if (dst != nullptr) *reinterpret_cast<u32x2*>(dst + 32 * o + 8 * (g + h)) = u32x2{x[0], x[1]};
+    }
+}
 
 }  // namespace wx

@@ -16,6 +16,7 @@ struct BwdArgs {
   const uint16_t *q, *k, *v, *g;  // g = dO
   int64_t qs[3], ks[3], vs[3], gs[3];
   const uint16_t* out;            // [batch, n_queries, n_q, D]
+  const uint8_t* rest;            // like out: what its rounding left (rest_of), or null
   const float* lse;               // [batch, n_kv, rows]
   uint16_t *dq, *dk, *dv;         // [batch, n_queries, n_q, D], [batch, n_keys, n_kv, D]
   AttnMask mask;
@@ -64,6 +65,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   const int in_row = live ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
   const MaskRow row_mask = mask_row(a.mask, b, qi, a.n_queries, a.n_keys);
   in_order();
+  u32x2 rf[T::kSteps] = {};
   u32x4 qf[T::kSteps], gf[T::kSteps], of[T::kSteps];  // (asked for behind the mask and before anything that waits for it; a row past the last reads the first)
   {
     const uint16_t* q = row_of(a.q, a.qs, b, hq, qi);
@@ -74,6 +76,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       qf[t] = *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h);
       gf[t] = *reinterpret_cast<const u32x4*>(g + 16 * t + 8 * h);
       of[t] = *reinterpret_cast<const u32x4*>(o + 16 * t + 8 * h);
+      if (a.rest != nullptr) rf[t] = *reinterpret_cast<const u32x2*>(a.rest + (o - a.out) + 16 * t + 8 * h);
     }
   }
   float lse = a.lse[static_cast<int64_t>(pair) * a.rows + in_row];
@@ -125,6 +128,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
     float x[8], y[8];
     unpack16<DT>(gf[t], x);
     unpack16<DT>(of[t], y);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const auto lo2 = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rf[t][u]), false), hi2 = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rf[t][u]), true);
+      y[4 * u] = __builtin_fmaf(lo2[0], 1.f / kRestUnits, y[4 * u]);
+      y[4 * u + 1] = __builtin_fmaf(lo2[1], 1.f / kRestUnits, y[4 * u + 1]);
+      y[4 * u + 2] = __builtin_fmaf(hi2[0], 1.f / kRestUnits, y[4 * u + 2]);
+      y[4 * u + 3] = __builtin_fmaf(hi2[1], 1.f / kRestUnits, y[4 * u + 3]);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
   }
@@ -635,8 +646,8 @@ extern "C" size_t wx_attention_bwd_workspace_bytes(int64_t batch, int n_q_heads,
   return layout(batch * n_kv_heads, n_queries * (n_q_heads / n_kv_heads), n_keys, head_dim).total;
 }
 
-extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* grad_out,
-                                void* grad_q, void* grad_k, void* grad_v, const int32_t* key_ranges, const int32_t* key_lengths,
+extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* rest,
+                                const void* grad_out, void* grad_q, void* grad_k, void* grad_v, const int32_t* key_ranges, const int32_t* key_lengths,
                                 int causal, int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys,
                                 int head_dim, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
                                 const int64_t grad_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
@@ -649,7 +660,7 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   if (group > 1024) return fail(WX_ERR_UNSUPPORTED, "%s: more than 1024 query heads to a key / value head", who);
   if ((n_queries > 0 && (!q || !out || !lse || !grad_out || !grad_q)) || (n_keys > 0 && (!k || !v || !grad_k || !grad_v)))
     return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  for (const void* p : {q, k, v, out, grad_out, static_cast<const void*>(grad_q), static_cast<const void*>(grad_k), static_cast<const void*>(grad_v),
+  for (const void* p : {q, k, v, out, rest, grad_out, static_cast<const void*>(grad_q), static_cast<const void*>(grad_k), static_cast<const void*>(grad_v),
                         static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(p) & 15) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
   if (reinterpret_cast<uintptr_t>(key_ranges) & 7) return fail(WX_ERR_INVALID_ARGUMENT, "%s: key_ranges must be 8-byte aligned", who);
@@ -660,7 +671,7 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   BwdArgs a{};
   a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v), a.g = static_cast<const uint16_t*>(grad_out);
   for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i], a.ks[i] = k_strides[i], a.vs[i] = v_strides[i], a.gs[i] = grad_strides[i];
-  a.out = static_cast<const uint16_t*>(out), a.lse = lse;
+  a.out = static_cast<const uint16_t*>(out), a.rest = static_cast<const uint8_t*>(rest), a.lse = lse;
   a.dq = static_cast<uint16_t*>(grad_q), a.dk = static_cast<uint16_t*>(grad_k), a.dv = static_cast<uint16_t*>(grad_v);
   a.mask = {reinterpret_cast<const int2*>(key_ranges), key_lengths, causal};
   a.batch = static_cast<int>(batch), a.n_q = n_q_heads, a.n_kv = n_kv_heads, a.n_queries = static_cast<int>(n_queries), a.n_keys = static_cast<int>(n_keys);

@@ -11,6 +11,7 @@ struct FwdArgs {
   const float *k_scale, *v_scale;  // e4m3: [batch, n_kv, n_keys]
   uint16_t* out;                 // [batch, n_queries, n_q, D]
   float* lse;                    // [batch, n_kv, n_queries * group], base 2, or null
+  uint8_t* rest;                 // with lse: what out's rounding left (rest_of), like out, or null
   AttnMask mask;
   int batch, n_q, n_kv, n_queries, n_keys, group;
   int rows, row_tiles, splits;
@@ -386,6 +387,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
         if (32 * o + 8 * (r / 4) < D) bad = bad || acc[o][r] != acc[o][r];
     const float inv = some && l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     store_row<DT, D>(acc, some ? inv : 0.f, live ? out : nullptr, lane);
+    if (a.rest != nullptr) store_rest<DT, D>(acc, inv, live && some ? a.rest + (out - a.out) : nullptr, lane);
     if (!some && live) {  // (0 * NaN above)
 #pragma unroll
       for (int c = 0; c < D / 8; c += 2) *reinterpret_cast<u32x4*>(out + 8 * (c + h)) = u32x4{0u, 0u, 0u, 0u};
@@ -402,7 +404,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
       uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.n_queries + row_r / a.group) * a.n_q + hk * a.group + row_r % a.group) * D;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(o2[u] / l2));
+        if (lane + 64 * u < D) {
+          dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(o2[u] / l2));
+          if (a.rest != nullptr) a.rest[dst - a.out + lane + 64 * u] = static_cast<uint8_t>(pack_rest(rest_of<DT>(o2[u] / l2), 0.f, 0.f, 0.f));
+        }
     }
   } else {
     // Every key group's sums to LDS, 64 channels at a time, scaled to the common maximum; then a thread adds up 8 channels of a row.
@@ -469,6 +474,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = some_r ? v[e] * inv : 0.f;
             *reinterpret_cast<u32x4*>(a.out + to + ch * 8) = pack16<DT>(w);
+            if (a.rest != nullptr)
+              *reinterpret_cast<u32x2*>(a.rest + to + ch * 8) = u32x2{pack_rest(rest_of<DT>(w[0]), rest_of<DT>(w[1]), rest_of<DT>(w[2]), rest_of<DT>(w[3])),
+                                                                      pack_rest(rest_of<DT>(w[4]), rest_of<DT>(w[5]), rest_of<DT>(w[6]), rest_of<DT>(w[7]))};
             if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(pair) * a.rows + row_r] = some_r ? __builtin_fmaf(top_r, a.c, __builtin_amdgcn_logf(l_r)) : kInf;
           }
         }
@@ -487,8 +495,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
               a.part[((static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_x) * D + c] = o2[c0 / 64] * scale;
             } else {
               const int i_x = a.by_group.div(row_x);
-              a.out[((static_cast<int64_t>(b) * a.n_queries + i_x) * a.n_q + hk * a.group + row_x - i_x * a.group) * D + c] =
-                  static_cast<uint16_t>(Elem<DT>::store(o2[c0 / 64] / l2));
+              const int64_t to_x = ((static_cast<int64_t>(b) * a.n_queries + i_x) * a.n_q + hk * a.group + row_x - i_x * a.group) * D + c;
+              a.out[to_x] = static_cast<uint16_t>(Elem<DT>::store(o2[c0 / 64] / l2));
+              if (a.rest != nullptr) a.rest[to_x] = static_cast<uint8_t>(pack_rest(rest_of<DT>(o2[c0 / 64] / l2), 0.f, 0.f, 0.f));
             }
           }
         }
@@ -541,7 +550,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
   key_range(a.mask, b, i, a.n_queries, a.n_keys, lo, hi);
   if (tid < D) {
     const float sum = (s_out[0][tid] + s_out[1][tid]) + (s_out[2][tid] + s_out[3][tid]);
-    a.out[((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D + tid] = static_cast<uint16_t>(Elem<DT>::store(hi > lo ? sum / l : 0.f));
+    const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D + tid;
+    const float x = hi > lo ? sum / l : 0.f;
+    a.out[to] = static_cast<uint16_t>(Elem<DT>::store(x));
+    if (a.rest != nullptr) a.rest[to] = static_cast<uint8_t>(pack_rest(rest_of<DT>(x), 0.f, 0.f, 0.f));
   }
   if (a.lse != nullptr && tid == 0) a.lse[at] = hi > lo ? __builtin_fmaf(top, a.c, __builtin_amdgcn_logf(l)) : kInf;
 }
@@ -646,14 +658,14 @@ extern "C" size_t wx_attention_workspace_bytes(int64_t batch, int n_q_heads, int
 }
 
 static int forward(const char* who, const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, bool f8,
-                   void* out, float* lse, const int32_t* key_ranges, const int32_t* key_lengths, int causal, int64_t batch,
+                   void* out, float* lse, void* rest, const int32_t* key_ranges, const int32_t* key_lengths, int causal, int64_t batch,
                    int n_q, int n_kv, int64_t n_queries, int64_t n_keys, int head_dim, const int64_t* qs, const int64_t* ks,
                    const int64_t* vs, float scale, int dtype, void* workspace, size_t workspace_bytes, wx_stream_t stream) {
   if (int rc = attention_check(who, batch, n_q, n_kv, n_queries, n_keys, head_dim, dtype, scale)) return rc;
   if (!qs || !ks || !vs) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null strides", who);
   if (batch == 0 || n_q == 0 || n_queries == 0) return WX_OK;
   if (!q || !out || (n_keys > 0 && (!k || !v || (f8 && (!k_scale || !v_scale))))) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out)) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
+  if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(rest)) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
   if (reinterpret_cast<uintptr_t>(key_ranges) & 7) return fail(WX_ERR_INVALID_ARGUMENT, "%s: key_ranges must be 8-byte aligned", who);
   const int group = n_q / n_kv;
   if (int rc = attention_check_strides(who, "q", qs, 2, 1, 1)) return rc;
@@ -663,7 +675,7 @@ static int forward(const char* who, const void* q, const void* k, const void* v,
   a.q = q, a.k = k, a.v = v;
   for (int i = 0; i < 3; ++i) a.qs[i] = qs[i], a.ks[i] = ks[i], a.vs[i] = vs[i];
   a.k_scale = k_scale, a.v_scale = v_scale;
-  a.out = static_cast<uint16_t*>(out), a.lse = lse;
+  a.out = static_cast<uint16_t*>(out), a.lse = lse, a.rest = static_cast<uint8_t*>(rest);
   a.mask = {reinterpret_cast<const int2*>(key_ranges), key_lengths, causal};
   a.batch = static_cast<int>(batch), a.n_q = n_q, a.n_kv = n_kv, a.n_queries = static_cast<int>(n_queries), a.n_keys = static_cast<int>(n_keys);
   a.group = group, a.rows = static_cast<int>(n_queries) * group;
@@ -678,12 +690,12 @@ static int forward(const char* who, const void* q, const void* k, const void* v,
   return f8 ? dispatch_fwd<true>(a, p, head_dim, dtype, as_stream(stream)) : dispatch_fwd<false>(a, p, head_dim, dtype, as_stream(stream));
 }
 
-extern "C" int wx_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_ranges,
+extern "C" int wx_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const int32_t* key_ranges,
                                 const int32_t* key_lengths, int causal, int64_t batch, int n_q_heads, int n_kv_heads,
                                 int64_t n_queries, int64_t n_keys, int head_dim, const int64_t q_strides[3], const int64_t k_strides[3],
                                 const int64_t v_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
                                 wx_stream_t stream) {
-  return forward("wx_attention_fwd", q, k, v, nullptr, nullptr, false, out, lse, key_ranges, key_lengths, causal, batch, n_q_heads,
+  return forward("wx_attention_fwd", q, k, v, nullptr, nullptr, false, out, lse, rest, key_ranges, key_lengths, causal, batch, n_q_heads,
                  n_kv_heads, n_queries, n_keys, head_dim, q_strides, k_strides, v_strides, scale, dtype, workspace, workspace_bytes, stream);
 }
 
@@ -693,6 +705,6 @@ extern "C" int wx_cached_attention(const void* q, const void* k_cache, const voi
                                    const int64_t q_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
                                    wx_stream_t stream) {
   const int64_t st[3] = {n_kv_heads * capacity * head_dim, capacity * head_dim, head_dim};
-  return forward("wx_cached_attention", q, k_cache, v_cache, k_scale, v_scale, true, out, nullptr, key_ranges, key_lengths, causal, batch,
+  return forward("wx_cached_attention", q, k_cache, v_cache, k_scale, v_scale, true, out, nullptr, nullptr, key_ranges, key_lengths, causal, batch,
                  n_q_heads, n_kv_heads, n_queries, capacity, head_dim, q_strides, st, st, scale, dtype, workspace, workspace_bytes, stream);
 }

@@ -415,18 +415,19 @@ struct Attention : torch::autograd::Function<Attention> {
                                const std::optional<at::Tensor>& key_lengths, bool causal, double scale) {
     const at::Tensor ranges = key_ranges.value_or(at::Tensor()), lengths = key_lengths.value_or(at::Tensor());
     const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
-    at::Tensor out, lse;
+    at::Tensor out, lse, rest;
     launch(q, [&] {
       out = token_major(B, Hq, Sq, D, q.options());
       if (ctx) lse = at::empty({B, Hk, Sq * (Hq / Hk)}, q.options().dtype(at::kFloat));
+      if (ctx) rest = at::empty({B, Sq, Hq, D}, q.options().dtype(at::kByte));
       const size_t bytes = entry.attention_bytes(B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D));
       const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
-      return entry.attention(ptr(q), ptr(k), ptr(v), ptr(out), ctx ? static_cast<float*>(ptr(lse)) : nullptr, ints(ranges), ints(lengths), causal, B,
+      return entry.attention(ptr(q), ptr(k), ptr(v), ptr(out), ctx ? static_cast<float*>(ptr(lse)) : nullptr, ctx ? ptr(rest) : nullptr, ints(ranges), ints(lengths), causal, B,
                              static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D), RowStrides(q).v, RowStrides(k).v, RowStrides(v).v,
                              static_cast<float>(scale), dtype_code(q.scalar_type()), bytes ? ptr(work) : nullptr, bytes, stream_of(q));
     });
     if (ctx) {
-      ctx->save_for_backward({q, k, v, out, lse, ranges, lengths});
+      ctx->save_for_backward({q, k, v, out, lse, rest, ranges, lengths});
       ctx->saved_data["causal"] = causal;
       ctx->saved_data["scale"] = scale;
     }
@@ -434,7 +435,7 @@ struct Attention : torch::autograd::Function<Attention> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &ranges = saved[5], &lengths = saved[6];
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &rest = saved[5], &ranges = saved[6], &lengths = saved[7];
     TORCH_CHECK(!at::GradMode::is_enabled(), "attention's backward is not differentiable");
     const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
     at::Tensor dq, dk, dv;
@@ -447,7 +448,7 @@ struct Attention : torch::autograd::Function<Attention> {
       if (!packed16(tokens)) tokens = tokens.clone(at::MemoryFormat::Contiguous);
       const size_t bytes = entry.attention_bwd_bytes(B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D));
       const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
-      return entry.attention_bwd(ptr(q), ptr(k), ptr(v), ptr(tokens), static_cast<const float*>(ptr(lse)), ptr(g), ptr(dq), ptr(dk), ptr(dv), ints(ranges),
+      return entry.attention_bwd(ptr(q), ptr(k), ptr(v), ptr(tokens), static_cast<const float*>(ptr(lse)), ptr(rest), ptr(g), ptr(dq), ptr(dk), ptr(dv), ints(ranges),
                                  ints(lengths), ctx->saved_data["causal"].toBool(), B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D),
                                  RowStrides(q).v, RowStrides(k).v, RowStrides(v).v, RowStrides(g).v, static_cast<float>(ctx->saved_data["scale"].toDouble()),
                                  dtype_code(q.scalar_type()), bytes ? ptr(work) : nullptr, bytes, stream_of(q));

@@ -86,9 +86,9 @@ PROTOTYPES = {
     "wx_qk_norm_rope_bwd": (_i32, [_vp] * 6 + [_f32] + [_vp] * 6 + [_i64, _i64, _i32, _i32, _i32] + [_c.POINTER(_i64)] * 4
                             + [_c.POINTER(_i32), _i32, _i32, _vp, _sz, _vp]),
     "wx_attention_workspace_bytes": (_sz, [_i64, _i32, _i32, _i64, _i64, _i32]),
-    "wx_attention_fwd": (_i32, [_vp] * 7 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32] + [_c.POINTER(_i64)] * 3 + [_f32, _i32, _vp, _sz, _vp]),
+    "wx_attention_fwd": (_i32, [_vp] * 8 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32] + [_c.POINTER(_i64)] * 3 + [_f32, _i32, _vp, _sz, _vp]),
     "wx_attention_bwd_workspace_bytes": (_sz, [_i64, _i32, _i32, _i64, _i64, _i32]),
-    "wx_attention_bwd": (_i32, [_vp] * 11 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32] + [_c.POINTER(_i64)] * 4 + [_f32, _i32, _vp, _sz, _vp]),
+    "wx_attention_bwd": (_i32, [_vp] * 12 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32] + [_c.POINTER(_i64)] * 4 + [_f32, _i32, _vp, _sz, _vp]),
     "wx_kv_cache_write": (_i32, [_vp] * 8 + [_i64, _i32, _i64, _i64, _i32] + [_c.POINTER(_i64)] * 2 + [_i32, _vp]),
     "wx_cached_attention": (_i32, [_vp] * 8 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32, _c.POINTER(_i64), _f32, _i32, _vp, _sz, _vp]),
     "wx_swiglu_bwd": (_i32, [_vp] * 6 + [_i64, _vp]),

@@ -114,9 +114,9 @@ def attention_fwd(q, k, v, key_ranges=None, key_lengths=None, causal=False, scal
     return native.attention_fwd(q, k, v, key_ranges, key_lengths, causal, scale, want_lse)
 
 
-def attention_bwd(grad_out, q, k, v, out, lse, key_ranges=None, key_lengths=None, causal=False, scale=None):
+def attention_bwd(grad_out, q, k, v, out, lse, rest, key_ranges=None, key_lengths=None, causal=False, scale=None):
     """No counterpart in backend.py: the gradients of attention_fwd."""
-    return native.attention_bwd(grad_out, q, k, v, out, lse, key_ranges, key_lengths, causal, scale)
+    return native.attention_bwd(grad_out, q, k, v, out, lse, rest, key_ranges, key_lengths, causal, scale)
 
 
 def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths=None):

@@ -530,20 +530,21 @@ def qk_norm_rope_from_positions(q, k, q_weight, k_weight, position_ids, inv_freq
 
 # ----------------------------------------------------------------------------- attention
 class Attention(torch.autograd.Function):
-    """Keeps q, k, v, the output and a number per row of the scores; the backward recomputes the probabilities."""
+    """Keeps q, k, v, the output with a byte per value of what its rounding left, and a number per row of the scores; the
+    backward recomputes the probabilities."""
 
     @staticmethod
     def forward(ctx, q, k, v, key_ranges, key_lengths, causal, scale):
-        out, lse = backend.attention_fwd(q, k, v, key_ranges, key_lengths, causal, scale, want_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, key_ranges, key_lengths)
+        out, lse, rest = backend.attention_fwd(q, k, v, key_ranges, key_lengths, causal, scale, want_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, rest, key_ranges, key_lengths)
         ctx.mask = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, key_ranges, key_lengths = ctx.saved_tensors
-        grads = backend.attention_bwd(grad_out, q, k, v, out, lse, key_ranges, key_lengths, *ctx.mask)
+        q, k, v, out, lse, rest, key_ranges, key_lengths = ctx.saved_tensors
+        grads = backend.attention_bwd(grad_out, q, k, v, out, lse, rest, key_ranges, key_lengths, *ctx.mask)
         return (*(g if w else None for g, w in zip(grads, ctx.needs_input_grad)), None, None, None, None)
 
 

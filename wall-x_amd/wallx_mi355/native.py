@@ -644,7 +644,7 @@ def _token_major(B, H, S, D, like):
 
 
 def attention_fwd(q, k, v, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None, want_lse: bool = False):
-    """(out [B, Hq, Sq, D] over token-major memory, lse or None): softmax(scale q k^T) v of q [B, Hq, Sq, D] over k and v
+    """(out [B, Hq, Sq, D] over token-major memory, lse, rest; the last two, for attention_bwd, None unless wanted): softmax(scale q k^T) v of q [B, Hq, Sq, D] over k and v
     [B, Hkv, Sk, D] (any strides), query i of row b seeing the keys [lo, hi) of key_ranges int32 [B, Sq, 2], below key_lengths
     int32 [B] and, with causal, up to its own position when the queries are the last of the keys."""
     _same_device(("q", q), ("k", k), ("v", v), ("key_ranges", key_ranges), ("key_lengths", key_lengths))
@@ -655,17 +655,18 @@ def attention_fwd(q, k, v, key_ranges=None, key_lengths=None, causal: bool = Fal
     Hk, Sk = k.size(1), k.size(2)
     out = _token_major(B, Hq, Sq, D, q)
     lse = torch.empty((B, Hk, Sq * (Hq // Hk)), dtype=torch.float32, device=q.device) if want_lse else None
+    rest = torch.empty((B, Sq, Hq, D), dtype=torch.uint8, device=q.device) if want_lse else None
     with _DeviceGuard(q):
         n_work = _lib.load().wx_attention_workspace_bytes(B, Hq, Hk, Sq, Sk, D)
         work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
-        _lib.call("wx_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(key_ranges), _ptr(key_lengths), int(bool(causal)), B, Hq, Hk,
-                  Sq, Sk, D, _row_strides(q), _row_strides(k), _row_strides(v), scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
-    return out, lse
+        _lib.call("wx_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(rest), _ptr(key_ranges), _ptr(key_lengths), int(bool(causal)), B, Hq,
+                  Hk, Sq, Sk, D, _row_strides(q), _row_strides(k), _row_strides(v), scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
+    return out, lse, rest
 
 
-def attention_bwd(grad_out, q, k, v, out, lse, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None):
+def attention_bwd(grad_out, q, k, v, out, lse, rest, key_ranges=None, key_lengths=None, causal: bool = False, scale: Optional[float] = None):
     """(grad_q, grad_k, grad_v) over token-major memory, from what attention_fwd took and returned."""
-    _same_device(("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse), ("gradient", grad_out), ("key_ranges", key_ranges), ("key_lengths", key_lengths))
+    _same_device(("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse), ("rest", rest), ("gradient", grad_out), ("key_ranges", key_ranges), ("key_lengths", key_lengths))
     _attention_shapes(q, k, v)
     key_ranges, key_lengths, scale = _attention_args(q, k.size(2), k.size(1), key_ranges, key_lengths, scale)
     if grad_out.shape != q.shape or grad_out.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
@@ -677,11 +678,13 @@ def attention_bwd(grad_out, q, k, v, out, lse, key_ranges=None, key_lengths=None
     tokens = _packed16(tokens)
     if lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hk, Sq * (Hq // Hk)) or not lse.is_contiguous():
         raise RuntimeError("lse must be what attention_fwd returned")
+    if rest is not None and (rest.dtype != torch.uint8 or tuple(rest.shape) != (B, Sq, Hq, D) or not rest.is_contiguous()):
+        raise RuntimeError("rest must be what attention_fwd returned")
     dq, dk, dv = _token_major(B, Hq, Sq, D, q), _token_major(B, Hk, Sk, D, q), _token_major(B, Hk, Sk, D, q)
     with _DeviceGuard(q):
         n_work = _lib.load().wx_attention_bwd_workspace_bytes(B, Hq, Hk, Sq, Sk, D)
         work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
-        _lib.call("wx_attention_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(tokens), _ptr(lse), _ptr(grad_out), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(key_ranges),
+        _lib.call("wx_attention_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(tokens), _ptr(lse), _ptr(rest), _ptr(grad_out), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(key_ranges),
                   _ptr(key_lengths), int(bool(causal)), B, Hq, Hk, Sq, Sk, D, _row_strides(q), _row_strides(k), _row_strides(v), _row_strides(grad_out),
                   scale, _DTYPES[q.dtype], _ptr(work), n_work, _stream(q))
     return dq, dk, dv
