@@ -257,27 +257,48 @@ __device__ __forceinline__ void wait_lds() {
   asm volatile("" ::: "memory");
 }
 
+// What rounding the output to its type leaves, as e5m2, for the backward's delta = rowsum(dO O): with O as rounded, delta's error is
+// a quarter of dQ's.  (Too small for e5m2 where the output is below 2^-7 or so: such a part of delta has no weight beside
+// the slopes.)
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, float c, float d) {
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_bf8_f32(c, d, __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false), true));
+}
+template <int DT>
+__device__ __forceinline__ float rest_of(float x) { return x - Elem<DT>::round(x); }
+template <int DT>
+__device__ __forceinline__ uint32_t pack_rest_of(float a, float b, float c, float d) {
+  return pack_rest(rest_of<DT>(a), rest_of<DT>(b), rest_of<DT>(c), rest_of<DT>(d));
+}
+
 // Transposed accumulators (channel 32 o + 8 g + 4 h + i, row lane & 31) to one row of 2-byte values: the halves trade groups so
-// that a lane stores 8 consecutive channels, 16 bytes, at a time.  `dst` is the lane's row or null.
-template <int DT, int D>
-__device__ __forceinline__ void store_row(const f32x16* acc, float factor, uint16_t* dst, int lane) {
+// that a lane stores 8 consecutive channels, 16 bytes, at a time.  `dst` is the lane's row or null; `rest` its row of rests or null.
+template <int DT, int D, bool REST = false>
+__device__ __forceinline__ void store_row(const f32x16* acc, float factor, uint16_t* dst, int lane, uint8_t* rest = nullptr) {
   const int h = lane >> 5;
 #pragma unroll
   for (int o = 0; o < AttnTile<D>::kOut; ++o)
 #pragma unroll
     for (int g = 0; g < 4; g += 2) {
       if (32 * o + 8 * g >= D) continue;
-      const f32x16& x = acc[o];
-      uint32_t a[2], b[2];
+      float x[8];
+      uint32_t a[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        a[u] = pack2<DT>(x[4 * g + 2 * u] * factor, x[4 * g + 2 * u + 1] * factor);
-        b[u] = pack2<DT>(x[4 * g + 4 + 2 * u] * factor, x[4 * g + 5 + 2 * u] * factor);
+      for (int u = 0; u < 8; ++u) x[u] = acc[o][4 * g + u] * factor;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a[u] = pack2<DT>(x[2 * u], x[2 * u + 1]);
+      if constexpr (REST) {
+        uint32_t r[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          r[u] = pack_rest(x[4 * u] - Elem<DT>::load(a[2 * u] & 0xffffu), x[4 * u + 1] - Elem<DT>::load(a[2 * u] >> 16),
+                           x[4 * u + 2] - Elem<DT>::load(a[2 * u + 1] & 0xffffu), x[4 * u + 3] - Elem<DT>::load(a[2 * u + 1] >> 16));
+        const auto y = __builtin_amdgcn_permlane32_swap(r[0], r[1], false, false);
+        if (rest != nullptr) *reinterpret_cast<u32x2*>(rest + 32 * o + 8 * (g + h)) = u32x2{y[0], y[1]};
       }
       u32x4 v;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const auto r = __builtin_amdgcn_permlane32_swap(a[u], b[u], false, false);
+        const auto r = __builtin_amdgcn_permlane32_swap(a[u], a[2 + u], false, false);
         v[u] = r[0];
         v[2 + u] = r[1];
       }
@@ -285,37 +306,19 @@ __device__ __forceinline__ void store_row(const f32x16* acc, float factor, uint1
     }
 }
 
-// What rounding the output to its type leaves, for the backward's delta = rowsum(dO O): with O as rounded, delta's error is a
-// quarter of dQ's.  e5m2, in units of 2^-10 (a value of 28672 and more keeps 57344 units of it).
-constexpr float kRestUnits = 1024.f;
+// acc + the products of two pairs of 16-bit values, in fp32
 template <int DT>
-__device__ __forceinline__ float rest_of(float x) {
-  const float r = (x - Elem<DT>::round(x)) * kRestUnits;
-  return fminf(fmaxf(r, -57344.f), 57344.f);
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float acc) {
+  if constexpr (DT == WX_BF16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(att_bf16x2, a), __builtin_bit_cast(att_bf16x2, b), acc, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(att_f16x2, a), __builtin_bit_cast(att_f16x2, b), acc, false);
 }
-__device__ __forceinline__ uint32_t pack_rest(float a, float b, float c, float d) {
-  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_bf8_f32(c, d, __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false), true));
-}
-// ... of a row of transposed accumulators, 8 bytes at a time as in store_row.
-template <int DT, int D>
-__device__ __forceinline__ void store_rest(const f32x16* acc, float factor, uint8_t* dst, int lane) {
-  const int h = lane >> 5;
-#pragma unroll
-  for (int o = 0; o < AttnTile<D>::kOut; ++o)
-#pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      if (32 * o + 8 * g >= D) continue;
-      uint32_t v[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = rest_of<DT>(acc[o][4 * (g + u) + i] * factor);
-        v[u] = pack_rest(r[0], r[1], r[2], r[3]);
-      }
-      const auto x = __builtin_amdgcn_permlane32_swap(v[0], v[1], false, false);
-      if (dst != nullptr) *reinterpret_cast<u32x2*>(dst + 32 * o + 8 * (g + h)) = u32x2{x[0], x[1]};
-    }
+// two e5m2 values to two of the compute type (exact)
+template <int DT, bool HI>
+__device__ __forceinline__ uint32_t widen_rest2(uint32_t x) {
+  if constexpr (DT == WX_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, 1.0f, HI));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(x, 1.0f, HI));
 }
 
 }  // namespace wx

@@ -122,24 +122,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   };
   if (iters > 0) fetch(0, lds0);
 
-  float delta = 0.f;
+  float sums[2] = {0.f, 0.f}, rests = 0.f;
 #pragma unroll
   for (int t = 0; t < T::kSteps; ++t) {
-    float x[8], y[8];
-    unpack16<DT>(gf[t], x);
-    unpack16<DT>(of[t], y);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const auto lo2 = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rf[t][u]), false), hi2 = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rf[t][u]), true);
-      y[4 * u] = __builtin_fmaf(lo2[0], 1.f / kRestUnits, y[4 * u]);
-      y[4 * u + 1] = __builtin_fmaf(lo2[1], 1.f / kRestUnits, y[4 * u + 1]);
-      y[4 * u + 2] = __builtin_fmaf(hi2[0], 1.f / kRestUnits, y[4 * u + 2]);
-      y[4 * u + 3] = __builtin_fmaf(hi2[1], 1.f / kRestUnits, y[4 * u + 3]);
-    }
+    for (int u = 0; u < 4; ++u) sums[u & 1] = dot2<DT>(gf[t][u], of[t][u], sums[u & 1]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+    for (int u = 0; u < 2; ++u) rests = dot2<DT>(gf[t][2 * u + 1], widen_rest2<DT, true>(rf[t][u]), dot2<DT>(gf[t][2 * u], widen_rest2<DT, false>(rf[t][u]), rests));
   }
-  delta = some ? both_sum(delta) : 0.f;
+  rests = both_sum(rests);
+  // (a rest that e5m2 does not hold, of outputs of 10^7 and more, is left out)
+  const float delta = some ? both_sum(sums[0] + sums[1]) + (fabsf(rests) < kInf ? rests : 0.f) : 0.f;
   lse = some ? lse : kInf;
   const int block = tile * 4 + wave;
   if (block < a.row_blocks) {

@@ -386,8 +386,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
       for (int r = 0; r < 16; ++r)
         if (32 * o + 8 * (r / 4) < D) bad = bad || acc[o][r] != acc[o][r];
     const float inv = some && l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    store_row<DT, D>(acc, some ? inv : 0.f, live ? out : nullptr, lane);
-    if (a.rest != nullptr) store_rest<DT, D>(acc, inv, live && some ? a.rest + (out - a.out) : nullptr, lane);
+    if (!F8 && a.rest != nullptr) store_row<DT, D, true>(acc, some ? inv : 0.f, live ? out : nullptr, lane, live ? a.rest + (out - a.out) : nullptr);
+    else store_row<DT, D>(acc, some ? inv : 0.f, live ? out : nullptr, lane);
     if (!some && live) {  // (0 * NaN above)
 #pragma unroll
       for (int c = 0; c < D / 8; c += 2) *reinterpret_cast<u32x4*>(out + 8 * (c + h)) = u32x4{0u, 0u, 0u, 0u};
@@ -475,8 +475,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
             for (int e = 0; e < 8; ++e) w[e] = some_r ? v[e] * inv : 0.f;
             *reinterpret_cast<u32x4*>(a.out + to + ch * 8) = pack16<DT>(w);
             if (a.rest != nullptr)
-              *reinterpret_cast<u32x2*>(a.rest + to + ch * 8) = u32x2{pack_rest(rest_of<DT>(w[0]), rest_of<DT>(w[1]), rest_of<DT>(w[2]), rest_of<DT>(w[3])),
-                                                                      pack_rest(rest_of<DT>(w[4]), rest_of<DT>(w[5]), rest_of<DT>(w[6]), rest_of<DT>(w[7]))};
+              *reinterpret_cast<u32x2*>(a.rest + to + ch * 8) = u32x2{pack_rest_of<DT>(w[0], w[1], w[2], w[3]), pack_rest_of<DT>(w[4], w[5], w[6], w[7])};
             if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(pair) * a.rows + row_r] = some_r ? __builtin_fmaf(top_r, a.c, __builtin_amdgcn_logf(l_r)) : kInf;
           }
         }
