@@ -1,8 +1,9 @@
 """Prefill harness for BASELINE config 5: a randomly initialised decoder with the Qwen2.5-VL-3B shape and the
 dual VL / action expert FFN in every layer (act.py:172-273, 397-530), with every layer's permute, grouped GEMM,
 M-RoPE and the position builder replaced by the MI355X kernels.  Attention stays on PyTorch-ROCm
-(F.scaled_dot_product_attention), as the configuration prescribes; the QKV / O projections run on this library's
-GEMM by default (they carry the rotary embedding and the residual add in their epilogues) or on the vendor's.
+(F.scaled_dot_product_attention), as the configuration prescribes, unless `attention_native=True` asks for this
+library's; the QKV / O projections run on this library's GEMM by default (they carry the rotary embedding and the
+residual add in their epilogues) or on the vendor's.
 
 This is a measurement harness, not a model port: no KV cache, no generation, no losses; one forward over a
 batch of full sequences (prefill).  What it states explicitly:
@@ -21,7 +22,10 @@ batch of full sequences (prefill).  What it states explicitly:
   * `fuse_qkv_rope=True` (default) replaces the vendor GEMM of the q / k / v projection and the rope kernel by one
     launch of this library's GEMM with bias and M-RoPE in its epilogue (vl.py:955-964); `o_proj_native=True`
     (default) runs the o projection with the residual add on this library's row-major GEMM.  With both False the
-    projections are vendor GEMMs.
+    projections are vendor GEMMs,
+  * `attention_native=True` (default False) runs every layer's attention as one launch of `ops.attention`.  The mask
+    of action tokens then goes in as a key range per token, built once per forward for any place of the action tokens
+    in a row as long as they are one run of positions (`action_suffix` is not needed and not read).
 """
 
 from contextlib import contextmanager
@@ -69,7 +73,8 @@ class PrefillHarness:
     def __init__(self, n_layers: int = 36, hidden: int = wl.HIDDEN, n_q: int = wl.N_Q_HEADS, n_kv: int = wl.N_KV_HEADS,
                  head_dim: int = wl.HEAD_DIM, inter=(wl.INTER_VL, wl.INTER_ACT), vocab: int = 151936,
                  eps: float = 1e-6, device="cuda:0", seed: int = 0, mask: str = "causal", keep_dense: bool = False,
-                 fuse: bool = True, fuse_qkv_rope: bool = True, o_proj_native: bool = True):
+                 fuse: bool = True, fuse_qkv_rope: bool = True, o_proj_native: bool = True,
+                 attention_native: bool = False):
         self.dev = torch.device(device)
         # the q / k / v projection with M-RoPE in its epilogue (one launch of this library's GEMM kernel) instead of
         # the vendor GEMM followed by the rope kernel; needs fuse=True (token-major q / k) and head_dim 128
@@ -77,6 +82,7 @@ class PrefillHarness:
         # the o projection with the attention residual added in its epilogue on this library's row-major GEMM
         # (wx_dual_gemm_add, second group empty) instead of the vendor's addmm; needs fuse=True
         self.o_proj_native = o_proj_native and fuse
+        self.attention_native = attention_native  # ops.attention instead of torch's; head_dim 64, 80 or 128
         self.n_layers, self.hidden, self.n_q, self.n_kv, self.head_dim = n_layers, hidden, n_q, n_kv, head_dim
         self.inter, self.eps, self.mask_mode, self.fuse = inter, eps, mask, fuse
         g = torch.Generator(device=self.dev).manual_seed(seed)
@@ -185,8 +191,12 @@ class PrefillHarness:
         if self.fuse_qkv_rope:
             with timer.section("mrope_table"):
                 rope_table = native.mrope_table(pos, self.inv_freq, wl.MROPE_SECTION)
-        attn_mask, n_tail = None, 0
-        if self.mask_mode == "action_block":
+        attn_mask, n_tail, key_ranges = None, 0, None
+        if self.attention_native:
+            if self.mask_mode == "action_block":
+                with timer.section("attention_ranges"):
+                    key_ranges = ops.attention_key_ranges(moe_token_types)
+        elif self.mask_mode == "action_block":
             if action_suffix is not None:
                 # the action tokens are the last `action_suffix` positions of every row: an action query then sees
                 # every key of its row (all earlier tokens causally, all action tokens through the block), the other
@@ -232,8 +242,10 @@ class PrefillHarness:
                     if capture is not None and li in capture.get("layers", ()):
                         capture[li] = {"q_in": q, "k_in": k, "q_out": qr, "k_out": kr}
                     q, k = qr, kr
-            with timer.section("sdpa_torch"):
-                if n_tail:
+            with timer.section("attention" if self.attention_native else "sdpa_torch"):
+                if self.attention_native:
+                    a = ops.attention(q, k, v, key_ranges, causal=key_ranges is None)
+                elif n_tail:
                     head = S - n_tail
                     a = torch.empty_like(q)
                     a[:, :, :head] = F.scaled_dot_product_attention(q[:, :, :head], k[:, :, :head], v[:, :, :head],
