@@ -309,6 +309,20 @@ void launch(const at::Tensor& t, F f) {
   TORCH_CHECK(rc == 0, "wallx_mi355: ", entry.last_error(), " (status ", rc, ")");
 }
 
+// A backward pass under capture must not hand its gradients to a node that was made on the default stream, as the accumulation into a
+// leaf is whose eager graph still lives: the engine makes that node's stream wait for the capturing one, which HIP does not allow the
+// default stream (id 0), and what is left of the capture ends the process.  Called before the first launch, under the node at work.
+void check_capture(const at::Tensor& t) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(reinterpret_cast<hipStream_t>(stream_of(t)), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges())
+    if (const auto made = edge.function ? edge.function->stream() : std::nullopt)
+      TORCH_CHECK(made->id() != 0, "a backward pass is captured while an earlier graph of the same leaves, made on the default stream, is alive: drop "
+                                   "that graph's outputs first, or capture the gradients of detached copies");
+}
+
 bool optional(PyObject* o, const at::Tensor*& t) {
   t = nullptr;
   return o == Py_None || (t = plain(o)) != nullptr;
@@ -347,8 +361,10 @@ struct NormRope : torch::autograd::Function<NormRope> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3], &source = saved[4], &freq = saved[5];
+    const at::Tensor q = as_rows16(saved[0]), k = as_rows16(saved[1]);  // (saved-tensor hooks may hand them back in another order)
+    const at::Tensor &wq = saved[2], &wk = saved[3], &source = saved[4], &freq = saved[5];
     TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope's backward is not differentiable");
+    check_capture(saved[0]);
     const std::vector<int64_t> section = ctx->saved_data["section"].toIntVector();
     const int sec[3] = {static_cast<int>(section[0]), static_cast<int>(section[1]), static_cast<int>(section[2])};
     const int layout = static_cast<int>(ctx->saved_data["layout"].toInt());
@@ -435,8 +451,10 @@ struct Attention : torch::autograd::Function<Attention> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &rest = saved[5], &ranges = saved[6], &lengths = saved[7];
+    const at::Tensor q = as_rows16(saved[0]), k = as_rows16(saved[1]), v = as_rows16(saved[2]);  // (see above)
+    const at::Tensor &out = saved[3], &lse = saved[4], &rest = saved[5], &ranges = saved[6], &lengths = saved[7];
     TORCH_CHECK(!at::GradMode::is_enabled(), "attention's backward is not differentiable");
+    check_capture(saved[0]);
     const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
     at::Tensor dq, dk, dv;
     launch(q, [&] {
@@ -444,7 +462,7 @@ struct Attention : torch::autograd::Function<Attention> {
       dq = token_major(B, Hq, Sq, D, q.options());
       dk = token_major(B, Hk, Sk, D, q.options());
       dv = token_major(B, Hk, Sk, D, q.options());
-      at::Tensor tokens = out.transpose(1, 2);  // (saved-tensor hooks may hand it back in another order)
+      at::Tensor tokens = out.transpose(1, 2);
       if (!packed16(tokens)) tokens = tokens.clone(at::MemoryFormat::Contiguous);
       const size_t bytes = entry.attention_bwd_bytes(B, static_cast<int>(Hq), static_cast<int>(Hk), Sq, Sk, static_cast<int>(D));
       const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
@@ -585,8 +603,17 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return none();
 }
 
+// capture_check(tensor): check_capture for the backward of a node in Python.
+PyObject* capture_check(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (const at::Tensor* t = n == 1 ? plain(args[0]) : nullptr) check_capture(*t);
+  return none();
+  END_HANDLE_TH_ERRORS
+}
+
 #define WX_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL
 PyMethodDef methods[] = {{"rope", WX_FAST(rope), nullptr},
+                         {"capture_check", WX_FAST(capture_check), nullptr},
                          {"permute", WX_FAST(permute), nullptr},
                          {"unpermute", WX_FAST(unpermute), nullptr},
                          {"unpermute_bwd", WX_FAST(unpermute_bwd), nullptr},

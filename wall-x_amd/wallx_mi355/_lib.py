@@ -134,7 +134,7 @@ def host_path() -> str:
 class _NoHost:
     """In the place of the host module where it is not built: every call goes on in the general path."""
 
-    rope = permute = unpermute = unpermute_bwd = norm_rope = attention = cached_attention = cache_write = staticmethod(lambda *args: None)
+    rope = permute = unpermute = unpermute_bwd = norm_rope = attention = cached_attention = cache_write = capture_check = staticmethod(lambda *args: None)
 
 
 def host():

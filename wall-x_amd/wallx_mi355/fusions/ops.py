@@ -489,6 +489,7 @@ class QKNormRoPE(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_q, grad_k):
         q, k, q_weight, k_weight, source, inv_freq = ctx.saved_tensors
+        _lib.host().capture_check(q)
         grads = backend.qk_norm_rope_bwd(grad_q, grad_k, q, k, q_weight, k_weight, source, inv_freq, *ctx.rope, want=ctx.needs_input_grad[:4])
         return (*grads, None, None, None, None, None)
 
@@ -544,6 +545,7 @@ class Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         q, k, v, out, lse, rest, key_ranges, key_lengths = ctx.saved_tensors
+        _lib.host().capture_check(q)
         grads = backend.attention_bwd(grad_out, q, k, v, out, lse, rest, key_ranges, key_lengths, *ctx.mask)
         return (*(g if w else None for g, w in zip(grads, ctx.needs_input_grad)), None, None, None, None)
 
