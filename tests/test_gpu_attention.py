@@ -131,6 +131,24 @@ def test_forward_and_gradients(dev, size, mask):
     assert all(torch.equal(a, b) for a, b in zip(grads, again)), "the gradients differ between two runs"
 
 
+LONG = [(1, 16, 1, 8300, 150, 64), (1, 4, 1, 40, 9000, 128), (1, 6, 2, 2900, 2900, 80)]
+
+
+@pytest.mark.parametrize("size,mask", [(s, m) for s in LONG for m in ("full", "causal", "any")] + [(LONG[2], "packed"), (LONG[2], "action")])
+def test_gradients_of_long_axes(dev, size, mask):
+    """More than 4096 blocks of 32 rows, more than 64 tiles of 64 keys, tiles whose rows are cut into many units."""
+    B, Hq, Hkv, Sq, Sk, D = size
+    g = torch.Generator(device=dev).manual_seed(Sq + D)
+    dtype = torch.float16 if D == 80 else torch.bfloat16
+    q, k, v, do = heads(B, Sq, Hq, D, dtype, g, dev), heads(B, Sk, Hkv, D, dtype, g, dev), heads(B, Sk, Hkv, D, dtype, g, dev), heads(B, Sq, Hq, D, dtype, g, dev)
+    kw = masks(mask, B, Sq, Sk, g, dev)
+    want = reference(q, k, v, see_of(kw, B, Sq, Sk, dev), do=do)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*leaves, **kw)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, do))):
+        check(got, want[name], f"{name} {dtype}")
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D", [64, 80, 128])
 @pytest.mark.parametrize("Hq,Hkv,Sq", [(16, 2, 912), (4, 4, 1000), (32, 1, 48), (8, 2, 6)])

@@ -25,14 +25,17 @@ struct BwdArgs {
   float c, scale;
   uint32_t* info;                 // [pair, row_block] blocks of kInfoWords
   int2* bounds;                   // [pair, row_block] the keys that any row of the block sees
-  int key_tiles, splits, unit;    // a workgroup walks at most `unit` row blocks of a key tile; splits of them cover all
-  Divider by_splits, by_pairs, by_kv, by_group, by_in_group, by_unit, by_tiles;  // by_pairs: of an XCD where they are dealt to XCDs, else all
-  float* part;                    // splits > 1: [pair, split, n_keys, 2, D]
-  int32_t* units;                 // splits > 1: [pair, key tile] the splits that wrote theirs
+  int key_tiles, more, units;     // of a pair: tiles of kKeyTile keys, what cutting them makes more than that at most, and the sum of both
+  Divider by_pairs, by_kv, by_group, by_in_group, by_tiles;  // by_pairs: of an XCD where they are dealt to XCDs, else all
+  int4* list;                     // [pair, unit] key tile (-1: none), row blocks from .. up to, place of its sums (-1: the whole tile)
+  int2* tiles;                    // [pair, key tile] number of its units, place of the first one's sums
+  float* part;                    // [pair, place, kKeyTile, 2, D]
 };
 
 // What the second kernel reads of 32 rows: L, delta, lo and hi of each, then the keys that all rows with keys see.
 constexpr int kInfoWords = 4 * 32 + 4;
+
+constexpr int kKeyTile = 64;
 
 __device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64_t* st, int b, int h, int i) {
   return p + b * st[0] + h * st[1] + i * st[2];
@@ -265,14 +268,77 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   }
 }
 
-// A wavefront holds 32 keys (K and V as B operands, dK^T and dV^T as accumulators) and takes every second block of 32 rows of Q and dO
-// that see them; two such wavefronts make the 64 keys of a workgroup, and the other two take the blocks in between.  S has rows in its
-// registers here and a key per column, so that P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+// What the workgroups of the next kernel do: a workgroup per pair, a lane per key tile, the row blocks dealt to 16 wavefronts.
 //
-// Under a causal mask the first keys are seen by all rows and the last by few: a tile's rows are cut into units of the same
-// length, so that the longest workgroup is a unit and not a tile.  A tile of one unit writes its gradients, the others' units write
-// their sums, which attn_dkv_join_kernel adds up.
-constexpr int kKeyTile = 64;
+// Under a causal mask the first keys are seen by all rows and the last by few, and of a row of packed sequences a tile is seen by those
+// of its own: a tile's row blocks, from the first to the last that sees it, are cut evenly into units of at most as many as make a pair's
+// units about `more` in all (16 where that is fewer), so that the longest workgroup is a unit and not a tile.
+__global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
+  constexpr int kChunk = 4096;
+  __shared__ int s_first[64], s_last[64];
+  __shared__ int2 s_bounds[kChunk];
+  const int pair = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int2* bounds = a.bounds + static_cast<int64_t>(pair) * a.row_blocks;
+  int2* tiles = a.tiles + static_cast<int64_t>(pair) * a.key_tiles;
+  int4* list = a.list + static_cast<int64_t>(pair) * a.units;
+  int work = 0;
+  for (int t0 = 0; t0 == 0 || t0 < a.row_blocks; t0 += kChunk) {
+    const int n = min(a.row_blocks - t0, kChunk);
+    __syncthreads();
+    for (int t = tid; t < n; t += 1024) s_bounds[t] = bounds[t0 + t];
+    for (int c = 0; c < a.key_tiles; c += 64) {
+      const bool mine = tid < 64 && c + lane < a.key_tiles;
+      if (tid < 64) {
+        const int2 before = mine && t0 > 0 ? tiles[c + lane] : int2{0x7fffffff, -1};
+        s_first[tid] = before.x, s_last[tid] = before.y;
+      }
+      __syncthreads();
+      const int k0 = (c + lane) * kKeyTile;
+      int first = 0x7fffffff, last = -1;
+#pragma unroll 4
+      for (int t = tid >> 6; t < n; t += 16) {
+        const int2 x = s_bounds[t];
+        const bool sees = x.x < k0 + kKeyTile && x.y > k0 && x.y > x.x;
+        first = sees ? min(first, t0 + t) : first;
+        last = sees ? t0 + t : last;
+      }
+      atomicMin(&s_first[lane], first);
+      atomicMax(&s_last[lane], last);
+      __syncthreads();
+      if (mine) tiles[c + lane] = int2{s_first[lane], s_last[lane]};
+    }
+  }
+  if (tid >= 64) return;
+  for (int t = lane; t < a.key_tiles; t += 64) work += max(tiles[t].y - tiles[t].x + 1, 0);
+#pragma unroll
+  for (int n = 1; n < 64; n *= 2) work += __shfl_xor(work, n);
+  const int unit = a.more == 0 ? 0x3fffffff : max(16, (work + a.more - 1) / a.more);
+  int next = 0;  // (never past a.units: the full units are no more than a.more, the last ones of the tiles no more than those)
+  for (int c = 0; c < a.key_tiles; c += 64) {
+    const bool is = c + lane < a.key_tiles;
+    const int2 t = is ? tiles[c + lane] : int2{0, 0};
+    const int blocks = max(t.y - t.x + 1, 0);
+    const int units = is ? max((blocks + unit - 1) / unit, 1) : 0;  // (a tile that nothing sees: one of no blocks, which writes zeros)
+    int up_to = units;
+#pragma unroll
+    for (int n = 1; n < 64; n *= 2) {
+      const int x = __shfl_up(up_to, n);
+      if (lane >= n) up_to += x;
+    }
+    const int at = next + up_to - units;
+    const int each = units > 0 ? (blocks + units - 1) / units : 0;
+    for (int u = 0; u < units; ++u)
+      list[at + u] = int4{c + lane, blocks > 0 ? t.x + min(blocks, u * each) : 0, blocks > 0 ? t.x + min(blocks, (u + 1) * each) : 0, units > 1 ? at + u : -1};
+    if (is) tiles[c + lane] = int2{units, at};
+    next += __shfl(up_to, 63);
+  }
+  for (int u = next + lane; u < a.units; u += 64) list[u] = int4{-1, 0, 0, -1};
+}
+
+// A wavefront holds 32 keys (K and V as B operands, dK^T and dV^T as accumulators) and takes every second block of 32 rows of Q and dO
+// of the workgroup's unit; two such wavefronts make the 64 keys of a workgroup, and the other two take the blocks in between.  S has
+// rows in its registers here and a key per column, so that P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+// A tile of one unit writes its gradients, the others' units write their sums, which attn_dkv_join_kernel adds up.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   using T = AttnTile<D>;
@@ -280,7 +346,6 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   constexpr int kSums = T::kOut * 16 * 64 * 4;  // one wavefront's sums of one gradient
   unsigned char* const lds0 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 0>();
   unsigned char* const lds1 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 1>();
-  __shared__ int s_first[4], s_last[4];
   __shared__ u32x4 s_offsets[256];
   // (D = 128: two of V's operands stand in LDS, read in front of their products; with all in registers one was spilled, and the wait
   // for its memory was a wait for the next block's as well)
@@ -289,45 +354,21 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int half = wave & 1, rg = wave >> 1;
   const int pairs = a.batch * a.n_kv;
-  // (the pair varies fastest: dealt to the XCDs by their split, a tile's first units, which are always there, all went to a few)
-  int pair, tile, split;
+  // (the pair varies fastest: dealt to the XCDs by their unit, a tile's first units all went to a few)
+  int pair;
+  int4 todo;
   {
     const int id = blockIdx.x, from = pairs % 8 == 0 ? id >> 3 : id, per = pairs % 8 == 0 ? pairs >> 3 : pairs;
-    const int rest = a.by_pairs.div(from);
-    pair = pairs % 8 == 0 ? (id & 7) + 8 * (from - rest * per) : from - rest * per;
-    tile = a.by_splits.div(rest);
-    split = rest - tile * a.splits + tile;  // (and turned from tile to tile, for few pairs)
-    split -= a.by_splits.div(split) * a.splits;
+    const int unit = a.by_pairs.div(from);
+    pair = pairs % 8 == 0 ? (id & 7) + 8 * (from - unit * per) : from - unit * per;
+    todo = a.list[static_cast<int64_t>(pair) * a.units + unit];
   }
+  const int tile = __builtin_amdgcn_readfirstlane(todo.x), first = __builtin_amdgcn_readfirstlane(todo.y), last = __builtin_amdgcn_readfirstlane(todo.z);
+  if (tile < 0) return;
+  const bool whole = todo.w < 0;
   const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
   const int k0 = tile * kKeyTile, wk = k0 + half * 32, key = wk + (lane & 31);
   const bool live = key < a.n_keys;
-
-  // the row blocks that see any of the workgroup's keys: from the first to the last that does
-  int first = 0x7fffffff, last = -1;
-  {
-    const int2* bounds = a.bounds + static_cast<int64_t>(pair) * a.row_blocks;
-    for (int t = tid; t < a.row_blocks; t += 256) {
-      const int2 x = bounds[t];
-      if (x.x < k0 + kKeyTile && x.y > k0 && x.y > x.x) {
-        first = min(first, t);
-        last = t;
-      }
-    }
-    const int w_first = min(wave_extreme<false>(first), wave_extreme<false>(__shfl_xor(first, 32)));
-    const int w_last = max(wave_extreme<true>(last), wave_extreme<true>(__shfl_xor(last, 32)));
-    if (lane == 0) s_first[wave] = w_first, s_last[wave] = w_last;
-    __syncthreads();
-    first = min(min(s_first[0], s_first[1]), min(s_first[2], s_first[3]));
-    last = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
-  }
-  const int blocks = last < first ? 0 : __builtin_amdgcn_readfirstlane(last - first + 1);
-  const int units = a.by_unit.div(blocks + a.unit - 1);  // (of a tile that nothing sees: none, and its first split writes zeros)
-  if (a.splits > 1 && split == 0 && tid == 0) a.units[static_cast<int64_t>(pair) * a.key_tiles + tile] = units;
-  if (split > 0 && split >= units) return;
-  first = blocks == 0 ? 0 : __builtin_amdgcn_readfirstlane(first + split * a.unit);
-  last = blocks == 0 ? 0 : first + min(a.unit, blocks - split * a.unit);  // blocks [first, last)
-  const bool whole = units <= 1;
 
   const uint16_t* qb = a.q + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[1];
   const uint16_t* gb = a.g + b * a.gs[0] + static_cast<int64_t>(hk) * a.group * a.gs[1];
@@ -493,11 +534,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
       if (32 * o + 8 * (r / 4) < D) bad = bad || dk[o][r] != dk[o][r];
   const float scale = rg == 0 ? a.scale : 1.f;
   uint16_t* const grad = rg == 0 ? a.dk : a.dv;
-  const int64_t part = (static_cast<int64_t>(pair) * a.splits + split) * a.n_keys * 2 * D + rg * D;
+  // (of this unit's first key)
+  float* const part = a.part + (static_cast<int64_t>(pair) * a.units + todo.w) * (kKeyTile * 2 * D) + rg * D;
   if (whole) {
     store_row<DT, D>(dk, scale, live ? grad + ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D : nullptr, lane);
   } else if (live) {
-    float* dst = a.part + part + static_cast<int64_t>(key) * 2 * D;
+    float* dst = part + (key - k0) * 2 * D;
 #pragma unroll
     for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
@@ -548,27 +590,29 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     for (int u = 0; u < 2; ++u)
       if (lane + 64 * u < D) {
         if (whole) grad[((static_cast<int64_t>(b) * a.n_keys + key_r) * a.n_kv + hk) * D + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sum[u] * scale));
-        else a.part[part + static_cast<int64_t>(key_r) * 2 * D + lane + 64 * u] = sum[u];
+        else part[(key_r - k0) * 2 * D + lane + 64 * u] = sum[u];
       }
   }
 }
 
-// dK and dV of the keys of a tile of several units, from the units' sums: a workgroup per tile, a thread per 4 channels.
+// dK and dV of the keys of a tile of several units, from the units' sums: four workgroups per tile, a thread per 4 channels  (one workgroup took 13 us for
+// 316 tiles of 6 units and head size 64, four take 7).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
-  const int pair = a.by_tiles.div(blockIdx.x), tile = blockIdx.x - pair * a.key_tiles;
-  const int units = a.units[static_cast<int64_t>(pair) * a.key_tiles + tile];
-  if (units <= 1) return;
+  const int at = blockIdx.x >> 2, pair = a.by_tiles.div(at), tile = at - pair * a.key_tiles;
+  const int2 of_tile = a.tiles[static_cast<int64_t>(pair) * a.key_tiles + tile];
+  if (of_tile.x <= 1) return;
   const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
-  const int64_t step = static_cast<int64_t>(a.n_keys) * 2 * D;
-  for (int i = threadIdx.x; i < kKeyTile * (2 * D / 4); i += 256) {
+  const float* part = a.part + (static_cast<int64_t>(pair) * a.units + of_tile.y) * (kKeyTile * 2 * D);
+  constexpr int kMine = kKeyTile * (2 * D / 4) / 4;
+  for (int i = (blockIdx.x & 3) * kMine + threadIdx.x; i < ((blockIdx.x & 3) + 1) * kMine; i += 256) {
     const int key = tile * kKeyTile + i / (2 * D / 4), e = i % (2 * D / 4) * 4;
     if (key >= a.n_keys) break;
-    const float* src = a.part + static_cast<int64_t>(pair) * a.splits * step + static_cast<int64_t>(key) * 2 * D + e;
+    const float* src = part + i * 4;
     float4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int u = 0; u < units; ++u) {
-      const float4 x = *reinterpret_cast<const float4*>(src + u * step);
+    for (int u = 0; u < of_tile.x; ++u) {
+      const float4 x = *reinterpret_cast<const float4*>(src + u * (kKeyTile * 2 * D));
       s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
     }
     const float f = e < D ? a.scale : 1.f;
@@ -577,52 +621,54 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
   }
 }
 
-// Units that the rows of a key tile are cut into: about three workgroups to each place on the chip (two to a CU), where the tiles alone
-// are fewer, of at least 16 blocks each.
-int bwd_splits(int64_t pairs, int64_t n_keys, int64_t row_blocks) {
+// Units that a pair's key tiles are cut into beyond one to each: about kUnits workgroups to each place on the chip (two to a CU) of all
+// pairs', where the tiles alone are fewer.  More units end more evenly, fewer write and join fewer sums (64 KB a unit of head size 128).
+// Forward and backward with 1 / 2 / 3 / 4 / 6: 8192 causal tokens of 16 / 2 heads 1464 / 1344 / 1321 / 1339 / 1372 us, 4096 tokens of 16 / 16
+// heads that see all 593 / 594 / 643 / 648 / 672, 16 rows of 912 causal tokens 379 / 384 / 404 / 413 / 442.
+constexpr int kUnits = 2;
+int more_units(int64_t pairs, int64_t n_keys) {
   const int64_t tiles = pairs * ((n_keys + kKeyTile - 1) / kKeyTile), places = 2 * device_cu_count();
-  if (tiles == 0 || tiles >= 3 * places) return 1;
-  const int64_t want = (3 * places + tiles - 1) / tiles, most = row_blocks / 16;
-  const int64_t n = want < most ? want : most;
-  return static_cast<int>(n < 1 ? 1 : (n > 64 ? 64 : n));
+  return tiles == 0 || tiles >= kUnits * places ? 0 : static_cast<int>((kUnits * places + pairs - 1) / pairs);
 }
 
 struct Workspace {
-  size_t info, bounds, units, part, total;
+  size_t info, bounds, tiles, list, part, total;
 };
 Workspace layout(int64_t pairs, int64_t rows, int64_t n_keys, int head_dim) {
-  const int64_t blocks = (rows + 31) / 32;
-  const int splits = bwd_splits(pairs, n_keys, blocks);
+  const size_t blocks = static_cast<size_t>(pairs) * ((rows + 31) / 32), tiles = static_cast<size_t>(pairs) * ((n_keys + kKeyTile - 1) / kKeyTile);
+  const size_t more = static_cast<size_t>(pairs) * more_units(pairs, n_keys);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   Workspace w{};
   w.info = 0;
-  w.bounds = up(static_cast<size_t>(pairs) * blocks * kInfoWords * 4);
-  w.units = w.bounds + up(static_cast<size_t>(pairs) * blocks * sizeof(int2));
-  w.part = w.units + up(static_cast<size_t>(pairs) * ((n_keys + kKeyTile - 1) / kKeyTile) * sizeof(int32_t));
-  w.total = w.part + (splits > 1 ? static_cast<size_t>(pairs) * splits * n_keys * 2 * head_dim * sizeof(float) : 0);
+  w.bounds = up(blocks * kInfoWords * 4);
+  w.tiles = w.bounds + up(blocks * sizeof(int2));
+  w.list = w.tiles + up(tiles * sizeof(int2));
+  w.part = w.list + up((tiles + more) * sizeof(int4));
+  w.total = w.part + (more > 0 ? (tiles + more) * kKeyTile * 2 * head_dim * sizeof(float) : 0);
   return w;
 }
 
 template <int DT, int D>
 int launch_bwd(BwdArgs& a, hipStream_t s) {
   const int64_t pairs = static_cast<int64_t>(a.batch) * a.n_kv;
-  const int64_t row_tiles = pairs * ((a.row_blocks + 3) / 4), key_tiles = pairs * a.key_tiles * a.splits;
-  const int64_t join = a.splits > 1 ? pairs * a.key_tiles : 0;
-  if (row_tiles > 0x7fffffffll || key_tiles > 0x7fffffffll || join > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows");
+  const int64_t row_tiles = pairs * ((a.row_blocks + 3) / 4), units = pairs * a.units;
+  if (row_tiles > 0x7fffffffll || units > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows");
   const int all = static_cast<int>(pairs);
-  a.by_splits = Divider(a.splits), a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_in_group = Divider(a.group < 32 ? a.group : 32);
-  a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all), a.by_unit = Divider(a.unit), a.by_tiles = Divider(a.key_tiles > 0 ? a.key_tiles : 1);
+  a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_in_group = Divider(a.group < 32 ? a.group : 32);
+  a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all), a.by_tiles = Divider(a.key_tiles > 0 ? a.key_tiles : 1);
   const dim3 block(256);
   if (row_tiles > 0) {
     hipLaunchKernelGGL((attn_dq_kernel<DT, D>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
     if (int rc = check_launch("attn_dq_kernel")) return rc;
   }
-  if (key_tiles > 0) {
-    hipLaunchKernelGGL((attn_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(key_tiles)), block, 0, s, a);
+  if (a.key_tiles > 0) {
+    hipLaunchKernelGGL(attn_plan_kernel, dim3(static_cast<unsigned>(pairs)), dim3(1024), 0, s, a);
+    if (int rc = check_launch("attn_plan_kernel")) return rc;
+    hipLaunchKernelGGL((attn_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(units)), block, 0, s, a);
     if (int rc = check_launch("attn_dkv_kernel")) return rc;
   }
-  if (join > 0) {
-    hipLaunchKernelGGL((attn_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(join)), block, 0, s, a);
+  if (a.more > 0) {
+    hipLaunchKernelGGL((attn_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(pairs * a.key_tiles * 4)), block, 0, s, a);
     return check_launch("attn_dkv_join_kernel");
   }
   return WX_OK;
@@ -672,12 +718,13 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   a.c = scale * kLog2e, a.scale = scale;
   const int64_t pairs = batch * n_kv_heads;
   a.key_tiles = (a.n_keys + kKeyTile - 1) / kKeyTile;
-  a.splits = bwd_splits(pairs, n_keys, a.row_blocks);
-  a.unit = a.row_blocks > 0 ? (a.row_blocks + a.splits - 1) / a.splits : 1;
+  a.more = more_units(pairs, n_keys);
+  a.units = a.key_tiles + a.more;
   const Workspace w = layout(pairs, a.rows, n_keys, head_dim);
   if (w.total > 0 && (!workspace || workspace_bytes < w.total)) return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_bwd_workspace_bytes)", who);
   char* ws = static_cast<char*>(workspace);
-  a.info = reinterpret_cast<uint32_t*>(ws + w.info), a.bounds = reinterpret_cast<int2*>(ws + w.bounds), a.units = reinterpret_cast<int32_t*>(ws + w.units), a.part = reinterpret_cast<float*>(ws + w.part);
+  a.info = reinterpret_cast<uint32_t*>(ws + w.info), a.bounds = reinterpret_cast<int2*>(ws + w.bounds), a.tiles = reinterpret_cast<int2*>(ws + w.tiles), a.list = reinterpret_cast<int4*>(ws + w.list);
+  a.part = reinterpret_cast<float*>(ws + w.part);
   hipStream_t s = as_stream(stream);
   if (dtype == WX_BF16) {
     if (head_dim == 64) return launch_bwd<WX_BF16, 64>(a, s);
