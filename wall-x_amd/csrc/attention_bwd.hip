@@ -41,14 +41,16 @@ __device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64
   return p + b * st[0] + h * st[1] + i * st[2];
 }
 
-template <int DT, int D>
+template <int DT, int D, int RW>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   using T = AttnTile<D>;
-  constexpr int KB = 64, kTileBytes = KB * T::kPitch;
+  constexpr int KB = 64, KW = 4 / RW, kTileBytes = KB * T::kPitch;
+  static_assert(KW == 1 || (KW == 2 && RW * T::kOut * 16 * 64 * 4 <= 2 * kTileBytes), "the second key group's sums fit a slot");
   unsigned char *const lds0 = lds_slot<2 * kTileBytes, 0>(), *const lds1 = lds_slot<2 * kTileBytes, 1>();
   __shared__ int2 s_bounds[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int pairs = a.batch * a.n_kv, row_tiles = (a.row_blocks + 3) / 4;
+  const int rw = wave % RW, kw = wave / RW;
+  const int pairs = a.batch * a.n_kv, row_tiles = (a.row_blocks + RW - 1) / RW;
   int pair, tile;
   {
     const int id = blockIdx.x;
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
     }
   }
   const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
-  const int row = tile * 128 + wave * 32 + (lane & 31);
+  const int row = (tile * RW + rw) * 32 + (lane & 31);
   const bool live = row < a.rows;
   const int in_row = live ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
   const MaskRow row_mask = mask_row(a.mask, b, qi, a.n_queries, a.n_keys);
@@ -137,8 +139,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   // (a rest that e5m2 does not hold, of outputs of 10^7 and more, is left out)
   const float delta = some ? both_sum(sums[0] + sums[1]) + (fabsf(rests) < kInf ? rests : 0.f) : 0.f;
   lse = some ? lse : kInf;
-  const int block = tile * 4 + wave;
-  if (block < a.row_blocks) {
+  const int block = tile * RW + rw;
+  if (kw == 0 && block < a.row_blocks) {
     const int64_t at = static_cast<int64_t>(pair) * a.row_blocks + block;
     uint32_t* info = a.info + at * kInfoWords;
     info[(h ? 64 : 0) + (lane & 31)] = h ? static_cast<uint32_t>(lo) : __float_as_uint(lse);
@@ -161,8 +163,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
     if (it + 1 < iters) fetch(it + 1, other);
     const unsigned char* tv = tk + kTileBytes;
 #pragma unroll
-    for (int n = 0; n < KB / 32; ++n) {
-      const int k0 = g_lo + it * KB + 32 * n;
+    for (int i = 0; i < KB / 32 / KW; ++i) {
+      const int n = KW == 1 ? i : kw, k0 = g_lo + it * KB + 32 * n;
       if (k0 >= w_hi || k0 + 32 <= w_lo) continue;
       // A product's operand is asked for kAhead products before it; the second half's powers are found under the first half's products.
       constexpr int kAhead = D == 80 ? 2 : 3, kScores = 2 * T::kSteps, kProducts = 2 * T::kOut;
@@ -214,6 +216,22 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   for (int it = 0; it < iters; it += 2) {
     turn(it, lds0, lds1);
     if (it + 1 < iters) turn(it + 1, lds1, lds0);
+  }
+  if constexpr (KW == 2) {  // the second key group's sums to the first
+    float* const at = reinterpret_cast<float*>(lds0) + rw * (T::kOut * 16 * 64) + lane;
+    __syncthreads();
+    if (kw == 1) {
+#pragma unroll
+      for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) at[(16 * o + r) * 64] = acc[o][r];
+    }
+    __syncthreads();
+    if (kw == 1) return;
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[o][r] += at[(16 * o + r) * 64];
   }
 
   bool bad = false;
@@ -651,14 +669,19 @@ Workspace layout(int64_t pairs, int64_t rows, int64_t n_keys, int head_dim) {
 template <int DT, int D>
 int launch_bwd(BwdArgs& a, hipStream_t s) {
   const int64_t pairs = static_cast<int64_t>(a.batch) * a.n_kv;
-  const int64_t row_tiles = pairs * ((a.row_blocks + 3) / 4), units = pairs * a.units;
+  // Rows that fill 128-row workgroups two to a CU take those, fewer take 64-row ones, whose wavefronts share the keys.  Forward and backward
+  // with 64 / 128: 5003 packed tokens 123 / 133 us, 4096 causal tokens of 8 heads 256 / 281 (472 and 256 large workgroups); 16 x 912 tokens
+  // 410 / 376, 4096 tokens of 16 heads that see all 629 / 610 (1824 and 512).
+  const int row_waves = pairs * ((a.row_blocks + 3) / 4) < 2 * device_cu_count() ? 2 : 4;
+  const int64_t row_tiles = pairs * ((a.row_blocks + row_waves - 1) / row_waves), units = pairs * a.units;
   if (row_tiles > 0x7fffffffll || units > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows");
   const int all = static_cast<int>(pairs);
   a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_in_group = Divider(a.group < 32 ? a.group : 32);
   a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all), a.by_tiles = Divider(a.key_tiles > 0 ? a.key_tiles : 1);
   const dim3 block(256);
   if (row_tiles > 0) {
-    hipLaunchKernelGGL((attn_dq_kernel<DT, D>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
+    if (row_waves == 2) hipLaunchKernelGGL((attn_dq_kernel<DT, D, 2>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
+    else hipLaunchKernelGGL((attn_dq_kernel<DT, D, 4>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
     if (int rc = check_launch("attn_dq_kernel")) return rc;
   }
   if (a.key_tiles > 0) {
