@@ -3,6 +3,7 @@
 // Of each token and key / value head: scale = max |x| / 448 (at least 2^-126), code = e4m3(x / scale), to nearest even.
 // One pass, HBM-bound: 2 D bytes in, D + 4 out, for keys and values alike.  A group of 8 or 16 lanes owns one such row of both (16
 // bytes of each a lane), finds the row's largest magnitude through lane exchanges and stores the 8 codes a lane as 8 bytes.
+#include "attention.h"
 #include "common.h"
 
 namespace wx {
@@ -14,9 +15,10 @@ struct CacheArgs {
   uint8_t *k_cache, *v_cache;  // [batch, n_kv, capacity, D]
   float *k_scale, *v_scale;    // [batch, n_kv, capacity]
   const int32_t *start, *lengths;
-  int64_t rows;                // batch * seq * n_kv
+  int rows;                    // of one of the batch: seq * n_kv
   int n_kv;
-  int64_t seq, capacity;
+  Divider by_kv, by_blocks;    // by_blocks: workgroups to one of the batch
+  int64_t capacity;
 };
 
 // x / scale, correctly rounded: r is 1 / scale to nearest, the remainder of x r is exact in one fused multiply-add
@@ -52,22 +54,22 @@ __device__ __forceinline__ void quantise(const float* x, float& scale, uint32_t 
   }
 }
 
+// A workgroup's rows are of one of the batch, whose start and length are then uniform.  64 x 880 tokens of 2 heads of 128 (66 MB): 14.0 us in
+// the kernel, 4.7 TB/s (17.9 with the rows numbered through in 64 bits and non-temporal
+// loads; two rows to a group of lanes change nothing).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void kv_cache_write_kernel(CacheArgs a) {
-  constexpr int L = D == 64 ? 8 : 16;  // lanes a row (10 of 16 work for D = 80)
-  const int64_t id = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
-  const int c = threadIdx.x % L;
-  if (id >= a.rows) return;  // (a whole group of lanes)
-  const int64_t token = id / a.n_kv;
-  const int hk = static_cast<int>(id - token * a.n_kv);
-  const int64_t b = token / a.seq, s = token - b * a.seq;
-  const int64_t to = static_cast<int64_t>(a.start[b]) + s;
-  if (to < 0 || to >= a.capacity || (a.lengths != nullptr && s >= a.lengths[b])) return;
+  constexpr int L = D == 64 ? 8 : 16, kGroups = 256 / L;  // lanes a row (10 of 16 work for D = 80)
+  const int b = a.by_blocks.div(blockIdx.x), c = threadIdx.x % L;
+  const int at = (static_cast<int>(blockIdx.x) - b * static_cast<int>(a.by_blocks.d)) * kGroups + static_cast<int>(threadIdx.x) / L;
+  const int s = a.by_kv.div(at), hk = at - s * a.n_kv;
+  const int64_t pos = static_cast<int64_t>(a.start[b]) + s;
+  if (at >= a.rows || pos < 0 || pos >= a.capacity || (a.lengths != nullptr && s >= a.lengths[b])) return;  // (a whole group of lanes)
   const bool mine = c * 8 < D;
   float xk[8] = {}, xv[8] = {};
   if (mine) {
-    const u32x4 k = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.k + b * a.ks[0] + hk * a.ks[1] + s * a.ks[2] + 8 * c));
-    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.v + b * a.vs[0] + hk * a.vs[1] + s * a.vs[2] + 8 * c));
+    const u32x4 k = *reinterpret_cast<const u32x4*>(a.k + b * a.ks[0] + hk * a.ks[1] + s * a.ks[2] + 8 * c);
+    const u32x4 v = *reinterpret_cast<const u32x4*>(a.v + b * a.vs[0] + hk * a.vs[1] + s * a.vs[2] + 8 * c);
     unpack16<DT>(k, xk);
     unpack16<DT>(v, xv);
   }
@@ -75,7 +77,7 @@ __global__ __launch_bounds__(256) void kv_cache_write_kernel(CacheArgs a) {
   uint32_t kc[2], vc[2];
   quantise<DT, L>(xk, k_scale, kc);
   quantise<DT, L>(xv, v_scale, vc);
-  const int64_t row = (b * a.n_kv + hk) * a.capacity + to;
+  const int64_t row = (static_cast<int64_t>(b) * a.n_kv + hk) * a.capacity + pos;
   if (mine) {
     *reinterpret_cast<uint2*>(a.k_cache + row * D + 8 * c) = uint2{kc[0], kc[1]};
     *reinterpret_cast<uint2*>(a.v_cache + row * D + 8 * c) = uint2{vc[0], vc[1]};
@@ -106,14 +108,15 @@ extern "C" int wx_kv_cache_write(const void* k, const void* v, void* k_cache, vo
     if (reinterpret_cast<uintptr_t>(p) & 15) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0) return fail(WX_ERR_UNSUPPORTED, "%s: strides must keep rows 16-byte aligned", who);
-  if (seq > 0x7fffffffll || batch > 0x7fffffffll / seq) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  if (seq > 0x7fffffffll / n_kv_heads || batch > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
   CacheArgs a{};
   a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
   for (int i = 0; i < 3; ++i) a.ks[i] = k_strides[i], a.vs[i] = v_strides[i];
   a.k_cache = static_cast<uint8_t*>(k_cache), a.v_cache = static_cast<uint8_t*>(v_cache), a.k_scale = k_scale, a.v_scale = v_scale;
   a.start = start, a.lengths = lengths;
-  a.rows = batch * seq * n_kv_heads, a.n_kv = n_kv_heads, a.seq = seq, a.capacity = capacity;
-  const int64_t lanes = head_dim == 64 ? 8 : 16, blocks = (a.rows + 256 / lanes - 1) / (256 / lanes);
+  a.rows = static_cast<int>(seq * n_kv_heads), a.n_kv = n_kv_heads, a.capacity = capacity;
+  const int64_t each = 256 / (head_dim == 64 ? 8 : 16), of_one = (a.rows + each - 1) / each, blocks = batch * of_one;
+  a.by_kv = Divider(n_kv_heads), a.by_blocks = Divider(static_cast<uint32_t>(of_one));
   if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
   hipStream_t s = as_stream(stream);
