@@ -54,9 +54,9 @@ __device__ __forceinline__ void quantise(const float* x, float& scale, uint32_t 
   }
 }
 
-// A workgroup's rows are of one of the batch, whose start and length are then uniform.  64 x 880 tokens of 2 heads of 128 (66 MB): 14.0 us in
-// the kernel, 4.7 TB/s (17.9 with the rows numbered through in 64 bits and non-temporal
-// loads; two rows to a group of lanes change nothing).
+// A workgroup's rows are of one of the batch, whose start and length are then uniform.  64 x 880 tokens of 2 heads of 128 (66 MB): 14.0 us
+// in the kernel, 4.7 TB/s (17.9 with the rows numbered through in 64 bits and non-temporal loads; two rows to a group of lanes change
+// nothing).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void kv_cache_write_kernel(CacheArgs a) {
   constexpr int L = D == 64 ? 8 : 16, kGroups = 256 / L;  // lanes a row (10 of 16 work for D = 80)
