@@ -84,7 +84,7 @@ __device__ __forceinline__ void plain_row(const FwdArgs& a, int b, int hk, int r
 // e4m3 tiles are widened to the compute type on their way to LDS (exactly); their scales multiply the scores and the
 // probabilities, a value per key.
 template <int DT, int D, bool F8, int RW>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
   using T = AttnTile<D>;
   constexpr int KW = 4 / RW, KB = RW == 4 ? 64 : 32, NT = KB / 32;
   constexpr bool kDirect = !F8 && RW > 1;
