@@ -1,5 +1,8 @@
 // Attention forward: O = softmax(scale Q K^T over the keys of each query's range) V, one pass over the keys with a running
 // maximum and sum, for keys and values in the queries' type or quantised to e4m3 with a scale per token (gfx950).
+#include <algorithm>
+#include <cmath>
+
 #include "attention.h"
 
 namespace wx {
@@ -15,7 +18,7 @@ struct FwdArgs {
   AttnMask mask;
   int batch, n_q, n_kv, n_queries, n_keys, group;
   int rows, row_tiles, splits;
-  Divider by_splits, by_pairs, by_kv, by_group;  // by_pairs: of an XCD where they are dealt to XCDs, else all
+  Divider by_splits, by_pairs, by_kv, by_group, by_rows;  // by_pairs: of an XCD where they are dealt to XCDs, else all
   float c;                       // scale * log2(e)
   float* part;                   // splits > 1: [pair, split, rows, D] sums, then [pair, split, rows] (maximum, sum)
 };
@@ -79,23 +82,30 @@ __device__ __forceinline__ void plain_row(const FwdArgs& a, int b, int hk, int r
 
 // RW of the workgroup's four wavefronts take 32 rows each; the other factor, KW = 4 / RW, shares the keys: wavefront group kw
 // takes every KW-th tile of KB keys, and the groups' sums are joined in LDS at the end.
-// Many rows (RW = 4): a tile of 64 keys serves 128 rows, loaded straight to LDS one tile ahead.  Few rows (RW = 1): 32 rows, four
-// tiles in flight per workgroup, each loaded through its wavefront's registers (no barrier in the loop).
-// e4m3 tiles are widened to the compute type on their way to LDS (exactly); their scales multiply the scores and the
-// probabilities, a value per key.
+// Many rows (RW = 4): a tile of 64 keys serves 128 rows.  Fewer (RW = 2): two tiles of 32 keys at a time serve 64 rows each.  Tiles
+// are loaded one ahead, straight to LDS; e4m3 ones through registers, where they are widened to the compute type (exactly); their
+// scales multiply the scores and the probabilities, a value per key.  (A form whose four wavefronts each walked tiles of their own for 32
+// rows, without a barrier, was no faster for single queries: 38 against 35 us over 8 x 32768 cached keys.)
+//
+// What bounds it: a step of 64 keys by 128 rows at head size 128 takes some 3600 cycles a CU with two workgroups, in which the matrix
+// units work 2048, the vector units about 2800 (a power is four passes) and LDS moves 384 KB (3072 cycles).  16384 causal tokens of
+// 16 / 2 heads of 128: 1.0 ms, 1.1 PFLOP/s, with the clock held at 1.8 GHz by its power (a large library product in the same type: 1.36
+// PFLOP/s); 16 rows of 912 tokens: 75 us, 0.64 PFLOP/s, of which the workgroups' first 10 thousand cycles, up to the first
+// product, are a quarter.  Over a cache it reads 112 MB for single queries in 27 us (4.1 TB/s) and joins them in 4.
+// (Heads of 80: 168 registers, one less than it would take, let three workgroups share a CU: 48 x 1024 patches in windows 131 us
+// instead of 136, 8 x 2000 causal tokens 126 instead of 132.  The others' sums and tiles leave two.)
 template <int DT, int D, bool F8, int RW>
 __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
   using T = AttnTile<D>;
   constexpr int KW = 4 / RW, KB = RW == 4 ? 64 : 32, NT = KB / 32;
-  constexpr bool kDirect = !F8 && RW > 1;
-  constexpr int kBufs = RW == 1 ? 1 : 2;
+  constexpr bool kDirect = !F8;
   constexpr int kTileBytes = KB * T::kPitch;
   constexpr int kScaleBytes = F8 ? 2 * KB * 4 : 0;
   constexpr int kSlot = 2 * kTileBytes + kScaleBytes;
   constexpr int kTiles = KW * kSlot;                                      // of one buffer
   constexpr int kJoinStats = 4 * 32 * (64 + 4) * 4, kJoin = KW > 1 ? kJoinStats + 4 * 32 * 8 : 0;  // 64 channels at a time
   unsigned char* const lds = lds_slot<(kTiles > kJoin ? kTiles : kJoin), 0>();
-  unsigned char* const lds1 = lds_slot<(kBufs == 2 ? kTiles : 16), 1>();
+  unsigned char* const lds1 = lds_slot<kTiles, 1>();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave % RW, kw = wave / RW, h = lane >> 5;
 
@@ -139,20 +149,17 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
   const int f_lo = wave_extreme<true>(some ? lo : 0), f_hi = wave_extreme<false>(some ? hi : 0x7fffffff);  // every row that sees something sees [f_lo, f_hi)
   if (w_lo > w_hi) w_lo = w_hi;
   // the workgroup's keys
-  int g_lo = w_lo, g_hi = w_hi;
-  if constexpr (RW > 1) {
-    __shared__ int2 bounds[RW];
-    if (kw == 0 && lane == 0) bounds[rw] = int2{w_hi > w_lo ? w_lo : 0x7fffffff, w_hi};
-    attn_lds_barrier();
-    g_lo = 0x7fffffff, g_hi = 0;
+  __shared__ int2 bounds[RW];
+  if (kw == 0 && lane == 0) bounds[rw] = int2{w_hi > w_lo ? w_lo : 0x7fffffff, w_hi};
+  attn_lds_barrier();
+  int g_lo = 0x7fffffff, g_hi = 0;
 #pragma unroll
-    for (int u = 0; u < RW; ++u) {
-      g_lo = min(g_lo, bounds[u].x);
-      g_hi = max(g_hi, bounds[u].y);
-    }
-    g_lo = __builtin_amdgcn_readfirstlane(min(g_lo, g_hi));
-    g_hi = __builtin_amdgcn_readfirstlane(g_hi);
+  for (int u = 0; u < RW; ++u) {
+    g_lo = min(g_lo, bounds[u].x);
+    g_hi = max(g_hi, bounds[u].y);
   }
+  g_lo = __builtin_amdgcn_readfirstlane(min(g_lo, g_hi));
+  g_hi = __builtin_amdgcn_readfirstlane(g_hi);
   {  // this split's share of the tiles
     const int n = (g_hi - g_lo + KB - 1) / KB;
     const int each = a.by_splits.div(n), more = n - each * a.splits;  // the first `more` splits take one more
@@ -189,7 +196,6 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
   auto key0 = [&](int it) { return g_lo + (it * KW + kw) * KB; };
   auto fetch = [&](int it, unsigned char* slot) {  // a tile on its way: to LDS, or into registers
     const int k0 = key0(it), left = g_hi - k0;  // (may be <= 0: zeros)
-    if (left <= 0 && RW == 1) return;
     const int64_t at = left > 0 ? k0 : 0;
     const auto rk = attn_rsrc(kp + at * k_step, kRsrcBytes), rv = attn_rsrc(vp + at * v_step, kRsrcBytes);
     if constexpr (kDirect) {
@@ -348,7 +354,7 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
     l += sums[0] + sums[1];
   };
 
-  unsigned char *mine = lds + kw * kSlot, *other_slot = lds1 + (kBufs == 2 ? kw * kSlot : 0);
+  unsigned char *mine = lds + kw * kSlot, *other_slot = lds1 + kw * kSlot;
   if (iters > 0) fetch(0, mine);
   auto turn = [&](int it, unsigned char* slot, unsigned char* other) {
     const int k0 = key0(it);
@@ -357,20 +363,16 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
       attn_barrier();
       if (it + 1 < iters) fetch(it + 1, other);
     } else {
-      if (RW > 1 || k0 < g_hi) put(slot);
+      put(slot);
       if (it + 1 < iters) fetch(it + 1, other);
       wait_lds();
-      if constexpr (RW > 1) attn_barrier();
+      attn_barrier();
     }
     if (k0 < w_hi && k0 + KB > w_lo && k0 < g_hi) step(slot, k0);
   };
-  if constexpr (kBufs == 1) {
-    for (int it = 0; it < iters; ++it) turn(it, mine, mine);
-  } else {
-    for (int it = 0; it < iters; it += 2) {
-      turn(it, mine, other_slot);
-      if (it + 1 < iters) turn(it + 1, other_slot, mine);
-    }
+  for (int it = 0; it < iters; it += 2) {
+    turn(it, mine, other_slot);
+    if (it + 1 < iters) turn(it + 1, other_slot, mine);
   }
   l = both_sum(l);
 
@@ -507,32 +509,43 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
 
 constexpr int kMaxSplits = 256;
 
-// Joins the splits of a row: a workgroup per row, every wavefront a quarter of the splits, lane l channels l and l + 64.
-// (A wavefront per row took 24 us for 128 rows of 32 splits: one dependent load after the other.)
-template <int DT, int D>
+// Joins the splits of a row, lane l channels l and l + 64.  ROWS = 4: a wavefront per row, for a few splits of many rows (a workgroup per
+// row took 26 us for 8000 rows of 3 splits).  ROWS = 1: a workgroup per row, every wavefront a quarter of the splits, for many (a
+// wavefront per row took 24 us for 128 rows of 32 splits: one dependent load after the other).
+template <int DT, int D, int ROWS>
 __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
   __shared__ float s_top[4], s_sum[4], s_weight[kMaxSplits], s_out[4][128];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t at = blockIdx.x;
-  const int pair = static_cast<int>(at / a.rows), row = static_cast<int>(at - static_cast<int64_t>(pair) * a.rows);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * ROWS + (ROWS == 4 ? wave : 0);
+  if (at >= static_cast<int64_t>(a.batch) * a.n_kv * a.rows) return;
+  const int pair = a.by_rows.div(static_cast<int>(at)), row = static_cast<int>(at) - pair * a.rows;
   const float2* stats = part_stats(a, D) + static_cast<int64_t>(pair) * a.splits * a.rows + row;
   const float* part = a.part + (static_cast<int64_t>(pair) * a.splits * a.rows + row) * D;
-  const float2 st = tid < a.splits ? stats[static_cast<int64_t>(tid) * a.rows] : float2{-kInf, 0.f};
-  const float wave_top = wave_max(st.x);
-  if (lane == 0) s_top[wave] = wave_top;
-  __syncthreads();
-  const float top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const int mine = ROWS == 4 ? lane : tid;
+  const float2 st = mine < a.splits ? stats[static_cast<int64_t>(mine) * a.rows] : float2{-kInf, 0.f};
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
+  const int i = a.by_group.div(row), hq = hk * a.group + row - i * a.group;
+  int lo, hi;
+  key_range(a.mask, b, i, a.n_queries, a.n_keys, lo, hi);
+  float top = wave_max(st.x);
+  if constexpr (ROWS == 1) {
+    if (lane == 0) s_top[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  }
   // (a split that the row sees nothing of has no part, whatever stands in its place)
   const float f = st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c);
-  s_weight[tid] = f;
-  const float wave_l = wave_sum(st.y * f);
-  if (lane == 0) s_sum[wave] = wave_l;
-  __syncthreads();
-  const float l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  float l = wave_sum(st.y * f);
+  if constexpr (ROWS == 1) {
+    s_weight[tid] = f;
+    if (lane == 0) s_sum[wave] = l;
+    __syncthreads();
+    l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  }
   float o[2] = {0.f, 0.f};
 #pragma unroll 4
-  for (int s = wave; s < a.splits; s += 4) {
-    const float w = s_weight[s];
+  for (int s = ROWS == 4 ? 0 : wave; s < a.splits; s += ROWS == 4 ? 1 : 4) {
+    const float w = ROWS == 4 ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s)) : s_weight[s];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       if (lane + 64 * u < D) {
@@ -540,39 +553,48 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
         o[u] += w == 0.f ? 0.f : x * w;
       }
   }
-#pragma unroll
-  for (int u = 0; u < 2; ++u) s_out[wave][lane + 64 * u] = o[u];
-  __syncthreads();
-  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
-  const int i = a.by_group.div(row), hq = hk * a.group + row - i * a.group;
-  int lo, hi;
-  key_range(a.mask, b, i, a.n_queries, a.n_keys, lo, hi);
-  if (tid < D) {
-    const float sum = (s_out[0][tid] + s_out[1][tid]) + (s_out[2][tid] + s_out[3][tid]);
-    const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D + tid;
+  const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D;
+  auto store = [&](int c, float sum) {
     const float x = hi > lo ? sum / l : 0.f;
-    a.out[to] = static_cast<uint16_t>(Elem<DT>::store(x));
-    if (a.rest != nullptr) a.rest[to] = static_cast<uint8_t>(pack_rest(rest_of<DT>(x), 0.f, 0.f, 0.f));
+    a.out[to + c] = static_cast<uint16_t>(Elem<DT>::store(x));
+    if (a.rest != nullptr) a.rest[to + c] = static_cast<uint8_t>(pack_rest(rest_of<DT>(x), 0.f, 0.f, 0.f));
+  };
+  if constexpr (ROWS == 4) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 64 * u < D) store(lane + 64 * u, o[u]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s_out[wave][lane + 64 * u] = o[u];
+    __syncthreads();
+    if (tid < D) store(tid, (s_out[0][tid] + s_out[1][tid]) + (s_out[2][tid] + s_out[3][tid]));
   }
-  if (a.lse != nullptr && tid == 0) a.lse[at] = hi > lo ? __builtin_fmaf(top, a.c, __builtin_amdgcn_logf(l)) : kInf;
+  if (a.lse != nullptr && (ROWS == 4 ? lane : tid) == 0) a.lse[at] = hi > lo ? __builtin_fmaf(top, a.c, __builtin_amdgcn_logf(l)) : kInf;
 }
 
 // How a call is spread over the chip: wavefronts of the workgroup that take rows (4, 2 or 1), and splits of the keys.
 struct FwdPlan {
   int row_waves, splits;
 };
-FwdPlan plan(int64_t pairs, int64_t rows, int64_t keys) {
+FwdPlan plan(int64_t pairs, int64_t rows, int64_t keys, int head_dim) {
   const int cus = device_cu_count();
   FwdPlan p{4, 1};
-  // Rows that fill 128-row workgroups two to a CU take those; otherwise smaller row tiles, whose wavefronts share the keys.
-  if (rows <= 32) p.row_waves = 1;
-  else if (rows <= 64 || pairs * ((rows + 127) / 128) < 2 * cus) p.row_waves = 2;
+  // Rows that fill 128-row workgroups two to a CU take those, fewer take 64-row ones, whose two pairs of wavefronts share the keys.  With
+  // 64 / 128: 5003 packed tokens of 12 / 4 heads of 64 28 / 38 us (472 large workgroups); 16 x 912 tokens of 16 / 2 heads of 128 107 / 74,
+  // 48 x 1024 patches of 16 heads of 80 in windows 203 / 131 (1824 and 6144).
+  if (rows <= 64 || pairs * ((rows + 127) / 128) < 2 * cus) p.row_waves = 2;
   const int64_t groups = pairs * ((rows + 32 * p.row_waves - 1) / (32 * p.row_waves));
   if (p.row_waves < 4 && groups > 0 && groups < 2 * cus) {
-    // too few workgroups for the chip: the keys in parts of at least two tiles for each of a workgroup's key groups
-    const int64_t want = (2 * cus + groups - 1) / groups, most = keys / (32 * (4 / p.row_waves) * 2);
-    const int64_t n = want < most ? want : most;
-    p.splits = static_cast<int>(n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n));
+    // Too few workgroups for the chip: the keys in n parts, up to two workgroups to a CU, of at least a tile for each key group.  A tile
+    // of 64 keys takes about 0.8 us, the join 4, and writing and reading the parts of n splits n times what one's take at 3 TB/s: the n of
+    // the least sum, if that is less than without.  Measured without / with: one query of 8 heads over 8 x 32768 cached keys of 2 heads 35 us
+    // in 32 parts, 40 over 64; 4 x 300 causal tokens of 16 / 2 heads 11 / 28 (2 parts), 2000 tokens 37 / 48 (2), 32 x 5 queries over 2400
+    // to 3000 cached keys of 8 heads of 64 45 / 33 (2).
+    const double tiles = 0.8 * (keys / 64.0), each = static_cast<double>(pairs) * rows * head_dim * 8 / 3e6;
+    const int64_t want = (2 * cus + groups - 1) / groups, most = keys / 64;
+    int64_t n = static_cast<int64_t>(std::sqrt(tiles / each));
+    n = std::min({n, want, most, static_cast<int64_t>(kMaxSplits)});
+    if (n > 1 && tiles / n + 4 + n * each < tiles) p.splits = static_cast<int>(n);
   }
   return p;
 }
@@ -586,16 +608,15 @@ int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
   const int64_t blocks = static_cast<int64_t>(a.batch) * a.n_kv * a.row_tiles * a.splits;
   if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
-  switch (p.row_waves) {
-    case 1: hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 1>), grid, block, 0, s, a); break;
-    case 2: hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 2>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 4>), grid, block, 0, s, a); break;
-  }
+  if (p.row_waves == 2) hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 2>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 4>), grid, block, 0, s, a);
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
   if (a.splits > 1) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.n_kv * a.rows;
     if (rows > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
-    hipLaunchKernelGGL((attn_join_kernel<DT, D>), dim3(static_cast<unsigned>(rows)), block, 0, s, a);
+    a.by_rows = Divider(a.rows);
+    if (a.splits <= 8) hipLaunchKernelGGL((attn_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>((rows + 3) / 4)), block, 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<DT, D, 1>), dim3(static_cast<unsigned>(rows)), block, 0, s, a);
     return check_launch("attn_join_kernel");
   }
   return WX_OK;
@@ -652,7 +673,7 @@ extern "C" size_t wx_attention_workspace_bytes(int64_t batch, int n_q_heads, int
                                                int head_dim) {
   if (batch <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_queries <= 0 || n_keys < 0 || head_dim <= 0) return 0;
   const int64_t rows = n_queries * (n_q_heads / n_kv_heads);
-  const FwdPlan p = plan(batch * n_kv_heads, rows, n_keys);
+  const FwdPlan p = plan(batch * n_kv_heads, rows, n_keys, head_dim);
   return p.splits == 1 ? 0 : static_cast<size_t>(batch) * n_kv_heads * p.splits * rows * (head_dim + 2) * sizeof(float);
 }
 
@@ -679,7 +700,7 @@ static int forward(const char* who, const void* q, const void* k, const void* v,
   a.batch = static_cast<int>(batch), a.n_q = n_q, a.n_kv = n_kv, a.n_queries = static_cast<int>(n_queries), a.n_keys = static_cast<int>(n_keys);
   a.group = group, a.rows = static_cast<int>(n_queries) * group;
   a.c = scale * kLog2e;
-  const FwdPlan p = plan(batch * n_kv, a.rows, n_keys);
+  const FwdPlan p = plan(batch * n_kv, a.rows, n_keys, head_dim);
   if (p.splits > 1) {
     if (!workspace || workspace_bytes < wx_attention_workspace_bytes(batch, n_q, n_kv, n_queries, n_keys, head_dim))
       return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_workspace_bytes)", who);
