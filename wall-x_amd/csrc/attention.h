@@ -60,6 +60,46 @@ __device__ __forceinline__ void key_range(const AttnMask& m, int b, int i, int n
   key_range(m, mask_row(m, b, i, n_queries, n_keys), i, n_queries, n_keys, lo, hi);
 }
 
+// n / d for n < 2^31 by a multiplication: the host makes the factor (a division by a number from memory is some 20 instructions,
+// and a workgroup's coordinates take half a dozen).
+struct Divider {
+  uint32_t d, factor, shift;
+  Divider() = default;
+  explicit Divider(uint32_t by) : d(by) {
+    shift = 0;
+    while ((1ull << shift) < by) ++shift;
+    factor = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), factor) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
+// Workgroup -> (pair, tile of it), the last tiles first: under a causal mask they are the longest.  Where the pairs divide by 8 every XCD
+// gets an eighth of them, in a row: their keys are read into one L2, and heads of 80, whose rows share cache lines with the next
+// head's, into no second one (48 x 1024 patches in windows 120 us; 132 with the pairs dealt round).  Of many pairs `wide` at a time, so that
+// their keys stay in that L2.
+struct Spread {
+  int pairs, wide, tiles;
+  Divider by_pass, by_wide;
+  Spread() = default;
+  Spread(int pairs_, int tiles_) : pairs(pairs_), wide(pairs_ % 8 == 0 ? pairs_ / 8 : pairs_), tiles(tiles_) {
+    if (pairs % 8 == 0 && wide > 8)
+      for (int n = 8; n >= 4; --n)
+        if (wide % n == 0) {
+          wide = n;
+          break;
+        }
+    by_pass = Divider(static_cast<uint32_t>(wide) * tiles), by_wide = Divider(wide);
+  }
+  __device__ __forceinline__ void place(int id, int& pair, int& tile) const {
+    const bool dealt = pairs % 8 == 0;
+    const int j = dealt ? id >> 3 : id, pass = by_pass.div(j), rest = j - pass * static_cast<int>(by_pass.d), t = by_wide.div(rest);
+    pair = (dealt ? (id & 7) * (pairs >> 3) : 0) + pass * wide + rest - t * wide;
+    tile = tiles - 1 - t;
+  }
+};
+
 template <int D>
 struct AttnTile {
   static constexpr int kPitch = D == 64 ? 128 : (D == 80 ? 192 : 256);
@@ -148,21 +188,6 @@ __device__ __forceinline__ int wave_extreme(int x) {
   const int a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
   return MAX ? max(a, b) : min(a, b);
 }
-
-// n / d for n < 2^31 by a multiplication: the host makes the factor (a division by a number from memory is some 20 instructions,
-// and a workgroup's coordinates take half a dozen).
-struct Divider {
-  uint32_t d, factor, shift;
-  Divider() = default;
-  explicit Divider(uint32_t by) : d(by) {
-    shift = 0;
-    while ((1ull << shift) < by) ++shift;
-    factor = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
-  }
-  __device__ __forceinline__ int div(int n) const {
-    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), factor) + static_cast<uint32_t>(n)) >> shift);
-  }
-};
 
 // Byte offsets, in a tile, of what a lane reads of its first block: the other blocks lie at constant distances and exclusive-ors.
 //   rows  A operand, contraction over the head: row lane & 31 of 32 rows, channels 16 t + 8 h .. + 7 of step t

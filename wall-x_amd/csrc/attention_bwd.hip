@@ -27,6 +27,7 @@ struct BwdArgs {
   int2* bounds;                   // [pair, row_block] the keys that any row of the block sees
   int key_tiles, more, units;     // of a pair: tiles of kKeyTile keys, what cutting them makes more than that at most, and the sum of both
   Divider by_pairs, by_kv, by_group, by_in_group, by_tiles;  // by_pairs: of an XCD where they are dealt to XCDs, else all
+  Spread spread;                  // of dQ's row tiles
   int4* list;                     // [pair, unit] key tile (-1: none), row blocks from .. up to, place of its sums (-1: the whole tile)
   int2* tiles;                    // [pair, key tile] number of its units, place of the first one's sums
   float* part;                    // [pair, place, kKeyTile, 2, D]
@@ -50,20 +51,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   __shared__ int2 s_bounds[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int rw = wave % RW, kw = wave / RW;
-  const int pairs = a.batch * a.n_kv, row_tiles = (a.row_blocks + RW - 1) / RW;
   int pair, tile;
-  {
-    const int id = blockIdx.x;
-    if (pairs % 8 == 0) {
-      const int j = id >> 3, t = a.by_pairs.div(j);
-      pair = (id & 7) + 8 * (j - t * (pairs >> 3));
-      tile = row_tiles - 1 - t;
-    } else {
-      const int t = a.by_pairs.div(id);
-      pair = id - t * pairs;
-      tile = row_tiles - 1 - t;
-    }
-  }
+  a.spread.place(blockIdx.x, pair, tile);
   const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
   const int row = (tile * RW + rw) * 32 + (lane & 31);
   const bool live = row < a.rows;
@@ -378,7 +367,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   {
     const int id = blockIdx.x, from = pairs % 8 == 0 ? id >> 3 : id, per = pairs % 8 == 0 ? pairs >> 3 : pairs;
     const int unit = a.by_pairs.div(from);
-    pair = pairs % 8 == 0 ? (id & 7) + 8 * (from - unit * per) : from - unit * per;
+    pair = pairs % 8 == 0 ? (id & 7) * per + (from - unit * per) : from - unit * per;
     todo = a.list[static_cast<int64_t>(pair) * a.units + unit];
   }
   const int tile = __builtin_amdgcn_readfirstlane(todo.x), first = __builtin_amdgcn_readfirstlane(todo.y), last = __builtin_amdgcn_readfirstlane(todo.z);
@@ -680,6 +669,7 @@ int launch_bwd(BwdArgs& a, hipStream_t s) {
   a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all), a.by_tiles = Divider(a.key_tiles > 0 ? a.key_tiles : 1);
   const dim3 block(256);
   if (row_tiles > 0) {
+    a.spread = Spread(all, (a.row_blocks + row_waves - 1) / row_waves);
     if (row_waves == 2) hipLaunchKernelGGL((attn_dq_kernel<DT, D, 2>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
     else hipLaunchKernelGGL((attn_dq_kernel<DT, D, 4>), dim3(static_cast<unsigned>(row_tiles)), block, 0, s, a);
     if (int rc = check_launch("attn_dq_kernel")) return rc;

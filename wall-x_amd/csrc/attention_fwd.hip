@@ -18,7 +18,8 @@ struct FwdArgs {
   AttnMask mask;
   int batch, n_q, n_kv, n_queries, n_keys, group;
   int rows, row_tiles, splits;
-  Divider by_splits, by_pairs, by_kv, by_group, by_rows;  // by_pairs: of an XCD where they are dealt to XCDs, else all
+  Divider by_splits, by_kv, by_group, by_rows;
+  Spread spread;
   float c;                       // scale * log2(e)
   float* part;                   // splits > 1: [pair, split, rows, D] sums, then [pair, split, rows] (maximum, sum)
 };
@@ -109,24 +110,13 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave % RW, kw = wave / RW, h = lane >> 5;
 
-  // Workgroup -> (pair, row tile, split).  Neighbouring workgroups go to different XCDs: with many pairs each XCD keeps its own
-  // pairs, whose keys then stay in its L2.  The last row tiles first: under a causal mask they are the longest.
-  const int pairs = a.batch * a.n_kv;
   int pair, tile, split;
   {
     int id = blockIdx.x;
     const int rest = a.by_splits.div(id);
     split = id - rest * a.splits;
     id = rest;
-    if (pairs % 8 == 0) {
-      const int j = id >> 3, t = a.by_pairs.div(j);
-      pair = (id & 7) + 8 * (j - t * (pairs >> 3));
-      tile = a.row_tiles - 1 - t;
-    } else {
-      const int t = a.by_pairs.div(id);
-      pair = id - t * pairs;
-      tile = a.row_tiles - 1 - t;
-    }
+    a.spread.place(id, pair, tile);
   }
   const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
   const int row = tile * 32 * RW + rw * 32 + (lane & 31);
@@ -604,7 +594,8 @@ int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
   a.splits = p.splits;
   a.row_tiles = (a.rows + 32 * p.row_waves - 1) / (32 * p.row_waves);
   const int pairs = a.batch * a.n_kv;
-  a.by_splits = Divider(p.splits), a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_pairs = Divider(pairs % 8 == 0 ? pairs / 8 : pairs);
+  a.by_splits = Divider(p.splits), a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group);
+  a.spread = Spread(pairs, a.row_tiles);
   const int64_t blocks = static_cast<int64_t>(a.batch) * a.n_kv * a.row_tiles * a.splits;
   if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
