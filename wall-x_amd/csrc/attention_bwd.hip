@@ -3,6 +3,10 @@
 // Two kernels, seven matrix products in place of the five that share one pass: the first walks the keys of a tile of rows (dQ),
 // the second the rows of a tile of keys (dK, dV, all heads of the group in turn).  Every sum is then one wavefront's own, in a
 // fixed order: no atomics, the same gradients every time.
+//
+// 16 rows of 912 causal tokens of 16 / 2 heads of 128 (72 GFLOP in three products, 96 in four): dQ 124 us, 0.58 PFLOP/s, matrix units busy
+// 31 % (the rows' four operands are on their way for a third of it); the plan 5; dK and dV 153 us, 0.63 PFLOP/s, 40 %, reading 0.6 GB of
+// which half is in L2; the join 15.  5003 packed tokens of 12 / 4 heads of 64: 29, 8, 39 and 7 us.
 #include "attention.h"
 
 namespace wx {
@@ -602,8 +606,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   }
 }
 
-// dK and dV of the keys of a tile of several units, from the units' sums: four workgroups per tile, a thread per 4 channels  (one workgroup took 13 us for
-// 316 tiles of 6 units and head size 64, four take 7).
+// dK and dV of the keys of a tile of several units, from the units' sums: four workgroups per tile, a thread per 4 channels (one
+// workgroup took 13 us for 316 tiles of 6 units and head size 64, four take 7).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
   const int at = blockIdx.x >> 2, pair = a.by_tiles.div(at), tile = at - pair * a.key_tiles;

@@ -88,11 +88,12 @@ __device__ __forceinline__ void plain_row(const FwdArgs& a, int b, int hk, int r
 // scales multiply the scores and the probabilities, a value per key.  (A form whose four wavefronts each walked tiles of their own for 32
 // rows, without a barrier, was no faster for single queries: 38 against 35 us over 8 x 32768 cached keys.)
 //
-// What bounds it: a step of 64 keys by 128 rows at head size 128 takes some 3600 cycles a CU with two workgroups, in which the matrix
-// units work 2048, the vector units about 2800 (a power is four passes) and LDS moves 384 KB (3072 cycles).  16384 causal tokens of
-// 16 / 2 heads of 128: 1.0 ms, 1.1 PFLOP/s, with the clock held at 1.8 GHz by its power (a large library product in the same type: 1.36
-// PFLOP/s); 16 rows of 912 tokens: 75 us, 0.64 PFLOP/s, of which the workgroups' first 10 thousand cycles, up to the first
-// product, are a quarter.  Over a cache it reads 112 MB for single queries in 27 us (4.1 TB/s) and joins them in 4.
+// What bounds it: 16384 causal tokens of 16 / 2 heads of 128 take 1.0 ms, 1.1 PFLOP/s (a large library product in the same type: 1.36
+// PFLOP/s); the matrix units are busy 58 % of the time and the vector units 56 % (a power is four passes), without bank conflicts,
+// at a clock that the power holds at 1.9 GHz.  16 rows of 912 tokens: 71 to 78 us, 0.65 PFLOP/s; of a workgroup's time a quarter lies
+// before its first product.  48 x 1024 patches in windows of 64, 16 heads of 80: 119 us, 4.2 TB/s.  64 x 32 queries over 800 to 912 cached
+// keys: 34 us, by the vector units (46 %) and the widening's way through LDS.  Single queries of 8 sequences over 20 to 32 thousand
+// cached keys: 112 MB in 28 us, 4.0 TB/s, and 4 for the join.
 // (Heads of 80: 168 registers, one less than it would take, let three workgroups share a CU: 48 x 1024 patches in windows 131 us
 // instead of 136, 8 x 2000 causal tokens 126 instead of 132.  The others' sums and tiles leave two.)
 template <int DT, int D, bool F8, int RW>
@@ -533,15 +534,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
     l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
   }
   float o[2] = {0.f, 0.f};
-#pragma unroll 4
-  for (int s = ROWS == 4 ? 0 : wave; s < a.splits; s += ROWS == 4 ? 1 : 4) {
-    const float w = ROWS == 4 ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s)) : s_weight[s];
+  constexpr int kStep = ROWS == 4 ? 1 : 4, kBatch = ROWS == 4 ? 4 : 8;
+  for (int s0 = ROWS == 4 ? 0 : wave; s0 < a.splits; s0 += kBatch * kStep) {
+    float x[kBatch][2], w[kBatch];  // (of splits past the last: the last one's, without weight)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < D) {
-        const float x = part[static_cast<int64_t>(s) * a.rows * D + lane + 64 * u];
-        o[u] += w == 0.f ? 0.f : x * w;
-      }
+    for (int n = 0; n < kBatch; ++n) {
+      const int s = min(s0 + n * kStep, a.splits - 1);
+      w[n] = ROWS == 4 ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s)) : s_weight[s];
+      if (s0 + n * kStep >= a.splits) w[n] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) x[n][u] = lane + 64 * u < D ? part[static_cast<int64_t>(s) * a.rows * D + lane + 64 * u] : 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) o[u] += w[n] == 0.f ? 0.f : x[n][u] * w[n];
   }
   const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i) * a.n_q + hq) * D;
   auto store = [&](int c, float sum) {
