@@ -515,7 +515,8 @@ int wx_qk_norm_rope_bwd(const void* grad_q_out, const void* grad_k_out, const vo
  * bf16 or fp16, head_dim 64, 80 or 128; scale > 0.  Scores, softmax and sums in fp32; the probabilities enter the second product in
  * the tensors' type.  lse (may be NULL): fp32 [batch, n_kv_heads, n_queries * group], group = n_q_heads / n_kv_heads, entry
  * i * group + g of query i and head g of the group: the base-2 logarithm of the sum of powers, what wx_attention_bwd reads.
- * rest (may be NULL): uint8 [batch, n_queries, n_q_heads, head_dim], what rounding out to its type left, as e5m2: with it the backward's sums of out times its gradient are those of out unrounded.
+ * rest (may be NULL): uint8 [batch, n_queries, n_q_heads, head_dim], what rounding out to its type left, as e5m2: with it the backward's
+ * sums of out times its gradient are those of out unrounded.  At most 1024 query heads to a key / value head.
  * workspace: wx_attention_workspace_bytes() bytes for the same sizes (0 for most; few rows over many keys are split). */
 size_t wx_attention_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys, int head_dim);
 int wx_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const int32_t* key_ranges,
@@ -525,7 +526,7 @@ int wx_attention_fwd(const void* q, const void* k, const void* v, void* out, flo
                      wx_stream_t stream);
 /* Its backward: the probabilities are recomputed from lse.  out, lse, rest (may be NULL): what the forward returned; grad_out through strides like q;
  * grad_q [batch, n_queries, n_q_heads, head_dim], grad_k and grad_v [batch, n_keys, n_kv_heads, head_dim], contiguous, every element
- * written.  No atomics: the same inputs give the same bits.  At most 1024 query heads to a key / value head. */
+ * written.  No atomics: the same inputs give the same bits. */
 size_t wx_attention_bwd_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys, int head_dim);
 int wx_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* rest,
                      const void* grad_out, void* grad_q, void* grad_k, void* grad_v, const int32_t* key_ranges, const int32_t* key_lengths, int causal,

@@ -255,6 +255,39 @@ def test_orders_in_memory(dev):
     check(got, reference(q, one, v[:1].expand(B, Hkv, S, D), visible(B, S, S, dev))["out"], "expanded")
 
 
+@pytest.mark.parametrize("size", [(1, 40, 1, 20, 50, 64), (2, 64, 1, 9, 70, 128), (1, 130, 2, 7, 33, 80), (600, 1, 1, 3, 5, 64), (70000, 1, 1, 1, 1, 64)])
+@pytest.mark.parametrize("mask", ["causal", "any"])
+def test_groups_and_batches(dev, size, mask):
+    """Groups of more than 32 heads, whole multiples of 32 and others, and batches of more rows than tiles."""
+    B, Hq, Hkv, Sq, Sk, D = size
+    g = torch.Generator(device=dev).manual_seed(Hq + B)
+    q, k, v, do = (heads(B, s, h, D, torch.bfloat16, g, dev) for s, h in ((Sq, Hq), (Sk, Hkv), (Sk, Hkv), (Sq, Hq)))
+    kw = masks(mask, B, Sq, Sk, g, dev)
+    want = reference(q, k, v, see_of(kw, B, Sq, Sk, dev), do=do)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*leaves, **kw)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, do))):
+        check(got, want[name], name)
+
+
+def test_broadcast_inputs(dev):
+    """One prompt's keys and values for a batch, one query row for all: read through strides of zero, gradients summed by autograd."""
+    g = torch.Generator(device=dev).manual_seed(12)
+    B, Hq, Hkv, S, D = 3, 4, 2, 50, 128
+    q, k, v = heads(1, 1, Hq, D, torch.bfloat16, g, dev), heads(1, S, Hkv, D, torch.bfloat16, g, dev), heads(1, S, 1, D, torch.bfloat16, g, dev)
+    do = heads(B, S, Hq, D, torch.bfloat16, g, dev)
+    wide = lambda q, k, v: (q.expand(B, Hq, S, D), k.expand(B, Hkv, S, D), v.expand(B, Hkv, S, D))  # noqa: E731
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*wide(*leaves), causal=True)
+    grads = torch.autograd.grad(out, leaves, do)
+    full = [t.contiguous().requires_grad_() for t in wide(q, k, v)]
+    ref = ops.attention(*full, causal=True)
+    assert torch.equal(out, ref)
+    for a, b, leaf in zip(grads, torch.autograd.grad(ref, full, do), leaves):
+        over = [d for d in range(4) if leaf.size(d) == 1 and b.size(d) > 1]
+        assert torch.equal(a, b.sum(over, keepdim=True)) or float((a.double() - b.double().sum(over, keepdim=True)).abs().max()) <= 2.0 ** -8 * float(b.double().abs().sum(over).max())
+
+
 def test_nothing_to_attend(dev):
     q = torch.randn(2, 4, 5, 64, device=dev, dtype=torch.bfloat16, requires_grad=True)
     e = torch.empty(2, 2, 0, 64, device=dev, dtype=torch.bfloat16, requires_grad=True)

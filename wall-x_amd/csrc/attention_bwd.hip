@@ -7,6 +7,8 @@
 // 16 rows of 912 causal tokens of 16 / 2 heads of 128 (72 GFLOP in three products, 96 in four): dQ 124 us, 0.58 PFLOP/s, matrix units busy
 // 31 % (the rows' four operands are on their way for a third of it); the plan 5; dK and dV 153 us, 0.63 PFLOP/s, 40 %, reading 0.6 GB of
 // which half is in L2; the join 15.  5003 packed tokens of 12 / 4 heads of 64: 29, 8, 39 and 7 us.
+#include <algorithm>
+
 #include "attention.h"
 
 namespace wx {
@@ -30,6 +32,7 @@ struct BwdArgs {
   uint32_t* info;                 // [pair, row_block] blocks of kInfoWords
   int2* bounds;                   // [pair, row_block] the keys that any row of the block sees
   int key_tiles, more, units;     // of a pair: tiles of kKeyTile keys, what cutting them makes more than that at most, and the sum of both
+  int aim;                        // what it should make more, if there is that much work
   Divider by_pairs, by_kv, by_group, by_in_group, by_tiles;  // by_pairs: of an XCD where they are dealt to XCDs, else all
   Spread spread;                  // of dQ's row tiles
   int4* list;                     // [pair, unit] key tile (-1: none), row blocks from .. up to, place of its sums (-1: the whole tile)
@@ -283,7 +286,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
 //
 // Under a causal mask the first keys are seen by all rows and the last by few, and of a row of packed sequences a tile is seen by those
 // of its own: a tile's row blocks, from the first to the last that sees it, are cut evenly into units of at most as many as make a pair's
-// units about `more` in all (16 where that is fewer), so that the longest workgroup is a unit and not a tile.
+// units about `aim` in all (kLeast where that is fewer), so that the longest workgroup is a unit and not a tile.
+constexpr int kLeast = 16;
 __global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
   constexpr int kChunk = 4096;
   __shared__ int s_first[64], s_last[64];
@@ -323,8 +327,8 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
   for (int t = lane; t < a.key_tiles; t += 64) work += max(tiles[t].y - tiles[t].x + 1, 0);
 #pragma unroll
   for (int n = 1; n < 64; n *= 2) work += __shfl_xor(work, n);
-  const int unit = a.more == 0 ? 0x3fffffff : max(16, (work + a.more - 1) / a.more);
-  int next = 0;  // (never past a.units: the full units are no more than a.more, the last ones of the tiles no more than those)
+  const int unit = a.more == 0 ? 0x3fffffff : max(kLeast, (work + a.aim - 1) / a.aim);
+  int next = 0;  // (never past a.units: the full units are no more than a.aim, the last ones of the tiles no more than those; and see more_units)
   for (int c = 0; c < a.key_tiles; c += 64) {
     const bool is = c + lane < a.key_tiles;
     const int2 t = is ? tiles[c + lane] : int2{0, 0};
@@ -637,9 +641,14 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
 // Forward and backward with 1 / 2 / 3 / 4 / 6: 8192 causal tokens of 16 / 2 heads 1464 / 1344 / 1321 / 1339 / 1372 us, 4096 tokens of 16 / 16
 // heads that see all 593 / 594 / 643 / 648 / 672, 16 rows of 912 causal tokens 379 / 384 / 404 / 413 / 442.
 constexpr int kUnits = 2;
-int more_units(int64_t pairs, int64_t n_keys) {
+int aim_units(int64_t pairs, int64_t n_keys) {
   const int64_t tiles = pairs * ((n_keys + kKeyTile - 1) / kKeyTile), places = 2 * device_cu_count();
   return tiles == 0 || tiles >= kUnits * places ? 0 : static_cast<int>((kUnits * places + pairs - 1) / pairs);
+}
+// No tile makes more than its rows' blocks do in units of the least length.
+int more_units(int64_t pairs, int64_t rows, int64_t n_keys) {
+  const int64_t of_tile = ((rows + 31) / 32 + kLeast - 1) / kLeast, most = (n_keys + kKeyTile - 1) / kKeyTile * std::max<int64_t>(of_tile - 1, 0);
+  return static_cast<int>(std::min<int64_t>(aim_units(pairs, n_keys), most));
 }
 
 struct Workspace {
@@ -647,7 +656,7 @@ struct Workspace {
 };
 Workspace layout(int64_t pairs, int64_t rows, int64_t n_keys, int head_dim) {
   const size_t blocks = static_cast<size_t>(pairs) * ((rows + 31) / 32), tiles = static_cast<size_t>(pairs) * ((n_keys + kKeyTile - 1) / kKeyTile);
-  const size_t more = static_cast<size_t>(pairs) * more_units(pairs, n_keys);
+  const size_t more = static_cast<size_t>(pairs) * more_units(pairs, rows, n_keys);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   Workspace w{};
   w.info = 0;
@@ -713,7 +722,6 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   if (!q_strides || !k_strides || !v_strides || !grad_strides) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null strides", who);
   if (batch == 0 || n_q_heads == 0) return WX_OK;
   const int group = n_q_heads / n_kv_heads;
-  if (group > 1024) return fail(WX_ERR_UNSUPPORTED, "%s: more than 1024 query heads to a key / value head", who);
   if ((n_queries > 0 && (!q || !out || !lse || !grad_out || !grad_q)) || (n_keys > 0 && (!k || !v || !grad_k || !grad_v)))
     return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   for (const void* p : {q, k, v, out, rest, grad_out, static_cast<const void*>(grad_q), static_cast<const void*>(grad_k), static_cast<const void*>(grad_v),
@@ -735,7 +743,7 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   a.c = scale * kLog2e, a.scale = scale;
   const int64_t pairs = batch * n_kv_heads;
   a.key_tiles = (a.n_keys + kKeyTile - 1) / kKeyTile;
-  a.more = more_units(pairs, n_keys);
+  a.aim = aim_units(pairs, n_keys), a.more = more_units(pairs, a.rows, n_keys);
   a.units = a.key_tiles + a.more;
   const Workspace w = layout(pairs, a.rows, n_keys, head_dim);
   if (w.total > 0 && (!workspace || workspace_bytes < w.total)) return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_bwd_workspace_bytes)", who);

@@ -647,6 +647,7 @@ int attention_check(const char* who, int64_t batch, int n_q, int n_kv, int64_t n
     return fail(WX_ERR_INVALID_ARGUMENT, "%s: %d query heads are no multiple of %d key / value heads", who, n_q, n_kv);
   if (!(scale > 0.f) || !(scale < 1e30f)) return fail(WX_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", who);
   const int64_t group = n_kv ? n_q / n_kv : 0;
+  if (group > 1024) return fail(WX_ERR_UNSUPPORTED, "%s: more than 1024 query heads to a key / value head", who);
   if (n_keys > 0x3fffffffll || (group && n_queries > 0x3fffffffll / group) || batch > 0x7fffffffll / (n_kv ? n_kv : 1))
     return fail(WX_ERR_UNSUPPORTED, "%s: more than 2^30 - 1 rows or keys", who);
   return WX_OK;
