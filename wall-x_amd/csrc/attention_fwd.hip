@@ -83,31 +83,35 @@ __device__ __forceinline__ void plain_row(const FwdArgs& a, int b, int hk, int r
 
 // RW of the workgroup's four wavefronts take 32 rows each; the other factor, KW = 4 / RW, shares the keys: wavefront group kw
 // takes every KW-th tile of KB keys, and the groups' sums are joined in LDS at the end.
-// Many rows (RW = 4): a tile of 64 keys serves 128 rows.  Fewer (RW = 2): two tiles of 32 keys at a time serve 64 rows each.  Tiles
+// Many rows (RW = 4): a tile of 64 keys serves 128 rows.  Fewer (RW = 2): two tiles of 32 keys at a time serve 64 rows each.  Long ones
+// (RW = 8): eight wavefronts, 256 rows, in two groups half a step apart (below; plan() has the rule and what each takes).  Tiles
 // are loaded one ahead, straight to LDS; e4m3 ones through registers, where they are widened to the compute type (exactly); their
 // scales multiply the scores and the probabilities, a value per key.  (A form whose four wavefronts each walked tiles of their own for 32
 // rows, without a barrier, was no faster for single queries: 38 against 35 us over 8 x 32768 cached keys.)
 //
-// What bounds it: 16384 causal tokens of 16 / 2 heads of 128 take 1.0 ms, 1.1 PFLOP/s (a large library product in the same type: 1.36
-// PFLOP/s); the matrix units are busy 58 % of the time and the vector units 56 % (a power is four passes), without bank conflicts,
-// at a clock that the power holds at 1.9 GHz.  16 rows of 912 tokens: 71 to 78 us, 0.65 PFLOP/s; of a workgroup's time a quarter lies
+// What bounds it: 16384 causal tokens of 16 / 2 heads of 128 take 0.98 ms, 1.13 PFLOP/s (a large library product in the same type: 1.36
+// PFLOP/s), without bank conflicts, at a clock that the power holds near 1.9 GHz.  Half a step of the two groups takes 1400 to 1800
+// cycles, in which a SIMD's products need 1024, the other group's powers some 930 (one is four passes) and the tiles' way out of
+// LDS, 128 KB, as long as the products.  With 128 rows, each wavefront at its own pace: 1.03 ms, matrix units busy 58 % of the time, vector
+// units 56 %.  16 rows of 912 tokens: 71 to 78 us, 0.65 PFLOP/s; of a workgroup's time a quarter lies
 // before its first product.  48 x 1024 patches in windows of 64, 16 heads of 80: 119 us, 4.2 TB/s.  64 x 32 queries over 800 to 912 cached
 // keys: 34 us, by the vector units (46 %) and the widening's way through LDS.  Single queries of 8 sequences over 20 to 32 thousand
 // cached keys: 112 MB in 28 us, 4.0 TB/s, and 4 for the join.
 // (Heads of 80: 168 registers, one less than it would take, let three workgroups share a CU: 48 x 1024 patches in windows 131 us
 // instead of 136, 8 x 2000 causal tokens 126 instead of 132.  The others' sums and tiles leave two.)
 template <int DT, int D, bool F8, int RW>
-__global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
   using T = AttnTile<D>;
-  constexpr int KW = 4 / RW, KB = RW == 4 ? 64 : 32, NT = KB / 32;
+  constexpr int KW = RW == 8 ? 1 : 4 / RW, KB = RW == 2 ? 32 : 64, NT = KB / 32;
   constexpr bool kDirect = !F8;
   constexpr int kTileBytes = KB * T::kPitch;
   constexpr int kScaleBytes = F8 ? 2 * KB * 4 : 0;
   constexpr int kSlot = 2 * kTileBytes + kScaleBytes;
   constexpr int kTiles = KW * kSlot;                                      // of one buffer
   constexpr int kJoinStats = 4 * 32 * (64 + 4) * 4, kJoin = KW > 1 ? kJoinStats + 4 * 32 * 8 : 0;  // 64 channels at a time
-  unsigned char* const lds = lds_slot<(kTiles > kJoin ? kTiles : kJoin), 0>();
-  unsigned char* const lds1 = lds_slot<kTiles, 1>();
+  constexpr int kFirst = kTiles > kJoin ? kTiles : kJoin;
+  unsigned char* const lds = lds_slot<RW == 8 ? 16 : kFirst, 0>();
+  unsigned char* const lds1 = lds_slot<RW == 8 ? 16 : kTiles, 1>();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave % RW, kw = wave / RW, h = lane >> 5;
 
@@ -190,7 +194,7 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
     const int64_t at = left > 0 ? k0 : 0;
     const auto rk = attn_rsrc(kp + at * k_step, kRsrcBytes), rv = attn_rsrc(vp + at * v_step, kRsrcBytes);
     if constexpr (kDirect) {
-      static_assert(KB == 16 * RW, "a wavefront loads 16 rows");
+      static_assert(RW == 8 || KB == 16 * RW, "a wavefront loads 16 rows");
       const int r0 = rw * 16;
       if (left >= KB) {  // all rows are there: the offsets stay the same from tile to tile
         stage16<D>(rk, slot + r0 * T::kPitch, k_off);
@@ -248,6 +252,38 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
     for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
   float m = -kInf, l = 0.f;  // running maximum (both halves alike) and this lane's share of the sum
 
+  // The mask on a tile's scores, and the running maximum.
+  auto soften = [&](f32x16 (&s)[NT], int k0) {
+    if (k0 < f_lo || k0 + KB > f_hi || k0 + KB > g_hi) {  // some row does not see all of the tile
+      const uint32_t span = static_cast<uint32_t>(s_hi > s_lo ? s_hi - s_lo : 0);
+      const int first = k0 + 4 * h - s_lo;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t at = static_cast<uint32_t>(first + 32 * n + 8 * (r / 4) + r % 4);
+          s[n][r] = at < span ? s[n][r] : -kInf;
+        }
+    }
+    float tops[4] = {-kInf, -kInf, -kInf, -kInf};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) tops[r / 2 % 4] = fmaxf(fmaxf(tops[r / 2 % 4], s[n][r]), s[n][r + 1]);
+    const float top = both_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+    // The maximum is only there to keep the powers in range: it moves (and the sums are rescaled) when a score exceeds it
+    // by more than 2^8, not with every new maximum.
+    if (__any((top - m) * a.c > 8.f)) {
+      const float mn = fmaxf(m, top), alpha = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[o][r] *= alpha;
+    }
+  };
+
   // One tile: the scores, then the powers and the products with the values.  A product's operand is asked for kAhead products
   // before it, and the second half's powers are found under the first half's products.
   auto step = [&](const unsigned char* tk, int k0) {
@@ -285,34 +321,7 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
           s[n][4 * g] *= x.x, s[n][4 * g + 1] *= x.y, s[n][4 * g + 2] *= x.z, s[n][4 * g + 3] *= x.w;
         }
     }
-    if (k0 < f_lo || k0 + KB > f_hi || k0 + KB > g_hi) {  // some row does not see all of the tile
-      const uint32_t span = static_cast<uint32_t>(s_hi > s_lo ? s_hi - s_lo : 0);
-      const int first = k0 + 4 * h - s_lo;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const uint32_t at = static_cast<uint32_t>(first + 32 * n + 8 * (r / 4) + r % 4);
-          s[n][r] = at < span ? s[n][r] : -kInf;
-        }
-    }
-    float tops[4] = {-kInf, -kInf, -kInf, -kInf};
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) tops[r / 2 % 4] = fmaxf(fmaxf(tops[r / 2 % 4], s[n][r]), s[n][r + 1]);
-    const float top = both_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-    // The maximum is only there to keep the powers in range: it moves (and the sums are rescaled) when a score exceeds it
-    // by more than 2^8, not with every new maximum.
-    if (__any((top - m) * a.c > 8.f)) {
-      const float mn = fmaxf(m, top), alpha = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int o = 0; o < T::kOut; ++o)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[o][r] *= alpha;
-    }
+    soften(s, k0);
     const float mc = m == -kInf ? 0.f : m * a.c;
     float sums[2] = {0.f, 0.f};
     auto power = [&](int n, int r) {  // of registers r and r + 1
@@ -345,8 +354,113 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
     l += sums[0] + sums[1];
   };
 
+  if constexpr (RW == 8) {
+    static_assert(!F8 && D == 128, "");
+    // Two groups of four wavefronts, one of each on every SIMD, half a step apart: while one group's matrix units work -- P V of the last
+    // tile, then the scores of the next -- the other finds its powers.  The first group loads the keys of the next tile, the second the
+    // values; a barrier ends each half.
+    unsigned char *const k_even = lds_slot<kTileBytes, 2>(), *const k_odd = lds_slot<kTileBytes, 3>(), *const v_even = lds_slot<kTileBytes, 4>(),
+                  *const v_odd = lds_slot<kTileBytes, 5>();
+    const bool late = rw >= 4;
+    const int r0 = (rw & 3) * 16, my_step = static_cast<int>(late ? v_step : k_step);
+    const char* const my = late ? vp : kp;
+    uint32_t my_off[T::kChunks / 4];
+#pragma unroll
+    for (int i = 0; i < T::kChunks / 4; ++i) my_off[i] = stage_offset<D>(i, lane, [&](int r) { return static_cast<uint32_t>((r0 + r) * my_step); });
+    auto load = [&](int t, unsigned char* slot) {
+      const int k0 = g_lo + t * KB, left = g_hi - k0;
+      const auto rs = attn_rsrc(my + static_cast<int64_t>(k0) * my_step, kRsrcBytes);
+      if (left >= KB) stage16<D>(rs, slot + r0 * T::kPitch, my_off);
+      else stage16<D>(rs, slot + r0 * T::kPitch, lane, [&](int r) { return r0 + r < left ? static_cast<uint32_t>((r0 + r) * my_step) : kOutside; });
+    };
+    auto visible = [&](int t) { const int k0 = g_lo + t * KB; return t < tiles && k0 < w_hi && k0 + KB > w_lo; };
+    f32x16 sc[NT];
+    u32x4 pr[2 * NT];
+    bool before = false;  // there are powers of the last tile
+    auto products = [&](int t, const unsigned char* tk, const unsigned char* tv) {
+      constexpr int kAhead = 4, kScores = NT * T::kSteps, kProducts = NT * 2 * T::kOut;
+      int rows_here = rows_at, cols_here = cols_at;
+      asm volatile("" : "+v"(rows_here), "+v"(cols_here));
+      auto read_k = [&](int i) { return read_rows<D>(tk, 32 * (i % NT), i / NT, rows_here); };
+      auto read_v = [&](int i) { return read_cols<D>(tv, 32 * (i / (2 * T::kOut)), i / T::kOut % 2, i % T::kOut, cols_here); };
+      u32x4 f[kAhead];
+      if (before) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f[i] = read_v(i);
+        in_order();
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) {
+          acc[i % T::kOut] = mfma<DT>(f[i % kAhead], pr[i / T::kOut], acc[i % T::kOut]);
+          if (i + kAhead < kProducts) f[i % kAhead] = read_v(i + kAhead);
+          else f[i % kAhead] = read_k(i + kAhead - kProducts);  // (of no use behind the last tile)
+          in_order();
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
+      }
+      if (!visible(t)) return;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[n][r] = 0.f;
+      in_order();
+#pragma unroll
+      for (int i = 0; i < kScores; ++i) {
+        sc[i % NT] = mfma<DT>(f[i % kAhead], qf[i / NT], sc[i % NT]);
+        if (i + kAhead < kScores) f[i % kAhead] = read_k(i + kAhead);
+        in_order();
+      }
+    };
+    auto powers = [&](int t) {
+      before = visible(t);
+      if (!before) return;
+      const int k0 = g_lo + t * KB;
+      soften(sc, k0);
+      const float mc = m == -kInf ? 0.f : m * a.c;
+      float sums[2] = {0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], a.c, -mc));
+          sc[n][r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r + 1], a.c, -mc));
+          sums[0] += sc[n][r];
+          sums[1] += sc[n][r + 1];
+        }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) pr[2 * n] = pack_step<DT>(sc[n], 0), pr[2 * n + 1] = pack_step<DT>(sc[n], 1);
+      l += sums[0] + sums[1];
+    };
+    auto turn = [&](int t, unsigned char* k_this, unsigned char* k_next, unsigned char* v_last, unsigned char* v_next) {
+      if (!late && t + 1 < tiles) load(t + 1, k_next);
+      products(t, k_this, v_last);
+      in_order();
+      if (late) wait_loads();
+      attn_barrier();
+      if (late && t + 1 < tiles) load(t + 1, v_next);
+      powers(t);
+      in_order();
+      if (!late) wait_loads();
+      attn_barrier();
+    };
+    if (!late && tiles > 0) {
+      load(0, k_even);
+      wait_loads();
+    }
+    attn_barrier();
+    if (late) {
+      if (tiles > 0) load(0, v_even);
+      attn_barrier();
+    }
+    for (int t = 0; t <= tiles; t += 2) {
+      turn(t, k_even, k_odd, v_odd, v_odd);
+      if (t + 1 <= tiles) turn(t + 1, k_odd, k_even, v_even, v_even);
+    }
+    if (!late) attn_barrier();
+  }
   unsigned char *mine = lds + kw * kSlot, *other_slot = lds1 + kw * kSlot;
-  if (iters > 0) fetch(0, mine);
+  if (RW != 8 && iters > 0) fetch(0, mine);
   auto turn = [&](int it, unsigned char* slot, unsigned char* other) {
     const int k0 = key0(it);
     if constexpr (kDirect) {
@@ -361,10 +475,11 @@ __global__ __launch_bounds__(256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_f
     }
     if (k0 < w_hi && k0 + KB > w_lo && k0 < g_hi) step(slot, k0);
   };
-  for (int it = 0; it < iters; it += 2) {
-    turn(it, mine, other_slot);
-    if (it + 1 < iters) turn(it + 1, other_slot, mine);
-  }
+  if constexpr (RW != 8)
+    for (int it = 0; it < iters; it += 2) {
+      turn(it, mine, other_slot);
+      if (it + 1 < iters) turn(it + 1, other_slot, mine);
+    }
   l = both_sum(l);
 
   // ---- the result: joined over the key groups, then either the row itself or this split's part of it
@@ -573,15 +688,20 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
 struct FwdPlan {
   int row_waves, splits;
 };
-FwdPlan plan(int64_t pairs, int64_t rows, int64_t keys, int head_dim) {
+FwdPlan plan(int64_t pairs, int64_t rows, int64_t keys, int head_dim, bool f8) {
   const int cus = device_cu_count();
   FwdPlan p{4, 1};
   // Rows that fill 128-row workgroups two to a CU take those, fewer take 64-row ones, whose two pairs of wavefronts share the keys.  With
   // 64 / 128: 5003 packed tokens of 12 / 4 heads of 64 28 / 38 us (472 large workgroups); 16 x 912 tokens of 16 / 2 heads of 128 107 / 74,
   // 48 x 1024 patches of 16 heads of 80 in windows 203 / 131 (1824 and 6144).
   if (rows <= 64 || pairs * ((rows + 127) / 128) < 2 * cus) p.row_waves = 2;
+  // Heads of 128 over many keys, of more rows than a 256-row workgroup to a CU takes: two groups of wavefronts in step with each other.
+  // Its start is not under another workgroup's work, so that it pays for long rows only.  128 / 256 rows: 8192 causal tokens of 16 / 2 heads
+  // 287 / 255 us, 2 x 4096 that see all 265 / 250, 16384 causal ones 1028 / 977, 4 x 8192 packed ones 301 / 309; 8 x 2048 causal ones 147 /
+  // 148, 4 x 2900 146 / 150, 16 x 912 73 / 82.
+  else if (head_dim == 128 && !f8 && keys >= 4096 && pairs * ((rows + 255) / 256) >= cus) p.row_waves = 8;
   const int64_t groups = pairs * ((rows + 32 * p.row_waves - 1) / (32 * p.row_waves));
-  if (p.row_waves < 4 && groups > 0 && groups < 2 * cus) {
+  if (p.row_waves == 2 && groups > 0 && groups < 2 * cus) {
     // Too few workgroups for the chip: the keys in n parts, up to two workgroups to a CU, of at least a tile for each key group.  A tile
     // of 64 keys takes about 0.8 us, the join 4, and writing and reading the parts of n splits n times what one's take at 3 TB/s: the n of
     // the least sum, if that is less than without.  Measured without / with: one query of 8 heads over 8 x 32768 cached keys of 2 heads 35 us
@@ -606,8 +726,13 @@ int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
   const int64_t blocks = static_cast<int64_t>(a.batch) * a.n_kv * a.row_tiles * a.splits;
   if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
-  if (p.row_waves == 2) hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 2>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 4>), grid, block, 0, s, a);
+  if (p.row_waves == 2) {
+    hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 2>), grid, block, 0, s, a);
+  } else if (p.row_waves == 4) {
+    hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 4>), grid, block, 0, s, a);
+  } else if constexpr (D == 128 && !F8) {
+    hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 8>), grid, dim3(512), 0, s, a);
+  }
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
   if (a.splits > 1) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.n_kv * a.rows;
@@ -672,7 +797,7 @@ extern "C" size_t wx_attention_workspace_bytes(int64_t batch, int n_q_heads, int
                                                int head_dim) {
   if (batch <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_queries <= 0 || n_keys < 0 || head_dim <= 0) return 0;
   const int64_t rows = n_queries * (n_q_heads / n_kv_heads);
-  const FwdPlan p = plan(batch * n_kv_heads, rows, n_keys, head_dim);
+  const FwdPlan p = plan(batch * n_kv_heads, rows, n_keys, head_dim, false);  // (of the splits, which do not depend on the type)
   return p.splits == 1 ? 0 : static_cast<size_t>(batch) * n_kv_heads * p.splits * rows * (head_dim + 2) * sizeof(float);
 }
 
@@ -699,7 +824,7 @@ static int forward(const char* who, const void* q, const void* k, const void* v,
   a.batch = static_cast<int>(batch), a.n_q = n_q, a.n_kv = n_kv, a.n_queries = static_cast<int>(n_queries), a.n_keys = static_cast<int>(n_keys);
   a.group = group, a.rows = static_cast<int>(n_queries) * group;
   a.c = scale * kLog2e;
-  const FwdPlan p = plan(batch * n_kv, a.rows, n_keys, head_dim);
+  const FwdPlan p = plan(batch * n_kv, a.rows, n_keys, head_dim, f8);
   if (p.splits > 1) {
     if (!workspace || workspace_bytes < wx_attention_workspace_bytes(batch, n_q, n_kv, n_queries, n_keys, head_dim))
       return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_workspace_bytes)", who);
