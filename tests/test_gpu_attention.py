@@ -149,6 +149,32 @@ def test_gradients_of_long_axes(dev, size, mask):
         check(got, want[name], f"{name} {dtype}")
 
 
+@pytest.mark.parametrize("mask", ["full", "causal", "lengths", "any"])
+def test_many_rows_over_many_keys(dev, mask):
+    """Rows enough for the widest workgroups over more than 4096 keys, of which the last tile is not full."""
+    B, Hq, Hkv, Sq, Sk, D = 4, 16, 2, 1030, 4111, 128
+    g = torch.Generator(device=dev).manual_seed(len(mask))
+    dtype = torch.float16 if mask == "any" else torch.bfloat16
+    q, k, v, do = (heads(B, s, h, D, dtype, g, dev) for s, h in ((Sq, Hq), (Sk, Hkv), (Sk, Hkv), (Sq, Hq)))
+    kw = masks(mask, B, Sq, Sk, g, dev)
+    see = see_of(kw, B, Sq, Sk, dev)
+    want = reference(q, k, v, see, do=do)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*leaves, **kw)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, do))):
+        check(got, want[name], f"{name} {dtype}")
+    if mask == "lengths":  # what no query sees may hold anything
+        unseen = ~see.any(2)[:, 0, :, None]
+        k, v = (torch.where(unseen[:, None], bad, t) for bad, t in ((float("nan"), k), (float("inf"), v)))
+        assert torch.equal(ops.attention(q, k, v, **kw), out)
+    if mask == "causal":  # nor what only the last three see, for the others
+        k, v = k.clone(), v.clone()
+        k[:, :, -3:], v[:, :, -3:] = float("inf"), float("nan")
+        got = ops.attention(q, k, v, **kw)
+        check(got[:, :, :-3], tuple(x[:, :, :-3] for x in want["out"]), "rows before")
+        assert torch.isnan(got[:, :, -3:]).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D", [64, 80, 128])
 @pytest.mark.parametrize("Hq,Hkv,Sq", [(16, 2, 912), (4, 4, 1000), (32, 1, 48), (8, 2, 6)])
