@@ -288,51 +288,55 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
 // of its own: a tile's row blocks, from the first to the last that sees it, are cut evenly into units of at most as many as make a pair's
 // units about `aim` in all (kLeast where that is fewer), so that the longest workgroup is a unit and not a tile.
 constexpr int kLeast = 16;
+constexpr int kPlanTiles = 1024;
 __global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
   constexpr int kChunk = 4096;
-  __shared__ int s_first[64], s_last[64];
+  __shared__ int s_first[kPlanTiles], s_last[kPlanTiles];
   __shared__ int2 s_bounds[kChunk];
   const int pair = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int2* bounds = a.bounds + static_cast<int64_t>(pair) * a.row_blocks;
-  int2* tiles = a.tiles + static_cast<int64_t>(pair) * a.key_tiles;
   int4* list = a.list + static_cast<int64_t>(pair) * a.units;
-  int work = 0;
-  for (int t0 = 0; t0 == 0 || t0 < a.row_blocks; t0 += kChunk) {
-    const int n = min(a.row_blocks - t0, kChunk);
-    __syncthreads();
-    for (int t = tid; t < n; t += 1024) s_bounds[t] = bounds[t0 + t];
-    for (int c = 0; c < a.key_tiles; c += 64) {
-      const bool mine = tid < 64 && c + lane < a.key_tiles;
-      if (tid < 64) {
-        const int2 before = mine && t0 > 0 ? tiles[c + lane] : int2{0x7fffffff, -1};
-        s_first[tid] = before.x, s_last[tid] = before.y;
-      }
+  for (int c0 = 0; c0 < a.key_tiles; c0 += kPlanTiles) {
+    const int n_tiles = min(a.key_tiles - c0, kPlanTiles);
+    s_first[tid] = 0x7fffffff, s_last[tid] = -1;
+    for (int t0 = 0; t0 < a.row_blocks; t0 += kChunk) {
+      const int n = min(a.row_blocks - t0, kChunk);
+      if (t0 > 0) __syncthreads();
+      for (int t = tid; t < n; t += 1024) s_bounds[t] = bounds[t0 + t];
       __syncthreads();
-      const int k0 = (c + lane) * kKeyTile;
-      int first = 0x7fffffff, last = -1;
+      for (int c = 0; c < n_tiles; c += 64) {
+        const int k0 = (c0 + c + lane) * kKeyTile;
+        int first = 0x7fffffff, last = -1;
 #pragma unroll 4
-      for (int t = tid >> 6; t < n; t += 16) {
-        const int2 x = s_bounds[t];
-        const bool sees = x.x < k0 + kKeyTile && x.y > k0 && x.y > x.x;
-        first = sees ? min(first, t0 + t) : first;
-        last = sees ? t0 + t : last;
+        for (int t = tid >> 6; t < n; t += 16) {
+          const int2 x = s_bounds[t];
+          const bool sees = x.x < k0 + kKeyTile && x.y > k0 && x.y > x.x;
+          first = sees ? min(first, t0 + t) : first;
+          last = sees ? t0 + t : last;
+        }
+        if (last >= 0) {
+          atomicMin(&s_first[c + lane], first);
+          atomicMax(&s_last[c + lane], last);
+        }
       }
-      atomicMin(&s_first[lane], first);
-      atomicMax(&s_last[lane], last);
+    }
+    __syncthreads();
+    if (a.more == 0) {  // every tile is a unit
+      if (tid < n_tiles) list[c0 + tid] = int4{c0 + tid, s_last[tid] < 0 ? 0 : s_first[tid], s_last[tid] + 1, -1};
       __syncthreads();
-      if (mine) tiles[c + lane] = int2{s_first[lane], s_last[lane]};
     }
   }
-  if (tid >= 64) return;
-  for (int t = lane; t < a.key_tiles; t += 64) work += max(tiles[t].y - tiles[t].x + 1, 0);
+  if (a.more == 0 || tid >= 64) return;
+  int2* tiles = a.tiles + static_cast<int64_t>(pair) * a.key_tiles;
+  int work = 0;
+  for (int t = lane; t < a.key_tiles; t += 64) work += max(s_last[t] - s_first[t] + 1, 0);
 #pragma unroll
   for (int n = 1; n < 64; n *= 2) work += __shfl_xor(work, n);
-  const int unit = a.more == 0 ? 0x3fffffff : max(kLeast, (work + a.aim - 1) / a.aim);
+  const int unit = max(kLeast, (work + a.aim - 1) / a.aim);
   int next = 0;  // (never past a.units: the full units are no more than a.aim, the last ones of the tiles no more than those; and see more_units)
   for (int c = 0; c < a.key_tiles; c += 64) {
     const bool is = c + lane < a.key_tiles;
-    const int2 t = is ? tiles[c + lane] : int2{0, 0};
-    const int blocks = max(t.y - t.x + 1, 0);
+    const int from = is ? s_first[c + lane] : 0, blocks = is ? max(s_last[c + lane] - from + 1, 0) : 0;
     const int units = is ? max((blocks + unit - 1) / unit, 1) : 0;  // (a tile that nothing sees: one of no blocks, which writes zeros)
     int up_to = units;
 #pragma unroll
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
     const int at = next + up_to - units;
     const int each = units > 0 ? (blocks + units - 1) / units : 0;
     for (int u = 0; u < units; ++u)
-      list[at + u] = int4{c + lane, blocks > 0 ? t.x + min(blocks, u * each) : 0, blocks > 0 ? t.x + min(blocks, (u + 1) * each) : 0, units > 1 ? at + u : -1};
+      list[at + u] = int4{c + lane, blocks > 0 ? from + min(blocks, u * each) : 0, blocks > 0 ? from + min(blocks, (u + 1) * each) : 0, units > 1 ? at + u : -1};
     if (is) tiles[c + lane] = int2{units, at};
     next += __shfl(up_to, 63);
   }
@@ -643,7 +647,7 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
 constexpr int kUnits = 2;
 int aim_units(int64_t pairs, int64_t n_keys) {
   const int64_t tiles = pairs * ((n_keys + kKeyTile - 1) / kKeyTile), places = 2 * device_cu_count();
-  return tiles == 0 || tiles >= kUnits * places ? 0 : static_cast<int>((kUnits * places + pairs - 1) / pairs);
+  return tiles == 0 || tiles >= kUnits * places || tiles > pairs * kPlanTiles ? 0 : static_cast<int>((kUnits * places + pairs - 1) / pairs);
 }
 // No tile makes more than its rows' blocks do in units of the least length.
 int more_units(int64_t pairs, int64_t rows, int64_t n_keys) {
