@@ -776,9 +776,9 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __r
 }
 
 // Workgroups of the forward (backward: at most kNormBlocks partial sums): tokens over x, and where those alone are fewer than two to a
-// CU groups of heads over y.  Forward / backward of 18 heads of 128 without groups, to two, four and eight workgroups to a CU: 64 tokens
-// 9.8 / 17.1, 5.4 / 7.2, 5.4 / 7.1, 5.4 / 7.2 us; 3711 tokens 12.6 / 20.1, 9.6 / 15.0, 9.5 / 15.2, 9.6 / 16.5; 7500 tokens 15.6 / 27.2,
-// 14.7 / 23.8, 14.9 / 24.8, 15.0 / 26.2.
+// CU groups of heads over y, down to a head.  Forward / backward of 18 heads of 128 without groups, to two and to eight workgroups to a
+// CU: 64 tokens 9.8 / 17.1, 3.4 / 6.0, 3.4 / 6.0 us; 3711 tokens 12.6 / 20.1, 9.6 / 15.0, 9.6 / 16.5; 7500 tokens 15.6 / 27.2, 14.7 / 23.8,
+// 15.0 / 26.2.
 constexpr int64_t kNormBlocks = 2048;
 struct NormGrid {
   int64_t x;
@@ -788,11 +788,10 @@ NormGrid norm_grid(int64_t n_tokens, int heads, int lanes, bool backward) {
   const int64_t cus = device_cu_count();
   NormGrid g;
   g.x = (n_tokens * lanes + 255) / 256;
-  const int batch = backward ? kNormBwdBatch : kRowsHeadBatch;
   int groups = 1;
   if (g.x < 2 * cus) {
-    const int64_t want = (2 * cus + g.x - 1) / (g.x > 0 ? g.x : 1), most = (heads + batch - 1) / batch;
-    groups = static_cast<int>(want < most ? want : most);
+    const int64_t want = (2 * cus + g.x - 1) / (g.x > 0 ? g.x : 1);
+    groups = static_cast<int>(want < heads ? want : heads);
   }
   if (groups < 1) groups = 1;
   if (groups > 256) groups = 256;
