@@ -487,7 +487,7 @@ int wx_swiglu_bwd_tiled(const void* gate_tiled, const void* up_tiled, int64_t ti
  * (batch, head, position) strides in elements, last dimension contiguous, rows 16-byte aligned; q_out and k_out contiguous in that
  * order of dimensions.  inv_freq == NULL: table_or_positions is the packed table of wx_mrope_table (bf16 tensors only); otherwise
  * it is position_ids int64 [3, batch, seq] and the angles are evaluated in the kernel, to better than fp32 at any position.
- * head_dim: a power of two of 16-byte chunks (2 to 64); sections that end on chunks of 8 channels.
+ * head_dim: a power of two of 16-byte chunks (2 to 64); any sections.
  * wx_qk_norm_rope_bwd: from the gradients of q_out and k_out those of q and k (contiguous; either may be NULL) and of the two
  * weights (either or both may be NULL; with one, workspace of wx_qk_norm_rope_bwd_workspace_bytes(head_dim) bytes). */
 int wx_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, float eps,

@@ -16,8 +16,8 @@ SECTIONS = {64: [8, 8, 16], 128: [16, 24, 24], 256: [32, 48, 48]}
 FP32 = 2.0 ** -20
 
 
-def angles(pos, inv_freq, D, layout):
-    s = SECTIONS[D]
+def angles(pos, inv_freq, D, layout, section=None):
+    s = section or SECTIONS[D]
     per = [0] * s[0] + [1] * s[1] + [2] * s[2]
     planes = per + per if layout == "hf" else [0] * (2 * s[0]) + [1] * (2 * s[1]) + [2] * (2 * s[2])
     a = torch.stack([pos[p].double() * inv_freq.double()[d % (D // 2)] for d, p in enumerate(planes)], -1)
@@ -103,6 +103,24 @@ def test_from_table(dev, B, S, Hq, Hkv, D, layout):
     cos, sin = (t << 16).view(torch.float32).double(), (t & -65536).view(torch.float32).double()
     got = run(lambda *a: ops.qk_norm_rope_from_table(*a, table, SECTIONS[D], layout=layout), q, k, wq, wk, gq, gk)
     compare(got, q, k, wq, wk, cos, sin, 1e-6, gq, gk, dtype)
+
+
+@pytest.mark.parametrize("layout", ["hf", "csrc"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D,section", [(64, [8, 12, 12]), (64, [1, 2, 29]), (128, [17, 20, 27]), (128, [64, 0, 0]), (32, [5, 6, 5])])
+def test_sections_that_end_anywhere(dev, D, section, dtype, layout):
+    B, S, Hq, Hkv = 2, 45, 6, 2
+    q, k, wq, wk, pos, gq, gk = inputs(B, S, Hq, Hkv, D, dtype, 5000, dev, 4)
+    freq = (10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().to(dev)
+    got = run(lambda *a: ops.qk_norm_rope_from_positions(*a, pos, freq, section, layout=layout), q, k, wq, wk, gq, gk)
+    compare(got, q, k, wq, wk, *angles(pos, freq, D, layout, section), 1e-6, gq, gk, dtype)
+    if dtype == torch.bfloat16:
+        table = ops.multimodal_rope_table(pos, freq, section, layout)
+        t = table.view(B, 1, S, -1)
+        t = torch.cat((t, t), -1) if t.size(-1) == D // 2 else t
+        cos, sin = (t << 16).view(torch.float32).double(), (t & -65536).view(torch.float32).double()
+        got = run(lambda *a: ops.qk_norm_rope_from_table(*a, table, section, layout=layout), q, k, wq, wk, gq, gk)
+        compare(got, q, k, wq, wk, cos, sin, 1e-6, gq, gk, dtype)
 
 
 def test_against_differences(dev):

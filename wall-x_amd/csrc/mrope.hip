@@ -578,10 +578,13 @@ __device__ __forceinline__ void cos_sin_f32(const NormRope& a, int64_t token, in
       }
     }
   } else {
-    const int64_t pos = static_cast<const int64_t*>(a.cos_t)[a.ax.axis[d0] * a.n_tokens + token];
+    const int64_t* positions = static_cast<const int64_t*>(a.cos_t) + token;
+    int64_t pos = positions[a.ax.axis[d0] * a.n_tokens];
     const float* inv_freq = static_cast<const float*>(a.sin_t) + (hi ? d0 - half : d0);
+    const bool cut = a.ax.uniform[d0 >> 3] == 0;  // a section ends among these channels
 #pragma unroll
     for (int e = 0; e < kEpc; ++e) {
+      if (cut) pos = positions[a.ax.axis[d0 + e] * a.n_tokens];
       const double angle = static_cast<double>(pos) * static_cast<double>(inv_freq[e]);
       const double turns = __builtin_rint(angle * 0.15915494309189535);
       const double rest = __builtin_fma(-turns, 2.4492935982947064e-16, __builtin_fma(-turns, 6.283185307179586, angle));
@@ -814,9 +817,7 @@ int launch_norm_rope(NormRope& a, bool backward, int64_t batch, void* dwq, void*
   a.n_tokens = batch * a.seq;
   const int heads = a.n_q + a.n_kv, epc = dtype == WX_F32 ? 4 : 8, lanes = a.head_dim / epc;
   if (int rc = build_axis_table(sec, a.head_dim, layout, a.ax)) return rc;
-  bool rows_ok = lanes >= 2 && lanes <= 64 && (lanes & (lanes - 1)) == 0;
-  for (int c = 0; c < a.head_dim / 8 && rows_ok; ++c) rows_ok = a.ax.uniform[c] != 0;
-  if (!rows_ok) return fail(WX_ERR_UNSUPPORTED, "%s: needs a head of 2..64 16-byte chunks (a power of two) and sections that end on chunk boundaries", who);
+  if (lanes < 2 || lanes > 64 || (lanes & (lanes - 1)) != 0) return fail(WX_ERR_UNSUPPORTED, "%s: needs a head of 2..64 16-byte chunks (a power of two)", who);
   hipStream_t s = as_stream(stream);
   const dim3 block(256);
   const bool empty = a.n_tokens == 0 || heads == 0;
