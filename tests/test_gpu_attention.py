@@ -314,6 +314,30 @@ def test_broadcast_inputs(dev):
         assert torch.equal(a, b.sum(over, keepdim=True)) or float((a.double() - b.double().sum(over, keepdim=True)).abs().max()) <= 2.0 ** -8 * float(b.double().abs().sum(over).max())
 
 
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("B,S,Hq,Hkv", [(5, 1, 12, 4), (1, 3, 64, 8), (2, 900, 3, 1), (9, 2000, 8, 2)])
+def test_rows_of_one_key(dev, B, S, Hq, Hkv, D):
+    """The probability of an only key does not move with its score: such rows give their queries and keys exactly nothing."""
+    g = torch.Generator(device=dev).manual_seed(S)
+    dtype = torch.float16 if S % 2 else torch.bfloat16
+    q, k, v, do = (heads(B, S, h, D, dtype, g, dev) for h in (Hq, Hkv, Hkv, Hq))
+    at = torch.arange(S, device=dev).expand(B, S)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    ranges = torch.stack((at, at + 1), -1).to(torch.int32)
+    out = ops.attention(*leaves, ranges)
+    dq, dk, dv = torch.autograd.grad(out, leaves, do)
+    assert torch.equal(out, v.repeat_interleave(Hq // Hkv, 1)) and not dq.any() and not dk.any()
+    check(dv, reference(q, k, v, visible(B, S, S, dev, ranges), do=do)["dv"], "dv")
+    # the first row of a causal mask among others; and an only key that is not finite
+    dq, dk, dv = torch.autograd.grad(ops.attention(*leaves, causal=True), leaves, do)
+    assert not dq[:, :, 0].any()
+    bad = v.clone()
+    bad[:, :, 0] = float("nan")
+    leaves[2] = bad.requires_grad_()
+    dq, dk, _ = torch.autograd.grad(ops.attention(*leaves, ranges), leaves, do)
+    assert torch.isnan(dq[:, :, 0]).all() and torch.isnan(dk[:, :, 0]).all() and not dq[:, :, 1:].any() and not dk[:, :, 1:].any()
+
+
 def test_nothing_to_attend(dev):
     q = torch.randn(2, 4, 5, 64, device=dev, dtype=torch.bfloat16, requires_grad=True)
     e = torch.empty(2, 2, 0, 64, device=dev, dtype=torch.bfloat16, requires_grad=True)

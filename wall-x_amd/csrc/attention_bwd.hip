@@ -40,7 +40,8 @@ struct BwdArgs {
   float* part;                    // [pair, place, kKeyTile, 2, D]
 };
 
-// What the second kernel reads of 32 rows: L, delta, lo and hi of each, then the keys that all rows with keys see.
+// What the second kernel reads of 32 rows: L, delta, lo and hi of each, then the keys that all rows with keys see, and whether some row
+// sees a single one.
 constexpr int kInfoWords = 4 * 32 + 4;
 
 constexpr int kKeyTile = 64;
@@ -135,14 +136,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   // (a rest that e5m2 does not hold, of outputs of 10^7 and more, is left out)
   const float delta = some ? both_sum(sums[0] + sums[1]) + (fabsf(rests) < kInf ? rests : 0.f) : 0.f;
   lse = some ? lse : kInf;
-  const int block = tile * RW + rw;
+  const int block = tile * RW + rw, one = __any(hi - lo == 1);
   if (kw == 0 && block < a.row_blocks) {
     const int64_t at = static_cast<int64_t>(pair) * a.row_blocks + block;
     uint32_t* info = a.info + at * kInfoWords;
     info[(h ? 64 : 0) + (lane & 31)] = h ? static_cast<uint32_t>(lo) : __float_as_uint(lse);
     info[(h ? 96 : 32) + (lane & 31)] = h ? static_cast<uint32_t>(hi) : __float_as_uint(delta);
     if (lane == 0) {
-      *reinterpret_cast<int4*>(info + 128) = int4{f_lo, f_hi, 0, 0};
+      *reinterpret_cast<int4*>(info + 128) = int4{f_lo, f_hi, one, 0};
       a.bounds[at] = int2{w_lo, w_hi};
     }
   }
@@ -242,7 +243,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
   }
-  store_row<DT, D>(acc, a.scale, live ? a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D : nullptr, lane);
+  // (a row of one key has no slope: its sum is what rounding left of dP - delta)
+  store_row<DT, D>(acc, hi - lo == 1 ? 0.f : a.scale, live ? a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D : nullptr, lane);
   // Rows whose sum is not a number, in plain loops over the keys that they see: 0 * inf may have come from one that they do not.
   uint64_t redo = __ballot(bad && some);
   redo = (redo | redo >> 32) & 0xffffffffull;
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
     uint16_t* dst = a.dq + ((static_cast<int64_t>(b) * a.n_queries + i_r) * a.n_q + hq_r) * D;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sum[u] * a.scale));
+      if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sum[u] * (hi_r - lo_r == 1 ? 0.f : a.scale)));
   }
 }
 
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     if (t >= last) return;
     const unsigned char* tg = tq + kTileBytes;
     const float* info = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
-    const int2 full = *reinterpret_cast<const int2*>(info + 128);
+    const int4 full = *reinterpret_cast<const int4*>(info + 128);
     const int f_lo = __builtin_amdgcn_readfirstlane(full.x), f_hi = __builtin_amdgcn_readfirstlane(full.y);
     // (an exclusive-or per read in place of an address register for each: the accumulators leave none)
     int rows_at = rows_first, cols_at = cols_first;
@@ -497,6 +499,16 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[4 * g + i] = ((key >= l4[i]) & (key < h4[i])) ? s[4 * g + i] : -kInf;
+      }
+    }
+    if (__builtin_amdgcn_readfirstlane(full.z) != 0) {  // some row sees one key: its slope is none
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at = 8 * (r / 4) + 4 * h + r % 4;
+        const int keys = __float_as_int(info[96 + at]) - __float_as_int(info[64 + at]);
+        const float delta = info[32 + at];
+        dp[r] = keys == 1 ? delta : dp[r];
+        in_order();
       }
     }
     auto slope = [&](int g) {  // P and dS of registers 4 g .. + 3
@@ -590,7 +602,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
             d = __builtin_fmaf(Elem<DT>::load(g[e]), Elem<DT>::load(vr[e]), d);
           }
           x = exp2f(s * a.c - __uint_as_float(info[0]));
-          if (rg == 0) x *= d - __uint_as_float(info[32]);
+          if (rg == 0) x *= (info[96] - info[64] == 1 ? __uint_as_float(info[32]) : d) - __uint_as_float(info[32]);
         }
       }
       uint64_t seen = __ballot(see);
