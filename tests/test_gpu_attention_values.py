@@ -88,3 +88,72 @@ def test_cached_scales_beyond_fp16(dev, B, Hq, Hkv, Sq, C, D):
         kd, vd = kc.double() * ks.double()[..., None], codes.double() * vs.double()[..., None]
         want = reference(q, kd, vd, visible(B, Sq, C, dev))["out"]
         check(ops.cached_attention(q, kc, codes, ks, vs), want, f"scale 2^{power}")
+
+
+GRADIENTS = [  # B, Hq, Hkv, Sq, Sk, D, causal: rows in workgroups of 64 and of 128, long keys in units and as they are, an odd group
+    (1, 2, 1, 4096, 4096, 128, True), (1, 4, 1, 70, 8192, 64, False), (2, 6, 2, 900, 900, 80, True), (40, 16, 2, 300, 300, 128, True)]
+
+
+def gradients(q, k, v, do, causal):
+    """{name: (value, tolerance)}: those of test_gpu_attention without what fp16 loses below 2^-14.  A probability enters its product 2^15 times as
+    large and is off by 2^-25 / 2^15 below 2^-29; a slope by 2^-40 likewise, or, where the slopes of the rows beside it are so large
+    that it is scaled by less, by 2^-34 of the largest of them."""
+    see = visible(q.size(0), q.size(2), k.size(2), q.device, causal=causal)
+    want = reference(q, k, v, see, do=do)
+    u, G, scale = torch.finfo(q.dtype).eps / 2, q.size(1) // k.size(1), q.size(3) ** -0.5
+    q, k, v, do = (t.double().contiguous() for t in (q, k.repeat_interleave(G, 1), v.repeat_interleave(G, 1), do))
+    T = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
+    p = torch.softmax((q @ T(k) * scale).masked_fill(~see, -float("inf")), -1)
+    o, most = want["out"]
+    o_tol = u * o.abs() + (u + 2.0 ** -12) * (p @ v.abs()) + TINY + TINY * (see.double() @ v.abs())
+    ds = p * (do @ T(v) - (do * o).sum(-1, keepdim=True))
+    lost = (2.0 ** -40 + 2.0 ** -34 * ds.abs().amax((1, 2, 3), keepdim=True)) * see
+    e = (u + 2.0 ** -12) * ds.abs() + p * ((do.abs() * o_tol).sum(-1, keepdim=True) + 2.0 ** -16 * (do.abs() @ T(v.abs()))) + lost
+    fold = lambda x: x.unflatten(1, (-1, G)).sum(2)  # noqa: E731
+    (dq, _), (dk, _), (dv, _) = want["dq"], want["dk"], want["dv"]
+    return {"dq": (dq, u * dq.abs() + scale * (e @ k.abs()) + TINY), "dk": (dk, u * dk.abs() + scale * fold(T(e) @ q.abs()) + TINY),
+            "dv": (dv, u * dv.abs() + fold((u + 2.0 ** -12) * (T(p) @ do.abs()) + 2.0 ** -40 * (T(see.double().expand_as(p)) @ do.abs())) + TINY)}
+
+
+def held(got, value, tol):
+    """65520 and more is infinity in fp16: a result that may be as large may be that, and counts as right here."""
+    beyond = torch.isinf(got) & (got.sign() == value.sign()) & (value.abs() + tol >= 65520) & (got.dtype == torch.float16)
+    return torch.where(beyond, 0, got), torch.where(beyond, 0, value), tol
+
+
+def take_gradients(q, k, v, do, **kw):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    return torch.autograd.grad(ops.attention(*leaves, **kw), leaves, do)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("grad,value", [(1e-4, 1.0), (1e-3, 1.0), (1.0, 1.0), (1.0, 1e-3), (1e3, 30.0)])
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Sk,D,causal", GRADIENTS)
+def test_gradients_of_any_size(dev, B, Hq, Hkv, Sq, Sk, D, causal, grad, value, dtype):
+    """Slopes far below fp16's normal numbers (a small gradient over many keys) and beyond its largest (the first rows of a causal mask
+    under a large one)."""
+    g = torch.Generator(device=dev).manual_seed(Sq + Sk)
+    q, k, v, do = heads(B, Sq, Hq, D, dtype, g, dev), heads(B, Sk, Hkv, D, dtype, g, dev), heads(B, Sk, Hkv, D, dtype, g, dev) * value, heads(B, Sq, Hq, D, dtype, g, dev) * grad
+    want = gradients(q, k, v, do, causal)
+    for name, got in zip(("dq", "dk", "dv"), take_gradients(q, k, v, do, causal=causal)):
+        got, value, tol = held(got, *want[name])
+        check(got, (value, tol), name)
+        near(got, value, name)
+
+
+def test_gradients_far_apart(dev):
+    """Packed sequences, one's gradients 2^28 times another's: blocks of rows hold both, and each sequence's are its own."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    Hq, Hkv, S, D, each = 8, 2, 1200, 128, 75
+    q, k, v, do = (heads(1, S, h, D, torch.float16, g, dev) for h in (Hq, Hkv, Hkv, Hq))
+    at = torch.arange(S, device=dev)
+    do = do * torch.where(at // each % 2 == 0, 2.0 ** 13, 2.0 ** -11)[:, None].to(torch.float16)
+    ranges = torch.stack((at // each * each, at + 1), -1).to(torch.int32)[None]
+    got = take_gradients(q, k, v, do, key_ranges=ranges)
+    for n in range(S // each):
+        part = slice(n * each, (n + 1) * each)
+        for name, a, (value, tol) in zip(("dq", "dk", "dv"), got, gradients(q[:, :, part], k[:, :, part], v[:, :, part], do[:, :, part], True).values()):
+            # (a block of 32 rows, 8 tokens of 4 heads, may hold rows of both kinds: their slopes then lose 2^-34 of the larger ones)
+            beside = 2.0 ** -34 * 2.0 ** 13 * 64 * (D ** -0.5 * 75 * 5 if name != "dv" else 0.0)
+            a, value, tol = held(a[:, :, part], value, tol + beside)
+            check(a, (value, tol), f"{name} of sequence {n}")

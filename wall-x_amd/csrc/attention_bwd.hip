@@ -40,9 +40,21 @@ struct BwdArgs {
   float* part;                    // [pair, place, kKeyTile, 2, D]
 };
 
-// What the second kernel reads of 32 rows: L, delta, lo and hi of each, then the keys that all rows with keys see, and whether some row
-// sees a single one.
+// What the second kernel reads of 32 rows: L (less kUp), delta, lo and hi of each, then the keys that all rows with keys see, whether some row
+// sees a single one, and (fp16) the power of two that the slopes of all its rows fit fp16 with.
 constexpr int kInfoWords = 4 * 32 + 4;
+
+// fp16's range is too short for probabilities of many keys and for their slopes: P is 1 / keys, dS as much smaller again as the gradient
+// that comes in, and beyond 65504 where few keys meet a large one.  P enters its product times 2^15, which it cannot leave the range with.  dS of
+// a row is formed times 2^15 as well (both are one subtraction from L), until a slope passes 2^15 (kMostSlope): then by as much less as
+// takes the largest to below 2^10, and the sums so far with it.  The second kernel, whose products sum over rows, takes the least of the
+// powers of the rows that it has met.  Powers of two are exact, and taken back from the sums.  Forward and backward of 16 x 912 tokens in fp16
+// 378 us, 368 with P and dS as they are; dQ's error for gradients of 0.001 over 8192 keys 0.096 % of its length (0.094 of it the result's own
+// rounding), 0.76 with them.
+template <int DT>
+constexpr int kUp = DT == WX_F16 ? 15 : 0;
+constexpr float kMostSlope = 32768.f;
+constexpr int kSlopeTo = 9;
 
 constexpr int kKeyTile = 64;
 
@@ -136,11 +148,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   // (a rest that e5m2 does not hold, of outputs of 10^7 and more, is left out)
   const float delta = some ? both_sum(sums[0] + sums[1]) + (fabsf(rests) < kInf ? rests : 0.f) : 0.f;
   lse = some ? lse : kInf;
+  constexpr bool kFit = DT == WX_F16;
+  int up = kUp<DT>;  // this row's slopes are formed times 2^up
+  float shifted = lse - kUp<DT>;
   const int block = tile * RW + rw, one = __any(hi - lo == 1);
   if (kw == 0 && block < a.row_blocks) {
     const int64_t at = static_cast<int64_t>(pair) * a.row_blocks + block;
     uint32_t* info = a.info + at * kInfoWords;
-    info[(h ? 64 : 0) + (lane & 31)] = h ? static_cast<uint32_t>(lo) : __float_as_uint(lse);
+    info[(h ? 64 : 0) + (lane & 31)] = h ? static_cast<uint32_t>(lo) : __float_as_uint(shifted);
     info[(h ? 96 : 32) + (lane & 31)] = h ? static_cast<uint32_t>(hi) : __float_as_uint(delta);
     if (lane == 0) {
       *reinterpret_cast<int4*>(info + 128) = int4{f_lo, f_hi, one, 0};
@@ -153,6 +168,21 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
+  // Keeps the row's slopes in fp16's range: `top` is the largest of what this lane is about to round.
+  auto fit = [&](f32x16& s, int from, float top) {
+    if (!__any(top > kMostSlope && top < kInf)) return;
+    top = both_max(top);
+    const int less = top > kMostSlope && top < kInf ? static_cast<int>(__float_as_uint(top) >> 23) - 127 - kSlopeTo : 0;
+    const float f = ldexpf(1.f, -less);
+    up -= less;
+    shifted += static_cast<float>(less);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s[from + r] *= f;
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[o][r] *= f;
+  };
   const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
   auto turn = [&](int it, unsigned char* tk, unsigned char* other) {
     wait_loads();
@@ -191,14 +221,25 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = static_cast<uint32_t>(k0 + 4 * h + 8 * (r / 4) + r % 4 - lo) < span ? s[r] : -kInf;
       }
-      auto slope = [&](int r) { s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta); };
+      float top = 0.f;
+      auto slope = [&](int r) {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -shifted)) * (dp[r] - delta);
+        if constexpr (kFit) top = fmaxf(top, fabsf(s[r]));
+      };
 #pragma unroll
       for (int r = 0; r < 8; ++r) slope(r);
+      if constexpr (kFit) {
+        fit(s, 0, top);
+        top = 0.f;
+      }
       u32x4 ds = pack_step<DT>(s, 0);
       in_order();
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
-        if (i == T::kOut) ds = pack_step<DT>(s, 1);
+        if (i == T::kOut) {
+          if constexpr (kFit) fit(s, 8, top);
+          ds = pack_step<DT>(s, 1);
+        }
         acc[i % T::kOut] = mfma<DT>(f[i % kAhead], ds, acc[i % T::kOut]);
         if (i + kAhead < kProducts) f[i % kAhead] = read_k(i + kAhead);
         if (i < T::kOut) {
@@ -214,6 +255,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
     turn(it, lds0, lds1);
     if (it + 1 < iters) turn(it + 1, lds1, lds0);
   }
+  int block_up = kUp<DT>;
+  if constexpr (kFit) {
+    block_up = wave_extreme<false>(up);
+    if (block_up < kUp<DT>) {  // (of the wavefront's rows: the sums of all in the same power again)
+      const float f = ldexpf(1.f, kUp<DT> - up);
+#pragma unroll
+      for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[o][r] *= f;
+    }
+  }
   if constexpr (KW == 2) {  // the second key group's sums to the first
     float* const at = reinterpret_cast<float*>(lds0) + rw * (T::kOut * 16 * 64) + lane;
     __syncthreads();
@@ -222,14 +274,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
         for (int r = 0; r < 16; ++r) at[(16 * o + r) * 64] = acc[o][r];
+      if (kFit && lane == 0) s_bounds[rw].x = block_up;
     }
     __syncthreads();
     if (kw == 1) return;
+    if constexpr (kFit) block_up = min(block_up, s_bounds[rw].x);
 #pragma unroll
     for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[o][r] += at[(16 * o + r) * 64];
   }
+  if (kFit && lane == 0 && block < a.row_blocks) a.info[(static_cast<int64_t>(pair) * a.row_blocks + block) * kInfoWords + 131] = static_cast<uint32_t>(block_up);
 
   bool bad = false;
 #pragma unroll
@@ -244,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
   }
   // (a row of one key has no slope: its sum is what rounding left of dP - delta)
-  store_row<DT, D>(acc, hi - lo == 1 ? 0.f : a.scale, live ? a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D : nullptr, lane);
+  store_row<DT, D>(acc, hi - lo == 1 ? 0.f : a.scale * ldexpf(1.f, -kUp<DT>), live ? a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D : nullptr, lane);
   // Rows whose sum is not a number, in plain loops over the keys that they see: 0 * inf may have come from one that they do not.
   uint64_t redo = __ballot(bad && some);
   redo = (redo | redo >> 32) & 0xffffffffull;
@@ -457,6 +512,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[o][r] = dv[o][r] = 0.f;
 
+  constexpr bool kFit = DT == WX_F16;
+  int up = kUp<DT>;         // dk holds its sums times 2^up, dv times 2^kUp
+  float of_slope = 1.f;     // 2^(up - kUp)
   const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
   auto turn = [&](int t, unsigned char* tq, unsigned char* next) {
     wait_loads();
@@ -467,6 +525,18 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     const float* info = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
     const int4 full = *reinterpret_cast<const int4*>(info + 128);
     const int f_lo = __builtin_amdgcn_readfirstlane(full.x), f_hi = __builtin_amdgcn_readfirstlane(full.y);
+    if constexpr (kFit) {
+      const int here = __builtin_amdgcn_readfirstlane(full.w);
+      if (here < up) {
+        const float f = ldexpf(1.f, here - up);
+        up = here;
+        of_slope = ldexpf(1.f, up - kUp<DT>);
+#pragma unroll
+        for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dk[o][r] *= f;
+      }
+    }
     // (an exclusive-or per read in place of an address register for each: the accumulators leave none)
     int rows_at = rows_first, cols_at = cols_first;
     asm volatile("" : "+v"(rows_at), "+v"(cols_at));
@@ -519,6 +589,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         const int r = 4 * g + i;
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -ls[i]));
         dp[r] = s[r] * (dp[r] - de[i]);
+        if constexpr (kFit) dp[r] *= of_slope;
       }
     };
     slope(0);
@@ -542,6 +613,13 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     if (t + 2 < last) turn(t + 2 + rg, other, mine);
   }
 
+  if constexpr (kFit) {
+    const float fk = ldexpf(1.f, -up), fv = ldexpf(1.f, -kUp<DT>);
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[o][r] *= fk, dv[o][r] *= fv;
+  }
   // The two row groups' sums: the first gets the others' dK and finishes it, the second dV.
   __syncthreads();
   {
@@ -601,7 +679,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
             s = __builtin_fmaf(Elem<DT>::load(q[e]), Elem<DT>::load(kr[e]), s);
             d = __builtin_fmaf(Elem<DT>::load(g[e]), Elem<DT>::load(vr[e]), d);
           }
-          x = exp2f(s * a.c - __uint_as_float(info[0]));
+          x = exp2f(s * a.c - (__uint_as_float(info[0]) + kUp<DT>));
           if (rg == 0) x *= (info[96] - info[64] == 1 ? __uint_as_float(info[32]) : d) - __uint_as_float(info[32]);
         }
       }
