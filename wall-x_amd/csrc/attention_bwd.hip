@@ -62,6 +62,81 @@ __device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64
   return p + b * st[0] + h * st[1] + i * st[2];
 }
 
+template <int D>
+__device__ __forceinline__ bool not_numbers(const f32x16* acc) {
+  bool bad = false;
+#pragma unroll
+  for (int o = 0; o < AttnTile<D>::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (32 * o + 8 * (r / 4) < D) bad = bad || acc[o][r] != acc[o][r];
+  return bad;
+}
+
+// Rows whose sum is not a number though their L and delta are: again (see Odd, attention.h), those of this wavefront's that `again` has a bit
+// for, times 2^up.  (A key that is not finite has no probability where L is a number, so that its slope times it is NaN.)  Their place is
+// found once more: kept over the kernel's loop for this rare case it costs that registers.
+template <int DT, int D, int RW>
+__device__ __forceinline__ void dq_again(const BwdArgs& a, uint32_t again, float lse, float delta, int up) {
+  using T = AttnTile<D>;
+  int id = blockIdx.x, tid = threadIdx.x;
+  asm volatile("" : "+s"(id), "+v"(tid));
+  const int lane = tid & 63, rw = __builtin_amdgcn_readfirstlane(tid >> 6) % RW, h = lane >> 5;
+  int pair, tile;
+  a.spread.place(id, pair, tile);
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
+  const int row = (tile * RW + rw) * 32 + (lane & 31), in_row = row < a.rows ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
+  const bool redo = again >> (lane & 31) & 1;
+  int lo = 0, hi = 0;
+  if (redo) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
+  const int from = wave_extreme<false>(redo ? lo : 0x7fffffff), up_to = wave_extreme<true>(hi);
+  const char* kp = reinterpret_cast<const char*>(a.k + b * a.ks[0] + hk * a.ks[1]);
+  const char* vp = reinterpret_cast<const char*>(a.v + b * a.vs[0] + hk * a.vs[1]);
+  const int64_t k_step = a.ks[2] * 2, v_step = a.vs[2] * 2;
+  const uint16_t *q = row_of(a.q, a.qs, b, hq, qi), *g = row_of(a.g, a.gs, b, hq, qi);
+  uint16_t* const dq = a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
+  const float factor = hi - lo == 1 ? 0.f : a.scale * ldexpf(1.f, -kUp<DT>), l_up = lse - static_cast<float>(up), back = ldexpf(1.f, kUp<DT> - up);
+  for (int o = 0; o < T::kOut; ++o) {
+    f32x16 sum = {};
+    const int c = 32 * o + (lane & 31);
+    for (int k0 = from; k0 < up_to; k0 += 32) {
+      auto in = [&](int i) { return min(i, a.n_keys - 1 - k0); };  // (a key past the last is the last, and not seen)
+      const char *kr = kp + k0 * k_step + in(lane & 31) * static_cast<int>(k_step), *vr = vp + k0 * v_step + in(lane & 31) * static_cast<int>(v_step);
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int t = 0; t < T::kSteps; ++t) {
+        s = mfma<DT>(*reinterpret_cast<const u32x4*>(kr + (16 * t + 8 * h) * 2), *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h), s);
+        dp = mfma<DT>(*reinterpret_cast<const u32x4*>(vr + (16 * t + 8 * h) * 2), *reinterpret_cast<const u32x4*>(g + 16 * t + 8 * h), dp);
+        in_order();
+      }
+      uint32_t seen = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = k0 + 8 * (r / 4) + 4 * h + r % 4;
+        const bool sees = redo && key >= lo && key < hi;
+        s[r] = sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -l_up)) * (dp[r] - delta) : 0.f;
+        seen |= sees ? 1u << r : 0u;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Odd odd;
+        const u32x4 x = gather_cols<DT>(t, h, odd, [&](int i) -> uint32_t {
+          return D % 32 != 0 && c >= D ? 0u : *reinterpret_cast<const uint16_t*>(kp + k0 * k_step + (in(i) * static_cast<int>(k_step) + 2 * c));
+        });
+        in_order();
+        sum = mfma<DT>(x, pack_step<DT>(s, t), sum);
+        odd.nan |= odd.plus | odd.minus, odd.plus = odd.minus = 0;
+        add_odd<DT>(sum, odd, seen, 0, t);
+        in_order();
+      }
+    }
+    if constexpr (DT == WX_F16)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[r] *= back;
+    store_cols<DT, D>(sum, o, factor, redo ? dq : nullptr, lane);
+  }
+}
+
 template <int DT, int D, int RW>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   using T = AttnTile<D>;
@@ -151,11 +226,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   constexpr bool kFit = DT == WX_F16;
   int up = kUp<DT>;  // this row's slopes are formed times 2^up
   float shifted = lse - kUp<DT>;
+  float l_info = shifted;
+  if (__any(delta != delta)) {  // a row whose gradient is NaN throughout makes all of dV NaN as well: said by its L, so that nothing is done again for it
+    bool all = delta != delta;
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float x = Elem<DT>::load(gf[t][u] & 0xffffu), y = Elem<DT>::load(gf[t][u] >> 16);
+        all = all && x != x && y != y;
+      }
+    const uint64_t rows = __ballot(all);
+    if ((rows & rows >> 32) >> (lane & 31) & 1) l_info = __builtin_nanf("");
+  }
   const int block = tile * RW + rw, one = __any(hi - lo == 1);
   if (kw == 0 && block < a.row_blocks) {
     const int64_t at = static_cast<int64_t>(pair) * a.row_blocks + block;
     uint32_t* info = a.info + at * kInfoWords;
-    info[(h ? 64 : 0) + (lane & 31)] = h ? static_cast<uint32_t>(lo) : __float_as_uint(shifted);
+    info[(h ? 64 : 0) + (lane & 31)] = h ? static_cast<uint32_t>(lo) : __float_as_uint(l_info);
     info[(h ? 96 : 32) + (lane & 31)] = h ? static_cast<uint32_t>(hi) : __float_as_uint(delta);
     if (lane == 0) {
       *reinterpret_cast<int4*>(info + 128) = int4{f_lo, f_hi, one, 0};
@@ -285,13 +373,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       for (int r = 0; r < 16; ++r) acc[o][r] += at[(16 * o + r) * 64];
   }
   if (kFit && lane == 0 && block < a.row_blocks) a.info[(static_cast<int64_t>(pair) * a.row_blocks + block) * kInfoWords + 131] = static_cast<uint32_t>(block_up);
-
-  bool bad = false;
-#pragma unroll
-  for (int o = 0; o < T::kOut; ++o)
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (32 * o + 8 * (r / 4) < D) bad = bad || acc[o][r] != acc[o][r];
+  const uint32_t again = columns(not_numbers<D>(acc) && some && lse == lse && delta == delta);
   if (!some) {
 #pragma unroll
     for (int o = 0; o < T::kOut; ++o)
@@ -299,44 +381,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
       for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
   }
   // (a row of one key has no slope: its sum is what rounding left of dP - delta)
-  store_row<DT, D>(acc, hi - lo == 1 ? 0.f : a.scale * ldexpf(1.f, -kUp<DT>), live ? a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D : nullptr, lane);
-  // Rows whose sum is not a number, in plain loops over the keys that they see: 0 * inf may have come from one that they do not.
-  uint64_t redo = __ballot(bad && some);
-  redo = (redo | redo >> 32) & 0xffffffffull;
-  while (redo != 0) {
-    const int r = __builtin_ctzll(redo);
-    redo &= redo - 1;
-    const int row_r = __shfl(row, r), lo_r = __shfl(lo, r), hi_r = __shfl(hi, r);
-    const float lse_r = __shfl(lse, r), delta_r = __shfl(delta, r);
-    const int i_r = row_r / a.group, hq_r = hk * a.group + row_r % a.group;
-    const uint16_t *q = row_of(a.q, a.qs, b, hq_r, i_r), *g = row_of(a.g, a.gs, b, hq_r, i_r);
-    float sum[2] = {0.f, 0.f};
-    for (int first = lo_r; first < hi_r; first += 64) {
-      const int key = first + lane;
-      float ds = 0.f;
-      if (key < hi_r) {
-        const uint16_t *kr = row_of(a.k, a.ks, b, hk, key), *vr = row_of(a.v, a.vs, b, hk, key);
-        float s = 0.f, dp = 0.f;
-        for (int d = 0; d < D; ++d) {
-          s = __builtin_fmaf(Elem<DT>::load(q[d]), Elem<DT>::load(kr[d]), s);
-          dp = __builtin_fmaf(Elem<DT>::load(g[d]), Elem<DT>::load(vr[d]), dp);
-        }
-        ds = exp2f(s * a.c - lse_r) * (dp - delta_r);
-      }
-      const int n = min(64, hi_r - first);
-      for (int j = 0; j < n; ++j) {
-        const float x = __shfl(ds, j);
-        const uint16_t* kr = row_of(a.k, a.ks, b, hk, first + j);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (lane + 64 * u < D) sum[u] = __builtin_fmaf(x, Elem<DT>::load(kr[lane + 64 * u]), sum[u]);
-      }
-    }
-    uint16_t* dst = a.dq + ((static_cast<int64_t>(b) * a.n_queries + i_r) * a.n_q + hq_r) * D;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < D) dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sum[u] * (hi_r - lo_r == 1 ? 0.f : a.scale)));
-  }
+  const float factor = hi - lo == 1 ? 0.f : a.scale * ldexpf(1.f, -kUp<DT>);
+  uint16_t* const dq = a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
+  store_row<DT, D>(acc, factor, live ? dq : nullptr, lane);
+  if (again != 0) dq_again<DT, D, RW>(a, again, lse, delta, block_up);
 }
 
 // What the workgroups of the next kernel do: a workgroup per pair, a lane per key tile, the row blocks dealt to 16 wavefronts.
@@ -411,6 +459,104 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
   for (int u = next + lane; u < a.units; u += 64) list[u] = int4{-1, 0, 0, -1};
 }
 
+// The pair of a workgroup of the next kernel, and which of its units it takes.  (The pair varies fastest: dealt to the XCDs by their unit, a
+// tile's first units all went to a few.)
+__device__ __forceinline__ int todo_pair(const BwdArgs& a, int* unit = nullptr) {
+  const int pairs = a.batch * a.n_kv, id = blockIdx.x, from = pairs % 8 == 0 ? id >> 3 : id, per = pairs % 8 == 0 ? pairs >> 3 : pairs;
+  const int u = a.by_pairs.div(from);
+  if (unit != nullptr) *unit = u;
+  return pairs % 8 == 0 ? (id & 7) * per + (from - u * per) : from - u * per;
+}
+
+// Keys whose sum is not a number: again (see Odd, attention.h), those of this wavefront's that `again` has a bit for, over all rows of its
+// unit, unless a row that sees the key makes the whole sum NaN (by its L, or for dK by its delta).  (A query that is not finite has no
+// probability where its L is a number, so that its slope times it is NaN.)  The place is found once more, as in dq_again.
+template <int DT, int D>
+__device__ __forceinline__ void dkv_again(const BwdArgs& a, uint32_t again, int4 todo) {
+  using T = AttnTile<D>;
+  int tid = threadIdx.x, pair = todo_pair(a), tile = __builtin_amdgcn_readfirstlane(todo.x), first = __builtin_amdgcn_readfirstlane(todo.y);
+  const int last = __builtin_amdgcn_readfirstlane(todo.z);
+  asm volatile("" : "+v"(tid), "+s"(pair), "+s"(tile), "+s"(first));
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, half = wave & 1, rg = wave >> 1;
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
+  const int k0 = tile * kKeyTile, key = k0 + half * 32 + (lane & 31);
+  const uint16_t* qb = a.q + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[1];
+  const uint16_t* gb = a.g + b * a.gs[0] + static_cast<int64_t>(hk) * a.group * a.gs[1];
+  const uint32_t* info_base = a.info + static_cast<int64_t>(pair) * a.row_blocks * kInfoWords;
+  for (int t = last - 1; t >= first && again != 0; --t) {  // (the last rows first: under a causal mask they see the most)
+    const uint32_t* info = info_base + static_cast<int64_t>(t) * kInfoWords;
+    const float l = __uint_as_float(info[lane & 31]), delta = __uint_as_float(info[32 + (lane & 31)]);
+    for (uint32_t rows = columns(l != l || (rg == 0 && delta != delta)); rows != 0 && again != 0; rows &= rows - 1) {
+      const int i = __builtin_ctz(rows);
+      again &= ~columns(key >= static_cast<int>(info[64 + i]) && key < static_cast<int>(info[96 + i]));
+    }
+  }
+  if (again == 0) return;
+  const bool redo = again >> (lane & 31) & 1, whole = todo.w < 0;
+  const int in_key = key < a.n_keys ? key : 0;
+  const uint16_t *k = row_of(a.k, a.ks, b, hk, in_key), *v = row_of(a.v, a.vs, b, hk, in_key);
+  const float scale = rg == 0 ? a.scale : 1.f;
+  uint16_t* const grad = rg == 0 ? a.dk : a.dv;
+  float* const part = a.part + (static_cast<int64_t>(pair) * a.units + todo.w) * (kKeyTile * 2 * D) + rg * D;
+  auto row_at = [&](const uint16_t* base, const int64_t* st, int t, int i) {  // (a row past the last is the last, and sees nothing here)
+    const int row = min(t * 32 + i, a.rows - 1), at = a.by_group.div(row);
+    return base + at * st[2] + (row - at * a.group) * st[1];
+  };
+  float of = 1.f, back = 1.f;  // dK's slopes times the power that all rows of the unit fit fp16 with, dV's probabilities as they are
+  if constexpr (DT == WX_F16) {
+    int least = kUp<DT>;
+    if (rg == 0)
+      for (int t = first; t < last; ++t) least = min(least, static_cast<int>(info_base[static_cast<int64_t>(t) * kInfoWords + 131]));
+    of = ldexpf(1.f, least - kUp<DT>), back = ldexpf(1.f, -least);
+  }
+  for (int o = 0; o < T::kOut; ++o) {
+    f32x16 sum = {};
+    const int c = 32 * o + (lane & 31);
+    for (int t = first; t < last; ++t) {
+      const uint32_t* info = info_base + static_cast<int64_t>(t) * kInfoWords;
+      const uint16_t *q = row_at(qb, a.qs, t, lane & 31), *g = row_at(gb, a.gs, t, lane & 31);
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int u = 0; u < T::kSteps; ++u) {
+        s = mfma<DT>(*reinterpret_cast<const u32x4*>(q + 16 * u + 8 * h), *reinterpret_cast<const u32x4*>(k + 16 * u + 8 * h), s);
+        dp = mfma<DT>(*reinterpret_cast<const u32x4*>(g + 16 * u + 8 * h), *reinterpret_cast<const u32x4*>(v + 16 * u + 8 * h), dp);
+        in_order();
+      }
+      uint32_t seen = 0, zero = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = 8 * (r / 4) + 4 * h + r % 4, lo = static_cast<int>(info[64 + i]), hi = static_cast<int>(info[96 + i]);
+        const bool sees = redo && key >= lo && key < hi;
+        float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -__uint_as_float(info[i])));
+        if (rg == 0) {
+          const float delta = __uint_as_float(info[32 + i]);
+          x *= ((hi - lo == 1 ? delta : dp[r]) - delta) * of;
+        }
+        s[r] = sees ? x : 0.f;
+        seen |= sees ? 1u << r : 0u;
+        zero |= sees && x == 0.f ? 1u << r : 0u;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        Odd odd;
+        const u32x4 x = gather_cols<DT>(u, h, odd, [&](int i) -> uint32_t {
+          return D % 32 != 0 && c >= D ? 0u : *((rg == 0 ? row_at(qb, a.qs, t, i) : row_at(gb, a.gs, t, i)) + c);
+        });
+        in_order();
+        sum = mfma<DT>(x, pack_step<DT>(s, u), sum);
+        if (rg == 0) odd.nan |= odd.plus | odd.minus, odd.plus = odd.minus = 0;
+        add_odd<DT>(sum, odd, seen, rg == 0 ? 0u : zero, u);
+        in_order();
+      }
+    }
+    if constexpr (DT == WX_F16)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[r] *= back;
+    if (whole) store_cols<DT, D>(sum, o, scale, redo ? grad + ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D : nullptr, lane);
+    else if (redo) store_sums<D>(sum, o, part + (key - k0) * 2 * D, lane);
+  }
+}
+
 // A wavefront holds 32 keys (K and V as B operands, dK^T and dV^T as accumulators) and takes every second block of 32 rows of Q and dO
 // of the workgroup's unit; two such wavefronts make the 64 keys of a workgroup, and the other two take the blocks in between.  S has
 // rows in its registers here and a key per column, so that P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
@@ -429,16 +575,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   __shared__ u32x4 s_v[kHeld < T::kSteps ? T::kSteps - kHeld : 1][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int half = wave & 1, rg = wave >> 1;
-  const int pairs = a.batch * a.n_kv;
-  // (the pair varies fastest: dealt to the XCDs by their unit, a tile's first units all went to a few)
-  int pair;
-  int4 todo;
-  {
-    const int id = blockIdx.x, from = pairs % 8 == 0 ? id >> 3 : id, per = pairs % 8 == 0 ? pairs >> 3 : pairs;
-    const int unit = a.by_pairs.div(from);
-    pair = pairs % 8 == 0 ? (id & 7) * per + (from - unit * per) : from - unit * per;
-    todo = a.list[static_cast<int64_t>(pair) * a.units + unit];
-  }
+  int unit;
+  const int pair = todo_pair(a, &unit);
+  const int4 todo = a.list[static_cast<int64_t>(pair) * a.units + unit];
   const int tile = __builtin_amdgcn_readfirstlane(todo.x), first = __builtin_amdgcn_readfirstlane(todo.y), last = __builtin_amdgcn_readfirstlane(todo.z);
   if (tile < 0) return;
   const bool whole = todo.w < 0;
@@ -635,73 +774,19 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dk[o][r] = (rg == 0 ? dk[o][r] : dv[o][r]) + take[(16 * o + r) * 64];  // (from here on: what this group finishes)
   }
-  bool bad = false;
-#pragma unroll
-  for (int o = 0; o < T::kOut; ++o)
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (32 * o + 8 * (r / 4) < D) bad = bad || dk[o][r] != dk[o][r];
   const float scale = rg == 0 ? a.scale : 1.f;
   uint16_t* const grad = rg == 0 ? a.dk : a.dv;
   // (of this unit's first key)
   float* const part = a.part + (static_cast<int64_t>(pair) * a.units + todo.w) * (kKeyTile * 2 * D) + rg * D;
+  uint32_t again = columns(live && not_numbers<D>(dk));
   if (whole) {
     store_row<DT, D>(dk, scale, live ? grad + ((static_cast<int64_t>(b) * a.n_keys + key) * a.n_kv + hk) * D : nullptr, lane);
   } else if (live) {
-    float* dst = part + (key - k0) * 2 * D;
 #pragma unroll
-    for (int o = 0; o < T::kOut; ++o)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * o + 8 * g < D) *reinterpret_cast<float4*>(dst + 32 * o + 8 * g + 4 * h) = float4{dk[o][4 * g], dk[o][4 * g + 1], dk[o][4 * g + 2], dk[o][4 * g + 3]};
+    for (int o = 0; o < T::kOut; ++o) store_sums<D>(dk[o], o, part + (key - k0) * 2 * D, lane);
   }
-  // Keys whose sums are not numbers, in plain loops over the rows that see them.
-  uint64_t redo = __ballot(bad && live);
-  redo = (redo | redo >> 32) & 0xffffffffull;
-  while (redo != 0) {
-    const int r = __builtin_ctzll(redo);
-    redo &= redo - 1;
-    const int key_r = wk + r;
-    const uint16_t *kr = row_of(a.k, a.ks, b, hk, key_r), *vr = row_of(a.v, a.vs, b, hk, key_r);
-    float sum[2] = {0.f, 0.f};
-    for (int t = first * 32; t < min(last * 32, a.rows); t += 64) {
-      const int row = t + lane;
-      float x = 0.f;  // the row's P, or its dS
-      bool see = false;
-      if (row < a.rows && row < last * 32) {
-        const uint32_t* info = info_base + static_cast<int64_t>(row / 32) * kInfoWords + row % 32;
-        see = key_r >= static_cast<int>(info[64]) && key_r < static_cast<int>(info[96]);
-        if (see) {
-          const int hq = hk * a.group + row % a.group;
-          const uint16_t *q = row_of(a.q, a.qs, b, hq, row / a.group), *g = row_of(a.g, a.gs, b, hq, row / a.group);
-          float s = 0.f, d = 0.f;
-          for (int e = 0; e < D; ++e) {
-            s = __builtin_fmaf(Elem<DT>::load(q[e]), Elem<DT>::load(kr[e]), s);
-            d = __builtin_fmaf(Elem<DT>::load(g[e]), Elem<DT>::load(vr[e]), d);
-          }
-          x = exp2f(s * a.c - (__uint_as_float(info[0]) + kUp<DT>));
-          if (rg == 0) x *= (info[96] - info[64] == 1 ? __uint_as_float(info[32]) : d) - __uint_as_float(info[32]);
-        }
-      }
-      uint64_t seen = __ballot(see);
-      while (seen != 0) {
-        const int j = __builtin_ctzll(seen);
-        seen &= seen - 1;
-        const float xj = __shfl(x, j);
-        const int hq = hk * a.group + (t + j) % a.group;
-        const uint16_t* w = rg == 0 ? row_of(a.q, a.qs, b, hq, (t + j) / a.group) : row_of(a.g, a.gs, b, hq, (t + j) / a.group);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (lane + 64 * u < D) sum[u] = __builtin_fmaf(xj, Elem<DT>::load(w[lane + 64 * u]), sum[u]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < D) {
-        if (whole) grad[((static_cast<int64_t>(b) * a.n_keys + key_r) * a.n_kv + hk) * D + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(sum[u] * scale));
-        else part[(key_r - k0) * 2 * D + lane + 64 * u] = sum[u];
-      }
-  }
+
+  if (again != 0) dkv_again<DT, D>(a, again, todo);
 }
 
 // dK and dV of the keys of a tile of several units, from the units' sums: four workgroups per tile, a thread per 4 channels (one

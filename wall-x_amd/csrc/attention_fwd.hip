@@ -43,49 +43,127 @@ __device__ __forceinline__ uint32_t widen2(uint32_t x, float power = 1.0f) {
 // of the result for values of 0.001, against 0.03 %).
 __device__ __forceinline__ uint32_t scale_power(float scale) { return min(__float_as_uint(scale) & 0x7f800000u, 134u << 23); }
 
-template <int DT, bool F8>
-__device__ __forceinline__ float load_kv(const void* p, int64_t i) {
-  if constexpr (F8) {
-    const uint32_t x = static_cast<const uint8_t*>(p)[i];
-    return Elem<DT>::load(widen2<DT, false>(x) & 0xffffu);
-  } else {
-    return Elem<DT>::load(static_cast<const uint16_t*>(p)[i]);
-  }
+// The keys of this workgroup's split.
+__device__ __forceinline__ int2* split_share() {
+  __shared__ int2 s;
+  return &s;
 }
 
-// One row by one wavefront in plain loops: for rows whose tile holds a key that they do not see with a value that is not
-// finite (0 * inf in the matrix product).  Lane l gets channels l and l + 64 of the unscaled sum.
-template <int DT, int D, bool F8>
-__device__ __forceinline__ void plain_row(const FwdArgs& a, int b, int hk, int row, int lo, int hi, int lane, float& m, float& l,
-                                          float (&o)[2]) {
-  const int i = row / a.group, hq = hk * a.group + row % a.group;
-  const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + hq * a.qs[1] + i * a.qs[2];
-  const int64_t kb = b * a.ks[0] + hk * a.ks[1], vb = b * a.vs[0] + hk * a.vs[1], sb = (static_cast<int64_t>(b) * a.n_kv + hk) * a.n_keys;
-  m = -kInf;
-  l = 0.f;
-  o[0] = o[1] = 0.f;
-  for (int first = lo; first < hi; first += 64) {
-    const int key = first + lane;
-    float s = -kInf;
-    if (key < hi) {
-      float dot = 0.f;
-      for (int d = 0; d < D; ++d) dot = __builtin_fmaf(Elem<DT>::load(q[d]), load_kv<DT, F8>(a.k, kb + key * a.ks[2] + d), dot);
-      s = F8 ? dot * a.k_scale[sb + key] : dot;
-    }
-    const float mn = fmaxf(m, wave_max(s)), mc = mn == -kInf ? 0.f : mn * a.c;
-    const float alpha = exp2f(m * a.c - mc), p = key < hi ? exp2f(s * a.c - mc) : 0.f;
-    l = l * alpha + wave_sum(p);
-    o[0] *= alpha;
-    o[1] *= alpha;
-    const int n = min(64, hi - first);
-    for (int j = 0; j < n; ++j) {
-      float pj = __shfl(p, j);
-      if constexpr (F8) pj *= a.v_scale[sb + first + j];
+// ---- Rows again (see Odd, attention.h), of this wavefront's those that `again` has a bit for, with the maximum and the sum that they ended
+// with.  Their place is found once more: kept over the kernel's loops for this rare case it costs them registers.
+template <int DT, int D, bool F8, int RW>
+__device__ __forceinline__ void rows_again(const FwdArgs& a, uint32_t again, float m, float l) {
+  using T = AttnTile<D>;
+  constexpr int KW = RW == 8 ? 1 : 4 / RW, kElem = F8 ? 1 : 2;
+  constexpr bool kPowers = F8 && DT == WX_F16;
+  int id = blockIdx.x, tid = threadIdx.x;
+  asm volatile("" : "+s"(id), "+v"(tid));
+  const int lane = tid & 63, rw = __builtin_amdgcn_readfirstlane(tid >> 6) % RW, h = lane >> 5;
+  const int rest = a.by_splits.div(id), split = id - rest * a.splits;
+  int pair, tile;
+  a.spread.place(rest, pair, tile);
+  const int b = a.by_kv.div(pair), hk = pair - b * a.n_kv;
+  const int row = tile * 32 * RW + rw * 32 + (lane & 31), in_row = row < a.rows ? row : 0, qi = a.by_group.div(in_row), hq = hk * a.group + in_row - qi * a.group;
+  const bool redo = again >> (lane & 31) & 1;
+  int lo = 0, hi = 0;
+  if (redo) key_range(a.mask, b, qi, a.n_queries, a.n_keys, lo, hi);
+  if constexpr (KW > 1) {
+    const int2 share = *split_share();
+    lo = max(lo, share.x), hi = min(hi, share.y);
+  }
+  const int from = wave_extreme<false>(redo ? lo : 0x7fffffff), up_to = wave_extreme<true>(hi);
+  const float mc = m == -kInf ? 0.f : m * a.c;
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + hq * a.qs[1] + qi * a.qs[2];
+  const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
+  const char* kp = static_cast<const char*>(a.k) + (b * a.ks[0] + hk * a.ks[1]) * kElem;
+  const char* vp = static_cast<const char*>(a.v) + (b * a.vs[0] + hk * a.vs[1]) * kElem;
+  const int64_t k_step = a.ks[2] * kElem, v_step = a.vs[2] * kElem;
+  const float* ksc = F8 ? a.k_scale + (static_cast<int64_t>(b) * a.n_kv + hk) * a.n_keys : nullptr;
+  const float* vsc = F8 ? a.v_scale + (static_cast<int64_t>(b) * a.n_kv + hk) * a.n_keys : nullptr;
+  auto in = [&](int k0, int i) { return min(i, a.n_keys - 1 - k0); };  // (a key past the last is the last, and not seen)
+  // the probabilities (times what scale their values do not carry) of keys k0 .. + 31, zeros for what is not seen and for other rows
+  auto powers = [&](int k0, f32x16& s, uint32_t& seen) {
+    const char* kr = kp + k0 * k_step + in(k0, lane & 31) * static_cast<int>(k_step);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < D) o[u] = __builtin_fmaf(pj, load_kv<DT, F8>(a.v, vb + (first + j) * a.vs[2] + lane + 64 * u), o[u]);
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      u32x4 x;
+      if constexpr (F8) {
+        const u32x2 y = *reinterpret_cast<const u32x2*>(kr + 16 * t + 8 * h);
+        x = u32x4{widen2<DT, false>(y[0]), widen2<DT, true>(y[0]), widen2<DT, false>(y[1]), widen2<DT, true>(y[1])};
+      } else {
+        x = *reinterpret_cast<const u32x4*>(kr + (16 * t + 8 * h) * 2);
+      }
+      s = mfma<DT>(x, *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h), s);
+      in_order();
     }
-    m = mn;
+    seen = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = 8 * (r / 4) + 4 * h + r % 4, key = k0 + i;
+      const bool sees = redo && key >= lo && key < hi;
+      if constexpr (F8) {
+        const int at = k0 + in(k0, i);
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r] * ksc[at], a.c, -mc)) * (kPowers ? vsc[at] * __uint_as_float((254u << 23) - scale_power(vsc[at])) : vsc[at]);
+      } else {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -mc));
+      }
+      s[r] = sees ? s[r] : 0.f;
+      seen |= sees ? 1u << r : 0u;
+    }
+  };
+  int less = 0;  // (fp16 codes) a power of two that brings the row's largest probability times scale into fp16
+  if constexpr (kPowers) {
+    float top = 0.f;
+    for (int k0 = from; k0 < up_to; k0 += 32) {
+      f32x16 s;
+      uint32_t seen;
+      powers(k0, s, seen);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[r]));
+    }
+    top = both_max(top);
+    less = top < kInf ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, 0) : 0;
+  }
+  const float f = ldexpf(1.f, -less), back = ldexpf(1.f, less);
+  for (int o = 0; o < T::kOut; ++o) {
+    f32x16 sum = {};
+    const int c = 32 * o + (lane & 31);
+    for (int k0 = from; k0 < up_to; k0 += 32) {
+      f32x16 s;
+      uint32_t seen, zero = 0;
+      powers(k0, s, seen);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        zero |= s[r] == 0.f ? seen & 1u << r : 0u;
+        if constexpr (kPowers) s[r] *= f;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Odd odd;
+        const u32x4 x = gather_cols<DT>(t, h, odd, [&](int i) -> uint32_t {
+          if (D % 32 != 0 && c >= D) return 0;
+          const char* v = vp + k0 * v_step + (in(k0, i) * static_cast<int>(v_step) + c * kElem);
+          if constexpr (F8) return widen2<DT, false>(*reinterpret_cast<const uint8_t*>(v), kPowers ? __uint_as_float(scale_power(vsc[k0 + in(k0, i)])) : 1.f) & 0xffffu;
+          else return *reinterpret_cast<const uint16_t*>(v);
+        });
+        in_order();
+        sum = mfma<DT>(x, pack_step<DT>(s, t), sum);
+        add_odd<DT>(sum, odd, seen, zero, t);
+        in_order();
+      }
+    }
+    if constexpr (kPowers)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[r] *= back;
+    if (KW > 1 && a.splits > 1) {
+      if (redo) store_sums<D>(sum, o, a.part + ((static_cast<int64_t>(pair) * a.splits + split) * a.rows + row) * D, lane);
+    } else if (!F8 && a.rest != nullptr) {
+      store_cols<DT, D, true>(sum, o, 1.f / l, redo ? a.out + to : nullptr, lane, redo ? a.rest + to : nullptr);
+    } else {
+      store_cols<DT, D>(sum, o, 1.f / l, redo ? a.out + to : nullptr, lane);
+    }
   }
 }
 
@@ -170,6 +248,7 @@ __global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 
     g_hi = min(g_hi, g_lo + t1 * KB);
     g_lo += t0 * KB;
   }
+  if (KW > 1 && tid == 0) *split_share() = int2{g_lo, g_hi};  // (behind the first of many barriers)
   const int s_lo = max(lo, g_lo), s_hi = min(hi, g_hi);
   const int tiles = __builtin_amdgcn_readfirstlane((g_hi - g_lo + KB - 1) / KB), iters = (tiles + KW - 1) / KW;
 
@@ -492,20 +571,19 @@ __global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 
       if (it + 1 < iters) turn(it + 1, other_slot, mine);
     }
   l = both_sum(l);
-
   // ---- the result: joined over the key groups, then either the row itself or this split's part of it
-  // (0 * inf from a key of a tile that this row does not see, or a value that is not finite that it does)
-  auto wrong_sum = [](float x) { return kPowers ? !(fabsf(x) < kInf) : x != x; };
+  // Rows whose sum is not a number though the sum of their powers is are made again at the end; of fp16 codes also rows whose probabilities
+  // times scales went beyond fp16.
   bool bad = false;
+#pragma unroll
+  for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (32 * o + 8 * (r / 4) < D) bad = bad || (kPowers ? !(fabsf(acc[o][r]) < kInf) : acc[o][r] != acc[o][r]);
+  uint32_t again = columns(bad && s_hi > s_lo);
   uint16_t* out = a.out + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
   const int64_t stat = static_cast<int64_t>(pair) * a.rows + row;
-  const int64_t part = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row;
   if constexpr (KW == 1) {
-#pragma unroll
-    for (int o = 0; o < T::kOut; ++o)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (32 * o + 8 * (r / 4) < D) bad = bad || wrong_sum(acc[o][r]);
     const float inv = some && l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     if (!F8 && a.rest != nullptr) store_row<DT, D, true>(acc, some ? inv : 0.f, live ? out : nullptr, lane, live ? a.rest + (out - a.out) : nullptr);
     else store_row<DT, D>(acc, some ? inv : 0.f, live ? out : nullptr, lane);
@@ -513,33 +591,27 @@ __global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 
 #pragma unroll
       for (int c = 0; c < D / 8; c += 2) *reinterpret_cast<u32x4*>(out + 8 * (c + h)) = u32x4{0u, 0u, 0u, 0u};
     }
+    again &= columns(l == l);
     if (a.lse != nullptr && live && h == 0) a.lse[stat] = some ? __builtin_fmaf(m, a.c, __builtin_amdgcn_logf(l)) : kInf;
-    uint64_t redo = __ballot(bad && some && live);
-    redo = (redo | redo >> 32) & 0xffffffffull;
-    while (redo != 0) {
-      const int r = __builtin_ctzll(redo);
-      redo &= redo - 1;
-      const int row_r = __shfl(row, r), lo_r = __shfl(lo, r), hi_r = __shfl(hi, r);
-      float m2, l2, o2[2];
-      plain_row<DT, D, F8>(a, b, hk, row_r, lo_r, hi_r, lane, m2, l2, o2);
-      uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.n_queries + row_r / a.group) * a.n_q + hk * a.group + row_r % a.group) * D;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < D) {
-          dst[lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(o2[u] / l2));
-          if (a.rest != nullptr) a.rest[dst - a.out + lane + 64 * u] = static_cast<uint8_t>(pack_rest(rest_of<DT>(o2[u] / l2), 0.f, 0.f, 0.f));
-        }
-    }
   } else {
     // Every key group's sums to LDS, 64 channels at a time, scaled to the common maximum; then a thread adds up 8 channels of a row.
     float2* stats = reinterpret_cast<float2*>(lds + kJoinStats);
     float* sums = reinterpret_cast<float*>(lds);
+    __shared__ uint32_t s_again[4];
     __syncthreads();
     if (h == 0) stats[wave * 32 + lane] = float2{m, l};
+    if (lane == 0) s_again[wave] = again;
     __syncthreads();
-    float top = -kInf;
+    float top = -kInf, l_all = 0.f;
 #pragma unroll
     for (int u = 0; u < KW; ++u) top = fmaxf(top, stats[(u * RW + rw) * 32 + (lane & 31)].x);
+#pragma unroll
+    for (int u = 0; u < KW; ++u) {
+      again |= s_again[u * RW + rw];
+      const float2 st = stats[(u * RW + rw) * 32 + (lane & 31)];
+      l_all += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top) * a.c);
+    }
+    again &= columns(l_all == l_all);
     const float f = m == -kInf ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.c);
 #pragma unroll
     for (int c0 = 0; c0 < D; c0 += 64) {
@@ -573,57 +645,38 @@ __global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 
           for (int u = 0; u < KW; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += sums[((u * RW + rw) * 32 + r) * 68 + (ch * 8 - c0) + e];
-        bool wrong = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) wrong = wrong || wrong_sum(v[e]);
         const int i_r = row_r < a.rows ? a.by_group.div(row_r) : 0;
         int lo_r = 0, hi_r = 0;
         if (row_r < a.rows) key_range(a.mask, b, i_r, a.n_queries, a.n_keys, lo_r, hi_r);
         const bool some_r = hi_r > lo_r;
-        const int slo = max(lo_r, g_lo), shi = min(hi_r, g_hi);
         const int64_t to = ((static_cast<int64_t>(b) * a.n_queries + i_r) * a.n_q + hk * a.group + row_r - i_r * a.group) * D;
         const int64_t to_part = (static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_r;
+        const bool store_r = !(again >> r & 1);
         if (mine_r) {
           if (a.splits > 1) {
             float4* dst = reinterpret_cast<float4*>(a.part + to_part * D + ch * 8);
-            dst[0] = float4{v[0], v[1], v[2], v[3]};
-            dst[1] = float4{v[4], v[5], v[6], v[7]};
+            if (store_r) {
+              dst[0] = float4{v[0], v[1], v[2], v[3]};
+              dst[1] = float4{v[4], v[5], v[6], v[7]};
+            }
             if (ch == 0) part_stats(a, D)[to_part] = float2{top_r, l_r};
           } else {
             const float inv = some_r ? 1.f / l_r : 0.f;
             float w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = some_r ? v[e] * inv : 0.f;
-            *reinterpret_cast<u32x4*>(a.out + to + ch * 8) = pack16<DT>(w);
-            if (a.rest != nullptr)
+            if (store_r) *reinterpret_cast<u32x4*>(a.out + to + ch * 8) = pack16<DT>(w);
+            if (store_r && a.rest != nullptr)
               *reinterpret_cast<u32x2*>(a.rest + to + ch * 8) = u32x2{pack_rest_of<DT>(w[0], w[1], w[2], w[3]), pack_rest_of<DT>(w[4], w[5], w[6], w[7])};
             if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(pair) * a.rows + row_r] = some_r ? __builtin_fmaf(top_r, a.c, __builtin_amdgcn_logf(l_r)) : kInf;
           }
         }
-        uint64_t redo = __ballot(wrong && mine_r && shi > slo);
-        while (redo != 0) {
-          const int at = __builtin_ctzll(redo) / kLanes * kLanes;
-          redo &= ~(0xffull << at);
-          const int row_x = __shfl(row_r, at), lo_x = __shfl(slo, at), hi_x = __shfl(shi, at);
-          const float top_x = __shfl(top_r, at);
-          float m2, l2, o2[2];
-          plain_row<DT, D, F8>(a, b, hk, row_x, lo_x, hi_x, lane, m2, l2, o2);
-          const int c = c0 + lane;
-          if (c < D) {  // the same channels and the same maximum as above
-            if (a.splits > 1) {
-              const float scale = m2 == -kInf ? 1.f : exp2f((m2 - top_x) * a.c);
-              a.part[((static_cast<int64_t>(pair) * a.splits + split) * a.rows + row_x) * D + c] = o2[c0 / 64] * scale;
-            } else {
-              const int i_x = a.by_group.div(row_x);
-              const int64_t to_x = ((static_cast<int64_t>(b) * a.n_queries + i_x) * a.n_q + hk * a.group + row_x - i_x * a.group) * D + c;
-              a.out[to_x] = static_cast<uint16_t>(Elem<DT>::store(o2[c0 / 64] / l2));
-              if (a.rest != nullptr) a.rest[to_x] = static_cast<uint8_t>(pack_rest(rest_of<DT>(o2[c0 / 64] / l2), 0.f, 0.f, 0.f));
-            }
-          }
-        }
       }
     }
+    if (kw != 0) return;
+    m = top, l = l_all;
   }
+  if (again != 0) rows_again<DT, D, F8, RW>(a, again, m, l);
 }
 
 constexpr int kMaxSplits = 256;
