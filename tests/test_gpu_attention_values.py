@@ -11,6 +11,7 @@ import torch
 
 from test_gpu_attention import check, heads, reference, visible
 from test_gpu_kv_cache import quantise
+from wallx_mi355 import native
 from wallx_mi355.fusions import ops
 
 pytestmark = pytest.mark.gpu
@@ -157,3 +158,19 @@ def test_gradients_far_apart(dev):
             beside = 2.0 ** -34 * 2.0 ** 13 * 64 * (D ** -0.5 * 75 * 5 if name != "dv" else 0.0)
             a, value, tol = held(a[:, :, part], value, tol + beside)
             check(a, (value, tol), f"{name} of sequence {n}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sigma", [64.0, 1.0, 2.0 ** -6, 2.0 ** -9])
+@pytest.mark.parametrize("B,Hq,Hkv,S,D", [(2, 4, 2, 64, 128), (40, 16, 2, 96, 64), (1, 3, 1, 100, 80)])
+def test_rests_of_the_output(dev, B, Hq, Hkv, S, D, sigma, dtype):
+    """delta = sum dO O is the difference of large numbers here: the values differ by a twentieth of their size, the keys by a tenth, so that dQ's
+    error is that of delta, sqrt(D) |dO| times what O's rounding leaves (u / sqrt 3 of it), which the rests take to an eighth: their
+    three bits.  Everything else is below a tenth of the error without them (a slope's rounding, u / sqrt 3 of P sigma sqrt(D) / 20 over S keys,
+    is 1 / (20 sqrt(S)) of it), so that half is more than what may be left."""
+    g = torch.Generator(device=dev).manual_seed(S)
+    q, k, v, do = heads(B, S, Hq, D, dtype, g, dev) * 0.1, 1 + 0.1 * heads(B, S, Hkv, D, dtype, g, dev), sigma * (1 + 0.05 * heads(B, S, Hkv, D, dtype, g, dev)), heads(B, S, Hq, D, dtype, g, dev)
+    want = reference(q, k, v, visible(B, S, S, dev), 1.0, do)["dq"][0]
+    out, lse, rest = native.attention_fwd(q, k, v, scale=1.0, want_lse=True)
+    errors = [float((native.attention_bwd(do, q, k, v, out, lse, r, scale=1.0)[0].double() - want).norm()) for r in (rest, None)]
+    assert errors[0] < 0.5 * errors[1], f"{errors[0] / errors[1]:.3f} of the error without"

@@ -283,13 +283,18 @@ __device__ __forceinline__ void wait_lds() {
 }
 
 // What rounding the output to its type leaves, as e5m2, for the backward's delta = rowsum(dO O): with O as rounded, delta's error is
-// a quarter of dQ's.  (Too small for e5m2 where the output is below 2^-7 or so: such a part of delta has no weight beside
-// the slopes.)
+// a quarter of dQ's, or most of it where the values differ by little of their size.  It is kept times a power of two that puts what
+// outputs can leave into e5m2's range, 2^-16 to 57344: all of fp16's (2^-25 to 16), and what outputs of 2^-16 to 2^16 leave in bf16.  (Beyond that
+// the backward leaves a row's rests out; below, they are zero.)
+template <int DT>
+constexpr float kRestUp = DT == WX_F16 ? 2048.f : 256.f;
 __device__ __forceinline__ uint32_t pack_rest(float a, float b, float c, float d) {
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_bf8_f32(c, d, __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false), true));
 }
 template <int DT>
-__device__ __forceinline__ float rest_of(float x) { return x - Elem<DT>::round(x); }
+__device__ __forceinline__ float rest_of(float x, float rounded) { return (x - rounded) * kRestUp<DT>; }
+template <int DT>
+__device__ __forceinline__ float rest_of(float x) { return rest_of<DT>(x, Elem<DT>::round(x)); }
 template <int DT>
 __device__ __forceinline__ uint32_t pack_rest_of(float a, float b, float c, float d) {
   return pack_rest(rest_of<DT>(a), rest_of<DT>(b), rest_of<DT>(c), rest_of<DT>(d));
@@ -313,8 +318,8 @@ __device__ __forceinline__ void store_cols(const f32x16& acc, int o, float facto
       uint32_t r[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        r[u] = pack_rest(x[4 * u] - Elem<DT>::load(a[2 * u] & 0xffffu), x[4 * u + 1] - Elem<DT>::load(a[2 * u] >> 16),
-                         x[4 * u + 2] - Elem<DT>::load(a[2 * u + 1] & 0xffffu), x[4 * u + 3] - Elem<DT>::load(a[2 * u + 1] >> 16));
+        r[u] = pack_rest(rest_of<DT>(x[4 * u], Elem<DT>::load(a[2 * u] & 0xffffu)), rest_of<DT>(x[4 * u + 1], Elem<DT>::load(a[2 * u] >> 16)),
+                         rest_of<DT>(x[4 * u + 2], Elem<DT>::load(a[2 * u + 1] & 0xffffu)), rest_of<DT>(x[4 * u + 3], Elem<DT>::load(a[2 * u + 1] >> 16)));
       const auto y = __builtin_amdgcn_permlane32_swap(r[0], r[1], false, false);
       if (rest != nullptr) *reinterpret_cast<u32x2*>(rest + 32 * o + 8 * (g + h)) = u32x2{y[0], y[1]};
     }

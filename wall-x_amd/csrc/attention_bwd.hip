@@ -22,7 +22,7 @@ struct BwdArgs {
   const uint16_t *q, *k, *v, *g;  // g = dO
   int64_t qs[3], ks[3], vs[3], gs[3];
   const uint16_t* out;            // [batch, n_queries, n_q, D]
-  const uint8_t* rest;            // like out: what its rounding left (rest_of), or null
+  const uint8_t* rest;            // like out: what its rounding left times kRestUp, or null
   const float* lse;               // [batch, n_kv, rows]
   uint16_t *dq, *dk, *dv;         // [batch, n_queries, n_q, D], [batch, n_keys, n_kv, D]
   AttnMask mask;
@@ -219,8 +219,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) rests = dot2<DT>(gf[t][2 * u + 1], widen_rest2<DT, true>(rf[t][u]), dot2<DT>(gf[t][2 * u], widen_rest2<DT, false>(rf[t][u]), rests));
   }
-  rests = both_sum(rests);
-  // (a rest that e5m2 does not hold, of outputs of 10^7 and more, is left out)
+  rests = both_sum(rests) * (1.f / kRestUp<DT>);
+  // (rests that e5m2 does not hold are left out)
   const float delta = some ? both_sum(sums[0] + sums[1]) + (fabsf(rests) < kInf ? rests : 0.f) : 0.f;
   lse = some ? lse : kInf;
   constexpr bool kFit = DT == WX_F16;

@@ -14,7 +14,7 @@ struct FwdArgs {
   const float *k_scale, *v_scale;  // e4m3: [batch, n_kv, n_keys]
   uint16_t* out;                 // [batch, n_queries, n_q, D]
   float* lse;                    // [batch, n_kv, n_queries * group], base 2, or null
-  uint8_t* rest;                 // with lse: what out's rounding left (rest_of), like out, or null
+  uint8_t* rest;                 // with lse: what out's rounding left times kRestUp, like out, or null
   AttnMask mask;
   int batch, n_q, n_kv, n_queries, n_keys, group;
   int rows, row_tiles, splits;
