@@ -886,7 +886,7 @@ using namespace wx;
 
 extern "C" size_t wx_attention_bwd_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys,
                                                    int head_dim) {
-  if (batch <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_queries < 0 || n_keys < 0 || head_dim <= 0) return 0;
+  if (batch <= 0 || n_q_heads < 0 || n_kv_heads <= 0 || n_queries < 0 || n_keys < 0 || head_dim <= 0) return 0;
   return layout(batch * n_kv_heads, n_queries * (n_q_heads / n_kv_heads), n_keys, head_dim).total;
 }
 
@@ -899,9 +899,10 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   const char* who = "wx_attention_bwd";
   if (int rc = attention_check(who, batch, n_q_heads, n_kv_heads, n_queries, n_keys, head_dim, dtype, scale)) return rc;
   if (!q_strides || !k_strides || !v_strides || !grad_strides) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null strides", who);
-  if (batch == 0 || n_q_heads == 0) return WX_OK;
-  const int group = n_q_heads / n_kv_heads;
-  if ((n_queries > 0 && (!q || !out || !lse || !grad_out || !grad_q)) || (n_keys > 0 && (!k || !v || !grad_k || !grad_v)))
+  if (batch == 0 || n_kv_heads == 0) return WX_OK;
+  const int group = std::max(n_q_heads / n_kv_heads, 1);
+  const int64_t rows = n_queries * (n_q_heads / n_kv_heads);  // (none without query heads: the keys' gradients are zeros then, as without queries)
+  if ((rows > 0 && (!q || !out || !lse || !grad_out || !grad_q)) || (n_keys > 0 && (!k || !v || !grad_k || !grad_v)))
     return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   for (const void* p : {q, k, v, out, rest, grad_out, static_cast<const void*>(grad_q), static_cast<const void*>(grad_k), static_cast<const void*>(grad_v),
                         static_cast<const void*>(workspace)})
@@ -918,7 +919,7 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   a.dq = static_cast<uint16_t*>(grad_q), a.dk = static_cast<uint16_t*>(grad_k), a.dv = static_cast<uint16_t*>(grad_v);
   a.mask = {reinterpret_cast<const int2*>(key_ranges), key_lengths, causal};
   a.batch = static_cast<int>(batch), a.n_q = n_q_heads, a.n_kv = n_kv_heads, a.n_queries = static_cast<int>(n_queries), a.n_keys = static_cast<int>(n_keys);
-  a.group = group, a.rows = static_cast<int>(n_queries) * group, a.row_blocks = (a.rows + 31) / 32;
+  a.group = group, a.rows = static_cast<int>(rows), a.row_blocks = (a.rows + 31) / 32;
   a.c = scale * kLog2e, a.scale = scale;
   const int64_t pairs = batch * n_kv_heads;
   a.key_tiles = (a.n_keys + kKeyTile - 1) / kKeyTile;
