@@ -405,6 +405,21 @@ __device__ __forceinline__ u32x4 gather_cols(int t, int h, Odd& odd, At at) {
   for (int j = 0; j < 8; ++j) x[j] = at(16 * t + 8 * (j / 4) + 4 * h + j % 4);
   return finite8<DT>(x, odd);
 }
+// Whether one of a lane's sums is NaN (or, with INF, not finite).  (One comparison tells of two values.)
+template <int D, bool INF = false>
+__device__ __forceinline__ bool not_numbers(const f32x16* acc) {
+  bool bad = false;
+  float top = 0.f;
+#pragma unroll
+  for (int o = 0; o < AttnTile<D>::kOut; ++o)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2)
+      if (32 * o + 8 * (r / 4) < D) {
+        bad = bad | __builtin_isunordered(acc[o][r], acc[o][r + 1]);
+        if constexpr (INF) top = fmaxf(top, fmaxf(fabsf(acc[o][r]), fabsf(acc[o][r + 1])));
+      }
+  return bad || top == kInf;
+}
 // Which of the wavefront's 32 columns a predicate of its lanes holds for, in either half.
 __device__ __forceinline__ uint32_t columns(bool x) {
   const uint64_t b = __ballot(x);

@@ -62,17 +62,6 @@ __device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64
   return p + b * st[0] + h * st[1] + i * st[2];
 }
 
-template <int D>
-__device__ __forceinline__ bool not_numbers(const f32x16* acc) {
-  bool bad = false;
-#pragma unroll
-  for (int o = 0; o < AttnTile<D>::kOut; ++o)
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (32 * o + 8 * (r / 4) < D) bad = bad || acc[o][r] != acc[o][r];
-  return bad;
-}
-
 // Rows whose sum is not a number though their L and delta are: again (see Odd, attention.h), those of this wavefront's that `again` has a bit
 // for, times 2^up.  (A key that is not finite has no probability where L is a number, so that its slope times it is NaN.)  Their place is
 // found once more: kept over the kernel's loop for this rare case it costs that registers.

@@ -188,7 +188,7 @@ __device__ __forceinline__ void rows_again(const FwdArgs& a, uint32_t again, flo
 template <int DT, int D, bool F8, int RW>
 __global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
   using T = AttnTile<D>;
-  constexpr int KW = RW == 8 ? 1 : 4 / RW, KB = RW == 2 ? 32 : 64, NT = KB / 32;
+  constexpr int KW = RW == 8 ? 1 : 4 / RW, KB = RW == 2 ? 32 : 64, NT = KB / 32;  // (one or two key groups)
   constexpr bool kDirect = !F8;
   constexpr int kTileBytes = KB * T::kPitch;
   constexpr int kScaleBytes = F8 ? 2 * KB * 4 : 0;
@@ -574,13 +574,7 @@ __global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 
   // ---- the result: joined over the key groups, then either the row itself or this split's part of it
   // Rows whose sum is not a number though the sum of their powers is are made again at the end; of fp16 codes also rows whose probabilities
   // times scales went beyond fp16.
-  bool bad = false;
-#pragma unroll
-  for (int o = 0; o < T::kOut; ++o)
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (32 * o + 8 * (r / 4) < D) bad = bad || (kPowers ? !(fabsf(acc[o][r]) < kInf) : acc[o][r] != acc[o][r]);
-  uint32_t again = columns(bad && s_hi > s_lo);
+  uint32_t again = columns(not_numbers<D, kPowers>(acc) && s_hi > s_lo);
   uint16_t* out = a.out + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
   const int64_t stat = static_cast<int64_t>(pair) * a.rows + row;
   if constexpr (KW == 1) {
@@ -605,13 +599,15 @@ __global__ __launch_bounds__(RW == 8 ? 512 : 256, D == 80 && !F8 && RW == 4 ? 3 
     float top = -kInf, l_all = 0.f;
 #pragma unroll
     for (int u = 0; u < KW; ++u) top = fmaxf(top, stats[(u * RW + rw) * 32 + (lane & 31)].x);
+    again = __builtin_amdgcn_readfirstlane(s_again[rw] | s_again[rw + RW * (KW - 1)]);
+    if (again != 0) {
 #pragma unroll
-    for (int u = 0; u < KW; ++u) {
-      again |= s_again[u * RW + rw];
-      const float2 st = stats[(u * RW + rw) * 32 + (lane & 31)];
-      l_all += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top) * a.c);
+      for (int u = 0; u < KW; ++u) {
+        const float2 st = stats[(u * RW + rw) * 32 + (lane & 31)];
+        l_all += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top) * a.c);
+      }
+      again &= columns(l_all == l_all);
     }
-    again &= columns(l_all == l_all);
     const float f = m == -kInf ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.c);
 #pragma unroll
     for (int c0 = 0; c0 < D; c0 += 64) {
