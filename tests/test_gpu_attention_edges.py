@@ -28,3 +28,37 @@ def test_no_query_heads(dev, host, Sq, Sk):
         del junk
         dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.empty_like(out))
         assert dq.shape == q.shape and torch.equal(dk, torch.zeros_like(k)) and torch.equal(dv, torch.zeros_like(v))
+
+
+def _norm_inputs(dev):
+    from wallx_mi355 import workloads as wl
+
+    q, k = (torch.randn(2, h, 20, 128, device=dev).to(torch.bfloat16) for h in (4, 2))
+    w = torch.ones(128, dtype=torch.bfloat16, device=dev)
+    pos, freq, section = torch.arange(20, device=dev).expand(3, 2, 20).contiguous(), wl.text_inv_freq(128).to(dev), list(wl.MROPE_SECTION)
+    table = ops.multimodal_rope_table(pos, freq, section)
+    return q, k, w, lambda q, k, wq, wk: ops.qk_norm_rope_from_table(q, k, wq, wk, table, section), lambda q, k, wq, wk: ops.qk_norm_rope_from_positions(q, k, wq, wk, pos, freq, section)
+
+
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_is_refused(dev, host, leaf):
+    """A tangent is never dropped without a word, whether its tensor requires grad or not, and neither under no_grad."""
+    from torch.autograd import forward_ad as fw
+
+    q, k, w, from_table, from_positions = _norm_inputs(dev)
+    cache = ops.quantized_kv_cache(2, 2, 40, 128, dev)
+    start = torch.zeros(2, dtype=torch.int32, device=dev)
+    calls = [lambda d: from_table(d(q), k, w, w), lambda d: from_table(q, k, w, d(w)), lambda d: from_positions(q, d(k), w, w),
+             lambda d: ops.attention(d(q), k, k), lambda d: ops.attention(q, k, d(k), causal=True), lambda d: ops.cached_attention(d(q), *cache),
+             lambda d: ops.kv_cache_write(k, d(k), *cache, start)]
+    before = [t.view(torch.uint8).clone() if t.dtype == torch.float8_e4m3fn else t.clone() for t in cache]
+    for i, call in enumerate(calls):
+        with fw.dual_level():
+            dual = lambda t: fw.make_dual(t.detach().clone().requires_grad_(leaf), torch.ones_like(t))  # noqa: E731
+            with pytest.raises(RuntimeError, match="forward-mode|forward AD|not differentiable"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+            call(lambda t: t)  # the level alone is no reason
+        if i < 6:
+            assert all(torch.equal(a, b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b) for a, b in zip(before, cache))

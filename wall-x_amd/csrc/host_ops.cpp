@@ -60,8 +60,9 @@ const char* const kNames[] = {"wx_last_error_string", "wx_mrope_apply", "wx_mrop
 constexpr int kEntries = sizeof(kNames) / sizeof(kNames[0]);
 static_assert(sizeof(Entry) == kEntries * sizeof(void*), "a name per entry point");
 
-// A tensor that is what it looks like: strided CUDA memory, no wrapper, no pending conjugation or negation -- and, as what is
-// allocated inside a transform is a wrapper whatever the inputs are, outside of all transforms.
+// A tensor that is what it looks like: strided CUDA memory, no wrapper, no pending conjugation or negation, no tangent of forward-mode
+// differentiation (what is launched here would drop it) -- and, as what is allocated inside a transform is a wrapper whatever the inputs
+// are, outside of all transforms.
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   for (const c10::DispatchKey transform : {c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::Functionalize})
@@ -71,7 +72,7 @@ const at::Tensor* plain(PyObject* o) {
   constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::FuncTorchBatched,
                                           c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
                                           c10::DispatchKey::ZeroTensor, c10::DispatchKey::Batched});
-  if (t.key_set().has_any(wrappers) || !t.has_storage()) return nullptr;
+  if (t.key_set().has_any(wrappers) || !t.has_storage() || t._fw_grad(0).defined()) return nullptr;
   return &t;
 }
 

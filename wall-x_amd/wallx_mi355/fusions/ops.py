@@ -475,6 +475,13 @@ def qkv_projection_with_rope(hidden_states, qkv_weight, qkv_bias, rope_table, nu
 
 
 # ----------------------------------------------------------------------------- norm of q and k with M-RoPE
+def _no_tangents(op, *tensors):
+    """Forward-mode differentiation is refused: a tangent would be dropped without a word."""
+    for t in tensors:
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{op} is not differentiable in forward-mode: its inputs may not carry tangents")
+
+
 class QKNormRoPE(torch.autograd.Function):
     """The RMS norm of every head of q and k and the rotary embedding of the result in one launch; the backward recomputes
     the norm from q and k, which are all it keeps."""
@@ -506,6 +513,7 @@ def _qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps
     if len(mrope_section) != 3:
         raise RuntimeError("[Error] The input `mrope_section` of qk_norm_rope op must be a list of 3 integers!")
     section = tuple(int(v) for v in mrope_section)
+    _no_tangents("qk_norm_rope", q, k, q_weight, k_weight)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
         return QKNormRoPE.apply(q, k, q_weight, k_weight, source, inv_freq, section, eps, layout)
     return backend.qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, section, eps, layout)
@@ -519,7 +527,8 @@ def qk_norm_rope_from_table(q, k, q_weight, k_weight, table, mrope_section, eps=
 
     q [B, Hq, S, D], k [B, Hkv, S, D] through their strides, weights [D] shared by the heads; contiguous outputs.  Everything
     between the input and the output is fp32 with one rounding (a norm op followed by the rope op rounds three times).  bf16;
-    `table`, `mrope_section` and `layout` as for multimodal_rope_from_table.  Differentiable in q, k and both weights."""
+    `table`, `mrope_section` and `layout` as for multimodal_rope_from_table.  Differentiable in q, k and both weights (not in
+    forward-mode, which is refused)."""
     return _qk_norm_rope(q, k, q_weight, k_weight, table, None, mrope_section, eps, layout)
 
 
@@ -560,13 +569,14 @@ def attention(q, k, v, key_ranges=None, key_lengths=None, causal=False, scale=No
     queries are the last Sq keys.  key_ranges int32 [B, Sq, 2] (attention_key_ranges builds the model's), key_lengths int32 [B], on
     the device and never read by the host.  A query that sees no key gets zeros, and keys that a query does not see do not
     influence its row whatever they hold.  Few queries over many keys (generation) are spread over the keys.  Differentiable in q, k
-    and v; the backward writes the same bits every time."""
+    and v (not in forward-mode, which is refused); the backward writes the same bits every time."""
     made = _lib.host().attention(q, k, v, key_ranges, key_lengths, causal, scale)
     if made is not None:
         return made
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.is_cpu:
             raise RuntimeError(f"[Error] The input `{name}` of attention op is on the device: CPU!")
+    _no_tangents("attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return Attention.apply(q, k, v, key_ranges, key_lengths, causal, scale)
     return backend.attention_fwd(q, k, v, key_ranges, key_lengths, causal, scale)[0]
@@ -620,6 +630,7 @@ def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths=None
     for name, t in (("k", k), ("v", v)):
         if t.is_cpu:
             raise RuntimeError(f"[Error] The input `{name}` of kv_cache_write op is on the device: CPU!")
+    _no_tangents("kv_cache_write", k, v)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise RuntimeError("kv_cache_write is not differentiable: call it under torch.no_grad() or on detached tensors")
     backend.kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, start, lengths)
@@ -634,6 +645,7 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key
         return made
     if q.is_cpu:
         raise RuntimeError("[Error] The input `q` of cached_attention op is on the device: CPU!")
+    _no_tangents("cached_attention", q)
     if torch.is_grad_enabled() and q.requires_grad:
         raise RuntimeError("cached_attention is not differentiable: call it under torch.no_grad() or on detached tensors")
     return backend.cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges, key_lengths, causal, scale)
