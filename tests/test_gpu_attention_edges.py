@@ -62,3 +62,38 @@ def test_forward_mode_is_refused(dev, host, leaf):
             call(lambda t: t)  # the level alone is no reason
         if i < 6:
             assert all(torch.equal(a, b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b) for a, b in zip(before, cache))
+
+
+def test_graphs_of_gradients(dev, host):
+    """create_graph=True is for what is differentiated twice: the ops' gradients come out the same, other paths' second derivatives are right, and
+    the ops' own are refused where they are asked for."""
+    q, k, w, from_table, from_positions = _norm_inputs(dev)
+    v = torch.randn_like(k)
+    for op, args in ((lambda *a: (ops.attention(*a, causal=True),), (q, k, v)), (from_table, (q, k, w, w)), (from_positions, (q, k, w, w))):
+        for transposed in (False, True):  # (what is copied first goes another way)
+            leaves = [t.detach().clone().requires_grad_() for t in args]
+            used = [t.transpose(-1, -2).contiguous().transpose(-1, -2) if transposed and t.dim() == 4 else t for t in leaves]
+            out = op(*used)
+            do = [torch.randn_like(y) for y in out]
+            want = torch.autograd.grad(out, leaves, do, retain_graph=True)
+            got = torch.autograd.grad(out, leaves, do, create_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+            # a penalty beside the op: its own second derivative
+            x = torch.tensor(3.0, device=dev, requires_grad=True)
+            total = sum(y.float().sum() for y in op(*used)) + x ** 3
+            (gx,) = torch.autograd.grad(total, x, create_graph=True)
+            (ggx,) = torch.autograd.grad(gx, x)
+            assert float(ggx) == 18.0
+            total.backward(create_graph=True)
+            assert float(x.grad) == 27.0 and all(torch.isfinite(t.grad).all() for t in leaves)
+            for t in (*leaves, x):
+                t.grad = None
+            # the op's: wherever a path leads through it, also beside another one, and from the gradient that came in
+            for leaf in leaves:
+                got = torch.autograd.grad(op(*used), leaves, do, create_graph=True)
+                with pytest.raises(RuntimeError, match="not differentiable|differentiate twice"):
+                    torch.autograd.grad(sum(g.float().square().sum() for g in got) + (leaf.float() ** 2).sum(), leaf)
+            sums = [d.clone().requires_grad_() for d in do]
+            got = torch.autograd.grad(op(*used), leaves, sums, create_graph=True)
+            with pytest.raises(RuntimeError, match="not differentiable|differentiate twice"):
+                got[0].float().sum().backward()

@@ -341,6 +341,33 @@ bool needs_grad(std::initializer_list<const at::Tensor*> ts) {
 }
 PyObject* wrap_all(const variable_list& v) { return v.size() == 1 ? wrap(v[0]) : pair(v[0], v[1]); }
 
+// What a graph of gradients (create_graph) gets of a backward pass that is not differentiable itself: its gradients, as results of a node that
+// hangs on everything they were made from and raises where a second derivative is asked through it.
+struct NoSecond : torch::autograd::Function<NoSecond> {
+  static variable_list forward(AutogradContext* ctx, at::TensorList grads_and_from, int64_t count, const std::string& what) {
+    ctx->saved_data["what"] = what;
+    variable_list out;
+    for (int64_t i = 0; i < count; ++i) out.push_back(grads_and_from[i].view_as(grads_and_from[i]));
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list&) {
+    TORCH_CHECK(false, ctx->saved_data["what"].toStringRef(), "'s backward is not differentiable");
+  }
+};
+void no_second(variable_list& grads, std::initializer_list<variable_list> from, const char* what) {
+  variable_list all;
+  for (const at::Tensor& g : grads)
+    if (g.defined()) all.push_back(g);
+  const int64_t count = static_cast<int64_t>(all.size());
+  for (const variable_list& list : from)
+    for (const at::Tensor& t : list)
+      if (t.defined()) all.push_back(t);
+  const variable_list held = NoSecond::apply(at::TensorList(all), count, std::string(what));
+  size_t i = 0;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = held[i++];
+}
+
 struct NormRope : torch::autograd::Function<NormRope> {
   static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k, const Variable& wq, const Variable& wk, const Variable& source,
                                const std::optional<at::Tensor>& inv_freq, at::IntArrayRef section, double eps, int64_t layout) {
@@ -362,10 +389,15 @@ struct NormRope : torch::autograd::Function<NormRope> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
+    check_capture(saved[0]);
+    variable_list out = gradients(ctx, saved, grads);
+    if (at::GradMode::is_enabled()) no_second(out, {grads, {saved[0], saved[1], saved[2], saved[3]}}, "qk_norm_rope");
+    return out;
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& saved, const variable_list& grads) {
+    const at::NoGradGuard no_grad;
     const at::Tensor q = as_rows16(saved[0]), k = as_rows16(saved[1]);  // (saved-tensor hooks may hand them back in another order)
     const at::Tensor &wq = saved[2], &wk = saved[3], &source = saved[4], &freq = saved[5];
-    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope's backward is not differentiable");
-    check_capture(saved[0]);
     const std::vector<int64_t> section = ctx->saved_data["section"].toIntVector();
     const int sec[3] = {static_cast<int>(section[0]), static_cast<int>(section[1]), static_cast<int>(section[2])};
     const int layout = static_cast<int>(ctx->saved_data["layout"].toInt());
@@ -452,10 +484,15 @@ struct Attention : torch::autograd::Function<Attention> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
+    check_capture(saved[0]);
+    variable_list out = gradients(ctx, saved, grads);
+    if (at::GradMode::is_enabled()) no_second(out, {grads, {saved[0], saved[1], saved[2]}}, "attention");
+    return out;
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& saved, const variable_list& grads) {
+    const at::NoGradGuard no_grad;
     const at::Tensor q = as_rows16(saved[0]), k = as_rows16(saved[1]), v = as_rows16(saved[2]);  // (see above)
     const at::Tensor &out = saved[3], &lse = saved[4], &rest = saved[5], &ranges = saved[6], &lengths = saved[7];
-    TORCH_CHECK(!at::GradMode::is_enabled(), "attention's backward is not differentiable");
-    check_capture(saved[0]);
     const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
     at::Tensor dq, dk, dv;
     launch(q, [&] {

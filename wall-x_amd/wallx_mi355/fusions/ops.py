@@ -482,6 +482,30 @@ def _no_tangents(op, *tensors):
             raise RuntimeError(f"{op} is not differentiable in forward-mode: its inputs may not carry tangents")
 
 
+class _NoSecond(torch.autograd.Function):
+    """The gradients of a backward pass that is not differentiable itself, in a graph of gradients (create_graph): results of a node
+    that hangs on everything they were made from and raises where a second derivative is asked through it."""
+
+    @staticmethod
+    def forward(ctx, what, count, *grads_and_from):
+        ctx.what = what
+        return tuple(g.view_as(g) for g in grads_and_from[:count])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what}'s backward is not differentiable")
+
+
+def _no_second(what, backward, ctx, grads, made_from):
+    """backward(ctx, *grads) for an autograd.Function whose second derivative is refused."""
+    with torch.no_grad():
+        out = backward(ctx, *grads)
+    if not torch.is_grad_enabled():
+        return out
+    held = iter(_NoSecond.apply(what, sum(g is not None for g in out), *(g for g in out if g is not None), *grads, *made_from))
+    return tuple(None if g is None else next(held) for g in out)
+
+
 class QKNormRoPE(torch.autograd.Function):
     """The RMS norm of every head of q and k and the rotary embedding of the result in one launch; the backward recomputes
     the norm from q and k, which are all it keeps."""
@@ -493,8 +517,11 @@ class QKNormRoPE(torch.autograd.Function):
         return backend.qk_norm_rope(q, k, q_weight, k_weight, source, inv_freq, mrope_section, eps, layout)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_q, grad_k):
+        return _no_second("qk_norm_rope", QKNormRoPE.gradients, ctx, (grad_q, grad_k), ctx.saved_tensors[:4])
+
+    @staticmethod
+    def gradients(ctx, grad_q, grad_k):
         q, k, q_weight, k_weight, source, inv_freq = ctx.saved_tensors
         _lib.host().capture_check(q)
         grads = backend.qk_norm_rope_bwd(grad_q, grad_k, q, k, q_weight, k_weight, source, inv_freq, *ctx.rope, want=ctx.needs_input_grad[:4])
@@ -551,8 +578,11 @@ class Attention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
+        return _no_second("attention", Attention.gradients, ctx, (grad_out,), ctx.saved_tensors[:3])
+
+    @staticmethod
+    def gradients(ctx, grad_out):
         q, k, v, out, lse, rest, key_ranges, key_lengths = ctx.saved_tensors
         _lib.host().capture_check(q)
         grads = backend.attention_bwd(grad_out, q, k, v, out, lse, rest, key_ranges, key_lengths, *ctx.mask)
