@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "attention.h"
+#include "attention_plan.h"
 
 namespace wx {
 
@@ -55,8 +56,6 @@ template <int DT>
 constexpr int kUp = DT == WX_F16 ? 15 : 0;
 constexpr float kMostSlope = 32768.f;
 constexpr int kSlopeTo = 9;
-
-constexpr int kKeyTile = 64;
 
 __device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64_t* st, int b, int h, int i) {
   return p + b * st[0] + h * st[1] + i * st[2];
@@ -376,13 +375,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   if (again != 0) dq_again<DT, D, RW>(a, again, lse, delta, block_up);
 }
 
-// What the workgroups of the next kernel do: a workgroup per pair, a lane per key tile, the row blocks dealt to 16 wavefronts.
-//
-// Under a causal mask the first keys are seen by all rows and the last by few, and of a row of packed sequences a tile is seen by those
-// of its own: a tile's row blocks, from the first to the last that sees it, are cut evenly into units of at most as many as make a pair's
-// units about `aim` in all (kLeast where that is fewer), so that the longest workgroup is a unit and not a tile.
-constexpr int kLeast = 16;
-constexpr int kPlanTiles = 1024;
+// What the workgroups of the next kernel do (attention_plan.h): a workgroup per pair, a lane per key tile, the row blocks dealt to 16
+// wavefronts.
 __global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
   constexpr int kChunk = 4096;
   __shared__ int s_first[kPlanTiles], s_last[kPlanTiles];
@@ -422,16 +416,16 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(BwdArgs a) {
   }
   if (a.more == 0 || tid >= 64) return;
   int2* tiles = a.tiles + static_cast<int64_t>(pair) * a.key_tiles;
-  int work = 0;
+  int64_t work = 0;
   for (int t = lane; t < a.key_tiles; t += 64) work += max(s_last[t] - s_first[t] + 1, 0);
 #pragma unroll
-  for (int n = 1; n < 64; n *= 2) work += __shfl_xor(work, n);
-  const int unit = max(kLeast, (work + a.aim - 1) / a.aim);
-  int next = 0;  // (never past a.units: the full units are no more than a.aim, the last ones of the tiles no more than those; and see more_units)
+  for (int n = 1; n < 64; n *= 2) work += __shfl_xor(static_cast<long long>(work), n);
+  const int unit = unit_blocks(work, a.aim);
+  int next = 0;  // (never past a.units)
   for (int c = 0; c < a.key_tiles; c += 64) {
     const bool is = c + lane < a.key_tiles;
     const int from = is ? s_first[c + lane] : 0, blocks = is ? max(s_last[c + lane] - from + 1, 0) : 0;
-    const int units = is ? max((blocks + unit - 1) / unit, 1) : 0;  // (a tile that nothing sees: one of no blocks, which writes zeros)
+    const int units = is ? tile_units(blocks, unit) : 0;
     int up_to = units;
 #pragma unroll
     for (int n = 1; n < 64; n *= 2) {
@@ -804,27 +798,12 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(BwdArgs a) {
   }
 }
 
-// Units that a pair's key tiles are cut into beyond one to each: about kUnits workgroups to each place on the chip (two to a CU) of all
-// pairs', where the tiles alone are fewer.  More units end more evenly, fewer write and join fewer sums (64 KB a unit of head size 128).
-// Forward and backward with 1 / 2 / 3 / 4 / 6: 8192 causal tokens of 16 / 2 heads 1464 / 1344 / 1321 / 1339 / 1372 us, 4096 tokens of 16 / 16
-// heads that see all 593 / 594 / 643 / 648 / 672, 16 rows of 912 causal tokens 379 / 384 / 404 / 413 / 442.
-constexpr int kUnits = 2;
-int aim_units(int64_t pairs, int64_t n_keys) {
-  const int64_t tiles = pairs * ((n_keys + kKeyTile - 1) / kKeyTile), places = 2 * device_cu_count();
-  return tiles == 0 || tiles >= kUnits * places || tiles > pairs * kPlanTiles ? 0 : static_cast<int>((kUnits * places + pairs - 1) / pairs);
-}
-// No tile makes more than its rows' blocks do in units of the least length.
-int more_units(int64_t pairs, int64_t rows, int64_t n_keys) {
-  const int64_t of_tile = ((rows + 31) / 32 + kLeast - 1) / kLeast, most = (n_keys + kKeyTile - 1) / kKeyTile * std::max<int64_t>(of_tile - 1, 0);
-  return static_cast<int>(std::min<int64_t>(aim_units(pairs, n_keys), most));
-}
-
 struct Workspace {
   size_t info, bounds, tiles, list, part, total;
 };
 Workspace layout(int64_t pairs, int64_t rows, int64_t n_keys, int head_dim) {
   const size_t blocks = static_cast<size_t>(pairs) * ((rows + 31) / 32), tiles = static_cast<size_t>(pairs) * ((n_keys + kKeyTile - 1) / kKeyTile);
-  const size_t more = static_cast<size_t>(pairs) * more_units(pairs, rows, n_keys);
+  const size_t more = static_cast<size_t>(pairs) * more_units(pairs, rows, n_keys, device_cu_count());
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   Workspace w{};
   w.info = 0;
@@ -912,7 +891,7 @@ extern "C" int wx_attention_bwd(const void* q, const void* k, const void* v, con
   a.c = scale * kLog2e, a.scale = scale;
   const int64_t pairs = batch * n_kv_heads;
   a.key_tiles = (a.n_keys + kKeyTile - 1) / kKeyTile;
-  a.aim = aim_units(pairs, n_keys), a.more = more_units(pairs, a.rows, n_keys);
+  a.aim = aim_units(pairs, n_keys, device_cu_count()), a.more = more_units(pairs, a.rows, n_keys, device_cu_count());
   a.units = a.key_tiles + a.more;
   const Workspace w = layout(pairs, a.rows, n_keys, head_dim);
   if (w.total > 0 && (!workspace || workspace_bytes < w.total)) return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_attention_bwd_workspace_bytes)", who);
