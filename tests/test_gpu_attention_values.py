@@ -143,7 +143,7 @@ def test_gradients_of_any_size(dev, B, Hq, Hkv, Sq, Sk, D, causal, grad, value, 
 
 
 def test_gradients_far_apart(dev):
-    """Packed sequences, one's gradients 2^28 times another's: blocks of rows hold both, and each sequence's are its own."""
+    """Packed sequences, one's gradients 2^24 times another's: blocks of rows and tiles of keys hold both, and each sequence's are its own."""
     g = torch.Generator(device=dev).manual_seed(3)
     Hq, Hkv, S, D, each = 8, 2, 1200, 128, 75
     q, k, v, do = (heads(1, S, h, D, torch.float16, g, dev) for h in (Hq, Hkv, Hkv, Hq))
@@ -154,9 +154,7 @@ def test_gradients_far_apart(dev):
     for n in range(S // each):
         part = slice(n * each, (n + 1) * each)
         for name, a, (value, tol) in zip(("dq", "dk", "dv"), got, gradients(q[:, :, part], k[:, :, part], v[:, :, part], do[:, :, part], True).values()):
-            # (a block of 32 rows, 8 tokens of 4 heads, may hold rows of both kinds: their slopes then lose 2^-34 of the larger ones)
-            beside = 2.0 ** -34 * 2.0 ** 13 * 64 * (D ** -0.5 * 75 * 5 if name != "dv" else 0.0)
-            a, value, tol = held(a[:, :, part], value, tol + beside)
+            a, value, tol = held(a[:, :, part], value, tol)
             check(a, (value, tol), f"{name} of sequence {n}")
 
 

@@ -42,20 +42,26 @@ struct BwdArgs {
 };
 
 // What the second kernel reads of 32 rows: L (less kUp), delta, lo and hi of each, then the keys that all rows with keys see, whether some row
-// sees a single one, and (fp16) the power of two that the slopes of all its rows fit fp16 with.
+// sees a single one, and (fp16) the power of two that the slopes of all of them fit fp16 with.
 constexpr int kInfoWords = 4 * 32 + 4;
 
 // fp16's range is too short for probabilities of many keys and for their slopes: P is 1 / keys, dS as much smaller again as the gradient
 // that comes in, and beyond 65504 where few keys meet a large one.  P enters its product times 2^15, which it cannot leave the range with.  dS of
 // a row is formed times 2^15 as well (both are one subtraction from L), until a slope passes 2^15 (kMostSlope): then by as much less as
-// takes the largest to below 2^10, and the sums so far with it.  The second kernel, whose products sum over rows, takes the least of the
-// powers of the rows that it has met.  Powers of two are exact, and taken back from the sums.  Forward and backward of 16 x 912 tokens in fp16
-// 378 us, 368 with P and dS as they are; dQ's error for gradients of 0.001 over 8192 keys 0.096 % of its length (0.094 of it the result's own
-// rounding), 0.76 with them.
+// takes the largest to below 2^10, and the sums so far with it.  The second kernel does the same for each key, of the rows that see it (so
+// that a sequence's large gradients take nothing from its neighbours in the row), where the first found a slope as large among 32 rows.  Powers
+// of two are exact, and taken back from the sums.  Forward and backward of 16 x 912 tokens in fp16 397 us, 386 with P and dS as they are; dQ's
+// error for gradients of 0.001 over 8192 keys 0.096 % of its length (0.094 of it the result's own rounding), 0.76 with them.
 template <int DT>
 constexpr int kUp = DT == WX_F16 ? 15 : 0;
 constexpr float kMostSlope = 32768.f;
 constexpr int kSlopeTo = 9;
+// By how many powers of two less a row's (key's) slopes go on, `top` being the largest of them that this lane is about to round; the same in
+// both halves of a column.
+__device__ __forceinline__ int slopes_less(float top) {
+  top = both_max(top);
+  return top > kMostSlope && top < kInf ? static_cast<int>(__float_as_uint(top) >> 23) - 127 - kSlopeTo : 0;
+}
 
 __device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64_t* st, int b, int h, int i) {
   return p + b * st[0] + h * st[1] + i * st[2];
@@ -247,8 +253,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   // Keeps the row's slopes in fp16's range: `top` is the largest of what this lane is about to round.
   auto fit = [&](f32x16& s, int from, float top) {
     if (!__any(top > kMostSlope && top < kInf)) return;
-    top = both_max(top);
-    const int less = top > kMostSlope && top < kInf ? static_cast<int>(__float_as_uint(top) >> 23) - 127 - kSlopeTo : 0;
+    const int less = slopes_less(top);
     const float f = ldexpf(1.f, -less);
     up -= less;
     shifted += static_cast<float>(less);
@@ -452,10 +457,10 @@ __device__ __forceinline__ int todo_pair(const BwdArgs& a, int* unit = nullptr) 
 }
 
 // Keys whose sum is not a number: again (see Odd, attention.h), those of this wavefront's that `again` has a bit for, over all rows of its
-// unit, unless a row that sees the key makes the whole sum NaN (by its L, or for dK by its delta).  (A query that is not finite has no
+// unit, dK's slopes times `of`, unless a row that sees the key makes the whole sum NaN (by its L, or for dK by its delta).  (A query that is not finite has no
 // probability where its L is a number, so that its slope times it is NaN.)  The place is found once more, as in dq_again.
 template <int DT, int D>
-__device__ __forceinline__ void dkv_again(const BwdArgs& a, uint32_t again, int4 todo) {
+__device__ __forceinline__ void dkv_again(const BwdArgs& a, uint32_t again, int4 todo, float of) {
   using T = AttnTile<D>;
   int tid = threadIdx.x, pair = todo_pair(a), tile = __builtin_amdgcn_readfirstlane(todo.x), first = __builtin_amdgcn_readfirstlane(todo.y);
   const int last = __builtin_amdgcn_readfirstlane(todo.z);
@@ -485,13 +490,7 @@ __device__ __forceinline__ void dkv_again(const BwdArgs& a, uint32_t again, int4
     const int row = min(t * 32 + i, a.rows - 1), at = a.by_group.div(row);
     return base + at * st[2] + (row - at * a.group) * st[1];
   };
-  float of = 1.f, back = 1.f;  // dK's slopes times the power that all rows of the unit fit fp16 with, dV's probabilities as they are
-  if constexpr (DT == WX_F16) {
-    int least = kUp<DT>;
-    if (rg == 0)
-      for (int t = first; t < last; ++t) least = min(least, static_cast<int>(info_base[static_cast<int64_t>(t) * kInfoWords + 131]));
-    of = ldexpf(1.f, least - kUp<DT>), back = ldexpf(1.f, -least);
-  }
+  const float back = ldexpf(1.f, -kUp<DT>) / of;
   for (int o = 0; o < T::kOut; ++o) {
     f32x16 sum = {};
     const int c = 32 * o + (lane & 31);
@@ -552,6 +551,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   unsigned char* const lds0 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 0>();
   unsigned char* const lds1 = lds_slot<(2 * kSlot > 2 * kSums ? 2 * kSlot : 2 * kSums), 1>();
   __shared__ u32x4 s_offsets[256];
+  __shared__ float s_slope[DT == WX_F16 ? 4 : 1][32];
   // (D = 128: two of V's operands stand in LDS, read in front of their products; with all in registers one was spilled, and the wait
   // for its memory was a wait for the next block's as well)
   constexpr int kHeld = D == 128 ? T::kSteps - 2 : T::kSteps;
@@ -635,8 +635,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     for (int r = 0; r < 16; ++r) dk[o][r] = dv[o][r] = 0.f;
 
   constexpr bool kFit = DT == WX_F16;
-  int up = kUp<DT>;         // dk holds its sums times 2^up, dv times 2^kUp
-  float of_slope = 1.f;     // 2^(up - kUp)
+  // dk holds its sums times 2^kUp and, for each key, s_slope's power of two, dv times 2^kUp.  (In LDS, for want of registers.)
+  if constexpr (kFit) s_slope[wave][lane & 31] = 1.f;
+  bool scaled = false;  // one of them is not 1
   const int rows_first = rows_base<D>(lane), cols_first = cols_base<D>(lane);
   auto turn = [&](int t, unsigned char* tq, unsigned char* next) {
     wait_loads();
@@ -646,19 +647,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     const unsigned char* tg = tq + kTileBytes;
     const float* info = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
     const int4 full = *reinterpret_cast<const int4*>(info + 128);
-    const int f_lo = __builtin_amdgcn_readfirstlane(full.x), f_hi = __builtin_amdgcn_readfirstlane(full.y);
-    if constexpr (kFit) {
-      const int here = __builtin_amdgcn_readfirstlane(full.w);
-      if (here < up) {
-        const float f = ldexpf(1.f, here - up);
-        up = here;
-        of_slope = ldexpf(1.f, up - kUp<DT>);
-#pragma unroll
-        for (int o = 0; o < T::kOut; ++o)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dk[o][r] *= f;
-      }
-    }
+    const int f_lo = __builtin_amdgcn_readfirstlane(full.x), f_hi = __builtin_amdgcn_readfirstlane(full.y), one = __builtin_amdgcn_readfirstlane(full.z);
+    const bool large = kFit && __builtin_amdgcn_readfirstlane(full.w) < kUp<DT>;
     // (an exclusive-or per read in place of an address register for each: the accumulators leave none)
     int rows_at = rows_first, cols_at = cols_first;
     asm volatile("" : "+v"(rows_at), "+v"(cols_at));
@@ -693,7 +683,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         for (int i = 0; i < 4; ++i) s[4 * g + i] = ((key >= l4[i]) & (key < h4[i])) ? s[4 * g + i] : -kInf;
       }
     }
-    if (__builtin_amdgcn_readfirstlane(full.z) != 0) {  // some row sees one key: its slope is none
+    if (one != 0) {  // some row sees one key: its slope is none
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int at = 8 * (r / 4) + 4 * h + r % 4;
@@ -711,17 +701,45 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
         const int r = 4 * g + i;
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -ls[i]));
         dp[r] = s[r] * (dp[r] - de[i]);
-        if constexpr (kFit) dp[r] *= of_slope;
       }
+    };
+    auto fit = [&](int from) {  // as in the first kernel, of this lane's key
+      if (!scaled && !large) return;
+      in_order();
+      float top = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) top = fmaxf(top, fabsf(dp[from + r]));
+      in_order();
+      int at = lane;
+      asm volatile("" : "+v"(at));
+      float of = s_slope[wave][at & 31];
+      top *= of;
+      if (__any(top > kMostSlope && top < kInf)) {
+        const float f = ldexpf(1.f, -slopes_less(top));
+        of *= f;
+        s_slope[wave][at & 31] = of;
+        scaled = true;
+#pragma unroll
+        for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dk[o][r] *= f;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) dp[from + r] *= of;
+      in_order();
     };
     slope(0);
     slope(1);
+    if constexpr (kFit) fit(0);
     u32x4 p = pack_step<DT>(s, 0), ds = pack_step<DT>(dp, 0);
     in_order();
 #pragma unroll
     for (int i = 0; i < kProducts; ++i) {
       const int o = i / 2 % T::kOut;
-      if (i == 2 * T::kOut) p = pack_step<DT>(s, 1), ds = pack_step<DT>(dp, 1);
+      if (i == 2 * T::kOut) {
+        if constexpr (kFit) fit(8);
+        p = pack_step<DT>(s, 1), ds = pack_step<DT>(dp, 1);
+      }
       if (i % 2 == 0) dv[o] = mfma<DT>(f[i % kAhead], p, dv[o]);
       else dk[o] = mfma<DT>(f[i % kAhead], ds, dk[o]);
       if (i + kAhead < kProducts) f[i % kAhead] = read_g(i + kAhead);
@@ -736,7 +754,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
   }
 
   if constexpr (kFit) {
-    const float fk = ldexpf(1.f, -up), fv = ldexpf(1.f, -kUp<DT>);
+    const float fv = ldexpf(1.f, -kUp<DT>), fk = fv / s_slope[wave][lane & 31];
 #pragma unroll
     for (int o = 0; o < T::kOut; ++o)
 #pragma unroll
@@ -769,7 +787,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BwdArgs a) {
     for (int o = 0; o < T::kOut; ++o) store_sums<D>(dk[o], o, part + (key - k0) * 2 * D, lane);
   }
 
-  if (again != 0) dkv_again<DT, D>(a, again, todo);
+  if (again != 0) dkv_again<DT, D>(a, again, todo, kFit && rg == 0 ? fminf(s_slope[half][lane & 31], s_slope[half + 2][lane & 31]) : 1.f);
 }
 
 // dK and dV of the keys of a tile of several units, from the units' sums: four workgroups per tile, a thread per 4 channels (one
