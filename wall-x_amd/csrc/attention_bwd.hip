@@ -68,10 +68,10 @@ __device__ __forceinline__ const uint16_t* row_of(const uint16_t* p, const int64
 }
 
 // Rows whose sum is not a number though their L and delta are: again (see Odd, attention.h), those of this wavefront's that `again` has a bit
-// for, times 2^up.  (A key that is not finite has no probability where L is a number, so that its slope times it is NaN.)  Their place is
-// found once more: kept over the kernel's loop for this rare case it costs that registers.
+// for.  (A key that is not finite has no probability where L is a number, so that its slope times it is NaN.)  Their place is found once more:
+// kept over the kernel's loop for this rare case it costs that registers.
 template <int DT, int D, int RW>
-__device__ __forceinline__ void dq_again(const BwdArgs& a, uint32_t again, float lse, float delta, int up) {
+__device__ __forceinline__ void dq_again(const BwdArgs& a, uint32_t again, float lse, float delta) {
   using T = AttnTile<D>;
   int id = blockIdx.x, tid = threadIdx.x;
   asm volatile("" : "+s"(id), "+v"(tid));
@@ -89,33 +89,55 @@ __device__ __forceinline__ void dq_again(const BwdArgs& a, uint32_t again, float
   const int64_t k_step = a.ks[2] * 2, v_step = a.vs[2] * 2;
   const uint16_t *q = row_of(a.q, a.qs, b, hq, qi), *g = row_of(a.g, a.gs, b, hq, qi);
   uint16_t* const dq = a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
-  const float factor = hi - lo == 1 ? 0.f : a.scale * ldexpf(1.f, -kUp<DT>), l_up = lse - static_cast<float>(up), back = ldexpf(1.f, kUp<DT> - up);
+  const float factor = hi - lo == 1 ? 0.f : a.scale * ldexpf(1.f, -kUp<DT>);
+  float shifted = lse - kUp<DT>, back = 1.f;
+  // the slopes of keys k0 .. + 31, zeros for what is not seen and for other rows
+  auto in = [&](int k0, int i) { return min(i, a.n_keys - 1 - k0); };  // (a key past the last is the last, and not seen)
+  auto slopes = [&](int k0, f32x16& s, uint32_t& seen) {
+    const char *kr = kp + k0 * k_step + in(k0, lane & 31) * static_cast<int>(k_step), *vr = vp + k0 * v_step + in(k0, lane & 31) * static_cast<int>(v_step);
+    f32x16 dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      s = mfma<DT>(*reinterpret_cast<const u32x4*>(kr + (16 * t + 8 * h) * 2), *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h), s);
+      dp = mfma<DT>(*reinterpret_cast<const u32x4*>(vr + (16 * t + 8 * h) * 2), *reinterpret_cast<const u32x4*>(g + 16 * t + 8 * h), dp);
+      in_order();
+    }
+    seen = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = k0 + 8 * (r / 4) + 4 * h + r % 4;
+      const bool sees = redo && key >= lo && key < hi;
+      s[r] = sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -shifted)) * (dp[r] - delta) : 0.f;
+      seen |= sees ? 1u << r : 0u;
+    }
+  };
+  if constexpr (DT == WX_F16) {
+    float top = 0.f;
+    for (int k0 = from; k0 < up_to; k0 += 32) {
+      f32x16 s;
+      uint32_t seen;
+      slopes(k0, s, seen);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (fabsf(s[r]) < kInf) top = fmaxf(top, fabsf(s[r]));
+    }
+    const int less = slopes_less(top);
+    shifted += static_cast<float>(less), back = ldexpf(1.f, less);
+  }
   for (int o = 0; o < T::kOut; ++o) {
     f32x16 sum = {};
     const int c = 32 * o + (lane & 31);
     for (int k0 = from; k0 < up_to; k0 += 32) {
-      auto in = [&](int i) { return min(i, a.n_keys - 1 - k0); };  // (a key past the last is the last, and not seen)
-      const char *kr = kp + k0 * k_step + in(lane & 31) * static_cast<int>(k_step), *vr = vp + k0 * v_step + in(lane & 31) * static_cast<int>(v_step);
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int t = 0; t < T::kSteps; ++t) {
-        s = mfma<DT>(*reinterpret_cast<const u32x4*>(kr + (16 * t + 8 * h) * 2), *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h), s);
-        dp = mfma<DT>(*reinterpret_cast<const u32x4*>(vr + (16 * t + 8 * h) * 2), *reinterpret_cast<const u32x4*>(g + 16 * t + 8 * h), dp);
-        in_order();
-      }
-      uint32_t seen = 0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = k0 + 8 * (r / 4) + 4 * h + r % 4;
-        const bool sees = redo && key >= lo && key < hi;
-        s[r] = sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -l_up)) * (dp[r] - delta) : 0.f;
-        seen |= sees ? 1u << r : 0u;
-      }
+      f32x16 s;
+      uint32_t seen;
+      slopes(k0, s, seen);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Odd odd;
         const u32x4 x = gather_cols<DT>(t, h, odd, [&](int i) -> uint32_t {
-          return D % 32 != 0 && c >= D ? 0u : *reinterpret_cast<const uint16_t*>(kp + k0 * k_step + (in(i) * static_cast<int>(k_step) + 2 * c));
+          return D % 32 != 0 && c >= D ? 0u : *reinterpret_cast<const uint16_t*>(kp + k0 * k_step + (in(k0, i) * static_cast<int>(k_step) + 2 * c));
         });
         in_order();
         sum = mfma<DT>(x, pack_step<DT>(s, t), sum);
@@ -377,7 +399,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BwdArgs a) {
   const float factor = hi - lo == 1 ? 0.f : a.scale * ldexpf(1.f, -kUp<DT>);
   uint16_t* const dq = a.dq + ((static_cast<int64_t>(b) * a.n_queries + qi) * a.n_q + hq) * D;
   store_row<DT, D>(acc, factor, live ? dq : nullptr, lane);
-  if (again != 0) dq_again<DT, D, RW>(a, again, lse, delta, block_up);
+  if (again != 0) dq_again<DT, D, RW>(a, again, lse, delta);
 }
 
 // What the workgroups of the next kernel do (attention_plan.h): a workgroup per pair, a lane per key tile, the row blocks dealt to 16
