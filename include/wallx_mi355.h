@@ -517,7 +517,9 @@ int wx_qk_norm_rope_bwd(const void* grad_q_out, const void* grad_k_out, const vo
  * i * group + g of query i and head g of the group: the base-2 logarithm of the sum of powers, what wx_attention_bwd reads.
  * rest (may be NULL): uint8 [batch, n_queries, n_q_heads, head_dim], what rounding out to its type left, as e5m2
  * times 2^-11 (fp16) or 2^-8 (bf16): with it the backward's sums of out times its gradient have three bits more of out (of bf16 outputs up
- * to 2^16; a row of larger ones does without).  At most 1024 query heads to a key / value head.
+ * to 2^16; a row of larger ones does without).  At most 1024 query heads to a key / value head, and
+ * 2^24 - 1 workgroups (of 64 rows of a pair of sequence and key / value head, or more); the backward at most 2^22 - 1 pairs, and 2^24 - 1
+ * tiles of 64 keys.
  * workspace: wx_attention_workspace_bytes() bytes for the same sizes (0 for most; few rows over many keys are split). */
 size_t wx_attention_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int64_t n_queries, int64_t n_keys, int head_dim);
 int wx_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const int32_t* key_ranges,

@@ -97,3 +97,34 @@ def test_graphs_of_gradients(dev, host):
             got = torch.autograd.grad(op(*used), leaves, sums, create_graph=True)
             with pytest.raises(RuntimeError, match="not differentiable|differentiate twice"):
                 got[0].float().sum().backward()
+
+
+def test_the_most_sequences(dev):
+    """As many sequences of one token as a launch has workgroups for, and one more, which is refused (in front of any launch)."""
+    most = 2 ** 24 - 1
+    x = torch.arange(most + 1, device=dev, dtype=torch.int32).bitwise_and(2047).to(torch.float16).view(-1, 1, 1, 1).expand(-1, 1, 1, 64).contiguous()
+    start = torch.zeros(most + 1, dtype=torch.int32, device=dev)
+    cache = ops.quantized_kv_cache(most + 1, 1, 1, 64, dev)
+    with pytest.raises(RuntimeError, match="too many"):
+        ops.kv_cache_write(x, x, *cache, start)
+    with pytest.raises(RuntimeError, match="too many"):
+        ops.attention(x, x, x)
+    with pytest.raises(RuntimeError, match="too many"):
+        ops.cached_attention(x, *cache)
+    assert not any(t.view(torch.uint8).any() for t in cache)
+    x, start, cache = x[:most], start[:most], ops.quantized_kv_cache(most, 1, 1, 64, dev)
+    # (scores of up to 2047 * 2047 * 64 / 8 = 2^25 natural units, 4.8e7 powers of two, where fp32 numbers are 4 apart: the only probability is
+    # 2^-2 to 2^2, and rounded to fp16 while the sum of them is not: half a step of it, and half a step of the result)
+    assert bool(((ops.attention(x, x, x).float() - x.float()).abs() <= 2.0 ** -10 * x.float()).all())
+    ops.kv_cache_write(x, x, *cache, start)
+    # (a row of one value: its code is 448, its scale a 448th of it to fp32)
+    assert float((ops.cached_attention(x, *cache).float() - x.float()).abs().max()) <= 2048 * 2.0 ** -11
+    del cache
+    most = 2 ** 22 - 1  # (the backward plans a pair with 1024 threads)
+    leaf = x[:most].clone().requires_grad_()
+    (g,) = torch.autograd.grad(ops.attention(leaf, leaf, leaf, scale=2.0 ** -20), leaf, x[:most])  # (scores below 2^9, as exact as they come)
+    assert torch.equal(g, x[:most])
+    leaf = x[:most + 1].clone().requires_grad_()
+    out = ops.attention(leaf, leaf, leaf)
+    with pytest.raises(RuntimeError, match="too many"):
+        torch.autograd.grad(out, leaf, x[:most + 1])

@@ -863,7 +863,8 @@ int launch_bwd(BwdArgs& a, hipStream_t s) {
   // 410 / 376, 4096 tokens of 16 heads that see all 629 / 610 (1824 and 512).
   const int row_waves = pairs * ((a.row_blocks + 3) / 4) < 2 * device_cu_count() ? 2 : 4;
   const int64_t row_tiles = pairs * ((a.row_blocks + row_waves - 1) / row_waves), units = pairs * a.units;
-  if (row_tiles > 0x7fffffffll || units > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows");
+  if (too_many_blocks(row_tiles, 256) || (a.key_tiles > 0 && (too_many_blocks(units, 256) || too_many_blocks(pairs, 1024))))
+    return fail(WX_ERR_UNSUPPORTED, "wx_attention_bwd: too many rows or keys");
   const int all = static_cast<int>(pairs);
   a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group), a.by_in_group = Divider(a.group < 32 ? a.group : 32);
   a.by_pairs = Divider(all % 8 == 0 ? all / 8 : all), a.by_tiles = Divider(a.key_tiles > 0 ? a.key_tiles : 1);

@@ -786,7 +786,8 @@ int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
   a.by_splits = Divider(p.splits), a.by_kv = Divider(a.n_kv), a.by_group = Divider(a.group);
   a.spread = Spread(pairs, a.row_tiles);
   const int64_t blocks = static_cast<int64_t>(a.batch) * a.n_kv * a.row_tiles * a.splits;
-  if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
+  const int64_t all_rows = static_cast<int64_t>(a.batch) * a.n_kv * a.rows, joins = a.splits <= 8 ? (all_rows + 3) / 4 : all_rows;
+  if (too_many_blocks(blocks, p.row_waves == 8 ? 512 : 256) || (a.splits > 1 && too_many_blocks(joins, 256))) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
   if (p.row_waves == 2) {
     hipLaunchKernelGGL((attn_fwd_kernel<DT, D, F8, 2>), grid, block, 0, s, a);
@@ -797,11 +798,9 @@ int launch_fwd(FwdArgs& a, const FwdPlan& p, hipStream_t s) {
   }
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
   if (a.splits > 1) {
-    const int64_t rows = static_cast<int64_t>(a.batch) * a.n_kv * a.rows;
-    if (rows > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "attention: too many rows");
     a.by_rows = Divider(a.rows);
-    if (a.splits <= 8) hipLaunchKernelGGL((attn_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>((rows + 3) / 4)), block, 0, s, a);
-    else hipLaunchKernelGGL((attn_join_kernel<DT, D, 1>), dim3(static_cast<unsigned>(rows)), block, 0, s, a);
+    if (a.splits <= 8) hipLaunchKernelGGL((attn_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>(joins)), block, 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<DT, D, 1>), dim3(static_cast<unsigned>(joins)), block, 0, s, a);
     return check_launch("attn_join_kernel");
   }
   return WX_OK;

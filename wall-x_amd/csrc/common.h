@@ -13,6 +13,9 @@ int fail(int code, const char* fmt, ...);
 // hipGetLastError() after a launch; WX_OK or WX_ERR_LAUNCH with the HIP error text recorded.
 int check_launch(const char* what);
 
+// A launch holds 2^32 - 1 threads along x.  Of more the runtime starts the rest modulo 2^32, without an error: such calls are refused.
+inline bool too_many_blocks(int64_t blocks, int threads) { return blocks > 0xffffffffll / threads; }
+
 // Bits of wx_last_gemm_path() for the calling thread: cleared at the start of a dual GEMM call, set as it launches.
 void gemm_path_reset();
 void gemm_path_note(int bit);

@@ -117,7 +117,7 @@ extern "C" int wx_kv_cache_write(const void* k, const void* v, void* k_cache, vo
   a.rows = static_cast<int>(seq * n_kv_heads), a.n_kv = n_kv_heads, a.capacity = capacity;
   const int64_t each = 256 / (head_dim == 64 ? 8 : 16), of_one = (a.rows + each - 1) / each, blocks = batch * of_one;
   a.by_kv = Divider(n_kv_heads), a.by_blocks = Divider(static_cast<uint32_t>(of_one));
-  if (blocks > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  if (too_many_blocks(blocks, 256)) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
   hipStream_t s = as_stream(stream);
 #define WX_CACHE(DT)                                                                                            \

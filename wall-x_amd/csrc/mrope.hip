@@ -458,7 +458,7 @@ int launch(const void* q, const void* k, const void* cos_t, const void* sin_t, v
   for (int cidx = 0; cidx < head_dim / 8 && rows_ok; ++cidx) rows_ok = ax.uniform[cidx] != 0;
   if (rows_ok) {
     const int64_t threads = n_tokens * lanes;
-    if ((threads + 255) / 256 > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
+    if (too_many_blocks((threads + 255) / 256, 256)) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
     const dim3 grid(static_cast<unsigned>((threads + 255) / 256)), block(256);
 #define WX_LAUNCH_ROWS(DT, L)                                                                                       \
   hipLaunchKernelGGL((mrope_rows_kernel<DT, BWD, L, SRC>), grid, block, 0, s, q, k, cos_t, sin_t, q_out, k_out, n_tokens, \
@@ -485,7 +485,7 @@ int launch(const void* q, const void* k, const void* cos_t, const void* sin_t, v
   const int groups = head_dim / 16;
   const int head_groups = (n_q + n_kv + kHeadsPerThread - 1) / kHeadsPerThread;
   const int64_t threads = n_tokens * groups;
-  if ((threads + 255) / 256 > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  if (too_many_blocks((threads + 255) / 256, 256)) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
   const dim3 grid(static_cast<unsigned>((threads + 255) / 256), static_cast<unsigned>(head_groups)), block(256);
 #define WX_LAUNCH(DT)                                                                                             \
   hipLaunchKernelGGL((mrope_kernel<DT, BWD>), grid, block, 0, s, q, k, cos_t, sin_t, q_out, k_out, n_tokens, seq, \
@@ -836,7 +836,7 @@ int launch_norm_rope(NormRope& a, bool backward, int64_t batch, void* dwq, void*
       a.sin_t = reinterpret_cast<const void*>(static_cast<uintptr_t>(packed_table_width(a.ax, a.head_dim)));
     }
     g = norm_grid(a.n_tokens, heads, lanes, backward);
-    if (g.x > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
+    if (too_many_blocks(g.x, 256)) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
     a.heads_per_group = g.heads_per_group;
     const dim3 grid(static_cast<unsigned>(g.x), static_cast<unsigned>(g.y));
 #define WX_NORM(DT, L)                                                                                     \
@@ -932,7 +932,7 @@ extern "C" int wx_mrope_table(const int64_t* position_ids, const float* inv_freq
   const int64_t n = batch * seq * width;
   if (n == 0) return WX_OK;
   if (!position_ids || !inv_freq || !table) return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  if ((n + 255) / 256 > 0x7fffffffll) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  if (too_many_blocks((n + 255) / 256, 256)) return fail(WX_ERR_UNSUPPORTED, "%s: too many tokens", who);
   hipLaunchKernelGGL(mrope_table_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, as_stream(stream),
                      position_ids, inv_freq, table, batch * seq, half, width, ax);
   return check_launch(who);
