@@ -543,7 +543,8 @@ int wx_attention_bwd(const void* q, const void* k, const void* v, const void* ou
  * [batch, n_kv_heads, seq, head_dim] (strides as above) at position start[b] + s, with scale = max(max |x| / 448, 2^-126) of its
  * row and code = x / scale rounded to nearest even; positions outside [0, capacity) are dropped and nothing else of the cache is
  * touched.  A row that holds NaN or an infinity reads back as NaN.
- * wx_cached_attention: wx_attention_fwd over such a cache (contiguous), without lse.  bf16 or fp16, head_dim 64, 80 or 128. */
+ * wx_cached_attention: wx_attention_fwd over such a cache (contiguous), without lse.  bf16 or fp16, head_dim 64, 80 or 128; in fp16 values
+ * below 2^-14 count to the nearest multiple of 2^-24, as fp16 results do, and values beyond 65504 count in full. */
 int wx_kv_cache_write(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
                       const int32_t* start, const int32_t* lengths, int64_t batch, int n_kv_heads, int64_t seq, int64_t capacity,
                       int head_dim, const int64_t k_strides[3], const int64_t v_strides[3], int dtype, wx_stream_t stream);

@@ -5,8 +5,8 @@
 // fixed order: no atomics, the same gradients every time.
 //
 // 16 rows of 912 causal tokens of 16 / 2 heads of 128 (72 GFLOP in three products, 96 in four): dQ 124 us, 0.58 PFLOP/s, matrix units busy
-// 31 % (the rows' four operands are on their way for a third of it); the plan 5; dK and dV 153 us, 0.63 PFLOP/s, 40 %, reading 0.6 GB of
-// which half is in L2; the join 15.  5003 packed tokens of 12 / 4 heads of 64: 29, 8, 39 and 7 us.
+// 31 % (the rows' four operands are on their way for a third of it); the plan 5; dK and dV 156 us, 0.62 PFLOP/s, 40 %, reading 0.6 GB of
+// which half is in L2; the join 15.  5003 packed tokens of 12 / 4 heads of 64, fp16: 30, 8, 40 and 7 us.
 #include <algorithm>
 
 #include "attention.h"

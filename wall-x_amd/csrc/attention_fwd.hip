@@ -175,11 +175,11 @@ __device__ __forceinline__ void rows_again(const FwdArgs& a, uint32_t again, flo
 // scales multiply the scores and the probabilities, a value per key.  (A form whose four wavefronts each walked tiles of their own for 32
 // rows, without a barrier, was no faster for single queries: 38 against 35 us over 8 x 32768 cached keys.)
 //
-// What bounds it: 16384 causal tokens of 16 / 2 heads of 128 take 0.98 ms, 1.13 PFLOP/s (a large library product in the same type: 1.36
+// What bounds it: 16384 causal tokens of 16 / 2 heads of 128 take 0.97 to 1.01 ms, 1.13 to 1.09 PFLOP/s (a large library product in the same type: 1.36
 // PFLOP/s), without bank conflicts, at a clock that the power holds near 1.9 GHz.  Half a step of the two groups takes 1400 to 1800
 // cycles, in which a SIMD's products need 1024, the other group's powers some 930 (one is four passes) and the tiles' way out of
 // LDS, 128 KB, as long as the products.  With 128 rows, each wavefront at its own pace: 1.03 ms, matrix units busy 58 % of the time, vector
-// units 56 %.  16 rows of 912 tokens: 71 to 78 us, 0.65 PFLOP/s; of a workgroup's time a quarter lies
+// units 56 %.  16 rows of 912 tokens: 71 to 80 us, 0.65 PFLOP/s; of a workgroup's time a quarter lies
 // before its first product.  48 x 1024 patches in windows of 64, 16 heads of 80: 119 us, 4.2 TB/s.  64 x 32 queries over 800 to 912 cached
 // keys: 34 us, by the vector units (46 %) and the widening's way through LDS.  Single queries of 8 sequences over 20 to 32 thousand
 // cached keys: 112 MB in 28 us, 4.0 TB/s, and 4 for the join.
