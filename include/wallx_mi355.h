@@ -553,6 +553,42 @@ int wx_cached_attention(const void* q, const void* k_cache, const void* v_cache,
                         int n_kv_heads, int64_t n_queries, int64_t capacity, int head_dim, const int64_t q_strides[3], float scale,
                         int dtype, void* workspace, size_t workspace_bytes, wx_stream_t stream);
 
+/* A paged key / value cache: a pool of pages [num_pages, n_kv_heads, page_size, head_dim] of keys and one of values, e4m3 with scales fp32
+ * [num_pages, n_kv_heads, page_size] as above, or in the tokens' own type (scales NULL).  Token i of request r lies in page
+ * page_table[r][i / page_size] at i % page_size (page_table int32 [requests, pages_per_request]); a slot is page * page_size + place in it.
+ * wx_paged_kv_resize brings requests from lengths[r] to wanted[r] tokens (int32 [requests], clamped to what a row of the table holds).
+ * A request owns ceil(length / page_size) pages, the first of its row.  Pages that nobody owns are a stack: free_count[0] entries of
+ * free_pages [free_capacity].  Freed page i, counted by request, then by place, goes to entry count + freed - 1 - i; the j-th page that
+ * growing requests take, counted alike, comes from entry count + freed - 1 - j: freed ones first, and a growth that is taken back leaves the
+ * stack as it was.  A request that the pages do not suffice for gets the tokens that it has pages for.
+ * new_lengths int32 [requests] and new_free_count int32 [1] are written, lengths and free_count are not (no buffer may be two of them); in
+ * page_table and free_pages only entries behind what is owned and free before are: the same call again does the same.  starts int32
+ * [requests + 1]: where each request's added tokens begin among all of them; slots int32 and positions int64 [max_tokens]: of each added
+ * token its slot and its position in its request, -1 and 0 behind the last.  max_tokens bounds the tokens that are added: of more, starts stays at it and the rest has no
+ * slot.  At most 4096 requests, 2^31 - 1 tokens and slots.
+ * wx_paged_kv_write puts token b * seq + s of k and v [batch, n_kv_heads, seq, head_dim] (strides as above) into slots[b * seq + s],
+ * quantised like wx_kv_cache_write's or, with scales NULL, as it is.  Tokens whose slot is not in [0, num_pages * page_size) are dropped; of
+ * two tokens of one slot either may stay. */
+int wx_paged_kv_resize(const int32_t* lengths, const int32_t* wanted, int32_t* page_table, int32_t* free_pages, const int32_t* free_count,
+                       int32_t* new_lengths, int32_t* new_free_count, int32_t* starts, int32_t* slots, int64_t* positions,
+                       int64_t requests, int64_t pages_per_request, int64_t free_capacity, int page_size, int64_t max_tokens,
+                       wx_stream_t stream);
+int wx_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages, float* k_scale, float* v_scale, const int32_t* slots,
+                      int64_t batch, int n_kv_heads, int64_t seq, int64_t num_pages, int page_size, int head_dim,
+                      const int64_t k_strides[3], const int64_t v_strides[3], int dtype, wx_stream_t stream);
+/* wx_attention_fwd of requests of different lengths over the pages.  q [batch, n_q_heads, seq, head_dim] through strides as above; token t
+ * is position t % seq of row t / seq, and request r's n queries are tokens starts[r] .. starts[r + 1] - 1 (starts NULL: requests == batch
+ * and a row of q is a request).  Query i of them sees its request's keys below lengths[r] and, with causal, below lengths[r] - n + i + 1:
+ * the queries are its newest tokens, whose keys are in the cache.  Lengths count up to what a row of the table holds; keys in pages outside
+ * of [0, num_pages) are not seen; starts are clamped to the tokens that there are.  out [batch, seq, n_q_heads, head_dim], contiguous; tokens
+ * of no request and queries that see nothing get zeros.  A token that two requests claim gets the result of one of them. */
+size_t wx_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int n_q_heads, int n_kv_heads, int head_dim);
+int wx_paged_attention(const void* q, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, void* out,
+                       const int32_t* page_table, const int32_t* lengths, const int32_t* starts, int causal, int64_t batch, int n_q_heads,
+                       int n_kv_heads, int64_t seq, int64_t requests, int64_t pages_per_request, int64_t num_pages, int page_size,
+                       int head_dim, const int64_t q_strides[3], float scale, int dtype, void* workspace, size_t workspace_bytes,
+                       wx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,12 +51,17 @@ struct Entry {
   decltype(&wx_attention_bwd) attention_bwd;
   decltype(&wx_kv_cache_write) cache_write;
   decltype(&wx_cached_attention) cached_attention;
+  decltype(&wx_paged_kv_resize) paged_resize;
+  decltype(&wx_paged_kv_write) paged_write;
+  decltype(&wx_paged_attention_workspace_bytes) paged_bytes;
+  decltype(&wx_paged_attention) paged_attention;
 } entry;
 const char* const kNames[] = {"wx_last_error_string", "wx_mrope_apply", "wx_mrope_apply_bwd", "wx_mrope_apply_positions",
                               "wx_mrope_apply_packed", "wx_mrope_table_width", "wx_partition_workspace_bytes", "wx_partition_build",
                               "wx_permute_rows", "wx_unpermute_rows", "wx_unpermute_rows_bwd_clear", "wx_qk_norm_rope",
                               "wx_qk_norm_rope_bwd_workspace_bytes", "wx_qk_norm_rope_bwd", "wx_attention_workspace_bytes", "wx_attention_fwd",
-                              "wx_attention_bwd_workspace_bytes", "wx_attention_bwd", "wx_kv_cache_write", "wx_cached_attention"};
+                              "wx_attention_bwd_workspace_bytes", "wx_attention_bwd", "wx_kv_cache_write", "wx_cached_attention",
+                              "wx_paged_kv_resize", "wx_paged_kv_write", "wx_paged_attention_workspace_bytes", "wx_paged_attention"};
 constexpr int kEntries = sizeof(kNames) / sizeof(kNames[0]);
 static_assert(sizeof(Entry) == kEntries * sizeof(void*), "a name per entry point");
 
@@ -619,6 +624,101 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the paged cache
+void written(const at::Tensor* t) {  // in place, as an in-place op would
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+bool is_ints(const at::Tensor* t, int64_t dim, const at::Tensor& like) {
+  return t && t->dim() == dim && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == like.device();
+}
+
+// paged_resize(lengths, wanted, page_table, free_pages, free_count, page_size, max_tokens) -> (lengths, free_count, starts, slots, positions) or None.
+PyObject* paged_resize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t page_size, max_tokens;
+  if (n != 7 || !entry.paged_resize || !to_int(args[5], page_size) || !to_int(args[6], max_tokens)) return none();
+  const at::Tensor *lengths = plain(args[0]), *wanted = plain(args[1]), *table = plain(args[2]), *stack = plain(args[3]), *count = plain(args[4]);
+  if (!lengths || !is_ints(lengths, 1, *lengths) || !is_ints(wanted, 1, *lengths) || !is_ints(table, 2, *lengths) || !is_ints(stack, 1, *lengths) ||
+      !is_ints(count, 1, *lengths))
+    return none();
+  const int64_t R = lengths->size(0);
+  if (wanted->size(0) != R || table->size(0) != R || count->size(0) != 1 || page_size <= 0 || page_size > INT32_MAX || max_tokens < 0) return none();
+  at::Tensor out[5];
+  const bool ok = run(*lengths, [&] {
+    const int64_t sizes[5] = {R, 1, R + 1, max_tokens, max_tokens};
+    for (int i = 0; i < 5; ++i) out[i] = at::empty({sizes[i]}, i < 4 ? lengths->options() : lengths->options().dtype(at::kLong));
+    auto to = [&](int i) { return static_cast<int32_t*>(ptr(out[i])); };
+    return entry.paged_resize(ints(*lengths), ints(*wanted), static_cast<int32_t*>(ptr(*table)), static_cast<int32_t*>(ptr(*stack)), ints(*count), to(0), to(1), to(2),
+                              to(3), static_cast<int64_t*>(ptr(out[4])), R, table->size(1), stack->size(0), static_cast<int>(page_size), max_tokens, stream_of(*lengths));
+  });
+  if (!ok) return nullptr;
+  written(table);
+  written(stack);
+  PyObject* const r = PyTuple_New(5);
+  for (int i = 0; r && i < 5; ++i) PyTuple_SET_ITEM(r, i, wrap(out[i]));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// k_pages, v_pages, k_scale, v_scale on q's device in the layout that the kernels take: e4m3 with scales, or q's type without
+bool pages_of(PyObject* const* args, const at::Tensor& q, const at::Tensor* (&c)[4]) {
+  for (int i = 0; i < 4; ++i)
+    if (i < 2 ? (c[i] = plain(args[i])) == nullptr : !optional(args[i], c[i])) return false;
+  if ((c[2] == nullptr) != (c[3] == nullptr) || c[0]->dim() != 4 || !c[1]->sizes().equals(c[0]->sizes()) || c[0]->size(3) != q.size(3) || q.size(3) > 1024) return false;
+  for (int i = 0; i < 4; ++i) {
+    if (!c[i]) continue;
+    if (!packed16(*c[i]) || c[i]->device() != q.device()) return false;
+    if (c[i]->scalar_type() != (i >= 2 ? at::kFloat : c[2] ? at::kFloat8_e4m3fn : q.scalar_type())) return false;
+    if (i >= 2 && !c[i]->sizes().equals(c[0]->sizes().slice(0, 3))) return false;
+  }
+  return c[0]->size(1) <= INT32_MAX && c[0]->size(2) > 0 && c[0]->size(2) <= INT32_MAX;
+}
+float* floats(const at::Tensor* t) { return t ? static_cast<float*>(t->data_ptr()) : nullptr; }
+
+// paged_write(k, v, k_pages, v_pages, k_scale, v_scale, slots) -> True or None.
+PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !entry.paged_write) return none();
+  const at::Tensor *k = plain(args[0]), *v = plain(args[1]), *c[4], *slots = plain(args[6]);
+  if (!k || !v || !slots || !rows16(*k) || !rows16(*v) || !attention_type(k->scalar_type()) || !pages_of(args + 2, *k, c)) return none();
+  if (!v->sizes().equals(k->sizes()) || v->scalar_type() != k->scalar_type() || v->device() != k->device() || c[0]->size(1) != k->size(1) || needs_grad({k, v})) return none();
+  const int64_t B = k->size(0), S = k->size(2);
+  if (!(is_ints(slots, 1, *k) && slots->size(0) == B * S) && !(is_ints(slots, 2, *k) && slots->size(0) == B && slots->size(1) == S)) return none();
+  const bool ok = run(*k, [&] {
+    return entry.paged_write(ptr(*k), ptr(*v), ptr(*c[0]), ptr(*c[1]), floats(c[2]), floats(c[3]), ints(*slots), B, static_cast<int>(k->size(1)), S, c[0]->size(0),
+                             static_cast<int>(c[0]->size(2)), static_cast<int>(k->size(3)), RowStrides(*k).v, RowStrides(*v).v, dtype_code(k->scalar_type()),
+                             stream_of(*k));
+  });
+  if (!ok) return nullptr;
+  for (const at::Tensor* t : c) written(t);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts, causal, scale) -> out or None.
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *c[4], *table, *lengths, *starts;
+  if (n != 10 || !entry.paged_attention || !(q = plain(args[0])) || !rows16(*q) || !attention_type(q->scalar_type()) || !pages_of(args + 1, *q, c)) return none();
+  if (!is_ints(table = plain(args[5]), 2, *q) || !is_ints(lengths = plain(args[6]), 1, *q) || !optional(args[7], starts) || !PyBool_Check(args[8])) return none();
+  double scale = 1.0 / std::sqrt(static_cast<double>(q->size(3)));
+  if (args[9] != Py_None && !to_double(args[9], scale)) return none();
+  const int64_t B = q->size(0), Hq = q->size(1), S = q->size(2), D = q->size(3), Hk = c[0]->size(1), R = table->size(0);
+  if (!heads_fit(Hq, Hk) || lengths->size(0) != R || (starts ? !is_ints(starts, 1, *q) || starts->size(0) != R + 1 : R != B) || needs_grad({q})) return none();
+  at::Tensor out;
+  const bool ok = run(*q, [&] {
+    out = token_major(B, Hq, S, D, q->options());
+    const size_t bytes = entry.paged_bytes(B * S, R, static_cast<int>(Hq), static_cast<int>(Hk), static_cast<int>(D));
+    const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q->options().dtype(at::kByte)) : at::Tensor();
+    return entry.paged_attention(ptr(*q), ptr(*c[0]), ptr(*c[1]), floats(c[2]), floats(c[3]), ptr(out), ints(*table), ints(*lengths), starts ? ints(*starts) : nullptr,
+                                 args[8] == Py_True, B, static_cast<int>(Hq), static_cast<int>(Hk), S, R, table->size(1), c[0]->size(0), static_cast<int>(c[0]->size(2)),
+                                 static_cast<int>(D), RowStrides(*q).v, static_cast<float>(scale), dtype_code(q->scalar_type()), bytes ? ptr(work) : nullptr, bytes,
+                                 stream_of(*q));
+  });
+  return ok ? wrap(out) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
 // names() -> the entry points in the order bind() takes their addresses in.
 PyObject* names(PyObject*, PyObject*) {
   PyObject* const r = PyTuple_New(kEntries);
@@ -659,6 +759,9 @@ PyMethodDef methods[] = {{"rope", WX_FAST(rope), nullptr},
                          {"attention", WX_FAST(attention), nullptr},
                          {"cached_attention", WX_FAST(cached_attention), nullptr},
                          {"cache_write", WX_FAST(cache_write), nullptr},
+                         {"paged_resize", WX_FAST(paged_resize), nullptr},
+                         {"paged_write", WX_FAST(paged_write), nullptr},
+                         {"paged_attention", WX_FAST(paged_attention), nullptr},
                          {"bind", WX_FAST(bind), nullptr},
                          {"names", names, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

@@ -91,6 +91,10 @@ PROTOTYPES = {
     "wx_attention_bwd": (_i32, [_vp] * 12 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32] + [_c.POINTER(_i64)] * 4 + [_f32, _i32, _vp, _sz, _vp]),
     "wx_kv_cache_write": (_i32, [_vp] * 8 + [_i64, _i32, _i64, _i64, _i32] + [_c.POINTER(_i64)] * 2 + [_i32, _vp]),
     "wx_cached_attention": (_i32, [_vp] * 8 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32, _c.POINTER(_i64), _f32, _i32, _vp, _sz, _vp]),
+    "wx_paged_kv_resize": (_i32, [_vp] * 10 + [_i64] * 3 + [_i32, _i64, _vp]),
+    "wx_paged_kv_write": (_i32, [_vp] * 7 + [_i64, _i32, _i64, _i64, _i32, _i32] + [_c.POINTER(_i64)] * 2 + [_i32, _vp]),
+    "wx_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i32, _i32, _i32]),
+    "wx_paged_attention": (_i32, [_vp] * 9 + [_i32, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _c.POINTER(_i64), _f32, _i32, _vp, _sz, _vp]),
     "wx_swiglu_bwd": (_i32, [_vp] * 6 + [_i64, _vp]),
     "wx_swiglu_bwd_tiled": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
 }
@@ -134,7 +138,7 @@ def host_path() -> str:
 class _NoHost:
     """In the place of the host module where it is not built: every call goes on in the general path."""
 
-    rope = permute = unpermute = unpermute_bwd = norm_rope = attention = cached_attention = cache_write = capture_check = staticmethod(lambda *args: None)
+    rope = permute = unpermute = unpermute_bwd = norm_rope = attention = cached_attention = cache_write = paged_write = paged_resize = paged_attention = capture_check = staticmethod(lambda *args: None)
 
 
 def host():

@@ -129,6 +129,21 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key
     return native.cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges, key_lengths, causal, scale)
 
 
+def paged_kv_resize(lengths, wanted, page_table, free_pages, free_count, page_size, max_tokens):
+    """No counterpart in backend.py: the bookkeeping of a paged cache."""
+    return native.paged_kv_resize(lengths, wanted, page_table, free_pages, free_count, page_size, max_tokens)
+
+
+def paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots):
+    """No counterpart in backend.py: keys and values into the pages of such a cache."""
+    return native.paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots)
+
+
+def paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts=None, causal=False, scale=None):
+    """No counterpart in backend.py: attention over it."""
+    return native.paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts, causal, scale)
+
+
 def get_rope_index(input_ids, image_grid_thw, video_grid_thw, second_per_grid_ts, attention_mask,
                    spatial_merge_size, image_token_id, video_token_id, vision_start_token_id, tokens_per_second):
     """backend.py:302-352 (forwards to the native op named rope_index)."""

@@ -681,6 +681,83 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key
     return backend.cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges, key_lengths, causal, scale)
 
 
+# ----------------------------------------------------------------------------- paged key / value cache
+def paged_kv_cache(num_pages, num_key_value_heads, page_size, head_dim, device, dtype=torch.float8_e4m3fn):
+    """(k_pages, v_pages, k_scale, v_scale) for paged_kv_write and paged_attention: pages [num_pages, Hkv, page_size, D], of e4m3 codes with
+    fp32 scales [num_pages, Hkv, page_size], or of the tokens' own dtype (bf16 or fp16) with scales None.  Zeroed."""
+    shape = (num_pages, num_key_value_heads, page_size, head_dim)
+    pages = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)]
+    if dtype != torch.float8_e4m3fn:
+        return (*pages, None, None)
+    return (*pages, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def paged_kv_tables(requests, pages_per_request, num_pages, device):
+    """(lengths, page_table, free_pages, free_count) of a paged cache that holds nothing yet, for paged_kv_resize: lengths int32
+    [requests], page_table int32 [requests, pages_per_request], and all pages free, page 0 the first to be taken."""
+    return (torch.zeros(requests, dtype=torch.int32, device=device), torch.full((requests, pages_per_request), -1, dtype=torch.int32, device=device),
+            torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device), torch.full((1,), num_pages, dtype=torch.int32, device=device))
+
+
+def paged_kv_resize(lengths, wanted, page_table, free_pages, free_count, page_size, max_tokens):
+    """Brings requests from lengths to wanted tokens (int32 [R], both): a request that ends or loses tokens (rejected drafts) gives its pages
+    back, one that grows gets pages, and its new tokens get slots.  Returns
+
+        (lengths [R], free_count [1], starts [R + 1], slots [max_tokens], positions [max_tokens])
+
+    as new tensors (int32, positions int64): lengths as they came out, where each request's new tokens begin among all new tokens, and of each
+    such token its slot in the pages and its position in its request; slots are -1 and positions 0 behind the last.  page_table
+    int32 [R, P] and free_pages int32 are updated in place, only behind the entries that lengths and free_count cover: until its caller takes the
+    new lengths and count over, a call can be made again and does the same.  free_pages is a stack that has room for all pages: the first page
+    freed (by request, then by place) is the first taken, and a growth that is taken back leaves it as it was.  Where pages do not suffice, a
+    request gets the tokens that it has pages for, in the requests' order: compare lengths with wanted.  max_tokens is the most that
+    is added (in checked mode, native.set_checked, more raises; otherwise the rest has no slot).  One launch, nothing read by the host; at
+    most 4096 requests."""
+    made = None if native.is_checked() else _lib.host().paged_resize(lengths, wanted, page_table, free_pages, free_count, page_size, max_tokens)
+    if made is not None:
+        return made
+    for name, t in (("lengths", lengths), ("wanted", wanted), ("page_table", page_table), ("free_pages", free_pages), ("free_count", free_count)):
+        if t.is_cpu:
+            raise RuntimeError(f"[Error] The input `{name}` of paged_kv_resize op is on the device: CPU!")
+    return backend.paged_kv_resize(lengths, wanted, page_table, free_pages, free_count, page_size, max_tokens)
+
+
+def paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots):
+    """Writes token b S + s of k and v [B, Hkv, S, D] (bf16 or fp16, through their strides) into slots[b S + s] of the pages in place:
+    slot = page * page_size + place.  e4m3 pages take it quantised as kv_cache_write does; with scales None pages of k's dtype take it as it
+    is.  slots int32 [B S] or [B, S] on the device, never read by the host; tokens whose slot is outside of the pages (-1: padding) are
+    dropped, the rest of the pages stays as it is.  Not differentiable."""
+    if _lib.host().paged_write(k, v, k_pages, v_pages, k_scale, v_scale, slots):
+        return
+    for name, t in (("k", k), ("v", v)):
+        if t.is_cpu:
+            raise RuntimeError(f"[Error] The input `{name}` of paged_kv_write op is on the device: CPU!")
+    _no_tangents("paged_kv_write", k, v)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise RuntimeError("paged_kv_write is not differentiable: call it under torch.no_grad() or on detached tensors")
+    backend.paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots)
+
+
+def paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts=None, causal=False, scale=None):
+    """`attention` of requests' newest tokens over their pages, each request with its own number of queries and keys: one token, a few drafted
+    ones, a denoise step's action tokens, a chunk of a prompt, side by side in one call.
+
+    q [B, Hq, S, D]; token b S + s of it is numbered so, and request r's queries are tokens starts[r] up to, not including, starts[r + 1] (int32
+    [R + 1], what paged_kv_resize returned; None: request r is row r of q).  Its keys are the first lengths[r] tokens (int32 [R]) of the pages in
+    page_table[r] (int32 [R, P]), its queries' own among them; with causal=True the queries are the last of these and see up to themselves,
+    without all see all.  Tokens of no request and queries that see nothing get zeros; what a query does not see does not influence it whatever it
+    holds, and pages outside of the pool are not seen.  Nothing of the tables is read by the host.  Inference only."""
+    made = _lib.host().paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts, causal, scale)
+    if made is not None:
+        return made
+    if q.is_cpu:
+        raise RuntimeError("[Error] The input `q` of paged_attention op is on the device: CPU!")
+    _no_tangents("paged_attention", q)
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError("paged_attention is not differentiable: call it under torch.no_grad() or on detached tensors")
+    return backend.paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts, causal, scale)
+
+
 # ----------------------------------------------------------------------------- index builders
 def get_rope_index(input_ids, spatial_merge_size, image_token_id, video_token_id, vision_start_token_id,
                    tokens_per_second, image_grid_thw=None, video_grid_thw=None, second_per_grid_ts=None,

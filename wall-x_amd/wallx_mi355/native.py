@@ -742,6 +742,111 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, key_ranges=None, key
     return out
 
 
+# ----------------------------------------------------------------------------- paged key / value cache
+def _int32_on(name, t, shape, like):
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 {list(shape)} tensor")
+    if not t.is_cuda or t.device != like.device:
+        raise RuntimeError(f"{name} must be on {like.device}")
+
+
+def paged_kv_resize(lengths, wanted, page_table, free_pages, free_count, page_size: int, max_tokens: int):
+    """Requests of lengths int32 [R] tokens brought to wanted int32 [R]: pages freed onto and taken from the stack free_pages
+    (free_count int32 [1] entries of it), page_table int32 [R, P] filled in in place.  Returns (lengths [R], free_count [1], starts
+    int32 [R + 1], slots int32 [max_tokens], positions int64 [max_tokens]), new tensors."""
+    _need_cuda("lengths", lengths)
+    if lengths.dim() != 1 or page_table.dim() != 2 or free_pages.dim() != 1:
+        raise RuntimeError("lengths must be [requests], page_table [requests, pages] and free_pages [pages]")
+    R, P = lengths.size(0), page_table.size(1)
+    for name, t, shape in (("lengths", lengths, (R,)), ("wanted", wanted, (R,)), ("page_table", page_table, (R, P)), ("free_pages", free_pages, free_pages.shape),
+                           ("free_count", free_count, (1,))):
+        _int32_on(name, t, shape, lengths)
+    page_size, max_tokens = int(page_size), int(max_tokens)
+    if max_tokens < 0:
+        raise RuntimeError("max_tokens must not be negative")
+    new = lambda n, dtype=torch.int32: torch.empty(n, dtype=dtype, device=lengths.device)
+    out = new(R), new(1), new(R + 1), new(max_tokens), new(max_tokens, torch.int64)
+    with _DeviceGuard(lengths):
+        _lib.call("wx_paged_kv_resize", _ptr(lengths), _ptr(wanted), _ptr(page_table), _ptr(free_pages), _ptr(free_count), *(_ptr(t) for t in out), R, P,
+                  free_pages.size(0), page_size, max_tokens, _stream(lengths))
+    for t in (page_table, free_pages):
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)  # (written in place, as an in-place op would)
+    if _checked and capture_id(_stream(lengths)) == 0:
+        added = int((out[0].long() - lengths.long()).clamp(min=0).sum())
+        if added > max_tokens:
+            raise ValueError(f"paged_kv_resize: {added} tokens were added, max_tokens is {max_tokens}")
+    return out
+
+
+def _paged_args(x, k_pages, v_pages, k_scale, v_scale):
+    if x.dtype not in _ATTENTION_DTYPES:
+        raise RuntimeError("the tokens must be BFloat16 or Half")
+    if k_pages.dim() != 4:
+        raise RuntimeError("the pages must be [pages, Hkv, page size, D] tensors")
+    if (k_scale is None) != (v_scale is None):
+        raise RuntimeError("k_scale and v_scale must both be given or both be None")
+    pages = torch.float8_e4m3fn if k_scale is not None else x.dtype
+    for name, t, like, dtype in (("k_pages", k_pages, k_pages.shape, pages), ("v_pages", v_pages, k_pages.shape, pages),
+                                 ("k_scale", k_scale, k_pages.shape[:3], torch.float32), ("v_scale", v_scale, k_pages.shape[:3], torch.float32)):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(like) or not t.is_contiguous()):
+            raise RuntimeError(f"{name} must be a contiguous {str(dtype).replace('torch.', '')} {list(like)} tensor")
+
+
+def paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots) -> None:
+    """Puts token b S + s of k and v [B, Hkv, S, D] (any strides) into slots (int32, B S of them) of the pages, e4m3
+    [N, Hkv, page size, D] with scales fp32 [N, Hkv, page size], or of k's type with scales None."""
+    _same_device(("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("k_scale", k_scale), ("v_scale", v_scale), ("slots", slots))
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise RuntimeError("k and v must be [B, Hkv, S, D] tensors of one shape and dtype")
+    _paged_args(k, k_pages, v_pages, k_scale, v_scale)
+    B, Hk, S, D = k.shape
+    N, _, ps, _ = k_pages.shape
+    if (k_pages.size(1), k_pages.size(3)) != (Hk, D):
+        raise RuntimeError("k and the pages differ in heads or head size")
+    if slots.dtype != torch.int32 or tuple(slots.shape) not in ((B * S,), (B, S)):
+        raise RuntimeError(f"slots must be int32 [{B * S}] or [{B}, {S}]")
+    k, v, slots = _rows16(k), _rows16(v), slots.contiguous()
+    with _DeviceGuard(k):
+        _lib.call("wx_paged_kv_write", _ptr(k), _ptr(v), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), _ptr(slots), B, Hk, S, N, ps, D, _row_strides(k),
+                  _row_strides(v), _DTYPES[k.dtype], _stream(k))
+    for t in (k_pages, v_pages, k_scale, v_scale):
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)  # (written in place, as an in-place op would)
+
+
+def paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts=None, causal: bool = False, scale: Optional[float] = None):
+    """attention_fwd's result for requests over such pages, [B, Hq, S, D] over token-major memory: request r's queries are tokens starts[r]
+    .. starts[r + 1] - 1 of q [B, Hq, S, D] (token b S + s; None: row r), its keys the first lengths[r] of its pages."""
+    _same_device(("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("k_scale", k_scale), ("v_scale", v_scale), ("page_table", page_table), ("lengths", lengths),
+                 ("starts", starts))
+    if q.dim() != 4:
+        raise RuntimeError("q must be a [B, H, S, D] tensor")
+    _paged_args(q, k_pages, v_pages, k_scale, v_scale)
+    B, Hq, S, D = q.shape
+    N, Hk, ps, _ = k_pages.shape
+    if k_pages.size(3) != D or Hk == 0 or Hq % Hk:
+        raise RuntimeError(f"{Hq} query heads of {D} do not go with {Hk} key / value heads of {k_pages.size(3)}")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32:
+        raise RuntimeError("page_table must be int32 [requests, pages]")
+    R, P = page_table.shape
+    for name, t, n in (("lengths", lengths, R), ("starts", starts, R + 1)):
+        if t is not None and (tuple(t.shape) != (n,) or t.dtype != torch.int32):
+            raise RuntimeError(f"{name} must be int32 [{n}]")
+    if starts is None and R != B:
+        raise RuntimeError(f"without starts q's {B} rows are the requests, page_table has {R}")
+    q, page_table, lengths = _rows16(q), page_table.contiguous(), lengths.contiguous()
+    starts = None if starts is None else starts.contiguous()
+    out = _token_major(B, Hq, S, D, q)
+    with _DeviceGuard(q):
+        n_work = _lib.load().wx_paged_attention_workspace_bytes(B * S, R, Hq, Hk, D)
+        work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
+        _lib.call("wx_paged_attention", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), _ptr(out), _ptr(page_table), _ptr(lengths), _ptr(starts),
+                  int(bool(causal)), B, Hq, Hk, S, R, P, N, ps, D, _row_strides(q), D ** -0.5 if scale is None else float(scale), _DTYPES[q.dtype], _ptr(work),
+                  n_work, _stream(q))
+    return out
+
+
 # ----------------------------------------------------------------------------- index builders
 def rope_index(input_ids, image_grid_thw, video_grid_thw, second_per_grid_ts, attention_mask,
                spatial_merge_size: int, image_token_id: int, video_token_id: int, vision_start_token_id: int,
