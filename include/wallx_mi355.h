@@ -582,7 +582,7 @@ int wx_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages
  * the queries are its newest tokens, whose keys are in the cache.  Lengths count up to what a row of the table holds; keys in pages outside
  * of [0, num_pages) are not seen; starts are clamped to the tokens that there are.  out [batch, seq, n_q_heads, head_dim], contiguous; tokens
  * of no request and queries that see nothing get zeros.  A token that two requests claim gets the result of one of them. */
-size_t wx_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int n_q_heads, int n_kv_heads, int head_dim);
+size_t wx_paged_attention_workspace_bytes(int64_t tokens, int n_q_heads, int n_kv_heads, int head_dim);
 int wx_paged_attention(const void* q, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, void* out,
                        const int32_t* page_table, const int32_t* lengths, const int32_t* starts, int causal, int64_t batch, int n_q_heads,
                        int n_kv_heads, int64_t seq, int64_t requests, int64_t pages_per_request, int64_t num_pages, int page_size,

@@ -708,7 +708,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   at::Tensor out;
   const bool ok = run(*q, [&] {
     out = token_major(B, Hq, S, D, q->options());
-    const size_t bytes = entry.paged_bytes(B * S, R, static_cast<int>(Hq), static_cast<int>(Hk), static_cast<int>(D));
+    const size_t bytes = entry.paged_bytes(B * S, static_cast<int>(Hq), static_cast<int>(Hk), static_cast<int>(D));
     const at::Tensor work = bytes ? at::empty({static_cast<int64_t>(bytes)}, q->options().dtype(at::kByte)) : at::Tensor();
     return entry.paged_attention(ptr(*q), ptr(*c[0]), ptr(*c[1]), floats(c[2]), floats(c[3]), ptr(out), ints(*table), ints(*lengths), starts ? ints(*starts) : nullptr,
                                  args[8] == Py_True, B, static_cast<int>(Hq), static_cast<int>(Hk), S, R, table->size(1), c[0]->size(0), static_cast<int>(c[0]->size(2)),

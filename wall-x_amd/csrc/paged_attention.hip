@@ -1,9 +1,35 @@
-// Attention of requests' newest tokens over a paged key / value cache (gfx950).
+// Attention of requests' newest tokens over a paged key / value cache: each request has its own number of queries and keys, none of which the
+// host knows (gfx950).
+//
+// Items.  A (request, key / value head, tile of rows) is an item; rows are (query, head of the group) pairs as in attention.h.  Requests of up
+// to 64 rows (single tokens, drafts) are one item a head, others tiles of 128 rows.  Every item has a measure, what it takes in keys: the
+// keys that it sees and some for its start.  The launch is a fixed number of workgroups, two to a CU; each finds the sum of all
+// measures for itself (a prefix sum over the requests) and takes an equal share of it, wherever in an item that begins or ends.  So one request
+// over 32768 keys and 64 over 900 fill the chip alike, without the host and without a plan in memory.  An item that lies in one share is
+// finished there; of one that is cut every share leaves a part (sums, maximum, sum of powers), which a second launch joins, in order.
+#include <algorithm>
+#include <type_traits>
+
 #include "attention.h"
 #include "common.h"
 
 namespace wx {
 namespace {
+
+#define WX_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
+
+constexpr int kFewRows = 64, kTileRows = 128;
+constexpr int kCut = 64;          // items are cut at multiples of so many keys
+constexpr int kStartFew = 64, kStartMany = 64;  // an item's start, in keys
+constexpr int kLeastFew = 256, kLeastMany = 256;  // the least that a workgroup takes
+
+struct Part {  // of the item that begins in a share and ends in a later one
+  int parts;   // 0: there is none
+  int head;    // key / value head
+  int first;   // the request's first token
+  int row0, rows;
+  int pad[3];
+};
 
 struct PagedArgs {
   const uint16_t* q;               // [batch, n_q, seq, D] through strides; token t is position t % seq of row t / seq
@@ -13,77 +39,916 @@ struct PagedArgs {
   uint16_t* out;                   // [tokens, n_q, D]
   const int32_t *table, *lengths, *starts;  // [requests, width], [requests], [requests + 1] or null: seq tokens each
   int causal, tokens, requests, n_q, n_kv, group, seq, width, page_size, n_pages;
-  Divider by_seq, by_page, by_q;
+  Divider by_seq, by_page, by_group;
   float c;                         // scale * log2(e)
+  int shares;                      // workgroups, a multiple of 8
+  int part_rows;                   // most rows of an item
+  float* sums;                     // parts: [2 shares, part_rows, D]
+  float2* stats;                   // [2 shares, part_rows] (maximum, sum of powers)
+  Part* part;                      // [shares]
 };
 
-// The first version: a wavefront per token and query head, a key per lane.
-template <int DT, int D, bool F8>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
-  const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = a.by_q.div(id), hq = id - t * a.n_q;
-  if (t >= a.tokens) return;
-  const int hk = hq / a.group;
-  int req = -1, i = 0, n = 0;
-  for (int r = 0; r < a.requests; ++r) {
-    const int from = a.starts ? min(max(a.starts[r], 0), a.tokens) : r * a.seq, to = a.starts ? min(a.starts[r + 1], a.tokens) : from + a.seq;
-    if (t >= from && t < to) req = r, i = t - from, n = to - from;
+struct Request {
+  int first, n, length;  // tokens first .. first + n - 1, `length` keys
+  int rows;              // n * group
+};
+__device__ __forceinline__ Request request(const PagedArgs& a, int r) {
+  Request q;
+  if (a.starts != nullptr) {
+    q.first = min(max(a.starts[r], 0), a.tokens);
+    q.n = min(max(a.starts[r + 1], q.first), a.tokens) - q.first;
+  } else {
+    q.first = r * a.seq, q.n = a.seq;
   }
-  float o[2] = {0.f, 0.f}, m = -kInf, l = 0.f;
-  if (req >= 0) {
-    const int b = a.by_seq.div(t);
-    const uint16_t* q = a.q + b * a.qs[0] + hq * a.qs[1] + static_cast<int64_t>(t - b * a.seq) * a.qs[2];
-    const int length = min(max(a.lengths[req], 0), a.width * a.page_size), hi = a.causal ? min(length, length - n + i + 1) : length;
-    for (int k0 = 0; k0 < hi; k0 += 64) {
-      const int key = min(k0 + lane, hi - 1), place = a.by_page.div(key), page = a.table[static_cast<int64_t>(req) * a.width + place];
-      const bool there = k0 + lane < hi && page >= 0 && page < a.n_pages;
-      const int64_t row = (static_cast<int64_t>(there ? page : 0) * a.n_kv + hk) * a.page_size + key - place * a.page_size;
-      float s = 0.f;
-      for (int c = 0; c < D; c += 2) {
-        float x0, x1;
-        if constexpr (F8) {
-          const int w = static_cast<const uint16_t*>(a.k)[(row * D + c) / 2];
-          x0 = __builtin_amdgcn_cvt_f32_fp8(w, 0), x1 = __builtin_amdgcn_cvt_f32_fp8(w, 1);
-        } else {
-          const uint32_t w = static_cast<const uint32_t*>(a.k)[(row * D + c) / 2];
-          x0 = Elem<DT>::load(w & 0xffffu), x1 = Elem<DT>::load(w >> 16);
-        }
-        s += x0 * Elem<DT>::load(q[c]);
-        s += x1 * Elem<DT>::load(q[c + 1]);
+  q.length = min(max(a.lengths[r], 0), a.width * a.page_size);
+  q.rows = q.n * a.group;
+  return q;
+}
+// keys that the last of the rows up to `row` sees
+__device__ __forceinline__ int keys_seen(const PagedArgs& a, const Request& q, int row) {
+  return a.causal ? min(max(q.length - q.n + a.by_group.div(row) + 1, 0), q.length) : q.length;
+}
+// Tiles of many rows: tile t's measure is base + step (t + 1), which follows the diagonal.
+struct Ramp {
+  int64_t base;
+  int step, tiles;
+  __device__ __forceinline__ int64_t before(int64_t t) const { return t * base + step * (t * (t + 1) / 2); }
+  __device__ __forceinline__ int64_t of(int t) const { return base + step * static_cast<int64_t>(t + 1); }
+};
+__device__ __forceinline__ Ramp ramp(const PagedArgs& a, const Request& q) {
+  const bool slope = a.causal && a.group < kTileRows;
+  return {(slope ? max(q.length - q.n, 0) : q.length) + kStartMany, slope ? (kTileRows + a.group - 1) / a.group : 0, (q.rows + kTileRows - 1) / kTileRows};
+}
+// measure of one head of a request
+__device__ __forceinline__ int64_t measure(const PagedArgs& a, const Request& q, bool few) {
+  if (q.n == 0 || (q.rows <= kFewRows) != few) return 0;
+  if (few) return q.length + kStartFew;
+  const Ramp p = ramp(a, q);
+  return p.before(p.tiles);
+}
+
+template <class T>
+__device__ __forceinline__ T uniform(T x) {
+  static_assert(sizeof(T) % 4 == 0, "");
+  uint32_t w[sizeof(T) / 4];
+  __builtin_memcpy(w, &x, sizeof(T));
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
+  __builtin_memcpy(&x, w, sizeof(T));
+  return x;
+}
+
+// A workgroup's share: [at, at + size) of its kind's measures begins `x` into request r's.
+struct Share {
+  int few, id, r;     // id: unique over both kinds
+  int64_t size, each, x;  // each: what a share of this kind takes
+};
+__device__ __forceinline__ Share share(const PagedArgs& a) {
+  __shared__ int64_t s_sums[4][2];
+  __shared__ int s_r;
+  __shared__ int64_t s_x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (a.requests + 255) / 256;
+  const int first = min(tid * each, a.requests), last = min(first + each, a.requests);
+  int64_t mine[2] = {0, 0}, sum[2];
+  for (int r = first; r < last; ++r) {
+    const Request q = request(a, r);
+    const bool few = q.rows <= kFewRows;
+    mine[few ? 0 : 1] += measure(a, q, few) * a.n_kv;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    long long s = mine[i];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const long long up = __shfl_up(s, d);
+      if (lane >= d) s += up;
+    }
+    sum[i] = s;
+    if (lane == 63) s_sums[wave][i] = s;
+  }
+  __syncthreads();
+  int64_t all[2], before[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    all[i] = s_sums[0][i] + s_sums[1][i] + s_sums[2][i] + s_sums[3][i];
+    before[i] = sum[i] - mine[i];
+    for (int w = 0; w < wave; ++w) before[i] += s_sums[w][i];
+    all[i] = uniform(all[i]);
+  }
+  // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
+  const int per_xcd = a.shares / 8, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+  int p = all[1] == 0 ? per_xcd : 0;
+  if (all[0] != 0 && all[1] != 0) {
+    const float part = static_cast<float>(all[0]) / (static_cast<float>(all[0]) + static_cast<float>(all[1]));
+    p = uniform(min(max(static_cast<int>(part * per_xcd + 0.5f), 1), per_xcd - 1));
+  }
+  Share s;
+  s.few = j < p;
+  const int count = s.few ? 8 * p : 8 * (per_xcd - p), w = s.few ? xcd * p + j : xcd * (per_xcd - p) + j - p;
+  s.id = s.few ? w : 8 * p + w;
+  const int64_t total = s.few ? all[0] : all[1], least = s.few ? kLeastFew : kLeastMany;
+  s.each = uniform(total / count + (total % count != 0));
+  if (s.each < least) s.each = least;
+  const int64_t at = w * s.each;
+  s.size = total - at < s.each ? total - at : s.each;
+  s.r = 0, s.x = 0;
+  s.few = uniform(s.few), s.id = uniform(s.id), s.size = uniform(s.size);
+  if (s.size <= 0) return s;  // (the whole workgroup)
+  int64_t from = before[s.few ? 0 : 1];
+  if (from <= at && at < from + mine[s.few ? 0 : 1])
+    for (int r = first; r < last; ++r) {
+      const int64_t m = measure(a, request(a, r), s.few) * a.n_kv;
+      if (at < from + m) {
+        s_r = r, s_x = at - from;
+        break;
       }
-      if constexpr (F8) s *= a.k_scale[row];
-      s = there ? s : -kInf;
-      const float top = wave_max(s), mn = fmaxf(m, top), alpha = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
-      m = mn;
-      const float p = there ? __builtin_amdgcn_exp2f((s - (m == -kInf ? 0.f : m)) * a.c) : 0.f;
-      l = l * alpha + wave_sum(p);
-      o[0] *= alpha, o[1] *= alpha;
-      const uint64_t seen = __ballot(there);
-      for (int j = 0; j < 64; ++j) {
-        if (!(seen >> j & 1)) continue;
-        const float pj = __shfl(p, j);
-        const int64_t r = (static_cast<int64_t>(__shfl(static_cast<int>(row >> 32), j)) << 32) | static_cast<uint32_t>(__shfl(static_cast<int>(row), j));
-        for (int u = 0; u < 2; ++u)
-          if (lane + 64 * u < D) {
-            const int64_t e = r * D + lane + 64 * u;
-            o[u] += pj * (F8 ? __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(a.v)[e], 0) * a.v_scale[r] : Elem<DT>::load(static_cast<const uint16_t*>(a.v)[e]));
+      from += m;
+    }
+  __syncthreads();
+  s.r = uniform(s_r), s.x = uniform(s_x);
+  return s;
+}
+
+// The next request of a kind, 64 looked at at a time; -1 if there is none.
+__device__ __forceinline__ int next_request(const PagedArgs& a, int r, bool few) {
+  for (; r < a.requests; r += 64) {
+    const int i = r + static_cast<int>(threadIdx.x & 63);
+    const uint64_t is = __ballot(i < a.requests && measure(a, request(a, min(i, a.requests - 1)), few) != 0);
+    if (is != 0) return r + __builtin_ctzll(is);
+  }
+  return -1;
+}
+
+// The type of the second product.  e4m3 codes are exact in both types, but fp16's range is too short for a probability times its key's
+// scale: there the codes are widened to bf16 and the probabilities enter as the sum of two bf16 numbers, which is more of them than fp16 keeps.
+template <int DT, bool F8>
+constexpr int kValues = F8 ? WX_BF16 : DT;
+template <int DT, bool F8>
+constexpr bool kTwice = F8 && DT == WX_F16;
+
+template <int DT, bool HI>
+__device__ __forceinline__ uint32_t widen2(uint32_t x) {
+  if constexpr (DT == WX_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, HI));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, HI));
+}
+template <int DT>
+__device__ __forceinline__ u32x4 widen8(uint32_t x, uint32_t y) {
+  return u32x4{widen2<DT, false>(x), widen2<DT, true>(x), widen2<DT, false>(y), widen2<DT, true>(y)};
+}
+// what rounding x to bf16 leaves (nothing of what is not finite)
+__device__ __forceinline__ float left_of(float x) {
+  const float r = x - round_bf16(x);
+  return r - r == 0.f ? r : 0.f;
+}
+__device__ __forceinline__ f32x16 left_of(const f32x16& x) {
+  f32x16 y;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) y[r] = left_of(x[r]);
+  return y;
+}
+
+// One segment: rows row0 .. row0 + rows - 1 of a request over the keys lo .. hi - 1.
+struct Segment {
+  Request q;
+  int r, head, row0, rows, lo, hi;
+  bool whole;  // all of its item: the result itself
+  int slot;    // otherwise its part's place
+};
+
+// This lane's key of a tile: its row in the pages, or that it has none.
+struct KeyRow {
+  uint32_t row;
+  bool ok;
+};
+__device__ __forceinline__ int page_of(const PagedArgs& a, const Segment& g, int key) {  // (key: below g.hi)
+  return a.table[static_cast<int64_t>(g.r) * a.width + a.by_page.div(key)];
+}
+__device__ __forceinline__ KeyRow row_of(const PagedArgs& a, const Segment& g, int key, int page) {
+  const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
+  const uint32_t in = static_cast<uint32_t>(key - a.by_page.div(key) * a.page_size);
+  return {ok ? (static_cast<uint32_t>(page) * a.n_kv + g.head) * a.page_size + in : 0u, ok};
+}
+
+// A lane's row: its query, where that lies, and the keys that it sees of the segment's.
+struct Row {
+  int at, hq, seen;
+  int token;
+  bool live;
+};
+__device__ __forceinline__ Row row_at(const PagedArgs& a, const Segment& g, int i) {
+  Row w;
+  w.live = i < g.rows;
+  w.at = w.live ? i : 0;
+  const int row = g.row0 + w.at, qi = a.by_group.div(row);
+  w.hq = g.head * a.group + row - qi * a.group;
+  w.token = g.q.first + qi;
+  w.seen = w.live ? min(keys_seen(a, g.q, row), g.hi) : g.hi;  // (rows that there are not see everything: they take no mask)
+  return w;
+}
+__device__ __forceinline__ const uint16_t* query(const PagedArgs& a, const Row& w) {
+  const int b = a.by_seq.div(w.token);
+  return a.q + b * a.qs[0] + w.hq * a.qs[1] + static_cast<int64_t>(w.token - b * a.seq) * a.qs[2];
+}
+__device__ __forceinline__ int64_t result(const PagedArgs& a, const Row& w, int d) { return (static_cast<int64_t>(w.token) * a.n_q + w.hq) * d; }
+
+// Rows whose sums are not numbers (see Odd, attention.h) again, of 32 of the segment's rows from `first` on those that `again` has a bit for,
+// from memory, with the maximum and the sum that they ended with.
+template <int DT, int D, bool F8>
+__device__ __forceinline__ void rows_again(const PagedArgs& a, const Segment& g, int first, uint32_t again, float m, float l) {
+  using T = AttnTile<D>;
+  constexpr int PT = kValues<DT, F8>;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const Row w = row_at(a, g, first + (lane & 31));
+  const bool redo = again >> (lane & 31) & 1;
+  const float mc = m == -kInf ? 0.f : m * a.c;
+  const uint16_t* q = query(a, w);
+  auto where = [&](int key) {
+    key = min(key, g.hi - 1);
+    return row_of(a, g, key, page_of(a, g, key));
+  };
+  for (int o = 0; o < T::kOut; ++o) {
+    f32x16 sum = {};
+    const int c = 32 * o + (lane & 31);
+    for (int k0 = g.lo; k0 < g.hi; k0 += 32) {
+      f32x16 s = {};
+      const KeyRow mine = where(k0 + (lane & 31));
+      for (int t = 0; t < T::kSteps; ++t) {
+        u32x4 x;
+        if constexpr (F8) {
+          const u32x2 y = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(a.k) + static_cast<uint64_t>(mine.row) * D + 16 * t + 8 * h);
+          x = widen8<DT>(y[0], y[1]);
+        } else {
+          x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.k) + static_cast<uint64_t>(mine.row) * D + 16 * t + 8 * h);
+        }
+        s = mfma<DT>(x, *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h), s);
+      }
+      uint32_t seen = 0, zero = 0, at[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = 8 * (r / 4) + 4 * h + r % 4;
+        const KeyRow key = where(k0 + i);
+        const bool sees = redo && k0 + i < w.seen && key.ok;
+        at[r] = key.row;
+        if constexpr (F8) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r] * a.k_scale[key.row], a.c, -mc)) * a.v_scale[key.row];
+        else s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -mc));
+        s[r] = sees ? s[r] : 0.f;
+        seen |= sees ? 1u << r : 0u;
+        zero |= sees && s[r] == 0.f ? 1u << r : 0u;
+      }
+      f32x16 rest;
+      if constexpr (kTwice<DT, F8>) rest = left_of(s);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Odd odd;
+        uint32_t y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // (rows of the step's keys: register 8 t + j of this half)
+          const uint64_t e = static_cast<uint64_t>(at[8 * t + j]) * D + c;
+          y[j] = 0;
+          if (D % 32 == 0 || c < D) {
+            if constexpr (F8) y[j] = widen2<PT, false>(static_cast<const uint8_t*>(a.v)[e]) & 0xffffu;
+            else y[j] = static_cast<const uint16_t*>(a.v)[e];
           }
+        }
+        const u32x4 x = finite8<PT>(y, odd);
+        sum = mfma<PT>(x, pack_step<PT>(s, t), sum);
+        if constexpr (kTwice<DT, F8>) sum = mfma<PT>(x, pack_step<PT>(rest, t), sum);
+        add_odd<PT>(sum, odd, seen, zero, t);
+      }
+    }
+    if (g.whole) store_cols<DT, D>(sum, o, 1.f / l, redo ? a.out + result(a, w, D) : nullptr, lane);
+    else if (redo) store_sums<D>(sum, o, a.sums + (static_cast<int64_t>(g.slot) * a.part_rows + w.at) * D, lane);
+  }
+}
+
+// ---- the mask on 32 keys' scores: bit i of `seen` tells of key i
+__device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u); }
+__device__ __forceinline__ void hide(f32x16& s, uint32_t seen, int h) {
+  const uint32_t mine = seen >> (4 * h);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = mine >> (8 * (r / 4) + r % 4) & 1u ? s[r] : -kInf;
+}
+
+// Running maximum, sum of powers and sums of 32 rows.
+template <int D>
+struct Sums {
+  f32x16 acc[AttnTile<D>::kOut];
+  float m, l;
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int o = 0; o < AttnTile<D>::kOut; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[o][r] = 0.f;
+    m = -kInf, l = 0.f;
+  }
+  // The maximum is only there to keep the powers in range: it moves when a score exceeds it by more than 2^8.
+  template <int NT>
+  __device__ __forceinline__ void raise(const f32x16 (&s)[NT], float c) {
+    float tops[4] = {-kInf, -kInf, -kInf, -kInf};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) tops[r / 2 % 4] = fmaxf(fmaxf(tops[r / 2 % 4], s[n][r]), s[n][r + 1]);
+    const float top = both_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+    if (__any((top - m) * c > 8.f)) {
+      const float mn = fmaxf(m, top), alpha = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int o = 0; o < AttnTile<D>::kOut; ++o)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[o][r] *= alpha;
+    }
+  }
+};
+
+template <int D>
+struct PagedLds {
+  static constexpr int kTiles = 2 * 64 * AttnTile<D>::kPitch;  // 64 keys and values, or 4 times 32 of one of them
+  static constexpr int kScales = 2 * 64 * 4;
+  static constexpr int kJoinStats = 4 * 32 * 36 * 4, kJoin = kJoinStats + 4 * 32 * 8;
+  static constexpr int kFirst = kTiles + kScales > kJoin ? kTiles + kScales : kJoin, kSecond = kTiles + kScales;
+};
+
+// ---- few rows.  Every wavefront walks 32-key tiles of its own, for 32 rows: up to 32 rows the four of a workgroup share the keys, up to 64 two
+// and two.  K and V of a tile go straight to LDS as they are in memory, each into one slot of the wavefront's own that is filled again as soon
+// as it is read: no barrier, some 8 (e4m3) to 16 KB on their way per wavefront, eight wavefronts a CU.  e4m3 is widened behind LDS, which
+// transposes bytes as well.
+template <int D>
+struct RawTile {  // 32 rows of D bytes
+  static constexpr int kChunks = D / 16, kLoads = (32 * kChunks + 63) / 64;
+  __device__ static __forceinline__ int swizzle(int row) {
+    if constexpr (D == 128) return (row & 3) | (((row >> 3) ^ (row >> 2)) & 1) << 2;
+    else if constexpr (D == 64) return (row >> 2) & 3;
+    else return 0;
+  }
+  __device__ static __forceinline__ int at(int row, int chunk) { return (row * kChunks + (chunk ^ swizzle(row))) * 16; }
+};
+
+template <int DT, int D, bool F8>
+__device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
+  using T = AttnTile<D>;
+  using R = RawTile<D>;
+  constexpr int PT = kValues<DT, F8>;
+  constexpr int kLoads = F8 ? R::kLoads : T::kChunks / 2, kElem = F8 ? 1 : 2, kSlot = F8 ? 32 * D : 32 * T::kPitch;
+  unsigned char *const lds_k = lds_slot<PagedLds<D>::kFirst, 0>(), *const lds_v = lds_slot<PagedLds<D>::kSecond, 1>();
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int blocks = g.rows <= 32 ? 1 : 2, kws = 4 / blocks, rb = wave & (blocks - 1), kw = wave / blocks;
+  unsigned char *const my_k = lds_k + wave * kSlot, *const my_v = lds_v + wave * kSlot, *const my_scales = lds_k + 4 * kSlot + wave * 256;
+  static_assert(!F8 || 4 * kSlot + 4 * 256 <= PagedLds<D>::kFirst, "");
+  const Row row = row_at(a, g, rb * 32 + (lane & 31));
+  u32x4 qf[T::kSteps];
+  {
+    const uint16_t* q = query(a, row);
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      // e4m3: two steps take 16 channels of a lane in a row
+      const int c = F8 && t / 2 * 2 + 1 < T::kSteps ? 32 * (t / 2) + 16 * h + 8 * (t % 2) : 16 * t + 8 * h;
+      qf[t] = *reinterpret_cast<const u32x4*>(q + c);
+    }
+  }
+  const int all_see = wave_extreme<false>(row.seen);  // every row sees the keys before
+  const int tiles = (g.hi - g.lo + 31) / 32, mine = tiles > kw ? (tiles - kw + kws - 1) / kws : 0;
+  auto key0 = [&](int i) { return g.lo + (i * kws + kw) * 32; };
+  auto ask = [&](int i) { return page_of(a, g, min(key0(i) + (lane & 31), g.hi - 1)); };
+  uint32_t src[kLoads], scale_row = 0, ok_next = 0;
+  auto find = [&](int i, int page) {  // rows of tile i: of this lane's pieces, and of its scale
+    const int key = key0(i) + (lane & 31);
+    const KeyRow k = row_of(a, g, min(key, g.hi - 1), page);
+    ok_next = static_cast<uint32_t>(__ballot(k.ok && key < g.hi));
+    scale_row = k.row;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) src[u] = __shfl(k.row, (u * 64 + lane) / (F8 ? R::kChunks : T::kChunks) & 31);
+  };
+  auto load = [&](const void* from, unsigned char* slot) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int n = u * 64 + lane, chunks = F8 ? R::kChunks : T::kChunks, r = n / chunks, c = (n % chunks) ^ (F8 ? R::swizzle(r) : T::swizzle(r));
+      const char* p = static_cast<const char*>(from) + static_cast<uint64_t>(src[u]) * (D * kElem) + c * 16;
+      if ((F8 ? 32 * R::kChunks % 64 == 0 : true) || n < 32 * R::kChunks)
+        if (F8 || T::kChunks * 8 == D || c < D / 8) __builtin_amdgcn_global_load_lds(WX_GLOBAL(p), WX_LDS(slot + u * 1024), 16, 0, 0);
+    }
+  };
+  auto load_k = [&] {
+    load(a.k, my_k);
+    if constexpr (F8) __builtin_amdgcn_global_load_lds(WX_GLOBAL((h ? a.v_scale : a.k_scale) + scale_row), WX_LDS(my_scales), 4, 0, 0);
+  };
+  constexpr int kLoadsK = kLoads + (F8 ? 1 : 0);
+  auto wait = [&](int later) {  // `later` younger loads may stay in flight
+    asm volatile("" ::: "memory");
+    if (later == 0) __builtin_amdgcn_s_waitcnt(attn_wait(0, 15));
+    else if (later == kLoads) __builtin_amdgcn_s_waitcnt(attn_wait(kLoads, 15));
+    else __builtin_amdgcn_s_waitcnt(attn_wait(kLoadsK, 15));
+    asm volatile("" ::: "memory");
+  };
+  Sums<D> sums;
+  sums.clear();
+  uint32_t ok = 0;
+  int page = 0;
+  if (mine > 0) {
+    const int p0 = ask(0), p1 = ask(1);
+    find(0, p0);
+    load_k();
+    load(a.v, my_v);
+    ok = ok_next;
+    find(1, p1);
+    page = ask(2);
+  }
+  const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
+  // e4m3: bytes 8 (lane & 1) of chunk 2 o + (lane / 16 & 1), of the row that the transposing read wants of this lane
+  const int raw_row = 8 * ((lane >> 3) & 1) + 4 * h + ((lane >> 1) & 3);
+  for (int i = 0; i < mine; ++i) {
+    const int k0 = key0(i);
+    const bool more = i + 1 < mine;
+    wait(kLoads);  // K is there, V may be on its way
+    f32x16 s[1] = {};
+    float ks[F8 ? 16 : 1], vs[F8 ? 16 : 1];
+    if constexpr (F8) {
+#pragma unroll
+      for (int u = 0; u < T::kSteps / 2; ++u) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(my_k + R::at(lane & 31, 2 * u + h));
+        s[0] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[2 * u], s[0]);
+        s[0] = mfma<DT>(widen8<DT>(x[2], x[3]), qf[2 * u + 1], s[0]);
+      }
+      if constexpr (T::kSteps % 2 != 0) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(my_k + R::at(lane & 31, T::kSteps - 1) + 8 * h);
+        s[0] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[T::kSteps - 1], s[0]);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(my_scales + (8 * w + 4 * h) * 4), y = *reinterpret_cast<const float4*>(my_scales + 128 + (8 * w + 4 * h) * 4);
+        ks[4 * w] = x.x, ks[4 * w + 1] = x.y, ks[4 * w + 2] = x.z, ks[4 * w + 3] = x.w;
+        vs[4 * w] = y.x, vs[4 * w + 1] = y.y, vs[4 * w + 2] = y.z, vs[4 * w + 3] = y.w;
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < T::kSteps; ++t) s[0] = mfma<DT>(read_rows<D>(my_k, 0, t, rows_at), qf[t], s[0]);
+    }
+    wait_lds();  // (the slot is read before it is filled again)
+    in_order();
+    if (more) load_k();
+    in_order();
+    if constexpr (F8)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] *= ks[r];
+    if (ok != ~0u || k0 + 32 > all_see) hide(s[0], ok & first_bits(row.seen - k0), h);
+    sums.raise(s, a.c);
+    const float mc = sums.m == -kInf ? 0.f : sums.m * a.c;
+    float l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.c, -mc));
+      l[r & 1] += s[0][r];
+      if constexpr (F8) s[0][r] *= vs[r];
+    }
+    sums.l += l[0] + l[1];
+    u32x4 p[2] = {pack_step<PT>(s[0], 0), pack_step<PT>(s[0], 1)}, p2[2];
+    if constexpr (kTwice<DT, F8>) {
+      const f32x16 rest = left_of(s[0]);
+      p2[0] = pack_step<PT>(rest, 0), p2[1] = pack_step<PT>(rest, 1);
+    }
+    in_order();
+    wait(more ? kLoadsK : 0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int o = 0; o < T::kOut; ++o) {
+        u32x4 x;
+        if constexpr (F8) {
+          typedef int i32x2 __attribute__((ext_vector_type(2)));
+          typedef __attribute__((address_space(3))) i32x2* P;
+          int chunk = 2 * o + ((lane >> 4) & 1);
+          if (R::kChunks % 2 != 0) chunk = min(chunk, R::kChunks - 1);  // (channels past the last: read, not used)
+          const i32x2 y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((P)(my_v + R::at(16 * t + raw_row, chunk) + 8 * (lane & 1)));
+          x = widen8<PT>(static_cast<uint32_t>(y[0]), static_cast<uint32_t>(y[1]));
+        } else {
+          x = read_cols<D>(my_v, 0, t, o, cols_at);
+        }
+        sums.acc[o] = mfma<PT>(x, p[t], sums.acc[o]);
+        if constexpr (kTwice<DT, F8>) sums.acc[o] = mfma<PT>(x, p2[t], sums.acc[o]);
+      }
+    wait_lds();
+    in_order();
+    if (more) load(a.v, my_v);
+    in_order();
+    ok = ok_next;
+    if (more) find(i + 2, page);
+    page = ask(i + 3);
+  }
+  // ---- the wavefronts' sums together, 32 channels at a time through LDS
+  const float l_mine = both_sum(sums.l);
+  float* const join = reinterpret_cast<float*>(lds_k);
+  float2* const stats = reinterpret_cast<float2*>(lds_k + PagedLds<D>::kJoinStats);
+  __shared__ uint32_t s_again[4];
+  const uint32_t odd = columns(not_numbers<D>(sums.acc) && row.live && mine > 0);
+  __syncthreads();
+  if (h == 0) stats[wave * 32 + lane] = float2{sums.m, l_mine};
+  if (lane == 0) s_again[wave] = odd;
+  __syncthreads();
+  float top = -kInf, l_all = 0.f;
+  uint32_t again = 0;
+  for (int u = 0; u < kws; ++u) {
+    top = fmaxf(top, stats[(u * blocks + rb) * 32 + (lane & 31)].x);
+    again |= s_again[u * blocks + rb];
+  }
+  for (int u = 0; u < kws; ++u) {
+    const float2 st = stats[(u * blocks + rb) * 32 + (lane & 31)];
+    l_all += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top) * a.c);
+  }
+  again = __builtin_amdgcn_readfirstlane(again) & columns(l_all == l_all);
+  const float f = sums.m == -kInf ? 0.f : __builtin_amdgcn_exp2f((sums.m - top) * a.c);
+  const int each = 32 / kws;  // rows that a wavefront finishes, 4 lanes a row
+  const int r = kw * each + (lane >> 2), src_lane = r & 31;
+  const bool finish = lane >> 2 < each && rb * 32 + r < g.rows && !(again >> src_lane & 1);
+  const Row fin = row_at(a, g, rb * 32 + src_lane);
+  const float l_r = __shfl(l_all, src_lane);
+#pragma unroll
+  for (int o = 0; o < T::kOut; ++o) {
+    if (o > 0) __syncthreads();
+    const f32x16& x = sums.acc[o];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      *reinterpret_cast<float4*>(join + (wave * 32 + (lane & 31)) * 36 + 8 * w + 4 * h) = float4{x[4 * w] * f, x[4 * w + 1] * f, x[4 * w + 2] * f, x[4 * w + 3] * f};
+    }
+    __syncthreads();
+    const int ch = 32 * o + 8 * (lane & 3);
+    if (finish && (D % 32 == 0 || ch < D)) {
+      float v[8] = {};
+      for (int u = 0; u < kws; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += join[((u * blocks + rb) * 32 + r) * 36 + 8 * (lane & 3) + e];
+      if (g.whole) {
+        const float inv = l_r == 0.f ? 0.f : 1.f / l_r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = l_r == 0.f ? 0.f : v[e] * inv;
+        *reinterpret_cast<u32x4*>(a.out + result(a, fin, D) + ch) = pack16<DT>(v);
+      } else {
+        float4* to = reinterpret_cast<float4*>(a.sums + (static_cast<int64_t>(g.slot) * a.part_rows + fin.at) * D + ch);
+        to[0] = float4{v[0], v[1], v[2], v[3]};
+        to[1] = float4{v[4], v[5], v[6], v[7]};
       }
     }
   }
-  for (int u = 0; u < 2; ++u)
-    if (lane + 64 * u < D) a.out[(static_cast<int64_t>(t) * a.n_q + hq) * D + lane + 64 * u] = static_cast<uint16_t>(Elem<DT>::store(m == -kInf && l == 0.f ? 0.f : o[u] / l));
+  if (!g.whole && kw == 0 && h == 0 && row.live) a.stats[static_cast<int64_t>(g.slot) * a.part_rows + row.at] = float2{top, l_all};
+  if (again != 0 && kw == 0) rows_again<DT, D, F8>(a, g, rb * 32, again, top, l_all);
+  __syncthreads();  // (LDS is the next segment's)
 }
 
+// ---- many rows: 32 to a wavefront, 128 to a workgroup, which walks tiles of 64 keys together, loaded one ahead: straight to LDS, e4m3 through
+// registers, where it is widened once for all four wavefronts.
+template <int DT, int D, bool F8>
+__device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) {
+  using T = AttnTile<D>;
+  constexpr int PT = kValues<DT, F8>, KB = 64, kTileBytes = KB * T::kPitch, kElem = F8 ? 1 : 2;
+  unsigned char *const lds0 = lds_slot<PagedLds<D>::kFirst, 0>(), *const lds1 = lds_slot<PagedLds<D>::kSecond, 1>();
+  const int tid = threadIdx.x, lane = tid & 63, rw = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const Row row = row_at(a, g, rw * 32 + (lane & 31));
+  u32x4 qf[T::kSteps];
+  {
+    const uint16_t* q = query(a, row);
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) qf[t] = *reinterpret_cast<const u32x4*>(q + 16 * t + 8 * h);
+  }
+  const bool wave_live = rw * 32 < g.rows;
+  const int all_see = wave_extreme<false>(row.seen), some_sees = wave_live ? wave_extreme<true>(row.live ? row.seen : 0) : 0;
+  const int tiles = (g.hi - g.lo + KB - 1) / KB;
+  // a lane finds the row of one of a tile's 64 keys
+  auto ask = [&](int i) { return page_of(a, g, min(g.lo + i * KB + lane, g.hi - 1)); };
+  constexpr int kChunk = D / 16, kPieces = (KB * kChunk + 255) / 256;  // e4m3: 16-byte pieces of a row, of a thread
+  constexpr int kLoads = T::kChunks / 4;                               // otherwise: 16 rows by a wavefront
+  uint32_t src[F8 ? kPieces : kLoads], scale_row = 0;
+  uint64_t ok_next = 0;
+  auto find = [&](int i, int page) {
+    const int key = g.lo + i * KB + lane;
+    const KeyRow k = row_of(a, g, min(key, g.hi - 1), page);
+    ok_next = __ballot(k.ok && key < g.hi);
+    scale_row = k.row;
+    if constexpr (F8) {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) src[u] = __shfl(k.row, (u * 256 + tid) / kChunk & 63);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) src[u] = __shfl(k.row, rw * 16 + (u * 64 + lane) / T::kChunks);
+    }
+  };
+  u32x4 pk[F8 ? kPieces : 1], pv[F8 ? kPieces : 1];
+  float scale = 0.f;
+  auto fetch = [&](unsigned char* slot) {
+    if constexpr (F8) {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        const int n = u * 256 + tid, c = n % kChunk;
+        const uint64_t at = static_cast<uint64_t>(src[u]) * D + c * 16;
+        if (KB * kChunk % 256 == 0 || n < KB * kChunk) {
+          pk[u] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.k) + at);
+          pv[u] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.v) + at);
+        }
+      }
+      if (rw < 2) scale = (rw ? a.v_scale : a.k_scale)[scale_row];
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int n = u * 64 + lane, c = (n % T::kChunks) ^ T::swizzle(n / T::kChunks);
+        const uint64_t at = static_cast<uint64_t>(src[u]) * (2 * D) + c * 16;
+        if (T::kChunks * 8 == D || c < D / 8) {
+          __builtin_amdgcn_global_load_lds(WX_GLOBAL(static_cast<const char*>(a.k) + at), WX_LDS(slot + rw * 16 * T::kPitch + u * 1024), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds(WX_GLOBAL(static_cast<const char*>(a.v) + at), WX_LDS(slot + kTileBytes + rw * 16 * T::kPitch + u * 1024), 16, 0, 0);
+        }
+      }
+    }
+  };
+  auto put = [&](unsigned char* slot) {
+    if constexpr (F8) {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        const int n = u * 256 + tid, r = n / kChunk, c = n % kChunk;
+        if (KB * kChunk % 256 != 0 && n >= KB * kChunk) continue;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          *reinterpret_cast<u32x4*>(slot + T::at(r, 2 * c + half)) = widen8<DT>(pk[u][2 * half], pk[u][2 * half + 1]);
+          *reinterpret_cast<u32x4*>(slot + kTileBytes + T::at(r, 2 * c + half)) = widen8<PT>(pv[u][2 * half], pv[u][2 * half + 1]);
+        }
+      }
+      if (rw < 2) reinterpret_cast<float*>(slot + 2 * kTileBytes)[rw * KB + lane] = scale;
+    }
+  };
+  Sums<D> sums;
+  sums.clear();
+  const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
+  auto step = [&](const unsigned char* tk, int k0, uint64_t ok) {
+    constexpr int kAhead = D == 80 ? 3 : 4, NT = 2, kScores = NT * T::kSteps, kProducts = NT * 2 * T::kOut;
+    const unsigned char* tv = tk + kTileBytes;
+    const float* scales = reinterpret_cast<const float*>(tk + 2 * kTileBytes);
+    int rows_here = rows_at, cols_here = cols_at;
+    asm volatile("" : "+v"(rows_here), "+v"(cols_here));
+    auto read_k = [&](int i) { return read_rows<D>(tk, 32 * (i % NT), i / NT, rows_here); };
+    auto read_v = [&](int i) { return read_cols<D>(tv, 32 * (i / (2 * T::kOut)), i / T::kOut % 2, i % T::kOut, cols_here); };
+    f32x16 s[NT];
+    u32x4 f[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+    in_order();
+#pragma unroll
+    for (int i = 0; i < kScores; ++i) {
+      s[i % NT] = mfma<DT>(f[i % kAhead], qf[i / NT], s[i % NT]);
+      if (i + kAhead < kScores) f[i % kAhead] = read_k(i + kAhead);
+      in_order();
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = read_v(i);
+    in_order();
+    if constexpr (F8) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(scales + 32 * n + 8 * w + 4 * h);
+          s[n][4 * w] *= x.x, s[n][4 * w + 1] *= x.y, s[n][4 * w + 2] *= x.z, s[n][4 * w + 3] *= x.w;
+        }
+    }
+    if (ok != ~0ull || k0 + KB > all_see)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) hide(s[n], static_cast<uint32_t>(ok >> (32 * n)) & first_bits(row.seen - k0 - 32 * n), h);
+    sums.raise(s, a.c);
+    const float mc = sums.m == -kInf ? 0.f : sums.m * a.c;
+    float l[2] = {0.f, 0.f};
+    auto power = [&](int n, int r) {  // of registers r and r + 1
+      s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.c, -mc));
+      s[n][r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r + 1], a.c, -mc));
+      l[0] += s[n][r];
+      l[1] += s[n][r + 1];
+      if constexpr (F8) {
+        const float2 x = *reinterpret_cast<const float2*>(scales + KB + 32 * n + 8 * (r / 4) + 4 * h + r % 4);
+        s[n][r] *= x.x, s[n][r + 1] *= x.y;
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < 8; ++u) power(0, 2 * u);
+    u32x4 p[2], p2[2];
+    auto pack = [&](int n) {
+      p[0] = pack_step<PT>(s[n], 0), p[1] = pack_step<PT>(s[n], 1);
+      if constexpr (kTwice<DT, F8>) {
+        const f32x16 rest = left_of(s[n]);
+        p2[0] = pack_step<PT>(rest, 0), p2[1] = pack_step<PT>(rest, 1);
+      }
+    };
+    pack(0);
+    in_order();
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i) {
+      const int n = i / (2 * T::kOut), t = i / T::kOut % 2, o = i % T::kOut, at = i % (2 * T::kOut);
+      if (n > 0 && at == 0) pack(n);
+      sums.acc[o] = mfma<PT>(f[i % kAhead], p[t], sums.acc[o]);
+      if constexpr (kTwice<DT, F8>) sums.acc[o] = mfma<PT>(f[i % kAhead], p2[t], sums.acc[o]);
+      if (i + kAhead < kProducts) f[i % kAhead] = read_v(i + kAhead);
+      if (n + 1 < NT) {
+        const int each = (8 + 2 * T::kOut - 1) / (2 * T::kOut);
+#pragma unroll
+        for (int u = at * each; u < (at + 1) * each && u < 8; ++u) power(n + 1, 2 * u);
+      }
+      in_order();
+    }
+    sums.l += l[0] + l[1];
+  };
+  uint64_t ok = 0;
+  int page = 0;
+  if (tiles > 0) {
+    const int p0 = ask(0), p1 = ask(1);
+    find(0, p0);
+    fetch(lds0);
+    ok = ok_next;
+    find(1, p1);
+    page = ask(2);
+  }
+  auto turn = [&](int i, unsigned char* slot, unsigned char* other) {
+    const int k0 = g.lo + i * KB;
+    const uint64_t seen = ok;
+    if constexpr (F8) {
+      put(slot);
+      if (i + 1 < tiles) fetch(other);
+      wait_lds();
+      attn_barrier();
+    } else {
+      wait_loads();
+      attn_barrier();
+      if (i + 1 < tiles) fetch(other);
+    }
+    ok = ok_next;
+    if (i + 2 < tiles) find(i + 2, page);
+    page = ask(i + 3);
+    in_order();
+    if (k0 < some_sees) step(slot, k0, seen);
+  };
+  for (int i = 0; i < tiles; i += 2) {
+    turn(i, lds0, lds1);
+    if (i + 1 < tiles) turn(i + 1, lds1, lds0);
+  }
+  const float l = both_sum(sums.l);
+  const uint32_t again = columns(not_numbers<D>(sums.acc) && row.live && some_sees > g.lo) & columns(l == l);
+  const bool store = row.live && !(again >> (lane & 31) & 1);
+  if (g.whole) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (store && l == 0.f) {  // (0 * NaN otherwise)
+#pragma unroll
+      for (int c = 0; c < D / 8; c += 2) *reinterpret_cast<u32x4*>(a.out + result(a, row, D) + 8 * (c + h)) = u32x4{0u, 0u, 0u, 0u};
+    }
+    store_row<DT, D>(sums.acc, inv, store && l != 0.f ? a.out + result(a, row, D) : nullptr, lane);
+  } else {
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+      if (store) store_sums<D>(sums.acc[o], o, a.sums + (static_cast<int64_t>(g.slot) * a.part_rows + row.at) * D, lane);
+    if (row.live && h == 0) a.stats[static_cast<int64_t>(g.slot) * a.part_rows + row.at] = float2{sums.m, l};
+  }
+  if (again != 0) rows_again<DT, D, F8>(a, g, rw * 32, again, sums.m, l);
+  __syncthreads();  // (LDS is the next segment's)
+}
+
+template <int DT, int D, bool F8>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
+  const Share s = share(a);
+  // tokens of no request
+  if (a.starts != nullptr) {
+    const int from = min(max(a.starts[0], 0), a.tokens), to = min(max(a.starts[a.requests], 0), a.tokens);
+    const int64_t row = static_cast<int64_t>(a.n_q) * (D / 8), none = (from + (a.tokens - max(to, from))) * row;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < none; i += static_cast<int64_t>(gridDim.x) * 256)
+      reinterpret_cast<u32x4*>(a.out)[i < from * row ? i : i - from * row + max(to, from) * row] = u32x4{0u, 0u, 0u, 0u};
+  }
+  Part part = {};
+  int64_t left = s.size, x = s.x;
+  int r = s.r;
+  while (left > 0) {
+    Segment g;
+    g.r = r;
+    g.q = request(a, r);
+    const int64_t of_head = measure(a, g.q, s.few);
+    Ramp p = {};
+    int t = 0;
+    g.head = 0;
+    if (x > 0) {  // (only a share's first request begins anywhere but in front)
+      g.head = static_cast<int>(x / of_head);
+      x -= g.head * of_head;
+    }
+    if (s.few) {
+      p = {of_head, 0, 1};
+    } else {
+      p = ramp(a, g.q);
+      int lo = 0, hi = p.tiles - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.before(mid) <= x) lo = mid;
+        else hi = mid - 1;
+      }
+      t = lo;
+      x -= p.before(t);
+    }
+    for (; left > 0 && g.head < a.n_kv; ++g.head, t = 0)
+      for (; left > 0 && t < p.tiles; ++t) {
+        const int64_t of_item = p.of(t), take = of_item - x < left ? of_item - x : left;
+        const int start = s.few ? kStartFew : kStartMany;
+        g.row0 = s.few ? 0 : t * kTileRows;
+        g.rows = min(g.q.rows - g.row0, kTileRows);
+        const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1);
+        auto cut = [&](int64_t at) { return at >= of_item ? seen : static_cast<int>(min(static_cast<int64_t>(seen), max(at - start, static_cast<int64_t>(0)) / kCut * kCut)); };
+        g.lo = cut(x), g.hi = cut(x + take);
+        g.whole = take == of_item;
+        g.slot = 2 * s.id + (x == 0);
+        if (x == 0 && take < of_item) {
+          part.parts = 1 + static_cast<int>((of_item - take + s.each - 1) / s.each);
+          part.head = g.head, part.first = g.q.first, part.row0 = g.row0, part.rows = g.rows;
+        }
+        if (s.few) few_rows<DT, D, F8>(a, g);
+        else many_rows<DT, D, F8>(a, g);
+        left -= take;
+        x = 0;
+      }
+    if (left > 0) r = next_request(a, r + 1, s.few);
+    if (r < 0) break;
+  }
+  if (threadIdx.x == 0) a.part[s.id] = part;
+}
+
+// Joins the parts of the item that begins in share blockIdx.x and ends in a later one: of few parts a wavefront to a row, of many a workgroup,
+// a quarter of them to a wavefront.  Lane l has channels 2 l and 2 l + 1.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+  __shared__ float s_top[4], s_sum[4];
+  __shared__ float2 s_out[4][64];
+  const int id = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Part p = uniform(a.part[id]);
+  if (p.parts == 0) return;
+  const bool split = p.parts > 8;  // (uniform over the workgroup)
+  const int each = split ? (p.parts + 3) / 4 : p.parts, first = split ? min(wave * each, p.parts) : 0, last = min(first + each, p.parts);
+  const int rows_at_once = (split ? 1 : 4) * gridDim.y;
+  for (int row0 = blockIdx.y * (split ? 1 : 4); row0 < p.rows; row0 += rows_at_once) {
+    const int row = split ? row0 : row0 + wave;
+    if (!split && row >= p.rows) continue;
+    auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * id + 1 : 2 * (id + i)) * a.part_rows + row; };
+    float top = -kInf, l = 0.f;
+    for (int i = first + lane; i < last; i += 64) top = fmaxf(top, a.stats[slot(i)].x);
+    top = wave_max(top);
+    if (split) {
+      if (lane == 0) s_top[wave] = top;
+      __syncthreads();
+      top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    }
+    float2 o = {0.f, 0.f};
+    for (int i0 = first; i0 < last; i0 += 64) {
+      const float2 st = i0 + lane < last ? a.stats[slot(i0 + lane)] : float2{-kInf, 0.f};
+      // (a part that the row sees nothing of counts nothing, unless its scores were NaN)
+      const float f = st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c);
+      l += st.x == -kInf ? 0.f * st.y : st.y * f;
+      const int n = min(64, last - i0);
+      for (int i = 0; i < n; i += 8) {
+        float2 y[8];
+        float w[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {  // (past the last: the last one's, without weight)
+          const int at = min(i + u, n - 1);
+          w[u] = i + u < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), at)) : 0.f;
+          y[u] = 2 * lane < D ? reinterpret_cast<const float2*>(a.sums + slot(i0 + at) * D)[lane] : float2{0.f, 0.f};
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          o.x += w[u] == 0.f ? 0.f : y[u].x * w[u];
+          o.y += w[u] == 0.f ? 0.f : y[u].y * w[u];
+        }
+      }
+    }
+    l = wave_sum(l);
+    if (split) {
+      if (lane == 0) s_sum[wave] = l;
+      s_out[wave][lane] = o;
+      __syncthreads();
+      l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+      o.x = (s_out[0][lane].x + s_out[1][lane].x) + (s_out[2][lane].x + s_out[3][lane].x);
+      o.y = (s_out[0][lane].y + s_out[1][lane].y) + (s_out[2][lane].y + s_out[3][lane].y);
+    }
+    const int at = p.row0 + row, i = a.by_group.div(at), hq = p.head * a.group + at - i * a.group;
+    if (2 * lane < D && (!split || wave == 0))
+      reinterpret_cast<uint32_t*>(a.out + (static_cast<int64_t>(p.first + i) * a.n_q + hq) * D)[lane] = l == 0.f ? 0u : pack2<DT>(o.x / l, o.y / l);
+    if (split) __syncthreads();
+  }
+}
+
+int shares() { return std::max(8, 2 * device_cu_count() / 8 * 8); }
+int part_rows(int64_t tokens, int group) { return static_cast<int>(std::min<int64_t>(kTileRows, tokens * group)); }
+
+template <int DT, int D, bool F8>
+int launch(PagedArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((paged_attn_kernel<DT, D, F8>), dim3(static_cast<unsigned>(a.shares)), dim3(256), 0, s, a);
+  if (int rc = check_launch("paged_attn_kernel")) return rc;
+  hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3(static_cast<unsigned>(a.shares), 8), dim3(256), 0, s, a);
+  return check_launch("paged_join_kernel");
+}
 template <int DT, bool F8>
-int launch(const PagedArgs& a, int head_dim, hipStream_t s) {
-  const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.n_q + 3) / 4;
-  if (too_many_blocks(blocks, 256)) return fail(WX_ERR_UNSUPPORTED, "wx_paged_attention: too many tokens");
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (head_dim == 64) hipLaunchKernelGGL((paged_attn_kernel<DT, 64, F8>), grid, dim3(256), 0, s, a);
-  else if (head_dim == 80) hipLaunchKernelGGL((paged_attn_kernel<DT, 80, F8>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((paged_attn_kernel<DT, 128, F8>), grid, dim3(256), 0, s, a);
-  return check_launch("wx_paged_attention");
+int launch(PagedArgs& a, int head_dim, hipStream_t s) {
+  if (head_dim == 64) return launch<DT, 64, F8>(a, s);
+  if (head_dim == 80) return launch<DT, 80, F8>(a, s);
+  return launch<DT, 128, F8>(a, s);
 }
 
 }  // namespace
@@ -91,9 +956,10 @@ int launch(const PagedArgs& a, int head_dim, hipStream_t s) {
 
 using namespace wx;
 
-extern "C" size_t wx_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int n_q_heads, int n_kv_heads, int head_dim) {
-  (void)tokens, (void)requests, (void)n_q_heads, (void)n_kv_heads, (void)head_dim;
-  return 0;
+extern "C" size_t wx_paged_attention_workspace_bytes(int64_t tokens, int n_q_heads, int n_kv_heads, int head_dim) {
+  if (tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0) return 0;
+  const int64_t n = shares(), rows = 2 * n * part_rows(tokens, n_q_heads / n_kv_heads);
+  return static_cast<size_t>(rows * (head_dim + 2) * 4 + n * static_cast<int64_t>(sizeof(Part)));
 }
 
 extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, void* out,
@@ -118,14 +984,15 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   if (group > 1024) return fail(WX_ERR_UNSUPPORTED, "%s: more than 1024 query heads to a key / value head", who);
   if (seq > 0x3fffffffll / n_q_heads || batch > 0x3fffffffll / (seq * n_q_heads)) return fail(WX_ERR_UNSUPPORTED, "%s: more than 2^30 - 1 rows", who);
   if (requests > 0x3fffffffll || pages_per_request > 0x3fffffffll / page_size) return fail(WX_ERR_UNSUPPORTED, "%s: more than 2^30 - 1 keys to a request", who);
-  if (num_pages > 0x7fffffffll / page_size) return fail(WX_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 slots", who);
+  if (num_pages > 0x7fffffffll / page_size || num_pages * page_size > 0xffffffffll / n_kv_heads) return fail(WX_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 slots or 2^32 - 1 rows of them", who);
   if (!q || !out || (requests > 0 && (!lengths || (pages_per_request > 0 && num_pages > 0 && (!page_table || !k_pages || !v_pages)))))
     return fail(WX_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  for (const void* p : {q, k_pages, v_pages, static_cast<const void*>(out)})
+  for (const void* p : {q, k_pages, v_pages, static_cast<const void*>(out), static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(p) & 15) return fail(WX_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8 != 0 || q_strides[i] < 0) return fail(WX_ERR_UNSUPPORTED, "%s: q's strides must be positive and keep rows 16-byte aligned", who);
-  (void)workspace, (void)workspace_bytes;
+  if (!workspace || workspace_bytes < wx_paged_attention_workspace_bytes(batch * seq, n_q_heads, n_kv_heads, head_dim))
+    return fail(WX_ERR_WORKSPACE, "%s: workspace too small (see wx_paged_attention_workspace_bytes)", who);
   PagedArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i];
@@ -133,8 +1000,13 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   a.table = page_table, a.lengths = lengths, a.starts = starts, a.causal = causal != 0;
   a.tokens = static_cast<int>(batch * seq), a.requests = static_cast<int>(requests), a.n_q = n_q_heads, a.n_kv = n_kv_heads, a.group = group;
   a.seq = static_cast<int>(seq), a.width = num_pages ? static_cast<int>(pages_per_request) : 0, a.page_size = page_size, a.n_pages = static_cast<int>(num_pages);
-  a.by_seq = Divider(static_cast<uint32_t>(seq)), a.by_page = Divider(page_size), a.by_q = Divider(n_q_heads);
+  a.by_seq = Divider(static_cast<uint32_t>(seq)), a.by_page = Divider(page_size), a.by_group = Divider(group);
   a.c = scale * kLog2e;
+  a.shares = shares(), a.part_rows = part_rows(a.tokens, group);
+  const int64_t rows = 2ll * a.shares * a.part_rows;
+  a.sums = static_cast<float*>(workspace);
+  a.stats = reinterpret_cast<float2*>(a.sums + rows * head_dim);
+  a.part = reinterpret_cast<Part*>(a.stats + rows);
   hipStream_t s = as_stream(stream);
   if (dtype == WX_BF16) return k_scale ? launch<WX_BF16, true>(a, head_dim, s) : launch<WX_BF16, false>(a, head_dim, s);
   return k_scale ? launch<WX_F16, true>(a, head_dim, s) : launch<WX_F16, false>(a, head_dim, s);

@@ -93,7 +93,7 @@ PROTOTYPES = {
     "wx_cached_attention": (_i32, [_vp] * 8 + [_i32, _i64, _i32, _i32, _i64, _i64, _i32, _c.POINTER(_i64), _f32, _i32, _vp, _sz, _vp]),
     "wx_paged_kv_resize": (_i32, [_vp] * 10 + [_i64] * 3 + [_i32, _i64, _vp]),
     "wx_paged_kv_write": (_i32, [_vp] * 7 + [_i64, _i32, _i64, _i64, _i32, _i32] + [_c.POINTER(_i64)] * 2 + [_i32, _vp]),
-    "wx_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i32, _i32, _i32]),
+    "wx_paged_attention_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "wx_paged_attention": (_i32, [_vp] * 9 + [_i32, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _c.POINTER(_i64), _f32, _i32, _vp, _sz, _vp]),
     "wx_swiglu_bwd": (_i32, [_vp] * 6 + [_i64, _vp]),
     "wx_swiglu_bwd_tiled": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),

@@ -839,7 +839,7 @@ def paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, 
     starts = None if starts is None else starts.contiguous()
     out = _token_major(B, Hq, S, D, q)
     with _DeviceGuard(q):
-        n_work = _lib.load().wx_paged_attention_workspace_bytes(B * S, R, Hq, Hk, D)
+        n_work = _lib.load().wx_paged_attention_workspace_bytes(B * S, Hq, Hk, D)
         work = torch.empty(n_work, dtype=torch.uint8, device=q.device) if n_work else None
         _lib.call("wx_paged_attention", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), _ptr(out), _ptr(page_table), _ptr(lengths), _ptr(starts),
                   int(bool(causal)), B, Hq, Hk, S, R, P, N, ps, D, _row_strides(q), D ** -0.5 if scale is None else float(scale), _DTYPES[q.dtype], _ptr(work),
