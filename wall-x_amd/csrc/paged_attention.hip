@@ -22,6 +22,7 @@ constexpr int kFewRows = 64, kTileRows = 128;
 constexpr int kCut = 64;          // items are cut at multiples of so many keys
 constexpr int kStartFew = 64, kStartMany = 64;  // an item's start, in keys
 constexpr int kLeastFew = 256, kLeastMany = 256;  // the least that a workgroup takes
+constexpr int kSnap = 8;          // an end of an item nearer than an eighth of a share is the share's end
 
 struct Part {  // of the item that begins in a share and ends in a later one
   int parts;   // 0: there is none
@@ -98,22 +99,70 @@ __device__ __forceinline__ T uniform(T x) {
   return x;
 }
 
-// A workgroup's share: [at, at + size) of its kind's measures begins `x` into request r's.
+// A workgroup's share: `size` of its kind's measures, from `x` into tile `tile` of `head` of request r.
 struct Share {
-  int few, id, r;     // id: unique over both kinds
-  int64_t size, each, x;  // each: what a share of this kind takes
+  int few, id;        // id: unique over both kinds
+  int64_t size, each; // each: what a share of this kind takes
+  int64_t snap;       // ends of items nearer than this to a share's end are the share's end
+  int r, head, tile;
+  int64_t x;
+  Request q;
+  int none_from, none_to;  // tokens [0, none_from) and [none_to, all) are no request's
 };
+// Where `at` of a request's measure lies, moved to an item's end if that is near.  Returns by how much it was moved.
+struct Place {
+  int head, tile;
+  int64_t x;
+};
+__device__ __forceinline__ int64_t locate(const PagedArgs& a, const Request& q, bool few, int64_t at, int64_t snap, Place& p) {
+  const int64_t of_head = measure(a, q, few);
+  auto part = [](double x, double y) { return static_cast<int>(x / y); };  // (to one off)
+  p.head = min(part(static_cast<double>(at), static_cast<double>(of_head)), a.n_kv - 1);
+  if (p.head * of_head > at) --p.head;
+  if ((p.head + 1) * of_head <= at) ++p.head;
+  p.x = at - p.head * of_head;
+  p.tile = 0;
+  int64_t of_item = of_head;
+  if (!few) {
+    const Ramp ramp_ = ramp(a, q);
+    int lo = 0, hi = ramp_.tiles - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (ramp_.before(mid) <= p.x) lo = mid;
+      else hi = mid - 1;
+    }
+    p.tile = lo;
+    p.x -= ramp_.before(lo);
+    of_item = ramp_.of(lo);
+  }
+  if (p.x < snap) {
+    const int64_t moved = -p.x;
+    p.x = 0;
+    return moved;
+  }
+  if (of_item - p.x < snap) {
+    const int64_t moved = of_item - p.x;
+    p.x = of_item;
+    return moved;
+  }
+  return 0;
+}
 __device__ __forceinline__ Share share(const PagedArgs& a) {
-  __shared__ int64_t s_sums[4][2];
-  __shared__ int s_r;
-  __shared__ int64_t s_x;
+  __shared__ int64_t s_sums[4][2], s_moved[2];
+  __shared__ Place s_place;
+  __shared__ Request s_q;
+  __shared__ int s_r, s_none[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (a.requests + 255) / 256;
   const int first = min(tid * each, a.requests), last = min(first + each, a.requests);
   int64_t mine[2] = {0, 0}, sum[2];
+  if (tid == 0) s_none[0] = a.requests ? 0 : a.tokens, s_none[1] = a.tokens, s_moved[0] = 0, s_moved[1] = 0;
+  Request q = {};
   for (int r = first; r < last; ++r) {
-    const Request q = request(a, r);
+    q = request(a, r);
     const bool few = q.rows <= kFewRows;
     mine[few ? 0 : 1] += measure(a, q, few) * a.n_kv;
+    if (r == 0) s_none[0] = q.first;
+    if (r == a.requests - 1) s_none[1] = q.first + q.n;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -142,30 +191,38 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     const float part = static_cast<float>(all[0]) / (static_cast<float>(all[0]) + static_cast<float>(all[1]));
     p = uniform(min(max(static_cast<int>(part * per_xcd + 0.5f), 1), per_xcd - 1));
   }
-  Share s;
-  s.few = j < p;
+  Share s = {};
+  s.few = uniform(static_cast<int>(j < p));
   const int count = s.few ? 8 * p : 8 * (per_xcd - p), w = s.few ? xcd * p + j : xcd * (per_xcd - p) + j - p;
   s.id = s.few ? w : 8 * p + w;
-  const int64_t total = s.few ? all[0] : all[1], least = s.few ? kLeastFew : kLeastMany;
-  s.each = uniform(total / count + (total % count != 0));
-  if (s.each < least) s.each = least;
-  const int64_t at = w * s.each;
-  s.size = total - at < s.each ? total - at : s.each;
-  s.r = 0, s.x = 0;
-  s.few = uniform(s.few), s.id = uniform(s.id), s.size = uniform(s.size);
-  if (s.size <= 0) return s;  // (the whole workgroup)
-  int64_t from = before[s.few ? 0 : 1];
-  if (from <= at && at < from + mine[s.few ? 0 : 1])
+  const int64_t total = s.few ? all[0] : all[1];
+  s.each = uniform(max(static_cast<int64_t>(static_cast<double>(total) / count) + 1, static_cast<int64_t>(s.few ? kLeastFew : kLeastMany)));
+  s.snap = s.each / kSnap;
+  const int64_t at = w * s.each, end = at + s.each;
+  s.size = at < total ? (total < end ? total : end) - at : 0;
+  const int kind = s.few ? 0 : 1;
+  const int64_t from = before[kind], to = from + mine[kind];
+  if (s.size > 0 && ((from <= at && at < to) || (from <= end && end < to))) {
+    int64_t m_from = from;
     for (int r = first; r < last; ++r) {
-      const int64_t m = measure(a, request(a, r), s.few) * a.n_kv;
-      if (at < from + m) {
-        s_r = r, s_x = at - from;
-        break;
+      if (each > 1) q = request(a, r);
+      const int64_t m = measure(a, q, s.few) * a.n_kv;
+      Place place;
+      if (m_from <= at && at < m_from + m) {
+        s_moved[0] = locate(a, q, s.few, at - m_from, s.snap, place);
+        s_place = place, s_q = q, s_r = r;
       }
-      from += m;
+      if (m_from <= end && end < m_from + m) s_moved[1] = locate(a, q, s.few, end - m_from, s.snap, place);
+      m_from += m;
     }
+  }
   __syncthreads();
-  s.r = uniform(s_r), s.x = uniform(s_x);
+  s.none_from = uniform(s_none[0]), s.none_to = uniform(s_none[1]);
+  if (s.size > 0) {
+    s.size += uniform(s_moved[1] - s_moved[0]);
+    const Place place = uniform(s_place);
+    s.r = uniform(s_r), s.q = uniform(s_q), s.head = place.head, s.tile = place.tile, s.x = place.x;
+  }
   return s;
 }
 
@@ -362,13 +419,10 @@ struct Sums {
   }
 };
 
+// Two arrays of LDS: of few rows the wavefronts' slots for keys and for values, of many tiles in turn.
+constexpr int kFewSlot = 8192;
 template <int D>
-struct PagedLds {
-  static constexpr int kTiles = 2 * 64 * AttnTile<D>::kPitch;  // 64 keys and values, or 4 times 32 of one of them
-  static constexpr int kScales = 2 * 64 * 4;
-  static constexpr int kJoinStats = 4 * 32 * 36 * 4, kJoin = kJoinStats + 4 * 32 * 8;
-  static constexpr int kFirst = kTiles + kScales > kJoin ? kTiles + kScales : kJoin, kSecond = kTiles + kScales;
-};
+constexpr int kPagedLds = 2 * 64 * AttnTile<D>::kPitch + 2 * 64 * 4 > 4 * kFewSlot ? 2 * 64 * AttnTile<D>::kPitch + 2 * 64 * 4 : 4 * kFewSlot;
 
 // ---- few rows.  Every wavefront walks 32-key tiles of its own, for 32 rows: up to 32 rows the four of a workgroup share the keys, up to 64 two
 // and two.  K and V of a tile go straight to LDS as they are in memory, each into one slot of the wavefront's own that is filled again as soon
@@ -391,11 +445,19 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
   using R = RawTile<D>;
   constexpr int PT = kValues<DT, F8>;
   constexpr int kLoads = F8 ? R::kLoads : T::kChunks / 2, kElem = F8 ? 1 : 2, kSlot = F8 ? 32 * D : 32 * T::kPitch;
-  unsigned char *const lds_k = lds_slot<PagedLds<D>::kFirst, 0>(), *const lds_v = lds_slot<PagedLds<D>::kSecond, 1>();
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  unsigned char *const lds_k = lds_slot<kPagedLds<D>, 0>(), *const lds_v = lds_slot<kPagedLds<D>, 1>();
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // (what is made from it is made here: kept over the segments it would be spilled)
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int blocks = g.rows <= 32 ? 1 : 2, kws = 4 / blocks, rb = wave & (blocks - 1), kw = wave / blocks;
-  unsigned char *const my_k = lds_k + wave * kSlot, *const my_v = lds_v + wave * kSlot, *const my_scales = lds_k + 4 * kSlot + wave * 256;
-  static_assert(!F8 || 4 * kSlot + 4 * 256 <= PagedLds<D>::kFirst, "");
+  unsigned char *const my_k = lds_k + wave * kFewSlot, *const my_v = lds_v + wave * kFewSlot, *const my_scales = my_k + kSlot;
+  static_assert(kSlot + (F8 ? 256 : 0) <= kFewSlot && 32 * 64 * 4 <= kFewSlot, "");
+  const int tiles = (g.hi - g.lo + 31) / 32, mine = tiles > kw ? (tiles - kw + kws - 1) / kws : 0;
+  auto key0 = [&](int i) { return g.lo + (i * kws + kw) * 32; };
+  auto ask = [&](int i) { return page_of(a, g, min(key0(i) + (lane & 31), g.hi - 1)); };
+  int p0 = 0, p1 = 0;
+  if (mine > 0) p0 = ask(0), p1 = ask(1);
+  in_order();
   const Row row = row_at(a, g, rb * 32 + (lane & 31));
   u32x4 qf[T::kSteps];
   {
@@ -408,9 +470,6 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
     }
   }
   const int all_see = wave_extreme<false>(row.seen);  // every row sees the keys before
-  const int tiles = (g.hi - g.lo + 31) / 32, mine = tiles > kw ? (tiles - kw + kws - 1) / kws : 0;
-  auto key0 = [&](int i) { return g.lo + (i * kws + kw) * 32; };
-  auto ask = [&](int i) { return page_of(a, g, min(key0(i) + (lane & 31), g.hi - 1)); };
   uint32_t src[kLoads], scale_row = 0, ok_next = 0;
   auto find = [&](int i, int page) {  // rows of tile i: of this lane's pieces, and of its scale
     const int key = key0(i) + (lane & 31);
@@ -446,7 +505,6 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
   uint32_t ok = 0;
   int page = 0;
   if (mine > 0) {
-    const int p0 = ask(0), p1 = ask(1);
     find(0, p0);
     load_k();
     load(a.v, my_v);
@@ -535,62 +593,79 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
     if (more) find(i + 2, page);
     page = ask(i + 3);
   }
-  // ---- the wavefronts' sums together, 32 channels at a time through LDS
-  const float l_mine = both_sum(sums.l);
-  float* const join = reinterpret_cast<float*>(lds_k);
-  float2* const stats = reinterpret_cast<float2*>(lds_k + PagedLds<D>::kJoinStats);
+  // ---- the wavefronts' sums together: each leaves its own where its slots were, 64 channels a row in either array, and 16 lanes (8 of 64
+  // channels) finish a row.
+  constexpr int kLanes = D == 64 ? 8 : 16, kFinish = 256 / kLanes;
+  __shared__ float2 s_stats[4][32];
   __shared__ uint32_t s_again[4];
+  auto sum_at = [&](int w, int r, int chunk) {  // 4 channels of row r that wavefront w left
+    return reinterpret_cast<float4*>((chunk < 16 ? lds_k : lds_v) + w * kFewSlot + r * 256 + ((chunk ^ r) & 15) * 16);
+  };
+  const float l_mine = both_sum(sums.l);
   const uint32_t odd = columns(not_numbers<D>(sums.acc) && row.live && mine > 0);
-  __syncthreads();
-  if (h == 0) stats[wave * 32 + lane] = float2{sums.m, l_mine};
+  if (row.live) {
+#pragma unroll
+    for (int o = 0; o < T::kOut; ++o)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if (32 * o + 8 * w < D) *sum_at(wave, lane & 31, 8 * o + 2 * w + h) = float4{sums.acc[o][4 * w], sums.acc[o][4 * w + 1], sums.acc[o][4 * w + 2], sums.acc[o][4 * w + 3]};
+    if (h == 0) s_stats[wave][lane] = float2{sums.m, l_mine};
+  }
   if (lane == 0) s_again[wave] = odd;
   __syncthreads();
-  float top = -kInf, l_all = 0.f;
-  uint32_t again = 0;
-  for (int u = 0; u < kws; ++u) {
-    top = fmaxf(top, stats[(u * blocks + rb) * 32 + (lane & 31)].x);
-    again |= s_again[u * blocks + rb];
-  }
-  for (int u = 0; u < kws; ++u) {
-    const float2 st = stats[(u * blocks + rb) * 32 + (lane & 31)];
-    l_all += st.x == -kInf ? 0.f * st.y : st.y * __builtin_amdgcn_exp2f((st.x - top) * a.c);
-  }
-  again = __builtin_amdgcn_readfirstlane(again) & columns(l_all == l_all);
-  const float f = sums.m == -kInf ? 0.f : __builtin_amdgcn_exp2f((sums.m - top) * a.c);
-  const int each = 32 / kws;  // rows that a wavefront finishes, 4 lanes a row
-  const int r = kw * each + (lane >> 2), src_lane = r & 31;
-  const bool finish = lane >> 2 < each && rb * 32 + r < g.rows && !(again >> src_lane & 1);
-  const Row fin = row_at(a, g, rb * 32 + src_lane);
-  const float l_r = __shfl(l_all, src_lane);
+  auto joined = [&](int block, int r, float& top, float& l, float (&f)[4]) {
+    top = -kInf, l = 0.f;
+    for (int u = 0; u < kws; ++u) top = fmaxf(top, s_stats[u * blocks + block][r].x);
 #pragma unroll
-  for (int o = 0; o < T::kOut; ++o) {
-    if (o > 0) __syncthreads();
-    const f32x16& x = sums.acc[o];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      *reinterpret_cast<float4*>(join + (wave * 32 + (lane & 31)) * 36 + 8 * w + 4 * h) = float4{x[4 * w] * f, x[4 * w + 1] * f, x[4 * w + 2] * f, x[4 * w + 3] * f};
+    for (int u = 0; u < 4; ++u) {
+      f[u] = 0.f;
+      if (u >= kws) continue;
+      const float2 st = s_stats[u * blocks + block][r];
+      f[u] = st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c);
+      l += st.x == -kInf ? 0.f * st.y : st.y * f[u];
     }
-    __syncthreads();
-    const int ch = 32 * o + 8 * (lane & 3);
-    if (finish && (D % 32 == 0 || ch < D)) {
-      float v[8] = {};
-      for (int u = 0; u < kws; ++u)
+  };
+  const int c = tid % kLanes;
+#pragma unroll 1
+  for (int i = tid / kLanes; i < g.rows; i += kFinish) {
+    float top, l, f[4];
+    joined(i >> 5, i & 31, top, l, f);
+    uint32_t again = 0;
+    float v[8] = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += join[((u * blocks + rb) * 32 + r) * 36 + 8 * (lane & 3) + e];
-      if (g.whole) {
-        const float inv = l_r == 0.f ? 0.f : 1.f / l_r;
+    for (int u = 0; u < 4; ++u) {
+      if (u >= kws) continue;
+      const int w = u * blocks + (i >> 5);
+      again |= s_again[w];
+      if (8 * c >= D) continue;
+      const float4 x = *sum_at(w, i & 31, 2 * c), y = *sum_at(w, i & 31, 2 * c + 1);
+      v[0] += x.x * f[u], v[1] += x.y * f[u], v[2] += x.z * f[u], v[3] += x.w * f[u];
+      v[4] += y.x * f[u], v[5] += y.y * f[u], v[6] += y.z * f[u], v[7] += y.w * f[u];
+    }
+    const bool store = 8 * c < D && !((again >> (i & 31) & 1) && l == l);
+    if (g.whole) {
+      const float inv = 1.f / l;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = l_r == 0.f ? 0.f : v[e] * inv;
-        *reinterpret_cast<u32x4*>(a.out + result(a, fin, D) + ch) = pack16<DT>(v);
-      } else {
-        float4* to = reinterpret_cast<float4*>(a.sums + (static_cast<int64_t>(g.slot) * a.part_rows + fin.at) * D + ch);
+      for (int e = 0; e < 8; ++e) v[e] = l == 0.f ? 0.f : v[e] * inv;
+      if (store) *reinterpret_cast<u32x4*>(a.out + result(a, row_at(a, g, i), D) + 8 * c) = pack16<DT>(v);
+    } else {
+      const int64_t at = static_cast<int64_t>(g.slot) * a.part_rows + i;
+      if (store) {
+        float4* to = reinterpret_cast<float4*>(a.sums + at * D + 8 * c);
         to[0] = float4{v[0], v[1], v[2], v[3]};
         to[1] = float4{v[4], v[5], v[6], v[7]};
       }
+      if (c == 0) a.stats[at] = float2{top, l};
     }
   }
-  if (!g.whole && kw == 0 && h == 0 && row.live) a.stats[static_cast<int64_t>(g.slot) * a.part_rows + row.at] = float2{top, l_all};
-  if (again != 0 && kw == 0) rows_again<DT, D, F8>(a, g, rb * 32, again, top, l_all);
+  if ((s_again[0] | s_again[1] | s_again[2] | s_again[3]) != 0 && kw == 0) {
+    uint32_t again = 0;
+    for (int u = 0; u < kws; ++u) again |= s_again[u * blocks + rb];
+    float top, l, f[4];
+    joined(rb, lane & 31, top, l, f);
+    again = __builtin_amdgcn_readfirstlane(again) & columns(row.live && l == l);
+    if (again != 0) rows_again<DT, D, F8>(a, g, rb * 32, again, top, l);
+  }
   __syncthreads();  // (LDS is the next segment's)
 }
 
@@ -600,8 +675,10 @@ template <int DT, int D, bool F8>
 __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) {
   using T = AttnTile<D>;
   constexpr int PT = kValues<DT, F8>, KB = 64, kTileBytes = KB * T::kPitch, kElem = F8 ? 1 : 2;
-  unsigned char *const lds0 = lds_slot<PagedLds<D>::kFirst, 0>(), *const lds1 = lds_slot<PagedLds<D>::kSecond, 1>();
-  const int tid = threadIdx.x, lane = tid & 63, rw = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  unsigned char *const lds0 = lds_slot<kPagedLds<D>, 0>(), *const lds1 = lds_slot<kPagedLds<D>, 1>();
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // (see few_rows)
+  const int lane = tid & 63, rw = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const Row row = row_at(a, g, rw * 32 + (lane & 31));
   u32x4 qf[T::kSteps];
   {
@@ -810,63 +887,42 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
 template <int DT, int D, bool F8>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
   const Share s = share(a);
-  // tokens of no request
-  if (a.starts != nullptr) {
-    const int from = min(max(a.starts[0], 0), a.tokens), to = min(max(a.starts[a.requests], 0), a.tokens);
-    const int64_t row = static_cast<int64_t>(a.n_q) * (D / 8), none = (from + (a.tokens - max(to, from))) * row;
+  if (s.none_from > 0 || s.none_to < a.tokens) {
+    const int64_t row = static_cast<int64_t>(a.n_q) * (D / 8), front = s.none_from * row, none = front + (a.tokens - s.none_to) * row;
     for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < none; i += static_cast<int64_t>(gridDim.x) * 256)
-      reinterpret_cast<u32x4*>(a.out)[i < from * row ? i : i - from * row + max(to, from) * row] = u32x4{0u, 0u, 0u, 0u};
+      reinterpret_cast<u32x4*>(a.out)[i < front ? i : i - front + s.none_to * row] = u32x4{0u, 0u, 0u, 0u};
   }
   Part part = {};
   int64_t left = s.size, x = s.x;
-  int r = s.r;
+  int t = s.tile;
+  Segment g;
+  g.r = s.r, g.q = s.q, g.head = s.head;
   while (left > 0) {
-    Segment g;
-    g.r = r;
-    g.q = request(a, r);
-    const int64_t of_head = measure(a, g.q, s.few);
-    Ramp p = {};
-    int t = 0;
-    g.head = 0;
-    if (x > 0) {  // (only a share's first request begins anywhere but in front)
-      g.head = static_cast<int>(x / of_head);
-      x -= g.head * of_head;
-    }
-    if (s.few) {
-      p = {of_head, 0, 1};
-    } else {
-      p = ramp(a, g.q);
-      int lo = 0, hi = p.tiles - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.before(mid) <= x) lo = mid;
-        else hi = mid - 1;
-      }
-      t = lo;
-      x -= p.before(t);
-    }
+    const Ramp p = s.few ? Ramp{g.q.length + kStartFew, 0, 1} : ramp(a, g.q);
     for (; left > 0 && g.head < a.n_kv; ++g.head, t = 0)
-      for (; left > 0 && t < p.tiles; ++t) {
+      for (; left > 0 && t < p.tiles; ++t, x = 0) {
         const int64_t of_item = p.of(t), take = of_item - x < left ? of_item - x : left;
+        if (take <= 0) continue;  // (a share that begins at an item's end)
         const int start = s.few ? kStartFew : kStartMany;
         g.row0 = s.few ? 0 : t * kTileRows;
         g.rows = min(g.q.rows - g.row0, kTileRows);
         const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1);
         auto cut = [&](int64_t at) { return at >= of_item ? seen : static_cast<int>(min(static_cast<int64_t>(seen), max(at - start, static_cast<int64_t>(0)) / kCut * kCut)); };
-        g.lo = cut(x), g.hi = cut(x + take);
+        g.lo = uniform(cut(x)), g.hi = uniform(cut(x + take));
         g.whole = take == of_item;
         g.slot = 2 * s.id + (x == 0);
-        if (x == 0 && take < of_item) {
-          part.parts = 1 + static_cast<int>((of_item - take + s.each - 1) / s.each);
+        if (x == 0 && take < of_item) {  // (the shares' ends behind this one that are inside of the item and not near its end)
+          part.parts = 2 + static_cast<int>(static_cast<double>(of_item - s.snap - take) / static_cast<double>(s.each));
           part.head = g.head, part.first = g.q.first, part.row0 = g.row0, part.rows = g.rows;
         }
         if (s.few) few_rows<DT, D, F8>(a, g);
         else many_rows<DT, D, F8>(a, g);
         left -= take;
-        x = 0;
       }
-    if (left > 0) r = next_request(a, r + 1, s.few);
-    if (r < 0) break;
+    if (left <= 0) break;
+    g.r = next_request(a, g.r + 1, s.few), g.head = 0;
+    if (g.r < 0) break;
+    g.q = request(a, g.r);
   }
   if (threadIdx.x == 0) a.part[s.id] = part;
 }
