@@ -18,7 +18,7 @@ namespace {
 
 #define WX_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
 
-constexpr int kFewRows = 64, kTileRows = 128;
+constexpr int kFewRows = 64, kManyRows = 128;  // rows of an item of either kind
 constexpr int kCut = 64;          // items are cut at multiples of so many keys
 constexpr int kStartFew = 64, kStartMany = 64;  // an item's start, in keys
 constexpr int kLeastFew = 256, kLeastMany = 256;  // the least that a workgroup takes
@@ -43,6 +43,7 @@ struct PagedArgs {
   Divider by_seq, by_page, by_group;
   float c;                         // scale * log2(e)
   int shares;                      // workgroups, a multiple of 8
+  int shift;                       // measures are in 2^shift keys, so that the sum of all fits 31 bits
   int part_rows;                   // most rows of an item
   float* sums;                     // parts: [2 shares, part_rows, D]
   float2* stats;                   // [2 shares, part_rows] (maximum, sum of powers)
@@ -69,22 +70,23 @@ __device__ __forceinline__ Request request(const PagedArgs& a, int r) {
 __device__ __forceinline__ int keys_seen(const PagedArgs& a, const Request& q, int row) {
   return a.causal ? min(max(q.length - q.n + a.by_group.div(row) + 1, 0), q.length) : q.length;
 }
-// Tiles of many rows: tile t's measure is base + step (t + 1), which follows the diagonal.
+__device__ __forceinline__ bool is_few(const PagedArgs& a, const Request& q) { return q.rows <= kFewRows; }
+// The items of one head of a request: tile t's measure is base + step (t + 1), which follows the diagonal.
 struct Ramp {
-  int64_t base;
-  int step, tiles;
-  __device__ __forceinline__ int64_t before(int64_t t) const { return t * base + step * (t * (t + 1) / 2); }
-  __device__ __forceinline__ int64_t of(int t) const { return base + step * static_cast<int64_t>(t + 1); }
+  int base, step, tiles;
+  __device__ __forceinline__ int before(int t) const { return t * base + static_cast<int>(step * (static_cast<int64_t>(t) * (t + 1) / 2)); }
+  __device__ __forceinline__ int of(int t) const { return base + step * (t + 1); }
 };
-__device__ __forceinline__ Ramp ramp(const PagedArgs& a, const Request& q) {
-  const bool slope = a.causal && a.group < kTileRows;
-  return {(slope ? max(q.length - q.n, 0) : q.length) + kStartMany, slope ? (kTileRows + a.group - 1) / a.group : 0, (q.rows + kTileRows - 1) / kTileRows};
+__device__ __forceinline__ int start_of(const PagedArgs& a, bool few) { return max((few ? kStartFew : kStartMany) >> a.shift, 1); }
+__device__ __forceinline__ Ramp ramp(const PagedArgs& a, const Request& q, bool few) {
+  const int rows = few ? kFewRows : kManyRows, tiles = (q.rows + rows - 1) / rows;
+  const int step = a.causal && tiles > 1 ? a.by_group.div(rows) >> a.shift : 0;
+  return {((step ? max(q.length - q.n, 0) : q.length) >> a.shift) + start_of(a, few), step, tiles};
 }
 // measure of one head of a request
-__device__ __forceinline__ int64_t measure(const PagedArgs& a, const Request& q, bool few) {
-  if (q.n == 0 || (q.rows <= kFewRows) != few) return 0;
-  if (few) return q.length + kStartFew;
-  const Ramp p = ramp(a, q);
+__device__ __forceinline__ int measure(const PagedArgs& a, const Request& q, bool few) {
+  if (q.n == 0 || is_few(a, q) != few) return 0;
+  const Ramp p = ramp(a, q, few);
   return p.before(p.tiles);
 }
 
@@ -99,90 +101,79 @@ __device__ __forceinline__ T uniform(T x) {
   return x;
 }
 
+__device__ __forceinline__ int wave_prefix(int x) {  // inclusive, over the wavefront's lanes
+#define WX_ADD(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false)
+  WX_ADD(0x111, 0xF);
+  WX_ADD(0x112, 0xF);
+  WX_ADD(0x114, 0xF);
+  WX_ADD(0x118, 0xF);
+  WX_ADD(0x142, 0xA);  // (the last lane of a row of 16 to the next row, of 32 to the next half)
+  WX_ADD(0x143, 0xC);
+#undef WX_ADD
+  return x;
+}
+
 // A workgroup's share: `size` of its kind's measures, from `x` into tile `tile` of `head` of request r.
 struct Share {
-  int few, id;        // id: unique over both kinds
-  int64_t size, each; // each: what a share of this kind takes
-  int64_t snap;       // ends of items nearer than this to a share's end are the share's end
-  int r, head, tile;
-  int64_t x;
+  int few, id;     // id: unique over both kinds
+  int size, each;  // each: what a share of this kind takes
+  int snap;        // an item's end nearer than this to a share's end is the share's end
+  int r, head, tile, x;
   Request q;
   int none_from, none_to;  // tokens [0, none_from) and [none_to, all) are no request's
 };
 // Where `at` of a request's measure lies, moved to an item's end if that is near.  Returns by how much it was moved.
 struct Place {
-  int head, tile;
-  int64_t x;
+  int head, tile, x;
 };
-__device__ __forceinline__ int64_t locate(const PagedArgs& a, const Request& q, bool few, int64_t at, int64_t snap, Place& p) {
-  const int64_t of_head = measure(a, q, few);
-  auto part = [](double x, double y) { return static_cast<int>(x / y); };  // (to one off)
-  p.head = min(part(static_cast<double>(at), static_cast<double>(of_head)), a.n_kv - 1);
-  if (p.head * of_head > at) --p.head;
-  if ((p.head + 1) * of_head <= at) ++p.head;
+__device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, bool few, int at, int snap, Place& p) {
+  const Ramp items = ramp(a, q, few);
+  const int of_head = items.before(items.tiles);
+  p.head = at / of_head;
   p.x = at - p.head * of_head;
-  p.tile = 0;
-  int64_t of_item = of_head;
-  if (!few) {
-    const Ramp ramp_ = ramp(a, q);
-    int lo = 0, hi = ramp_.tiles - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (ramp_.before(mid) <= p.x) lo = mid;
-      else hi = mid - 1;
-    }
-    p.tile = lo;
-    p.x -= ramp_.before(lo);
-    of_item = ramp_.of(lo);
+  int lo = 0, hi = items.tiles - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (items.before(mid) <= p.x) lo = mid;
+    else hi = mid - 1;
   }
-  if (p.x < snap) {
-    const int64_t moved = -p.x;
-    p.x = 0;
-    return moved;
-  }
-  if (of_item - p.x < snap) {
-    const int64_t moved = of_item - p.x;
-    p.x = of_item;
-    return moved;
-  }
-  return 0;
+  p.tile = lo;
+  p.x -= items.before(lo);
+  const int of_item = items.of(lo), to = p.x < snap ? 0 : (of_item - p.x < snap ? of_item : p.x), moved = to - p.x;
+  p.x = to;
+  return moved;
 }
 __device__ __forceinline__ Share share(const PagedArgs& a) {
-  __shared__ int64_t s_sums[4][2], s_moved[2];
+  __shared__ int s_sums[4][2], s_moved[2];
   __shared__ Place s_place;
   __shared__ Request s_q;
   __shared__ int s_r, s_none[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (a.requests + 255) / 256;
   const int first = min(tid * each, a.requests), last = min(first + each, a.requests);
-  int64_t mine[2] = {0, 0}, sum[2];
+  int mine[2] = {0, 0}, sum[2];
   if (tid == 0) s_none[0] = a.requests ? 0 : a.tokens, s_none[1] = a.tokens, s_moved[0] = 0, s_moved[1] = 0;
   Request q = {};
   for (int r = first; r < last; ++r) {
     q = request(a, r);
-    const bool few = q.rows <= kFewRows;
-    mine[few ? 0 : 1] += measure(a, q, few) * a.n_kv;
+    const bool few = is_few(a, q);
+    const int m = measure(a, q, few) * a.n_kv;
+    mine[0] += few ? m : 0;
+    mine[1] += few ? 0 : m;
     if (r == 0) s_none[0] = q.first;
     if (r == a.requests - 1) s_none[1] = q.first + q.n;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    long long s = mine[i];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const long long up = __shfl_up(s, d);
-      if (lane >= d) s += up;
-    }
-    sum[i] = s;
-    if (lane == 63) s_sums[wave][i] = s;
+    sum[i] = wave_prefix(mine[i]);
+    if (lane == 63) s_sums[wave][i] = sum[i];
   }
   __syncthreads();
-  int64_t all[2], before[2];
+  int all[2], before[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    all[i] = s_sums[0][i] + s_sums[1][i] + s_sums[2][i] + s_sums[3][i];
-    before[i] = sum[i] - mine[i];
-    for (int w = 0; w < wave; ++w) before[i] += s_sums[w][i];
-    all[i] = uniform(all[i]);
+    const int w0 = s_sums[0][i], w1 = s_sums[1][i], w2 = s_sums[2][i];
+    before[i] = sum[i] - mine[i] + (wave > 0 ? w0 : 0) + (wave > 1 ? w1 : 0) + (wave > 2 ? w2 : 0);
+    all[i] = uniform(w0 + w1 + w2 + s_sums[3][i]);
   }
   // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
   const int per_xcd = a.shares / 8, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
@@ -192,34 +183,33 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     p = uniform(min(max(static_cast<int>(part * per_xcd + 0.5f), 1), per_xcd - 1));
   }
   Share s = {};
-  s.few = uniform(static_cast<int>(j < p));
+  s.few = j < p;
   const int count = s.few ? 8 * p : 8 * (per_xcd - p), w = s.few ? xcd * p + j : xcd * (per_xcd - p) + j - p;
   s.id = s.few ? w : 8 * p + w;
-  const int64_t total = s.few ? all[0] : all[1];
-  s.each = uniform(max(static_cast<int64_t>(static_cast<double>(total) / count) + 1, static_cast<int64_t>(s.few ? kLeastFew : kLeastMany)));
+  const int total = s.few ? all[0] : all[1];
+  s.each = uniform(max(total / count + 1, (s.few ? kLeastFew : kLeastMany) >> a.shift));
   s.snap = s.each / kSnap;
-  const int64_t at = w * s.each, end = at + s.each;
-  s.size = at < total ? (total < end ? total : end) - at : 0;
-  const int kind = s.few ? 0 : 1;
-  const int64_t from = before[kind], to = from + mine[kind];
+  const int64_t at = static_cast<int64_t>(w) * s.each, end = at + s.each;
+  s.size = at < total ? static_cast<int>((total < end ? total : end) - at) : 0;
+  const int from = s.few ? before[0] : before[1], to = from + (s.few ? mine[0] : mine[1]);
   if (s.size > 0 && ((from <= at && at < to) || (from <= end && end < to))) {
-    int64_t m_from = from;
+    int r_from = from;
     for (int r = first; r < last; ++r) {
       if (each > 1) q = request(a, r);
-      const int64_t m = measure(a, q, s.few) * a.n_kv;
+      const int m = measure(a, q, s.few) * a.n_kv;
       Place place;
-      if (m_from <= at && at < m_from + m) {
-        s_moved[0] = locate(a, q, s.few, at - m_from, s.snap, place);
+      if (r_from <= at && at < r_from + m) {
+        s_moved[0] = locate(a, q, s.few, static_cast<int>(at) - r_from, s.snap, place);
         s_place = place, s_q = q, s_r = r;
       }
-      if (m_from <= end && end < m_from + m) s_moved[1] = locate(a, q, s.few, end - m_from, s.snap, place);
-      m_from += m;
+      if (r_from <= end && end < r_from + m) s_moved[1] = locate(a, q, s.few, static_cast<int>(end) - r_from, s.snap, place);
+      r_from += m;
     }
   }
   __syncthreads();
   s.none_from = uniform(s_none[0]), s.none_to = uniform(s_none[1]);
   if (s.size > 0) {
-    s.size += uniform(s_moved[1] - s_moved[0]);
+    s.size = uniform(s.size + s_moved[1] - s_moved[0]);
     const Place place = uniform(s_place);
     s.r = uniform(s_r), s.q = uniform(s_q), s.head = place.head, s.tile = place.tile, s.x = place.x;
   }
@@ -420,17 +410,17 @@ struct Sums {
 };
 
 // Two arrays of LDS: of few rows the wavefronts' slots for keys and for values, of many tiles in turn.
-constexpr int kFewSlot = 8192;
+constexpr int kFewSlot = 8192 + 512;
 template <int D>
 constexpr int kPagedLds = 2 * 64 * AttnTile<D>::kPitch + 2 * 64 * 4 > 4 * kFewSlot ? 2 * 64 * AttnTile<D>::kPitch + 2 * 64 * 4 : 4 * kFewSlot;
 
-// ---- few rows.  Every wavefront walks 32-key tiles of its own, for 32 rows: up to 32 rows the four of a workgroup share the keys, up to 64 two
-// and two.  K and V of a tile go straight to LDS as they are in memory, each into one slot of the wavefront's own that is filled again as soon
-// as it is read: no barrier, some 8 (e4m3) to 16 KB on their way per wavefront, eight wavefronts a CU.  e4m3 is widened behind LDS, which
-// transposes bytes as well.
+// ---- few rows.  Every wavefront walks tiles of its own, of 64 (e4m3) or 32 keys, for 32 rows: up to 32 rows the four of a workgroup share the
+// keys, up to 64 two and two.  K and V of a tile go straight to LDS as they are in memory, each into one slot of the wavefront's own that is
+// filled again as soon as it is read: no barrier, 16 KB on their way per wavefront, eight wavefronts a CU.  e4m3 is widened behind LDS,
+// which transposes bytes as well.
 template <int D>
-struct RawTile {  // 32 rows of D bytes
-  static constexpr int kChunks = D / 16, kLoads = (32 * kChunks + 63) / 64;
+struct RawTile {  // rows of D bytes
+  static constexpr int kChunks = D / 16;
   __device__ static __forceinline__ int swizzle(int row) {
     if constexpr (D == 128) return (row & 3) | (((row >> 3) ^ (row >> 2)) & 1) << 2;
     else if constexpr (D == 64) return (row >> 2) & 3;
@@ -443,18 +433,19 @@ template <int DT, int D, bool F8>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
   using T = AttnTile<D>;
   using R = RawTile<D>;
-  constexpr int PT = kValues<DT, F8>;
-  constexpr int kLoads = F8 ? R::kLoads : T::kChunks / 2, kElem = F8 ? 1 : 2, kSlot = F8 ? 32 * D : 32 * T::kPitch;
+  constexpr int PT = kValues<DT, F8>, KB = F8 ? 64 : 32, NT = KB / 32;
+  constexpr int kChunks = F8 ? R::kChunks : T::kChunks, kLoads = KB * kChunks / 64, kElem = F8 ? 1 : 2, kSlot = KB * kChunks * 16;
   unsigned char *const lds_k = lds_slot<kPagedLds<D>, 0>(), *const lds_v = lds_slot<kPagedLds<D>, 1>();
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));  // (what is made from it is made here: kept over the segments it would be spilled)
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int blocks = g.rows <= 32 ? 1 : 2, kws = 4 / blocks, rb = wave & (blocks - 1), kw = wave / blocks;
   unsigned char *const my_k = lds_k + wave * kFewSlot, *const my_v = lds_v + wave * kFewSlot, *const my_scales = my_k + kSlot;
-  static_assert(kSlot + (F8 ? 256 : 0) <= kFewSlot && 32 * 64 * 4 <= kFewSlot, "");
-  const int tiles = (g.hi - g.lo + 31) / 32, mine = tiles > kw ? (tiles - kw + kws - 1) / kws : 0;
-  auto key0 = [&](int i) { return g.lo + (i * kws + kw) * 32; };
-  auto ask = [&](int i) { return page_of(a, g, min(key0(i) + (lane & 31), g.hi - 1)); };
+  static_assert(kLoads * 64 == KB * kChunks && kSlot + (F8 ? 512 : 0) <= kFewSlot && 32 * 64 * 4 <= kFewSlot, "");
+  const int tiles = (g.hi - g.lo + KB - 1) / KB, mine = tiles > kw ? (tiles - kw + kws - 1) / kws : 0;
+  auto key0 = [&](int i) { return g.lo + (i * kws + kw) * KB; };
+  const int in_tile = lane & (KB - 1);  // a lane finds the row of one of a tile's keys
+  auto ask = [&](int i) { return page_of(a, g, min(key0(i) + in_tile, g.hi - 1)); };
   int p0 = 0, p1 = 0;
   if (mine > 0) p0 = ask(0), p1 = ask(1);
   in_order();
@@ -470,44 +461,45 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
     }
   }
   const int all_see = wave_extreme<false>(row.seen);  // every row sees the keys before
-  uint32_t src[kLoads], scale_row = 0, ok_next = 0;
-  auto find = [&](int i, int page) {  // rows of tile i: of this lane's pieces, and of its scale
-    const int key = key0(i) + (lane & 31);
+  uint32_t src[kLoads], scale_row = 0;
+  uint64_t ok_next = 0;
+  auto find = [&](int i, int page) {  // rows of tile i: of this lane's pieces, and of its scales
+    const int key = key0(i) + in_tile;
     const KeyRow k = row_of(a, g, min(key, g.hi - 1), page);
-    ok_next = static_cast<uint32_t>(__ballot(k.ok && key < g.hi));
+    ok_next = __ballot(k.ok && key < g.hi);
     scale_row = k.row;
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) src[u] = __shfl(k.row, (u * 64 + lane) / (F8 ? R::kChunks : T::kChunks) & 31);
+    for (int u = 0; u < kLoads; ++u) src[u] = __shfl(k.row, (u * 64 + lane) / kChunks);
   };
   auto load = [&](const void* from, unsigned char* slot) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const int n = u * 64 + lane, chunks = F8 ? R::kChunks : T::kChunks, r = n / chunks, c = (n % chunks) ^ (F8 ? R::swizzle(r) : T::swizzle(r));
+      const int n = u * 64 + lane, r = n / kChunks, c = (n % kChunks) ^ (F8 ? R::swizzle(r) : T::swizzle(r));
       const char* p = static_cast<const char*>(from) + static_cast<uint64_t>(src[u]) * (D * kElem) + c * 16;
-      if ((F8 ? 32 * R::kChunks % 64 == 0 : true) || n < 32 * R::kChunks)
-        if (F8 || T::kChunks * 8 == D || c < D / 8) __builtin_amdgcn_global_load_lds(WX_GLOBAL(p), WX_LDS(slot + u * 1024), 16, 0, 0);
+      if (F8 || T::kChunks * 8 == D || c < D / 8) __builtin_amdgcn_global_load_lds(WX_GLOBAL(p), WX_LDS(slot + u * 1024), 16, 0, 0);
     }
   };
-  auto load_k = [&] {
-    load(a.k, my_k);
-    if constexpr (F8) __builtin_amdgcn_global_load_lds(WX_GLOBAL((h ? a.v_scale : a.k_scale) + scale_row), WX_LDS(my_scales), 4, 0, 0);
+  auto load_values = [&] {  // and the scales, in front of them: they are there when the next keys are
+    if constexpr (F8) {
+      __builtin_amdgcn_global_load_lds(WX_GLOBAL(a.k_scale + scale_row), WX_LDS(my_scales), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds(WX_GLOBAL(a.v_scale + scale_row), WX_LDS(my_scales + 256), 4, 0, 0);
+    }
+    load(a.v, my_v);
   };
-  constexpr int kLoadsK = kLoads + (F8 ? 1 : 0);
-  auto wait = [&](int later) {  // `later` younger loads may stay in flight
+  auto wait = [&](bool younger) {  // the loads of one slot that are younger than what is waited for may stay in flight
     asm volatile("" ::: "memory");
-    if (later == 0) __builtin_amdgcn_s_waitcnt(attn_wait(0, 15));
-    else if (later == kLoads) __builtin_amdgcn_s_waitcnt(attn_wait(kLoads, 15));
-    else __builtin_amdgcn_s_waitcnt(attn_wait(kLoadsK, 15));
+    if (younger) __builtin_amdgcn_s_waitcnt(attn_wait(kLoads, 15));
+    else __builtin_amdgcn_s_waitcnt(attn_wait(0, 15));
     asm volatile("" ::: "memory");
   };
   Sums<D> sums;
   sums.clear();
-  uint32_t ok = 0;
+  uint64_t ok = 0;
   int page = 0;
   if (mine > 0) {
     find(0, p0);
-    load_k();
-    load(a.v, my_v);
+    load(a.k, my_k);
+    load_values();
     ok = ok_next;
     find(1, p1);
     page = ask(2);
@@ -518,57 +510,71 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
   for (int i = 0; i < mine; ++i) {
     const int k0 = key0(i);
     const bool more = i + 1 < mine;
-    wait(kLoads);  // K is there, V may be on its way
-    f32x16 s[1] = {};
-    float ks[F8 ? 16 : 1], vs[F8 ? 16 : 1];
+    wait(true);  // keys and scales are there, values may be on their way
+    f32x16 s[NT] = {};
     if constexpr (F8) {
 #pragma unroll
-      for (int u = 0; u < T::kSteps / 2; ++u) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(my_k + R::at(lane & 31, 2 * u + h));
-        s[0] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[2 * u], s[0]);
-        s[0] = mfma<DT>(widen8<DT>(x[2], x[3]), qf[2 * u + 1], s[0]);
-      }
-      if constexpr (T::kSteps % 2 != 0) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(my_k + R::at(lane & 31, T::kSteps - 1) + 8 * h);
-        s[0] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[T::kSteps - 1], s[0]);
-      }
+      for (int u = 0; u < T::kSteps / 2; ++u)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float4 x = *reinterpret_cast<const float4*>(my_scales + (8 * w + 4 * h) * 4), y = *reinterpret_cast<const float4*>(my_scales + 128 + (8 * w + 4 * h) * 4);
-        ks[4 * w] = x.x, ks[4 * w + 1] = x.y, ks[4 * w + 2] = x.z, ks[4 * w + 3] = x.w;
-        vs[4 * w] = y.x, vs[4 * w + 1] = y.y, vs[4 * w + 2] = y.z, vs[4 * w + 3] = y.w;
-      }
+        for (int n = 0; n < NT; ++n) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(my_k + R::at(32 * n + (lane & 31), 2 * u + h));
+          s[n] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[2 * u], s[n]);
+          s[n] = mfma<DT>(widen8<DT>(x[2], x[3]), qf[2 * u + 1], s[n]);
+        }
+      if constexpr (T::kSteps % 2 != 0)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(my_k + R::at(32 * n + (lane & 31), T::kSteps - 1) + 8 * h);
+          s[n] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[T::kSteps - 1], s[n]);
+        }
     } else {
 #pragma unroll
       for (int t = 0; t < T::kSteps; ++t) s[0] = mfma<DT>(read_rows<D>(my_k, 0, t, rows_at), qf[t], s[0]);
     }
     wait_lds();  // (the slot is read before it is filled again)
     in_order();
-    if (more) load_k();
+    if (more) load(a.k, my_k);
     in_order();
+    const float* scales = reinterpret_cast<const float*>(my_scales);
     if constexpr (F8)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[0][r] *= ks[r];
-    if (ok != ~0u || k0 + 32 > all_see) hide(s[0], ok & first_bits(row.seen - k0), h);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(scales + 32 * n + 8 * w + 4 * h);
+          s[n][4 * w] *= x.x, s[n][4 * w + 1] *= x.y, s[n][4 * w + 2] *= x.z, s[n][4 * w + 3] *= x.w;
+        }
+    if (ok != (KB == 64 ? ~0ull : 0xffffffffull) || k0 + KB > all_see)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) hide(s[n], static_cast<uint32_t>(ok >> (32 * n)) & first_bits(row.seen - k0 - 32 * n), h);
     sums.raise(s, a.c);
     const float mc = sums.m == -kInf ? 0.f : sums.m * a.c;
     float l[2] = {0.f, 0.f};
+    u32x4 p[2 * NT], p2[kTwice<DT, F8> ? 2 * NT : 1];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.c, -mc));
-      l[r & 1] += s[0][r];
-      if constexpr (F8) s[0][r] *= vs[r];
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.c, -mc));
+        l[r & 1] += s[n][r];
+      }
+      if constexpr (F8)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(scales + KB + 32 * n + 8 * w + 4 * h);
+          s[n][4 * w] *= x.x, s[n][4 * w + 1] *= x.y, s[n][4 * w + 2] *= x.z, s[n][4 * w + 3] *= x.w;
+        }
+      p[2 * n] = pack_step<PT>(s[n], 0), p[2 * n + 1] = pack_step<PT>(s[n], 1);
+      if constexpr (kTwice<DT, F8>) {
+        const f32x16 rest = left_of(s[n]);
+        p2[2 * n] = pack_step<PT>(rest, 0), p2[2 * n + 1] = pack_step<PT>(rest, 1);
+      }
     }
     sums.l += l[0] + l[1];
-    u32x4 p[2] = {pack_step<PT>(s[0], 0), pack_step<PT>(s[0], 1)}, p2[2];
-    if constexpr (kTwice<DT, F8>) {
-      const f32x16 rest = left_of(s[0]);
-      p2[0] = pack_step<PT>(rest, 0), p2[1] = pack_step<PT>(rest, 1);
-    }
     in_order();
-    wait(more ? kLoadsK : 0);
+    wait(more);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
       for (int o = 0; o < T::kOut; ++o) {
         u32x4 x;
@@ -587,7 +593,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
       }
     wait_lds();
     in_order();
-    if (more) load(a.v, my_v);
+    if (more) load_values();
     in_order();
     ok = ok_next;
     if (more) find(i + 2, page);
@@ -893,26 +899,28 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
       reinterpret_cast<u32x4*>(a.out)[i < front ? i : i - front + s.none_to * row] = u32x4{0u, 0u, 0u, 0u};
   }
   Part part = {};
-  int64_t left = s.size, x = s.x;
-  int t = s.tile;
+  int left = s.size, x = s.x, t = s.tile;
   Segment g;
   g.r = s.r, g.q = s.q, g.head = s.head;
   while (left > 0) {
-    const Ramp p = s.few ? Ramp{g.q.length + kStartFew, 0, 1} : ramp(a, g.q);
+    const Ramp items = ramp(a, g.q, s.few);
     for (; left > 0 && g.head < a.n_kv; ++g.head, t = 0)
-      for (; left > 0 && t < p.tiles; ++t, x = 0) {
-        const int64_t of_item = p.of(t), take = of_item - x < left ? of_item - x : left;
+      for (; left > 0 && t < items.tiles; ++t, x = 0) {
+        const int of_item = items.of(t), take = min(of_item - x, left);
         if (take <= 0) continue;  // (a share that begins at an item's end)
-        const int start = s.few ? kStartFew : kStartMany;
-        g.row0 = s.few ? 0 : t * kTileRows;
-        g.rows = min(g.q.rows - g.row0, kTileRows);
-        const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1);
-        auto cut = [&](int64_t at) { return at >= of_item ? seen : static_cast<int>(min(static_cast<int64_t>(seen), max(at - start, static_cast<int64_t>(0)) / kCut * kCut)); };
-        g.lo = uniform(cut(x)), g.hi = uniform(cut(x + take));
+        g.row0 = t * (s.few ? kFewRows : kManyRows);
+        g.rows = min(g.q.rows - g.row0, s.few ? kFewRows : kManyRows);
+        const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1), start = start_of(a, s.few);
+        auto cut = [&](int at) {
+          if (at >= of_item) return seen;
+          const int64_t key = static_cast<int64_t>(max(at - start, 0)) << a.shift;
+          return key < seen ? static_cast<int>(key) / kCut * kCut : seen;
+        };
+        g.lo = cut(x), g.hi = cut(x + take);
         g.whole = take == of_item;
         g.slot = 2 * s.id + (x == 0);
         if (x == 0 && take < of_item) {  // (the shares' ends behind this one that are inside of the item and not near its end)
-          part.parts = 2 + static_cast<int>(static_cast<double>(of_item - s.snap - take) / static_cast<double>(s.each));
+          part.parts = 2 + (of_item - s.snap - take) / s.each;
           part.head = g.head, part.first = g.q.first, part.row0 = g.row0, part.rows = g.rows;
         }
         if (s.few) few_rows<DT, D, F8>(a, g);
@@ -991,7 +999,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 }
 
 int shares() { return std::max(8, 2 * device_cu_count() / 8 * 8); }
-int part_rows(int64_t tokens, int group) { return static_cast<int>(std::min<int64_t>(kTileRows, tokens * group)); }
+int part_rows(int64_t tokens, int group) { return static_cast<int>(std::min<int64_t>(kManyRows, tokens * group)); }
 
 template <int DT, int D, bool F8>
 int launch(PagedArgs& a, hipStream_t s) {
@@ -1058,6 +1066,11 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   a.seq = static_cast<int>(seq), a.width = num_pages ? static_cast<int>(pages_per_request) : 0, a.page_size = page_size, a.n_pages = static_cast<int>(num_pages);
   a.by_seq = Divider(static_cast<uint32_t>(seq)), a.by_page = Divider(page_size), a.by_group = Divider(group);
   a.c = scale * kLog2e;
+  const int64_t tiles = n_kv_heads * (static_cast<int64_t>(a.tokens) * group / kFewRows + requests);
+  const int64_t keys = std::max<int64_t>(static_cast<int64_t>(a.width) * page_size, a.tokens) + 2 * kManyRows;
+  for (a.shift = 0; a.shift < 30 && tiles * ((keys >> a.shift) + kStartFew + kStartMany) > 0x3fffffff; ++a.shift) {
+  }
+  if (a.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
   a.shares = shares(), a.part_rows = part_rows(a.tokens, group);
   const int64_t rows = 2ll * a.shares * a.part_rows;
   a.sums = static_cast<float*>(workspace);
