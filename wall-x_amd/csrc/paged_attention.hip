@@ -461,12 +461,17 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
     }
   }
   const int all_see = wave_extreme<false>(row.seen);  // every row sees the keys before
+  wait_loads();  // (queries and pages: what waits for them later would wait for the keys as well)
   uint32_t src[kLoads], scale_row = 0;
   uint64_t ok_next = 0;
-  auto find = [&](int i, int page) {  // rows of tile i: of this lane's pieces, and of its scales
+  auto find = [&](int i, int page) {
     const int key = key0(i) + in_tile;
-    const KeyRow k = row_of(a, g, min(key, g.hi - 1), page);
-    ok_next = __ballot(k.ok && key < g.hi);
+    KeyRow k = row_of(a, g, min(key, g.hi - 1), page);
+    k.ok = k.ok && key < g.hi;
+    return k;
+  };
+  auto take = [&](const KeyRow& k) {  // rows of a tile: of this lane's pieces, and of its scales
+    ok_next = __ballot(k.ok);
     scale_row = k.row;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) src[u] = __shfl(k.row, (u * 64 + lane) / kChunks);
@@ -497,12 +502,13 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
   uint64_t ok = 0;
   int page = 0;
   if (mine > 0) {
-    find(0, p0);
+    take(find(0, p0));
+    const KeyRow next = find(1, p1);
     load(a.k, my_k);
+    page = ask(2);
     load_values();
     ok = ok_next;
-    find(1, p1);
-    page = ask(2);
+    take(next);
   }
   const int rows_at = rows_base<D>(lane), cols_at = cols_base<D>(lane);
   // e4m3: bytes 8 (lane & 1) of chunk 2 o + (lane / 16 & 1), of the row that the transposing read wants of this lane
@@ -512,24 +518,40 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
     const bool more = i + 1 < mine;
     wait(true);  // keys and scales are there, values may be on their way
     f32x16 s[NT] = {};
-    if constexpr (F8) {
+    if constexpr (F8) {  // operands are asked for a few products ahead
+      constexpr int kReads = NT * (T::kSteps / 2), kAhead = 4;
+      auto read = [&](int j) { return *reinterpret_cast<const u32x4*>(my_k + R::at(32 * (j % NT) + (lane & 31), 2 * (j / NT) + h)); };
+      u32x4 f[kAhead];
 #pragma unroll
-      for (int u = 0; u < T::kSteps / 2; ++u)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(my_k + R::at(32 * n + (lane & 31), 2 * u + h));
-          s[n] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[2 * u], s[n]);
-          s[n] = mfma<DT>(widen8<DT>(x[2], x[3]), qf[2 * u + 1], s[n]);
-        }
+      for (int j = 0; j < kAhead && j < kReads; ++j) f[j] = read(j);
+      u32x2 odd[NT];
       if constexpr (T::kSteps % 2 != 0)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(my_k + R::at(32 * n + (lane & 31), T::kSteps - 1) + 8 * h);
-          s[n] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[T::kSteps - 1], s[n]);
-        }
-    } else {
+        for (int n = 0; n < NT; ++n) odd[n] = *reinterpret_cast<const u32x2*>(my_k + R::at(32 * n + (lane & 31), T::kSteps - 1) + 8 * h);
+      in_order();
 #pragma unroll
-      for (int t = 0; t < T::kSteps; ++t) s[0] = mfma<DT>(read_rows<D>(my_k, 0, t, rows_at), qf[t], s[0]);
+      for (int j = 0; j < kReads; ++j) {
+        const u32x4 x = f[j % kAhead];
+        s[j % NT] = mfma<DT>(widen8<DT>(x[0], x[1]), qf[2 * (j / NT)], s[j % NT]);
+        s[j % NT] = mfma<DT>(widen8<DT>(x[2], x[3]), qf[2 * (j / NT) + 1], s[j % NT]);
+        if (j + kAhead < kReads) f[j % kAhead] = read(j + kAhead);
+        in_order();
+      }
+      if constexpr (T::kSteps % 2 != 0)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n] = mfma<DT>(widen8<DT>(odd[n][0], odd[n][1]), qf[T::kSteps - 1], s[n]);
+    } else {
+      constexpr int kAhead = 4;
+      u32x4 f[kAhead];
+#pragma unroll
+      for (int t = 0; t < kAhead; ++t) f[t] = read_rows<D>(my_k, 0, t, rows_at);
+      in_order();
+#pragma unroll
+      for (int t = 0; t < T::kSteps; ++t) {
+        s[0] = mfma<DT>(f[t % kAhead], qf[t], s[0]);
+        if (t + kAhead < T::kSteps) f[t % kAhead] = read_rows<D>(my_k, 0, t + kAhead, rows_at);
+        in_order();
+      }
     }
     wait_lds();  // (the slot is read before it is filled again)
     in_order();
@@ -573,31 +595,46 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
     sums.l += l[0] + l[1];
     in_order();
     wait(more);
-#pragma unroll
-    for (int t = 0; t < 2 * NT; ++t)
-#pragma unroll
-      for (int o = 0; o < T::kOut; ++o) {
-        u32x4 x;
+    {
+      constexpr int kReads = 2 * NT * T::kOut, kAhead = F8 ? 6 : 4;
+      using Read = std::conditional_t<F8, u32x2, u32x4>;
+      auto read = [&](int j) -> Read {
+        const int t = j / T::kOut, o = j % T::kOut;
         if constexpr (F8) {
           typedef int i32x2 __attribute__((ext_vector_type(2)));
           typedef __attribute__((address_space(3))) i32x2* P;
           int chunk = 2 * o + ((lane >> 4) & 1);
           if (R::kChunks % 2 != 0) chunk = min(chunk, R::kChunks - 1);  // (channels past the last: read, not used)
-          const i32x2 y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((P)(my_v + R::at(16 * t + raw_row, chunk) + 8 * (lane & 1)));
-          x = widen8<PT>(static_cast<uint32_t>(y[0]), static_cast<uint32_t>(y[1]));
+          return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((P)(my_v + R::at(16 * t + raw_row, chunk) + 8 * (lane & 1))));
         } else {
-          x = read_cols<D>(my_v, 0, t, o, cols_at);
+          return read_cols<D>(my_v, 0, t, o, cols_at);
         }
+      };
+      Read f[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) f[j] = read(j);
+      in_order();
+#pragma unroll
+      for (int j = 0; j < kReads; ++j) {
+        const int t = j / T::kOut, o = j % T::kOut;
+        u32x4 x;
+        if constexpr (F8) x = widen8<PT>(f[j % kAhead][0], f[j % kAhead][1]);
+        else x = f[j % kAhead];
         sums.acc[o] = mfma<PT>(x, p[t], sums.acc[o]);
         if constexpr (kTwice<DT, F8>) sums.acc[o] = mfma<PT>(x, p2[t], sums.acc[o]);
+        if (j + kAhead < kReads) f[j % kAhead] = read(j + kAhead);
+        in_order();
       }
+    }
     wait_lds();
+    in_order();
+    const KeyRow next = find(i + 2, page);
+    page = ask(i + 3);
     in_order();
     if (more) load_values();
     in_order();
     ok = ok_next;
-    if (more) find(i + 2, page);
-    page = ask(i + 3);
+    take(next);
   }
   // ---- the wavefronts' sums together: each leaves its own where its slots were, 64 channels a row in either array, and 16 lanes (8 of 64
   // channels) finish a row.
@@ -685,6 +722,11 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));  // (see few_rows)
   const int lane = tid & 63, rw = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int tiles = (g.hi - g.lo + KB - 1) / KB;
+  auto ask = [&](int i) { return page_of(a, g, min(g.lo + i * KB + lane, g.hi - 1)); };  // a lane finds the row of one of a tile's 64 keys
+  int p0 = 0, p1 = 0;
+  if (tiles > 0) p0 = ask(0), p1 = ask(1);
+  in_order();
   const Row row = row_at(a, g, rw * 32 + (lane & 31));
   u32x4 qf[T::kSteps];
   {
@@ -694,17 +736,19 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
   }
   const bool wave_live = rw * 32 < g.rows;
   const int all_see = wave_extreme<false>(row.seen), some_sees = wave_live ? wave_extreme<true>(row.live ? row.seen : 0) : 0;
-  const int tiles = (g.hi - g.lo + KB - 1) / KB;
-  // a lane finds the row of one of a tile's 64 keys
-  auto ask = [&](int i) { return page_of(a, g, min(g.lo + i * KB + lane, g.hi - 1)); };
+  wait_loads();  // (queries and pages, see few_rows)
   constexpr int kChunk = D / 16, kPieces = (KB * kChunk + 255) / 256;  // e4m3: 16-byte pieces of a row, of a thread
   constexpr int kLoads = T::kChunks / 4;                               // otherwise: 16 rows by a wavefront
   uint32_t src[F8 ? kPieces : kLoads], scale_row = 0;
   uint64_t ok_next = 0;
   auto find = [&](int i, int page) {
     const int key = g.lo + i * KB + lane;
-    const KeyRow k = row_of(a, g, min(key, g.hi - 1), page);
-    ok_next = __ballot(k.ok && key < g.hi);
+    KeyRow k = row_of(a, g, min(key, g.hi - 1), page);
+    k.ok = k.ok && key < g.hi;
+    return k;
+  };
+  auto take = [&](const KeyRow& k) {
+    ok_next = __ballot(k.ok);
     scale_row = k.row;
     if constexpr (F8) {
 #pragma unroll
@@ -840,29 +884,33 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
   uint64_t ok = 0;
   int page = 0;
   if (tiles > 0) {
-    const int p0 = ask(0), p1 = ask(1);
-    find(0, p0);
+    take(find(0, p0));
+    const KeyRow next = find(1, p1);
     fetch(lds0);
-    ok = ok_next;
-    find(1, p1);
     page = ask(2);
+    ok = ok_next;
+    take(next);
   }
   auto turn = [&](int i, unsigned char* slot, unsigned char* other) {
     const int k0 = g.lo + i * KB;
     const uint64_t seen = ok;
+    KeyRow next;
     if constexpr (F8) {
       put(slot);
+      next = find(i + 2, page);
       if (i + 1 < tiles) fetch(other);
+      page = ask(i + 3);
       wait_lds();
       attn_barrier();
     } else {
       wait_loads();
+      next = find(i + 2, page);
       attn_barrier();
       if (i + 1 < tiles) fetch(other);
+      page = ask(i + 3);
     }
     ok = ok_next;
-    if (i + 2 < tiles) find(i + 2, page);
-    page = ask(i + 3);
+    take(next);
     in_order();
     if (k0 < some_sees) step(slot, k0, seen);
   };
