@@ -29,8 +29,7 @@ struct Part {  // of the item that begins in a share and ends in a later one
   int head;    // key / value head
   int first;   // the request's first token
   int row0, rows;
-  int pad[3];
-};
+};  // (no arrays in it: they are put into LDS, at an address made from the dispatch packet, which lies in host memory: 12 us)
 
 struct PagedArgs {
   const uint16_t* q;               // [batch, n_q, seq, D] through strides; token t is position t % seq of row t / seq
@@ -304,7 +303,9 @@ template <int DT, int D, bool F8>
 __device__ __forceinline__ void rows_again(const PagedArgs& a, const Segment& g, int first, uint32_t again, float m, float l) {
   using T = AttnTile<D>;
   constexpr int PT = kValues<DT, F8>;
-  const int lane = threadIdx.x & 63, h = lane >> 5;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (see few_rows)
+  const int h = lane >> 5;
   const Row w = row_at(a, g, first + (lane & 31));
   const bool redo = again >> (lane & 31) & 1;
   const float mc = m == -kInf ? 0.f : m * a.c;
