@@ -20,9 +20,9 @@ namespace {
 
 constexpr int kFewRows = 64, kManyRows = 128;  // rows of an item of either kind
 constexpr int kCut = 64;          // items are cut at multiples of so many keys
-constexpr int kStartFew = 64, kStartMany = 64;  // an item's start, in keys
+constexpr int kStartFew = 192, kStartMany = 128;  // an item's start, in keys
 constexpr int kLeastFew = 256, kLeastMany = 256;  // the least that a workgroup takes
-constexpr int kSnap = 8;          // an end of an item nearer than an eighth of a share is the share's end
+constexpr int kSnapFew = 256, kSnapMany = 192;  // an item's end nearer than this to a share's end (and than 3/8 of a share) is the share's end
 
 struct Part {  // of the item that begins in a share and ends in a later one
   int parts;   // 0: there is none
@@ -187,7 +187,7 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   s.id = s.few ? w : 8 * p + w;
   const int total = s.few ? all[0] : all[1];
   s.each = uniform(max(total / count + 1, (s.few ? kLeastFew : kLeastMany) >> a.shift));
-  s.snap = s.each / kSnap;
+  s.snap = min(s.each / 8 * 3, (s.few ? kSnapFew : kSnapMany) >> a.shift);
   const int64_t at = static_cast<int64_t>(w) * s.each, end = at + s.each;
   s.size = at < total ? static_cast<int>((total < end ? total : end) - at) : 0;
   const int from = s.few ? before[0] : before[1], to = from + (s.few ? mine[0] : mine[1]);
@@ -984,8 +984,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
   if (threadIdx.x == 0) a.part[s.id] = part;
 }
 
-// Joins the parts of the item that begins in share blockIdx.x and ends in a later one: of few parts a wavefront to a row, of many a workgroup,
-// a quarter of them to a wavefront.  Lane l has channels 2 l and 2 l + 1.
+// Joins the parts of the item that begins in share blockIdx.x and ends in a later one.  Of up to kJoinInWave parts 16 lanes have a row, 8
+// channels each, and 8 parts are on their way at a time; of more a workgroup has a row, a quarter of the parts to a wavefront, lane l channels 2 l
+// and 2 l + 1.
+constexpr int kJoinInWave = 16, kJoinBlocks = 8;
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   __shared__ float s_top[4], s_sum[4];
@@ -993,27 +995,61 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const int id = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Part p = uniform(a.part[id]);
   if (p.parts == 0) return;
-  const bool split = p.parts > 8;  // (uniform over the workgroup)
-  const int each = split ? (p.parts + 3) / 4 : p.parts, first = split ? min(wave * each, p.parts) : 0, last = min(first + each, p.parts);
-  const int rows_at_once = (split ? 1 : 4) * gridDim.y;
-  for (int row0 = blockIdx.y * (split ? 1 : 4); row0 < p.rows; row0 += rows_at_once) {
-    const int row = split ? row0 : row0 + wave;
-    if (!split && row >= p.rows) continue;
-    auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * id + 1 : 2 * (id + i)) * a.part_rows + row; };
-    float top = -kInf, l = 0.f;
-    for (int i = first + lane; i < last; i += 64) top = fmaxf(top, a.stats[slot(i)].x);
-    top = wave_max(top);
-    if (split) {
-      if (lane == 0) s_top[wave] = top;
-      __syncthreads();
-      top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  auto slot = [&](int i, int row) { return static_cast<int64_t>(i == 0 ? 2 * id + 1 : 2 * (id + i)) * a.part_rows + row; };
+  auto result = [&](int row) {
+    const int at = p.row0 + row, i = a.by_group.div(at), hq = p.head * a.group + at - i * a.group;
+    return a.out + (static_cast<int64_t>(p.first + i) * a.n_q + hq) * D;
+  };
+  // (a part that the row sees nothing of has the weight 0 and counts nothing, unless its scores were NaN)
+  auto weight = [&](float2 st, float top) { return st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c); };
+  auto share_of = [](float2 st, float w) { return st.x == -kInf ? 0.f * st.y : st.y * w; };
+  if (p.parts <= kJoinInWave) {
+    const int row = (blockIdx.y * 4 + wave) * 4 + (lane >> 4), c = lane & 15;
+    if (row >= p.rows || 8 * c >= D) return;
+    float2 st[kJoinInWave];
+    float top = -kInf, l = 0.f, o[8] = {};
+#pragma unroll
+    for (int i = 0; i < kJoinInWave; ++i) st[i] = i < p.parts ? a.stats[slot(i, row)] : float2{-kInf, 0.f};
+#pragma unroll
+    for (int i0 = 0; i0 < kJoinInWave; i0 += 8) {
+      if (i0 >= p.parts) break;
+      float4 x[8], y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float4* from = reinterpret_cast<const float4*>(a.sums + slot(min(i0 + u, p.parts - 1), row) * D + 8 * c);
+        x[u] = from[0], y[u] = from[1];
+      }
+      if (i0 == 0)
+#pragma unroll
+        for (int i = 0; i < kJoinInWave; ++i) top = fmaxf(top, st[i].x);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = weight(st[i0 + u], top);
+        l += share_of(st[i0 + u], w);
+        if (w == 0.f) continue;
+        o[0] += x[u].x * w, o[1] += x[u].y * w, o[2] += x[u].z * w, o[3] += x[u].w * w;
+        o[4] += y[u].x * w, o[5] += y[u].y * w, o[6] += y[u].z * w, o[7] += y[u].w * w;
+      }
     }
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
+    *reinterpret_cast<u32x4*>(result(row) + 8 * c) = pack16<DT>(o);
+    return;
+  }
+  const int each = (p.parts + 3) / 4, first = min(wave * each, p.parts), last = min(first + each, p.parts);
+  for (int row = blockIdx.y; row < p.rows; row += kJoinBlocks) {
+    float top = -kInf, l = 0.f;
+    for (int i = first + lane; i < last; i += 64) top = fmaxf(top, a.stats[slot(i, row)].x);
+    top = wave_max(top);
+    if (lane == 0) s_top[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
     float2 o = {0.f, 0.f};
     for (int i0 = first; i0 < last; i0 += 64) {
-      const float2 st = i0 + lane < last ? a.stats[slot(i0 + lane)] : float2{-kInf, 0.f};
-      // (a part that the row sees nothing of counts nothing, unless its scores were NaN)
-      const float f = st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c);
-      l += st.x == -kInf ? 0.f * st.y : st.y * f;
+      const float2 st = i0 + lane < last ? a.stats[slot(i0 + lane, row)] : float2{-kInf, 0.f};
+      const float f = weight(st, top);
+      l += share_of(st, f);
       const int n = min(64, last - i0);
       for (int i = 0; i < n; i += 8) {
         float2 y[8];
@@ -1022,7 +1058,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
         for (int u = 0; u < 8; ++u) {  // (past the last: the last one's, without weight)
           const int at = min(i + u, n - 1);
           w[u] = i + u < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), at)) : 0.f;
-          y[u] = 2 * lane < D ? reinterpret_cast<const float2*>(a.sums + slot(i0 + at) * D)[lane] : float2{0.f, 0.f};
+          y[u] = 2 * lane < D ? reinterpret_cast<const float2*>(a.sums + slot(i0 + at, row) * D)[lane] : float2{0.f, 0.f};
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
@@ -1032,18 +1068,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
       }
     }
     l = wave_sum(l);
-    if (split) {
-      if (lane == 0) s_sum[wave] = l;
-      s_out[wave][lane] = o;
-      __syncthreads();
-      l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-      o.x = (s_out[0][lane].x + s_out[1][lane].x) + (s_out[2][lane].x + s_out[3][lane].x);
-      o.y = (s_out[0][lane].y + s_out[1][lane].y) + (s_out[2][lane].y + s_out[3][lane].y);
-    }
-    const int at = p.row0 + row, i = a.by_group.div(at), hq = p.head * a.group + at - i * a.group;
-    if (2 * lane < D && (!split || wave == 0))
-      reinterpret_cast<uint32_t*>(a.out + (static_cast<int64_t>(p.first + i) * a.n_q + hq) * D)[lane] = l == 0.f ? 0u : pack2<DT>(o.x / l, o.y / l);
-    if (split) __syncthreads();
+    if (lane == 0) s_sum[wave] = l;
+    s_out[wave][lane] = o;
+    __syncthreads();
+    l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    o.x = (s_out[0][lane].x + s_out[1][lane].x) + (s_out[2][lane].x + s_out[3][lane].x);
+    o.y = (s_out[0][lane].y + s_out[1][lane].y) + (s_out[2][lane].y + s_out[3][lane].y);
+    if (2 * lane < D && wave == 0) reinterpret_cast<uint32_t*>(result(row))[lane] = l == 0.f ? 0u : pack2<DT>(o.x / l, o.y / l);
+    __syncthreads();
   }
 }
 
@@ -1054,7 +1086,7 @@ template <int DT, int D, bool F8>
 int launch(PagedArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((paged_attn_kernel<DT, D, F8>), dim3(static_cast<unsigned>(a.shares)), dim3(256), 0, s, a);
   if (int rc = check_launch("paged_attn_kernel")) return rc;
-  hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3(static_cast<unsigned>(a.shares), 8), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3(static_cast<unsigned>(a.shares), kJoinBlocks), dim3(256), 0, s, a);
   return check_launch("paged_join_kernel");
 }
 template <int DT, bool F8>
