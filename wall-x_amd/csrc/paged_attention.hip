@@ -22,7 +22,9 @@ constexpr int kFewRows = 64, kManyRows = 128;  // rows of an item of either kind
 constexpr int kCut = 64;          // items are cut at multiples of so many keys
 constexpr int kStartFew = 192, kStartMany = 128;  // an item's start, in keys
 constexpr int kLeastFew = 256, kLeastMany = 256;  // the least that a workgroup takes
-constexpr int kSnapFew = 256, kSnapMany = 192;  // an item's end nearer than this to a share's end (and than 3/8 of a share) is the share's end
+// An end of an item near to a share's end is the share's end: nearer than this in keys, which is about what a cut costs (a start, a part, its
+// join), and than 3/8 of a share.  Items of up to half a share are not cut at all.
+constexpr int kSnap = 128;
 
 struct Part {  // of the item that begins in a share and ends in a later one
   int parts;   // 0: there is none
@@ -116,7 +118,6 @@ __device__ __forceinline__ int wave_prefix(int x) {  // inclusive, over the wave
 struct Share {
   int few, id;     // id: unique over both kinds
   int size, each;  // each: what a share of this kind takes
-  int snap;        // an item's end nearer than this to a share's end is the share's end
   int r, head, tile, x;
   Request q;
   int none_from, none_to;  // tokens [0, none_from) and [none_to, all) are no request's
@@ -125,7 +126,11 @@ struct Share {
 struct Place {
   int head, tile, x;
 };
-__device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, bool few, int at, int snap, Place& p) {
+__device__ __forceinline__ int snap_of(const PagedArgs& a, int of_item, int each) {
+  const int most = each / 8 * 3;
+  return 2 * of_item <= each ? most : min(most, kSnap >> a.shift);
+}
+__device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, bool few, int at, int each, Place& p) {
   const Ramp items = ramp(a, q, few);
   const int of_head = items.before(items.tiles);
   p.head = at / of_head;
@@ -138,7 +143,7 @@ __device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, bool
   }
   p.tile = lo;
   p.x -= items.before(lo);
-  const int of_item = items.of(lo), to = p.x < snap ? 0 : (of_item - p.x < snap ? of_item : p.x), moved = to - p.x;
+  const int of_item = items.of(lo), snap = snap_of(a, of_item, each), to = p.x < snap ? 0 : (of_item - p.x < snap ? of_item : p.x), moved = to - p.x;
   p.x = to;
   return moved;
 }
@@ -187,7 +192,6 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   s.id = s.few ? w : 8 * p + w;
   const int total = s.few ? all[0] : all[1];
   s.each = uniform(max(total / count + 1, (s.few ? kLeastFew : kLeastMany) >> a.shift));
-  s.snap = min(s.each / 8 * 3, (s.few ? kSnapFew : kSnapMany) >> a.shift);
   const int64_t at = static_cast<int64_t>(w) * s.each, end = at + s.each;
   s.size = at < total ? static_cast<int>((total < end ? total : end) - at) : 0;
   const int from = s.few ? before[0] : before[1], to = from + (s.few ? mine[0] : mine[1]);
@@ -198,10 +202,10 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
       const int m = measure(a, q, s.few) * a.n_kv;
       Place place;
       if (r_from <= at && at < r_from + m) {
-        s_moved[0] = locate(a, q, s.few, static_cast<int>(at) - r_from, s.snap, place);
+        s_moved[0] = locate(a, q, s.few, static_cast<int>(at) - r_from, s.each, place);
         s_place = place, s_q = q, s_r = r;
       }
-      if (r_from <= end && end < r_from + m) s_moved[1] = locate(a, q, s.few, static_cast<int>(end) - r_from, s.snap, place);
+      if (r_from <= end && end < r_from + m) s_moved[1] = locate(a, q, s.few, static_cast<int>(end) - r_from, s.each, place);
       r_from += m;
     }
   }
@@ -820,12 +824,14 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
     in_order();
+    __builtin_amdgcn_s_setprio(1);  // (products go before the other wavefront's powers: 341 -> 331 us for 2048 tokens over 16384 keys)
 #pragma unroll
     for (int i = 0; i < kScores; ++i) {
       s[i % NT] = mfma<DT>(f[i % kAhead], qf[i / NT], s[i % NT]);
       if (i + kAhead < kScores) f[i % kAhead] = read_k(i + kAhead);
       in_order();
     }
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) f[i] = read_v(i);
     in_order();
@@ -866,6 +872,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
     };
     pack(0);
     in_order();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < kProducts; ++i) {
       const int n = i / (2 * T::kOut), t = i / T::kOut % 2, o = i % T::kOut, at = i % (2 * T::kOut);
@@ -880,6 +887,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
       }
       in_order();
     }
+    __builtin_amdgcn_s_setprio(0);
     sums.l += l[0] + l[1];
   };
   uint64_t ok = 0;
@@ -969,7 +977,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         g.whole = take == of_item;
         g.slot = 2 * s.id + (x == 0);
         if (x == 0 && take < of_item) {  // (the shares' ends behind this one that are inside of the item and not near its end)
-          part.parts = 2 + (of_item - s.snap - take) / s.each;
+          part.parts = 2 + (of_item - snap_of(a, of_item, s.each) - take) / s.each;
           part.head = g.head, part.first = g.q.first, part.row0 = g.row0, part.rows = g.rows;
         }
         if (s.few) few_rows<DT, D, F8>(a, g);
