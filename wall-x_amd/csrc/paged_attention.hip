@@ -21,7 +21,8 @@ namespace {
 constexpr int kFewRows = 64, kManyRows = 128;  // rows of an item of either kind
 constexpr int kCut = 64;          // items are cut at multiples of so many keys
 constexpr int kStartFew = 192, kStartMany = 128;  // an item's start, in keys
-constexpr int kLeastFew = 256, kLeastMany = 256;  // the least that a workgroup takes
+constexpr int kLeast = 256;       // the least that a workgroup takes
+constexpr int kShort = 2048;      // (see share)
 // An end of an item near to a share's end is the share's end: nearer than this in keys, which is about what a cut costs (a start, a part, its
 // join), and than 3/8 of a share.  Items of up to half a share are not cut at all.
 constexpr int kSnap = 128;
@@ -71,7 +72,8 @@ __device__ __forceinline__ Request request(const PagedArgs& a, int r) {
 __device__ __forceinline__ int keys_seen(const PagedArgs& a, const Request& q, int row) {
   return a.causal ? min(max(q.length - q.n + a.by_group.div(row) + 1, 0), q.length) : q.length;
 }
-__device__ __forceinline__ bool is_few(const PagedArgs& a, const Request& q) { return q.rows <= kFewRows; }
+// Which requests: those of few rows, those of many, or all of them in tiles of few rows.
+enum Kind { kFew, kMany, kAllFew };
 // The items of one head of a request: tile t's measure is base + step (t + 1), which follows the diagonal.
 struct Ramp {
   int base, step, tiles;
@@ -85,9 +87,9 @@ __device__ __forceinline__ Ramp ramp(const PagedArgs& a, const Request& q, bool 
   return {((step ? max(q.length - q.n, 0) : q.length) >> a.shift) + start_of(a, few), step, tiles};
 }
 // measure of one head of a request
-__device__ __forceinline__ int measure(const PagedArgs& a, const Request& q, bool few) {
-  if (q.n == 0 || is_few(a, q) != few) return 0;
-  const Ramp p = ramp(a, q, few);
+__device__ __forceinline__ int measure(const PagedArgs& a, const Request& q, int kind) {
+  if (q.n == 0 || (kind != kAllFew && (q.rows <= kFewRows) != (kind == kFew))) return 0;
+  const Ramp p = ramp(a, q, kind != kMany);
   return p.before(p.tiles);
 }
 
@@ -114,9 +116,10 @@ __device__ __forceinline__ int wave_prefix(int x) {  // inclusive, over the wave
   return x;
 }
 
-// A workgroup's share: `size` of its kind's measures, from `x` into tile `tile` of `head` of request r.
+// A workgroup's share: `size` of its kind's measures, from `x` into tile `tile` of `head` of request r; or part x of that item.
 struct Share {
-  int few, id;     // id: unique over both kinds
+  int kind, id;    // id: unique over all kinds
+  int parts;       // not 0: every item is cut in so many parts, a share each
   int size, each;  // each: what a share of this kind takes
   int r, head, tile, x;
   Request q;
@@ -130,8 +133,8 @@ __device__ __forceinline__ int snap_of(const PagedArgs& a, int of_item, int each
   const int most = each / 8 * 3;
   return 2 * of_item <= each ? most : min(most, kSnap >> a.shift);
 }
-__device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, bool few, int at, int each, Place& p) {
-  const Ramp items = ramp(a, q, few);
+__device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, int kind, int at, int each, Place& p) {
+  const Ramp items = ramp(a, q, kind != kMany);
   const int of_head = items.before(items.tiles);
   p.head = at / of_head;
   p.x = at - p.head * of_head;
@@ -148,82 +151,114 @@ __device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, bool
   return moved;
 }
 __device__ __forceinline__ Share share(const PagedArgs& a) {
-  __shared__ int s_sums[4][2], s_moved[2];
+  enum { kSums = 4 };  // measures of each Kind, number of items of few rows
+  __shared__ int s_sums[4][kSums], s_longest[4], s_moved[2];
   __shared__ Place s_place;
   __shared__ Request s_q;
   __shared__ int s_r, s_none[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (a.requests + 255) / 256;
   const int first = min(tid * each, a.requests), last = min(first + each, a.requests);
-  int mine[2] = {0, 0}, sum[2];
+  int mine[kSums] = {}, sum[kSums], longest = 0;
   if (tid == 0) s_none[0] = a.requests ? 0 : a.tokens, s_none[1] = a.tokens, s_moved[0] = 0, s_moved[1] = 0;
+  auto items_of = [&](const Request& q) { return (q.rows + kFewRows - 1) / kFewRows * a.n_kv; };
   Request q = {};
   for (int r = first; r < last; ++r) {
     q = request(a, r);
-    const bool few = is_few(a, q);
-    const int m = measure(a, q, few) * a.n_kv;
-    mine[0] += few ? m : 0;
-    mine[1] += few ? 0 : m;
+    const int m = measure(a, q, kAllFew) * a.n_kv;
+    const bool few = q.rows <= kFewRows;
+    mine[kFew] += few ? m : 0;
+    mine[kMany] += few ? 0 : measure(a, q, kMany) * a.n_kv;
+    mine[kAllFew] += m;
+    mine[3] += items_of(q);
+    longest = max(longest, q.n == 0 ? 0 : q.length);
     if (r == 0) s_none[0] = q.first;
     if (r == a.requests - 1) s_none[1] = q.first + q.n;
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < kSums; ++i) {
     sum[i] = wave_prefix(mine[i]);
     if (lane == 63) s_sums[wave][i] = sum[i];
   }
+  longest = max(wave_extreme<true>(longest), __builtin_amdgcn_readlane(wave_extreme<true>(__shfl_xor(longest, 32)), 0));
+  if (lane == 0) s_longest[wave] = longest;
   __syncthreads();
-  int all[2], before[2];
+  int all[kSums], before[kSums];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < kSums; ++i) {
     const int w0 = s_sums[0][i], w1 = s_sums[1][i], w2 = s_sums[2][i];
     before[i] = sum[i] - mine[i] + (wave > 0 ? w0 : 0) + (wave > 1 ? w1 : 0) + (wave > 2 ? w2 : 0);
     all[i] = uniform(w0 + w1 + w2 + s_sums[3][i]);
   }
+  longest = uniform(max(max(s_longest[0], s_longest[1]), max(s_longest[2], s_longest[3])));
+  // Tiles of few rows for all where they give every workgroup one item at most and the keys are few: 64 x 32 queries over 800 to 912 keys 51 us
+  // in two parts for each tile of many rows.
+  const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, per_xcd = a.shares / 8;
+  const bool all_few = all[kMany] == 0 || (all[3] <= a.shares && longest <= kShort);
+  Share s = {};
   // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
-  const int per_xcd = a.shares / 8, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
-  int p = all[1] == 0 ? per_xcd : 0;
-  if (all[0] != 0 && all[1] != 0) {
-    const float part = static_cast<float>(all[0]) / (static_cast<float>(all[0]) + static_cast<float>(all[1]));
+  int p = all_few ? per_xcd : 0;
+  if (!all_few && all[kFew] != 0) {
+    const float part = static_cast<float>(all[kFew]) / (static_cast<float>(all[kFew]) + static_cast<float>(all[kMany]));
     p = uniform(min(max(static_cast<int>(part * per_xcd + 0.5f), 1), per_xcd - 1));
   }
-  Share s = {};
-  s.few = j < p;
-  const int count = s.few ? 8 * p : 8 * (per_xcd - p), w = s.few ? xcd * p + j : xcd * (per_xcd - p) + j - p;
-  s.id = s.few ? w : 8 * p + w;
-  const int total = s.few ? all[0] : all[1];
-  s.each = uniform(max(total / count + 1, (s.few ? kLeastFew : kLeastMany) >> a.shift));
-  const int64_t at = static_cast<int64_t>(w) * s.each, end = at + s.each;
-  s.size = at < total ? static_cast<int>((total < end ? total : end) - at) : 0;
-  const int from = s.few ? before[0] : before[1], to = from + (s.few ? mine[0] : mine[1]);
+  s.kind = all_few ? kAllFew : (j < p ? kFew : kMany);
+  const int count = j < p ? 8 * p : 8 * (per_xcd - p), w = j < p ? xcd * p + j : xcd * (per_xcd - p) + j - p;
+  s.id = j < p ? w : 8 * p + w;
+  const int total = all_few ? all[kAllFew] : (j < p ? all[kFew] : all[kMany]);
+  s.each = uniform(max(total / count + 1, kLeast >> a.shift));
+  // Items of about one length, no more than there are workgroups: a like number of workgroups to each, without second items, where the longest
+  // one's parts are no longer than shares are.
+  if (all_few && all[3] > 0 && all[3] <= a.shares) {
+    const int parts = min(a.shares / all[3], max((longest + kLeast - 1) / kLeast, 1));
+    if ((longest / parts >> a.shift) <= s.each) s.parts = uniform(parts);
+  }
+  int from, to, at, end;
+  if (s.parts) {
+    const int item = w / s.parts;
+    s.x = w - item * s.parts;
+    s.size = item < all[3];
+    from = before[3], to = from + mine[3], at = item, end = -1;
+  } else {
+    const int64_t at_ = static_cast<int64_t>(w) * s.each;
+    s.size = at_ < total ? min(total - static_cast<int>(at_), s.each) : 0;
+    from = all_few ? before[kAllFew] : (j < p ? before[kFew] : before[kMany]);
+    to = from + (all_few ? mine[kAllFew] : (j < p ? mine[kFew] : mine[kMany]));
+    at = s.size > 0 ? static_cast<int>(at_) : -1, end = s.size == s.each ? at + s.each : -1;
+  }
   if (s.size > 0 && ((from <= at && at < to) || (from <= end && end < to))) {
     int r_from = from;
     for (int r = first; r < last; ++r) {
       if (each > 1) q = request(a, r);
-      const int m = measure(a, q, s.few) * a.n_kv;
-      Place place;
+      const int m = s.parts ? items_of(q) : measure(a, q, s.kind) * a.n_kv;
+      Place place = {};
       if (r_from <= at && at < r_from + m) {
-        s_moved[0] = locate(a, q, s.few, static_cast<int>(at) - r_from, s.each, place);
+        if (s.parts) {
+          const int tiles = (q.rows + kFewRows - 1) / kFewRows;
+          place.head = (at - r_from) / tiles, place.tile = at - r_from - place.head * tiles;
+        } else {
+          s_moved[0] = locate(a, q, s.kind, at - r_from, s.each, place);
+        }
         s_place = place, s_q = q, s_r = r;
       }
-      if (r_from <= end && end < r_from + m) s_moved[1] = locate(a, q, s.few, static_cast<int>(end) - r_from, s.each, place);
+      if (r_from <= end && end < r_from + m) s_moved[1] = locate(a, q, s.kind, end - r_from, s.each, place);
       r_from += m;
     }
   }
   __syncthreads();
   s.none_from = uniform(s_none[0]), s.none_to = uniform(s_none[1]);
   if (s.size > 0) {
-    s.size = uniform(s.size + s_moved[1] - s_moved[0]);
     const Place place = uniform(s_place);
-    s.r = uniform(s_r), s.q = uniform(s_q), s.head = place.head, s.tile = place.tile, s.x = place.x;
+    s.r = uniform(s_r), s.q = uniform(s_q), s.head = place.head, s.tile = place.tile;
+    if (!s.parts) s.size = uniform(s.size + s_moved[1] - s_moved[0]), s.x = place.x;
   }
   return s;
 }
 
 // The next request of a kind, 64 looked at at a time; -1 if there is none.
-__device__ __forceinline__ int next_request(const PagedArgs& a, int r, bool few) {
+__device__ __forceinline__ int next_request(const PagedArgs& a, int r, int kind) {
   for (; r < a.requests; r += 64) {
     const int i = r + static_cast<int>(threadIdx.x & 63);
-    const uint64_t is = __ballot(i < a.requests && measure(a, request(a, min(i, a.requests - 1)), few) != 0);
+    const uint64_t is = __ballot(i < a.requests && measure(a, request(a, min(i, a.requests - 1)), kind) != 0);
     if (is != 0) return r + __builtin_ctzll(is);
   }
   return -1;
@@ -956,36 +991,44 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
       reinterpret_cast<u32x4*>(a.out)[i < front ? i : i - front + s.none_to * row] = u32x4{0u, 0u, 0u, 0u};
   }
   Part part = {};
+  const bool few = s.kind != kMany;
+  const int tile_rows = few ? kFewRows : kManyRows;
   int left = s.size, x = s.x, t = s.tile;
   Segment g;
   g.r = s.r, g.q = s.q, g.head = s.head;
   while (left > 0) {
-    const Ramp items = ramp(a, g.q, s.few);
+    const Ramp items = ramp(a, g.q, few);
     for (; left > 0 && g.head < a.n_kv; ++g.head, t = 0)
       for (; left > 0 && t < items.tiles; ++t, x = 0) {
-        const int of_item = items.of(t), take = min(of_item - x, left);
-        if (take <= 0) continue;  // (a share that begins at an item's end)
-        g.row0 = t * (s.few ? kFewRows : kManyRows);
-        g.rows = min(g.q.rows - g.row0, s.few ? kFewRows : kManyRows);
-        const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1), start = start_of(a, s.few);
-        auto cut = [&](int at) {
-          if (at >= of_item) return seen;
-          const int64_t key = static_cast<int64_t>(max(at - start, 0)) << a.shift;
-          return key < seen ? static_cast<int>(key) / kCut * kCut : seen;
-        };
-        g.lo = cut(x), g.hi = cut(x + take);
-        g.whole = take == of_item;
-        g.slot = 2 * s.id + (x == 0);
-        if (x == 0 && take < of_item) {  // (the shares' ends behind this one that are inside of the item and not near its end)
-          part.parts = 2 + (of_item - snap_of(a, of_item, s.each) - take) / s.each;
-          part.head = g.head, part.first = g.q.first, part.row0 = g.row0, part.rows = g.rows;
+        g.row0 = t * tile_rows;
+        g.rows = min(g.q.rows - g.row0, tile_rows);
+        const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1);
+        int parts = s.parts, take = 1;
+        if (s.parts) {
+          auto cut = [&](int i) { return i == s.parts ? seen : static_cast<int>(static_cast<int64_t>(seen) * i / s.parts) / kCut * kCut; };
+          g.lo = cut(x), g.hi = cut(x + 1);
+        } else {
+          const int of_item = items.of(t), start = start_of(a, few);
+          take = min(of_item - x, left);
+          if (take <= 0) continue;  // (a share that begins at an item's end)
+          auto cut = [&](int at) {
+            if (at >= of_item) return seen;
+            const int64_t key = static_cast<int64_t>(max(at - start, 0)) << a.shift;
+            return key < seen ? static_cast<int>(key) / kCut * kCut : seen;
+          };
+          g.lo = cut(x), g.hi = cut(x + take);
+          // (the shares' ends behind this one that are inside of the item and not near its end)
+          parts = take == of_item ? 1 : 2 + (of_item - snap_of(a, of_item, s.each) - take) / s.each;
         }
-        if (s.few) few_rows<DT, D, F8>(a, g);
+        g.whole = parts == 1;
+        g.slot = 2 * s.id + (x == 0);
+        if (x == 0 && parts > 1) part.parts = parts, part.head = g.head, part.first = g.q.first, part.row0 = g.row0, part.rows = g.rows;
+        if (few) few_rows<DT, D, F8>(a, g);
         else many_rows<DT, D, F8>(a, g);
         left -= take;
       }
     if (left <= 0) break;
-    g.r = next_request(a, g.r + 1, s.few), g.head = 0;
+    g.r = next_request(a, g.r + 1, s.kind), g.head = 0;
     if (g.r < 0) break;
     g.q = request(a, g.r);
   }
