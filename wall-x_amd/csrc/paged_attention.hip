@@ -280,6 +280,15 @@ template <int DT>
 __device__ __forceinline__ u32x4 widen8(uint32_t x, uint32_t y) {
   return u32x4{widen2<DT, false>(x), widen2<DT, true>(x), widen2<DT, false>(y), widen2<DT, true>(y)};
 }
+// pack_step's operand in bf16, and what that rounding leaves as another (of what is not finite NaN: such rows are made again).
+__device__ __forceinline__ void pack_twice(const f32x16& p, int t, u32x4& hi, u32x4& lo) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float x = p[8 * t + 2 * u], y = p[8 * t + 2 * u + 1];
+    hi[u] = pack2<WX_BF16>(x, y);
+    lo[u] = pack2<WX_BF16>(x - __uint_as_float(hi[u] << 16), y - __uint_as_float(hi[u] & 0xffff0000u));
+  }
+}
 // what rounding x to bf16 leaves (nothing of what is not finite)
 __device__ __forceinline__ float left_of(float x) {
   const float r = x - round_bf16(x);
@@ -413,7 +422,10 @@ __device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? ~0u : (
 __device__ __forceinline__ void hide(f32x16& s, uint32_t seen, int h) {
   const uint32_t mine = seen >> (4 * h);
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = mine >> (8 * (r / 4) + r % 4) & 1u ? s[r] : -kInf;
+  for (int r = 0; r < 16; ++r) {
+    const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(mine), 8 * (r / 4) + r % 4, 1));
+    s[r] = __uint_as_float((__float_as_uint(s[r]) & keep) | (0xff800000u & ~keep));
+  }
 }
 
 // Running maximum, sum of powers and sums of 32 rows.
@@ -626,10 +638,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const Segment& g) {
           const float4 x = *reinterpret_cast<const float4*>(scales + KB + 32 * n + 8 * w + 4 * h);
           s[n][4 * w] *= x.x, s[n][4 * w + 1] *= x.y, s[n][4 * w + 2] *= x.z, s[n][4 * w + 3] *= x.w;
         }
-      p[2 * n] = pack_step<PT>(s[n], 0), p[2 * n + 1] = pack_step<PT>(s[n], 1);
-      if constexpr (kTwice<DT, F8>) {
-        const f32x16 rest = left_of(s[n]);
-        p2[2 * n] = pack_step<PT>(rest, 0), p2[2 * n + 1] = pack_step<PT>(rest, 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (kTwice<DT, F8>) pack_twice(s[n], t, p[2 * n + t], p2[2 * n + t]);
+        else p[2 * n + t] = pack_step<PT>(s[n], t);
       }
     }
     sums.l += l[0] + l[1];
@@ -899,10 +911,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
     for (int u = 0; u < 8; ++u) power(0, 2 * u);
     u32x4 p[2], p2[2];
     auto pack = [&](int n) {
-      p[0] = pack_step<PT>(s[n], 0), p[1] = pack_step<PT>(s[n], 1);
-      if constexpr (kTwice<DT, F8>) {
-        const f32x16 rest = left_of(s[n]);
-        p2[0] = pack_step<PT>(rest, 0), p2[1] = pack_step<PT>(rest, 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (kTwice<DT, F8>) pack_twice(s[n], t, p[t], p2[t]);
+        else p[t] = pack_step<PT>(s[n], t);
       }
     };
     pack(0);
