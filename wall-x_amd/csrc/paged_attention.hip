@@ -1047,97 +1047,98 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
   if (threadIdx.x == 0) a.part[s.id] = part;
 }
 
-// Joins the parts of the item that begins in share blockIdx.x and ends in a later one.  Of up to kJoinInWave parts 16 lanes have a row, 8
-// channels each, and 8 parts are on their way at a time; of more a workgroup has a row, a quarter of the parts to a wavefront, lane l channels 2 l
-// and 2 l + 1.
-constexpr int kJoinInWave = 16, kJoinBlocks = 8;
+// Joins the parts of the item that begins in share blockIdx.x and ends in a later one.  16 lanes have a row, 8 channels each, and ask for 8 parts at
+// a time.  Of up to 8 parts a wavefront has four rows; of more a workgroup, each wavefront a quarter of the parts.
+constexpr int kJoinBlocks = 8;
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-  __shared__ float s_top[4], s_sum[4];
-  __shared__ float2 s_out[4][64];
-  const int id = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float4 s_sums[4][64][2];
+  __shared__ float2 s_stats[4][4];
+  const int id = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15;
   const Part p = uniform(a.part[id]);
   if (p.parts == 0) return;
-  auto slot = [&](int i, int row) { return static_cast<int64_t>(i == 0 ? 2 * id + 1 : 2 * (id + i)) * a.part_rows + row; };
-  auto result = [&](int row) {
-    const int at = p.row0 + row, i = a.by_group.div(at), hq = p.head * a.group + at - i * a.group;
-    return a.out + (static_cast<int64_t>(p.first + i) * a.n_q + hq) * D;
-  };
   // (a part that the row sees nothing of has the weight 0 and counts nothing, unless its scores were NaN)
   auto weight = [&](float2 st, float top) { return st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c); };
   auto share_of = [](float2 st, float w) { return st.x == -kInf ? 0.f * st.y : st.y * w; };
-  if (p.parts <= kJoinInWave) {
-    const int row = (blockIdx.y * 4 + wave) * 4 + (lane >> 4), c = lane & 15;
-    if (row >= p.rows || 8 * c >= D) return;
-    float2 st[kJoinInWave];
-    float top = -kInf, l = 0.f, o[8] = {};
-#pragma unroll
-    for (int i = 0; i < kJoinInWave; ++i) st[i] = i < p.parts ? a.stats[slot(i, row)] : float2{-kInf, 0.f};
-#pragma unroll
-    for (int i0 = 0; i0 < kJoinInWave; i0 += 8) {
-      if (i0 >= p.parts) break;
+  struct Sum {
+    float top, l, o[8];
+  };
+  auto add = [&](Sum& s, float w, const float4& x, const float4& y) {
+    if (w == 0.f) return;
+    s.o[0] += x.x * w, s.o[1] += x.y * w, s.o[2] += x.z * w, s.o[3] += x.w * w;
+    s.o[4] += y.x * w, s.o[5] += y.y * w, s.o[6] += y.z * w, s.o[7] += y.w * w;
+  };
+  auto parts_of = [&](int row, int first, int last) {
+    Sum s{-kInf, 0.f, {}};
+    for (int i0 = first; i0 < last; i0 += 8) {
+      float2 st[8];
       float4 x[8], y[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float4* from = reinterpret_cast<const float4*>(a.sums + slot(min(i0 + u, p.parts - 1), row) * D + 8 * c);
+      for (int u = 0; u < 8; ++u) {  // (past the last: the last one's, without weight)
+        const int i = min(i0 + u, last - 1);
+        const int64_t at = static_cast<int64_t>(i == 0 ? 2 * id + 1 : 2 * (id + i)) * a.part_rows + row;
+        st[u] = a.stats[at];
+        const float4* from = reinterpret_cast<const float4*>(a.sums + at * D + 8 * c);
         x[u] = from[0], y[u] = from[1];
       }
-      if (i0 == 0)
-#pragma unroll
-        for (int i = 0; i < kJoinInWave; ++i) top = fmaxf(top, st[i].x);
+      float top = s.top;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const float w = weight(st[i0 + u], top);
-        l += share_of(st[i0 + u], w);
-        if (w == 0.f) continue;
-        o[0] += x[u].x * w, o[1] += x[u].y * w, o[2] += x[u].z * w, o[3] += x[u].w * w;
-        o[4] += y[u].x * w, o[5] += y[u].y * w, o[6] += y[u].z * w, o[7] += y[u].w * w;
+        if (i0 + u >= last) st[u] = float2{-kInf, 0.f};
+        top = fmaxf(top, st[u].x);
+      }
+      const float f = weight(float2{s.top, 0.f}, top);
+      s.l = share_of(float2{s.top, s.l}, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s.o[e] = f == 0.f ? 0.f : s.o[e] * f;
+      s.top = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = weight(st[u], top);
+        s.l += share_of(st[u], w);
+        add(s, w, x[u], y[u]);
       }
     }
-    const float inv = 1.f / l;
+    return s;
+  };
+  auto store = [&](int row, Sum& s) {
+    const float inv = 1.f / s.l;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
-    *reinterpret_cast<u32x4*>(result(row) + 8 * c) = pack16<DT>(o);
+    for (int e = 0; e < 8; ++e) s.o[e] = s.l == 0.f ? 0.f : s.o[e] * inv;
+    const int at = p.row0 + row, i = a.by_group.div(at), hq = p.head * a.group + at - i * a.group;
+    *reinterpret_cast<u32x4*>(a.out + (static_cast<int64_t>(p.first + i) * a.n_q + hq) * D + 8 * c) = pack16<DT>(s.o);
+  };
+  if (p.parts <= 8) {
+    const int row = (blockIdx.y * 4 + wave) * 4 + (lane >> 4);
+    if (row >= p.rows || 8 * c >= D) return;
+    Sum s = parts_of(row, 0, p.parts);
+    store(row, s);
     return;
   }
   const int each = (p.parts + 3) / 4, first = min(wave * each, p.parts), last = min(first + each, p.parts);
-  for (int row = blockIdx.y; row < p.rows; row += kJoinBlocks) {
-    float top = -kInf, l = 0.f;
-    for (int i = first + lane; i < last; i += 64) top = fmaxf(top, a.stats[slot(i, row)].x);
-    top = wave_max(top);
-    if (lane == 0) s_top[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-    float2 o = {0.f, 0.f};
-    for (int i0 = first; i0 < last; i0 += 64) {
-      const float2 st = i0 + lane < last ? a.stats[slot(i0 + lane, row)] : float2{-kInf, 0.f};
-      const float f = weight(st, top);
-      l += share_of(st, f);
-      const int n = min(64, last - i0);
-      for (int i = 0; i < n; i += 8) {
-        float2 y[8];
-        float w[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {  // (past the last: the last one's, without weight)
-          const int at = min(i + u, n - 1);
-          w[u] = i + u < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), at)) : 0.f;
-          y[u] = 2 * lane < D ? reinterpret_cast<const float2*>(a.sums + slot(i0 + at, row) * D)[lane] : float2{0.f, 0.f};
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          o.x += w[u] == 0.f ? 0.f : y[u].x * w[u];
-          o.y += w[u] == 0.f ? 0.f : y[u].y * w[u];
-        }
-      }
+  for (int row0 = blockIdx.y * 4; row0 < p.rows; row0 += 4 * kJoinBlocks) {
+    const int row = row0 + (lane >> 4);
+    const bool live = row < p.rows && 8 * c < D;
+    if (live) {
+      const Sum s = parts_of(row, first, last);
+      s_sums[wave][lane][0] = float4{s.o[0], s.o[1], s.o[2], s.o[3]};
+      s_sums[wave][lane][1] = float4{s.o[4], s.o[5], s.o[6], s.o[7]};
+      if (c == 0) s_stats[wave][lane >> 4] = float2{s.top, s.l};
     }
-    l = wave_sum(l);
-    if (lane == 0) s_sum[wave] = l;
-    s_out[wave][lane] = o;
     __syncthreads();
-    l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-    o.x = (s_out[0][lane].x + s_out[1][lane].x) + (s_out[2][lane].x + s_out[3][lane].x);
-    o.y = (s_out[0][lane].y + s_out[1][lane].y) + (s_out[2][lane].y + s_out[3][lane].y);
-    if (2 * lane < D && wave == 0) reinterpret_cast<uint32_t*>(result(row))[lane] = l == 0.f ? 0u : pack2<DT>(o.x / l, o.y / l);
+    if (live && wave == 0) {
+      Sum s{-kInf, 0.f, {}};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) s.top = fmaxf(s.top, s_stats[w][lane >> 4].x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 st = s_stats[w][lane >> 4];
+        const float f = weight(st, s.top);
+        s.l += share_of(st, f);
+        add(s, f, s_sums[w][lane][0], s_sums[w][lane][1]);
+      }
+      store(row, s);
+    }
     __syncthreads();
   }
 }
