@@ -150,16 +150,29 @@ __device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, int 
   p.x = to;
   return moved;
 }
+template <class T>
+__device__ __forceinline__ T of_lane(T x, int lane) {
+  static_assert(sizeof(T) % 4 == 0, "");
+  uint32_t w[sizeof(T) / 4];
+  __builtin_memcpy(w, &x, sizeof(T));
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) w[i] = __builtin_amdgcn_readlane(w[i], lane);
+  __builtin_memcpy(&x, w, sizeof(T));
+  return x;
+}
+// Up to 64 requests are a wavefront's, and every wavefront finds the share for itself, without a barrier (64 single tokens 20.6 -> 19.6 us); more are
+// spread over the workgroup's threads.
 __device__ __forceinline__ Share share(const PagedArgs& a) {
   enum { kSums = 4 };  // measures of each Kind, number of items of few rows
   __shared__ int s_sums[4][kSums], s_longest[4], s_moved[2];
   __shared__ Place s_place;
   __shared__ Request s_q;
   __shared__ int s_r, s_none[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (a.requests + 255) / 256;
-  const int first = min(tid * each, a.requests), last = min(first + each, a.requests);
+  const bool alone = a.requests <= 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = alone ? 1 : (a.requests + 255) / 256;
+  const int first = min((alone ? lane : tid) * each, a.requests), last = min(first + each, a.requests);
   int mine[kSums] = {}, sum[kSums], longest = 0;
-  if (tid == 0) s_none[0] = a.requests ? 0 : a.tokens, s_none[1] = a.tokens, s_moved[0] = 0, s_moved[1] = 0;
+  if (tid == 0) s_moved[0] = 0, s_moved[1] = 0;
   auto items_of = [&](const Request& q) { return (q.rows + kFewRows - 1) / kFewRows * a.n_kv; };
   Request q = {};
   for (int r = first; r < last; ++r) {
@@ -171,25 +184,30 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     mine[kAllFew] += m;
     mine[3] += items_of(q);
     longest = max(longest, q.n == 0 ? 0 : q.length);
-    if (r == 0) s_none[0] = q.first;
-    if (r == a.requests - 1) s_none[1] = q.first + q.n;
+    if (!alone && r == 0) s_none[0] = q.first;
+    if (!alone && r == a.requests - 1) s_none[1] = q.first + q.n;
   }
 #pragma unroll
-  for (int i = 0; i < kSums; ++i) {
-    sum[i] = wave_prefix(mine[i]);
-    if (lane == 63) s_sums[wave][i] = sum[i];
-  }
+  for (int i = 0; i < kSums; ++i) sum[i] = wave_prefix(mine[i]);
   longest = max(wave_extreme<true>(longest), __builtin_amdgcn_readlane(wave_extreme<true>(__shfl_xor(longest, 32)), 0));
-  if (lane == 0) s_longest[wave] = longest;
-  __syncthreads();
   int all[kSums], before[kSums];
 #pragma unroll
+  for (int i = 0; i < kSums; ++i) all[i] = __builtin_amdgcn_readlane(sum[i], 63), before[i] = sum[i] - mine[i];
+  if (!alone) {
+    if (lane == 0) s_longest[wave] = longest;
+    if (lane == 63)
+#pragma unroll
+      for (int i = 0; i < kSums; ++i) s_sums[wave][i] = sum[i];
+    __syncthreads();
+  }
+#pragma unroll
   for (int i = 0; i < kSums; ++i) {
+    if (alone) continue;
     const int w0 = s_sums[0][i], w1 = s_sums[1][i], w2 = s_sums[2][i];
-    before[i] = sum[i] - mine[i] + (wave > 0 ? w0 : 0) + (wave > 1 ? w1 : 0) + (wave > 2 ? w2 : 0);
+    before[i] += (wave > 0 ? w0 : 0) + (wave > 1 ? w1 : 0) + (wave > 2 ? w2 : 0);
     all[i] = uniform(w0 + w1 + w2 + s_sums[3][i]);
   }
-  longest = uniform(max(max(s_longest[0], s_longest[1]), max(s_longest[2], s_longest[3])));
+  longest = alone ? uniform(longest) : uniform(max(max(s_longest[0], s_longest[1]), max(s_longest[2], s_longest[3])));
   // Tiles of few rows for all where they give every workgroup one item at most and the keys are few: 64 x 32 queries over 800 to 912 keys 51 us
   // in two parts for each tile of many rows.
   const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, per_xcd = a.shares / 8;
@@ -225,32 +243,45 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     to = from + (all_few ? mine[kAllFew] : (j < p ? mine[kFew] : mine[kMany]));
     at = s.size > 0 ? static_cast<int>(at_) : -1, end = s.size == s.each ? at + s.each : -1;
   }
+  Place place = {};
+  int moved[2] = {0, 0};
   if (s.size > 0 && ((from <= at && at < to) || (from <= end && end < to))) {
     int r_from = from;
     for (int r = first; r < last; ++r) {
       if (each > 1) q = request(a, r);
       const int m = s.parts ? items_of(q) : measure(a, q, s.kind) * a.n_kv;
-      Place place = {};
       if (r_from <= at && at < r_from + m) {
         if (s.parts) {
           const int tiles = (q.rows + kFewRows - 1) / kFewRows;
           place.head = (at - r_from) / tiles, place.tile = at - r_from - place.head * tiles;
         } else {
-          s_moved[0] = locate(a, q, s.kind, at - r_from, s.each, place);
+          moved[0] = locate(a, q, s.kind, at - r_from, s.each, place);
         }
-        s_place = place, s_q = q, s_r = r;
+        if (!alone) s_moved[0] = moved[0], s_place = place, s_q = q, s_r = r;
       }
-      if (r_from <= end && end < r_from + m) s_moved[1] = locate(a, q, s.kind, end - r_from, s.each, place);
+      Place end_place;
+      if (r_from <= end && end < r_from + m) {
+        moved[1] = locate(a, q, s.kind, end - r_from, s.each, end_place);
+        if (!alone) s_moved[1] = moved[1];
+      }
       r_from += m;
     }
   }
-  __syncthreads();
-  s.none_from = uniform(s_none[0]), s.none_to = uniform(s_none[1]);
-  if (s.size > 0) {
-    const Place place = uniform(s_place);
-    s.r = uniform(s_r), s.q = uniform(s_q), s.head = place.head, s.tile = place.tile;
-    if (!s.parts) s.size = uniform(s.size + s_moved[1] - s_moved[0]), s.x = place.x;
+  if (alone) {  // (the lane that has the request, for the share's begin and for its end; lane 63 has none, or nothing to move)
+    const uint64_t begins = __ballot(from <= at && at < to), ends = __ballot(from <= end && end < to);
+    const int l = begins ? __builtin_ctzll(begins) : 0;
+    place = of_lane(place, l), s.q = of_lane(q, l), s.r = l;
+    moved[0] = __builtin_amdgcn_readlane(moved[0], l), moved[1] = ends ? __builtin_amdgcn_readlane(moved[1], __builtin_ctzll(ends)) : 0;
+    s.none_from = a.requests ? __builtin_amdgcn_readlane(q.first, 0) : a.tokens;
+    s.none_to = a.requests ? __builtin_amdgcn_readlane(q.first + q.n, a.requests - 1) : a.tokens;
+  } else {
+    __syncthreads();
+    s.none_from = uniform(s_none[0]), s.none_to = uniform(s_none[1]);
+    place = uniform(s_place), s.q = uniform(s_q), s.r = uniform(s_r);
+    moved[0] = uniform(s_moved[0]), moved[1] = uniform(s_moved[1]);
   }
+  s.head = place.head, s.tile = place.tile;
+  if (!s.parts) s.size = uniform(s.size + (s.size > 0 ? moved[1] - moved[0] : 0)), s.x = place.x;
   return s;
 }
 
