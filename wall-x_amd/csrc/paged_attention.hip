@@ -18,7 +18,7 @@ namespace {
 
 #define WX_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
 
-constexpr int kFewRows = 64, kManyRows = 128;  // rows of an item of either kind
+constexpr int kFewLog = 6, kManyLog = 7, kFewRows = 1 << kFewLog, kManyRows = 1 << kManyLog;  // rows of an item of either kind
 constexpr int kCut = 64;          // items are cut at multiples of so many keys
 constexpr int kStartFew = 192, kStartMany = 128;  // an item's start, in keys
 constexpr int kLeast = 256;       // the least that a workgroup takes
@@ -82,7 +82,7 @@ struct Ramp {
 };
 __device__ __forceinline__ int start_of(const PagedArgs& a, bool few) { return max((few ? kStartFew : kStartMany) >> a.shift, 1); }
 __device__ __forceinline__ Ramp ramp(const PagedArgs& a, const Request& q, bool few) {
-  const int rows = few ? kFewRows : kManyRows, tiles = (q.rows + rows - 1) / rows;
+  const int log = few ? kFewLog : kManyLog, rows = 1 << log, tiles = (q.rows + rows - 1) >> log;
   const int step = a.causal && tiles > 1 ? a.by_group.div(rows) >> a.shift : 0;
   return {((step ? max(q.length - q.n, 0) : q.length) >> a.shift) + start_of(a, few), step, tiles};
 }
@@ -150,6 +150,7 @@ __device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, int 
   p.x = to;
   return moved;
 }
+__device__ __forceinline__ int quotient(int x, int y) { return static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y)) + 0x1p-11f); }
 template <class T>
 __device__ __forceinline__ T of_lane(T x, int lane) {
   static_assert(sizeof(T) % 4 == 0, "");
@@ -223,16 +224,18 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   const int count = j < p ? 8 * p : 8 * (per_xcd - p), w = j < p ? xcd * p + j : xcd * (per_xcd - p) + j - p;
   s.id = j < p ? w : 8 * p + w;
   const int total = all_few ? all[kAllFew] : (j < p ? all[kFew] : all[kMany]);
-  s.each = uniform(max(total / count + 1, kLeast >> a.shift));
+  // (quotients of whole numbers by way of floats, which take a tenth of an exact division's instructions: a little more than total / count, ...)
+  s.each = uniform(max(static_cast<int>(static_cast<float>(total) * __builtin_amdgcn_rcpf(static_cast<float>(count)) * 1.000001f) + 2, kLeast >> a.shift));
   // Items of about one length, no more than there are workgroups: a like number of workgroups to each, without second items, where the longest
   // one's parts are no longer than shares are.
   if (all_few && all[3] > 0 && all[3] <= a.shares) {
-    const int parts = min(a.shares / all[3], max((longest + kLeast - 1) / kLeast, 1));
-    if ((longest / parts >> a.shift) <= s.each) s.parts = uniform(parts);
+    // (... and exact where both are below 1024: the quotient is off by less than 1 / 1024 then, and so far from the next whole number)
+    const int parts = min(quotient(a.shares, all[3]), max((longest + kLeast - 1) / kLeast, 1));
+    if (longest >> a.shift <= static_cast<int64_t>(s.each) * parts) s.parts = uniform(parts);
   }
   int from, to, at, end;
   if (s.parts) {
-    const int item = w / s.parts;
+    const int item = quotient(w, s.parts);
     s.x = w - item * s.parts;
     s.size = item < all[3];
     from = before[3], to = from + mine[3], at = item, end = -1;
@@ -1048,7 +1051,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1);
         int parts = s.parts, take = 1;
         if (s.parts) {
-          auto cut = [&](int i) { return i == s.parts ? seen : static_cast<int>(static_cast<int64_t>(seen) * i / s.parts) / kCut * kCut; };
+          const float each = static_cast<float>(seen) * (1.f / kCut) * __builtin_amdgcn_rcpf(static_cast<float>(s.parts));
+          auto cut = [&](int i) { return i == s.parts ? seen : min(seen, static_cast<int>(each * static_cast<float>(i)) * kCut); };
           g.lo = cut(x), g.hi = cut(x + 1);
         } else {
           const int of_item = items.of(t), start = start_of(a, few);
