@@ -563,7 +563,7 @@ int wx_cached_attention(const void* q, const void* k_cache, const void* v_cache,
  * stack as it was.  A request that the pages do not suffice for gets the tokens that it has pages for.
  * new_lengths int32 [requests] and new_free_count int32 [1] are written, lengths and free_count are not (no buffer may be two of them); in
  * page_table and free_pages only entries behind what is owned and free before are: the same call again does the same.  starts int32
- * [requests + 1]: where each request's added tokens begin among all of them; slots int32 and positions int64 [max_tokens]: of each added
+ * [requests + 1]: where each request's added tokens begin among all of them; slots int32 and positions int64 [max_tokens] (16-byte aligned): of each added
  * token its slot and its position in its request, -1 and 0 behind the last.  max_tokens bounds the tokens that are added: of more, starts stays at it and the rest has no
  * slot.  At most 4096 requests, 2^31 - 1 tokens and slots.
  * wx_paged_kv_write puts token b * seq + s of k and v [batch, n_kv_heads, seq, head_dim] (strides as above) into slots[b * seq + s],

@@ -29,6 +29,7 @@ def test_resize_refuses(p):
     assert resize(capacity=2 ** 27) == -2 and b"slots" in lib.wx_last_error_string()
     assert resize(requests=4096, width=2 ** 16) == -2 and resize(tokens=2 ** 30) == -2
     assert resize(x=None) == -1 and resize(count=None) == -1 and resize(slots=None) == -1 and b"null pointer" in lib.wx_last_error_string()
+    assert resize(slots=p + 8) == -1 and b"16-byte" in lib.wx_last_error_string()
 
 
 def test_write_refuses(p):

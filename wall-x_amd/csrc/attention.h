@@ -189,6 +189,18 @@ __device__ __forceinline__ int wave_extreme(int x) {
   return MAX ? max(a, b) : min(a, b);
 }
 
+__device__ __forceinline__ int wave_prefix(int x) {  // inclusive, over the wavefront's lanes
+#define WX_ADD(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false)
+  WX_ADD(0x111, 0xF);
+  WX_ADD(0x112, 0xF);
+  WX_ADD(0x114, 0xF);
+  WX_ADD(0x118, 0xF);
+  WX_ADD(0x142, 0xA);  // (the last lane of a row of 16 to the next row, of 32 to the next half)
+  WX_ADD(0x143, 0xC);
+#undef WX_ADD
+  return x;
+}
+
 // Byte offsets, in a tile, of what a lane reads of its first block: the other blocks lie at constant distances and exclusive-ors.
 //   rows  A operand, contraction over the head: row lane & 31 of 32 rows, channels 16 t + 8 h .. + 7 of step t
 //   cols  A operand, contraction over the tile's rows: channel 32 o + (lane & 31), rows 16 t + 8 (j / 4) + 4 h + j % 4

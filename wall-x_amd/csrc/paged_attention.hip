@@ -104,18 +104,6 @@ __device__ __forceinline__ T uniform(T x) {
   return x;
 }
 
-__device__ __forceinline__ int wave_prefix(int x) {  // inclusive, over the wavefront's lanes
-#define WX_ADD(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false)
-  WX_ADD(0x111, 0xF);
-  WX_ADD(0x112, 0xF);
-  WX_ADD(0x114, 0xF);
-  WX_ADD(0x118, 0xF);
-  WX_ADD(0x142, 0xA);  // (the last lane of a row of 16 to the next row, of 32 to the next half)
-  WX_ADD(0x143, 0xC);
-#undef WX_ADD
-  return x;
-}
-
 // A workgroup's share: `size` of its kind's measures, from `x` into tile `tile` of `head` of request r; or part x of that item.
 struct Share {
   int kind, id;    // id: unique over all kinds
