@@ -256,6 +256,57 @@ def test_rows_are_requests(dev, B, S, D, e4m3):
             check(out, wanted(q, cache, table, lengths, starts, causal), "starts")
 
 
+@pytest.mark.parametrize("counts,lengths", [
+    ([1] * 64, [800 + 7 * i % 113 for i in range(64)]),              # items of about one length: a like number of workgroups each
+    ([1] * 300, [1 + 17 * i % 90 for i in range(300)]),              # more requests than a workgroup has threads
+    ([0, 2, 0, 0] * 300, [5, 40, 0, 9] * 300),                       # most of them without queries
+    ([1] * 40 + [70] + [0] * 30 + [3] * 5 + [150, 65], [200] * 40 + [300] + [10] * 30 + [2500, 1, 64, 63, 65] + [150, 1000]),  # tiles of both kinds
+    ([33] * 20, [40 + 90 * i for i in range(20)]),                   # tiles of few rows alone, lengths far apart
+    ([9, 1, 100], [5, 0, 60]),                                       # fewer keys than queries
+    ([1], [20000]), ([2] * 3, [9000, 1, 4000]),
+])
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_schedules(dev, counts, lengths, e4m3):
+    rng, g = random.Random(len(counts)), torch.Generator(device=dev).manual_seed(len(counts))
+    ps, D, pages = 16, 64, sum(-(-n // 16) for n in lengths) + 2
+    cache = pool(pages, 2, ps, D, torch.bfloat16, e4m3, g, dev)
+    table = tables(lengths, ps, pages, -(-max(lengths) // ps), rng, dev)
+    starts = prefix(counts)
+    q = torch.randn(1, starts[-1], 16, D, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    for causal in (True, False):
+        out = ops.paged_attention(q, *cache, table, ints(lengths, dev), ints(starts, dev), causal=causal)
+        check(out, wanted(q, cache, table, lengths, starts, causal), "schedule")
+
+
+def test_wide_tables(dev):
+    """Tables that could hold 2^30 keys a request (measures in more than a key), few of which are there; tokens before the first request."""
+    rng, g = random.Random(5), torch.Generator(device=dev).manual_seed(5)
+    ps, width, lengths, counts = 65536, 16383, [70000, 131000, 3, 65537], [2, 40, 0, 1]
+    cache = pool(8, 2, ps, 64, torch.bfloat16, True, g, dev)
+    table = tables(lengths, ps, 8, 2, rng, dev)
+    table = torch.cat((table, table.new_full((4, width - 2), -1)), 1)
+    starts = [7 + x for x in prefix(counts)]
+    q = torch.randn(1, starts[-1] + 2, 8, 64, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    for causal in (True, False):
+        out = ops.paged_attention(q, *cache, table, ints(lengths, dev), ints(starts, dev), causal=causal)
+        check(out, wanted(q, cache, table[:, :2], lengths, starts, causal), "wide")
+        assert not out[0, :, :7].any() and not out[0, :, -2:].any()
+
+
+def test_nothing_to_attend_to(dev):
+    cache = ops.paged_kv_cache(3, 2, 16, 64, dev)
+    q = torch.randn(1, 9, 4, 64, device=dev).to(torch.bfloat16).transpose(1, 2)
+    none = torch.zeros(0, 5, dtype=torch.int32, device=dev)
+    assert not ops.paged_attention(q, *cache, none, ints([], dev), ints([4], dev)).any()                                        # no requests
+    assert not ops.paged_attention(q, *cache, ints([[0]] * 3, dev), ints([0, -5, 0], dev), ints([0, 4, 4, 9], dev)).any()     # no keys
+    assert not ops.paged_attention(q, *cache, ints([[0]] * 3, dev), ints([9, 9, 9], dev), ints([4, 4, 4, 4], dev)).any()      # no queries
+    assert not ops.paged_attention(q, *cache, torch.zeros(3, 0, dtype=torch.int32, device=dev), ints([9, 9, 9], dev), ints([0, 4, 4, 9], dev)).any()  # no pages to a request
+    empty = ops.paged_kv_cache(0, 2, 16, 64, dev)
+    assert not ops.paged_attention(q, *empty, ints([[0]], dev), ints([9], dev)).any()                                          # no pages at all
+    assert ops.paged_attention(q[:, :, :0], *cache, none, ints([], dev), ints([0], dev)).shape == (1, 4, 0, 64)
+    ops.paged_kv_write(q[:, :2], q[:, :2], *empty, torch.zeros(9, dtype=torch.int32, device=dev))
+
+
 @pytest.mark.parametrize("e4m3", [True, False])
 @pytest.mark.parametrize("n", [1, 4, 70])
 def test_pages_that_are_none(dev, n, e4m3):

@@ -6,7 +6,15 @@
 // keys that it sees and some for its start.  The launch is a fixed number of workgroups, two to a CU; each finds the sum of all
 // measures for itself (a prefix sum over the requests) and takes an equal share of it, wherever in an item that begins or ends.  So one request
 // over 32768 keys and 64 over 900 fill the chip alike, without the host and without a plan in memory.  An item that lies in one share is
-// finished there; of one that is cut every share leaves a part (sums, maximum, sum of powers), which a second launch joins, in order.
+// finished there; of one that is cut every share leaves a part (sums, maximum, sum of powers), which a second launch joins, in order.  (Joined by the
+// workgroup whose part is the last to arrive, with stores and loads past the XCDs' L2: 64 x 32 queries 81 us for 52, 8 long requests 42 for 37.)
+//
+// What bounds it.  Single tokens over long caches: memory; 112 MB of 8 requests over 20 to 32 thousand keys stream in some 24 us, 4.7 TB/s, and
+// 6 before and 7 behind that go into the plan, the first pages and keys, and the join: 37 to 39 us in all.  32 requests of up to 5 tokens over up to 16000
+// bf16 keys: 262 MB in 67 us.  Short caches: the chain of loads alone; of 20.5 us for 64 single tokens over 900 keys 2.6 go into the plan,
+// 1.8 to the first keys' request, 2.8 into the one tile a wavefront has, 2.1 into the wavefronts' join, 4 into the parts'.  Chunks: 2048 queries over 16384
+// e4m3 keys 324 us, 0.79 PFLOP/s (the contiguous cache's kernel: 392); a tile of 64 keys takes a SIMD's two wavefronts 5200 cycles, in which
+// their products need 2048 and their other instructions 3600.  16 prompts of 912 bf16 tokens: 101 us, 62 to 102 by the workgroup, whose items are not cut.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,12 +27,18 @@ namespace {
 #define WX_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
 
 constexpr int kFewLog = 6, kManyLog = 7, kFewRows = 1 << kFewLog, kManyRows = 1 << kManyLog;  // rows of an item of either kind
-constexpr int kCut = 64;          // items are cut at multiples of so many keys
-constexpr int kStartFew = 192, kStartMany = 128;  // an item's start, in keys
-constexpr int kLeast = 256;       // the least that a workgroup takes
-constexpr int kShort = 2048;      // (see share)
-// An end of an item near to a share's end is the share's end: nearer than this in keys, which is about what a cut costs (a start, a part, its
-// join), and than 3/8 of a share.  Items of up to half a share are not cut at all.
+constexpr int kCut = 64;  // items are cut at multiples of so many keys
+// What an item takes besides its keys, in keys: about 4.5 us where 64 keys take 1.2 to 2.5.  With 64 / 192 and 128: 64 single tokens over 800 to 912
+// keys 23.5 / 22.0 us, 16 prompts of 912 tokens 123 / 111 (the items at a prompt's beginning are short).
+constexpr int kStartFew = 192, kStartMany = 128;
+// The least that a workgroup takes.  With 256 / 512 / 1024: 64 single tokens over 800 to 912 keys 35 / 39 / 48 us (when starts took longer).
+constexpr int kLeast = 256;
+// Tiles of few rows for everything where they are no more than the workgroups and their keys are no more than this: 64 x 32 queries over 800 to 912
+// keys 52 us in tiles of many rows, two workgroups to each, 40 so; 2048 queries over 16384 keys 324 and 390.
+constexpr int kShort = 2048;
+// An item's end near to a share's end is the share's end: nearer than this in keys, which is about what a cut costs (a start, a part, its
+// join), and than 3/8 of a share.  With 128 / 320: 64 mixed requests 64 / 67 us.  Items of up to half a share are not cut at all: 16 prompts of 912
+// tokens 113 -> 100 us.
 constexpr int kSnap = 128;
 
 struct Part {  // of the item that begins in a share and ends in a later one
@@ -149,8 +163,8 @@ __device__ __forceinline__ T of_lane(T x, int lane) {
   __builtin_memcpy(&x, w, sizeof(T));
   return x;
 }
-// Up to 64 requests are a wavefront's, and every wavefront finds the share for itself, without a barrier (64 single tokens 20.6 -> 19.6 us); more are
-// spread over the workgroup's threads.
+// Up to 64 requests are a wavefront's, and every wavefront finds the share for itself, without a barrier (32 requests of drafts 69 -> 67 us, 16 prompts
+// 104 -> 102); more are spread over the workgroup's threads.
 __device__ __forceinline__ Share share(const PagedArgs& a) {
   enum { kSums = 4 };  // measures of each Kind, number of items of few rows
   __shared__ int s_sums[4][kSums], s_longest[4], s_moved[2];
@@ -197,8 +211,6 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     all[i] = uniform(w0 + w1 + w2 + s_sums[3][i]);
   }
   longest = alone ? uniform(longest) : uniform(max(max(s_longest[0], s_longest[1]), max(s_longest[2], s_longest[3])));
-  // Tiles of few rows for all where they give every workgroup one item at most and the keys are few: 64 x 32 queries over 800 to 912 keys 51 us
-  // in two parts for each tile of many rows.
   const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, per_xcd = a.shares / 8;
   const bool all_few = all[kMany] == 0 || (all[3] <= a.shares && longest <= kShort);
   Share s = {};
@@ -215,7 +227,7 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   // (quotients of whole numbers by way of floats, which take a tenth of an exact division's instructions: a little more than total / count, ...)
   s.each = uniform(max(static_cast<int>(static_cast<float>(total) * __builtin_amdgcn_rcpf(static_cast<float>(count)) * 1.000001f) + 2, kLeast >> a.shift));
   // Items of about one length, no more than there are workgroups: a like number of workgroups to each, without second items, where the longest
-  // one's parts are no longer than shares are.
+  // one's parts are no longer than shares are.  64 single tokens over 800 to 912 keys 22.1 -> 20.6 us.
   if (all_few && all[3] > 0 && all[3] <= a.shares) {
     // (... and exact where both are below 1024: the quotient is off by less than 1 / 1024 then, and so far from the next whole number)
     const int parts = min(quotient(a.shares, all[3]), max((longest + kLeast - 1) / kLeast, 1));
