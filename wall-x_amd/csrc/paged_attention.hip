@@ -58,7 +58,7 @@ struct PagedArgs {
   int causal, tokens, requests, n_q, n_kv, group, seq, width, page_size, n_pages;
   Divider by_seq, by_page, by_group;
   float c;                         // scale * log2(e)
-  int shares;                      // workgroups, a multiple of 8
+  int shares, blocks;              // workgroups that take shares, a multiple of 8, and all of them, where each may take an item
   int shift;                       // measures are in 2^shift keys, so that the sum of all fits 31 bits
   int part_rows;                   // most rows of an item
   float* sums;                     // parts: [2 shares, part_rows, D]
@@ -166,7 +166,7 @@ __device__ __forceinline__ T of_lane(T x, int lane) {
 // Up to 64 requests are a wavefront's, and every wavefront finds the share for itself, without a barrier (32 requests of drafts 69 -> 67 us, 16 prompts
 // 104 -> 102); more are spread over the workgroup's threads.
 __device__ __forceinline__ Share share(const PagedArgs& a) {
-  enum { kSums = 4 };  // measures of each Kind, number of items of few rows
+  enum { kFewItems = 3, kManyItems, kSums };  // measures of each Kind, numbers of items of few rows (all requests') and of many (such requests')
   __shared__ int s_sums[4][kSums], s_longest[4], s_moved[2];
   __shared__ Place s_place;
   __shared__ Request s_q;
@@ -176,7 +176,7 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   const int first = min((alone ? lane : tid) * each, a.requests), last = min(first + each, a.requests);
   int mine[kSums] = {}, sum[kSums], longest = 0;
   if (tid == 0) s_moved[0] = 0, s_moved[1] = 0;
-  auto items_of = [&](const Request& q) { return (q.rows + kFewRows - 1) / kFewRows * a.n_kv; };
+  auto tiles_of = [&](const Request& q, bool few) { return few ? (q.rows + kFewRows - 1) >> kFewLog : (q.rows > kFewRows ? (q.rows + kManyRows - 1) >> kManyLog : 0); };
   Request q = {};
   for (int r = first; r < last; ++r) {
     q = request(a, r);
@@ -185,7 +185,8 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     mine[kFew] += few ? m : 0;
     mine[kMany] += few ? 0 : measure(a, q, kMany) * a.n_kv;
     mine[kAllFew] += m;
-    mine[3] += items_of(q);
+    mine[kFewItems] += tiles_of(q, true) * a.n_kv;
+    mine[kManyItems] += tiles_of(q, false) * a.n_kv;
     longest = max(longest, q.n == 0 ? 0 : q.length);
     if (!alone && r == 0) s_none[0] = q.first;
     if (!alone && r == a.requests - 1) s_none[1] = q.first + q.n;
@@ -212,7 +213,7 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   }
   longest = alone ? uniform(longest) : uniform(max(max(s_longest[0], s_longest[1]), max(s_longest[2], s_longest[3])));
   const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, per_xcd = a.shares / 8;
-  const bool all_few = all[kMany] == 0 || (all[3] <= a.shares && longest <= kShort);
+  const bool all_few = all[kMany] == 0 || (all[kFewItems] <= a.shares && longest <= kShort);
   Share s = {};
   // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
   int p = all_few ? per_xcd : 0;
@@ -221,27 +222,37 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     p = uniform(min(max(static_cast<int>(part * per_xcd + 0.5f), 1), per_xcd - 1));
   }
   s.kind = all_few ? kAllFew : (j < p ? kFew : kMany);
-  const int count = j < p ? 8 * p : 8 * (per_xcd - p), w = j < p ? xcd * p + j : xcd * (per_xcd - p) + j - p;
+  int count = j < p ? 8 * p : 8 * (per_xcd - p), w = j < p ? xcd * p + j : xcd * (per_xcd - p) + j - p;
   s.id = j < p ? w : 8 * p + w;
   const int total = all_few ? all[kAllFew] : (j < p ? all[kFew] : all[kMany]);
   // (quotients of whole numbers by way of floats, which take a tenth of an exact division's instructions: a little more than total / count, ...)
   s.each = uniform(max(static_cast<int>(static_cast<float>(total) * __builtin_amdgcn_rcpf(static_cast<float>(count)) * 1.000001f) + 2, kLeast >> a.shift));
   // Items of about one length, no more than there are workgroups: a like number of workgroups to each, without second items, where the longest
   // one's parts are no longer than shares are.  64 single tokens over 800 to 912 keys 22.1 -> 20.6 us.
-  if (all_few && all[3] > 0 && all[3] <= a.shares) {
+  if (all_few && all[kFewItems] > 0 && all[kFewItems] <= a.shares) {
     // (... and exact where both are below 1024: the quotient is off by less than 1 / 1024 then, and so far from the next whole number)
-    const int parts = min(quotient(a.shares, all[3]), max((longest + kLeast - 1) / kLeast, 1));
+    const int parts = min(quotient(a.shares, all[kFewItems]), max((longest + kLeast - 1) / kLeast, 1));
     if (longest >> a.shift <= static_cast<int64_t>(s.each) * parts) s.parts = uniform(parts);
   }
+  // Many items of many rows, two and more to a share: a workgroup for each instead, where the launch has as many (an XCD has neighbouring ones), long
+  // ones of a request first.  Which of the chip's places takes the next is found as they end: 16 prompts of 912 tokens 105 -> 97 us.
+  const int each_xcd = (all[kManyItems] + 7) / 8;
+  if (s.kind == kMany && all[kManyItems] >= 2 * count && each_xcd <= static_cast<int>(gridDim.x >> 3) - p) {
+    s.parts = 1;
+    w = j - p < each_xcd ? xcd * each_xcd + j - p : all[kManyItems];
+  } else if (j >= per_xcd) {
+    w = count;  // (nothing: the launch is wider than the shares for the sake of the items)
+  }
   int from, to, at, end;
+  const bool few = s.kind != kMany;
   if (s.parts) {
-    const int item = quotient(w, s.parts);
+    const int item = s.parts == 1 ? w : quotient(w, s.parts), n = few ? all[kFewItems] : all[kManyItems];
     s.x = w - item * s.parts;
-    s.size = item < all[3];
-    from = before[3], to = from + mine[3], at = item, end = -1;
+    s.size = item < n;
+    from = few ? before[kFewItems] : before[kManyItems], to = from + (few ? mine[kFewItems] : mine[kManyItems]), at = item, end = -1;
   } else {
     const int64_t at_ = static_cast<int64_t>(w) * s.each;
-    s.size = at_ < total ? min(total - static_cast<int>(at_), s.each) : 0;
+    s.size = at_ < total && w < count ? min(total - static_cast<int>(at_), s.each) : 0;
     from = all_few ? before[kAllFew] : (j < p ? before[kFew] : before[kMany]);
     to = from + (all_few ? mine[kAllFew] : (j < p ? mine[kFew] : mine[kMany]));
     at = s.size > 0 ? static_cast<int>(at_) : -1, end = s.size == s.each ? at + s.each : -1;
@@ -252,11 +263,11 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     int r_from = from;
     for (int r = first; r < last; ++r) {
       if (each > 1) q = request(a, r);
-      const int m = s.parts ? items_of(q) : measure(a, q, s.kind) * a.n_kv;
+      const int m = s.parts ? tiles_of(q, few) * a.n_kv : measure(a, q, s.kind) * a.n_kv;
       if (r_from <= at && at < r_from + m) {
         if (s.parts) {
-          const int tiles = (q.rows + kFewRows - 1) / kFewRows;
-          place.head = (at - r_from) / tiles, place.tile = at - r_from - place.head * tiles;
+          const int tiles = tiles_of(q, few);
+          place.head = (at - r_from) / tiles, place.tile = tiles - 1 - (at - r_from - place.head * tiles);
         } else {
           moved[0] = locate(a, q, s.kind, at - r_from, s.each, place);
         }
@@ -1079,7 +1090,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     if (g.r < 0) break;
     g.q = request(a, g.r);
   }
-  if (threadIdx.x == 0) a.part[s.id] = part;
+  if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.shares) a.part[s.id] = part;
 }
 
 // Joins the parts of the item that begins in share blockIdx.x and ends in a later one.  16 lanes have a row, 8 channels each, and ask for 8 parts at
@@ -1183,7 +1194,7 @@ int part_rows(int64_t tokens, int group) { return static_cast<int>(std::min<int6
 
 template <int DT, int D, bool F8>
 int launch(PagedArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((paged_attn_kernel<DT, D, F8>), dim3(static_cast<unsigned>(a.shares)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((paged_attn_kernel<DT, D, F8>), dim3(static_cast<unsigned>(a.blocks)), dim3(256), 0, s, a);
   if (int rc = check_launch("paged_attn_kernel")) return rc;
   hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3(static_cast<unsigned>(a.shares), kJoinBlocks), dim3(256), 0, s, a);
   return check_launch("paged_join_kernel");
@@ -1251,7 +1262,10 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   for (a.shift = 0; a.shift < 30 && tiles * ((keys >> a.shift) + kStartFew + kStartMany) > 0x3fffffff; ++a.shift) {
   }
   if (a.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
-  a.shares = shares(), a.part_rows = part_rows(a.tokens, group);
+  a.shares = a.blocks = shares();
+  const int64_t items = n_kv_heads * (static_cast<int64_t>(a.tokens) * group / kManyRows + requests);  // at most, of many rows
+  if (items >= 2 * a.shares && !too_many_blocks(items + 16 + a.shares, 256)) a.blocks = static_cast<int>((items + 7) / 8 * 8) + a.shares;
+  a.part_rows = part_rows(a.tokens, group);
   const int64_t rows = 2ll * a.shares * a.part_rows;
   a.sums = static_cast<float*>(workspace);
   a.stats = reinterpret_cast<float2*>(a.sums + rows * head_dim);
