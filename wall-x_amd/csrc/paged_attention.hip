@@ -40,6 +40,10 @@ constexpr int kShort = 2048;
 // join), and than 3/8 of a share.  With 128 / 320: 64 mixed requests 64 / 67 us.  Items of up to half a share are not cut at all: 16 prompts of 912
 // tokens 113 -> 100 us.
 constexpr int kSnap = 128;
+// What an e4m3 key takes of a tile of many rows, in those of few rows, which take their bytes' time; 16-bit keys take the same.  With 1 / 2 / 3, 62 single tokens
+// and two chunks of 509: heads of 64 in fp16 59 / 53 / 54 us, of 128 in bf16 77 / 66 / 70, of 8 heads of their own with chunks of 200 55 / 44 / 43;
+// 30 tokens over 8 to 16 thousand keys with two chunks of 128 96 / 90 / 91.  Of a bf16 cache 74 / 75 / 86, the long one 105 / 116 / 120.
+constexpr float kManyToFew = 2.f;
 
 struct Part {  // of the item that begins in a share and ends in a later one
   int parts;   // 0: there is none
@@ -165,6 +169,7 @@ __device__ __forceinline__ T of_lane(T x, int lane) {
 }
 // Up to 64 requests are a wavefront's, and every wavefront finds the share for itself, without a barrier (32 requests of drafts 69 -> 67 us, 16 prompts
 // 104 -> 102); more are spread over the workgroup's threads.
+template <bool F8>
 __device__ __forceinline__ Share share(const PagedArgs& a) {
   enum { kFewItems = 3, kManyItems, kSums };  // measures of each Kind, numbers of items of few rows (all requests') and of many (such requests')
   __shared__ int s_sums[4][kSums], s_longest[4], s_moved[2];
@@ -218,7 +223,7 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
   int p = all_few ? per_xcd : 0;
   if (!all_few && all[kFew] != 0) {
-    const float part = static_cast<float>(all[kFew]) / (static_cast<float>(all[kFew]) + static_cast<float>(all[kMany]));
+    const float part = static_cast<float>(all[kFew]) / (static_cast<float>(all[kFew]) + (F8 ? kManyToFew : 1.f) * static_cast<float>(all[kMany]));
     p = uniform(min(max(static_cast<int>(part * per_xcd + 0.5f), 1), per_xcd - 1));
   }
   s.kind = all_few ? kAllFew : (j < p ? kFew : kMany);
@@ -1041,7 +1046,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
 
 template <int DT, int D, bool F8>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
-  const Share s = share(a);
+  const Share s = share<F8>(a);
   if (s.none_from > 0 || s.none_to < a.tokens) {
     const int64_t row = static_cast<int64_t>(a.n_q) * (D / 8), front = s.none_from * row, none = front + (a.tokens - s.none_to) * row;
     for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < none; i += static_cast<int64_t>(gridDim.x) * 256)
