@@ -95,6 +95,20 @@ def test_a_growth_taken_back_restores_the_stack(dev):
     assert not starts.any() and bool((slots == -1).all())
 
 
+@pytest.mark.parametrize("inference", [False, True])
+@pytest.mark.parametrize("max_tokens", [0, 1, 37])
+def test_resize_results_are_tensors_of_their_own(dev, max_tokens, inference):
+    with torch.inference_mode(inference):
+        lengths, table, free, count = ops.paged_kv_tables(3, 4, 12, dev)
+        got = ops.paged_kv_resize(lengths, ints([1, 0, max(0, max_tokens - 1)], dev), table, free, count, 16, max_tokens)
+        for x, (size, dtype) in zip(got, ((3, torch.int32), (1, torch.int32), (4, torch.int32), (max_tokens, torch.int32), (max_tokens, torch.int64))):
+            assert x.shape == (size,) and x.dtype == dtype and x.is_contiguous() and x.data_ptr() % 16 == 0 and x.is_inference() == inference
+        for i, x in enumerate(got):  # (whatever is done to one leaves the others)
+            others = [(y, y.clone(), y._version if not inference else 0) for j, y in enumerate(got) if j != i]
+            x.add_(1).fill_(-77)
+            assert all(torch.equal(y, z) and (inference or y._version == v) for y, z, v in others)
+
+
 def test_resize_checked(dev):
     lengths, table, free, count = ops.paged_kv_tables(2, 4, 8, dev)
     native.set_checked(True)
