@@ -393,6 +393,16 @@ def test_what_is_not_seen_does_not_count(dev, n, dtype, e4m3):
         assert bool((torch.isnan(out[mine]) if what == "key" or e4m3 else torch.isinf(out[mine])).all()), what
 
 
+def test_requests_that_claim_the_same_tokens_over_and_over(dev):
+    """starts that descend 2300 times: more work than any that ascend can ask for, and none of it is done."""
+    R, T, width, ps = 4600, 4096, 512, 16
+    k, v, ks, vs = ops.paged_kv_cache(2, 1, ps, 64, dev)
+    q = torch.ones(1, 1, T, 64, dtype=torch.bfloat16, device=dev)
+    starts = ints([T * (r % 2) for r in range(R + 1)], dev)
+    out = ops.paged_attention(q, k, v, ks, vs, torch.zeros(R, width, dtype=torch.int32, device=dev), ints([width * ps] * R, dev), starts)
+    assert not out.any()
+
+
 def test_large_and_small_values_in_fp16(dev):
     """Scales beyond fp16's range in both directions."""
     rng, g = random.Random(1), torch.Generator(device=dev).manual_seed(1)

@@ -111,6 +111,8 @@ __device__ __forceinline__ int measure(const PagedArgs& a, const Request& q, int
   return p.before(p.tiles);
 }
 
+constexpr int kMostMeasure = 0x3fffffff, kMostHigh = kMostMeasure >> 8;  // of all requests together (the host chooses `shift` so)
+
 template <class T>
 __device__ __forceinline__ T uniform(T x) {
   static_assert(sizeof(T) % 4 == 0, "");
@@ -171,7 +173,9 @@ __device__ __forceinline__ T of_lane(T x, int lane) {
 // 104 -> 102); more are spread over the workgroup's threads.
 template <bool F8>
 __device__ __forceinline__ Share share(const PagedArgs& a) {
-  enum { kFewItems = 3, kManyItems, kSums };  // measures of each Kind, numbers of items of few rows (all requests') and of many (such requests')
+  // measures of each Kind, numbers of items of few rows (all requests') and of many (such requests'), and of kAllFew's measures a sum in 256ths that stays
+  // in range whatever starts hold
+  enum { kFewItems = 3, kManyItems, kHigh, kSums };
   __shared__ int s_sums[4][kSums], s_longest[4], s_moved[2];
   __shared__ Place s_place;
   __shared__ Request s_q;
@@ -190,6 +194,7 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     mine[kFew] += few ? m : 0;
     mine[kMany] += few ? 0 : measure(a, q, kMany) * a.n_kv;
     mine[kAllFew] += m;
+    mine[kHigh] = min(mine[kHigh] + (m >> 8), kMostHigh + 1);
     mine[kFewItems] += tiles_of(q, true) * a.n_kv;
     mine[kManyItems] += tiles_of(q, false) * a.n_kv;
     longest = max(longest, q.n == 0 ? 0 : q.length);
@@ -218,6 +223,11 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   }
   longest = alone ? uniform(longest) : uniform(max(max(s_longest[0], s_longest[1]), max(s_longest[2], s_longest[3])));
   const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, per_xcd = a.shares / 8;
+  if (all[kHigh] > kMostHigh) {  // (only of starts that do not ascend, whose requests overlap)
+    Share s = {};
+    s.id = blockIdx.x, s.none_from = a.tokens, s.none_to = a.tokens;
+    return s;
+  }
   const bool all_few = all[kMany] == 0 || (all[kFewItems] <= a.shares && longest <= kShort);
   Share s = {};
   // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
@@ -1264,7 +1274,7 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   a.c = scale * kLog2e;
   const int64_t tiles = n_kv_heads * (static_cast<int64_t>(a.tokens) * group / kFewRows + requests);
   const int64_t keys = std::max<int64_t>(static_cast<int64_t>(a.width) * page_size, a.tokens) + 2 * kManyRows;
-  for (a.shift = 0; a.shift < 30 && tiles * ((keys >> a.shift) + kStartFew + kStartMany) > 0x3fffffff; ++a.shift) {
+  for (a.shift = 0; a.shift < 30 && tiles * ((keys >> a.shift) + kStartFew + kStartMany) > kMostMeasure; ++a.shift) {
   }
   if (a.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
   a.shares = a.blocks = shares();

@@ -743,7 +743,7 @@ def paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, 
     ones, a denoise step's action tokens, a chunk of a prompt, side by side in one call.
 
     q [B, Hq, S, D]; token b S + s of it is numbered so, and request r's queries are tokens starts[r] up to, not including, starts[r + 1] (int32
-    [R + 1], what paged_kv_resize returned; None: request r is row r of q).  Its keys are the first lengths[r] tokens (int32 [R]) of the pages in
+    [R + 1], ascending, what paged_kv_resize returned; None: request r is row r of q).  Its keys are the first lengths[r] tokens (int32 [R]) of the pages in
     page_table[r] (int32 [R, P]), its queries' own among them; with causal=True the queries are the last of these and see up to themselves,
     without all see all.  Tokens of no request and queries that see nothing get zeros; what a query does not see does not influence it whatever it
     holds, and pages outside of the pool are not seen.  Nothing of the tables is read by the host.  Inference only."""
