@@ -14,7 +14,7 @@
 // bf16 keys: 262 MB in 67 us.  Short caches: the chain of loads alone; of 20.5 us for 64 single tokens over 900 keys 2.6 go into the plan,
 // 1.8 to the first keys' request, 2.8 into the one tile a wavefront has, 2.1 into the wavefronts' join, 4 into the parts'.  Chunks: 2048 queries over 16384
 // e4m3 keys 324 us, 0.79 PFLOP/s (the contiguous cache's kernel: 392); a tile of 64 keys takes a SIMD's two wavefronts 5200 cycles, in which
-// their products need 2048 and their other instructions 3600.  16 prompts of 912 bf16 tokens: 101 us, 62 to 102 by the workgroup, whose items are not cut.
+// their products need 2048 and their other instructions 3600.  16 prompts of 912 bf16 tokens: 92 to 97 us, a workgroup to an item.
 #include <algorithm>
 #include <type_traits>
 
