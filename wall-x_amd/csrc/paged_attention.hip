@@ -922,6 +922,16 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
     asm volatile("" : "+v"(rows_here), "+v"(cols_here));
     auto read_k = [&](int i) { return read_rows<D>(tk, 32 * (i % NT), i / NT, rows_here); };
     auto read_v = [&](int i) { return read_cols<D>(tv, 32 * (i / (2 * T::kOut)), i / T::kOut % 2, i % T::kOut, cols_here); };
+    // (Scales are asked for as operands are, ahead: each read where it is used was a wait of its own.  2048 tokens over 16384 keys 348 -> 328 us.)
+    float4 x0[F8 ? 4 : 1], x1[F8 ? 4 : 1];
+    auto read_scales = [&](float4* x, int from) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) x[w] = *reinterpret_cast<const float4*>(scales + from + 8 * w + 4 * h);
+    };
+    auto times = [&](f32x16& s, const float4* x) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) s[4 * w] *= x[w].x, s[4 * w + 1] *= x[w].y, s[4 * w + 2] *= x[w].z, s[4 * w + 3] *= x[w].w;
+    };
     f32x16 s[NT];
     u32x4 f[kAhead];
 #pragma unroll
@@ -936,26 +946,32 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
     for (int i = 0; i < kScores; ++i) {
       s[i % NT] = mfma<DT>(f[i % kAhead], qf[i / NT], s[i % NT]);
       if (i + kAhead < kScores) f[i % kAhead] = read_k(i + kAhead);
+      if (F8 && i + kAhead == kScores) read_scales(x0, 0);
       in_order();
     }
     __builtin_amdgcn_s_setprio(0);
+    if constexpr (F8) {
+      read_scales(x1, 32);
+      in_order();
+      times(s[0], x0);
+    }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) f[i] = read_v(i);
     in_order();
     if constexpr (F8) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(scales + 32 * n + 8 * w + 4 * h);
-          s[n][4 * w] *= x.x, s[n][4 * w + 1] *= x.y, s[n][4 * w + 2] *= x.z, s[n][4 * w + 3] *= x.w;
-        }
+      times(s[1], x1);
+      read_scales(x0, KB);
+      in_order();
     }
     if (ok != ~0ull || k0 + KB > all_see)
 #pragma unroll
       for (int n = 0; n < NT; ++n) hide(s[n], static_cast<uint32_t>(ok >> (32 * n)) & first_bits(row.seen - k0 - 32 * n), h);
     sums.raise(s, a.c);
     const float mc = sums.m == -kInf ? 0.f : sums.m * a.c;
+    if constexpr (F8) {
+      read_scales(x1, KB + 32);
+      in_order();
+    }
     float l[2] = {0.f, 0.f};
     auto power = [&](int n, int r) {  // of registers r and r + 1
       s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.c, -mc));
@@ -963,8 +979,8 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
       l[0] += s[n][r];
       l[1] += s[n][r + 1];
       if constexpr (F8) {
-        const float2 x = *reinterpret_cast<const float2*>(scales + KB + 32 * n + 8 * (r / 4) + 4 * h + r % 4);
-        s[n][r] *= x.x, s[n][r + 1] *= x.y;
+        const float4 x = (n ? x1 : x0)[r / 4];
+        s[n][r] *= r % 4 ? x.z : x.x, s[n][r + 1] *= r % 4 ? x.w : x.y;
       }
     };
 #pragma unroll
