@@ -33,8 +33,9 @@ constexpr int kCut = 64;  // items are cut at multiples of so many keys
 constexpr int kStartFew = 192, kStartMany = 128;
 // The least that a workgroup takes.  With 256 / 512 / 1024: 64 single tokens over 800 to 912 keys 35 / 39 / 48 us (when starts took longer).
 constexpr int kLeast = 256;
-// Tiles of few rows for everything where they are no more than the workgroups and their keys are no more than this: 64 x 32 queries over 800 to 912
-// keys 52 us in tiles of many rows, two workgroups to each, 40 so; 2048 queries over 16384 keys 324 and 390.
+// Tiles of few rows for everything where no request has more keys than this and either every item gets a like number of workgroups (see share()) or there are a
+// quarter as many items as workgroups.  64 x 32 queries over 800 to 912 keys 45 us in tiles of many rows, 35 so; 512 queries over 2012 keys 44 and 40; but 2048
+// queries over themselves 53 and 59 (bf16 keys: 47 and 60), 2 x 1000 over 2000 43 and 47, 4 x 500 37 and 40, 2048 over 16384 keys 324 and 390.
 constexpr int kShort = 2048;
 // An item's end near to a share's end is the share's end: nearer than this in keys, which is about what a cut costs (a start, a part, its
 // join), and than 3/8 of a share.  With 128 / 320: 64 mixed requests 64 / 67 us.  Items of up to half a share are not cut at all: 16 prompts of 912
@@ -228,7 +229,20 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     s.id = blockIdx.x, s.none_from = a.tokens, s.none_to = a.tokens;
     return s;
   }
-  const bool all_few = all[kMany] == 0 || (all[kFewItems] <= a.shares && longest <= kShort);
+  // (quotients of whole numbers by way of floats, which take a tenth of an exact division's instructions: a little more than total / count, ...)
+  auto each_of = [&](int total, int count) {
+    return max(static_cast<int>(static_cast<float>(total) * __builtin_amdgcn_rcpf(static_cast<float>(count)) * 1.000001f) + 2, kLeast >> a.shift);
+  };
+  // Items of about one length, no more than there are workgroups: a like number of workgroups to each, without second items, where the longest
+  // one's parts are no longer than shares are.  64 single tokens over 800 to 912 keys 22.1 -> 20.6 us.
+  const int each_few = each_of(all[kAllFew], a.shares);
+  int parts = 0;
+  if (all[kFewItems] > 0 && all[kFewItems] <= a.shares) {
+    // (... and exact where both are below 1024: the quotient is off by less than 1 / 1024 then, and so far from the next whole number)
+    parts = min(quotient(a.shares, all[kFewItems]), max((longest + kLeast - 1) / kLeast, 1));
+    if (longest >> a.shift > static_cast<int64_t>(each_few) * parts) parts = 0;
+  }
+  const bool all_few = all[kMany] == 0 || (longest <= kShort && (parts != 0 || 4 * all[kFewItems] <= a.shares));
   Share s = {};
   // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
   int p = all_few ? per_xcd : 0;
@@ -240,15 +254,8 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   int count = j < p ? 8 * p : 8 * (per_xcd - p), w = j < p ? xcd * p + j : xcd * (per_xcd - p) + j - p;
   s.id = j < p ? w : 8 * p + w;
   const int total = all_few ? all[kAllFew] : (j < p ? all[kFew] : all[kMany]);
-  // (quotients of whole numbers by way of floats, which take a tenth of an exact division's instructions: a little more than total / count, ...)
-  s.each = uniform(max(static_cast<int>(static_cast<float>(total) * __builtin_amdgcn_rcpf(static_cast<float>(count)) * 1.000001f) + 2, kLeast >> a.shift));
-  // Items of about one length, no more than there are workgroups: a like number of workgroups to each, without second items, where the longest
-  // one's parts are no longer than shares are.  64 single tokens over 800 to 912 keys 22.1 -> 20.6 us.
-  if (all_few && all[kFewItems] > 0 && all[kFewItems] <= a.shares) {
-    // (... and exact where both are below 1024: the quotient is off by less than 1 / 1024 then, and so far from the next whole number)
-    const int parts = min(quotient(a.shares, all[kFewItems]), max((longest + kLeast - 1) / kLeast, 1));
-    if (longest >> a.shift <= static_cast<int64_t>(s.each) * parts) s.parts = uniform(parts);
-  }
+  s.each = uniform(all_few ? each_few : each_of(total, count));
+  if (all_few) s.parts = uniform(parts);
   // Many items of many rows, two and more to a share: a workgroup for each instead, where the launch has as many (an XCD has neighbouring ones), long
   // ones of a request first.  Which of the chip's places takes the next is found as they end: 16 prompts of 912 tokens 105 -> 97 us.
   const int each_xcd = (all[kManyItems] + 7) / 8;
@@ -944,7 +951,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
       s[i % NT] = mfma<DT>(f[i % kAhead], qf[i / NT], s[i % NT]);
       if (i + kAhead < kScores) f[i % kAhead] = read_k(i + kAhead);
       if (F8 && i + kAhead == kScores) read_scales(x0, 0);
-      // (16 bits: the next tile's loads one at a time between the products.  All at once they wait for each other: 16 prompts of 912 tokens 96 -> 93 us.)
+      // (16 bits: the next tile's loads one at a time between the products.  All at once they wait for each other: 16 prompts of 912 tokens 99 -> 97 us.)
 #pragma unroll
       for (int w = 0; !F8 && w < kWork; ++w)
         if (w * kScores / kWork == i && more) fetch(w, other);
