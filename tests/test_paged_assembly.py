@@ -17,4 +17,4 @@ def test_assembly(tmp_path, source):
     assert (len(loops) > 0) == (source == "paged_attention.hip")
     for kernel, loop in loops:
         assert not any("scratch_" in line for line in loop), kernel
-    assert all(int(n) <= 32 for n in re.findall(r"; ScratchSize: (\d+)", text))
+    assert all(int(n) <= 48 for n in re.findall(r"; ScratchSize: (\d+)", text))  # (some words outside of the loops)

@@ -937,6 +937,8 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
     auto read_k = [&](int i) { return read_rows<D>(tk, 32 * (i % NT), i / NT, rows_here); };
     auto read_v = [&](int i) { return read_cols<D>(tv, 32 * (i / (2 * T::kOut)), i / T::kOut % 2, i % T::kOut, cols_here); };
     // (Scales are asked for as operands are, ahead: each read where it is used was a wait of its own.  2048 tokens over 16384 keys 348 -> 328 us.)
+    // (Of fp16 with 128 channels half of them later: together they take registers that there are not, and a reload in the loop.)
+    constexpr bool kLate = kTwice<DT, F8> && D == 128;
     float4 x0[F8 ? 4 : 1], x1[F8 ? 4 : 1];
     auto read_scales = [&](float4* x, int from) {
 #pragma unroll
@@ -969,9 +971,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
     }
     __builtin_amdgcn_s_setprio(0);
     if constexpr (F8) {
-      read_scales(x1, 32);
+      if constexpr (!kLate) read_scales(x1, 32);
       in_order();
       times(s[0], x0);
+      if constexpr (kLate) read_scales(x1, 32);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) f[i] = read_v(i);
@@ -986,7 +989,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
       for (int n = 0; n < NT; ++n) hide(s[n], static_cast<uint32_t>(ok >> (32 * n)) & first_bits(row.seen - k0 - 32 * n), h);
     sums.raise(s, a.c);
     const float mc = sums.m == -kInf ? 0.f : sums.m * a.c;
-    if constexpr (F8) {
+    if constexpr (F8 && !kLate) {
       read_scales(x1, KB + 32);
       in_order();
     }
@@ -1003,6 +1006,11 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
     };
 #pragma unroll
     for (int u = 0; u < 8; ++u) power(0, 2 * u);
+    if constexpr (kLate) {
+      in_order();
+      read_scales(x1, KB + 32);
+      in_order();
+    }
     u32x4 p[2], p2[2];
     auto pack = [&](int n) {
 #pragma unroll
