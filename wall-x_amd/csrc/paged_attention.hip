@@ -10,11 +10,11 @@
 // workgroup whose part is the last to arrive, with stores and loads past the XCDs' L2: 64 x 32 queries 81 us for 52, 8 long requests 42 for 37.)
 //
 // What bounds it.  Single tokens over long caches: memory; 112 MB of 8 requests over 20 to 32 thousand keys stream in some 24 us, 4.7 TB/s, and
-// 6 before and 7 behind that go into the plan, the first pages and keys, and the join: 37 to 39 us in all.  32 requests of up to 5 tokens over up to 16000
+// 6 before and 7 behind that go into the plan, the first pages and keys, and the join: 35 to 40 us in all.  32 requests of up to 5 tokens over up to 16000
 // bf16 keys: 262 MB in 67 us.  Short caches: the chain of loads alone; of 20.5 us for 64 single tokens over 900 keys 2.6 go into the plan,
 // 1.8 to the first keys' request, 2.8 into the one tile a wavefront has, 2.1 into the wavefronts' join, 4 into the parts'.  Chunks: 2048 queries over 16384
-// e4m3 keys 324 us, 0.79 PFLOP/s (the contiguous cache's kernel: 392); a tile of 64 keys takes a SIMD's two wavefronts 5200 cycles, in which
-// their products need 2048 and their other instructions 3600.  16 prompts of 912 bf16 tokens: 92 to 97 us, a workgroup to an item.
+// e4m3 keys 303 us, 0.85 PFLOP/s (the contiguous cache's kernel: 392), bf16 keys 290 (contiguous 313); a tile of 64 keys takes a SIMD's two wavefronts 4800
+// cycles, in which their products need 2048 and their other instructions 3300.  16 prompts of 912 bf16 tokens: 88 to 97 us, a workgroup to an item.
 #include <algorithm>
 #include <type_traits>
 
