@@ -14,7 +14,7 @@
 // bf16 keys: 262 MB in 67 us.  Short caches: the chain of loads alone; of 20.5 us for 64 single tokens over 900 keys 2.6 go into the plan,
 // 1.8 to the first keys' request, 2.8 into the one tile a wavefront has, 2.1 into the wavefronts' join, 4 into the parts'.  Chunks: 2048 queries over 16384
 // e4m3 keys 303 us, 0.85 PFLOP/s (the contiguous cache's kernel: 392), bf16 keys 290 (contiguous 313); a tile of 64 keys takes a SIMD's two wavefronts 4800
-// cycles, in which their products need 2048 and their other instructions 3300.  16 prompts of 912 bf16 tokens: 88 to 97 us, a workgroup to an item.
+// cycles, in which their products need 2048 and their other instructions 3300.  16 prompts of 912 bf16 tokens: 88 to 97 us, a workgroup to an item; 8 of them 48.
 #include <algorithm>
 #include <type_traits>
 
@@ -256,10 +256,11 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   const int total = all_few ? all[kAllFew] : (j < p ? all[kFew] : all[kMany]);
   s.each = uniform(all_few ? each_few : each_of(total, count));
   if (all_few) s.parts = uniform(parts);
-  // Many items of many rows, two and more to a share: a workgroup for each instead, where the launch has as many (an XCD has neighbouring ones), long
-  // ones of a request first.  Which of the chip's places takes the next is found as they end: 16 prompts of 912 tokens 105 -> 97 us.
+  // Many items of many rows, three and more to two shares: a workgroup for each instead, where the launch has as many (an XCD has neighbouring ones), long
+  // ones of a request first.  Which of the chip's places takes the next is found as they end: 16 prompts of 912 tokens 105 -> 97 us, 8 of them 68 -> 48;
+  // from one to a share on 6 prompts 57 and 50, but 5 of 1000 behind as many 103 and 121.
   const int each_xcd = (all[kManyItems] + 7) / 8;
-  if (s.kind == kMany && all[kManyItems] >= 2 * count && each_xcd <= static_cast<int>(gridDim.x >> 3) - p) {
+  if (s.kind == kMany && 2 * all[kManyItems] >= 3 * count && each_xcd <= static_cast<int>(gridDim.x >> 3) - p) {
     s.parts = 1;
     w = j - p < each_xcd ? xcd * each_xcd + j - p : all[kManyItems];
   } else if (j >= per_xcd) {
@@ -1334,7 +1335,7 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   if (a.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
   a.shares = a.blocks = shares();
   const int64_t items = n_kv_heads * (static_cast<int64_t>(a.tokens) * group / kManyRows + requests);  // at most, of many rows
-  if (items >= 2 * a.shares && !too_many_blocks(items + 16 + a.shares, 256)) a.blocks = static_cast<int>((items + 7) / 8 * 8) + a.shares;
+  if (2 * items >= 3 * a.shares && !too_many_blocks(items + 16 + a.shares, 256)) a.blocks = static_cast<int>((items + 7) / 8 * 8) + a.shares;
   a.part_rows = part_rows(a.tokens, group);
   const int64_t rows = 2ll * a.shares * a.part_rows;
   a.sums = static_cast<float*>(workspace);
