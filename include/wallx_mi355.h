@@ -567,8 +567,8 @@ int wx_cached_attention(const void* q, const void* k_cache, const void* v_cache,
  * token its slot and its position in its request, -1 and 0 behind the last.  max_tokens bounds the tokens that are added: of more, starts stays at it and the rest has no
  * slot.  At most 4096 requests, 2^31 - 1 tokens and slots.
  * wx_paged_kv_write puts token b * seq + s of k and v [batch, n_kv_heads, seq, head_dim] (strides as above) into slots[b * seq + s],
- * quantised like wx_kv_cache_write's or, with scales NULL, as it is.  Tokens whose slot is not in [0, num_pages * page_size) are dropped; of
- * two tokens of one slot either may stay. */
+ * quantised like wx_kv_cache_write's or, with scales NULL, as it is.  Tokens whose slot is not in [0, num_pages * page_size) are dropped; what
+ * a slot that two tokens name holds then is unspecified. */
 int wx_paged_kv_resize(const int32_t* lengths, const int32_t* wanted, int32_t* page_table, int32_t* free_pages, const int32_t* free_count,
                        int32_t* new_lengths, int32_t* new_free_count, int32_t* starts, int32_t* slots, int64_t* positions,
                        int64_t requests, int64_t pages_per_request, int64_t free_capacity, int page_size, int64_t max_tokens,

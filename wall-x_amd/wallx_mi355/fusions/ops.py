@@ -726,7 +726,7 @@ def paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots):
     """Writes token b S + s of k and v [B, Hkv, S, D] (bf16 or fp16, through their strides) into slots[b S + s] of the pages in place:
     slot = page * page_size + place.  e4m3 pages take it quantised as kv_cache_write does; with scales None pages of k's dtype take it as it
     is.  slots int32 [B S] or [B, S] on the device, never read by the host; tokens whose slot is outside of the pages (-1: padding) are
-    dropped, the rest of the pages stays as it is.  Not differentiable."""
+    dropped, the rest of the pages stays as it is.  No two tokens may name one slot.  Not differentiable."""
     if _lib.host().paged_write(k, v, k_pages, v_pages, k_scale, v_scale, slots):
         return
     for name, t in (("k", k), ("v", v)):
