@@ -1334,8 +1334,12 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   }
   if (a.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
   a.shares = a.blocks = shares();
-  const int64_t items = n_kv_heads * (static_cast<int64_t>(a.tokens) * group / kManyRows + requests);  // at most, of many rows
-  if (2 * items >= 3 * a.shares && !too_many_blocks(items + 16 + a.shares, 256)) a.blocks = static_cast<int>((items + 7) / 8 * 8) + a.shares;
+  // Room for an item of many rows to a workgroup (see share()), where there may be so many; of more than four to a share (eight where the plan is a wavefront's)
+  // the shares are as good, and a plan over more than 256 requests is too long to be made for an item: 1024 requests of 64 tokens 280 us so, 167 in shares.
+  const int64_t all_rows = static_cast<int64_t>(a.tokens) * group;
+  const int64_t long_ones = starts ? std::min<int64_t>(requests, all_rows / (kFewRows + 1)) : (seq * group > kFewRows ? requests : 0);
+  const int64_t items = long_ones ? n_kv_heads * (all_rows / kManyRows + long_ones) : 0;  // at most
+  if (2 * items >= 3 * a.shares && requests <= 256) a.blocks = static_cast<int>(std::min<int64_t>((items + 7) / 8 * 8 + a.shares, (requests <= 64 ? 8 : 4) * a.shares));
   a.part_rows = part_rows(a.tokens, group);
   const int64_t rows = 2ll * a.shares * a.part_rows;
   a.sums = static_cast<float*>(workspace);
