@@ -278,6 +278,9 @@ def test_rows_are_requests(dev, B, S, D, e4m3):
     ([33] * 20, [40 + 90 * i for i in range(20)]),                   # tiles of few rows alone, lengths far apart
     ([9, 1, 100], [5, 0, 60]),                                       # fewer keys than queries
     ([1], [20000]), ([2] * 3, [9000, 1, 4000]),
+    # items of many rows, 768 to 2048 of them (of up to 64 requests 4096): a workgroup for each; of more, or more requests than 256, shares
+    ([17] * 200, [20 + i for i in range(200)]), ([100] * 60, [100 + 3 * i for i in range(60)]), ([1, 250] * 30, [30, 260] * 30),
+    ([80] * 250, [80 + i % 7 for i in range(250)]), ([17] * 300, [17 + i % 50 for i in range(300)]),
 ])
 @pytest.mark.parametrize("e4m3", [True, False])
 def test_schedules(dev, counts, lengths, e4m3):
