@@ -1,0 +1,87 @@
+"""The paged cache at the edges of what its calls allow: buffers with room for many more tokens than a step has, against the formulas in 64 bits
+(as in test_gpu_paged_cache)."""
+
+import random
+
+import pytest
+import torch
+
+from test_gpu_attention import check
+from test_gpu_paged_cache import ints, pool, prefix, tables, wanted
+from wallx_mi355 import _lib
+from wallx_mi355.fusions import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("counts,lengths,T,Hq,Hkv,D,causal", [
+    ([1] * 16, [912] * 16, 16 * 912, 16, 2, 128, True),                                  # a token each, in equal parts
+    ([1] * 64, [800 + 7 * i % 113 for i in range(64)], 8192, 16, 2, 128, True),
+    ([3, 5, 1, 0] * 8, [700 + i for i in range(32)], 16 * 912, 16, 2, 128, True),        # drafts
+    ([32] * 16, [860 + i for i in range(16)], 16 * 912, 16, 2, 128, False),              # a denoise step's
+    ([1] * 8, [20000 + 700 * i for i in range(8)], 8192, 16, 2, 64, True),               # long contexts
+    ([1] * 63 + [600], [400] * 63 + [1700], 16384, 16, 2, 64, True),                     # a chunk among them: both kinds of items
+    ([1] * 100, [1 + 31 * i % 300 for i in range(100)], 9000, 16, 4, 80, True),          # more requests than a wavefront has lanes
+    ([1] * 32, [500] * 32, 1024, 64, 8, 128, True),
+])
+def test_room_for_more_tokens(dev, counts, lengths, T, Hq, Hkv, D, causal, e4m3):
+    """The launch is as wide as the buffer's items could be; nothing is done twice, or outside of the workspace."""
+    rng, g = random.Random(T), torch.Generator(device=dev).manual_seed(T)
+    ps, pages = 16, sum(-(-n // 16) for n in lengths) + 2
+    cache = pool(pages, Hkv, ps, D, torch.bfloat16, e4m3, g, dev)
+    table = tables(lengths, ps, pages, -(-max(lengths) // ps), rng, dev)
+    starts = prefix(counts)
+    q = torch.randn(1, T, Hq, D, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    want = wanted(q, cache, table, lengths, starts, causal)
+    out = ops.paged_attention(q, *cache, table, ints(lengths, dev), ints(starts, dev), causal=causal)
+    check(out, want, "room")
+    assert not out[0, :, starts[-1]:].any()
+    exact = ops.paged_attention(q[:, :, : starts[-1]], *cache, table, ints(lengths, dev), ints(starts, dev), causal=causal)
+    check(exact, [x[:, :, : starts[-1]] for x in want], "no room")
+    # the same in a workspace of just its size, between others' memory
+    n, guard = _lib.load().wx_paged_attention_workspace_bytes(T, Hq, Hkv, D), 64 << 20
+    work = torch.full((n + 2 * guard,), 0x5A, dtype=torch.uint8, device=dev)
+    again = torch.empty(1, T, Hq, D, dtype=torch.bfloat16, device=dev)
+    k_pages, v_pages, k_scale, v_scale = (None if t is None else t.data_ptr() for t in cache)
+    length, start = ints(lengths, dev), ints(starts, dev)
+    _lib.call("wx_paged_attention", q.data_ptr(), k_pages, v_pages, k_scale, v_scale, again.data_ptr(), table.data_ptr(), length.data_ptr(), start.data_ptr(), int(causal), 1, Hq, Hkv, T,
+              len(lengths), table.size(1), pages, ps, D, _lib.i64x3((0, D, Hq * D)), D ** -0.5, _lib.WX_BF16, work.data_ptr() + guard, n, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(again.transpose(1, 2), out)
+    assert bool((work[:guard] == 0x5A).all()) and bool((work[guard + n:] == 0x5A).all())
+
+
+def test_a_captured_step_with_room_for_prompts(dev):
+    """A step captured with max_tokens of sixteen prompts, replayed by prompts, by single tokens, by drafts and by nothing at all."""
+    g, rng = torch.Generator(device=dev).manual_seed(8), random.Random(8)
+    R, Hq, Hkv, D, ps, pages, T = 16, 16, 2, 128, 16, 1600, 16 * 912
+    state, cache = list(ops.paged_kv_tables(R, 100, pages, dev)), ops.paged_kv_cache(pages, Hkv, ps, D, dev)
+    want_lengths = torch.zeros(R, dtype=torch.int32, device=dev)
+    qkv = torch.randn(1, T, (Hq + 2 * Hkv) * D, generator=g, device=dev).to(torch.bfloat16)
+    q, k, v = (x.view(1, T, -1, D).transpose(1, 2) for x in qkv.split([Hq * D, Hkv * D, Hkv * D], -1))
+
+    def step(state, cache):
+        lengths, table, free, count = state
+        new, left, starts, slots, _ = ops.paged_kv_resize(lengths, want_lengths, table, free, count, ps, T)
+        ops.paged_kv_write(k, v, *cache, slots)
+        out = ops.paged_attention(q, *cache, table, new, starts, causal=True)
+        lengths.copy_(new)
+        count.copy_(left)
+        return out, starts
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step([t.clone() for t in state], [t.clone() for t in cache])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, starts = step(state, cache)
+    held = [0] * R
+    for i, grow in enumerate((lambda r: 912, lambda r: 1, lambda r: 1, lambda r: rng.randint(0, 5), lambda r: 32, lambda r: 0, lambda r: 1 if r else 300, lambda r: 1)):
+        held = [n + grow(r) for r, n in enumerate(held)]
+        qkv.copy_(torch.randn(qkv.shape, generator=g, device=dev))
+        want_lengths.copy_(ints(held, dev))
+        graph.replay()
+        assert state[0].tolist() == held
+        check(out, wanted(q, cache, state[1], held, starts.tolist(), True), f"replay {i}")

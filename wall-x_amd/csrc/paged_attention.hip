@@ -1,13 +1,10 @@
 // Attention of requests' newest tokens over a paged key / value cache: each request has its own number of queries and keys, none of which the
 // host knows (gfx950).
 //
-// Items.  A (request, key / value head, tile of rows) is an item; rows are (query, head of the group) pairs as in attention.h.  Requests of up
-// to 64 rows (single tokens, drafts) are one item a head, others tiles of 128 rows.  Every item has a measure, what it takes in keys: the
-// keys that it sees and some for its start.  The launch is a fixed number of workgroups, two to a CU; each finds the sum of all
-// measures for itself (a prefix sum over the requests) and takes an equal share of it, wherever in an item that begins or ends.  So one request
-// over 32768 keys and 64 over 900 fill the chip alike, without the host and without a plan in memory.  An item that lies in one share is
-// finished there; of one that is cut every share leaves a part (sums, maximum, sum of powers), which a second launch joins, in order.  (Joined by the
-// workgroup whose part is the last to arrive, with stores and loads past the XCDs' L2: 64 x 32 queries 81 us for 52, 8 long requests 42 for 37.)
+// The host knows neither number, so the launch is of a fixed number of workgroups, each of which finds its share of all the work by itself, from
+// the lengths (paged_plan.h): one request over 32768 keys and 64 over 900 fill the chip alike, without the host and without a plan in memory.  What
+// shares leave of items that they cut is joined by a second launch, in order.  (Joined by the workgroup whose part is the last to arrive, with stores and
+// loads past the XCDs' L2: 64 x 32 queries 81 us for 52, 8 long requests 42 for 37.)
 //
 // What bounds it.  Single tokens over long caches: memory; 112 MB of 8 requests over 20 to 32 thousand keys stream in some 24 us, 4.7 TB/s, and
 // 6 before and 7 behind that go into the plan, the first pages and keys, and the join: 35 to 40 us in all.  32 requests of up to 5 tokens over up to 16000
@@ -20,38 +17,14 @@
 
 #include "attention.h"
 #include "common.h"
+#include "paged_plan.h"
 
 namespace wx {
 namespace {
 
+using namespace paged;
+
 #define WX_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
-
-constexpr int kFewLog = 6, kManyLog = 7, kFewRows = 1 << kFewLog, kManyRows = 1 << kManyLog;  // rows of an item of either kind
-constexpr int kCut = 64;  // items are cut at multiples of so many keys
-// What an item takes besides its keys, in keys: about 4.5 us where 64 keys take 1.2 to 2.5.  With 64 / 192 and 128: 64 single tokens over 800 to 912
-// keys 23.5 / 22.0 us, 16 prompts of 912 tokens 123 / 111 (the items at a prompt's beginning are short).
-constexpr int kStartFew = 192, kStartMany = 128;
-// The least that a workgroup takes.  With 256 / 512 / 1024: 64 single tokens over 800 to 912 keys 35 / 39 / 48 us (when starts took longer).
-constexpr int kLeast = 256;
-// Tiles of few rows for everything where no request has more keys than this and either every item gets a like number of workgroups (see share()) or there are a
-// quarter as many items as workgroups.  64 x 32 queries over 800 to 912 keys 45 us in tiles of many rows, 35 so; 512 queries over 2012 keys 44 and 40; but 2048
-// queries over themselves 53 and 59 (bf16 keys: 47 and 60), 2 x 1000 over 2000 43 and 47, 4 x 500 37 and 40, 2048 over 16384 keys 324 and 390.
-constexpr int kShort = 2048;
-// An item's end near to a share's end is the share's end: nearer than this in keys, which is about what a cut costs (a start, a part, its
-// join), and than 3/8 of a share.  With 128 / 320: 64 mixed requests 64 / 67 us.  Items of up to half a share are not cut at all: 16 prompts of 912
-// tokens 113 -> 100 us.
-constexpr int kSnap = 128;
-// What an e4m3 key takes of a tile of many rows, in those of few rows, which take their bytes' time; 16-bit keys take the same.  With 1 / 2 / 3, 62 single tokens
-// and two chunks of 509: heads of 64 in fp16 59 / 53 / 54 us, of 128 in bf16 77 / 66 / 70, of 8 heads of their own with chunks of 200 55 / 44 / 43;
-// 30 tokens over 8 to 16 thousand keys with two chunks of 128 96 / 90 / 91.  Of a bf16 cache 74 / 75 / 86, the long one 105 / 116 / 120.
-constexpr float kManyToFew = 2.f;
-
-struct Part {  // of the item that begins in a share and ends in a later one
-  int parts;   // 0: there is none
-  int head;    // key / value head
-  int first;   // the request's first token
-  int row0, rows;
-};  // (no arrays in it: they are put into LDS, at an address made from the dispatch packet, which lies in host memory: 12 us)
 
 struct PagedArgs {
   const uint16_t* q;               // [batch, n_q, seq, D] through strides; token t is position t % seq of row t / seq
@@ -61,58 +34,17 @@ struct PagedArgs {
   uint16_t* out;                   // [tokens, n_q, D]
   const int32_t *table, *lengths, *starts;  // [requests, width], [requests], [requests + 1] or null: seq tokens each
   int causal, tokens, requests, n_q, n_kv, group, seq, width, page_size, n_pages;
+  int most_keys;                   // width * page_size
   Divider by_seq, by_page, by_group;
   float c;                         // scale * log2(e)
-  int shares, blocks;              // workgroups that take shares, a multiple of 8, and all of them, where each may take an item
-  int shift;                       // measures are in 2^shift keys, so that the sum of all fits 31 bits
+  int shares, blocks, shift;       // see paged_plan.h
   int part_rows;                   // most rows of an item
   float* sums;                     // parts: [2 shares, part_rows, D]
   float2* stats;                   // [2 shares, part_rows] (maximum, sum of powers)
   Part* part;                      // [shares]
+  __device__ __forceinline__ float reciprocal(float x) const { return __builtin_amdgcn_rcpf(x); }
+  __device__ __forceinline__ int uniform(int x) const { return __builtin_amdgcn_readfirstlane(x); }
 };
-
-struct Request {
-  int first, n, length;  // tokens first .. first + n - 1, `length` keys
-  int rows;              // n * group
-};
-__device__ __forceinline__ Request request(const PagedArgs& a, int r) {
-  Request q;
-  if (a.starts != nullptr) {
-    q.first = min(max(a.starts[r], 0), a.tokens);
-    q.n = min(max(a.starts[r + 1], q.first), a.tokens) - q.first;
-  } else {
-    q.first = r * a.seq, q.n = a.seq;
-  }
-  q.length = min(max(a.lengths[r], 0), a.width * a.page_size);
-  q.rows = q.n * a.group;
-  return q;
-}
-// keys that the last of the rows up to `row` sees
-__device__ __forceinline__ int keys_seen(const PagedArgs& a, const Request& q, int row) {
-  return a.causal ? min(max(q.length - q.n + a.by_group.div(row) + 1, 0), q.length) : q.length;
-}
-// Which requests: those of few rows, those of many, or all of them in tiles of few rows.
-enum Kind { kFew, kMany, kAllFew };
-// The items of one head of a request: tile t's measure is base + step (t + 1), which follows the diagonal.
-struct Ramp {
-  int base, step, tiles;
-  __device__ __forceinline__ int before(int t) const { return t * base + static_cast<int>(step * (static_cast<int64_t>(t) * (t + 1) / 2)); }
-  __device__ __forceinline__ int of(int t) const { return base + step * (t + 1); }
-};
-__device__ __forceinline__ int start_of(const PagedArgs& a, bool few) { return max((few ? kStartFew : kStartMany) >> a.shift, 1); }
-__device__ __forceinline__ Ramp ramp(const PagedArgs& a, const Request& q, bool few) {
-  const int log = few ? kFewLog : kManyLog, rows = 1 << log, tiles = (q.rows + rows - 1) >> log;
-  const int step = a.causal && tiles > 1 ? a.by_group.div(rows) >> a.shift : 0;
-  return {((step ? max(q.length - q.n, 0) : q.length) >> a.shift) + start_of(a, few), step, tiles};
-}
-// measure of one head of a request
-__device__ __forceinline__ int measure(const PagedArgs& a, const Request& q, int kind) {
-  if (q.n == 0 || (kind != kAllFew && (q.rows <= kFewRows) != (kind == kFew))) return 0;
-  const Ramp p = ramp(a, q, kind != kMany);
-  return p.before(p.tiles);
-}
-
-constexpr int kMostMeasure = 0x3fffffff, kMostHigh = kMostMeasure >> 8;  // of all requests together (the host chooses `shift` so)
 
 template <class T>
 __device__ __forceinline__ T uniform(T x) {
@@ -125,41 +57,6 @@ __device__ __forceinline__ T uniform(T x) {
   return x;
 }
 
-// A workgroup's share: `size` of its kind's measures, from `x` into tile `tile` of `head` of request r; or part x of that item.
-struct Share {
-  int kind, id;    // id: unique over all kinds
-  int parts;       // not 0: every item is cut in so many parts, a share each
-  int size, each;  // each: what a share of this kind takes
-  int r, head, tile, x;
-  Request q;
-  int none_from, none_to;  // tokens [0, none_from) and [none_to, all) are no request's
-};
-// Where `at` of a request's measure lies, moved to an item's end if that is near.  Returns by how much it was moved.
-struct Place {
-  int head, tile, x;
-};
-__device__ __forceinline__ int snap_of(const PagedArgs& a, int of_item, int each) {
-  const int most = each / 8 * 3;
-  return 2 * of_item <= each ? most : min(most, kSnap >> a.shift);
-}
-__device__ __forceinline__ int locate(const PagedArgs& a, const Request& q, int kind, int at, int each, Place& p) {
-  const Ramp items = ramp(a, q, kind != kMany);
-  const int of_head = items.before(items.tiles);
-  p.head = at / of_head;
-  p.x = at - p.head * of_head;
-  int lo = 0, hi = items.tiles - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (items.before(mid) <= p.x) lo = mid;
-    else hi = mid - 1;
-  }
-  p.tile = lo;
-  p.x -= items.before(lo);
-  const int of_item = items.of(lo), snap = snap_of(a, of_item, each), to = p.x < snap ? 0 : (of_item - p.x < snap ? of_item : p.x), moved = to - p.x;
-  p.x = to;
-  return moved;
-}
-__device__ __forceinline__ int quotient(int x, int y) { return static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y)) + 0x1p-11f); }
 template <class T>
 __device__ __forceinline__ T of_lane(T x, int lane) {
   static_assert(sizeof(T) % 4 == 0, "");
@@ -171,12 +68,9 @@ __device__ __forceinline__ T of_lane(T x, int lane) {
   return x;
 }
 // Up to 64 requests are a wavefront's, and every wavefront finds the share for itself, without a barrier (32 requests of drafts 69 -> 67 us, 16 prompts
-// 104 -> 102); more are spread over the workgroup's threads.
+// 104 -> 102); more are spread over the workgroup's threads.  Tokens [0, none_from) and [none_to, all) are no request's.
 template <bool F8>
-__device__ __forceinline__ Share share(const PagedArgs& a) {
-  // measures of each Kind, numbers of items of few rows (all requests') and of many (such requests'), and of kAllFew's measures a sum in 256ths that stays
-  // in range whatever starts hold
-  enum { kFewItems = 3, kManyItems, kHigh, kSums };
+__device__ __forceinline__ Share share(const PagedArgs& a, int& none_from, int& none_to) {
   __shared__ int s_sums[4][kSums], s_longest[4], s_moved[2];
   __shared__ Place s_place;
   __shared__ Request s_q;
@@ -186,19 +80,10 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
   const int first = min((alone ? lane : tid) * each, a.requests), last = min(first + each, a.requests);
   int mine[kSums] = {}, sum[kSums], longest = 0;
   if (tid == 0) s_moved[0] = 0, s_moved[1] = 0;
-  auto tiles_of = [&](const Request& q, bool few) { return few ? (q.rows + kFewRows - 1) >> kFewLog : (q.rows > kFewRows ? (q.rows + kManyRows - 1) >> kManyLog : 0); };
   Request q = {};
   for (int r = first; r < last; ++r) {
     q = request(a, r);
-    const int m = measure(a, q, kAllFew) * a.n_kv;
-    const bool few = q.rows <= kFewRows;
-    mine[kFew] += few ? m : 0;
-    mine[kMany] += few ? 0 : measure(a, q, kMany) * a.n_kv;
-    mine[kAllFew] += m;
-    mine[kHigh] = min(mine[kHigh] + (m >> 8), kMostHigh + 1);
-    mine[kFewItems] += tiles_of(q, true) * a.n_kv;
-    mine[kManyItems] += tiles_of(q, false) * a.n_kv;
-    longest = max(longest, q.n == 0 ? 0 : q.length);
+    add_request(a, q, mine, longest);
     if (!alone && r == 0) s_none[0] = q.first;
     if (!alone && r == a.requests - 1) s_none[1] = q.first + q.n;
   }
@@ -223,97 +108,39 @@ __device__ __forceinline__ Share share(const PagedArgs& a) {
     all[i] = uniform(w0 + w1 + w2 + s_sums[3][i]);
   }
   longest = alone ? uniform(longest) : uniform(max(max(s_longest[0], s_longest[1]), max(s_longest[2], s_longest[3])));
-  const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, per_xcd = a.shares / 8;
-  if (all[kHigh] > kMostHigh) {  // (only of starts that do not ascend, whose requests overlap)
-    Share s = {};
-    s.id = blockIdx.x, s.none_from = a.tokens, s.none_to = a.tokens;
-    return s;
-  }
-  // (quotients of whole numbers by way of floats, which take a tenth of an exact division's instructions: a little more than total / count, ...)
-  auto each_of = [&](int total, int count) {
-    return max(static_cast<int>(static_cast<float>(total) * __builtin_amdgcn_rcpf(static_cast<float>(count)) * 1.000001f) + 2, kLeast >> a.shift);
-  };
-  // Items of about one length, no more than there are workgroups: a like number of workgroups to each, without second items, where the longest
-  // one's parts are no longer than shares are.  64 single tokens over 800 to 912 keys 22.1 -> 20.6 us.
-  const int each_few = each_of(all[kAllFew], a.shares);
-  int parts = 0;
-  if (all[kFewItems] > 0 && all[kFewItems] <= a.shares) {
-    // (... and exact where both are below 1024: the quotient is off by less than 1 / 1024 then, and so far from the next whole number)
-    parts = min(quotient(a.shares, all[kFewItems]), max((longest + kLeast - 1) / kLeast, 1));
-    if (longest >> a.shift > static_cast<int64_t>(each_few) * parts) parts = 0;
-  }
-  const bool all_few = all[kMany] == 0 || (longest <= kShort && (parts != 0 || 4 * all[kFewItems] <= a.shares));
-  Share s = {};
-  // the kinds' workgroups, a like number of each on every XCD, neighbouring shares on the same
-  int p = all_few ? per_xcd : 0;
-  if (!all_few && all[kFew] != 0) {
-    const float part = static_cast<float>(all[kFew]) / (static_cast<float>(all[kFew]) + (F8 ? kManyToFew : 1.f) * static_cast<float>(all[kMany]));
-    p = uniform(min(max(static_cast<int>(part * per_xcd + 0.5f), 1), per_xcd - 1));
-  }
-  s.kind = all_few ? kAllFew : (j < p ? kFew : kMany);
-  int count = j < p ? 8 * p : 8 * (per_xcd - p), w = j < p ? xcd * p + j : xcd * (per_xcd - p) + j - p;
-  s.id = j < p ? w : 8 * p + w;
-  const int total = all_few ? all[kAllFew] : (j < p ? all[kFew] : all[kMany]);
-  s.each = uniform(all_few ? each_few : each_of(total, count));
-  if (all_few) s.parts = uniform(parts);
-  // Many items of many rows, three and more to two shares: a workgroup for each instead, where the launch has as many (an XCD has neighbouring ones), long
-  // ones of a request first.  Which of the chip's places takes the next is found as they end: 16 prompts of 912 tokens 105 -> 97 us, 8 of them 68 -> 48;
-  // from one to a share on 6 prompts 57 and 50, but 5 of 1000 behind as many 103 and 121.
-  const int each_xcd = (all[kManyItems] + 7) / 8;
-  if (s.kind == kMany && 2 * all[kManyItems] >= 3 * count && each_xcd <= static_cast<int>(gridDim.x >> 3) - p) {
-    s.parts = 1;
-    w = j - p < each_xcd ? xcd * each_xcd + j - p : all[kManyItems];
-  } else if (j >= per_xcd) {
-    w = count;  // (nothing: the launch is wider than the shares for the sake of the items)
-  }
-  int from, to, at, end;
-  const bool few = s.kind != kMany;
-  if (s.parts) {
-    const int item = s.parts == 1 ? w : quotient(w, s.parts), n = few ? all[kFewItems] : all[kManyItems];
-    s.x = w - item * s.parts;
-    s.size = item < n;
-    from = few ? before[kFewItems] : before[kManyItems], to = from + (few ? mine[kFewItems] : mine[kManyItems]), at = item, end = -1;
-  } else {
-    const int64_t at_ = static_cast<int64_t>(w) * s.each;
-    s.size = at_ < total && w < count ? min(total - static_cast<int>(at_), s.each) : 0;
-    from = all_few ? before[kAllFew] : (j < p ? before[kFew] : before[kMany]);
-    to = from + (all_few ? mine[kAllFew] : (j < p ? mine[kFew] : mine[kMany]));
-    at = s.size > 0 ? static_cast<int>(at_) : -1, end = s.size == s.each ? at + s.each : -1;
-  }
+  if (all[kHigh] > kMostHigh) none_from = a.tokens, none_to = a.tokens;
+  Share s = share_of<F8>(a, blockIdx.x, gridDim.x, all, longest);
+  if (all[kHigh] > kMostHigh) return s;
+  const int from = of_share(s, before), to = from + of_share(s, mine);
   Place place = {};
   int moved[2] = {0, 0};
-  if (s.size > 0 && ((from <= at && at < to) || (from <= end && end < to))) {
+  if (s.size > 0 && ((from <= s.at && s.at < to) || (from <= s.end && s.end < to))) {
     int r_from = from;
     for (int r = first; r < last; ++r) {
       if (each > 1) q = request(a, r);
-      const int m = s.parts ? tiles_of(q, few) * a.n_kv : measure(a, q, s.kind) * a.n_kv;
-      if (r_from <= at && at < r_from + m) {
-        if (s.parts) {
-          const int tiles = tiles_of(q, few);
-          place.head = (at - r_from) / tiles, place.tile = tiles - 1 - (at - r_from - place.head * tiles);
-        } else {
-          moved[0] = locate(a, q, s.kind, at - r_from, s.each, place);
-        }
+      const int m = extent(a, s, q);
+      if (r_from <= s.at && s.at < r_from + m) {
+        moved[0] = begin_of(a, s, q, s.at - r_from, place);
         if (!alone) s_moved[0] = moved[0], s_place = place, s_q = q, s_r = r;
       }
       Place end_place;
-      if (r_from <= end && end < r_from + m) {
-        moved[1] = locate(a, q, s.kind, end - r_from, s.each, end_place);
+      if (r_from <= s.end && s.end < r_from + m) {
+        moved[1] = locate(a, q, s.kind, s.end - r_from, s.each, end_place);
         if (!alone) s_moved[1] = moved[1];
       }
       r_from += m;
     }
   }
   if (alone) {  // (the lane that has the request, for the share's begin and for its end; lane 63 has none, or nothing to move)
-    const uint64_t begins = __ballot(from <= at && at < to), ends = __ballot(from <= end && end < to);
+    const uint64_t begins = __ballot(from <= s.at && s.at < to), ends = __ballot(from <= s.end && s.end < to);
     const int l = begins ? __builtin_ctzll(begins) : 0;
     place = of_lane(place, l), s.q = of_lane(q, l), s.r = l;
     moved[0] = __builtin_amdgcn_readlane(moved[0], l), moved[1] = ends ? __builtin_amdgcn_readlane(moved[1], __builtin_ctzll(ends)) : 0;
-    s.none_from = a.requests ? __builtin_amdgcn_readlane(q.first, 0) : a.tokens;
-    s.none_to = a.requests ? __builtin_amdgcn_readlane(q.first + q.n, a.requests - 1) : a.tokens;
+    none_from = a.requests ? __builtin_amdgcn_readlane(q.first, 0) : a.tokens;
+    none_to = a.requests ? __builtin_amdgcn_readlane(q.first + q.n, a.requests - 1) : a.tokens;
   } else {
     __syncthreads();
-    s.none_from = uniform(s_none[0]), s.none_to = uniform(s_none[1]);
+    none_from = uniform(s_none[0]), none_to = uniform(s_none[1]);
     place = uniform(s_place), s.q = uniform(s_q), s.r = uniform(s_r);
     moved[0] = uniform(s_moved[0]), moved[1] = uniform(s_moved[1]);
   }
@@ -368,14 +195,6 @@ __device__ __forceinline__ f32x16 left_of(const f32x16& x) {
   for (int r = 0; r < 16; ++r) y[r] = left_of(x[r]);
   return y;
 }
-
-// One segment: rows row0 .. row0 + rows - 1 of a request over the keys lo .. hi - 1.
-struct Segment {
-  Request q;
-  int r, head, row0, rows, lo, hi;
-  bool whole;  // all of its item: the result itself
-  int slot;    // otherwise its part's place
-};
 
 // This lane's key of a tile: its row in the pages, or that it has none.
 struct KeyRow {
@@ -1112,55 +931,19 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const Segment& g) 
 
 template <int DT, int D, bool F8>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
-  const Share s = share<F8>(a);
-  if (s.none_from > 0 || s.none_to < a.tokens) {
-    const int64_t row = static_cast<int64_t>(a.n_q) * (D / 8), front = s.none_from * row, none = front + (a.tokens - s.none_to) * row;
+  int none_from, none_to;
+  const Share s = share<F8>(a, none_from, none_to);
+  if (none_from > 0 || none_to < a.tokens) {
+    const int64_t row = static_cast<int64_t>(a.n_q) * (D / 8), front = none_from * row, none = front + (a.tokens - none_to) * row;
     for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < none; i += static_cast<int64_t>(gridDim.x) * 256)
-      reinterpret_cast<u32x4*>(a.out)[i < front ? i : i - front + s.none_to * row] = u32x4{0u, 0u, 0u, 0u};
+      reinterpret_cast<u32x4*>(a.out)[i < front ? i : i - front + none_to * row] = u32x4{0u, 0u, 0u, 0u};
   }
-  Part part = {};
-  const bool few = s.kind != kMany;
-  const int tile_rows = few ? kFewRows : kManyRows;
-  int left = s.size, x = s.x, t = s.tile;
-  Segment g;
-  g.r = s.r, g.q = s.q, g.head = s.head;
-  while (left > 0) {
-    const Ramp items = ramp(a, g.q, few);
-    for (; left > 0 && g.head < a.n_kv; ++g.head, t = 0)
-      for (; left > 0 && t < items.tiles; ++t, x = 0) {
-        g.row0 = t * tile_rows;
-        g.rows = min(g.q.rows - g.row0, tile_rows);
-        const int seen = keys_seen(a, g.q, g.row0 + g.rows - 1);
-        int parts = s.parts, take = 1;
-        if (s.parts) {
-          const float each = static_cast<float>(seen) * (1.f / kCut) * __builtin_amdgcn_rcpf(static_cast<float>(s.parts));
-          auto cut = [&](int i) { return i == s.parts ? seen : min(seen, static_cast<int>(each * static_cast<float>(i)) * kCut); };
-          g.lo = cut(x), g.hi = cut(x + 1);
-        } else {
-          const int of_item = items.of(t), start = start_of(a, few);
-          take = min(of_item - x, left);
-          if (take <= 0) continue;  // (a share that begins at an item's end)
-          auto cut = [&](int at) {
-            if (at >= of_item) return seen;
-            const int64_t key = static_cast<int64_t>(max(at - start, 0)) << a.shift;
-            return key < seen ? static_cast<int>(key) / kCut * kCut : seen;
-          };
-          g.lo = cut(x), g.hi = cut(x + take);
-          // (the shares' ends behind this one that are inside of the item and not near its end)
-          parts = take == of_item ? 1 : 2 + (of_item - snap_of(a, of_item, s.each) - take) / s.each;
-        }
-        g.whole = parts == 1;
-        g.slot = 2 * s.id + (x == 0);
-        if (x == 0 && parts > 1) part.parts = parts, part.head = g.head, part.first = g.q.first, part.row0 = g.row0, part.rows = g.rows;
+  const Part part = segments(
+      a, s, [&](int r, int kind) { return next_request(a, r, kind); },
+      [&](bool few, const Segment& g) {
         if (few) few_rows<DT, D, F8>(a, g);
         else many_rows<DT, D, F8>(a, g);
-        left -= take;
-      }
-    if (left <= 0) break;
-    g.r = next_request(a, g.r + 1, s.kind), g.head = 0;
-    if (g.r < 0) break;
-    g.q = request(a, g.r);
-  }
+      });
   if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.shares) a.part[s.id] = part;
 }
 
@@ -1328,18 +1111,11 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   a.seq = static_cast<int>(seq), a.width = num_pages ? static_cast<int>(pages_per_request) : 0, a.page_size = page_size, a.n_pages = static_cast<int>(num_pages);
   a.by_seq = Divider(static_cast<uint32_t>(seq)), a.by_page = Divider(page_size), a.by_group = Divider(group);
   a.c = scale * kLog2e;
-  const int64_t tiles = n_kv_heads * (static_cast<int64_t>(a.tokens) * group / kFewRows + requests);
-  const int64_t keys = std::max<int64_t>(static_cast<int64_t>(a.width) * page_size, a.tokens) + 2 * kManyRows;
-  for (a.shift = 0; a.shift < 30 && tiles * ((keys >> a.shift) + kStartFew + kStartMany) > kMostMeasure; ++a.shift) {
-  }
-  if (a.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
-  a.shares = a.blocks = shares();
-  // Room for an item of many rows to a workgroup (see share()), where there may be so many; of more than four to a share (eight where the plan is a wavefront's)
-  // the shares are as good, and a plan over more than 256 requests is too long to be made for an item: 1024 requests of 64 tokens 280 us so, 167 in shares.
-  const int64_t all_rows = static_cast<int64_t>(a.tokens) * group;
-  const int64_t long_ones = starts ? std::min<int64_t>(requests, all_rows / (kFewRows + 1)) : (seq * group > kFewRows ? requests : 0);
-  const int64_t items = long_ones ? n_kv_heads * (all_rows / kManyRows + long_ones) : 0;  // at most
-  if (2 * items >= 3 * a.shares && requests <= 256) a.blocks = static_cast<int>(std::min<int64_t>((items + 7) / 8 * 8 + a.shares, (requests <= 64 ? 8 : 4) * a.shares));
+  a.most_keys = a.width * page_size;
+  a.shares = shares();
+  const Launch l = launch_of(a.tokens, group, n_kv_heads, requests, seq, a.most_keys, starts != nullptr, a.shares);
+  if (l.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
+  a.shift = l.shift, a.blocks = l.blocks;
   a.part_rows = part_rows(a.tokens, group);
   const int64_t rows = 2ll * a.shares * a.part_rows;
   a.sums = static_cast<float*>(workspace);
