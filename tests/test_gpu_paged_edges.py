@@ -85,3 +85,16 @@ def test_a_captured_step_with_room_for_prompts(dev):
         graph.replay()
         assert state[0].tolist() == held
         check(out, wanted(q, cache, state[1], held, starts.tolist(), True), f"replay {i}")
+
+
+def test_cuts_of_wide_tables(dev):
+    """Tables that could hold 2^30 keys a request, of which some ten thousand are there: measures in hundreds of keys, cuts on items' ends."""
+    rng, g = random.Random(6), torch.Generator(device=dev).manual_seed(6)
+    ps, width, counts, lengths = 65536, 16383, [702, 263, 8, 5, 187, 7], [10691, 11389, 10062, 10170, 11209, 10193]
+    cache = pool(6, 4, ps, 64, torch.bfloat16, True, g, dev)
+    table = tables(lengths, ps, 6, 1, rng, dev)
+    starts = prefix(counts)
+    q = torch.randn(1, starts[-1] + 5, 16, 64, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    wide = torch.cat((table, table.new_full((6, width - 1), -1)), 1)
+    out = ops.paged_attention(q, *cache, wide, ints(lengths, dev), ints(starts, dev), causal=True)
+    check(out, wanted(q, cache, table, lengths, starts, True), "wide")

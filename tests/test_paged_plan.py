@@ -209,6 +209,14 @@ def test_schedules(plan, seed):
     assert sum(launched > case[8] for (launched, _, _), case in zip(done, cases)) > 50 and sum(cut > 0 for *_, cut in done) > 100
 
 
+@pytest.mark.parametrize("seed", range(6))
+def test_schedules_of_wide_tables(plan, seed):
+    """Tables that could hold so many keys that measures are in hundreds of them, and a cut may fall on an item's end to the key."""
+    rng = random.Random(100 + seed)
+    done = plan([random_case(rng, (2 ** 20, 2 ** 25, 2 ** 28, 2 ** 30 - 2 ** 17)) for _ in range(300)])
+    assert sum(cut > 0 for *_, cut in done) > 50
+
+
 def test_requests_that_overlap(plan):
     """More work than requests that ascend can ask for: none of it is begun."""
     R, T = 4600, 4096

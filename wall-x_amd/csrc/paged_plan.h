@@ -220,9 +220,9 @@ struct Place {
   int head, tile, x;
 };
 template <class A>
-WX_PLAN int snap_of(const A& a, int of_item, int each) {
+WX_PLAN int snap_of(const A& a, int of_item, int each) {  // (at least 1: a share's end that is the item's own is no cut in it)
   const int most = each / 8 * 3;
-  return 2 * of_item <= each ? most : min(most, kSnap >> a.shift);
+  return max(2 * of_item <= each ? most : min(most, kSnap >> a.shift), 1);
 }
 template <class A>
 WX_PLAN int locate(const A& a, const Request& q, int kind, int at, int each, Place& p) {
