@@ -217,6 +217,26 @@ def test_schedules_of_wide_tables(plan, seed):
     assert sum(cut > 0 for *_, cut in done) > 50
 
 
+def overlapping(rng, case):
+    """Starts that do not ascend, or lie outside of the tokens."""
+    return (*case[:5], [rng.randint(-5, case[0] + 5) for _ in range(len(case[6]) + 1)], *case[6:])
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_schedules_of_starts_that_descend(plan, seed):
+    """Requests that claim the same tokens: each has its items all the same, or none has any."""
+    rng = random.Random(200 + seed)
+    done = plan([overlapping(rng, random_case(rng, (None, 77, 2 ** 25))) for _ in range(100)])
+    assert sum(working > 0 for _, working, _ in done) > 40
+
+
+def test_more_work_in_tiles_of_many_rows_than_of_few(plan):
+    """Far more queries than keys and 24 heads to a key / value head: a diagonal that tiles of few rows are too short to count."""
+    R, T = 199, 33336
+    case = packed([1], [500] * R, T - 1, group=24, n_kv=8, most_keys=1518)
+    assert plan([(*case[:5], [T // 50 * (r % 50) * (r % 2) for r in range(R + 1)], *case[6:])])
+
+
 def test_requests_that_overlap(plan):
     """More work than requests that ascend can ask for: none of it is begun."""
     R, T = 4600, 4096

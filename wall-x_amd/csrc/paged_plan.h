@@ -119,17 +119,18 @@ WX_PLAN int tiles_of(const Request& q, bool few) {
   return few ? (q.rows + kFewRows - 1) >> kFewLog : (q.rows > kFewRows ? (q.rows + kManyRows - 1) >> kManyLog : 0);
 }
 
-// ---- sums over the requests: measures of each Kind, numbers of items of few rows (all requests') and of many (such requests'), and of kAllFew's
-// measures a sum in 256ths that stays in range whatever starts hold; beside them the longest request
+// ---- sums over the requests: measures of each Kind, numbers of items of few rows (all requests') and of many (such requests'), and of the greater of a
+// request's measures in few rows and in many (whose steps are rounded each for itself) a sum in 256ths that stays in range whatever starts hold; beside them
+// the longest request
 enum { kFewItems = 3, kManyItems, kHigh, kSums };
 template <class A>
 WX_PLAN void add_request(const A& a, const Request& q, int (&sums)[kSums], int& longest) {
-  const int m = measure(a, q, kAllFew) * a.n_kv;
   const bool few = q.rows <= kFewRows;
+  const int m = measure(a, q, kAllFew) * a.n_kv, many = few ? 0 : measure(a, q, kMany) * a.n_kv;
   sums[kFew] += few ? m : 0;
-  sums[kMany] += few ? 0 : measure(a, q, kMany) * a.n_kv;
+  sums[kMany] += many;
   sums[kAllFew] += m;
-  sums[kHigh] = min(sums[kHigh] + (m >> 8), kMostHigh + 1);
+  sums[kHigh] = min(sums[kHigh] + (max(m, many) >> 8), kMostHigh + 1);
   sums[kFewItems] += tiles_of(q, true) * a.n_kv;
   sums[kManyItems] += tiles_of(q, false) * a.n_kv;
   longest = max(longest, q.n == 0 ? 0 : q.length);
