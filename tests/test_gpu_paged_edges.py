@@ -98,3 +98,56 @@ def test_cuts_of_wide_tables(dev):
     wide = torch.cat((table, table.new_full((6, width - 1), -1)), 1)
     out = ops.paged_attention(q, *cache, wide, ints(lengths, dev), ints(starts, dev), causal=True)
     check(out, wanted(q, cache, table, lengths, starts, True), "wide")
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,length", [(9, 5), (64, 40), (100, 60), (300, 170)])
+def test_queries_before_the_first_key(dev, n, length, dtype, e4m3):
+    """More queries than keys: those in front of the first key see nothing and get zeros, whatever the others see."""
+    rng, g = random.Random(n), torch.Generator(device=dev).manual_seed(n)
+    Hq, Hkv, D, ps = 2, 1, 64, 16
+    cache = pool(30, Hkv, ps, D, dtype, e4m3, g, dev)
+    table = tables([length], ps, 30, 20, rng, dev)
+    q = torch.randn(1, n, Hq, D, generator=g, device=dev).to(dtype).transpose(1, 2)
+    value, tol = wanted(q, cache, table, [length], [0, n], True)
+    first = n - length  # the first query that sees a key
+    page = int(table[0, 0])
+    for odd in (float("nan"), float("inf")):
+        bad = [None if t is None else t.clone() for t in cache]
+        if not e4m3:
+            bad[1][page, 0, 0, 5] = odd  # (of e4m3's codes only NaN is not finite)
+        elif odd == float("inf"):
+            bad[3][page, 0, 0] = odd     # a scale
+        else:
+            bad[1].view(torch.uint8)[page, 0, 0, 5] = 0x7F
+        out = ops.paged_attention(q, *bad, table, ints([length], dev), ints([0, n], dev), causal=True)
+        assert not out[0, :, :first].any(), "a query that sees nothing"  # (NaN counts as true)
+        sees = torch.zeros_like(out, dtype=torch.bool)
+        sees[0, :, first:] = True
+        hit = sees.clone() if e4m3 and odd == float("inf") else sees & (torch.arange(D, device=dev) == 5)
+        assert not bool(torch.isfinite(out[hit]).any())
+        check(out.masked_fill(hit, 0), (value.masked_fill(hit, 0), tol), "what is finite")
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,length", [(1, 1), (1, 20), (5, 900), (1, 9000), (70, 200), (300, 3000)])
+def test_a_request_whose_pages_are_all_none(dev, n, length, dtype, e4m3):
+    """Zeros, though the pool's first slot, which another request owns, holds NaN and infinities."""
+    Hq, Hkv, D, ps = 8, 2, 128, 16
+    g = torch.Generator(device=dev).manual_seed(n)
+    cache = pool(3, Hkv, ps, D, dtype, e4m3, g, dev)
+    table = torch.full((2, -(-length // ps)), -1, dtype=torch.int32, device=dev)
+    table[1, 0] = 0
+    q = torch.randn(1, n + 1, Hq, D, generator=g, device=dev).to(dtype).transpose(1, 2)
+    for odd in (float("nan"), float("inf")):
+        for i in range(2):
+            if e4m3:
+                cache[i].view(torch.uint8)[0, :, 0] = 0x7F
+                cache[2 + i][0, :, 0] = odd
+            else:
+                cache[i][0, :, 0] = odd
+        for causal in (True, False):
+            out = ops.paged_attention(q, *cache, table, ints([length, 1], dev), ints([0, n, n + 1], dev), causal=causal)
+            assert not out[0, :, :n].any() and bool(torch.isnan(out[0, :, n]).all())

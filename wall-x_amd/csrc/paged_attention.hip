@@ -233,7 +233,8 @@ __device__ __forceinline__ const uint16_t* query(const PagedArgs& a, const Row& 
 __device__ __forceinline__ int64_t result(const PagedArgs& a, const Row& w, int d) { return (static_cast<int64_t>(w.token) * a.n_q + w.hq) * d; }
 
 // Rows whose sums are not numbers (see Odd, attention.h) again, of 32 of the segment's rows from `first` on those that `again` has a bit for,
-// from memory, with the maximum and the sum that they ended with.
+// from memory, with the maximum and the sum that they ended with.  A row that sees nothing is among them where a tile of its keys, which others see or
+// which are the pool's first in the place of pages that there are none of, holds such values: its sums are zeros here, as its sum of powers is.
 template <int DT, int D, bool F8>
 __device__ __forceinline__ void rows_again(const PagedArgs& a, const Segment& g, int first, uint32_t again, float m, float l) {
   using T = AttnTile<D>;
@@ -299,7 +300,7 @@ __device__ __forceinline__ void rows_again(const PagedArgs& a, const Segment& g,
         add_odd<PT>(sum, odd, seen, zero, t);
       }
     }
-    if (g.whole) store_cols<DT, D>(sum, o, 1.f / l, redo ? a.out + result(a, w, D) : nullptr, lane);
+    if (g.whole) store_cols<DT, D>(sum, o, l == 0.f ? 0.f : 1.f / l, redo ? a.out + result(a, w, D) : nullptr, lane);
     else if (redo) store_sums<D>(sum, o, a.sums + (static_cast<int64_t>(g.slot) * a.part_rows + w.at) * D, lane);
   }
 }
