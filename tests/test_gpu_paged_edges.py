@@ -151,3 +151,25 @@ def test_a_request_whose_pages_are_all_none(dev, n, length, dtype, e4m3):
         for causal in (True, False):
             out = ops.paged_attention(q, *cache, table, ints([length, 1], dev), ints([0, n, n + 1], dev), causal=causal)
             assert not out[0, :, :n].any() and bool(torch.isnan(out[0, :, n]).all())
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,length", [(1, 100), (1, 300), (1, 30000), (40, 9000), (200, 12000)])
+def test_a_value_that_is_none_counts_at_any_distance(dev, n, length, dtype, e4m3):
+    """0 * NaN and 0 * infinity are no numbers: a value whose probability is 0 in 32 bits beside another's counts wherever its request is cut."""
+    Hq, Hkv, D, ps = 8, 2, 128, 64
+    pages = -(-length // ps)
+    cache = list(ops.paged_kv_cache(pages, Hkv, ps, D, dev, *([] if e4m3 else [dtype])))
+    for t in cache[2:] if e4m3 else ():
+        t.fill_(1.0)
+    cache[1].copy_(torch.randn(cache[1].shape, generator=torch.Generator(device=dev).manual_seed(1), device=dev))
+    table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+    q = torch.full((1, n, Hq, D), 8.0, dtype=dtype, device=dev).transpose(1, 2)
+    cache[0][(length - n) // ps, :, (length - n) % ps] = 8.0  # scores 8 * 8 * sqrt(128) = 724 there, 0 elsewhere; all queries see it
+    for odd in ([float("nan")] if e4m3 else [float("nan"), float("inf")]):
+        cache[1][0, 1, 3, 7] = odd
+        out = ops.paged_attention(q, *cache, table, ints([length], dev), ints([0, n], dev), causal=True)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit[0, Hq // 2:, :, 7] = True
+        assert not bool(torch.isfinite(out[hit]).any()) and bool(torch.isfinite(out[~hit]).all())

@@ -958,14 +958,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const int id = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15;
   const Part p = uniform(a.part[id]);
   if (p.parts == 0) return;
-  // (a part that the row sees nothing of has the weight 0 and counts nothing, unless its scores were NaN)
+  // (a part that the row sees nothing of has the weight 0 and sums of 0; what a row does see counts at the weight 0 as well, as NaN if it is not finite)
   auto weight = [&](float2 st, float top) { return st.x == -kInf ? 0.f : __builtin_amdgcn_exp2f((st.x - top) * a.c); };
   auto share_of = [](float2 st, float w) { return st.x == -kInf ? 0.f * st.y : st.y * w; };
   struct Sum {
     float top, l, o[8];
   };
   auto add = [&](Sum& s, float w, const float4& x, const float4& y) {
-    if (w == 0.f) return;
     s.o[0] += x.x * w, s.o[1] += x.y * w, s.o[2] += x.z * w, s.o[3] += x.w * w;
     s.o[4] += y.x * w, s.o[5] += y.y * w, s.o[6] += y.z * w, s.o[7] += y.w * w;
   };
@@ -975,7 +974,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
       float2 st[8];
       float4 x[8], y[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {  // (past the last: the last one's, without weight)
+      for (int u = 0; u < 8; ++u) {  // (past the last: the last one's, not added)
         const int i = min(i0 + u, last - 1);
         const int64_t at = static_cast<int64_t>(i == 0 ? 2 * id + 1 : 2 * (id + i)) * a.part_rows + row;
         st[u] = a.stats[at];
@@ -991,10 +990,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
       const float f = weight(float2{s.top, 0.f}, top);
       s.l = share_of(float2{s.top, s.l}, f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s.o[e] = f == 0.f ? 0.f : s.o[e] * f;
+      for (int e = 0; e < 8; ++e) s.o[e] *= f;
       s.top = top;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
+        if (i0 + u >= last) continue;
         const float w = weight(st[u], top);
         s.l += share_of(st[u], w);
         add(s, w, x[u], y[u]);
