@@ -173,3 +173,39 @@ def test_a_value_that_is_none_counts_at_any_distance(dev, n, length, dtype, e4m3
         hit = torch.zeros_like(out, dtype=torch.bool)
         hit[0, Hq // 2:, :, 7] = True
         assert not bool(torch.isfinite(out[hit]).any()) and bool(torch.isfinite(out[~hit]).all())
+
+
+def both_hosts(monkeypatch):
+    yield "native host"
+    monkeypatch.setattr(_lib, "_host", _lib._NoHost)
+    yield "Python host"
+
+
+def test_derivatives_of_the_pages_are_refused(dev, monkeypatch):
+    """Pages and scales that need gradients or carry tangents, as queries, keys and values that do."""
+    x = torch.randn(1, 2, 3, 64, device=dev).to(torch.bfloat16)
+    table, lengths, starts, slots = ints([[0, 1]], dev), ints([20], dev), ints([0, 3], dev), ints([0, 1, 2], dev)
+    for host in both_hosts(monkeypatch):
+        for dtype in (torch.float8_e4m3fn, torch.bfloat16):
+            cache = ops.paged_kv_cache(2, 2, 16, 64, dev, dtype)
+            attend = lambda c: ops.paged_attention(x, *c, table, lengths, starts, causal=True)  # noqa: E731
+            write = lambda c: ops.paged_kv_write(x, x, *c, slots)  # noqa: E731
+            write(cache)
+            want = attend(cache)
+            for i, t in enumerate(cache):
+                if t is None:
+                    continue
+                needs = [*cache[:i], t.clone().requires_grad_(), *cache[i + 1:]]
+                for call in (attend, write):
+                    with pytest.raises(RuntimeError, match="differentiable"):
+                        call(needs)
+                    with torch.no_grad():
+                        call(needs)
+                assert torch.equal(attend([None if y is None else y.detach() for y in needs]), want), host
+                if dtype == torch.float8_e4m3fn and i < 2:
+                    continue  # (codes carry no tangents)
+                with torch.autograd.forward_ad.dual_level():
+                    dual = [*cache[:i], torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)), *cache[i + 1:]]
+                    for call in (attend, write):
+                        with pytest.raises(RuntimeError, match="forward-mode"):
+                            call(dual)

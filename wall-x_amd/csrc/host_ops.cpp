@@ -341,7 +341,7 @@ bool to_double(PyObject* o, double& v) {
 bool needs_grad(std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
-    if (t->requires_grad()) return true;
+    if (t && t->requires_grad()) return true;
   return false;
 }
 PyObject* wrap_all(const variable_list& v) { return v.size() == 1 ? wrap(v[0]) : pair(v[0], v[1]); }
@@ -689,7 +689,9 @@ PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 7 || !entry.paged_write) return none();
   const at::Tensor *k = plain(args[0]), *v = plain(args[1]), *c[4], *slots = plain(args[6]);
   if (!k || !v || !slots || !rows16(*k) || !rows16(*v) || !attention_type(k->scalar_type()) || !pages_of(args + 2, *k, c)) return none();
-  if (!v->sizes().equals(k->sizes()) || v->scalar_type() != k->scalar_type() || v->device() != k->device() || c[0]->size(1) != k->size(1) || needs_grad({k, v})) return none();
+  if (!v->sizes().equals(k->sizes()) || v->scalar_type() != k->scalar_type() || v->device() != k->device() || c[0]->size(1) != k->size(1) ||
+      needs_grad({k, v, c[0], c[1], c[2], c[3]}))
+    return none();
   const int64_t B = k->size(0), S = k->size(2);
   if (!(is_ints(slots, 1, *k) && slots->size(0) == B * S) && !(is_ints(slots, 2, *k) && slots->size(0) == B && slots->size(1) == S)) return none();
   const bool ok = run(*k, [&] {
@@ -712,7 +714,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   double scale = 1.0 / std::sqrt(static_cast<double>(q->size(3)));
   if (args[9] != Py_None && !to_double(args[9], scale)) return none();
   const int64_t B = q->size(0), Hq = q->size(1), S = q->size(2), D = q->size(3), Hk = c[0]->size(1), R = table->size(0);
-  if (!heads_fit(Hq, Hk) || lengths->size(0) != R || (starts ? !is_ints(starts, 1, *q) || starts->size(0) != R + 1 : R != B) || needs_grad({q})) return none();
+  if (!heads_fit(Hq, Hk) || lengths->size(0) != R || (starts ? !is_ints(starts, 1, *q) || starts->size(0) != R + 1 : R != B) ||
+      needs_grad({q, c[0], c[1], c[2], c[3]}))
+    return none();
   at::Tensor out;
   const bool ok = run(*q, [&] {
     out = token_major(B, Hq, S, D, q->options());

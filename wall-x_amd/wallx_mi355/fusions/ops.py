@@ -482,6 +482,14 @@ def _no_tangents(op, *tensors):
             raise RuntimeError(f"{op} is not differentiable in forward-mode: its inputs may not carry tangents")
 
 
+def _no_derivatives(op, *tensors):
+    """Both kinds: of the tensors that there are none may need a gradient or carry a tangent."""
+    tensors = [t for t in tensors if t is not None]
+    _no_tangents(op, *tensors)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op} is not differentiable: call it under torch.no_grad() or on detached tensors")
+
+
 class _NoSecond(torch.autograd.Function):
     """The gradients of a backward pass that is not differentiable itself, in a graph of gradients (create_graph): results of a node
     that hangs on everything they were made from and raises where a second derivative is asked through it."""
@@ -726,15 +734,14 @@ def paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots):
     """Writes token b S + s of k and v [B, Hkv, S, D] (bf16 or fp16, through their strides) into slots[b S + s] of the pages in place:
     slot = page * page_size + place.  e4m3 pages take it quantised as kv_cache_write does; with scales None pages of k's dtype take it as it
     is.  slots int32 [B S] or [B, S] on the device, never read by the host; tokens whose slot is outside of the pages (-1: padding) are
-    dropped, the rest of the pages stays as it is.  No two tokens may name one slot.  Not differentiable."""
+    dropped, the rest of the pages stays as it is.  No two tokens may name one slot.  Not differentiable: tokens, pages and scales that
+    need a gradient or carry a tangent are refused."""
     if _lib.host().paged_write(k, v, k_pages, v_pages, k_scale, v_scale, slots):
         return
     for name, t in (("k", k), ("v", v)):
         if t.is_cpu:
             raise RuntimeError(f"[Error] The input `{name}` of paged_kv_write op is on the device: CPU!")
-    _no_tangents("paged_kv_write", k, v)
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
-        raise RuntimeError("paged_kv_write is not differentiable: call it under torch.no_grad() or on detached tensors")
+    _no_derivatives("paged_kv_write", k, v, k_pages, v_pages, k_scale, v_scale)
     backend.paged_kv_write(k, v, k_pages, v_pages, k_scale, v_scale, slots)
 
 
@@ -746,15 +753,14 @@ def paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, 
     [R + 1], ascending, what paged_kv_resize returned; None: request r is row r of q).  Its keys are the first lengths[r] tokens (int32 [R]) of the pages in
     page_table[r] (int32 [R, P]), its queries' own among them; with causal=True the queries are the last of these and see up to themselves,
     without all see all.  Tokens of no request and queries that see nothing get zeros; what a query does not see does not influence it whatever it
-    holds, and pages outside of the pool are not seen.  Nothing of the tables is read by the host.  Inference only."""
+    holds, and pages outside of the pool are not seen.  Nothing of the tables is read by the host.  Inference only: queries, pages and scales that
+    need a gradient or carry a tangent are refused."""
     made = _lib.host().paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts, causal, scale)
     if made is not None:
         return made
     if q.is_cpu:
         raise RuntimeError("[Error] The input `q` of paged_attention op is on the device: CPU!")
-    _no_tangents("paged_attention", q)
-    if torch.is_grad_enabled() and q.requires_grad:
-        raise RuntimeError("paged_attention is not differentiable: call it under torch.no_grad() or on detached tensors")
+    _no_derivatives("paged_attention", q, k_pages, v_pages, k_scale, v_scale)
     return backend.paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, lengths, starts, causal, scale)
 
 
