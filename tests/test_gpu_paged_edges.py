@@ -209,3 +209,21 @@ def test_derivatives_of_the_pages_are_refused(dev, monkeypatch):
                     for call in (attend, write):
                         with pytest.raises(RuntimeError, match="forward-mode"):
                             call(dual)
+
+
+@pytest.mark.parametrize("max_tokens", [0, 5, 4096])
+def test_resize_results_own_their_memory(dev, monkeypatch, max_tokens):
+    """Each result alone in its memory, in both hosts: growing one leaves the others, saving one saves it alone."""
+    for host in both_hosts(monkeypatch):
+        lengths, table, free, count = ops.paged_kv_tables(3, 4, 12, dev)
+        got = ops.paged_kv_resize(lengths, ints([1, 0, 4], dev), table, free, count, 16, max_tokens)
+        for x in got:
+            assert x.untyped_storage().nbytes() == x.numel() * x.element_size() and x.storage_offset() == 0 and x._base is None, host
+        assert len({x.untyped_storage().data_ptr() for x in got if x.numel()}) == sum(x.numel() > 0 for x in got)
+        before = [x.clone() for x in got]
+        for i, x in enumerate(got):
+            x.resize_(x.numel() + 100)[before[i].numel():].fill_(-9)
+            assert all(torch.equal(y[: z.numel()], z) for y, z in zip(got, before)), host
+        side = torch.cuda.Stream()
+        for x in got:
+            x.record_stream(side)

@@ -645,16 +645,9 @@ PyObject* paged_resize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (wanted->size(0) != R || table->size(0) != R || count->size(0) != 1 || page_size <= 0 || page_size > INT32_MAX || max_tokens < 0) return none();
   at::Tensor out[5];
   const bool ok = run(*lengths, [&] {
-    // (one allocation for the five, each at a place of its own in it: five take 2 us of 9)
+    // (an allocation each: as parts of one, 4.3 us a call for 6.1, each grew over its neighbours and kept them)
     const int64_t sizes[5] = {R, 1, R + 1, max_tokens, max_tokens};
-    int64_t place[6] = {};
-    for (int i = 0; i < 5; ++i) place[i + 1] = place[i] + (sizes[i] * (i < 4 ? 4 : 8) + 63) / 64 * 64;
-    const at::Tensor all = at::empty({place[5]}, lengths->options().dtype(at::kByte));
-    for (int i = 0; i < 5; ++i) {
-      out[i] = at::detail::make_tensor<at::TensorImpl>(at::Storage(all.storage()), all.key_set(), caffe2::TypeMeta::fromScalarType(i < 4 ? at::kInt : at::kLong));
-      out[i].unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
-      out[i].unsafeGetTensorImpl()->set_storage_offset(place[i] / (i < 4 ? 4 : 8));
-    }
+    for (int i = 0; i < 5; ++i) out[i] = at::empty({sizes[i]}, i < 4 ? lengths->options() : lengths->options().dtype(at::kLong));
     auto to = [&](int i) { return static_cast<int32_t*>(ptr(out[i])); };
     return entry.paged_resize(ints(*lengths), ints(*wanted), static_cast<int32_t*>(ptr(*table)), static_cast<int32_t*>(ptr(*stack)), ints(*count), to(0), to(1), to(2),
                               to(3), static_cast<int64_t*>(ptr(out[4])), R, table->size(1), stack->size(0), static_cast<int>(page_size), max_tokens, stream_of(*lengths));
