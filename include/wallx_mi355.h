@@ -564,8 +564,10 @@ int wx_cached_attention(const void* q, const void* k_cache, const void* v_cache,
  * new_lengths int32 [requests] and new_free_count int32 [1] are written, lengths and free_count are not (no buffer may be two of them); in
  * page_table and free_pages only entries behind what is owned and free before are: the same call again does the same.  starts int32
  * [requests + 1]: where each request's added tokens begin among all of them; slots int32 and positions int64 [max_tokens] (16-byte aligned): of each added
- * token its slot and its position in its request, -1 and 0 behind the last.  max_tokens bounds the tokens that are added: of more, starts stays at it and the rest has no
- * slot.  At most 4096 requests, 2^31 - 1 tokens and slots.
+ * token its slot and its position in its request, -1 and 0 behind the last.  max_tokens is the most that may be added: of more, starts stays at it and the rest has no
+ * slot, though new_lengths counts it and it has pages.  Such a call's results are not for wx_paged_attention, which takes a request's tokens for its
+ * newest ones; starts[requests] below the sum of what new_lengths has over lengths tells, and the same call with a larger max_tokens does it right.
+ * At most 4096 requests, 2^31 - 1 tokens and slots.
  * wx_paged_kv_write puts token b * seq + s of k and v [batch, n_kv_heads, seq, head_dim] (strides as above) into slots[b * seq + s],
  * quantised like wx_kv_cache_write's or, with scales NULL, as it is.  Tokens whose slot is not in [0, num_pages * page_size) are dropped; what
  * a slot that two tokens name holds then is unspecified. */

@@ -227,3 +227,16 @@ def test_resize_results_own_their_memory(dev, monkeypatch, max_tokens):
         side = torch.cuda.Stream()
         for x in got:
             x.record_stream(side)
+
+
+def test_more_tokens_than_max_tokens(dev):
+    """They show in starts, and the call made again with room for them is as if it had been the first."""
+    for wanted_ in ([9, 3, 40, 0], [9, 3, 1000, 30]):  # (of 12 pages; of more than there are)
+        state, other = ops.paged_kv_tables(4, 20, 12, dev), ops.paged_kv_tables(4, 20, 12, dev)
+        short = ops.paged_kv_resize(state[0], ints(wanted_, dev), *state[1:], 4, 11)
+        grown = int((short[0] - state[0]).clamp(min=0).sum())
+        assert int(short[2][-1]) == 11 < grown and int((short[3] >= 0).sum()) == 11
+        again, first = (ops.paged_kv_resize(s[0], ints(wanted_, dev), *s[1:], 4, 60) for s in (state, other))
+        assert all(torch.equal(a, b) for a, b in zip(again, first)) and int(again[2][-1]) == grown
+        for r, n in enumerate(again[0].tolist()):  # (what a request owns)
+            assert torch.equal(state[1][r, : -(-n // 4)], other[1][r, : -(-n // 4)])

@@ -719,8 +719,9 @@ def paged_kv_resize(lengths, wanted, page_table, free_pages, free_count, page_si
     new lengths and count over, a call can be made again and does the same.  free_pages is a stack that has room for all pages: the first page
     freed (by request, then by place) is the first taken, and a growth that is taken back leaves it as it was.  Where pages do not suffice, a
     request gets the tokens that it has pages for, in the requests' order: compare lengths with wanted.  max_tokens is the most that
-    is added (in checked mode, native.set_checked, more raises; otherwise the rest has no slot).  One launch, nothing read by the host; at
-    most 4096 requests."""
+    may be added: in checked mode (native.set_checked) more raises.  Otherwise the rest has no slot, though lengths count it, and such results are not for
+    paged_attention, which takes a request's tokens for its newest: starts[R] < (new - old lengths).clamp(min=0).sum() tells, and the call made again with a
+    larger max_tokens does it right.  One launch, nothing read by the host; at most 4096 requests."""
     made = None if native.is_checked() else _lib.host().paged_resize(lengths, wanted, page_table, free_pages, free_count, page_size, max_tokens)
     if made is not None:
         return made
