@@ -14,6 +14,21 @@ from wallx_mi355.fusions import ops
 pytestmark = pytest.mark.gpu
 
 
+def guarded(q, cache, table, lengths, starts, causal):
+    """The call in a workspace of just its size and with a result of its own, both between other memory, which stays as it is."""
+    _, Hq, T, D = q.shape
+    pages, Hkv, ps, _ = cache[0].shape
+    guard, n, size = 64 << 20, _lib.load().wx_paged_attention_workspace_bytes(T, Hq, Hkv, D), T * Hq * D * 2
+    work, out = (torch.full((x + 2 * guard,), 0x5A, dtype=torch.uint8, device=q.device) for x in (n, size))
+    k_pages, v_pages, k_scale, v_scale = (None if t is None else t.data_ptr() for t in cache)
+    _lib.call("wx_paged_attention", q.data_ptr(), k_pages, v_pages, k_scale, v_scale, out.data_ptr() + guard, table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), int(causal), 1, Hq,
+              Hkv, T, lengths.numel(), table.size(1), pages, ps, D, _lib.i64x3((0, q.stride(1), q.stride(2))), D ** -0.5, _lib.WX_BF16, work.data_ptr() + guard, n,
+              torch.cuda.current_stream().cuda_stream)
+    for buffer, x in ((work, n), (out, size)):
+        assert bool((buffer[:guard] == 0x5A).all()) and bool((buffer[guard + x:] == 0x5A).all())
+    return out[guard: guard + size].view(torch.bfloat16).view(1, T, Hq, D).transpose(1, 2)
+
+
 @pytest.mark.parametrize("e4m3", [True, False])
 @pytest.mark.parametrize("counts,lengths,T,Hq,Hkv,D,causal", [
     ([1] * 16, [912] * 16, 16 * 912, 16, 2, 128, True),                                  # a token each, in equal parts
@@ -39,16 +54,7 @@ def test_room_for_more_tokens(dev, counts, lengths, T, Hq, Hkv, D, causal, e4m3)
     assert not out[0, :, starts[-1]:].any()
     exact = ops.paged_attention(q[:, :, : starts[-1]], *cache, table, ints(lengths, dev), ints(starts, dev), causal=causal)
     check(exact, [x[:, :, : starts[-1]] for x in want], "no room")
-    # the same in a workspace of just its size, between others' memory
-    n, guard = _lib.load().wx_paged_attention_workspace_bytes(T, Hq, Hkv, D), 64 << 20
-    work = torch.full((n + 2 * guard,), 0x5A, dtype=torch.uint8, device=dev)
-    again = torch.empty(1, T, Hq, D, dtype=torch.bfloat16, device=dev)
-    k_pages, v_pages, k_scale, v_scale = (None if t is None else t.data_ptr() for t in cache)
-    length, start = ints(lengths, dev), ints(starts, dev)
-    _lib.call("wx_paged_attention", q.data_ptr(), k_pages, v_pages, k_scale, v_scale, again.data_ptr(), table.data_ptr(), length.data_ptr(), start.data_ptr(), int(causal), 1, Hq, Hkv, T,
-              len(lengths), table.size(1), pages, ps, D, _lib.i64x3((0, D, Hq * D)), D ** -0.5, _lib.WX_BF16, work.data_ptr() + guard, n, torch.cuda.current_stream().cuda_stream)
-    assert torch.equal(again.transpose(1, 2), out)
-    assert bool((work[:guard] == 0x5A).all()) and bool((work[guard + n:] == 0x5A).all())
+    assert torch.equal(guarded(q, cache, table, ints(lengths, dev), ints(starts, dev), causal), out)
 
 
 def test_a_captured_step_with_room_for_prompts(dev):
@@ -240,3 +246,36 @@ def test_more_tokens_than_max_tokens(dev):
         assert all(torch.equal(a, b) for a, b in zip(again, first)) and int(again[2][-1]) == grown
         for r, n in enumerate(again[0].tolist()):  # (what a request owns)
             assert torch.equal(state[1][r, : -(-n // 4)], other[1][r, : -(-n // 4)])
+
+
+def test_nothing_to_attend_to_in_pages_that_hold_something(dev):
+    g = torch.Generator(device=dev).manual_seed(2)
+    q = torch.randn(1, 9, 4, 64, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    none, zero = torch.zeros(0, 5, dtype=torch.int32, device=dev), ints([[0]] * 3, dev)
+    for e4m3 in (True, False):
+        cache = pool(3, 2, 16, 64, torch.bfloat16, e4m3, g, dev)
+        for causal in (True, False):
+            attend = lambda *args: ops.paged_attention(q, *cache, *args, causal=causal)  # noqa: E731
+            assert attend(ints([[0]], dev), ints([9], dev)).any()
+            assert not attend(none, ints([], dev), ints([4], dev)).any()                                                      # no requests
+            assert not attend(zero, ints([0, -5, 0], dev), ints([0, 4, 4, 9], dev)).any()                                     # no keys
+            assert not attend(zero, ints([9, 9, 9], dev), ints([4, 4, 4, 4], dev)).any()                                      # no queries
+            assert not attend(torch.zeros(3, 0, dtype=torch.int32, device=dev), ints([9, 9, 9], dev), ints([0, 4, 4, 9], dev)).any()  # no pages to a request
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_requests_that_claim_the_same_tokens(dev, e4m3):
+    """Whatever stands in their tokens, nothing else is written; of more work than any requests that ascend can ask for nothing is done."""
+    rng, g = random.Random(3), torch.Generator(device=dev).manual_seed(3)
+    cache = pool(40, 1, 16, 64, torch.bfloat16, e4m3, g, dev)
+    for R, T, Hq, most in ((7, 300, 2, 500), (200, 4096, 8, 2000), (60, 9000, 4, 90), (600, 700, 1, 600)):
+        table = torch.randint(0, 40, (R, most // 16 + 1), generator=g, device=dev).to(torch.int32)
+        lengths, starts = ([rng.randint(0, most) for _ in range(R)], [rng.randint(-3, T + 3) for _ in range(R + 1)])
+        q = torch.randn(1, T, Hq, 64, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+        for causal in (True, False):
+            guarded(q, cache, table, ints(lengths, dev), ints(starts, dev), causal)
+    R, T, width = 4600, 4096, 512
+    q = torch.randn(1, T, 1, 64, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    args = (torch.zeros(R, width, dtype=torch.int32, device=dev), ints([width * 16] * R, dev))
+    assert guarded(q, cache, *args, ints([min(r, T) for r in range(R + 1)], dev), False).any()
+    assert not guarded(q, cache, *args, ints([T * (r % 2) for r in range(R + 1)], dev), False).any()
