@@ -279,3 +279,61 @@ def test_requests_that_claim_the_same_tokens(dev, e4m3):
     args = (torch.zeros(R, width, dtype=torch.int32, device=dev), ints([width * 16] * R, dev))
     assert guarded(q, cache, *args, ints([min(r, T) for r in range(R + 1)], dev), False).any()
     assert not guarded(q, cache, *args, ints([T * (r % 2) for r in range(R + 1)], dev), False).any()
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("n", [2, 70])
+def test_pools_of_more_than_2_32_values(dev, n, e4m3):
+    """Pages on either side of 2^31 and 2^32 values into the pool, written through slots and read."""
+    Hq, Hkv, D, ps, dtype = 8, 4, 128, 256, torch.bfloat16
+    pages, g = 2 ** 32 // (Hkv * D * ps) + 9, torch.Generator(device=dev).manual_seed(n)
+    cache = [torch.empty(pages, Hkv, ps, D, dtype=torch.float8_e4m3fn if e4m3 else dtype, device=dev) for _ in range(2)]
+    cache += [torch.empty(pages, Hkv, ps, dtype=torch.float32, device=dev) if e4m3 else None for _ in range(2)]
+    half = pages // 2
+    table, lengths = ints([[pages - 1, half, 3], [half - 6, pages - 9, pages - 3]], dev), [700, 513]
+    at = torch.arange(max(lengths), device=dev)
+    slots = torch.cat([table[r].long()[at[:x] // ps] * ps + at[:x] % ps for r, x in enumerate(lengths)]).to(torch.int32)
+    k, v = (torch.randn(1, slots.numel(), Hkv, D, generator=g, device=dev).to(dtype).transpose(1, 2) for _ in range(2))
+    ops.paged_kv_write(k, v, *cache, slots)
+    own = [None if t is None else t[table.flatten().long()] for t in cache]
+    small = torch.arange(6, dtype=torch.int32, device=dev).view(2, 3)
+    q = torch.randn(1, 2 * n, Hq, D, generator=g, device=dev).to(dtype).transpose(1, 2)
+    out = ops.paged_attention(q, *cache, table, ints(lengths, dev), ints([0, n, 2 * n], dev), causal=True)
+    check(out, wanted(q, own, small, lengths, [0, n, 2 * n], True), "large pool")
+    flat = torch.cat([own[1][r * 3 + at[:x] // ps, :, at[:x] % ps].double() * (own[3][r * 3 + at[:x] // ps, :, at[:x] % ps].double()[..., None] if e4m3 else 1) for r, x in enumerate(lengths)])
+    # (e4m3: a code is off by half a step, 2^-4 of the value or, below the least normal code, 2^-10 of the scale, a 448th of a row's largest value, which is below 8)
+    assert bool(((flat - v[0].transpose(0, 1).double()).abs() <= (v[0].transpose(0, 1).double().abs() * 2 ** -4 + 2 ** -10 * 8 / 448 if e4m3 else 0)).all())
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(1024, 1), (100, 1), (66, 2)])
+def test_many_query_heads_to_a_key_head(dev, Hq, Hkv):
+    """Groups of more heads than a tile has rows."""
+    rng, g = random.Random(Hq), torch.Generator(device=dev).manual_seed(Hq)
+    counts, lengths = [1, 2, 0, 3], [70, 1300, 9, 200]
+    cache = pool(120, Hkv, 16, 64, torch.bfloat16, True, g, dev)
+    table, starts = tables(lengths, 16, 120, 90, rng, dev), prefix(counts)
+    q = torch.randn(1, 7, Hq, 64, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    for causal in (True, False):
+        out = ops.paged_attention(q, *cache, table, ints(lengths, dev), ints(starts, dev), causal=causal)
+        check(out, wanted(q, cache, table, lengths, starts, causal), "group")
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("n", [3, 100])
+def test_queries_that_are_no_numbers(dev, n, e4m3):
+    """A query of NaN is its own affair; queries that lie in memory as one do, seen through strides of 0, are many."""
+    rng, g = random.Random(n), torch.Generator(device=dev).manual_seed(n)
+    lengths, starts = [n + 500, n + 30], [0, n, 2 * n]
+    cache = pool(120, 2, 16, 128, torch.bfloat16, e4m3, g, dev)
+    table = tables(lengths, 16, 120, 60, rng, dev)
+    q = torch.randn(1, 2 * n, 8, 128, generator=g, device=dev).to(torch.bfloat16).transpose(1, 2)
+    args = (*cache, table, ints(lengths, dev), ints(starts, dev))
+    clean = ops.paged_attention(q, *args, causal=True)
+    odd = q.clone()
+    odd[0, 2, 1, 7], odd[0, 5, n, 0] = float("nan"), float("nan")
+    out = ops.paged_attention(odd, *args, causal=True)
+    assert bool(torch.isnan(out[0, 2, 1]).all()) and bool(torch.isnan(out[0, 5, n]).all())
+    out[0, 2, 1], out[0, 5, n] = clean[0, 2, 1], clean[0, 5, n]
+    assert torch.equal(out, clean)
+    same = q[:, :1, :1].expand(1, 8, 2 * n, 128)
+    assert torch.equal(ops.paged_attention(same, *args, causal=True), ops.paged_attention(same.contiguous(), *args, causal=True))

@@ -217,6 +217,17 @@ def test_schedules_of_wide_tables(plan, seed):
     assert sum(cut > 0 for *_, cut in done) > 50
 
 
+def test_schedules_of_many_query_heads_to_a_key_head(plan):
+    """Rows of one query in several tiles; a diagonal that tiles are too short to count."""
+    rng = random.Random(300)
+    cases = []
+    for _ in range(300):
+        counts = [rng.choice([0, 1, 1, 2, 5]) for _ in range(rng.randint(1, 12))]
+        lengths = [n + int(2 ** rng.uniform(0, 14)) for n in counts]
+        cases.append(packed(counts, lengths, rng.choice([0, 3, 200]), 0, rng.choice([65, 100, 130, 1024]), rng.choice([1, 2]), rng.random() < 0.7, None, 512, rng.random() < 0.5, rng.choice([-1, 0, 1])))
+    plan(cases)
+
+
 def overlapping(rng, case):
     """Starts that do not ascend, or lie outside of the tokens."""
     return (*case[:5], [rng.randint(-5, case[0] + 5) for _ in range(len(case[6]) + 1)], *case[6:])

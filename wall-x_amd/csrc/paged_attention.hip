@@ -1115,7 +1115,7 @@ extern "C" int wx_paged_attention(const void* q, const void* k_pages, const void
   a.most_keys = a.width * page_size;
   a.shares = shares();
   const Launch l = launch_of(a.tokens, group, n_kv_heads, requests, seq, a.most_keys, starts != nullptr, a.shares);
-  if (l.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests", who);
+  if (l.shift == 30) return fail(WX_ERR_UNSUPPORTED, "%s: too many requests or rows", who);
   a.shift = l.shift, a.blocks = l.blocks;
   a.part_rows = part_rows(a.tokens, group);
   const int64_t rows = 2ll * a.shares * a.part_rows;
