@@ -584,7 +584,8 @@ int wx_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages
  * the queries are its newest tokens, whose keys are in the cache.  Lengths count up to what a row of the table holds; keys in pages outside
  * of [0, num_pages) are not seen; starts ascend and are clamped to the tokens that there are.  out [batch, seq, n_q_heads, head_dim],
  * contiguous; tokens in front of the first request and behind the last and queries that see nothing get zeros.  Where starts descend, requests
- * claim the same tokens: what out holds then is unspecified, and nothing else is touched. */
+ * claim the same tokens: what out holds then is unspecified, and nothing else is touched.  Up to 2^30 - 1 rows and keys of a request and 2^31 - 1
+ * slots, and 3.3 million requests and tiles of 64 rows times key / value heads. */
 size_t wx_paged_attention_workspace_bytes(int64_t tokens, int n_q_heads, int n_kv_heads, int head_dim);
 int wx_paged_attention(const void* q, const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, void* out,
                        const int32_t* page_table, const int32_t* lengths, const int32_t* starts, int causal, int64_t batch, int n_q_heads,
