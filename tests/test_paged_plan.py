@@ -252,3 +252,40 @@ def test_requests_that_overlap(plan):
     """More work than requests that ascend can ask for: none of it is begun."""
     R, T = 4600, 4096
     assert plan([(T, T, 1, 1, False, [T * (r % 2) for r in range(R + 1)], [8192] * R, 8192, 512, True, 0)]) == [(512, 0, 0)]
+
+
+LAUNCHES = r"""
+#include <cstdio>
+#include "paged_plan.h"
+int main() {
+  long long tokens, requests, seq, most_keys;
+  int group, n_kv, has_starts;
+  while (std::scanf("%lld %d %d %lld %lld %lld %d", &tokens, &group, &n_kv, &requests, &seq, &most_keys, &has_starts) == 7) {
+    const wx::paged::Launch l = wx::paged::launch_of(tokens, group, n_kv, requests, seq, most_keys, has_starts, 512);
+    std::printf("%d %d\n", l.shift, l.blocks);
+  }
+}
+"""
+
+
+def test_launches_of_the_largest_calls(tmp_path):
+    """Measures are scaled so that all of them fit 31 bits, up to the sizes that a call is refused at and far beyond, against Python's integers."""
+    (tmp_path / "launch.cpp").write_text(LAUNCHES)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=undefined", "-Wall", "-Werror", f"-I{CSRC}", str(tmp_path / "launch.cpp"), "-o",
+                    str(tmp_path / "launch")], check=True)
+    rng = random.Random(1)
+    most = 2 ** 30 - 1
+    cases = [(1, 1, 64, most, 1, most, 1), (1, 1, most, most, 1, most, 1), (most, 1, 1, 1, most, most, 0), (2 ** 20, 1024, 1, 1, 2 ** 20, 1, 0), (4096, 1, 8, 3340000 // 8, 4096, 1, 1)]
+    for _ in range(3000):
+        n_kv, group = int(2 ** rng.uniform(0, 10)), int(2 ** rng.uniform(0, 10))
+        tokens = max(1, int(2 ** rng.uniform(0, 30)) // (n_kv * group))
+        cases.append((tokens, group, n_kv, int(2 ** rng.uniform(0, 30)), tokens, int(2 ** rng.uniform(0, 30)), 1))
+    out = subprocess.run([str(tmp_path / "launch")], input="\n".join(" ".join(map(str, c)) for c in cases), capture_output=True, text=True, check=True).stdout.splitlines()
+    fits = 0
+    for (tokens, group, n_kv, requests, _, keys, _), line in zip(cases, out, strict=True):
+        shift, blocks = map(int, line.split())
+        tiles, keys = n_kv * (tokens * group // 64 + requests), max(keys, tokens) + 256
+        need = next((s for s in range(30) if tiles * ((keys >> s) + 320) <= most), 30)
+        assert shift == need and 512 <= blocks <= 4096, (tiles, keys, shift, need, blocks)
+        fits += shift < 30
+    assert 300 < fits < len(cases) - 300

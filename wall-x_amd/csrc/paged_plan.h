@@ -57,6 +57,7 @@ inline Launch launch_of(int64_t tokens, int group, int n_kv, int64_t requests, i
   Launch l{0, shares};
   const int64_t rows = tokens * group, tiles = n_kv * (rows / kFewRows + requests);
   const int64_t keys = (most_keys > tokens ? most_keys : tokens) + 2 * kManyRows;
+  if (tiles > kMostMeasure / (kStartFew + kStartMany)) l.shift = 30;  // (none will do, and the product below could pass 63 bits)
   while (l.shift < 30 && tiles * ((keys >> l.shift) + kStartFew + kStartMany) > kMostMeasure) ++l.shift;
   // Room for an item of many rows to a workgroup (see share_of()), where there may be so many; of more than four to a share (eight where the plan is a
   // wavefront's) the shares are as good, and a plan over more than 256 requests is too long to be made for an item: 1024 requests of 64 tokens 280 us so, 167 in shares.
